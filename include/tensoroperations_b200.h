@@ -37,7 +37,11 @@ typedef enum to_status {
   TO_ERR_GRID = 9              /* a LabelWhole label longer than its tile   */
 } to_status;
 
-typedef enum to_dtype { TO_F32 = 0, TO_F64 = 1 } to_dtype;
+typedef enum to_dtype {
+  TO_F32 = 0,
+  TO_F64 = 1,
+  TO_BF16 = 2 /* the sequence operators only; the others reject it */
+} to_dtype;
 
 /* ---------------------------------------------------------------------- */
 /* Library                                                                 */
@@ -534,6 +538,168 @@ typedef struct to_level_launch {
 
 int to_level_plan_lower(const to_level_plan_desc* desc, int32_t query_device,
                         to_level_launch* out);
+
+/* ---------------------------------------------------------------------- */
+/* Sequence operators: rows of heads                                       */
+/* ---------------------------------------------------------------------- */
+/*
+ * Values of [tokens][heads][width], the width contiguous; strides count
+ * elements, so a head's rows may lie inside wider packed rows.  dtype is the
+ * descriptor's (TO_BF16 or TO_F32).  64-bit offsets throughout.
+ */
+typedef struct to_rows {
+  void* data;
+  int64_t token_stride;
+  int64_t head_stride;
+} to_rows;
+
+/* ---------------------------------------------------------------------- */
+/* Query / key norm of each head with the rotation by position             */
+/* ---------------------------------------------------------------------- */
+/*
+ * For every head x of q and of k (head_dim values):
+ *   y = w * x / sqrt(mean(x^2) + eps),
+ * then the first rotary_dim values of y turn in pairs: pair j by the angle
+ *   positions[axis(j)][t] * theta^(-2 j / rotary_dim),
+ * (a, b) -> (a cos - b sin, b cos + a sin).  Pair j is (j, j + rotary_dim/2),
+ * or (2j, 2j+1) with interleaved = 1.  Axis a owns section[a] consecutive
+ * pairs (sections sum to rotary_dim / 2): one axis for text, three for
+ * (time, height, width).  Angles are reduced exactly (64-bit fixed-point
+ * turns), so any int32 position, negative ones included, keeps f32 accuracy.
+ * wq, wk: [head_dim] f32, NULL for 1.  Sums are f32; one rounding at the end.
+ * head_dim even, at most 256.  k_heads may be 0 (no keys).
+ * Outputs may be the inputs themselves (same pointer and strides); they may
+ * not overlap them otherwise.
+ */
+typedef struct to_qk_desc {
+  int32_t dtype;
+  int32_t q_heads;
+  int32_t k_heads;
+  int32_t head_dim;
+  int32_t rotary_dim;  /* even, 0 (no rotation) .. head_dim                  */
+  int32_t axes;        /* 1 .. 4                                             */
+  int32_t section[4];  /* pairs of each axis                                 */
+  int32_t interleaved; /* 0: halves, 1: neighbours                           */
+  int32_t reserved0;
+  double theta;        /* > 0                                                */
+  double eps;          /* >= 0                                               */
+} to_qk_desc;
+
+typedef struct to_qk_plan to_qk_plan;
+
+int to_qk_plan_create(const to_qk_desc* desc, to_qk_plan** out);
+int to_qk_plan_destroy(to_qk_plan* plan);
+
+/* positions: device int32 [axes][tokens] (may be NULL when rotary_dim is 0). */
+int to_qk_norm_rotary(const to_qk_plan* plan, int64_t tokens, const to_rows* q, const to_rows* k,
+                      const int32_t* positions, const float* wq, const float* wk,
+                      const to_rows* q_out, const to_rows* k_out, void* stream);
+
+/*
+ * Gradients: gq, gk of the outputs -> dq, dk of the inputs q, k (which are the
+ * forward pass's inputs) and dwq, dwk ([head_dim] f32, overwritten; both are
+ * computed even where wq / wk is NULL, and either may be NULL to leave it
+ * out).  Sums run in a fixed order.  workspace: 16-byte aligned device memory
+ * of at least to_qk_norm_rotary_workspace_bytes.  dq / dk may be gq / gk.
+ */
+size_t to_qk_norm_rotary_workspace_bytes(const to_qk_plan* plan, int64_t tokens);
+int to_qk_norm_rotary_backward(const to_qk_plan* plan, int64_t tokens, const to_rows* q,
+                               const to_rows* k, const int32_t* positions, const float* wq,
+                               const float* wk, const to_rows* gq, const to_rows* gk,
+                               const to_rows* dq, const to_rows* dk, float* dwq, float* dwk,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------- */
+/* Linear attention with a decay for each head                             */
+/* ---------------------------------------------------------------------- */
+/*
+ * Query head h reads key / value head h / (q_heads / kv_heads).  Within a
+ * sequence of L tokens, t = 0 .. L-1, with l = exp(log_decay[h]):
+ *   S_t = l S_{t-1} + k_t v_t^T          (f32 state [key_dim][value_dim])
+ *   o_t = scale * S_t^T q_t
+ * S_{-1} is the entering state (state_in, zero when NULL); S_{L-1} is written
+ * to state_out (when not NULL).  log_decay: device f32 [q_heads], values <= 0
+ * (a positive one counts as 0); -inf forgets everything at once.
+ *
+ * Sequences are packed: sequence n holds the tokens cu_seqlens[n] ..
+ * cu_seqlens[n+1]-1 (device int32 [nseq + 1], non-decreasing, within
+ * [0, tokens]; values outside are clamped).  Lengths 0 and 1 are ordinary: an
+ * empty sequence hands its entering state on.  Rows of o that belong to no
+ * sequence are left as they are.
+ *
+ * States are [slots][q_heads][key_dim][value_dim] f32, contiguous, 16-byte
+ * aligned.  slots (device int32 [nseq]) names each sequence's slot in
+ * state_in and state_out; NULL: slot n is sequence n.  A slot outside
+ * [0, num_slots) stands for no state: the sequence starts from zero and writes
+ * none.  Two sequences may not share a slot.  state_out may be state_in.
+ *
+ * key_dim and value_dim 1 .. 256.  Products of bf16 rows run on the tensor
+ * cores with f32 sums; states and their updates keep f32 accuracy.  The
+ * chunked form multiplies masked pairs of a 128-token chunk by zero, so a
+ * non-finite value in one token's row can reach earlier tokens of its own
+ * chunk; it never reaches another sequence.
+ *
+ * Results do not depend on timing (every sum has a fixed order).  Calls on
+ * different streams need workspaces of their own.
+ */
+typedef struct to_linear_attention_desc {
+  int32_t dtype;
+  int32_t q_heads;
+  int32_t kv_heads;  /* divides q_heads                                      */
+  int32_t key_dim;
+  int32_t value_dim;
+  int32_t nseq;      /* >= 0                                                 */
+  int64_t tokens;    /* rows of q, k, v, o; < 2^31                           */
+  int64_t num_slots; /* slots of state_in / state_out (with slots NULL: nseq) */
+  double scale;      /* finite                                               */
+} to_linear_attention_desc;
+
+typedef struct to_linear_attention_args {
+  to_rows q, k, v, o;
+  const float* log_decay;
+  const int32_t* cu_seqlens;
+  const int32_t* slots;
+  const float* state_in;
+  float* state_out;
+  void* workspace; /* device, 256-byte aligned                               */
+  size_t workspace_bytes;
+} to_linear_attention_args;
+
+size_t to_linear_attention_workspace_bytes(const to_linear_attention_desc* desc);
+int to_linear_attention(const to_linear_attention_desc* desc, const to_linear_attention_args* args,
+                        void* stream);
+
+/*
+ * Gradients of the call above with respect to q, k, v and the entering state,
+ * from d_o and dstate_out (the gradient of the state left; NULL: zero).
+ * log_decay is a constant of the model.  States and their gradients are
+ * [nseq][q_heads][key_dim][value_dim] (no slots).  Gradients of heads that
+ * share a key / value head are summed in f32 before their one rounding.
+ */
+typedef struct to_linear_attention_grad_args {
+  to_rows q, k, v, d_o, dq, dk, dv;
+  const float* log_decay;
+  const int32_t* cu_seqlens;
+  const float* state_in;
+  const float* dstate_out;
+  float* dstate_in; /* NULL: not wanted; may not be dstate_out               */
+  void* workspace;  /* device, 256-byte aligned                              */
+  size_t workspace_bytes;
+} to_linear_attention_grad_args;
+
+size_t to_linear_attention_backward_workspace_bytes(const to_linear_attention_desc* desc);
+int to_linear_attention_backward(const to_linear_attention_desc* desc,
+                                 const to_linear_attention_grad_args* args, void* stream);
+
+/*
+ * One token of each of desc->tokens requests: the state in the request's slot
+ * becomes l S + k v^T in place and o = scale * S^T q.  A request whose slot
+ * lies outside [0, num_slots) touches no state and gets a row of zeros.
+ * nseq, cu_seqlens, state_in and the workspace are not used; state_out is the
+ * state.
+ */
+int to_linear_attention_step(const to_linear_attention_desc* desc,
+                             const to_linear_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

@@ -1,0 +1,653 @@
+// linear_attention.cu -- linear attention with a decay for each head: the
+// chunked form and its gradients (one chain, linear_attention.cuh) on the CUDA
+// cores, the segment scan, the single-token step, and the C-ABI entries.
+#include <algorithm>
+#include <cmath>
+#include <mutex>
+
+#include "linear_attention.cuh"
+
+namespace to_b200 {
+namespace {
+
+using lin::Chain;
+using lin::Segment;
+using seq::Rows;
+
+constexpr int kMaxDim = 256;
+
+// ---- the chain on the CUDA cores ---------------------------------------------------
+// f32 rows, and bf16 rows whose widths or addresses the tensor-core form does
+// not take.  One CTA: one segment, one head, DCB columns of c.  Chunks of 64
+// tokens: P = (a b^T) masked and decayed, out = P c + decay (a X), then X, all
+// in f32 in shared memory, 4 x 4 results a thread.  At most 128 flops come
+// from 8 16-byte shared loads, so the shared-memory pipe bounds it at about
+// half of the f32 rate.
+constexpr int kRows = 64;  // tokens of a chunk
+constexpr int kThreads = 256;
+
+template <int DCB>
+struct SimtShape {
+  static constexpr int kColPad = DCB + 4;
+  static size_t bytes(int dbp) {
+    return sizeof(float) * (2 * size_t(kRows) * (dbp + 4) + size_t(kRows) * kColPad +
+                            size_t(kRows) * (kRows + 4) + size_t(dbp) * kColPad + 2 * (kRows + 4));
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void load_rows(float* dst, int ld, const Rows& r, int head, long long row0,
+                                          int step, int cnt, int first, int width, int padded) {
+  // rows past cnt and columns past width become zero
+  for (int e = threadIdx.x; e < kRows * padded; e += kThreads) {
+    const int i = e / padded, x = e - i * padded;
+    float v = 0.f;
+    if (i < cnt && x < width)
+      v = seq::to_f32(seq::row_ptr<const T>(r, row0 + static_cast<long long>(step) * i, head)[first + x]);
+    dst[i * ld + x] = v;
+  }
+}
+
+template <typename T, typename TO, int DCB, bool STATES>
+__global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_constant__ Chain C) {
+  constexpr int kColPad = SimtShape<DCB>::kColPad;
+  constexpr int VC = DCB / 16;  // columns of a thread
+  const Segment g = lin::segment_of(C, blockIdx.x);
+  if (g.idx < 0 || (STATES && g.idx == g.count - 1)) return;
+  const int head = blockIdx.z, col0 = blockIdx.y * DCB;
+  const int dbp = (C.db + 3) & ~3, lda = dbp + 4;
+  extern __shared__ __align__(16) float sm[];
+  float* A = sm;
+  float* B = A + kRows * lda;
+  float* V = B + kRows * lda;
+  float* P = V + kRows * kColPad;
+  float* X = P + kRows * (kRows + 4);
+  float* dec = X + dbp * kColPad;  // l^n, n = 0 .. kRows
+  const int tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
+  const int ncols = min(DCB, C.dc - col0);
+  const float gl = lin::log_decay_of(C, head);
+  if (tid <= kRows) dec[tid] = expf(gl * static_cast<float>(tid));
+
+  // entering X
+  const long long slot = lin::state_slot(C, g.seq);
+  const float* src = nullptr;
+  int src_t = 0;
+  if (!STATES) {
+    if (C.seg_state) {
+      src = C.seg_state + (static_cast<long long>(blockIdx.x) * C.heads + head) * C.db * C.dc;
+    } else if (C.init && slot >= 0) {
+      src = C.init + (slot * C.heads + head) * C.db * C.dc;
+      src_t = C.init_t;
+    }
+  }
+  for (int e = tid; e < dbp * DCB; e += kThreads) {
+    const int b = e / DCB, c = e - b * DCB;
+    X[b * kColPad + c] =
+        src && b < C.db && c < ncols ? src[lin::state_index(C, src_t, b, col0 + c)] : 0.f;
+  }
+
+  const long long s0 = g.idx * C.seg;
+  const long long s1 = min(s0 + C.seg, g.tokens);
+  const int step = C.rev ? -1 : 1;
+  for (long long t = s0; t < s1; t += kRows) {
+    const int cnt = static_cast<int>(min(static_cast<long long>(kRows), s1 - t));
+    const long long row0 = C.rev ? g.first + g.tokens - 1 - t : g.first + t;
+    __syncthreads();  // the last chunk's readers are done
+    if (!STATES) load_rows<T>(A, lda, C.a, head / C.a_div, row0, step, cnt, 0, C.db, dbp);
+    load_rows<T>(B, lda, C.b, head / C.b_div, row0, step, cnt, 0, C.db, dbp);
+    load_rows<T>(V, kColPad, C.c, head / C.c_div, row0, step, cnt, col0, ncols, DCB);
+    __syncthreads();
+    if (!STATES) {
+      float acc[4][4] = {};
+      for (int k = 0; k < dbp; k += 4) {
+        float4 x[4], y[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[r] = *reinterpret_cast<const float4*>(A + (ty + 16 * r) * lda + k);
+          y[r] = *reinterpret_cast<const float4*>(B + (tx + 16 * r) * lda + k);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            acc[r][q] = fmaf(x[r].w, y[q].w, fmaf(x[r].z, y[q].z, fmaf(x[r].y, y[q].y, fmaf(x[r].x, y[q].x, acc[r][q]))));
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int i = ty + 16 * r, j = tx + 16 * q;
+          P[i * (kRows + 4) + j] = j <= i && j < cnt ? acc[r][q] * dec[i - j] * C.intra : 0.f;
+        }
+      __syncthreads();
+      // out = P V + inter * l^(i+1-rev) A X
+      float o[4][VC] = {}, w[4][VC] = {};
+      for (int j = 0; j < kRows; j += 4) {
+        float4 p[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[r] = *reinterpret_cast<const float4*>(P + (ty + 16 * r) * (kRows + 4) + j);
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+          float v[VC];
+          seq::load_vec<float, VC>(V + (j + jj) * kColPad + tx * VC, v);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float pv = jj == 0 ? p[r].x : jj == 1 ? p[r].y : jj == 2 ? p[r].z : p[r].w;
+#pragma unroll
+            for (int c = 0; c < VC; ++c) o[r][c] = fmaf(pv, v[c], o[r][c]);
+          }
+        }
+      }
+      for (int k = 0; k < dbp; k += 4) {
+        float4 p[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[r] = *reinterpret_cast<const float4*>(A + (ty + 16 * r) * lda + k);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          float v[VC];
+          seq::load_vec<float, VC>(X + (k + kk) * kColPad + tx * VC, v);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float pv = kk == 0 ? p[r].x : kk == 1 ? p[r].y : kk == 2 ? p[r].z : p[r].w;
+#pragma unroll
+            for (int c = 0; c < VC; ++c) w[r][c] = fmaf(pv, v[c], w[r][c]);
+          }
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = ty + 16 * r;
+        if (i >= cnt) continue;
+        TO* dst = seq::row_ptr<TO>(C.out, row0 + static_cast<long long>(step) * i, head / C.out_div) + col0;
+        const float f = C.inter * dec[i + 1 - C.rev];
+#pragma unroll
+        for (int c = 0; c < VC; ++c)
+          if (tx * VC + c < ncols) dst[tx * VC + c] = seq::from_f32<TO>(fmaf(f, w[r][c], o[r][c]));
+      }
+      __syncthreads();  // X has been read
+    }
+    // X = l^cnt X + upd * sum_j l^(cnt-1+rev-j) b_j c_j
+    const float keep = dec[cnt];
+    for (int k0 = 0; k0 < dbp; k0 += 64) {
+      const int k = k0 + ty * 4;
+      if (k >= dbp) continue;
+      float u[4][VC] = {};
+      for (int j = 0; j < cnt; ++j) {
+        const float d = C.upd * dec[cnt - 1 + C.rev - j];
+        const float4 b = *reinterpret_cast<const float4*>(B + j * lda + k);
+        float v[VC];
+        seq::load_vec<float, VC>(V + j * kColPad + tx * VC, v);
+#pragma unroll
+        for (int c = 0; c < VC; ++c) {
+          const float x = d * v[c];
+          u[0][c] = fmaf(b.x, x, u[0][c]);
+          u[1][c] = fmaf(b.y, x, u[1][c]);
+          u[2][c] = fmaf(b.z, x, u[2][c]);
+          u[3][c] = fmaf(b.w, x, u[3][c]);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < VC; ++c) {
+          float* x = X + (k + r) * kColPad + tx * VC + c;
+          *x = fmaf(keep, *x, u[r][c]);
+        }
+    }
+  }
+  __syncthreads();
+  float* dst = nullptr;
+  int dst_t = 0;
+  if (STATES) {
+    dst = C.seg_state + (static_cast<long long>(blockIdx.x) * C.heads + head) * C.db * C.dc;
+  } else if (C.fin && slot >= 0 && g.idx == g.count - 1) {
+    dst = C.fin + (slot * C.heads + head) * C.db * C.dc;
+    dst_t = C.fin_t;
+  }
+  if (dst)
+    for (int e = tid; e < C.db * DCB; e += kThreads) {
+      const int b = e / DCB, c = e - b * DCB;
+      if (c < ncols) dst[lin::state_index(C, dst_t, b, col0 + c)] = X[b * kColPad + c];
+    }
+}
+
+// ---- scan over the segments ---------------------------------------------------------
+// In place: slot s holds segment s's own X (the last one's is not read) and
+// gets the X that enters it.
+__global__ void __launch_bounds__(256) chain_scan_kernel(const __grid_constant__ Chain C) {
+  const int s = blockIdx.z, head = blockIdx.y;
+  const Segment g = lin::sequence_of(C, s);
+  const long long w0 = lin::first_slot(C, s), n = static_cast<long long>(C.db) * C.dc;
+  const long long slots = lin::segment_slots(C.tokens, C.nseq, C.seg);
+  const long long e = blockIdx.x * 256ll + threadIdx.x;
+  if (e >= n) return;
+  const long long slot = lin::state_slot(C, s);
+  float x = 0.f;
+  if (C.init && slot >= 0) {
+    const int b = static_cast<int>(e / C.dc), c = static_cast<int>(e - static_cast<long long>(b) * C.dc);
+    x = C.init[(slot * C.heads + head) * n + lin::state_index(C, C.init_t, b, c)];
+  }
+  const float keep = expf(lin::log_decay_of(C, head) * static_cast<float>(C.seg));
+  const long long hop = C.heads * n;
+  float* p = C.seg_state + (w0 * C.heads + head) * n + e;
+  const int count = static_cast<int>(min(static_cast<long long>(g.count), slots - w0));
+  for (int i = 0; i < count; i += 4) {
+    float own[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) own[j] = i + j < count - 1 ? p[(i + j) * hop] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < count) {
+        p[(i + j) * hop] = x;
+        x = fmaf(keep, x, own[j]);
+      }
+  }
+}
+
+// ---- shared heads: sum the gradients of the heads of a group ---------------------------
+template <typename T>
+__global__ void __launch_bounds__(256) group_sum_kernel(const float* __restrict__ part, Rows out,
+                                                        long long tokens, int kv_heads, int group, int width) {
+  const long long per = static_cast<long long>(kv_heads) * width, total = tokens * per;
+  for (long long e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
+    const long long t = e / per;
+    const int r = static_cast<int>(e - t * per), h = r / width, x = r - h * width;
+    const float* p = part + ((t * kv_heads + h) * group) * width + x;
+    float v = 0.f;
+    for (int i = 0; i < group; ++i) v += p[static_cast<long long>(i) * width];
+    seq::row_ptr<T>(out, t, h)[x] = seq::from_f32<T>(v);
+  }
+}
+
+// ---- one token of each request ------------------------------------------------------------
+// Memory bound: the state is read and written once, 8 bytes a value, for 4
+// flops.  A CTA takes `cols` columns of one request's head; a lane holds VEC
+// consecutive columns and walks the rows of the state, kUnroll of them in flight.
+struct StepArgs {
+  Rows q, k, v, o;
+  const float* log_decay;
+  const int32_t* slots;
+  float* state;
+  long long num_slots;
+  int heads, group, dk, dv, cols;
+  float scale;
+};
+
+constexpr int kStepThreads = 128;
+constexpr int kUnroll = 8;
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constant__ StepArgs A) {
+  __shared__ float sq[kMaxDim], sk[kMaxDim];
+  __shared__ float part[kStepThreads * VEC];
+  const int head = blockIdx.y, col0 = blockIdx.z * A.cols;
+  const long long req = blockIdx.x;
+  const int lanes = A.cols / VEC;  // a power of two, at most the CTA
+  const int row = threadIdx.x / lanes, cl = threadIdx.x - row * lanes, rows = kStepThreads / lanes;
+  const int c = col0 + cl * VEC;
+  long long slot = A.slots ? static_cast<long long>(__ldg(A.slots + req)) : req;
+  if (slot < 0 || slot >= A.num_slots) slot = -1;
+  const T* q = seq::row_ptr<const T>(A.q, req, head);
+  const T* k = seq::row_ptr<const T>(A.k, req, head / A.group);
+  for (int i = threadIdx.x; i < A.dk; i += kStepThreads) {
+    sq[i] = seq::to_f32(q[i]);
+    sk[i] = seq::to_f32(k[i]);
+  }
+  const bool on = c < A.dv;
+  float v[VEC], acc[VEC];
+#pragma unroll
+  for (int x = 0; x < VEC; ++x) v[x] = acc[x] = 0.f;
+  if (on) {
+    const T* vr = seq::row_ptr<const T>(A.v, req, head / A.group) + c;
+#pragma unroll
+    for (int x = 0; x < VEC; ++x) v[x] = seq::to_f32(vr[x]);
+  }
+  const float g = __ldg(A.log_decay + head);
+  const float l = expf(g > 0.f ? 0.f : g);
+  __syncthreads();
+  if (on && slot >= 0) {
+    float* S = A.state + (slot * A.heads + head) * static_cast<long long>(A.dk) * A.dv + c;
+    for (int r0 = row; r0 < A.dk; r0 += rows * kUnroll) {
+      float s[kUnroll][VEC];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int r = r0 + u * rows;
+        if (r < A.dk) seq::load_vec<float, VEC>(S + static_cast<long long>(r) * A.dv, s[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int r = r0 + u * rows;
+        if (r < A.dk) {
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) {
+            s[u][x] = fmaf(l, s[u][x], sk[r] * v[x]);
+            acc[x] = fmaf(sq[r], s[u][x], acc[x]);
+          }
+          seq::store_vec<float, VEC>(S + static_cast<long long>(r) * A.dv, s[u]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < VEC; ++x) part[threadIdx.x * VEC + x] = acc[x];
+  __syncthreads();
+  for (int x = threadIdx.x; x < A.cols; x += kStepThreads)
+    if (col0 + x < A.dv) {
+      float o = 0.f;
+      for (int r = 0; r < rows; ++r) o += part[r * A.cols + x];
+      seq::row_ptr<T>(A.o, req, head)[col0 + x] = seq::from_f32<T>(A.scale * o);
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------
+
+int check_desc(const char* who, const to_linear_attention_desc* d) {
+  if (!d) return set_error(TO_ERR_INVALID_ARGUMENT, "%s: null descriptor", who);
+  if (d->dtype != TO_F32 && d->dtype != TO_BF16)
+    return set_error(TO_ERR_UNSUPPORTED, "%s: dtype %d (built: f32, bf16)", who, d->dtype);
+  if (d->q_heads <= 0 || d->kv_heads <= 0 || d->q_heads > 65535 || d->q_heads % d->kv_heads)
+    return set_error(TO_ERR_INVALID_ARGUMENT, "%s: %d query heads on %d key heads", who, d->q_heads, d->kv_heads);
+  if (d->key_dim < 1 || d->key_dim > kMaxDim || d->value_dim < 1 || d->value_dim > kMaxDim)
+    return set_error(TO_ERR_UNSUPPORTED, "%s: key_dim %d, value_dim %d (1 .. 256)", who, d->key_dim, d->value_dim);
+  if (d->tokens < 0 || d->tokens > INT32_MAX || d->nseq < 0 || d->nseq > 65535 || d->num_slots < 0)
+    return set_error(TO_ERR_INVALID_ARGUMENT, "%s: %lld tokens, %d sequences, %lld slots", who,
+                     (long long)d->tokens, d->nseq, (long long)d->num_slots);
+  if (!std::isfinite(d->scale)) return set_error(TO_ERR_INVALID_ARGUMENT, "%s: scale %g", who, d->scale);
+  return ok();
+}
+
+int check_state(const char* who, const char* name, const void* p) {
+  if (p && !aligned(p, 16)) return set_error(TO_ERR_ALIGNMENT, "%s: %s is not 16-byte aligned", who, name);
+  return ok();
+}
+
+int check_list(const char* who, const char* name, const void* p, bool need) {
+  if (need && !p) return set_error(TO_ERR_INVALID_ARGUMENT, "%s: %s is null", who, name);
+  if (p && !aligned(p, 4)) return set_error(TO_ERR_ALIGNMENT, "%s: %s is not 4-byte aligned", who, name);
+  return ok();
+}
+
+// Tokens of a segment.  Enough segments that four CTAs for each SM have one;
+// at least four chunks of 128 a segment, so that the states that pass through
+// memory (8 db dc bytes a segment and head) stay below the rows' own bytes.
+// One segment for all where no sequence can be longer than one.
+long long plan_segment(const to_linear_attention_desc& d) {
+  const long long chunks = (d.tokens + 127) / 128;
+  long long per = (chunks * d.q_heads + 4 * 148 - 1) / (4 * 148);
+  per = per < 4 ? 4 : per;
+  return per >= chunks ? (1ll << 40) : per * 128;
+}
+
+constexpr size_t kAlign = 256;
+size_t rounded(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
+
+size_t state_bytes(const to_linear_attention_desc& d) {
+  const long long seg = plan_segment(d);
+  if (seg > d.tokens) return 0;
+  return rounded(size_t(lin::segment_slots(d.tokens, d.nseq, seg)) * d.q_heads * d.key_dim * d.value_dim * 4);
+}
+
+template <typename T, typename TO, int DCB, bool STATES>
+int launch_simt(const Chain& C, cudaStream_t s) {
+  static std::once_flag once;
+  static cudaError_t attr = cudaSuccess;
+  const size_t most = SimtShape<DCB>::bytes(DCB == 64 ? 128 : 256);
+  std::call_once(once, [&] {
+    attr = cudaFuncSetAttribute(chain_simt_kernel<T, TO, DCB, STATES>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+  });
+  TO_CUDA_TRY(attr);
+  const long long slots = C.seg_state ? lin::segment_slots(C.tokens, C.nseq, C.seg) : C.nseq;
+  const dim3 grid(static_cast<unsigned>(slots), (C.dc + DCB - 1) / DCB, C.heads);
+  chain_simt_kernel<T, TO, DCB, STATES><<<grid, kThreads, SimtShape<DCB>::bytes((C.db + 3) & ~3), s>>>(C);
+  TO_CUDA_TRY(cudaGetLastError());
+  return ok();
+}
+
+template <typename T, typename TO, bool STATES>
+int launch_simt(const Chain& C, cudaStream_t s) {
+  // wider b takes narrower columns: both operands and X share 227 KB
+  return C.db <= 128 ? launch_simt<T, TO, 64, STATES>(C, s) : launch_simt<T, TO, 32, STATES>(C, s);
+}
+
+template <typename T, typename TO>
+int run_chain(const Chain& C, cudaStream_t s) {
+  if (C.seg_state) {
+    if (int st = launch_simt<T, TO, true>(C, s)) return st;
+    const dim3 grid(static_cast<unsigned>((C.db * C.dc + 255) / 256), C.heads, C.nseq);
+    chain_scan_kernel<<<grid, 256, 0, s>>>(C);
+    TO_CUDA_TRY(cudaGetLastError());
+  }
+  return launch_simt<T, TO, false>(C, s);
+}
+
+int run_chain(const Chain& C, int32_t dtype, bool f32_out, cudaStream_t s) {
+  if (dtype == TO_F32) return run_chain<float, float>(C, s);
+  if (f32_out) return run_chain<__nv_bfloat16, float>(C, s);
+  return run_chain<__nv_bfloat16, __nv_bfloat16>(C, s);
+}
+
+Chain base_chain(const to_linear_attention_desc& d, const int32_t* cu, const float* log_decay, void* states) {
+  Chain C{};
+  C.heads = d.q_heads;
+  C.nseq = d.nseq;
+  C.tokens = d.tokens;
+  C.cu = cu;
+  C.log_decay = log_decay;
+  C.seg = plan_segment(d);
+  C.seg_state = C.seg > d.tokens ? nullptr : static_cast<float*>(states);
+  C.a_div = C.b_div = C.c_div = C.out_div = 1;
+  return C;
+}
+
+template <typename T>
+int group_sum(const float* part, const to_rows& out, const to_linear_attention_desc& d, int width, cudaStream_t s) {
+  const long long total = d.tokens * d.kv_heads * width, want = (total + 255) / 256;
+  group_sum_kernel<T><<<static_cast<unsigned>(std::min(want, 148ll * 16)), 256, 0, s>>>(
+      part, seq::rows_of(out), d.tokens, d.kv_heads, d.q_heads / d.kv_heads, width);
+  TO_CUDA_TRY(cudaGetLastError());
+  return ok();
+}
+
+}  // namespace
+}  // namespace to_b200
+
+using namespace to_b200;
+
+extern "C" {
+
+size_t to_linear_attention_workspace_bytes(const to_linear_attention_desc* desc) {
+  if (check_desc("to_linear_attention_workspace_bytes", desc)) return 0;
+  return state_bytes(*desc);
+}
+
+size_t to_linear_attention_backward_workspace_bytes(const to_linear_attention_desc* desc) {
+  if (check_desc("to_linear_attention_backward_workspace_bytes", desc)) return 0;
+  const to_linear_attention_desc& d = *desc;
+  size_t n = state_bytes(d);
+  if (d.q_heads != d.kv_heads)  // f32 gradients of each query head, before the heads of a group are summed
+    n += rounded(size_t(d.tokens) * d.q_heads * std::max(d.key_dim, d.value_dim) * 4);
+  return n;
+}
+
+int to_linear_attention(const to_linear_attention_desc* desc, const to_linear_attention_args* args,
+                        void* stream) {
+  const char* who = "to_linear_attention";
+  if (int st = check_desc(who, desc)) return st;
+  if (!args) return set_error(TO_ERR_INVALID_ARGUMENT, "%s: null arguments", who);
+  const to_linear_attention_desc& d = *desc;
+  const to_linear_attention_args& a = *args;
+  if (d.nseq == 0) return ok();
+  int st = seq::check_rows(who, "q", &a.q, d.tokens, d.q_heads, d.key_dim, d.dtype);
+  if (!st) st = seq::check_rows(who, "k", &a.k, d.tokens, d.kv_heads, d.key_dim, d.dtype);
+  if (!st) st = seq::check_rows(who, "v", &a.v, d.tokens, d.kv_heads, d.value_dim, d.dtype);
+  if (!st) st = seq::check_rows(who, "o", &a.o, d.tokens, d.q_heads, d.value_dim, d.dtype);
+  if (!st) st = check_list(who, "log_decay", a.log_decay, true);
+  if (!st) st = check_list(who, "cu_seqlens", a.cu_seqlens, true);
+  if (!st) st = check_list(who, "slots", a.slots, false);
+  if (!st) st = check_state(who, "state_in", a.state_in);
+  if (!st) st = check_state(who, "state_out", a.state_out);
+  if (st) return st;
+  const size_t need = state_bytes(d);
+  if (need && (!a.workspace || a.workspace_bytes < need))
+    return set_error(TO_ERR_INVALID_ARGUMENT, "%s: workspace %zu < %zu bytes", who,
+                     a.workspace ? a.workspace_bytes : 0, need);
+  if (need && !aligned(a.workspace, kAlign))
+    return set_error(TO_ERR_ALIGNMENT, "%s: workspace is not 256-byte aligned", who);
+  Chain C = base_chain(d, a.cu_seqlens, a.log_decay, a.workspace);
+  C.a = seq::rows_of(a.q);
+  C.b = seq::rows_of(a.k);
+  C.c = seq::rows_of(a.v);
+  C.out = seq::rows_of(a.o);
+  C.b_div = C.c_div = d.q_heads / d.kv_heads;
+  C.db = d.key_dim;
+  C.dc = d.value_dim;
+  C.intra = C.inter = static_cast<float>(d.scale);
+  C.upd = 1.f;
+  C.init = a.state_in;
+  C.fin = a.state_out;
+  C.slots = a.slots;
+  C.num_slots = d.num_slots;
+  return run_chain(C, d.dtype, false, static_cast<cudaStream_t>(stream));
+}
+
+int to_linear_attention_backward(const to_linear_attention_desc* desc,
+                                 const to_linear_attention_grad_args* args, void* stream) {
+  const char* who = "to_linear_attention_backward";
+  if (int st = check_desc(who, desc)) return st;
+  if (!args) return set_error(TO_ERR_INVALID_ARGUMENT, "%s: null arguments", who);
+  const to_linear_attention_desc& d = *desc;
+  const to_linear_attention_grad_args& a = *args;
+  if (d.nseq == 0) return ok();
+  int st = seq::check_rows(who, "q", &a.q, d.tokens, d.q_heads, d.key_dim, d.dtype);
+  if (!st) st = seq::check_rows(who, "k", &a.k, d.tokens, d.kv_heads, d.key_dim, d.dtype);
+  if (!st) st = seq::check_rows(who, "v", &a.v, d.tokens, d.kv_heads, d.value_dim, d.dtype);
+  if (!st) st = seq::check_rows(who, "d_o", &a.d_o, d.tokens, d.q_heads, d.value_dim, d.dtype);
+  if (!st) st = seq::check_rows(who, "dq", &a.dq, d.tokens, d.q_heads, d.key_dim, d.dtype);
+  if (!st) st = seq::check_rows(who, "dk", &a.dk, d.tokens, d.kv_heads, d.key_dim, d.dtype);
+  if (!st) st = seq::check_rows(who, "dv", &a.dv, d.tokens, d.kv_heads, d.value_dim, d.dtype);
+  if (!st) st = check_list(who, "log_decay", a.log_decay, true);
+  if (!st) st = check_list(who, "cu_seqlens", a.cu_seqlens, true);
+  if (!st) st = check_state(who, "state_in", a.state_in);
+  if (!st) st = check_state(who, "dstate_out", a.dstate_out);
+  if (!st) st = check_state(who, "dstate_in", a.dstate_in);
+  if (st) return st;
+  if (a.dstate_in && a.dstate_in == a.dstate_out)
+    return set_error(TO_ERR_INVALID_ARGUMENT, "%s: dstate_in is dstate_out", who);
+  const size_t need = to_linear_attention_backward_workspace_bytes(desc);
+  if (need && (!a.workspace || a.workspace_bytes < need))
+    return set_error(TO_ERR_INVALID_ARGUMENT, "%s: workspace %zu < %zu bytes", who,
+                     a.workspace ? a.workspace_bytes : 0, need);
+  if (need && !aligned(a.workspace, kAlign))
+    return set_error(TO_ERR_ALIGNMENT, "%s: workspace is not 256-byte aligned", who);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const int group = d.q_heads / d.kv_heads;
+  const float scale = static_cast<float>(d.scale);
+  Chain C = base_chain(d, a.cu_seqlens, a.log_decay, a.workspace);
+  // dq: forwards, a = do, b = v, c = k
+  C.a = seq::rows_of(a.d_o);
+  C.b = seq::rows_of(a.v);
+  C.c = seq::rows_of(a.k);
+  C.out = seq::rows_of(a.dq);
+  C.b_div = C.c_div = group;
+  C.db = d.value_dim;
+  C.dc = d.key_dim;
+  C.intra = C.inter = scale;
+  C.upd = 1.f;
+  C.init = a.state_in;
+  C.init_t = 1;
+  if ((st = run_chain(C, d.dtype, false, s))) return st;
+  // backwards; the gradients of shared heads go through f32 partial rows
+  float* part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + state_bytes(d));
+  auto target = [&](const to_rows& r, int width) {
+    if (group == 1) return seq::rows_of(r);
+    return Rows{reinterpret_cast<char*>(part), static_cast<long long>(d.q_heads) * width, width};
+  };
+  C.rev = 1;
+  C.intra = scale;
+  C.inter = 1.f;
+  C.upd = scale;
+  C.init = a.dstate_out;
+  // dk: a = v, b = do, c = q
+  C.a = seq::rows_of(a.v);
+  C.b = seq::rows_of(a.d_o);
+  C.c = seq::rows_of(a.q);
+  C.out = target(a.dk, d.key_dim);
+  C.a_div = group;
+  C.b_div = C.c_div = 1;
+  C.db = d.value_dim;
+  C.dc = d.key_dim;
+  C.init_t = 1;
+  if ((st = run_chain(C, d.dtype, group > 1, s))) return st;
+  if (group > 1) {
+    st = d.dtype == TO_BF16 ? group_sum<__nv_bfloat16>(part, a.dk, d, d.key_dim, s)
+                            : group_sum<float>(part, a.dk, d, d.key_dim, s);
+    if (st) return st;
+  }
+  // dv: a = k, b = q, c = do
+  C.a = seq::rows_of(a.k);
+  C.b = seq::rows_of(a.q);
+  C.c = seq::rows_of(a.d_o);
+  C.out = target(a.dv, d.value_dim);
+  C.db = d.key_dim;
+  C.dc = d.value_dim;
+  C.init_t = 0;
+  C.fin = a.dstate_in;
+  if ((st = run_chain(C, d.dtype, group > 1, s))) return st;
+  if (group > 1)
+    return d.dtype == TO_BF16 ? group_sum<__nv_bfloat16>(part, a.dv, d, d.value_dim, s)
+                              : group_sum<float>(part, a.dv, d, d.value_dim, s);
+  return ok();
+}
+
+int to_linear_attention_step(const to_linear_attention_desc* desc,
+                             const to_linear_attention_args* args, void* stream) {
+  const char* who = "to_linear_attention_step";
+  if (int st = check_desc(who, desc)) return st;
+  if (!args) return set_error(TO_ERR_INVALID_ARGUMENT, "%s: null arguments", who);
+  const to_linear_attention_desc& d = *desc;
+  const to_linear_attention_args& a = *args;
+  if (d.tokens == 0) return ok();
+  int st = seq::check_rows(who, "q", &a.q, d.tokens, d.q_heads, d.key_dim, d.dtype);
+  if (!st) st = seq::check_rows(who, "k", &a.k, d.tokens, d.kv_heads, d.key_dim, d.dtype);
+  if (!st) st = seq::check_rows(who, "v", &a.v, d.tokens, d.kv_heads, d.value_dim, d.dtype);
+  if (!st) st = seq::check_rows(who, "o", &a.o, d.tokens, d.q_heads, d.value_dim, d.dtype);
+  if (!st) st = check_list(who, "log_decay", a.log_decay, true);
+  if (!st) st = check_list(who, "slots", a.slots, false);
+  if (st) return st;
+  if (!a.state_out) return set_error(TO_ERR_INVALID_ARGUMENT, "%s: state_out is null", who);
+  if ((st = check_state(who, "state_out", a.state_out))) return st;
+  StepArgs A{};
+  A.q = seq::rows_of(a.q);
+  A.k = seq::rows_of(a.k);
+  A.v = seq::rows_of(a.v);
+  A.o = seq::rows_of(a.o);
+  A.log_decay = a.log_decay;
+  A.slots = a.slots;
+  A.state = a.state_out;
+  A.num_slots = d.num_slots;
+  A.heads = d.q_heads;
+  A.group = d.q_heads / d.kv_heads;
+  A.dk = d.key_dim;
+  A.dv = d.value_dim;
+  A.scale = static_cast<float>(d.scale);
+  const bool vec = d.value_dim % 4 == 0;  // rows of the state stay 16-byte aligned
+  // columns of a CTA: up to 128, fewer (32 at least) while the CTAs are fewer than two an SM
+  int cols = 128;
+  const long long work = d.tokens * d.q_heads;
+  while (cols > 32 && (cols / 2 >= d.value_dim || work * ((d.value_dim + cols - 1) / cols) < 2 * 148)) cols /= 2;
+  A.cols = cols;
+  const dim3 grid(static_cast<unsigned>(d.tokens), d.q_heads, (d.value_dim + cols - 1) / cols);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (d.dtype == TO_BF16) {
+    if (vec) step_kernel<__nv_bfloat16, 4><<<grid, kStepThreads, 0, s>>>(A);
+    else step_kernel<__nv_bfloat16, 1><<<grid, kStepThreads, 0, s>>>(A);
+  } else {
+    if (vec) step_kernel<float, 4><<<grid, kStepThreads, 0, s>>>(A);
+    else step_kernel<float, 1><<<grid, kStepThreads, 0, s>>>(A);
+  }
+  TO_CUDA_TRY(cudaGetLastError());
+  return ok();
+}
+
+}  // extern "C"
