@@ -47,6 +47,7 @@
 
 #include "common.hpp"
 #include "sm100_primitives.cuh"
+#include "tensor_map.hpp"
 
 namespace to_b200 {
 // This file's device status word (device symbols are per translation unit);
@@ -571,30 +572,6 @@ __global__ void tf32_split_regroup_b_kernel(const float* __restrict__ B, float* 
 }
 
 // ---- host: tensor maps through the driver entry point ---------------------------
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                 const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encode_fn(int* st) {
-  static std::once_flag once;
-  static EncodeTiled fn = nullptr;
-  static int status = TO_OK;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess || !p) {
-      cudaGetLastError();
-      status = set_error(TO_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-      return;
-    }
-    fn = reinterpret_cast<EncodeTiled>(p);
-  });
-  *st = status;
-  return fn;
-}
-
 int make_map(EncodeTiled enc, CUtensorMap* m, const void* ptr, int rank, const cuuint64_t* dims,
              const cuuint64_t* strides_bytes, const cuuint32_t* box) {
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
@@ -622,6 +599,25 @@ int launch_chain(dim3 grid, const CUtensorMap& a, const CUtensorMap& al, const C
 }
 
 }  // namespace
+
+EncodeTiled tensor_map_encoder(int* st) {
+  static std::once_flag once;
+  static EncodeTiled fn = nullptr;
+  static int status = TO_OK;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess || !p) {
+      cudaGetLastError();
+      status = set_error(TO_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+      return;
+    }
+    fn = reinterpret_cast<EncodeTiled>(p);
+  });
+  *st = status;
+  return fn;
+}
 
 int chain_device_status(int reset, int* value) {
   int v = 0;
@@ -661,7 +657,7 @@ int to_chain_f32(int32_t E, const float* A, const float* B, const float* C, floa
   if (!aligned(R, 4) || !aligned(C, 4) || (T && !aligned(T, 4)))
     return set_error(TO_ERR_ALIGNMENT, "to_chain_f32: misaligned output");
   int st = TO_OK;
-  EncodeTiled enc = encode_fn(&st);
+  EncodeTiled enc = tensor_map_encoder(&st);
   if (!enc) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const long long n = (long long)E * E * E * E;
@@ -720,7 +716,7 @@ int to_gemm_tf32x3(int64_t Mp, int64_t Np, int64_t Kp, const float* Ahi, const f
     if (!aligned(p, 16)) return set_error(TO_ERR_ALIGNMENT, "to_gemm_tf32x3: operands must be 16-byte aligned");
   }
   int st = TO_OK;
-  EncodeTiled enc = encode_fn(&st);
+  EncodeTiled enc = tensor_map_encoder(&st);
   if (!enc) return st;
   const cuuint64_t fb = 4;
   const cuuint64_t adims[2] = {cuuint64_t(Kp), cuuint64_t(Mp)};

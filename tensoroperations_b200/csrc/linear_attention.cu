@@ -410,21 +410,31 @@ int launch_simt(const Chain& C, cudaStream_t s) {
   return C.db <= 128 ? launch_simt<T, TO, 64, STATES>(C, s) : launch_simt<T, TO, 32, STATES>(C, s);
 }
 
+int launch_scan(const Chain& C, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>((C.db * C.dc + 255) / 256), C.heads, C.nseq);
+  chain_scan_kernel<<<grid, 256, 0, s>>>(C);
+  TO_CUDA_TRY(cudaGetLastError());
+  return ok();
+}
+
 template <typename T, typename TO>
-int run_chain(const Chain& C, cudaStream_t s) {
+int run_simt(const Chain& C, cudaStream_t s) {
   if (C.seg_state) {
     if (int st = launch_simt<T, TO, true>(C, s)) return st;
-    const dim3 grid(static_cast<unsigned>((C.db * C.dc + 255) / 256), C.heads, C.nseq);
-    chain_scan_kernel<<<grid, 256, 0, s>>>(C);
-    TO_CUDA_TRY(cudaGetLastError());
+    if (int st = launch_scan(C, s)) return st;
   }
   return launch_simt<T, TO, false>(C, s);
 }
 
 int run_chain(const Chain& C, int32_t dtype, bool f32_out, cudaStream_t s) {
-  if (dtype == TO_F32) return run_chain<float, float>(C, s);
-  if (f32_out) return run_chain<__nv_bfloat16, float>(C, s);
-  return run_chain<__nv_bfloat16, __nv_bfloat16>(C, s);
+  if (dtype == TO_F32) return run_simt<float, float>(C, s);
+  if (!lin::tc_takes(C, f32_out))
+    return f32_out ? run_simt<__nv_bfloat16, float>(C, s) : run_simt<__nv_bfloat16, __nv_bfloat16>(C, s);
+  if (C.seg_state) {
+    if (int st = lin::tc_states(C, s)) return st;
+    if (int st = launch_scan(C, s)) return st;
+  }
+  return lin::tc_outputs(C, f32_out, s);
 }
 
 Chain base_chain(const to_linear_attention_desc& d, const int32_t* cu, const float* log_decay, void* states) {

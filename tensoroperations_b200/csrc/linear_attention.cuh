@@ -111,5 +111,11 @@ __device__ __forceinline__ long long state_index(const Chain& C, int transposed,
   return transposed ? static_cast<long long>(c) * C.db + b : static_cast<long long>(b) * C.dc + c;
 }
 
+// The tensor-core form (linear_attention_tc.cu): whether it takes the chain's
+// rows, every segment's own X, and the outputs.
+bool tc_takes(const Chain& C, bool f32_out);
+int tc_states(const Chain& C, cudaStream_t s);
+int tc_outputs(const Chain& C, bool f32_out, cudaStream_t s);
+
 }  // namespace lin
 }  // namespace to_b200

@@ -607,6 +607,8 @@ int to_device_status(int32_t reset) {
   int w = 0;
   if (int st = chain_device_status(reset, &w)) return st;
   if (!v) v = w;
+  if (int st = sequence_device_status(reset, &w)) return st;
+  if (!v) v = w;
   if (v) return set_error(v, "a kernel reported %s", to_status_string(v));
   return ok();
 }
