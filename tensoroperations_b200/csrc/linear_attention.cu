@@ -86,11 +86,10 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
         src && b < C.db && c < ncols ? src[lin::state_index(C, src_t, b, col0 + c)] : 0.f;
   }
 
-  const long long s0 = g.idx * C.seg;
-  const long long s1 = min(s0 + C.seg, g.tokens);
+  const int s0 = g.idx * C.seg, len = min(C.seg, g.tokens - s0);
   const int step = C.rev ? -1 : 1;
-  for (long long t = s0; t < s1; t += kRows) {
-    const int cnt = static_cast<int>(min(static_cast<long long>(kRows), s1 - t));
+  for (int done = 0; done < len; done += kRows) {
+    const int cnt = min(kRows, len - done), t = s0 + done;
     const long long row0 = C.rev ? g.first + g.tokens - 1 - t : g.first + t;
     __syncthreads();  // the last chunk's readers are done
     if (!STATES) load_rows<T>(A, lda, C.a, head / C.a_div, row0, step, cnt, 0, C.db, dbp);
@@ -217,8 +216,9 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
 __global__ void __launch_bounds__(256) chain_scan_kernel(const __grid_constant__ Chain C) {
   const int s = blockIdx.z, head = blockIdx.y;
   const Segment g = lin::sequence_of(C, s);
-  const long long w0 = lin::first_slot(C, s), n = static_cast<long long>(C.db) * C.dc;
-  const long long slots = lin::segment_slots(C.tokens, C.nseq, C.seg);
+  const int w0 = lin::first_slot(C, s);
+  const long long n = static_cast<long long>(C.db) * C.dc;
+  const int slots = lin::segment_slots(C.tokens, C.nseq, C.seg);
   const long long e = blockIdx.x * 256ll + threadIdx.x;
   if (e >= n) return;
   const long long slot = lin::state_slot(C, s);
@@ -229,8 +229,8 @@ __global__ void __launch_bounds__(256) chain_scan_kernel(const __grid_constant__
   }
   const float keep = expf(lin::log_decay_of(C, head) * static_cast<float>(C.seg));
   const long long hop = C.heads * n;
-  float* p = C.seg_state + (w0 * C.heads + head) * n + e;
-  const int count = static_cast<int>(min(static_cast<long long>(g.count), slots - w0));
+  float* p = C.seg_state + (static_cast<long long>(w0) * C.heads + head) * n + e;
+  const int count = min(g.count, slots - w0);
   for (int i = 0; i < count; i += 4) {
     float own[4];
 #pragma unroll
@@ -371,20 +371,22 @@ int check_list(const char* who, const char* name, const void* p, bool need) {
 // at least four chunks of 128 a segment, so that the states that pass through
 // memory (8 db dc bytes a segment and head) stay below the rows' own bytes.
 // One segment for all where no sequence can be longer than one.
-long long plan_segment(const to_linear_attention_desc& d) {
+constexpr int kOneSegment = 1 << 30;
+
+int plan_segment(const to_linear_attention_desc& d) {
   const long long chunks = (d.tokens + 127) / 128;
   long long per = (chunks * d.q_heads + 4 * 148 - 1) / (4 * 148);
   per = per < 4 ? 4 : per;
-  return per >= chunks ? (1ll << 40) : per * 128;
+  return per >= chunks ? kOneSegment : static_cast<int>(per * 128);
 }
 
 constexpr size_t kAlign = 256;
 size_t rounded(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
 size_t state_bytes(const to_linear_attention_desc& d) {
-  const long long seg = plan_segment(d);
-  if (seg > d.tokens) return 0;
-  return rounded(size_t(lin::segment_slots(d.tokens, d.nseq, seg)) * d.q_heads * d.key_dim * d.value_dim * 4);
+  const int seg = plan_segment(d);
+  if (seg == kOneSegment) return 0;
+  return rounded(size_t(lin::segment_slots(static_cast<int>(d.tokens), d.nseq, seg)) * d.q_heads * d.key_dim * d.value_dim * 4);
 }
 
 template <typename T, typename TO, int DCB, bool STATES>
@@ -397,7 +399,7 @@ int launch_simt(const Chain& C, cudaStream_t s) {
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
   });
   TO_CUDA_TRY(attr);
-  const long long slots = C.seg_state ? lin::segment_slots(C.tokens, C.nseq, C.seg) : C.nseq;
+  const int slots = C.seg_state ? lin::segment_slots(C.tokens, C.nseq, C.seg) : C.nseq;
   const dim3 grid(static_cast<unsigned>(slots), (C.dc + DCB - 1) / DCB, C.heads);
   chain_simt_kernel<T, TO, DCB, STATES><<<grid, kThreads, SimtShape<DCB>::bytes((C.db + 3) & ~3), s>>>(C);
   TO_CUDA_TRY(cudaGetLastError());
@@ -441,11 +443,11 @@ Chain base_chain(const to_linear_attention_desc& d, const int32_t* cu, const flo
   Chain C{};
   C.heads = d.q_heads;
   C.nseq = d.nseq;
-  C.tokens = d.tokens;
+  C.tokens = static_cast<int>(d.tokens);
   C.cu = cu;
   C.log_decay = log_decay;
   C.seg = plan_segment(d);
-  C.seg_state = C.seg > d.tokens ? nullptr : static_cast<float*>(states);
+  C.seg_state = C.seg == kOneSegment ? nullptr : static_cast<float*>(states);
   C.a_div = C.b_div = C.c_div = C.out_div = 1;
   return C;
 }

@@ -34,7 +34,7 @@ struct Chain {
   int a_div, b_div, c_div, out_div;  // head h reads head h / div
   int heads, nseq;
   int db, dc;  // widths of b (and a) and of c (and out)
-  long long tokens;
+  int tokens;
   const int32_t* cu;
   const float* log_decay;
   float intra, inter, upd;
@@ -47,17 +47,17 @@ struct Chain {
   const int32_t* slots;
   long long num_slots;
   float* seg_state;  // [segment slots][heads][db][dc]; null: one segment a sequence
-  long long seg;     // tokens of a segment
+  int seg;           // tokens of a segment
 };
 
 // Where a segment lies.  idx < 0: an unused slot.
 struct Segment {
-  int seq, idx, count;     // its sequence, its place among the sequence's `count`
-  long long first, tokens; // the sequence's first row, its length
+  int seq, idx, count;  // its sequence, its place among the sequence's `count`
+  int first, tokens;    // the sequence's first row, its length
 };
 
-__device__ __forceinline__ long long clamped(const Chain& C, int s) {
-  const long long x = __ldg(C.cu + s);
+__device__ __forceinline__ int clamped(const Chain& C, int s) {
+  const int x = __ldg(C.cu + s);
   return x < 0 ? 0 : x > C.tokens ? C.tokens : x;
 }
 
@@ -65,19 +65,19 @@ __device__ __forceinline__ Segment sequence_of(const Chain& C, int s) {
   Segment g;
   g.seq = s;
   g.first = clamped(C, s);
-  const long long end = clamped(C, s + 1);
+  const int end = clamped(C, s + 1);
   g.tokens = end > g.first ? end - g.first : 0;
-  g.count = g.tokens ? static_cast<int>((g.tokens + C.seg - 1) / C.seg) : 1;
+  g.count = g.tokens ? (g.tokens - 1) / C.seg + 1 : 1;
   g.idx = 0;
   return g;
 }
 
-__device__ __forceinline__ long long first_slot(const Chain& C, int s) {
+__device__ __forceinline__ int first_slot(const Chain& C, int s) {
   return clamped(C, s) / C.seg + s;
 }
 
 // The last sequence whose first slot is at most w, by bisection.
-__device__ __forceinline__ Segment segment_of(const Chain& C, long long w) {
+__device__ __forceinline__ Segment segment_of(const Chain& C, int w) {
   int lo = 0, hi = C.nseq - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -85,12 +85,13 @@ __device__ __forceinline__ Segment segment_of(const Chain& C, long long w) {
     else hi = mid - 1;
   }
   Segment g = sequence_of(C, lo);
-  const long long idx = w - first_slot(C, lo);
-  g.idx = idx >= 0 && idx < g.count ? static_cast<int>(idx) : -1;
+  const int idx = w - first_slot(C, lo);
+  g.idx = idx >= 0 && idx < g.count ? idx : -1;
   return g;
 }
 
-__host__ __device__ inline long long segment_slots(long long tokens, int nseq, long long seg) {
+// At most 2^31 / 512 + 65535, or one a sequence and one more.
+__host__ __device__ inline int segment_slots(int tokens, int nseq, int seg) {
   return tokens / seg + nseq;
 }
 

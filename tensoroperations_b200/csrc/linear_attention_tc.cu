@@ -4,13 +4,15 @@
 // A work item is one segment of one head; a CTA walks its items and their
 // chunks of 128 tokens.  With Q, K, V the chunk's rows of a, b, c (tiles of
 // 128 x 128, narrower widths zero-filled by TMA) and X the state:
-//   Sc = Q K^T                    P = Sc masked and decayed, bf16, in TMEM
-//   O1 = Q X (bf16 X)             O2 = P V
-//   U  = (decayed K)^T V          out = intra O2 + inter l^(..) O1
-//   X  = l^n X + U                (f32, in registers)
-// all M = N = 128.  Six products of 128^3 a chunk (7 with three planes of K):
-// 3072 tensor cycles at the dense bf16 rate against about 5600 for the chunk's
-// 128 KB at this SM's share of the HBM, so the products hide behind the copies.
+//   Sc = Q K^T                    P = Sc masked, decayed and scaled, bf16, in TMEM
+//   O  = Q X (bf16 X), its rows scaled in TMEM by inter l^(..), then O += P V
+//   U  = (decayed K)^T V          X = l^n X + U (f32, in registers)
+// all M = N = 128.  Six products of 128^3 a chunk with three planes of K, 3072
+// tensor cycles at the dense bf16 rate, against about 5600 for the chunk's 128
+// KB at this SM's share of the HBM.  What else bounds it is the shared memory's
+// 128 bytes a cycle: a product of two shared operands of this size takes all of
+// it, so P and decayed K are TMEM operands (K transposed into its lanes by
+// ldmatrix), which leaves 256 KB a chunk to the products.
 //
 // Precision: P and X each enter their product with one bf16 rounding, as the
 // result's own.  The state stays f32: decayed K is split into PLANES bf16
@@ -18,14 +20,14 @@
 // state), smallest plane first, so few sums pass through the accumulator at
 // full size; a chunk's U is added to X in IEEE f32 registers.
 //
-// Roles (20 warps): one lane issues TMA loads into a ring of 32 KB tiles, one
-// the products; warps 4-11 turn Sc into P and store the results (a thread: one
-// row, 64 columns); warps 12-19 make the planes (plane 0 in place of K, which
-// Sc has read by then), and hold X (a thread: one row, 64 columns).  Products
-// are issued Sc, O1, O2, U: the next chunk's Sc and P run under the state's
-// update.  Rows past a chunk's end are masked: P and the planes by selection,
-// V by zeroing its rows, since 0 * NaN is not 0.  Rows of a reversed chain keep
-// their order in memory; only the masks and decays turn round.
+// Roles (20 warps): one lane issues TMA loads into a ring of six 32 KB tiles
+// (two chunks), one the products; warps 4-11 turn Sc into P, scale O and store
+// the results (a thread: one row, 64 columns); warps 12-19 make the planes and
+// hold X (a thread: one row, 64 columns).  Products are issued Sc, Q X, U, P V:
+// the next chunk's Sc and the row warps run under the state's update.  Rows
+// past a chunk's end are masked: P and the planes by selection, V by zeroing
+// its rows, since 0 * NaN is not 0.  Rows of a reversed chain keep their order
+// in memory; only the masks and decays turn round.
 //
 // Every wait is bounded; on a timeout the kernel records TO_ERR_TIMEOUT in the
 // device status word, waits (bounded) for its copies in flight, frees its TMEM
@@ -53,14 +55,20 @@ constexpr int kRowWarps = 8, kStateWarps = 8;    // P and out; planes and X
 constexpr int kFirstRow = 4, kFirstState = kFirstRow + kRowWarps;  // warps 0, 1: loads, products; 2, 3: none
 constexpr int kThreads = 32 * (kFirstState + kStateWarps);
 constexpr uint32_t kMaxPolls = 1u << 22;
-constexpr int kMaxSlots = 5;
+constexpr int kSlots = 6;                        // tiles of the ring
 
-// TMEM columns
-constexpr uint32_t kColS = 0, kColO1 = 128, kColO2 = 256, kColU = 384;
+// TMEM columns.  P of tokens [0, 64) and [64, 128) overwrites the first halves
+// of those tokens' columns of Sc; plane 0 takes the second halves, once Sc has
+// been read; planes 1 and 2 (the smaller ones) have columns of their own.
+constexpr uint32_t kColS = 0, kColO = 128, kColU = 256, kColPlane = 384;
+template <bool STATES>
+__device__ __forceinline__ uint32_t plane_col(int plane, int token64) {
+  return plane == 0 ? kColS + 64 * token64 + (STATES ? 0 : 32) : kColPlane + 64 * (plane - 1) + 32 * token64;
+}
 
 struct Barriers {
-  uint64_t full[kMaxSlots], empty[kMaxSlots];
-  uint64_t sc_full, p_ready, o1_full, o2_full, o_free;
+  uint64_t full[kSlots], empty[kSlots];
+  uint64_t sc_full, p_ready, o1_full, o_ready, o2_full, o_free;
   uint64_t planes_ready, u_full, u_free, x_ready;
   uint64_t row_table, state_table;
   uint32_t tmem;
@@ -80,6 +88,13 @@ __device__ __forceinline__ bool wait_for(Barriers* b, uint64_t* bar, uint32_t pa
 // The same by a whole warp, with one answer.
 __device__ __forceinline__ bool warp_wait(Barriers* b, uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, wait_for(b, bar, parity));
+}
+
+// The same value, which the compiler takes for a new one: what is computed from
+// it is not kept in registers from one chunk to the next.
+__device__ __forceinline__ uint32_t fresh(uint32_t x) {
+  asm volatile("" : "+r"(x));
+  return x;
 }
 
 __device__ __forceinline__ void arrive(uint64_t* bar) {
@@ -108,10 +123,10 @@ __device__ __forceinline__ uint64_t desc_k(uint32_t tile, int step) {  // 16 K v
 }
 __device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int step) { return desc(tile + step * 2048, kPanel); }
 
-// D f32, A and B bf16, M = N = 128; bits 15 / 16: A / B are MN-major
+// D f32, A and B bf16, M = N = 128; bit 16: B is MN-major
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kTile >> 3) << 17) |
                             (uint32_t(kTile >> 4) << 24);
-constexpr uint32_t kMnA = 1u << 15, kMnB = 1u << 16;
+constexpr uint32_t kMnB = 1u << 16;
 
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
   asm volatile(
@@ -148,13 +163,59 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&x)[32]) {
       : "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&x)[32]) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(x);
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n\t"
-      "tcgen05.wait::st.sync.aligned;"
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
       ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+// 16 lanes x 8 columns: register 2i / 2i+1 holds columns 4i .. 4i+3 of lanes
+// 0-7 / 8-15, thread t lane t/4 (or 8 + t/4) and column t%4 of the four --
+// what ldmatrix gives of 8 x 8 tiles.
+__device__ __forceinline__ void tmem_st_tiles(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};"
+               ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Four transposed 8 x 8 tiles of bf16; lane l gives the row address l%8 of tile l/8.
+__device__ __forceinline__ void ldmatrix_t4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&x)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(x);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+__device__ __forceinline__ float lds(uint32_t addr) {
+  float x;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(addr));
+  return x;
+}
+__device__ __forceinline__ uint4 lds4(uint32_t addr) {
+  uint4 x;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(addr));
+  return x;
+}
+__device__ __forceinline__ void sts4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
 // (lo, hi) as two bf16 in one register, lo in the low half
@@ -166,83 +227,102 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ float low_half(uint32_t r) { return __uint_as_float(r << 16); }
 __device__ __forceinline__ float high_half(uint32_t r) { return __uint_as_float(r & 0xffff0000u); }
 
-// l^n, n = 0 .. 128, made by the eight warps of a group for their item.  Two
-// tables in turn: a warp that has passed an item's barrier knows that all have
-// left the table before the last.
-constexpr int kTable = kTile + 1;
-__device__ __forceinline__ const float* make_table(Barriers* b, uint64_t* bar, float* tables, uint32_t count, int t,
-                                                   float gl, bool* ok) {
-  float* dec = tables + (count & 1) * kTable;
-  if (t < kTable) dec[t] = expf(gl * static_cast<float>(t));
+// A table that the eight warps of a group make for their item, f(n) for n <
+// count.  Two tables in turn: a warp that has passed an item's barrier knows
+// that all have left the table before the last.
+constexpr int kRowTable = 164;    // l^n, n = 0 .. 128; the 32 factors of a block's columns from 132 on
+constexpr int kStateTable = 128;  // decay of each token of a full chunk
+template <typename F>
+__device__ __forceinline__ uint32_t make_table(Barriers* b, uint64_t* bar, float* tables, int size, uint32_t turn,
+                                               int t, bool* ok, F f) {
+  float* mine = tables + (turn & 1) * size;
+  if (t < size) mine[t] = f(t);
   __syncwarp();
   if ((t & 31) == 0) arrive(bar);
-  *ok = warp_wait(b, bar, count & 1);
-  return dec;
+  *ok = warp_wait(b, bar, turn & 1);
+  return smem_u32(mine);
 }
 
-// The chunks of a segment: `n` of them; chunk i's first row in memory and its rows.
+// The chunks of an item (a segment of one head).
 struct Walk {
-  Segment g;
-  int head, n;
-  long long s0, s1;
-  __device__ __forceinline__ int rows(int i) const {
-    const long long left = s1 - s0 - static_cast<long long>(i) * kTile;
-    return left < kTile ? static_cast<int>(left) : kTile;
-  }
-  __device__ __forceinline__ long long first(const Chain& C, int i) const {
-    const long long t = s0 + static_cast<long long>(i) * kTile;
-    return C.rev ? g.first + g.tokens - t - rows(i) : g.first + t;
+  int seq, head, last;  // last: the sequence's last segment
+  int edge;             // first row of the segment (forwards), or the row after it (backwards)
+  int len;              // its tokens
+  int n, updates;       // chunks; those whose state is wanted (not the last's, where no one reads it)
+  __device__ __forceinline__ int rows(int i) const { return min(len - i * kTile, kTile); }
+  // First row in memory of chunk i.
+  __device__ __forceinline__ int first(const Chain& C, int i) const {
+    return C.rev ? edge - i * kTile - rows(i) : edge + i * kTile;
   }
 };
 
-// Item -> its walk; false: nothing to do there.
+// False: nothing to do there.
 template <bool STATES>
-__device__ __forceinline__ bool walk_of(const Chain& C, long long item, Walk* w) {
-  const long long slot = item / C.heads;
-  w->head = static_cast<int>(item - slot * C.heads);
-  w->g = lin::segment_of(C, slot);
-  if (w->g.idx < 0 || (STATES && w->g.idx == w->g.count - 1)) return false;
-  w->s0 = w->g.idx * C.seg;
-  w->s1 = min(w->s0 + C.seg, w->g.tokens);
-  w->n = static_cast<int>((w->s1 - w->s0 + kTile - 1) / kTile);
+__device__ __forceinline__ bool walk_of(const Chain& C, int item, Walk* w) {
+  const int slot = item / C.heads;
+  const Segment g = lin::segment_of(C, slot);
+  if (g.idx < 0 || (STATES && g.idx == g.count - 1)) return false;
+  const int s0 = g.idx * C.seg;  // no overflow: below the sequence's length
+  w->seq = g.seq;
+  w->head = item - slot * C.heads;
+  w->last = g.idx == g.count - 1;
+  w->len = min(C.seg, g.tokens - s0);
+  w->edge = C.rev ? g.first + g.tokens - s0 : g.first + s0;
+  w->n = (w->len + kTile - 1) / kTile;
+  w->updates = STATES || (C.fin && w->last) ? w->n : w->n - 1;
   return true;
 }
 
-template <bool STATES>
-struct Shape {
-  static constexpr int kSlots = STATES ? 5 : 4;
-  static constexpr uint32_t kPlanes = kSlots * kTileBytes;             // planes 1 and 2
-  static constexpr uint32_t kX = kPlanes + 2 * kTileBytes;             // bf16 X
-  static constexpr uint32_t kTables = kX + (STATES ? 0 : kTileBytes);  // tables of l^n
-  static constexpr uint32_t kBars = kTables + 4 * kTable * 4;
-  static constexpr uint32_t kBytes = kBars + sizeof(Barriers);
+template <int N>
+struct Int {
+  static constexpr int value = N;
 };
-static_assert(Shape<false>::kBars % 8 == 0 && Shape<true>::kBars % 8 == 0, "aligned barriers");
-static_assert(Shape<false>::kBytes <= 232448 && Shape<true>::kBytes <= 232448, "shared memory of a CTA");
+
+// Shared memory
+constexpr uint32_t kX = kSlots * kTileBytes;                             // bf16 X
+constexpr uint32_t kRowTables = kX + kTileBytes;
+constexpr uint32_t kStateTables = kRowTables + 2 * kRowTable * 4;
+constexpr uint32_t kBars = kStateTables + 2 * kStateTable * 4;
+constexpr uint32_t kSmem = kBars + sizeof(Barriers);
+static_assert(kBars % 8 == 0 && kSmem <= 232448, "shared memory of a CTA");
+
+// Registers: the launch gives each of the 20 warps 96; the idle-handed warps
+// return some of theirs (4 * 48 + 8 * 104 + 8 * 112 = 1920 = 20 * 96).  No kernel may
+// spill: with the shared memory taken, a spilled register comes back from L2.  Loops
+// stay rolled where registers allow it: the roles run different code at the same time,
+// and unrolled they outgrow the instruction caches (stalls for want of instructions were
+// three times the issued ones).
+template <int N>
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <typename TO, bool STATES, int PLANES>
 __global__ void __launch_bounds__(kThreads, 1)
     chain_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
                     const __grid_constant__ CUtensorMap mapC, const __grid_constant__ Chain C,
-                    const long long items) {
-  using L = Shape<STATES>;
-  constexpr int kSlots = L::kSlots, kPer = STATES ? 2 : 3;  // tiles of a chunk: (Q,) K, V
+                    const int items) {
+  constexpr int kPer = STATES ? 2 : 3;  // tiles of a chunk: (Q,) K, V
   extern __shared__ __align__(1024) unsigned char sm[];
   if (smem_u32(sm) & 1023) {  // the swizzled tiles need it; there is no room left to round up in
     if (threadIdx.x == 0) atomicExch(&g_sequence_status, int(TO_ERR_SCRATCH));
     return;
   }
-  Barriers* bar = reinterpret_cast<Barriers*>(sm + L::kBars);
+  Barriers* bar = reinterpret_cast<Barriers*>(sm + kBars);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kMaxSlots; ++i) {
+    for (int i = 0; i < kSlots; ++i) {
       mbar_init(&bar->full[i], 1);
-      mbar_init(&bar->empty[i], 1);
+      // V is freed by a commit, K by one and by the warps that read it into the planes,
+      // Q by the warps that the results pass through it
+      const int x = i % kPer;
+      mbar_init(&bar->empty[i], x == kPer - 1 ? 1 : x == kPer - 2 ? kStateWarps + (STATES ? 0 : 1) : kRowWarps);
     }
     mbar_init(&bar->sc_full, 1);
     mbar_init(&bar->p_ready, kRowWarps);
     mbar_init(&bar->o1_full, 1);
+    mbar_init(&bar->o_ready, kRowWarps);
     mbar_init(&bar->o2_full, 1);
     mbar_init(&bar->o_free, kRowWarps);
     mbar_init(&bar->planes_ready, kStateWarps);
@@ -266,15 +346,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto slot_of = [&](uint32_t tile) { return sm + (tile % kSlots) * kTileBytes; };
   Walk w;
 
-  if (warp == 0) {
-    if (lane == 0) {
-      // ---- loads: Q, K, V of each chunk, in ring order (Q's slot is free first) ----
+  if (warp < kFirstRow) {
+    registers_down<48>();
+    if (warp == 0 && lane == 0) {
+      // ---- loads: (Q,) K, V of each chunk, in ring order ----
       uint32_t tile = 0;
       bool ok = true;
-      for (long long item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
         if (!walk_of<STATES>(C, item, &w)) continue;
         for (int i = 0; i < w.n && ok; ++i) {
-          const int token = static_cast<int>(w.first(C, i));
+          const int token = w.first(C, i);
           for (int x = 0; x < kPer; ++x, ++tile) {
             const uint32_t s = tile % kSlots;
             if (tile >= kSlots && !(ok = wait_for(bar, &bar->empty[s], (tile / kSlots - 1) & 1))) break;
@@ -288,169 +369,243 @@ __global__ void __launch_bounds__(kThreads, 1)
       // copies still in flight land before the CTA ends
       for (uint32_t t = tile > kSlots ? tile - kSlots : 0; t < tile; ++t)
         mbar_wait_bounded(&bar->full[t % kSlots], (t / kSlots) & 1, kMaxPolls);
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
+    } else if (warp == 1 && lane == 0) {
       // ---- products ----
-      uint32_t n = 0;  // chunks so far
+      uint32_t n = 0, nu = 0;  // chunks and updates so far
       bool ok = true;
-      for (long long item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
         if (!walk_of<STATES>(C, item, &w)) continue;
         for (int i = 0; i < w.n && ok; ++i, ++n) {
           const uint32_t tq = n * kPer, tk = tq + kPer - 2, tv = tk + 1;
-          const uint32_t sk = smem_u32(slot_of(tk)), sv = smem_u32(slot_of(tv));
+          const uint32_t sk = fresh(smem_u32(slot_of(tk))), sv = fresh(smem_u32(slot_of(tv)));
           auto full = [&](uint32_t t) { return wait_for(bar, &bar->full[t % kSlots], (t / kSlots) & 1); };
           if (!STATES) {
-            const uint32_t sq = smem_u32(slot_of(tq)), sx = smem_u32(sm + L::kX);
-            if (!(ok = full(tk) && full(tq))) break;
+            const uint32_t sq = fresh(smem_u32(slot_of(tq))), sx = fresh(smem_u32(sm + kX));
+            if (!(ok = full(tq) && full(tk))) break;
             fence_after();
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)
               mma(tmem + kColS, desc_k(sq, k), desc_k(sk, k), kIdesc, k > 0);
             commit(&bar->sc_full);
+            commit(&bar->empty[tk % kSlots]);
             if (!(ok = wait_for(bar, &bar->x_ready, n & 1) && (n == 0 || wait_for(bar, &bar->o_free, (n - 1) & 1)))) break;
             fence_after();
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)
-              mma(tmem + kColO1, desc_k(sq, k), desc_mn(sx, k), kIdesc | kMnB, k > 0);
+              mma(tmem + kColO, desc_k(sq, k), desc_mn(sx, k), kIdesc | kMnB, k > 0);
             commit(&bar->o1_full);
-            commit(&bar->empty[tq % kSlots]);
           }
+          // planes_ready also says that V's rows past the end are zero
           if (!(ok = full(tv) && wait_for(bar, &bar->planes_ready, n & 1))) break;
-          if (!STATES) {
-            if (!(ok = wait_for(bar, &bar->p_ready, n & 1))) break;
+          if (i < w.updates) {
+            if (nu > 0 && !(ok = wait_for(bar, &bar->u_free, (nu - 1) & 1))) break;
             fence_after();
 #pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)  // 16 tokens: 8 columns; tokens 64 .. start at column 64
-              mma_ts(tmem + kColO2, tmem + kColS + (k >> 2) * 64 + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB, k > 0);
-            commit(&bar->o2_full);
+            for (int p = PLANES - 1; p >= 0; --p)
+#pragma unroll 4
+              for (int k = 0; k < kTile / 16; ++k)  // 16 tokens: 8 columns
+                mma_ts(tmem + kColU, tmem + plane_col<STATES>(p, k >> 2) + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB,
+                       p < PLANES - 1 || k > 0);
+            commit(&bar->u_full);
+            ++nu;
           }
-          if (n > 0 && !(ok = wait_for(bar, &bar->u_free, (n - 1) & 1))) break;
-          fence_after();
-#pragma unroll
-          for (int p = PLANES - 1; p >= 0; --p) {
-            const uint32_t sp = p == 0 ? sk : smem_u32(sm + L::kPlanes + (p - 1) * kTileBytes);
+          if (!STATES) {
+            if (!(ok = wait_for(bar, &bar->p_ready, n & 1) && wait_for(bar, &bar->o_ready, n & 1))) break;
+            fence_after();
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)
-              mma(tmem + kColU, desc_mn(sp, k), desc_mn(sv, k), kIdesc | kMnA | kMnB, p < PLANES - 1 || k > 0);
+              mma_ts(tmem + kColO, tmem + kColS + (k >> 2) * 64 + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB, true);
+            commit(&bar->o2_full);
           }
-          commit(&bar->u_full);
-          commit(&bar->empty[tk % kSlots]);
           commit(&bar->empty[tv % kSlots]);
         }
       }
     }
-  } else if (warp < kFirstRow) {
   } else if (warp < kFirstState) {
+    registers_up<104>();
     if (!STATES) {
-      // ---- P and the results: row r of the chunk, columns [64 h, 64 h + 64) ----
+      // ---- P, O and the results: row r of the chunk, columns [64 h, 64 h + 64) ----
       const int q = warp & 3, h = (warp - kFirstRow) >> 2;
       const int r = q * 32 + lane;
       const uint32_t lanes = tmem + (uint32_t(q * 32) << 16);
+      const bool rev = C.rev != 0;
+      const float intra = C.intra, inter = C.inter;
+      const long long pitch = C.out.ts;
       uint32_t n = 0, tables = 0;
       bool ok = true;
-      for (long long item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
         if (!walk_of<STATES>(C, item, &w)) continue;
         const float gl = lin::log_decay_of(C, w.head);
-        const float* dec = make_table(bar, &bar->row_table, reinterpret_cast<float*>(sm + L::kTables), tables++,
-                                      threadIdx.x - 32 * kFirstRow, gl, &ok);
+        const uint32_t dec = make_table(bar, &bar->row_table, reinterpret_cast<float*>(sm + kRowTables), kRowTable, tables++, threadIdx.x - 32 * kFirstRow, &ok, [&](int t) {
+                                        const int e = t < 132 ? t : C.rev ? t - 132 : 163 - t;
+                                        return expf(gl * static_cast<float>(e));
+                                      });
         if (!ok) break;
         for (int i = 0; i < w.n; ++i, ++n) {
           const int cnt = w.rows(i);
-          // P[r][j] = Sc[r][j] l^|r - j| where j has been seen by r
+          // P[r][j] = intra Sc[r][j] l^|r - j| where j has been seen by r: blocks of 16
+          // columns, of which this warp's rows see all, a triangle, or nothing.  (Each block's
+          // P lands on columns of Sc that this warp has read by then.)
           if (!(ok = warp_wait(bar, &bar->sc_full, n & 1))) break;
           fence_after();
+#pragma unroll 1
+          for (int part = 0; part < 4; ++part) {
+            const int block = 4 * h + part, j0 = 16 * block;
+            uint32_t p[8];
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            float x[32];
-            tmem_ld32(lanes + kColS + h * 64 + part * 32, x);
-            const int j0 = h * 64 + part * 32;
-            uint32_t p[16];
+            for (int j = 0; j < 8; ++j) p[j] = 0;
+            const bool diagonal = block >> 1 == q;
+            if (diagonal || (block < 2 * q) != rev) {
+              float x[16];
+              tmem_ld16(lanes + kColS + j0, x);
+              if (diagonal) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              float y[2];
+                for (int j8 = 0; j8 < 16; j8 += 8) {
+                  float d[8];
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int far = C.rev ? j0 + j + e - r : r - (j0 + j + e);
-                y[e] = far >= 0 && j0 + j + e < cnt ? x[j + e] * dec[far >= 0 ? far : 0] : 0.f;
+                  for (int j = 0; j < 8; ++j) d[j] = lds(dec + 4 * abs(r - j0 - j8 - j));
+#pragma unroll
+                  for (int j = 0; j < 8; ++j) {
+                    const int at = j0 + j8 + j;
+                    x[j8 + j] = (rev ? at >= r : at <= r) ? x[j8 + j] * (intra * d[j]) : 0.f;
+                  }
+                }
+              } else {
+                const float base = intra * lds(dec + 4 * (rev ? j0 - r : r - j0 - 15));
+                const float2 b2 = make_float2(base, base);
+                const uint32_t col = dec + 4 * (rev ? 132 : 148);
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                  const uint4 d = lds4(col + 4 * j);
+                  const float2 y0 = __fmul2_rn(make_float2(x[j], x[j + 1]),
+                                               __fmul2_rn(b2, make_float2(__uint_as_float(d.x), __uint_as_float(d.y))));
+                  const float2 y1 = __fmul2_rn(make_float2(x[j + 2], x[j + 3]),
+                                               __fmul2_rn(b2, make_float2(__uint_as_float(d.z), __uint_as_float(d.w))));
+                  x[j] = y0.x;
+                  x[j + 1] = y0.y;
+                  x[j + 2] = y1.x;
+                  x[j + 3] = y1.y;
+                }
               }
-              p[j >> 1] = pack2(y[0], y[1]);
+              if (cnt < kTile) {  // the columns of rows that are not this chunk's
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = j0 + j < cnt ? x[j] : 0.f;
+              }
+#pragma unroll
+              for (int j = 0; j < 16; j += 2) p[j >> 1] = pack2(x[j], x[j + 1]);
             }
-            tmem_st16(lanes + kColS + h * 64 + part * 16, p);
+            tmem_st8(lanes + kColS + h * 64 + part * 8, p);
           }
+          tmem_st_wait();
           fence_before();
           __syncwarp();
           if (lane == 0) arrive(&bar->p_ready);
-          // results
-          if (!(ok = warp_wait(bar, &bar->o2_full, n & 1) && warp_wait(bar, &bar->o1_full, n & 1))) break;
+          // Q X, decayed from the chunk's beginning
+          const float f = inter * lds(dec + 4 * max(rev ? cnt - 1 - r : r + 1, 0));
+          if (!(ok = warp_wait(bar, &bar->o1_full, n & 1))) break;
           fence_after();
-          const int age = C.rev ? cnt - 1 - r : r + 1;
-          const float f = C.inter * dec[age > 0 ? age : 0];
-          const long long token = w.first(C, i) + r;
-          TO* dst = seq::row_ptr<TO>(C.out, token, w.head / C.out_div) + h * 64;
-#pragma unroll
+#pragma unroll 1
           for (int part = 0; part < 2; ++part) {
-            float x[32], y[32];
-            tmem_ld32(lanes + kColO1 + h * 64 + part * 32, x);
-            tmem_ld32(lanes + kColO2 + h * 64 + part * 32, y);
+            float x[32];
+            tmem_ld32(lanes + kColO + h * 64 + part * 32, x);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] *= f;
+            tmem_st32(lanes + kColO + h * 64 + part * 32, x);
+          }
+          tmem_st_wait();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) arrive(&bar->o_ready);
+          // results
+          if (!(ok = warp_wait(bar, &bar->o2_full, n & 1))) break;
+          fence_after();
+          // through this warp's 4 KB of Q's tile (its products are done), 128 bytes a row:
+          // eight lanes then store a row's piece, instead of 32 rows at a time
+          const uint32_t tq = n * kPer;
+          const uint32_t stage = smem_u32(slot_of(tq)) + (warp - kFirstRow) * 4096;
+          constexpr int kParts = sizeof(TO) == 2 ? 1 : 2, kCols = 64 / kParts, kV = 16 / int(sizeof(TO));
+          const int piece = lane & 7, row0 = 32 * q + (lane >> 3);
+          TO* dst = reinterpret_cast<TO*>(C.out.p) + (w.first(C, i) + row0) * pitch + w.head / C.out_div * C.out.hs +
+                    h * 64 + piece * kV;
+#pragma unroll 1
+          for (int part = 0; part < 2; ++part) {
+            float x[32];
+            tmem_ld32(lanes + kColO + h * 64 + part * 32, x);
             if (part == 1) {  // everything has been read
               fence_before();
               __syncwarp();
               if (lane == 0) arrive(&bar->o_free);
             }
-            if (r < cnt) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) x[j] = fmaf(f, x[j], C.intra * y[j]);
-              constexpr int kV = 16 / int(sizeof(TO));
+            for (int j = 0; j < 32; j += kV) {
+              const uint32_t at = stage + lane * 128 + ((((part * 32 % kCols + j) / kV) ^ (lane & 7)) << 4);
+              if (sizeof(TO) == 2)
+                sts4(at, pack2(x[j], x[j + 1]), pack2(x[j + 2], x[j + 3]), pack2(x[j + 4], x[j + 5]),
+                     pack2(x[j + 6], x[j + 7]));
+              else
+                sts4(at, __float_as_uint(x[j]), __float_as_uint(x[j + 1]), __float_as_uint(x[j + 2]),
+                     __float_as_uint(x[j + 3]));
+            }
+            if (part == 1 || kParts == 2) {
+              __syncwarp();
+              const bool wide = h * 64 + (kParts == 2 ? part * 32 : 0) + piece * kV < C.dc;
+              TO* at = dst + (kParts == 2 ? part * 32 : 0);
+#pragma unroll 1
+              for (int k0 = 0; k0 < 8; k0 += 4) {
+                uint4 v[4];
 #pragma unroll
-              for (int j = 0; j < 32; j += kV)
-                if (h * 64 + part * 32 + j < C.dc) {
-                  float t[kV];
-#pragma unroll
-                  for (int e = 0; e < kV; ++e) t[e] = x[j + e];
-                  seq::store_vec<TO, kV>(dst + part * 32 + j, t);
+                for (int k = 0; k < 4; ++k) {
+                  const int row = 4 * (k0 + k) + (lane >> 3);
+                  v[k] = lds4(stage + row * 128 + ((piece ^ (row & 7)) << 4));
                 }
+#pragma unroll
+                for (int k = 0; k < 4; ++k, at += 4 * pitch)
+                  if (wide && row0 + 4 * (k0 + k) < cnt) *reinterpret_cast<uint4*>(at) = v[k];
+              }
+              __syncwarp();
             }
           }
+          fence_async();  // before the tile is loaded again
+          __syncwarp();
+          if (lane == 0) arrive(&bar->empty[tq % kSlots]);
         }
       }
     }
   } else {
-    // ---- planes of decayed K, and the state: row b of X, columns [64 h, 64 h + 64) ----
+    registers_up<112>();
+    // ---- planes of decayed K, and the state: row b of X, columns [64 h, 64 h + 64).  Planes: the
+    // same rows of K^T (lanes of TMEM), tokens [64 h, 64 h + 64) ----
     const int q = warp & 3, h = (warp - kFirstState) >> 2;
     const int b = q * 32 + lane, t = threadIdx.x - 32 * kFirstState;
     const uint32_t lanes = tmem + (uint32_t(q * 32) << 16);
-    uint32_t n = 0, tables = 0;
+    const bool rev = C.rev != 0;
+    uint32_t n = 0, nu = 0, tables = 0;
     bool ok = true;
     auto write_x = [&](const float (&X)[64]) {
-      unsigned char* row = sm + L::kX + h * kPanel + b * 128;
+      const uint32_t row = smem_u32(sm + kX) + h * kPanel + b * 128;
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint4 v;
-        v.x = pack2(X[8 * c], X[8 * c + 1]);
-        v.y = pack2(X[8 * c + 2], X[8 * c + 3]);
-        v.z = pack2(X[8 * c + 4], X[8 * c + 5]);
-        v.w = pack2(X[8 * c + 6], X[8 * c + 7]);
-        *reinterpret_cast<uint4*>(row + ((c ^ (b & 7)) << 4)) = v;
-      }
+      for (int c = 0; c < 8; ++c)
+        sts4(row + ((c ^ (b & 7)) << 4), pack2(X[8 * c], X[8 * c + 1]), pack2(X[8 * c + 2], X[8 * c + 3]),
+             pack2(X[8 * c + 4], X[8 * c + 5]), pack2(X[8 * c + 6], X[8 * c + 7]));
       fence_async();
       __syncwarp();
       if (lane == 0) arrive(&bar->x_ready);
     };
-    for (long long item = blockIdx.x; item < items && ok; item += gridDim.x) {
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
       if (!walk_of<STATES>(C, item, &w)) continue;
-      const long long entry = item;  // slot * heads + head
-      const long long slot = lin::state_slot(C, w.g.seq);
+      const long long slot = lin::state_slot(C, w.seq);
       const float gl = lin::log_decay_of(C, w.head);
-      const float* dec = make_table(bar, &bar->state_table, reinterpret_cast<float*>(sm + L::kTables) + 2 * kTable,
-                                    tables++, t, gl, &ok);
+      // forwards, token j of a full chunk decays by l^(127 - j); backwards by l^(j + 1)
+      const uint32_t dec = make_table(bar, &bar->state_table, reinterpret_cast<float*>(sm + kStateTables), kStateTable, tables++, t, &ok, [&](int j) {
+                                      return C.upd * expf(gl * static_cast<float>(C.rev ? j + 1 : kTile - 1 - j));
+                                    });
       if (!ok) break;
       float X[64];
       const float* src = nullptr;
       int src_t = 0;
       if (!STATES) {
         if (C.seg_state) {
-          src = C.seg_state + entry * C.db * C.dc;
+          src = C.seg_state + static_cast<long long>(item) * C.db * C.dc;  // item = segment slot * heads + head
         } else if (C.init && slot >= 0) {
           src = C.init + (slot * C.heads + w.head) * C.db * C.dc;
           src_t = C.init_t;
@@ -476,14 +631,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 64; ++c) X[c] = 0.f;
       }
-      if (!STATES && w.n > 0) {
-        // the product that read the last chunk's X is done
-        if (n > 0 && !(ok = warp_wait(bar, &bar->o1_full, (n - 1) & 1))) break;
-        write_x(X);
-      }
       for (int i = 0; i < w.n; ++i, ++n) {
         const int cnt = w.rows(i);
         const uint32_t tk = n * kPer + kPer - 2, tv = tk + 1;
+        const bool update = i < w.updates;
+        if (!STATES) {  // once the product that read the last chunk's X is done
+          if (n > 0 && !(ok = warp_wait(bar, &bar->o1_full, (n - 1) & 1))) break;
+          write_x(X);
+        }
         if (!(ok = warp_wait(bar, &bar->full[tk % kSlots], (tk / kSlots) & 1))) break;
         if (cnt < kTile) {
           if (!(ok = warp_wait(bar, &bar->full[tv % kSlots], (tv / kSlots) & 1))) break;
@@ -491,60 +646,86 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = t; e < (kTile - cnt) * 16; e += 256)
             *reinterpret_cast<uint4*>(v + (e & 1) * kPanel + (cnt + (e >> 4)) * 128 + ((e >> 1) & 7) * 16) =
                 make_uint4(0, 0, 0, 0);
+          fence_async();
         }
-        if (!STATES && !(ok = warp_wait(bar, &bar->sc_full, n & 1))) break;  // Sc has read K
-        unsigned char* k = slot_of(tk);
-        unsigned char* more = sm + L::kPlanes;
-#pragma unroll 2
-        for (int e = t; e < 2 * kTile * 8; e += 256) {
-          const int j = (e >> 3) & (kTile - 1);  // 16-byte piece e of the tile; its row
-          const int age = C.rev ? j + 1 : cnt - 1 - j;
-          const float d = C.upd * dec[age >= 0 ? age : 0];
-          uint4 raw4 = *reinterpret_cast<const uint4*>(k + e * 16);
-          uint32_t in[4] = {raw4.x, raw4.y, raw4.z, raw4.w}, out[3][4];
+        if (update) {
+          // tile m of an ldmatrix: rows 8 (m & 1) .. of 16 lanes, tokens 8 (m >> 1) .. of 16
+          const int m = lane >> 3;
+          const uint32_t panel = smem_u32(slot_of(tk)) + (q >> 1) * kPanel;
+          const int shift = rev ? 0 : kTile - cnt;
+          auto make_planes = [&](auto from, auto to) {  // planes from .. to - 1
+#pragma unroll 1
+            for (int g = 0; g < 4; ++g) {
+              const int row = 64 * h + 16 * g + 8 * (m >> 1) + (lane & 7);
+              float2 d[2];
 #pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            float lo = j < cnt ? low_half(in[z]) * d : 0.f, hi = j < cnt ? high_half(in[z]) * d : 0.f;
+              for (int z = 0; z < 2; ++z) {  // (rows past the end are zero whatever their decay)
+                const int j = 64 * h + 16 * g + 8 * z + 2 * (lane & 3) + shift;
+                d[z] = make_float2(lds(dec + 4 * min(j, kTile - 1)), lds(dec + 4 * min(j + 1, kTile - 1)));
+              }
 #pragma unroll
-            for (int p = 0; p < PLANES; ++p) {
-              out[p][z] = pack2(lo, hi);
-              lo -= low_half(out[p][z]);
-              hi -= high_half(out[p][z]);
+              for (int half = 0; half < 2; ++half) {
+                uint32_t k[4], out[PLANES][4];
+                ldmatrix_t4(panel + row * 128 + (((4 * (q & 1) + 2 * half + (m & 1)) ^ (row & 7)) << 4), k);
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                  if (cnt < kTile) {
+                    const int j = 64 * h + 16 * g + 8 * (z >> 1) + 2 * (lane & 3);
+                    k[z] &= (j < cnt ? 0xffffu : 0u) | (j + 1 < cnt ? 0xffff0000u : 0u);
+                  }
+                  float2 x = __fmul2_rn(make_float2(low_half(k[z]), high_half(k[z])), d[z >> 1]);
+#pragma unroll
+                  for (int p = 0; p < to.value; ++p) {
+                    out[p][z] = pack2(x.x, x.y);
+                    x = __fadd2_rn(x, make_float2(-low_half(out[p][z]), -high_half(out[p][z])));
+                  }
+                }
+                const uint32_t at = lanes + (uint32_t(16 * half) << 16) + 8 * g;
+#pragma unroll
+                for (int p = from.value; p < to.value; ++p) tmem_st_tiles(at + plane_col<STATES>(p, h), out[p]);
+              }
             }
+          };
+          if (STATES) {
+            make_planes(Int<0>{}, Int<PLANES>{});
+          } else {
+            make_planes(Int<1>{}, Int<PLANES>{});
+            // plane 0's columns are Sc's until P is made
+            if (!(ok = warp_wait(bar, &bar->p_ready, n & 1))) break;
+            fence_after();
+            make_planes(Int<0>{}, Int<1>{});
           }
-          *reinterpret_cast<uint4*>(k + e * 16) = make_uint4(out[0][0], out[0][1], out[0][2], out[0][3]);
-#pragma unroll
-          for (int p = 1; p < PLANES; ++p)
-            *reinterpret_cast<uint4*>(more + (p - 1) * kTileBytes + e * 16) =
-                make_uint4(out[p][0], out[p][1], out[p][2], out[p][3]);
+          tmem_st_wait();
+          fence_before();
         }
-        fence_async();
         __syncwarp();
-        if (lane == 0) arrive(&bar->planes_ready);
-        if (!(ok = warp_wait(bar, &bar->u_full, n & 1))) break;
-        fence_after();
-        const float keep = dec[cnt];
-#pragma unroll
-        for (int part = 0; part < 2; ++part) {
-          float x[32];
-          tmem_ld32(lanes + kColU + h * 64 + part * 32, x);
-#pragma unroll
-          for (int c = 0; c < 32; ++c) X[part * 32 + c] = fmaf(keep, X[part * 32 + c], x[c]);
+        if (lane == 0) {
+          arrive(&bar->planes_ready);
+          arrive(&bar->empty[tk % kSlots]);
         }
-        fence_before();
-        __syncwarp();
-        if (lane == 0) arrive(&bar->u_free);
-        if (!STATES && i + 1 < w.n) {
-          if (!(ok = warp_wait(bar, &bar->o1_full, n & 1))) break;  // O1 has read X
-          write_x(X);
+        if (update) {
+          if (!(ok = warp_wait(bar, &bar->u_full, nu & 1))) break;
+          ++nu;
+          fence_after();
+          const float keep = expf(gl * static_cast<float>(cnt));
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            float x[32];
+            tmem_ld32(lanes + kColU + h * 64 + part * 32, x);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) X[part * 32 + c] = fmaf(keep, X[part * 32 + c], x[c]);
+          }
+          fence_before();
+          __syncwarp();
+          if (lane == 0) arrive(&bar->u_free);
         }
       }
       if (!ok) break;
       float* dst = nullptr;
       int dst_t = 0;
       if (STATES) {
-        dst = C.seg_state + entry * C.db * C.dc;
-      } else if (C.fin && slot >= 0 && w.g.idx == w.g.count - 1) {
+        dst = C.seg_state + static_cast<long long>(item) * C.db * C.dc;
+      } else if (C.fin && slot >= 0 && w.last) {
         dst = C.fin + (slot * C.heads + w.head) * C.db * C.dc;
         dst_t = C.fin_t;
       }
@@ -598,12 +779,12 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, con
   static cudaError_t attr = cudaSuccess;
   std::call_once(once, [] {
     attr = cudaFuncSetAttribute(chain_tc_kernel<TO, STATES, PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                int(Shape<STATES>::kBytes));
+                                int(kSmem));
   });
   TO_CUDA_TRY(attr);
-  const long long items = (C.seg_state ? lin::segment_slots(C.tokens, C.nseq, C.seg) : C.nseq) * C.heads;
+  const int items = (C.seg_state ? lin::segment_slots(C.tokens, C.nseq, C.seg) : C.nseq) * C.heads;
   chain_tc_kernel<TO, STATES, PLANES>
-      <<<unsigned(items < sms ? items : sms), kThreads, Shape<STATES>::kBytes, s>>>(a, b, c, C, items);
+      <<<unsigned(items < sms ? items : sms), kThreads, kSmem, s>>>(a, b, c, C, items);
   TO_CUDA_TRY(cudaGetLastError());
   return ok();
 }
@@ -636,7 +817,8 @@ namespace lin {
 // whose results can be stored 16 bytes at a time.
 bool tc_takes(const Chain& C, bool f32_out) {
   const int per = f32_out ? 4 : 8;
-  return C.tokens > 0 && C.db <= kTile && C.dc <= kTile && rows_fit(C.a, C.heads / C.a_div, C.tokens) &&
+  const long long items = (C.seg_state ? lin::segment_slots(C.tokens, C.nseq, C.seg) : C.nseq) * 1ll * C.heads;
+  return C.tokens > 0 && items < INT32_MAX / 2 && C.db <= kTile && C.dc <= kTile && rows_fit(C.a, C.heads / C.a_div, C.tokens) &&
          rows_fit(C.b, C.heads / C.b_div, C.tokens) && rows_fit(C.c, C.heads / C.c_div, C.tokens) &&
          C.dc % per == 0 && aligned(C.out.p, 16) && C.out.ts % per == 0 && C.out.hs % per == 0;
 }
