@@ -20,10 +20,10 @@
 // state), smallest plane first, so few sums pass through the accumulator at
 // full size; a chunk's U is added to X in IEEE f32 registers.
 //
-// Roles (20 warps): one lane issues TMA loads into a ring of six 32 KB tiles
-// (two chunks), one the products; warps 4-11 turn Sc into P, scale O and store
-// the results (a thread: one row, 64 columns); warps 12-19 make the planes and
-// hold X (a thread: one row, 64 columns).  Products are issued Sc, Q X, U, P V:
+// Roles (20 warps): one lane issues TMA loads into two stages of three
+// 32 KB tiles, one the products; warps 4-11 turn Sc into P (and make plane 0,
+// whose columns are theirs), scale O and store the results (a thread: one row,
+// 64 columns); warps 12-19 make the other planes and hold X (a thread: one row, 64 columns).  Products are issued Sc, Q X, U, P V:
 // the next chunk's Sc and the row warps run under the state's update.  Rows
 // past a chunk's end are masked: P and the planes by selection, V by zeroing
 // its rows, since 0 * NaN is not 0.  Rows of a reversed chain keep their order
@@ -55,7 +55,8 @@ constexpr int kRowWarps = 8, kStateWarps = 8;    // P and out; planes and X
 constexpr int kFirstRow = 4, kFirstState = kFirstRow + kRowWarps;  // warps 0, 1: loads, products; 2, 3: none
 constexpr int kThreads = 32 * (kFirstState + kStateWarps);
 constexpr uint32_t kMaxPolls = 1u << 22;
-constexpr int kSlots = 6;                        // tiles of the ring
+constexpr int kStages = 2;                       // chunks in shared memory: tiles Q, K, V of each
+constexpr uint32_t kStageBytes = 3 * kTileBytes;
 
 // TMEM columns.  P of tokens [0, 64) and [64, 128) overwrites the first halves
 // of those tokens' columns of Sc; plane 0 takes the second halves, once Sc has
@@ -67,9 +68,9 @@ __device__ __forceinline__ uint32_t plane_col(int plane, int token64) {
 }
 
 struct Barriers {
-  uint64_t full[kSlots], empty[kSlots];
+  uint64_t full[kStages], empty[kStages];
   uint64_t sc_full, p_ready, o1_full, o_ready, o2_full, o_free;
-  uint64_t planes_ready, u_full, u_free, x_ready;
+  uint64_t planes_ready, u_full, x_ready;
   uint64_t row_table, state_table;
   uint32_t tmem;
   int abort;
@@ -90,8 +91,9 @@ __device__ __forceinline__ bool warp_wait(Barriers* b, uint64_t* bar, uint32_t p
   return __all_sync(0xffffffffu, wait_for(b, bar, parity));
 }
 
-// The same value, which the compiler takes for a new one: what is computed from
-// it is not kept in registers from one chunk to the next.
+// The same value, which the compiler takes for a new one: the descriptors made
+// from it are not kept from one chunk to the next (they overflowed the uniform
+// registers).
 __device__ __forceinline__ uint32_t fresh(uint32_t x) {
   asm volatile("" : "+r"(x));
   return x;
@@ -101,12 +103,12 @@ __device__ __forceinline__ void arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-__device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, int head, int token, uint64_t* bar) {
+__device__ __forceinline__ void tma_tile(uint32_t dst, const CUtensorMap* map, int head, int token, uint64_t* bar) {
 #pragma unroll
   for (int p = 0; p < 2; ++p)
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-        ::"r"(smem_u32(dst) + p * kPanel), "l"(map), "r"(64 * p), "r"(head), "r"(token), "r"(smem_u32(bar))
+        ::"r"(dst + p * kPanel), "l"(map), "r"(64 * p), "r"(head), "r"(token), "r"(smem_u32(bar))
         : "memory");
 }
 
@@ -114,31 +116,33 @@ __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, int 
 // contiguous K values): 8-row groups 1024 bytes apart.  MN-major ones (rows of
 // 64 contiguous M or N values, one row a K value): 8-K groups 1024 bytes apart
 // (stride offset), the two 64-value panels kPanel apart (leading offset).
-__device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t lbo) {
-  return (uint64_t((saddr >> 4) & 0x3FFFu)) | (uint64_t((lbo >> 4) & 0x3FFFu) << 16) |
-         (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+// The upper word is the same for both; steps add to the lower one (no carry:
+// shared addresses end below 2^18).
+constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t tile, int step) {  // 16 K values a step
+  return ((tile >> 4) | (1u << 16)) + (step >> 2) * (kPanel >> 4) + (step & 3) * 2;
 }
-__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int step) {  // 16 K values a step
-  return desc(tile + (step >> 2) * kPanel + (step & 3) * 32, 16);
+__device__ __forceinline__ uint32_t desc_mn(uint32_t tile, int step) {
+  return ((tile >> 4) | ((kPanel >> 4) << 16)) + step * 128;
 }
-__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int step) { return desc(tile + step * 2048, kPanel); }
 
 // D f32, A and B bf16, M = N = 128; bit 16: B is MN-major
 constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(kTile >> 3) << 17) |
                             (uint32_t(kTile >> 4) << 24);
 constexpr uint32_t kMnB = 1u << 16;
 
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(kDescHigh), "r"(uint32_t(add)) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add)) : "memory");
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 db, {%2, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(kDescHigh), "r"(uint32_t(add)) : "memory");
 }
 __device__ __forceinline__ void commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
@@ -231,7 +235,7 @@ __device__ __forceinline__ float high_half(uint32_t r) { return __uint_as_float(
 // count.  Two tables in turn: a warp that has passed an item's barrier knows
 // that all have left the table before the last.
 constexpr int kRowTable = 164;    // l^n, n = 0 .. 128; the 32 factors of a block's columns from 132 on
-constexpr int kStateTable = 128;  // decay of each token of a full chunk
+constexpr int kStateTable = 132;  // l^n, n = 0 .. 128
 template <typename F>
 __device__ __forceinline__ uint32_t make_table(Barriers* b, uint64_t* bar, float* tables, int size, uint32_t turn,
                                                int t, bool* ok, F f) {
@@ -273,21 +277,67 @@ __device__ __forceinline__ bool walk_of(const Chain& C, int item, Walk* w) {
   return true;
 }
 
-template <int N>
-struct Int {
-  static constexpr int value = N;
-};
+// Planes FROM .. TO-1 of decayed K: lanes [32 q, 32 q + 32) of K^T, tokens [64 h,
+// 64 h + 64), from the chunk's tile of K.  All but the last plane are cut off, not
+// rounded, so each is the product's own next eight bits.
+template <bool STATES, int PLANES, int FROM, int TO>
+__device__ __forceinline__ void make_planes(uint32_t tile, uint32_t lanes, uint32_t dec, int cnt, bool rev, float upd,
+                                            int q, int h, int lane) {
+  const uint32_t panel = tile + (q >> 1) * kPanel;
+  if (cnt < kTile) {  // rows past the end: zero what this warp reads
+    for (int e = lane; e < 256; e += 32) {
+      const int row = 64 * h + (e >> 2);
+      if (row >= cnt) sts4(panel + row * 128 + (((4 * (q & 1) + (e & 3)) ^ (row & 7)) << 4), 0, 0, 0, 0);
+    }
+    fence_async();  // before the tile is loaded again
+    __syncwarp();
+  }
+  // tile m of an ldmatrix: rows 8 (m & 1) .. of 16 lanes, tokens 8 (m >> 1) .. of 16
+  const int m = lane >> 3;
+#pragma unroll 1
+  for (int g = 0; g < 4; ++g) {
+    const int row = 64 * h + 16 * g + 8 * (m >> 1) + (lane & 7);
+    float2 d[2];
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const int j = 64 * h + 16 * g + 8 * z + 2 * (lane & 3), age = rev ? j + 1 : cnt - 1 - j;
+      d[z] = make_float2(upd * lds(dec + 4 * max(age, 0)), upd * lds(dec + 4 * max(rev ? age + 1 : age - 1, 0)));
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t k[4], out[PLANES][4];
+      ldmatrix_t4(panel + row * 128 + (((4 * (q & 1) + 2 * half + (m & 1)) ^ (row & 7)) << 4), k);
+#pragma unroll
+      for (int z = 0; z < 4; ++z) {
+        float2 x = __fmul2_rn(make_float2(low_half(k[z]), high_half(k[z])), d[z >> 1]);
+#pragma unroll
+        for (int p = 0; p < TO; ++p) {
+          out[p][z] = p == PLANES - 1 ? pack2(x.x, x.y)
+                                      : __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
+          if (p + 1 < TO)
+            x = __ffma2_rn(make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffff0000u),
+                                       __uint_as_float(__float_as_uint(x.y) & 0xffff0000u)),
+                           make_float2(-1.f, -1.f), x);
+        }
+      }
+#pragma unroll
+      for (int p = FROM; p < TO; ++p)
+        tmem_st_tiles(lanes + (uint32_t(16 * half) << 16) + 8 * g + plane_col<STATES>(p, h), out[p]);
+    }
+  }
+  tmem_st_wait();
+}
 
 // Shared memory
-constexpr uint32_t kX = kSlots * kTileBytes;                             // bf16 X
+constexpr uint32_t kX = kStages * kStageBytes;                             // bf16 X
 constexpr uint32_t kRowTables = kX + kTileBytes;
 constexpr uint32_t kStateTables = kRowTables + 2 * kRowTable * 4;
 constexpr uint32_t kBars = kStateTables + 2 * kStateTable * 4;
 constexpr uint32_t kSmem = kBars + sizeof(Barriers);
 static_assert(kBars % 8 == 0 && kSmem <= 232448, "shared memory of a CTA");
 
-// Registers: the launch gives each of the 20 warps 96; the idle-handed warps
-// return some of theirs (4 * 48 + 8 * 104 + 8 * 112 = 1920 = 20 * 96).  No kernel may
+// Registers: the launch gives each of the 20 warps 96; those that hold X take some of
+// the others' (4 * 64 + 8 * 88 + 8 * 120 = 1920 = 20 * 96).  No kernel may
 // spill: with the shared memory taken, a spilled register comes back from L2.  Loops
 // stay rolled where registers allow it: the roles run different code at the same time,
 // and unrolled they outgrow the instruction caches (stalls for want of instructions were
@@ -302,7 +352,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     chain_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
                     const __grid_constant__ CUtensorMap mapC, const __grid_constant__ Chain C,
                     const int items) {
-  constexpr int kPer = STATES ? 2 : 3;  // tiles of a chunk: (Q,) K, V
   extern __shared__ __align__(1024) unsigned char sm[];
   if (smem_u32(sm) & 1023) {  // the swizzled tiles need it; there is no room left to round up in
     if (threadIdx.x == 0) atomicExch(&g_sequence_status, int(TO_ERR_SCRATCH));
@@ -312,12 +361,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kSlots; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(&bar->full[i], 1);
-      // V is freed by a commit, K by one and by the warps that read it into the planes,
-      // Q by the warps that the results pass through it
-      const int x = i % kPer;
-      mbar_init(&bar->empty[i], x == kPer - 1 ? 1 : x == kPer - 2 ? kStateWarps + (STATES ? 0 : 1) : kRowWarps);
+      // a chunk's tiles are free when its products are done (a commit), its planes made and
+      // its results, which pass through Q's tile, stored
+      mbar_init(&bar->empty[i], 1 + kStateWarps + (STATES ? 0 : kRowWarps));
     }
     mbar_init(&bar->sc_full, 1);
     mbar_init(&bar->p_ready, kRowWarps);
@@ -327,7 +375,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar->o_free, kRowWarps);
     mbar_init(&bar->planes_ready, kStateWarps);
     mbar_init(&bar->u_full, 1);
-    mbar_init(&bar->u_free, kStateWarps);
     mbar_init(&bar->x_ready, kStateWarps);
     mbar_init(&bar->row_table, kRowWarps);
     mbar_init(&bar->state_table, kStateWarps);
@@ -343,86 +390,80 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = bar->tmem;
-  auto slot_of = [&](uint32_t tile) { return sm + (tile % kSlots) * kTileBytes; };
+  const uint32_t base = smem_u32(sm);
+  auto stage_of = [&](uint32_t n) { return base + (n & 1) * kStageBytes; };
   Walk w;
 
   if (warp < kFirstRow) {
-    registers_down<48>();
+    registers_down<64>();
     if (warp == 0 && lane == 0) {
-      // ---- loads: (Q,) K, V of each chunk, in ring order ----
-      uint32_t tile = 0;
+      // ---- loads: (Q,) K, V of each chunk ----
+      uint32_t n = 0;
       bool ok = true;
       for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
         if (!walk_of<STATES>(C, item, &w)) continue;
-        for (int i = 0; i < w.n && ok; ++i) {
+        for (int i = 0; i < w.n; ++i, ++n) {
           const int token = w.first(C, i);
-          for (int x = 0; x < kPer; ++x, ++tile) {
-            const uint32_t s = tile % kSlots;
-            if (tile >= kSlots && !(ok = wait_for(bar, &bar->empty[s], (tile / kSlots - 1) & 1))) break;
-            mbar_arrive_expect_tx(&bar->full[s], kTileBytes);
-            if (x == kPer - 1) tma_tile(slot_of(tile), &mapC, w.head / C.c_div, token, &bar->full[s]);
-            else if (x == kPer - 2) tma_tile(slot_of(tile), &mapB, w.head / C.b_div, token, &bar->full[s]);
-            else tma_tile(slot_of(tile), &mapA, w.head / C.a_div, token, &bar->full[s]);
-          }
+          uint64_t* full = &bar->full[n & 1];
+          if (n >= kStages && !(ok = wait_for(bar, &bar->empty[n & 1], (n / kStages - 1) & 1))) break;
+          mbar_arrive_expect_tx(full, STATES ? 2 * kTileBytes : kStageBytes);
+          if (!STATES) tma_tile(stage_of(n), &mapA, w.head / C.a_div, token, full);
+          tma_tile(stage_of(n) + kTileBytes, &mapB, w.head / C.b_div, token, full);
+          tma_tile(stage_of(n) + 2 * kTileBytes, &mapC, w.head / C.c_div, token, full);
         }
       }
       // copies still in flight land before the CTA ends
-      for (uint32_t t = tile > kSlots ? tile - kSlots : 0; t < tile; ++t)
-        mbar_wait_bounded(&bar->full[t % kSlots], (t / kSlots) & 1, kMaxPolls);
+      for (uint32_t t = n > kStages ? n - kStages : 0; t < n; ++t)
+        mbar_wait_bounded(&bar->full[t & 1], (t / kStages) & 1, kMaxPolls);
     } else if (warp == 1 && lane == 0) {
       // ---- products ----
-      uint32_t n = 0, nu = 0;  // chunks and updates so far
+      uint32_t n = 0;  // chunks so far
       bool ok = true;
       for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
         if (!walk_of<STATES>(C, item, &w)) continue;
-        for (int i = 0; i < w.n && ok; ++i, ++n) {
-          const uint32_t tq = n * kPer, tk = tq + kPer - 2, tv = tk + 1;
-          const uint32_t sk = fresh(smem_u32(slot_of(tk))), sv = fresh(smem_u32(slot_of(tv)));
-          auto full = [&](uint32_t t) { return wait_for(bar, &bar->full[t % kSlots], (t / kSlots) & 1); };
+        for (int i = 0; i < w.n; ++i, ++n) {
+          const uint32_t turn = n & 1, sq = fresh(stage_of(n)), sk = sq + kTileBytes, sv = sk + kTileBytes;
+          const uint32_t tm = fresh(tmem), sx = fresh(base) + kX;
+          if (!(ok = wait_for(bar, &bar->full[turn], (n / kStages) & 1))) break;
           if (!STATES) {
-            const uint32_t sq = fresh(smem_u32(slot_of(tq))), sx = fresh(smem_u32(sm + kX));
-            if (!(ok = full(tq) && full(tk))) break;
             fence_after();
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)
-              mma(tmem + kColS, desc_k(sq, k), desc_k(sk, k), kIdesc, k > 0);
+              mma(tm + kColS, desc_k(sq, k), desc_k(sk, k), kIdesc, k > 0);
             commit(&bar->sc_full);
-            commit(&bar->empty[tk % kSlots]);
-            if (!(ok = wait_for(bar, &bar->x_ready, n & 1) && (n == 0 || wait_for(bar, &bar->o_free, (n - 1) & 1)))) break;
+            if (!(ok = wait_for(bar, &bar->x_ready, turn) && (n == 0 || wait_for(bar, &bar->o_free, turn ^ 1)))) break;
             fence_after();
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)
-              mma(tmem + kColO, desc_k(sq, k), desc_mn(sx, k), kIdesc | kMnB, k > 0);
+              mma(tm + kColO, desc_k(sq, k), desc_mn(sx, k), kIdesc | kMnB, k > 0);
             commit(&bar->o1_full);
           }
-          // planes_ready also says that V's rows past the end are zero
-          if (!(ok = full(tv) && wait_for(bar, &bar->planes_ready, n & 1))) break;
+          // also: V's rows past the end are zero, and the last chunk's U has been read
+          if (!(ok = wait_for(bar, &bar->planes_ready, turn) && (STATES || wait_for(bar, &bar->p_ready, turn)))) break;
+          fence_after();
           if (i < w.updates) {
-            if (nu > 0 && !(ok = wait_for(bar, &bar->u_free, (nu - 1) & 1))) break;
-            fence_after();
-#pragma unroll
+#pragma unroll 1
             for (int p = PLANES - 1; p >= 0; --p)
-#pragma unroll 4
+#pragma unroll
               for (int k = 0; k < kTile / 16; ++k)  // 16 tokens: 8 columns
-                mma_ts(tmem + kColU, tmem + plane_col<STATES>(p, k >> 2) + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB,
+                mma_ts(tm + kColU, tm + plane_col<STATES>(p, k >> 2) + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB,
                        p < PLANES - 1 || k > 0);
             commit(&bar->u_full);
-            ++nu;
           }
           if (!STATES) {
-            if (!(ok = wait_for(bar, &bar->p_ready, n & 1) && wait_for(bar, &bar->o_ready, n & 1))) break;
+            if (!(ok = wait_for(bar, &bar->o_ready, turn))) break;
             fence_after();
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)
-              mma_ts(tmem + kColO, tmem + kColS + (k >> 2) * 64 + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB, true);
+              mma_ts(tm + kColO, tm + kColS + (k >> 2) * 64 + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB, true);
             commit(&bar->o2_full);
           }
-          commit(&bar->empty[tv % kSlots]);
+          commit(&bar->empty[turn]);
         }
       }
     }
   } else if (warp < kFirstState) {
-    registers_up<104>();
+    registers_down<88>();
     if (!STATES) {
       // ---- P, O and the results: row r of the chunk, columns [64 h, 64 h + 64) ----
       const int q = warp & 3, h = (warp - kFirstRow) >> 2;
@@ -496,7 +537,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_st8(lanes + kColS + h * 64 + part * 8, p);
           }
-          tmem_st_wait();
+          // plane 0 into the other half of this warp's columns of Sc
+          if (i < w.updates)
+            make_planes<STATES, PLANES, 0, 1>(stage_of(n) + kTileBytes, lanes, dec, cnt, rev, C.upd, q, h, lane);
+          else
+            tmem_st_wait();
           fence_before();
           __syncwarp();
           if (lane == 0) arrive(&bar->p_ready);
@@ -521,8 +566,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_after();
           // through this warp's 4 KB of Q's tile (its products are done), 128 bytes a row:
           // eight lanes then store a row's piece, instead of 32 rows at a time
-          const uint32_t tq = n * kPer;
-          const uint32_t stage = smem_u32(slot_of(tq)) + (warp - kFirstRow) * 4096;
+          const uint32_t stage = stage_of(n) + (warp - kFirstRow) * 4096;
           constexpr int kParts = sizeof(TO) == 2 ? 1 : 2, kCols = 64 / kParts, kV = 16 / int(sizeof(TO));
           const int piece = lane & 7, row0 = 32 * q + (lane >> 3);
           TO* dst = reinterpret_cast<TO*>(C.out.p) + (w.first(C, i) + row0) * pitch + w.head / C.out_div * C.out.hs +
@@ -567,12 +611,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           fence_async();  // before the tile is loaded again
           __syncwarp();
-          if (lane == 0) arrive(&bar->empty[tq % kSlots]);
+          if (lane == 0) arrive(&bar->empty[n & 1]);
         }
       }
     }
   } else {
-    registers_up<112>();
+    registers_up<120>();
     // ---- planes of decayed K, and the state: row b of X, columns [64 h, 64 h + 64).  Planes: the
     // same rows of K^T (lanes of TMEM), tokens [64 h, 64 h + 64) ----
     const int q = warp & 3, h = (warp - kFirstState) >> 2;
@@ -593,17 +637,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
       if (!walk_of<STATES>(C, item, &w)) continue;
-      const long long slot = lin::state_slot(C, w.seq);
       const float gl = lin::log_decay_of(C, w.head);
-      // forwards, token j of a full chunk decays by l^(127 - j); backwards by l^(j + 1)
-      const uint32_t dec = make_table(bar, &bar->state_table, reinterpret_cast<float*>(sm + kStateTables), kStateTable, tables++, t, &ok, [&](int j) {
-                                      return C.upd * expf(gl * static_cast<float>(C.rev ? j + 1 : kTile - 1 - j));
-                                    });
+      const uint32_t dec = make_table(bar, &bar->state_table, reinterpret_cast<float*>(sm + kStateTables), kStateTable,
+                                      tables++, t, &ok, [&](int e) { return expf(gl * static_cast<float>(e)); });
       if (!ok) break;
       float X[64];
       const float* src = nullptr;
       int src_t = 0;
       if (!STATES) {
+        const long long slot = lin::state_slot(C, w.seq);
         if (C.seg_state) {
           src = C.seg_state + static_cast<long long>(item) * C.db * C.dc;  // item = segment slot * heads + head
         } else if (C.init && slot >= 0) {
@@ -633,81 +675,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int i = 0; i < w.n; ++i, ++n) {
         const int cnt = w.rows(i);
-        const uint32_t tk = n * kPer + kPer - 2, tv = tk + 1;
         const bool update = i < w.updates;
         if (!STATES) {  // once the product that read the last chunk's X is done
           if (n > 0 && !(ok = warp_wait(bar, &bar->o1_full, (n - 1) & 1))) break;
           write_x(X);
         }
-        if (!(ok = warp_wait(bar, &bar->full[tk % kSlots], (tk / kSlots) & 1))) break;
+        if (!(ok = warp_wait(bar, &bar->full[n & 1], (n / kStages) & 1))) break;
         if (cnt < kTile) {
-          if (!(ok = warp_wait(bar, &bar->full[tv % kSlots], (tv / kSlots) & 1))) break;
-          unsigned char* v = slot_of(tv);
+          const uint32_t v = stage_of(n) + 2 * kTileBytes;
           for (int e = t; e < (kTile - cnt) * 16; e += 256)
-            *reinterpret_cast<uint4*>(v + (e & 1) * kPanel + (cnt + (e >> 4)) * 128 + ((e >> 1) & 7) * 16) =
-                make_uint4(0, 0, 0, 0);
+            sts4(v + (e & 1) * kPanel + (cnt + (e >> 4)) * 128 + ((e >> 1) & 7) * 16, 0, 0, 0, 0);
           fence_async();
         }
         if (update) {
-          // tile m of an ldmatrix: rows 8 (m & 1) .. of 16 lanes, tokens 8 (m >> 1) .. of 16
-          const int m = lane >> 3;
-          const uint32_t panel = smem_u32(slot_of(tk)) + (q >> 1) * kPanel;
-          const int shift = rev ? 0 : kTile - cnt;
-          auto make_planes = [&](auto from, auto to) {  // planes from .. to - 1
-#pragma unroll 1
-            for (int g = 0; g < 4; ++g) {
-              const int row = 64 * h + 16 * g + 8 * (m >> 1) + (lane & 7);
-              float2 d[2];
-#pragma unroll
-              for (int z = 0; z < 2; ++z) {  // (rows past the end are zero whatever their decay)
-                const int j = 64 * h + 16 * g + 8 * z + 2 * (lane & 3) + shift;
-                d[z] = make_float2(lds(dec + 4 * min(j, kTile - 1)), lds(dec + 4 * min(j + 1, kTile - 1)));
-              }
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                uint32_t k[4], out[PLANES][4];
-                ldmatrix_t4(panel + row * 128 + (((4 * (q & 1) + 2 * half + (m & 1)) ^ (row & 7)) << 4), k);
-#pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                  if (cnt < kTile) {
-                    const int j = 64 * h + 16 * g + 8 * (z >> 1) + 2 * (lane & 3);
-                    k[z] &= (j < cnt ? 0xffffu : 0u) | (j + 1 < cnt ? 0xffff0000u : 0u);
-                  }
-                  float2 x = __fmul2_rn(make_float2(low_half(k[z]), high_half(k[z])), d[z >> 1]);
-#pragma unroll
-                  for (int p = 0; p < to.value; ++p) {
-                    out[p][z] = pack2(x.x, x.y);
-                    x = __fadd2_rn(x, make_float2(-low_half(out[p][z]), -high_half(out[p][z])));
-                  }
-                }
-                const uint32_t at = lanes + (uint32_t(16 * half) << 16) + 8 * g;
-#pragma unroll
-                for (int p = from.value; p < to.value; ++p) tmem_st_tiles(at + plane_col<STATES>(p, h), out[p]);
-              }
-            }
-          };
-          if (STATES) {
-            make_planes(Int<0>{}, Int<PLANES>{});
-          } else {
-            make_planes(Int<1>{}, Int<PLANES>{});
-            // plane 0's columns are Sc's until P is made
-            if (!(ok = warp_wait(bar, &bar->p_ready, n & 1))) break;
-            fence_after();
-            make_planes(Int<0>{}, Int<1>{});
-          }
-          tmem_st_wait();
+          make_planes<STATES, PLANES, STATES ? 0 : 1, PLANES>(stage_of(n) + kTileBytes, lanes, dec, cnt, rev, C.upd, q, h,
+                                                              lane);
           fence_before();
         }
         __syncwarp();
         if (lane == 0) {
           arrive(&bar->planes_ready);
-          arrive(&bar->empty[tk % kSlots]);
+          arrive(&bar->empty[n & 1]);
         }
         if (update) {
           if (!(ok = warp_wait(bar, &bar->u_full, nu & 1))) break;
           ++nu;
           fence_after();
-          const float keep = expf(gl * static_cast<float>(cnt));
+          const float keep = lds(dec + 4 * cnt);
 #pragma unroll
           for (int part = 0; part < 2; ++part) {
             float x[32];
@@ -715,9 +709,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int c = 0; c < 32; ++c) X[part * 32 + c] = fmaf(keep, X[part * 32 + c], x[c]);
           }
-          fence_before();
-          __syncwarp();
-          if (lane == 0) arrive(&bar->u_free);
+          fence_before();  // (the next chunk's planes_ready says that U has been read)
         }
       }
       if (!ok) break;
@@ -725,8 +717,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       int dst_t = 0;
       if (STATES) {
         dst = C.seg_state + static_cast<long long>(item) * C.db * C.dc;
-      } else if (C.fin && slot >= 0 && w.last) {
-        dst = C.fin + (slot * C.heads + w.head) * C.db * C.dc;
+      } else if (C.fin && w.last) {
+        const long long slot = lin::state_slot(C, w.seq);
+        if (slot >= 0) dst = C.fin + (slot * C.heads + w.head) * C.db * C.dc;
         dst_t = C.fin_t;
       }
       if (dst && b < C.db) {
