@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
   const float* src = nullptr;
   int src_t = 0;
   if (!STATES) {
-    if (C.seg_state) {
+    if (g.count > 1) {
       src = C.seg_state + (static_cast<long long>(blockIdx.x) * C.heads + head) * C.db * C.dc;
     } else if (C.init && slot >= 0) {
       src = C.init + (slot * C.heads + head) * C.db * C.dc;
@@ -212,36 +212,43 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
 
 // ---- scan over the segments ---------------------------------------------------------
 // In place: slot s holds segment s's own X (the last one's is not read) and
-// gets the X that enters it.
+// gets the X that enters it.  Sequences of one segment have nothing to scan.
+// A thread follows VEC values; the next kAhead segments are on their way while
+// one group is written, so a long sequence is not one memory latency a segment.
+template <int VEC>
 __global__ void __launch_bounds__(256) chain_scan_kernel(const __grid_constant__ Chain C) {
+  constexpr int kAhead = 8;
   const int s = blockIdx.z, head = blockIdx.y;
   const Segment g = lin::sequence_of(C, s);
   const int w0 = lin::first_slot(C, s);
-  const long long n = static_cast<long long>(C.db) * C.dc;
+  const int n = C.db * C.dc, e = (blockIdx.x * 256 + threadIdx.x) * VEC;
   const int slots = lin::segment_slots(C.tokens, C.nseq, C.seg);
-  const long long e = blockIdx.x * 256ll + threadIdx.x;
-  if (e >= n) return;
+  const int count = min(g.count, slots - w0);
+  if (count < 2 || e >= n) return;
   const long long slot = lin::state_slot(C, s);
-  float x = 0.f;
-  if (C.init && slot >= 0) {
-    const int b = static_cast<int>(e / C.dc), c = static_cast<int>(e - static_cast<long long>(b) * C.dc);
-    x = C.init[(slot * C.heads + head) * n + lin::state_index(C, C.init_t, b, c)];
+  float x[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    x[v] = 0.f;
+    if (C.init && slot >= 0)
+      x[v] = C.init[(slot * C.heads + head) * n + lin::state_index(C, C.init_t, (e + v) / C.dc, (e + v) % C.dc)];
   }
   const float keep = expf(lin::log_decay_of(C, head) * static_cast<float>(C.seg));
-  const long long hop = C.heads * n;
+  const long long hop = static_cast<long long>(C.heads) * n;
   float* p = C.seg_state + (static_cast<long long>(w0) * C.heads + head) * n + e;
-  const int count = min(g.count, slots - w0);
-  for (int i = 0; i < count; i += 4) {
-    float own[4];
+  float own[kAhead][VEC];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) own[j] = i + j < count - 1 ? p[(i + j) * hop] : 0.f;
+  for (int j = 0; j < kAhead; ++j)
+    if (j < count - 1) seq::load_vec<float, VEC>(p + j * hop, own[j]);
+  for (int i = 0; i < count; i += kAhead)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i + j < count) {
-        p[(i + j) * hop] = x;
-        x = fmaf(keep, x, own[j]);
-      }
-  }
+    for (int j = 0; j < kAhead; ++j) {
+      if (i + j >= count) break;
+      seq::store_vec<float, VEC>(p + (i + j) * hop, x);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) x[v] = fmaf(keep, x[v], own[j][v]);
+      if (i + j + kAhead < count - 1) seq::load_vec<float, VEC>(p + (i + j + kAhead) * hop, own[j]);
+    }
 }
 
 // ---- shared heads: sum the gradients of the heads of a group ---------------------------
@@ -367,17 +374,32 @@ int check_list(const char* who, const char* name, const void* p, bool need) {
   return ok();
 }
 
-// Tokens of a segment.  Enough segments that four CTAs for each SM have one;
-// at least four chunks of 128 a segment, so that the states that pass through
-// memory (8 db dc bytes a segment and head) stay below the rows' own bytes.
-// One segment for all where no sequence can be longer than one.
+// Tokens of a segment, from what the host knows: the tokens, the sequences and
+// the heads (taken for sequences of equal length).  Among cuts of a sequence
+// into k segments, the one with the least estimated time: rounds of items over
+// 148 SMs, a chunk of 128 tokens taking 2 units in the states' launch and 4 in
+// the outputs', an item 3 units to begin, the scan and its launch 6 and what
+// its bytes cost (4 / 148 for a segment and head).  A segment is at most 1.5
+// times an SM's share of all chunks, so that one long sequence among short ones
+// is cut too.  One segment for all where no sequence can be longer than one.
 constexpr int kOneSegment = 1 << 30;
 
 int plan_segment(const to_linear_attention_desc& d) {
-  const long long chunks = (d.tokens + 127) / 128;
-  long long per = (chunks * d.q_heads + 4 * 148 - 1) / (4 * 148);
-  per = per < 4 ? 4 : per;
-  return per >= chunks ? kOneSegment : static_cast<int>(per * 128);
+  constexpr long long kSms = 148;
+  const long long chunks = (d.tokens + 127) / 128, pairs = static_cast<long long>(d.nseq) * d.q_heads;
+  if (chunks <= 2 || pairs == 0) return kOneSegment;
+  const long long mean = std::max(1ll, (chunks + d.nseq - 1) / d.nseq);
+  long long best = mean, least = INT64_MAX;
+  for (long long k = 1; k <= 64 && k <= mean; ++k) {
+    const long long per = (mean + k - 1) / k;
+    long long cost = 148 * ((pairs * k + kSms - 1) / kSms) * (4 * per + 3);
+    if (k > 1) cost += 148 * (((pairs * (k - 1) + kSms - 1) / kSms) * (2 * per + 3) + 6) + 4 * pairs * k;
+    if (cost < least) least = cost, best = per;
+  }
+  const long long share = std::max(4ll, (3 * chunks * d.q_heads / 2 + kSms - 1) / kSms);
+  if (best == mean) best = std::max(best, std::min(chunks, 2 * mean));  // ragged ones stay whole too
+  best = std::min(best, std::max(share, mean / 64 + 1));
+  return best >= chunks ? kOneSegment : static_cast<int>(best * 128);
 }
 
 constexpr size_t kAlign = 256;
@@ -413,8 +435,10 @@ int launch_simt(const Chain& C, cudaStream_t s) {
 }
 
 int launch_scan(const Chain& C, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>((C.db * C.dc + 255) / 256), C.heads, C.nseq);
-  chain_scan_kernel<<<grid, 256, 0, s>>>(C);
+  const int n = C.db * C.dc;
+  const dim3 grid(n % 4 ? (n + 255) / 256 : (n / 4 + 255) / 256, C.heads, C.nseq);
+  if (n % 4) chain_scan_kernel<1><<<grid, 256, 0, s>>>(C);
+  else chain_scan_kernel<4><<<grid, 256, 0, s>>>(C);
   TO_CUDA_TRY(cudaGetLastError());
   return ok();
 }

@@ -23,8 +23,9 @@
 // Roles (20 warps): one lane issues TMA loads into two stages of three
 // 32 KB tiles, one the products; warps 4-11 turn Sc into P (and make plane 0,
 // whose columns are theirs), scale O and store the results (a thread: one row,
-// 64 columns); warps 12-19 make the other planes and hold X (a thread: one row, 64 columns).  Products are issued Sc, Q X, U, P V:
-// the next chunk's Sc and the row warps run under the state's update.  Rows
+// 64 columns); warps 12-19 make the other planes and hold X (a thread: one row, 64 columns).  Products are issued Sc, Q X, P V, U:
+// the results are stored under U, and the next chunk's Sc runs under the state's
+// update.  Rows
 // past a chunk's end are masked: P and the planes by selection, V by zeroing
 // its rows, since 0 * NaN is not 0.  Rows of a reversed chain keep their order
 // in memory; only the masks and decays turn round.
@@ -69,7 +70,7 @@ __device__ __forceinline__ uint32_t plane_col(int plane, int token64) {
 
 struct Barriers {
   uint64_t full[kStages], empty[kStages];
-  uint64_t sc_full, p_ready, o1_full, o_ready, o2_full, o_free;
+  uint64_t sc_full, p_ready, o1_full, o2_full, o_free;
   uint64_t planes_ready, u_full, x_ready;
   uint64_t row_table, state_table;
   uint32_t tmem;
@@ -249,7 +250,8 @@ __device__ __forceinline__ uint32_t make_table(Barriers* b, uint64_t* bar, float
 
 // The chunks of an item (a segment of one head).
 struct Walk {
-  int seq, head, last;  // last: the sequence's last segment
+  int seq, head;
+  bool last, only;      // the sequence's last segment; its only one
   int edge;             // first row of the segment (forwards), or the row after it (backwards)
   int len;              // its tokens
   int n, updates;       // chunks; those whose state is wanted (not the last's, where no one reads it)
@@ -270,6 +272,7 @@ __device__ __forceinline__ bool walk_of(const Chain& C, int item, Walk* w) {
   w->seq = g.seq;
   w->head = item - slot * C.heads;
   w->last = g.idx == g.count - 1;
+  w->only = g.count == 1;
   w->len = min(C.seg, g.tokens - s0);
   w->edge = C.rev ? g.first + g.tokens - s0 : g.first + s0;
   w->n = (w->len + kTile - 1) / kTile;
@@ -370,10 +373,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar->sc_full, 1);
     mbar_init(&bar->p_ready, kRowWarps);
     mbar_init(&bar->o1_full, 1);
-    mbar_init(&bar->o_ready, kRowWarps);
     mbar_init(&bar->o2_full, 1);
     mbar_init(&bar->o_free, kRowWarps);
-    mbar_init(&bar->planes_ready, kStateWarps);
+    mbar_init(&bar->planes_ready, kStateWarps + (STATES ? 0 : kRowWarps));
     mbar_init(&bar->u_full, 1);
     mbar_init(&bar->x_ready, kStateWarps);
     mbar_init(&bar->row_table, kRowWarps);
@@ -438,25 +440,25 @@ __global__ void __launch_bounds__(kThreads, 1)
               mma(tm + kColO, desc_k(sq, k), desc_mn(sx, k), kIdesc | kMnB, k > 0);
             commit(&bar->o1_full);
           }
-          // also: V's rows past the end are zero, and the last chunk's U has been read
-          if (!(ok = wait_for(bar, &bar->planes_ready, turn) && (STATES || wait_for(bar, &bar->p_ready, turn)))) break;
-          fence_after();
+          if (!STATES) {
+            if (!(ok = wait_for(bar, &bar->p_ready, turn))) break;
+            fence_after();
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k)  // 16 tokens: 8 columns
+              mma_ts(tm + kColO, tm + kColS + (k >> 2) * 64 + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB, true);
+            commit(&bar->o2_full);
+          }
           if (i < w.updates) {
+            // also: the last chunk's U has been read
+            if (!(ok = wait_for(bar, &bar->planes_ready, turn))) break;
+            fence_after();
 #pragma unroll 1
             for (int p = PLANES - 1; p >= 0; --p)
 #pragma unroll
-              for (int k = 0; k < kTile / 16; ++k)  // 16 tokens: 8 columns
+              for (int k = 0; k < kTile / 16; ++k)
                 mma_ts(tm + kColU, tm + plane_col<STATES>(p, k >> 2) + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB,
                        p < PLANES - 1 || k > 0);
             commit(&bar->u_full);
-          }
-          if (!STATES) {
-            if (!(ok = wait_for(bar, &bar->o_ready, turn))) break;
-            fence_after();
-#pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
-              mma_ts(tm + kColO, tm + kColS + (k >> 2) * 64 + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB, true);
-            commit(&bar->o2_full);
           }
           commit(&bar->empty[turn]);
         }
@@ -537,14 +539,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_st8(lanes + kColS + h * 64 + part * 8, p);
           }
-          // plane 0 into the other half of this warp's columns of Sc
-          if (i < w.updates)
-            make_planes<STATES, PLANES, 0, 1>(stage_of(n) + kTileBytes, lanes, dec, cnt, rev, C.upd, q, h, lane);
-          else
-            tmem_st_wait();
-          fence_before();
-          __syncwarp();
-          if (lane == 0) arrive(&bar->p_ready);
           // Q X, decayed from the chunk's beginning
           const float f = inter * lds(dec + 4 * max(rev ? cnt - 1 - r : r + 1, 0));
           if (!(ok = warp_wait(bar, &bar->o1_full, n & 1))) break;
@@ -560,7 +554,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_st_wait();
           fence_before();
           __syncwarp();
-          if (lane == 0) arrive(&bar->o_ready);
+          if (lane == 0) arrive(&bar->p_ready);
+          // plane 0 into the other half of this warp's columns of Sc
+          if (i < w.updates)
+            make_planes<STATES, PLANES, 0, 1>(stage_of(n) + kTileBytes, lanes, dec, cnt, rev, C.upd, q, h, lane);
+          fence_before();
+          __syncwarp();
+          if (lane == 0) arrive(&bar->planes_ready);
           // results
           if (!(ok = warp_wait(bar, &bar->o2_full, n & 1))) break;
           fence_after();
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int src_t = 0;
       if (!STATES) {
         const long long slot = lin::state_slot(C, w.seq);
-        if (C.seg_state) {
+        if (!w.only) {
           src = C.seg_state + static_cast<long long>(item) * C.db * C.dc;  // item = segment slot * heads + head
         } else if (C.init && slot >= 0) {
           src = C.init + (slot * C.heads + w.head) * C.db * C.dc;
@@ -676,16 +676,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < w.n; ++i, ++n) {
         const int cnt = w.rows(i);
         const bool update = i < w.updates;
-        if (!STATES) {  // once the product that read the last chunk's X is done
-          if (n > 0 && !(ok = warp_wait(bar, &bar->o1_full, (n - 1) & 1))) break;
-          write_x(X);
-        }
         if (!(ok = warp_wait(bar, &bar->full[n & 1], (n / kStages) & 1))) break;
         if (cnt < kTile) {
           const uint32_t v = stage_of(n) + 2 * kTileBytes;
           for (int e = t; e < (kTile - cnt) * 16; e += 256)
             sts4(v + (e & 1) * kPanel + (cnt + (e >> 4)) * 128 + ((e >> 1) & 7) * 16, 0, 0, 0, 0);
           fence_async();
+        }
+        if (!STATES) {  // once the product that read the last chunk's X is done; x_ready is V's too
+          if (n > 0 && !(ok = warp_wait(bar, &bar->o1_full, (n - 1) & 1))) break;
+          write_x(X);
         }
         if (update) {
           make_planes<STATES, PLANES, STATES ? 0 : 1, PLANES>(stage_of(n) + kTileBytes, lanes, dec, cnt, rev, C.upd, q, h,
@@ -777,7 +777,7 @@ int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, con
   TO_CUDA_TRY(attr);
   const int items = (C.seg_state ? lin::segment_slots(C.tokens, C.nseq, C.seg) : C.nseq) * C.heads;
   chain_tc_kernel<TO, STATES, PLANES>
-      <<<unsigned(items < sms ? items : sms), kThreads, kSmem, s>>>(a, b, c, C, items);
+      <<<unsigned(items), kThreads, kSmem, s>>>(a, b, c, C, items);
   TO_CUDA_TRY(cudaGetLastError());
   return ok();
 }

@@ -9,8 +9,8 @@
 // once.  A pair's two values sit in one lane, so the rotation needs no
 // exchange; `lanes` lanes hold a row (VP pairs a unit, 16-byte accesses where
 // widths and addresses allow) and exchange only the row's sum.  A lane keeps
-// its pairs over all the heads that it visits of one token, so their sines are
-// computed once a token.
+// its pairs (and their weights) over all the heads that it visits of one token,
+// so their sines are computed once a token, by the warp's lanes together.
 //
 // Angles: a pair's frequency is a 64-bit fixed-point number of turns F =
 // theta^(-2j/R) / 2 pi * 2^64, so position * F modulo 2^64 is the angle's
@@ -35,30 +35,30 @@ using seq::Rows;
 
 constexpr int kMaxPairs = 128;
 constexpr int kWarps = 8;  // warps a CTA
-constexpr float kNoSum = 0.f;
 
 struct QkArgs {
   Rows in[2], g[2], out[2];  // q, k: x; gradients of y (backward); y or dx
   const float* w[2];
-  float* partial;  // backward: [CTAs][2][dim] sums of u n
+  float* partial;  // backward: [CTAs][dim] sums of u n
   const int32_t* positions;
   long long tokens;
   int heads[2];
   int dim, rotary, interleaved;
   float eps;
   int lanes;       // lanes that hold a row: a power of two
-  int splits;      // warps that share a token's heads
-  int units;       // ceil(pairs / VP)
+  int splits[2];   // warps that share a token's heads
+  int units;       // pairs / VP
+  int q_ctas;      // CTAs [0, q_ctas) take q, the others k
   int axis_end[4]; // first pair past each axis
   uint64_t turns[kMaxPairs];
 };
 
-// The place of a unit's values: VP pairs starting at pair p.
+// First elements of the two halves of the VP pairs that start at pair p (b is
+// not used for neighbours).
 struct Place {
-  int a, b;  // first elements of the two halves (halves), or a alone (neighbours)
+  int a, b;
 };
 
-template <int VP>
 __device__ __forceinline__ Place place_of(const QkArgs& A, int p) {
   const int rot = A.rotary >> 1;
   if (A.interleaved) return {2 * p, 0};
@@ -101,149 +101,156 @@ __device__ __forceinline__ void store_pairs(T* row, const Place& pl, int interle
   }
 }
 
-// cos and sin of a unit's pairs at one token (1, 0 past the rotated part).
-template <int VP>
-__device__ __forceinline__ void unit_angles(const QkArgs& A, long long token, int p0,
-                                            float (&c)[VP], float (&s)[VP]) {
-  const int rot = A.rotary >> 1;
-#pragma unroll
-  for (int i = 0; i < VP; ++i) {
-    const int p = p0 + i;
-    c[i] = 1.f;
-    s[i] = 0.f;
-    if (p < rot) {
-      const int axis = (p >= A.axis_end[0]) + (p >= A.axis_end[1]) + (p >= A.axis_end[2]);
-      const long long pos = __ldg(A.positions + axis * A.tokens + token);
-      const uint64_t turn = static_cast<uint64_t>(pos) * A.turns[p];
-      const int top = static_cast<int>(turn >> 32);  // [-1/2, 1/2) turns, 2^-32 each
-      sincospif(static_cast<float>(top) * 4.656612873077393e-10f, &s[i], &c[i]);
-    }
-  }
-}
-
 __device__ __forceinline__ float sum_over(float x, int lanes) {
   for (int o = lanes >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   return x;
 }
 
-// One warp: `splits` warps share a token's heads; in each step the warp's
-// 32 / lanes groups take one head each.  UPL units of VP pairs a lane.
-template <typename T, int VP, int UPL, bool BACKWARD>
+// One warp takes a token's heads, or one of `splits` equal parts of them; in
+// each step its 32 / lanes groups of lanes take HEADS heads each.  UPL units of
+// VP pairs a lane.  SHARE groups (of those that there are) compute a token's
+// sines together, VP / SHARE pairs each, and hand them round.
+template <typename T, int VP, int UPL, int SHARE, int HEADS, bool BACKWARD>
 __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__ QkArgs A) {
-  extern __shared__ float sums[];  // backward: [kWarps][2][dim]
+  extern __shared__ float sums[];  // backward: [kWarps][dim]
+  constexpr int kOwn = VP / SHARE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int groups = 32 / A.lanes, group = lane / A.lanes, gl = lane & (A.lanes - 1);
-  const float inv_dim = 1.f / static_cast<float>(A.dim);
+  const int t = static_cast<int>(blockIdx.x) >= A.q_ctas;  // q or k
+  const int first_cta = t ? A.q_ctas : 0, ctas = t ? gridDim.x - A.q_ctas : A.q_ctas;
+  const int heads = A.heads[t], splits = A.splits[t], rot = A.rotary >> 1, interleaved = A.interleaved;
+  const float inv_dim = 1.f / static_cast<float>(A.dim), eps = A.eps;
+  const Rows in = A.in[t], gr = A.g[t], out = A.out[t];
   bool on[UPL];
   Place pl[UPL];
+  float wa[UPL][VP], wb[UPL][VP];
+  uint64_t turn[UPL][kOwn];
+  const int32_t* pos[UPL][kOwn];
+  float dwa[BACKWARD ? UPL : 1][VP], dwb[BACKWARD ? UPL : 1][VP];
 #pragma unroll
   for (int u = 0; u < UPL; ++u) {
     const int unit = gl + u * A.lanes;
     on[u] = unit < A.units;
-    pl[u] = place_of<VP>(A, on[u] ? unit * VP : 0);
+    const int p0 = on[u] ? unit * VP : 0;
+    pl[u] = place_of(A, p0);
+#pragma unroll
+    for (int i = 0; i < VP; ++i) {
+      const int ia = pl[u].a + (interleaved ? 2 * i : i), ib = interleaved ? ia + 1 : pl[u].b + i;
+      wa[u][i] = A.w[t] ? __ldg(A.w[t] + ia) : 1.f;
+      wb[u][i] = A.w[t] ? __ldg(A.w[t] + ib) : 1.f;
+      if (BACKWARD) dwa[BACKWARD ? u : 0][i] = dwb[BACKWARD ? u : 0][i] = 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) {
+      const int p = p0 + k * SHARE + (group & (SHARE - 1));
+      const int axis = (p >= A.axis_end[0]) + (p >= A.axis_end[1]) + (p >= A.axis_end[2]);
+      const bool turns = on[u] && p < rot;  // the others stay: no position, no angle
+      turn[u][k] = turns ? A.turns[p] : 0;
+      pos[u][k] = turns ? A.positions + axis * A.tokens : nullptr;
+    }
   }
-  float dwa[BACKWARD ? 2 : 1][UPL][VP], dwb[BACKWARD ? 2 : 1][UPL][VP];
-  if (BACKWARD) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int u = 0; u < UPL; ++u)
-#pragma unroll
-        for (int i = 0; i < VP; ++i) dwa[BACKWARD ? t : 0][u][i] = dwb[BACKWARD ? t : 0][u][i] = kNoSum;
-  }
-  const long long items = A.tokens * A.splits;
-  for (long long item = static_cast<long long>(blockIdx.x) * kWarps + warp; item < items;
-       item += static_cast<long long>(gridDim.x) * kWarps) {
-    const long long token = item / A.splits;
-    const int part = static_cast<int>(item - token * A.splits);
+  const long long items = A.tokens * splits, stride = static_cast<long long>(ctas) * kWarps;
+  for (long long item = static_cast<long long>(blockIdx.x - first_cta) * kWarps + warp; item < items; item += stride) {
+    const long long token = splits == 1 ? item : item / splits;
+    const int part = splits == 1 ? 0 : static_cast<int>(item - token * splits);
     float c[UPL][VP], s[UPL][VP];
 #pragma unroll
-    for (int u = 0; u < UPL; ++u)
-      if (on[u]) unit_angles<VP>(A, token, (gl + u * A.lanes) * VP, c[u], s[u]);
+    for (int u = 0; u < UPL; ++u) {
+      float oc[kOwn], os[kOwn];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      float wa[UPL][VP], wb[UPL][VP];
+      for (int k = 0; k < kOwn; ++k) {
+        const long long x = pos[u][k] ? __ldg(pos[u][k] + token) : 0;
+        const int top = static_cast<int>((static_cast<uint64_t>(x) * turn[u][k]) >> 32);  // [-1/2, 1/2) turns
+        sincospif(static_cast<float>(top) * 4.656612873077393e-10f, &os[k], &oc[k]);
+      }
 #pragma unroll
-      for (int u = 0; u < UPL; ++u) {
-#pragma unroll
-        for (int i = 0; i < VP; ++i) wa[u][i] = wb[u][i] = 1.f;
-        if (on[u] && A.w[t]) {
-#pragma unroll
-          for (int i = 0; i < VP; ++i) {
-            wa[u][i] = __ldg(A.w[t] + pl[u].a + (A.interleaved ? 2 * i : i));
-            wb[u][i] = __ldg(A.w[t] + (A.interleaved ? pl[u].a + 2 * i + 1 : pl[u].b + i));
-          }
+      for (int i = 0; i < VP; ++i) {
+        if (SHARE == 1) {
+          c[u][i] = oc[i];
+          s[u][i] = os[i];
+        } else {  // pair i is made by the groups whose number is i modulo SHARE
+          const int from = (i & (SHARE - 1)) * A.lanes + gl;
+          c[u][i] = __shfl_sync(0xffffffffu, oc[i / SHARE], from);
+          s[u][i] = __shfl_sync(0xffffffffu, os[i / SHARE], from);
         }
       }
-      // every lane of the warp takes every step (the sums are warp-wide)
-      for (int h0 = part * groups; h0 < A.heads[t]; h0 += A.splits * groups) {
-        const int h = h0 + group;
-        const bool live = h < A.heads[t];
-        float xa[UPL][VP], xb[UPL][VP], ga[UPL][VP], gb[UPL][VP];
-        const T* xr = seq::row_ptr<const T>(A.in[t], token, live ? h : 0);
-        const T* gr = BACKWARD ? seq::row_ptr<const T>(A.g[t], token, live ? h : 0) : nullptr;
+    }
+    // every lane of the warp takes every step (the sums are warp-wide)
+    for (int h0 = part * groups * HEADS; h0 < heads; h0 += splits * groups * HEADS) {
+      bool live[HEADS];
+      float xa[HEADS][UPL][VP], xb[HEADS][UPL][VP];
+      float ga[BACKWARD ? HEADS : 1][UPL][VP], gb[BACKWARD ? HEADS : 1][UPL][VP];
+#pragma unroll
+      for (int e = 0; e < HEADS; ++e) {
+        const int h = h0 + e * groups + group;
+        live[e] = h < heads;
+        const T* xr = seq::row_ptr<const T>(in, token, live[e] ? h : 0);
+        const T* gp = BACKWARD ? seq::row_ptr<const T>(gr, token, live[e] ? h : 0) : nullptr;
+#pragma unroll
+        for (int u = 0; u < UPL; ++u)
+          if (on[u] && live[e]) {
+            load_pairs<T, VP>(xr, pl[u], interleaved, xa[e][u], xb[e][u]);
+            if (BACKWARD) load_pairs<T, VP>(gp, pl[u], interleaved, ga[BACKWARD ? e : 0][u], gb[BACKWARD ? e : 0][u]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < VP; ++i) {
+              xa[e][u][i] = xb[e][u][i] = 0.f;
+              if (BACKWARD) ga[BACKWARD ? e : 0][u][i] = gb[BACKWARD ? e : 0][u][i] = 0.f;
+            }
+          }
+      }
+#pragma unroll
+      for (int e = 0; e < HEADS; ++e) {
+        const int h = h0 + e * groups + group;
         float ss = 0.f;
 #pragma unroll
         for (int u = 0; u < UPL; ++u)
-          if (on[u] && live) {
-            load_pairs<T, VP>(xr, pl[u], A.interleaved, xa[u], xb[u]);
-            if (BACKWARD) load_pairs<T, VP>(gr, pl[u], A.interleaved, ga[u], gb[u]);
-          }
 #pragma unroll
-        for (int u = 0; u < UPL; ++u)
-          if (on[u] && live) {
-#pragma unroll
-            for (int i = 0; i < VP; ++i) ss = fmaf(xa[u][i], xa[u][i], fmaf(xb[u][i], xb[u][i], ss));
-          }
+          for (int i = 0; i < VP; ++i) ss = fmaf(xa[e][u][i], xa[e][u][i], fmaf(xb[e][u][i], xb[e][u][i], ss));
         ss = sum_over(ss, A.lanes);
-        const float r = 1.f / sqrtf(ss * inv_dim + A.eps);
+        const float r = rsqrtf(ss * inv_dim + eps);
+        T* row = seq::row_ptr<T>(out, token, live[e] ? h : 0);
         if (!BACKWARD) {
-          T* yr = seq::row_ptr<T>(A.out[t], token, live ? h : 0);
 #pragma unroll
-          for (int u = 0; u < UPL; ++u)
-            if (on[u] && live) {
-              float ya[VP], yb[VP];
+          for (int u = 0; u < UPL; ++u) {
+            float ya[VP], yb[VP];
 #pragma unroll
-              for (int i = 0; i < VP; ++i) {
-                const float a = xa[u][i] * r * wa[u][i], b = xb[u][i] * r * wb[u][i];
-                ya[i] = a * c[u][i] - b * s[u][i];
-                yb[i] = b * c[u][i] + a * s[u][i];
-              }
-              store_pairs<T, VP>(yr, pl[u], A.interleaved, ya, yb);
+            for (int i = 0; i < VP; ++i) {
+              const float a = xa[e][u][i] * (r * wa[u][i]), b = xb[e][u][i] * (r * wb[u][i]);
+              ya[i] = a * c[u][i] - b * s[u][i];
+              yb[i] = b * c[u][i] + a * s[u][i];
             }
+            if (on[u] && live[e]) store_pairs<T, VP>(row, pl[u], interleaved, ya, yb);
+          }
         } else {
+          constexpr int kB = BACKWARD ? 1 : 0;
           float dot = 0.f;
 #pragma unroll
           for (int u = 0; u < UPL; ++u)
-            if (on[u] && live) {
 #pragma unroll
-              for (int i = 0; i < VP; ++i) {
-                const float ua = ga[u][i] * c[u][i] + gb[u][i] * s[u][i];
-                const float ub = gb[u][i] * c[u][i] - ga[u][i] * s[u][i];
-                const float na = xa[u][i] * r, nb = xb[u][i] * r;
-                const int k = BACKWARD ? t : 0;
-                dwa[k][u][i] = fmaf(ua, na, dwa[k][u][i]);
-                dwb[k][u][i] = fmaf(ub, nb, dwb[k][u][i]);
-                xa[u][i] = na;
-                xb[u][i] = nb;
-                ga[u][i] = ua * wa[u][i];
-                gb[u][i] = ub * wb[u][i];
-                dot = fmaf(ga[u][i], na, fmaf(gb[u][i], nb, dot));
-              }
+            for (int i = 0; i < VP; ++i) {
+              const float gx = ga[kB * e][u][i], gy = gb[kB * e][u][i];
+              const float ua = gx * c[u][i] + gy * s[u][i], ub = gy * c[u][i] - gx * s[u][i];
+              const float na = xa[e][u][i] * r, nb = xb[e][u][i] * r;
+              dwa[kB * u][i] = fmaf(ua, na, dwa[kB * u][i]);
+              dwb[kB * u][i] = fmaf(ub, nb, dwb[kB * u][i]);
+              xa[e][u][i] = na;
+              xb[e][u][i] = nb;
+              ga[kB * e][u][i] = ua * wa[u][i];
+              gb[kB * e][u][i] = ub * wb[u][i];
+              dot = fmaf(ga[kB * e][u][i], na, fmaf(gb[kB * e][u][i], nb, dot));
             }
           const float m = sum_over(dot, A.lanes) * inv_dim;
-          T* dr = seq::row_ptr<T>(A.out[t], token, live ? h : 0);
 #pragma unroll
-          for (int u = 0; u < UPL; ++u)
-            if (on[u] && live) {
-              float da[VP], db[VP];
+          for (int u = 0; u < UPL; ++u) {
+            float da[VP], db[VP];
 #pragma unroll
-              for (int i = 0; i < VP; ++i) {
-                da[i] = r * (ga[u][i] - xa[u][i] * m);
-                db[i] = r * (gb[u][i] - xb[u][i] * m);
-              }
-              store_pairs<T, VP>(dr, pl[u], A.interleaved, da, db);
+            for (int i = 0; i < VP; ++i) {
+              da[i] = r * (ga[kB * e][u][i] - xa[e][u][i] * m);
+              db[i] = r * (gb[kB * e][u][i] - xb[e][u][i] * m);
             }
+            if (on[u] && live[e]) store_pairs<T, VP>(row, pl[u], interleaved, da, db);
+          }
         }
       }
     }
@@ -251,67 +258,75 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
   if (BACKWARD) {
     // groups of a warp, then warps of the CTA, in a fixed order
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int u = 0; u < UPL; ++u)
 #pragma unroll
-      for (int u = 0; u < UPL; ++u)
-#pragma unroll
-        for (int i = 0; i < VP; ++i) {
-          const int k = BACKWARD ? t : 0;
-          float a = dwa[k][u][i], b = dwb[k][u][i];
-          for (int o = A.lanes; o < 32; o <<= 1) {
-            a += __shfl_xor_sync(0xffffffffu, a, o);
-            b += __shfl_xor_sync(0xffffffffu, b, o);
-          }
-          if (group == 0 && on[u]) {
-            float* row = sums + (warp * 2 + t) * A.dim;
-            row[pl[u].a + (A.interleaved ? 2 * i : i)] = a;
-            row[A.interleaved ? pl[u].a + 2 * i + 1 : pl[u].b + i] = b;
-          }
+      for (int i = 0; i < VP; ++i) {
+        float a = dwa[BACKWARD ? u : 0][i], b = dwb[BACKWARD ? u : 0][i];
+        for (int o = A.lanes; o < 32; o <<= 1) {
+          a += __shfl_xor_sync(0xffffffffu, a, o);
+          b += __shfl_xor_sync(0xffffffffu, b, o);
         }
+        if (group == 0 && on[u]) {
+          float* row = sums + warp * A.dim;
+          row[pl[u].a + (interleaved ? 2 * i : i)] = a;
+          row[interleaved ? pl[u].a + 2 * i + 1 : pl[u].b + i] = b;
+        }
+      }
     __syncthreads();
-    for (int e = threadIdx.x; e < 2 * A.dim; e += 32 * kWarps) {
+    for (int e = threadIdx.x; e < A.dim; e += 32 * kWarps) {
       float v = 0.f;
-      for (int w = 0; w < kWarps; ++w) v += sums[w * 2 * A.dim + e];
-      A.partial[static_cast<long long>(blockIdx.x) * 2 * A.dim + e] = v;
+      for (int w = 0; w < kWarps; ++w) v += sums[w * A.dim + e];
+      A.partial[static_cast<long long>(blockIdx.x) * A.dim + e] = v;
     }
   }
 }
 
 // dw[e] = sum over CTAs of their partial sums, in a fixed order, in f64 (a few
-// hundred terms; the order of magnitude of f32's own rounding would double).
-__global__ void __launch_bounds__(256) qk_sum_kernel(const float* __restrict__ partial, int ctas,
+// hundred terms: f32 would add as much rounding again as the terms have).  A
+// warp takes one value of dwq or dwk, its lanes every 32nd CTA.
+__global__ void __launch_bounds__(256) qk_sum_kernel(const float* __restrict__ partial, int q_ctas, int ctas,
                                                      int dim, float* dwq, float* dwk) {
-  __shared__ double part[8][32];
-  const int e = blockIdx.x * 32 + (threadIdx.x & 31), row = threadIdx.x >> 5;
+  const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (e >= 2 * dim) return;
+  const bool q = e < dim;
+  const int x = q ? e : e - dim, first = q ? 0 : q_ctas, last = q ? q_ctas : ctas;
   double v = 0;
-  if (e < 2 * dim)
-    for (int c = row; c < ctas; c += 8) v += partial[static_cast<long long>(c) * 2 * dim + e];
-  part[row][threadIdx.x & 31] = v;
-  __syncthreads();
-  if (row == 0 && e < 2 * dim) {
-    for (int k = 1; k < 8; ++k) v += part[k][threadIdx.x & 31];
-    float* dst = e < dim ? dwq : dwk;
-    if (dst) dst[e < dim ? e : e - dim] = static_cast<float>(v);
-  }
+#pragma unroll 8
+  for (int c = first + lane; c < last; c += 32) v += partial[static_cast<long long>(c) * dim + x];
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  float* dst = q ? dwq : dwk;
+  if (lane == 0 && dst) dst[x] = static_cast<float>(v);
 }
 
-long long backward_ctas(long long tokens, int sms) {
-  // two CTAs of eight warps an SM hold the gradients' registers; fewer tokens, fewer CTAs
-  const long long want = (tokens + kWarps - 1) / kWarps;
-  const long long cap = 2ll * sms;
-  return want < cap ? (want > 0 ? want : 1) : cap;
+// CTAs for q and for k, in proportion to their heads: `cap` CTAs in all, fewer
+// where the warps would have no token.
+struct QkGrid {
+  int q, k;
+};
+QkGrid grid_of(const to_qk_desc& d, long long items_q, long long items_k, long long cap) {
+  auto part = [&](long long heads, long long items) {
+    if (!heads) return 0;
+    const long long share = (cap * heads + d.q_heads + d.k_heads - 1) / (d.q_heads + d.k_heads);
+    const long long want = (items + kWarps - 1) / kWarps;
+    return static_cast<int>(want < 1 ? 1 : want < share ? want : share);
+  };
+  return {part(d.q_heads, items_q), part(d.k_heads, items_k)};
 }
 
-template <typename T, int VP, int UPL>
-int launch(const QkArgs& A, bool backward, int sms, cudaStream_t s) {
+// Two CTAs of eight warps an SM hold the gradients' registers.
+QkGrid backward_grid(const to_qk_desc& d, long long tokens, int sms) { return grid_of(d, tokens, tokens, 2ll * sms); }
+
+template <typename T, int VP, int UPL, int SHARE>
+int launch(QkArgs& A, const to_qk_desc& d, bool backward, int sms, cudaStream_t s) {
   if (backward) {
-    const int ctas = static_cast<int>(backward_ctas(A.tokens, sms));
-    qk_kernel<T, VP, UPL, true>
-        <<<ctas, 32 * kWarps, size_t(kWarps) * 2 * A.dim * sizeof(float), s>>>(A);
+    const QkGrid g = backward_grid(d, A.tokens, sms);
+    A.q_ctas = g.q;
+    qk_kernel<T, VP, UPL, SHARE, 1, true><<<g.q + g.k, 32 * kWarps, size_t(kWarps) * A.dim * sizeof(float), s>>>(A);
   } else {
-    const long long want = (A.tokens * A.splits + kWarps - 1) / kWarps, cap = 64ll * sms;
-    qk_kernel<T, VP, UPL, false>
-        <<<static_cast<int>(want < cap ? want : cap), 32 * kWarps, 0, s>>>(A);
+    const QkGrid g = grid_of(d, A.tokens * A.splits[0], A.tokens * A.splits[1], 32ll * sms);
+    A.q_ctas = g.q;
+    // two heads a step (more loads in flight) where a lane holds one unit
+    qk_kernel<T, VP, UPL, SHARE, UPL == 1 ? 2 : 1, false><<<g.q + g.k, 32 * kWarps, 0, s>>>(A);
   }
   TO_CUDA_TRY(cudaGetLastError());
   return ok();
@@ -321,27 +336,33 @@ int launch(const QkArgs& A, bool backward, int sms, cudaStream_t s) {
 // neighbours, f32 halves) and 2 (f32 neighbours); widths or addresses that do
 // not allow them go down to single pairs.
 template <typename T>
-int dispatch(QkArgs& A, int vp, bool backward, int sms, cudaStream_t s) {
+int dispatch(QkArgs& A, const to_qk_desc& d, int vp, bool backward, int sms, cudaStream_t s) {
   const int pairs = A.dim / 2;
   A.units = pairs / vp;
   A.lanes = 1;
   while (A.lanes < 32 && A.lanes < A.units) A.lanes *= 2;
-  const int upl = (A.units + A.lanes - 1) / A.lanes;
-  // warps that share a token: one, unless the tokens are too few to give every
-  // SM sixteen warps; then at most one a step of heads
-  const int steps = (A.heads[0] + 32 / A.lanes - 1) / (32 / A.lanes);
-  long long splits = backward ? 1 : (16ll * sms + A.tokens - 1) / A.tokens;
-  A.splits = static_cast<int>(splits < 1 ? 1 : splits > steps ? steps : splits);
-  if (A.splits < 1) A.splits = 1;
-  if (vp == 8 && sizeof(T) == 2) return launch<__nv_bfloat16, 8, 1>(A, backward, sms, s);
-  if (vp == 4) return launch<T, 4, 1>(A, backward, sms, s);
-  if (vp == 2) {
-    if (upl == 1) return launch<T, 2, 1>(A, backward, sms, s);
-    return launch<T, 2, 2>(A, backward, sms, s);
+  const int upl = (A.units + A.lanes - 1) / A.lanes, groups = 32 / A.lanes;
+  // warps that share a token's heads: one, unless the tokens are too few to give
+  // every SM sixteen warps; then at most one a step of heads
+  for (int t = 0; t < 2; ++t) {
+    const long long steps = (A.heads[t] + groups - 1) / groups;
+    long long n = backward || A.tokens == 0 ? 1 : (16ll * sms + A.tokens - 1) / A.tokens;
+    A.splits[t] = static_cast<int>(n > steps ? (steps > 0 ? steps : 1) : n);
   }
-  if (upl == 1) return launch<T, 1, 1>(A, backward, sms, s);
-  if (upl == 2) return launch<T, 1, 2>(A, backward, sms, s);
-  return launch<T, 1, 4>(A, backward, sms, s);
+  if (vp == 8 && sizeof(T) == 2)
+    return groups >= 4 ? launch<__nv_bfloat16, 8, 1, 4>(A, d, backward, sms, s)
+                       : launch<__nv_bfloat16, 8, 1, 2>(A, d, backward, sms, s);
+  if (vp == 4)
+    return groups >= 4   ? launch<T, 4, 1, 4>(A, d, backward, sms, s)
+           : groups >= 2 ? launch<T, 4, 1, 2>(A, d, backward, sms, s)
+                         : launch<T, 4, 1, 1>(A, d, backward, sms, s);
+  if (vp == 2) {
+    if (upl == 1) return launch<T, 2, 1, 1>(A, d, backward, sms, s);
+    return launch<T, 2, 2, 1>(A, d, backward, sms, s);
+  }
+  if (upl == 1) return launch<T, 1, 1, 1>(A, d, backward, sms, s);
+  if (upl == 2) return launch<T, 1, 2, 1>(A, d, backward, sms, s);
+  return launch<T, 1, 4, 1>(A, d, backward, sms, s);
 }
 
 int run(const char* who, const to_qk_plan* plan, int64_t tokens, const to_rows* q, const to_rows* k,
@@ -415,8 +436,8 @@ int run(const char* who, const to_qk_plan* plan, int64_t tokens, const to_rows* 
   int dev = 0;
   const int sms = device_sm_count(&dev);
   if (sms <= 0) return -sms;
-  return d.dtype == TO_BF16 ? dispatch<__nv_bfloat16>(A, vp, backward, sms, s)
-                            : dispatch<float>(A, vp, backward, sms, s);
+  return d.dtype == TO_BF16 ? dispatch<__nv_bfloat16>(A, d, vp, backward, sms, s)
+                            : dispatch<float>(A, d, vp, backward, sms, s);
 }
 
 }  // namespace
@@ -484,7 +505,8 @@ size_t to_qk_norm_rotary_workspace_bytes(const to_qk_plan* plan, int64_t tokens)
   if (!plan || tokens < 0) return 0;
   int dev = 0;
   const int sms = device_sm_count(&dev);
-  return size_t(backward_ctas(tokens, sms > 0 ? sms : 148)) * 2 * plan->desc.head_dim * sizeof(float);
+  const QkGrid g = backward_grid(plan->desc, tokens, sms > 0 ? sms : 148);
+  return size_t(g.q + g.k) * plan->desc.head_dim * sizeof(float);
 }
 
 int to_qk_norm_rotary_backward(const to_qk_plan* plan, int64_t tokens, const to_rows* q,
@@ -510,8 +532,8 @@ int to_qk_norm_rotary_backward(const to_qk_plan* plan, int64_t tokens, const to_
   const int sms = device_sm_count(&dev);
   if (sms <= 0) return -sms;
   const int dim = plan->desc.head_dim;
-  qk_sum_kernel<<<(2 * dim + 31) / 32, 256, 0, s>>>(partial, static_cast<int>(backward_ctas(tokens, sms)),
-                                                    dim, dwq, dwk);
+  const QkGrid g = backward_grid(plan->desc, tokens, sms);
+  qk_sum_kernel<<<(2 * dim + 7) / 8, 256, 0, s>>>(partial, g.q, g.q + g.k, dim, dwq, dwk);
   TO_CUDA_TRY(cudaGetLastError());
   return ok();
 }
