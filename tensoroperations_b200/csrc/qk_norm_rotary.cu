@@ -67,39 +67,86 @@ __device__ __forceinline__ Place place_of(const QkArgs& A, int p) {
   return {A.rotary + p - rot, A.rotary + p - rot + rest};
 }
 
+// A unit of a row as it lies in memory, and as f32 values two to a register
+// pair (the packed f32x2 instructions).  N pairs of halves or neighbours; where
+// VP is odd (1) the second lane of a register pair is unused.
 template <typename T, int VP>
-__device__ __forceinline__ void load_pairs(const T* row, const Place& pl, int interleaved,
-                                           float (&a)[VP], float (&b)[VP]) {
-  if (interleaved) {
-    float t[2 * VP];
-    seq::load_vec<T, 2 * VP>(row + pl.a, t);
-#pragma unroll
-    for (int i = 0; i < VP; ++i) {
-      a[i] = t[2 * i];
-      b[i] = t[2 * i + 1];
-    }
-  } else {
-    seq::load_vec<T, VP>(row + pl.a, a);
-    seq::load_vec<T, VP>(row + pl.b, b);
-  }
-}
+struct Unit {
+  static constexpr int kBytes = VP * int(sizeof(T));  // of one half
+  static constexpr int kWords = kBytes < 4 ? 1 : kBytes / 4;
+  static constexpr int kPacked = (VP + 1) / 2;
+  uint32_t raw[2 * kWords];
 
-template <typename T, int VP>
-__device__ __forceinline__ void store_pairs(T* row, const Place& pl, int interleaved,
-                                            const float (&a)[VP], const float (&b)[VP]) {
-  if (interleaved) {
-    float t[2 * VP];
+  __device__ __forceinline__ void load(const T* row, const Place& pl, int interleaved) {
+    if (interleaved) {
+      read<2 * kBytes>(row + pl.a, raw);
+    } else {
+      read<kBytes>(row + pl.a, raw);
+      read<kBytes>(row + pl.b, raw + kWords);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < 2 * kWords; ++i) raw[i] = 0;
+  }
+  // a: the pairs' first values, b: their second ones
+  __device__ __forceinline__ void unpack(int interleaved, float2 (&a)[kPacked], float2 (&b)[kPacked]) const {
+    float x[2 * VP];
+#pragma unroll
+    for (int i = 0; i < 2 * VP; ++i) {
+      if (sizeof(T) == 4) {
+        x[i] = __uint_as_float(raw[i % (2 * kWords)]);
+      } else {
+        // one value a half: each half has a word of its own (neighbours share the first)
+        const uint32_t w = VP == 1 ? (interleaved ? raw[0] : raw[i]) : raw[i / 2];
+        const bool high = VP == 1 ? interleaved && i == 1 : i & 1;
+        x[i] = __uint_as_float(high ? w & 0xffff0000u : w << 16);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPacked; ++i) {
+      const int j = 2 * i + 1 < VP ? 2 * i + 1 : 2 * i;
+      a[i] = interleaved ? make_float2(x[4 * i], x[2 * j]) : make_float2(x[2 * i], x[j]);
+      b[i] = interleaved ? make_float2(x[4 * i + 1], x[2 * j + 1]) : make_float2(x[VP + 2 * i], x[VP + j]);
+    }
+  }
+  __device__ __forceinline__ static void store(T* row, const Place& pl, int interleaved, const float2 (&a)[kPacked],
+                                               const float2 (&b)[kPacked]) {
+    float x[VP], y[VP], t[2 * VP];
 #pragma unroll
     for (int i = 0; i < VP; ++i) {
-      t[2 * i] = a[i];
-      t[2 * i + 1] = b[i];
+      x[i] = i & 1 ? a[i / 2].y : a[i / 2].x;
+      y[i] = i & 1 ? b[i / 2].y : b[i / 2].x;
+      t[2 * i] = x[i];
+      t[2 * i + 1] = y[i];
     }
-    seq::store_vec<T, 2 * VP>(row + pl.a, t);
-  } else {
-    seq::store_vec<T, VP>(row + pl.a, a);
-    seq::store_vec<T, VP>(row + pl.b, b);
+    if (interleaved) {
+      seq::store_vec<T, 2 * VP>(row + pl.a, t);
+    } else {
+      seq::store_vec<T, VP>(row + pl.a, x);
+      seq::store_vec<T, VP>(row + pl.b, y);
+    }
   }
-}
+
+ private:
+  template <int BYTES>
+  __device__ __forceinline__ static void read(const T* p, uint32_t* dst) {
+    if (BYTES == 2) {
+      dst[0] = *reinterpret_cast<const uint16_t*>(p);
+    } else if (BYTES == 4) {
+      dst[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else if (BYTES == 8) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      dst[0] = v.x, dst[1] = v.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i) {
+        const uint4 v = *(reinterpret_cast<const uint4*>(p) + i);
+        dst[4 * i] = v.x, dst[4 * i + 1] = v.y, dst[4 * i + 2] = v.z, dst[4 * i + 3] = v.w;
+      }
+    }
+  }
+};
 
 __device__ __forceinline__ float sum_over(float x, int lanes) {
   for (int o = lanes >> 1; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
@@ -107,13 +154,15 @@ __device__ __forceinline__ float sum_over(float x, int lanes) {
 }
 
 // One warp takes a token's heads, or one of `splits` equal parts of them; in
-// each step its 32 / lanes groups of lanes take HEADS heads each.  UPL units of
-// VP pairs a lane.  SHARE groups (of those that there are) compute a token's
-// sines together, VP / SHARE pairs each, and hand them round.
+// each step its 32 / lanes groups of lanes take HEADS heads each, and the next
+// step's rows (the next token's, at the end) are on their way meanwhile.  UPL
+// units of VP pairs a lane.  SHARE groups (of those that there are) compute a
+// token's sines together, VP / SHARE pairs each, and hand them round.
 template <typename T, int VP, int UPL, int SHARE, int HEADS, bool BACKWARD>
-__global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__ QkArgs A) {
+__global__ void __launch_bounds__(32 * kWarps, 2) qk_kernel(const __grid_constant__ QkArgs A) {
   extern __shared__ float sums[];  // backward: [kWarps][dim]
-  constexpr int kOwn = VP / SHARE;
+  using U = Unit<T, VP>;
+  constexpr int kOwn = VP / SHARE, kP = U::kPacked, kB = BACKWARD ? 1 : 0;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int groups = 32 / A.lanes, group = lane / A.lanes, gl = lane & (A.lanes - 1);
   const int t = static_cast<int>(blockIdx.x) >= A.q_ctas;  // q or k
@@ -123,10 +172,10 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
   const Rows in = A.in[t], gr = A.g[t], out = A.out[t];
   bool on[UPL];
   Place pl[UPL];
-  float wa[UPL][VP], wb[UPL][VP];
+  float2 wa[UPL][kP], wb[UPL][kP];
   uint64_t turn[UPL][kOwn];
   const int32_t* pos[UPL][kOwn];
-  float dwa[BACKWARD ? UPL : 1][VP], dwb[BACKWARD ? UPL : 1][VP];
+  float2 dwa[kB * (UPL - 1) + 1][kP], dwb[kB * (UPL - 1) + 1][kP];
 #pragma unroll
   for (int u = 0; u < UPL; ++u) {
     const int unit = gl + u * A.lanes;
@@ -134,11 +183,15 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
     const int p0 = on[u] ? unit * VP : 0;
     pl[u] = place_of(A, p0);
 #pragma unroll
-    for (int i = 0; i < VP; ++i) {
-      const int ia = pl[u].a + (interleaved ? 2 * i : i), ib = interleaved ? ia + 1 : pl[u].b + i;
-      wa[u][i] = A.w[t] ? __ldg(A.w[t] + ia) : 1.f;
-      wb[u][i] = A.w[t] ? __ldg(A.w[t] + ib) : 1.f;
-      if (BACKWARD) dwa[BACKWARD ? u : 0][i] = dwb[BACKWARD ? u : 0][i] = 0.f;
+    for (int i = 0; i < kP; ++i) {
+      const int j = 2 * i + 1 < VP ? 2 * i + 1 : 2 * i;
+      auto weight = [&](int first, int k) {
+        return A.w[t] ? __ldg(A.w[t] + first + (interleaved ? 2 * k : k)) : 1.f;
+      };
+      const int second = interleaved ? pl[u].a + 1 : pl[u].b;
+      wa[u][i] = make_float2(weight(pl[u].a, 2 * i), weight(pl[u].a, j));
+      wb[u][i] = make_float2(weight(second, 2 * i), weight(second, j));
+      if (BACKWARD) dwa[kB * u][i] = dwb[kB * u][i] = make_float2(0.f, 0.f);
     }
 #pragma unroll
     for (int k = 0; k < kOwn; ++k) {
@@ -150,110 +203,137 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
     }
   }
   const long long items = A.tokens * splits, stride = static_cast<long long>(ctas) * kWarps;
-  for (long long item = static_cast<long long>(blockIdx.x - first_cta) * kWarps + warp; item < items; item += stride) {
-    const long long token = splits == 1 ? item : item / splits;
-    const int part = splits == 1 ? 0 : static_cast<int>(item - token * splits);
-    float c[UPL][VP], s[UPL][VP];
+  long long item = static_cast<long long>(blockIdx.x - first_cta) * kWarps + warp;
+  auto token_of = [&](long long i) { return splits == 1 ? i : i / splits; };
+  auto first_of = [&](long long i) {  // first head of an item
+    return splits == 1 ? 0 : static_cast<int>(i - i / splits * splits) * groups * HEADS;
+  };
+  U x[HEADS][UPL], g[kB * (HEADS - 1) + 1][UPL], nx[HEADS][UPL], ng[kB * (HEADS - 1) + 1][UPL];
+  auto fetch = [&](U (&fx)[HEADS][UPL], U (&fg)[kB * (HEADS - 1) + 1][UPL], long long token, int h0) {
+#pragma unroll
+    for (int e = 0; e < HEADS; ++e) {
+      const int h = h0 + e * groups + group;
+      const T* xr = seq::row_ptr<const T>(in, token, h < heads ? h : 0);
+      const T* gp = BACKWARD ? seq::row_ptr<const T>(gr, token, h < heads ? h : 0) : nullptr;
+#pragma unroll
+      for (int u = 0; u < UPL; ++u) {
+        if (on[u] && h < heads) {
+          fx[e][u].load(xr, pl[u], interleaved);
+          if (BACKWARD) fg[kB * e][u].load(gp, pl[u], interleaved);
+        } else {
+          fx[e][u].clear();
+          if (BACKWARD) fg[kB * e][u].clear();
+        }
+      }
+    }
+  };
+  if (item < items) fetch(x, g, token_of(item), first_of(item));
+  while (item < items) {
+    const long long token = token_of(item), next = item + stride;
+    float2 c[UPL][kP], s[UPL][kP];
 #pragma unroll
     for (int u = 0; u < UPL; ++u) {
-      float oc[kOwn], os[kOwn];
+      float oc[kOwn], os[kOwn], cc[2 * kP], ss[2 * kP];
 #pragma unroll
       for (int k = 0; k < kOwn; ++k) {
-        const long long x = pos[u][k] ? __ldg(pos[u][k] + token) : 0;
-        const int top = static_cast<int>((static_cast<uint64_t>(x) * turn[u][k]) >> 32);  // [-1/2, 1/2) turns
+        const long long at = pos[u][k] ? __ldg(pos[u][k] + token) : 0;
+        const int top = static_cast<int>((static_cast<uint64_t>(at) * turn[u][k]) >> 32);  // [-1/2, 1/2) turns
         sincospif(static_cast<float>(top) * 4.656612873077393e-10f, &os[k], &oc[k]);
       }
 #pragma unroll
-      for (int i = 0; i < VP; ++i) {
-        if (SHARE == 1) {
-          c[u][i] = oc[i];
-          s[u][i] = os[i];
+      for (int i = 0; i < 2 * kP; ++i) {
+        if (SHARE == 1 || VP == 1) {
+          cc[i] = oc[i % kOwn];
+          ss[i] = os[i % kOwn];
         } else {  // pair i is made by the groups whose number is i modulo SHARE
           const int from = (i & (SHARE - 1)) * A.lanes + gl;
-          c[u][i] = __shfl_sync(0xffffffffu, oc[i / SHARE], from);
-          s[u][i] = __shfl_sync(0xffffffffu, os[i / SHARE], from);
+          cc[i] = __shfl_sync(0xffffffffu, oc[i / SHARE], from);
+          ss[i] = __shfl_sync(0xffffffffu, os[i / SHARE], from);
         }
+      }
+#pragma unroll
+      for (int i = 0; i < kP; ++i) {
+        c[u][i] = make_float2(cc[2 * i], cc[2 * i + 1]);
+        s[u][i] = make_float2(ss[2 * i], ss[2 * i + 1]);
       }
     }
     // every lane of the warp takes every step (the sums are warp-wide)
-    for (int h0 = part * groups * HEADS; h0 < heads; h0 += splits * groups * HEADS) {
-      bool live[HEADS];
-      float xa[HEADS][UPL][VP], xb[HEADS][UPL][VP];
-      float ga[BACKWARD ? HEADS : 1][UPL][VP], gb[BACKWARD ? HEADS : 1][UPL][VP];
+    const int step = splits * groups * HEADS;
+    for (int h0 = first_of(item); h0 < heads; h0 += step) {
+      if (h0 + step < heads) fetch(nx, ng, token, h0 + step);
+      else if (next < items) fetch(nx, ng, token_of(next), first_of(next));
 #pragma unroll
       for (int e = 0; e < HEADS; ++e) {
         const int h = h0 + e * groups + group;
-        live[e] = h < heads;
-        const T* xr = seq::row_ptr<const T>(in, token, live[e] ? h : 0);
-        const T* gp = BACKWARD ? seq::row_ptr<const T>(gr, token, live[e] ? h : 0) : nullptr;
+        float2 xa[UPL][kP], xb[UPL][kP], sq = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int u = 0; u < UPL; ++u)
-          if (on[u] && live[e]) {
-            load_pairs<T, VP>(xr, pl[u], interleaved, xa[e][u], xb[e][u]);
-            if (BACKWARD) load_pairs<T, VP>(gp, pl[u], interleaved, ga[BACKWARD ? e : 0][u], gb[BACKWARD ? e : 0][u]);
-          } else {
+        for (int u = 0; u < UPL; ++u) {
+          x[e][u].unpack(interleaved, xa[u], xb[u]);
 #pragma unroll
-            for (int i = 0; i < VP; ++i) {
-              xa[e][u][i] = xb[e][u][i] = 0.f;
-              if (BACKWARD) ga[BACKWARD ? e : 0][u][i] = gb[BACKWARD ? e : 0][u][i] = 0.f;
-            }
+          for (int i = 0; i < kP; ++i) {
+            if (VP == 1) xa[u][i].y = xb[u][i].y = 0.f;
+            sq = __ffma2_rn(xa[u][i], xa[u][i], __ffma2_rn(xb[u][i], xb[u][i], sq));
           }
-      }
-#pragma unroll
-      for (int e = 0; e < HEADS; ++e) {
-        const int h = h0 + e * groups + group;
-        float ss = 0.f;
-#pragma unroll
-        for (int u = 0; u < UPL; ++u)
-#pragma unroll
-          for (int i = 0; i < VP; ++i) ss = fmaf(xa[e][u][i], xa[e][u][i], fmaf(xb[e][u][i], xb[e][u][i], ss));
-        ss = sum_over(ss, A.lanes);
-        const float r = rsqrtf(ss * inv_dim + eps);
-        T* row = seq::row_ptr<T>(out, token, live[e] ? h : 0);
+        }
+        const float r = rsqrtf(sum_over(sq.x + sq.y, A.lanes) * inv_dim + eps);
+        const float2 r2 = make_float2(r, r);
+        T* row = seq::row_ptr<T>(out, token, h < heads ? h : 0);
         if (!BACKWARD) {
 #pragma unroll
           for (int u = 0; u < UPL; ++u) {
-            float ya[VP], yb[VP];
+            float2 ya[kP], yb[kP];
 #pragma unroll
-            for (int i = 0; i < VP; ++i) {
-              const float a = xa[e][u][i] * (r * wa[u][i]), b = xb[e][u][i] * (r * wb[u][i]);
-              ya[i] = a * c[u][i] - b * s[u][i];
-              yb[i] = b * c[u][i] + a * s[u][i];
+            for (int i = 0; i < kP; ++i) {
+              const float2 a = __fmul2_rn(xa[u][i], __fmul2_rn(r2, wa[u][i]));
+              const float2 b = __fmul2_rn(xb[u][i], __fmul2_rn(r2, wb[u][i]));
+              const float2 m = __fmul2_rn(b, s[u][i]);
+              ya[i] = __ffma2_rn(a, c[u][i], make_float2(-m.x, -m.y));
+              yb[i] = __ffma2_rn(b, c[u][i], __fmul2_rn(a, s[u][i]));
             }
-            if (on[u] && live[e]) store_pairs<T, VP>(row, pl[u], interleaved, ya, yb);
+            if (on[u] && h < heads) U::store(row, pl[u], interleaved, ya, yb);
           }
         } else {
-          constexpr int kB = BACKWARD ? 1 : 0;
-          float dot = 0.f;
-#pragma unroll
-          for (int u = 0; u < UPL; ++u)
-#pragma unroll
-            for (int i = 0; i < VP; ++i) {
-              const float gx = ga[kB * e][u][i], gy = gb[kB * e][u][i];
-              const float ua = gx * c[u][i] + gy * s[u][i], ub = gy * c[u][i] - gx * s[u][i];
-              const float na = xa[e][u][i] * r, nb = xb[e][u][i] * r;
-              dwa[kB * u][i] = fmaf(ua, na, dwa[kB * u][i]);
-              dwb[kB * u][i] = fmaf(ub, nb, dwb[kB * u][i]);
-              xa[e][u][i] = na;
-              xb[e][u][i] = nb;
-              ga[kB * e][u][i] = ua * wa[u][i];
-              gb[kB * e][u][i] = ub * wb[u][i];
-              dot = fmaf(ga[kB * e][u][i], na, fmaf(gb[kB * e][u][i], nb, dot));
-            }
-          const float m = sum_over(dot, A.lanes) * inv_dim;
+          float2 da[UPL][kP], db[UPL][kP], dot = make_float2(0.f, 0.f);
 #pragma unroll
           for (int u = 0; u < UPL; ++u) {
-            float da[VP], db[VP];
+            float2 ga[kP], gb[kP];
+            g[kB * e][u].unpack(interleaved, ga, gb);
 #pragma unroll
-            for (int i = 0; i < VP; ++i) {
-              da[i] = r * (ga[kB * e][u][i] - xa[e][u][i] * m);
-              db[i] = r * (gb[kB * e][u][i] - xb[e][u][i] * m);
+            for (int i = 0; i < kP; ++i) {
+              const float2 m = __fmul2_rn(ga[i], s[u][i]);
+              const float2 ua = __ffma2_rn(ga[i], c[u][i], __fmul2_rn(gb[i], s[u][i]));
+              const float2 ub = __ffma2_rn(gb[i], c[u][i], make_float2(-m.x, -m.y));
+              xa[u][i] = __fmul2_rn(xa[u][i], r2);  // n
+              xb[u][i] = __fmul2_rn(xb[u][i], r2);
+              dwa[kB * u][i] = __ffma2_rn(ua, xa[u][i], dwa[kB * u][i]);
+              dwb[kB * u][i] = __ffma2_rn(ub, xb[u][i], dwb[kB * u][i]);
+              da[u][i] = __fmul2_rn(ua, wa[u][i]);
+              db[u][i] = __fmul2_rn(ub, wb[u][i]);
+              dot = __ffma2_rn(da[u][i], xa[u][i], __ffma2_rn(db[u][i], xb[u][i], dot));
             }
-            if (on[u] && live[e]) store_pairs<T, VP>(row, pl[u], interleaved, da, db);
+          }
+          const float m = -sum_over(dot.x + dot.y, A.lanes) * inv_dim;
+          const float2 m2 = make_float2(m, m);
+#pragma unroll
+          for (int u = 0; u < UPL; ++u) {
+#pragma unroll
+            for (int i = 0; i < kP; ++i) {
+              da[u][i] = __fmul2_rn(r2, __ffma2_rn(xa[u][i], m2, da[u][i]));
+              db[u][i] = __fmul2_rn(r2, __ffma2_rn(xb[u][i], m2, db[u][i]));
+            }
+            if (on[u] && h < heads) U::store(row, pl[u], interleaved, da[u], db[u]);
           }
         }
       }
+#pragma unroll
+      for (int e = 0; e < HEADS; ++e)
+#pragma unroll
+        for (int u = 0; u < UPL; ++u) {
+          x[e][u] = nx[e][u];
+          if (BACKWARD) g[kB * e][u] = ng[kB * e][u];
+        }
     }
+    item = next;
   }
   if (BACKWARD) {
     // groups of a warp, then warps of the CTA, in a fixed order
@@ -261,7 +341,8 @@ __global__ void __launch_bounds__(32 * kWarps) qk_kernel(const __grid_constant__
     for (int u = 0; u < UPL; ++u)
 #pragma unroll
       for (int i = 0; i < VP; ++i) {
-        float a = dwa[BACKWARD ? u : 0][i], b = dwb[BACKWARD ? u : 0][i];
+        float a = i & 1 ? dwa[kB * u][i / 2].y : dwa[kB * u][i / 2].x;
+        float b = i & 1 ? dwb[kB * u][i / 2].y : dwb[kB * u][i / 2].x;
         for (int o = A.lanes; o < 32; o <<= 1) {
           a += __shfl_xor_sync(0xffffffffu, a, o);
           b += __shfl_xor_sync(0xffffffffu, b, o);
@@ -379,7 +460,7 @@ int run(const char* who, const to_qk_plan* plan, int64_t tokens, const to_rows* 
   A.heads[0] = d.q_heads;
   A.heads[1] = d.k_heads;
   const int width = d.head_dim, half = d.rotary_dim / 2, rest = width / 2 - half;
-  int vp = d.dtype == TO_BF16 ? (d.interleaved ? 4 : 8) : (d.interleaved ? 2 : 4);
+  int vp = d.dtype == TO_BF16 ? (d.interleaved ? 4 : 8) : 4;
   const to_rows none{nullptr, 0, 0};
   for (int t = 0; t < 2; ++t) {
     if (!A.heads[t]) {
