@@ -379,23 +379,25 @@ __global__ void __launch_bounds__(256) qk_sum_kernel(const float* __restrict__ p
   if (lane == 0 && dst) dst[x] = static_cast<float>(v);
 }
 
-// CTAs for q and for k, in proportion to their heads: `cap` CTAs in all, fewer
+// CTAs for q and for k: `cap` CTAs in all, shared by the time that a token takes
+// (its steps over four heads, and about two steps more for its sines), fewer
 // where the warps would have no token.
 struct QkGrid {
   int q, k;
 };
 QkGrid grid_of(const to_qk_desc& d, long long items_q, long long items_k, long long cap) {
-  auto part = [&](long long heads, long long items) {
-    if (!heads) return 0;
-    const long long share = (cap * heads + d.q_heads + d.k_heads - 1) / (d.q_heads + d.k_heads);
+  const long long cost_q = (d.q_heads + 3) / 4 + 2, cost_k = d.k_heads ? (d.k_heads + 3) / 4 + 2 : 0;
+  auto part = [&](long long cost, long long items) {
+    if (!cost) return 0;
+    const long long share = (cap * cost + cost_q + cost_k - 1) / (cost_q + cost_k);
     const long long want = (items + kWarps - 1) / kWarps;
     return static_cast<int>(want < 1 ? 1 : want < share ? want : share);
   };
-  return {part(d.q_heads, items_q), part(d.k_heads, items_k)};
+  return {part(cost_q, items_q), part(cost_k, items_k)};
 }
 
-// Two CTAs of eight warps an SM hold the gradients' registers.
-QkGrid backward_grid(const to_qk_desc& d, long long tokens, int sms) { return grid_of(d, tokens, tokens, 2ll * sms); }
+// Two CTAs of eight warps fit an SM; three rounds of them even out their lengths.
+QkGrid backward_grid(const to_qk_desc& d, long long tokens, int sms) { return grid_of(d, tokens, tokens, 6ll * sms); }
 
 template <typename T, int VP, int UPL, int SHARE>
 int launch(QkArgs& A, const to_qk_desc& d, bool backward, int sms, cudaStream_t s) {
