@@ -376,39 +376,57 @@ int check_list(const char* who, const char* name, const void* p, bool need) {
 
 // Tokens of a segment, from what the host knows: the tokens, the sequences and
 // the heads (taken for sequences of equal length).  Among cuts of a sequence
-// into k segments, the one with the least estimated time: rounds of items over
-// 148 SMs, a chunk of 128 tokens taking 2 units in the states' launch and 4 in
-// the outputs', an item 3 units to begin, the scan and its launch 6 and what
-// its bytes cost (4 / 148 for a segment and head).  A segment is at most 1.5
-// times an SM's share of all chunks, so that one long sequence among short ones
-// is cut too.  One segment for all where no sequence can be longer than one.
+// into k segments, the one with the least estimated time, in units of a quarter
+// of a chunk's outputs: rounds of items over the CTAs that run at a time, a
+// chunk taking 4 units in the outputs' launch and `states` in the states', an
+// item `begin` to begin, the scan and its launch 6 and what its bytes cost.  A
+// segment is at most 1.5 times an SM's share of all chunks, so that one long
+// sequence among short ones is cut too.  One segment for all where no sequence
+// can be longer than one.
+// Tensor cores: chunks of 128 tokens (about 4.7 us), one CTA an SM.  CUDA cores:
+// chunks of 64 (about 10 us), one CTA for each 64 or 32 columns; narrow rows
+// leave shared memory for two an SM.
 constexpr int kOneSegment = 1 << 30;
 
-int plan_segment(const to_linear_attention_desc& d) {
-  constexpr long long kSms = 148;
-  const long long chunks = (d.tokens + 127) / 128, pairs = static_cast<long long>(d.nseq) * d.q_heads;
+int plan_segment(const to_linear_attention_desc& d, bool tc, int db, int dc) {
+  const long long chunk = tc ? 128 : kRows, states = tc ? 2 : 1, begin = tc ? 3 : 2;
+  const long long at_once = 148 * (!tc && db <= 64 ? 2 : 1);
+  const long long blocks = tc ? 1 : db <= 128 ? (dc + 63) / 64 : (dc + 31) / 32;
+  const long long chunks = (d.tokens + chunk - 1) / chunk, pairs = d.nseq * blocks * d.q_heads;
   if (chunks <= 2 || pairs == 0) return kOneSegment;
   const long long mean = std::max(1ll, (chunks + d.nseq - 1) / d.nseq);
   long long best = mean, least = INT64_MAX;
   for (long long k = 1; k <= 64 && k <= mean; ++k) {
     const long long per = (mean + k - 1) / k;
-    long long cost = 148 * ((pairs * k + kSms - 1) / kSms) * (4 * per + 3);
-    if (k > 1) cost += 148 * (((pairs * (k - 1) + kSms - 1) / kSms) * (2 * per + 3) + 6) + 4 * pairs * k;
+    long long cost = at_once * ((pairs * k + at_once - 1) / at_once) * (4 * per + begin);
+    if (k > 1)
+      cost += at_once * (((pairs * (k - 1) + at_once - 1) / at_once) * (states * per + begin) + 6) + 4 * pairs * k;
     if (cost < least) least = cost, best = per;
   }
-  const long long share = std::max(4ll, (3 * chunks * d.q_heads / 2 + kSms - 1) / kSms);
+  const long long share = std::max(tc ? 4ll : 2ll, (3 * chunks * blocks * d.q_heads / 2 + at_once - 1) / at_once);
   if (best == mean) best = std::max(best, std::min(chunks, 2 * mean));  // ragged ones stay whole too
   best = std::min(best, std::max(share, mean / 64 + 1));
-  return best >= chunks ? kOneSegment : static_cast<int>(best * 128);
+  return best >= chunks ? kOneSegment : static_cast<int>(best * chunk);
 }
 
 constexpr size_t kAlign = 256;
 size_t rounded(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
-size_t state_bytes(const to_linear_attention_desc& d) {
-  const int seg = plan_segment(d);
-  if (seg == kOneSegment) return 0;
-  return rounded(size_t(lin::segment_slots(static_cast<int>(d.tokens), d.nseq, seg)) * d.q_heads * d.key_dim * d.value_dim * 4);
+// Bytes of the segments' states of a chain of these widths, on either kind of cores.
+size_t state_bytes(const to_linear_attention_desc& d, int db, int dc) {
+  size_t most = 0;
+  for (const bool tc : {false, true}) {
+    const int seg = plan_segment(d, tc, db, dc);
+    if (seg == kOneSegment || (tc && d.dtype == TO_F32)) continue;
+    const size_t slots = size_t(lin::segment_slots(static_cast<int>(d.tokens), d.nseq, seg));
+    most = std::max(most, rounded(slots * d.q_heads * db * dc * 4));
+  }
+  return most;
+}
+size_t state_bytes(const to_linear_attention_desc& d) { return state_bytes(d, d.key_dim, d.value_dim); }
+// The backward pass runs chains of (key, value) and of (value, key) widths.
+size_t backward_state_bytes(const to_linear_attention_desc& d) {
+  return std::max(state_bytes(d), state_bytes(d, d.value_dim, d.key_dim));
 }
 
 template <typename T, typename TO, int DCB, bool STATES>
@@ -452,26 +470,32 @@ int run_simt(const Chain& C, cudaStream_t s) {
   return launch_simt<T, TO, false>(C, s);
 }
 
-int run_chain(const Chain& C, int32_t dtype, bool f32_out, cudaStream_t s) {
-  if (dtype == TO_F32) return run_simt<float, float>(C, s);
-  if (!lin::tc_takes(C, f32_out))
-    return f32_out ? run_simt<__nv_bfloat16, float>(C, s) : run_simt<__nv_bfloat16, __nv_bfloat16>(C, s);
-  if (C.seg_state) {
-    if (int st = lin::tc_states(C, s)) return st;
-    if (int st = launch_scan(C, s)) return st;
+// `states`: workspace for the segments' states.
+int run_chain(Chain C, const to_linear_attention_desc& d, bool f32_out, void* states, cudaStream_t s) {
+  auto cut = [&](bool tc) {
+    C.seg = plan_segment(d, tc, C.db, C.dc);
+    C.seg_state = C.seg == kOneSegment ? nullptr : static_cast<float*>(states);
+  };
+  cut(true);
+  if (d.dtype == TO_BF16 && lin::tc_takes(C, f32_out)) {
+    if (C.seg_state) {
+      if (int st = lin::tc_states(C, s)) return st;
+      if (int st = launch_scan(C, s)) return st;
+    }
+    return lin::tc_outputs(C, f32_out, s);
   }
-  return lin::tc_outputs(C, f32_out, s);
+  cut(false);
+  if (d.dtype == TO_F32) return run_simt<float, float>(C, s);
+  return f32_out ? run_simt<__nv_bfloat16, float>(C, s) : run_simt<__nv_bfloat16, __nv_bfloat16>(C, s);
 }
 
-Chain base_chain(const to_linear_attention_desc& d, const int32_t* cu, const float* log_decay, void* states) {
+Chain base_chain(const to_linear_attention_desc& d, const int32_t* cu, const float* log_decay) {
   Chain C{};
   C.heads = d.q_heads;
   C.nseq = d.nseq;
   C.tokens = static_cast<int>(d.tokens);
   C.cu = cu;
   C.log_decay = log_decay;
-  C.seg = plan_segment(d);
-  C.seg_state = C.seg == kOneSegment ? nullptr : static_cast<float*>(states);
   C.a_div = C.b_div = C.c_div = C.out_div = 1;
   return C;
 }
@@ -500,7 +524,7 @@ size_t to_linear_attention_workspace_bytes(const to_linear_attention_desc* desc)
 size_t to_linear_attention_backward_workspace_bytes(const to_linear_attention_desc* desc) {
   if (check_desc("to_linear_attention_backward_workspace_bytes", desc)) return 0;
   const to_linear_attention_desc& d = *desc;
-  size_t n = state_bytes(d);
+  size_t n = backward_state_bytes(d);
   if (d.q_heads != d.kv_heads)  // f32 gradients of each query head, before the heads of a group are summed
     n += rounded(size_t(d.tokens) * d.q_heads * std::max(d.key_dim, d.value_dim) * 4);
   return n;
@@ -530,7 +554,7 @@ int to_linear_attention(const to_linear_attention_desc* desc, const to_linear_at
                      a.workspace ? a.workspace_bytes : 0, need);
   if (need && !aligned(a.workspace, kAlign))
     return set_error(TO_ERR_ALIGNMENT, "%s: workspace is not 256-byte aligned", who);
-  Chain C = base_chain(d, a.cu_seqlens, a.log_decay, a.workspace);
+  Chain C = base_chain(d, a.cu_seqlens, a.log_decay);
   C.a = seq::rows_of(a.q);
   C.b = seq::rows_of(a.k);
   C.c = seq::rows_of(a.v);
@@ -544,7 +568,7 @@ int to_linear_attention(const to_linear_attention_desc* desc, const to_linear_at
   C.fin = a.state_out;
   C.slots = a.slots;
   C.num_slots = d.num_slots;
-  return run_chain(C, d.dtype, false, static_cast<cudaStream_t>(stream));
+  return run_chain(C, d, false, a.workspace, static_cast<cudaStream_t>(stream));
 }
 
 int to_linear_attention_backward(const to_linear_attention_desc* desc,
@@ -579,7 +603,7 @@ int to_linear_attention_backward(const to_linear_attention_desc* desc,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int group = d.q_heads / d.kv_heads;
   const float scale = static_cast<float>(d.scale);
-  Chain C = base_chain(d, a.cu_seqlens, a.log_decay, a.workspace);
+  Chain C = base_chain(d, a.cu_seqlens, a.log_decay);
   // dq: forwards, a = do, b = v, c = k
   C.a = seq::rows_of(a.d_o);
   C.b = seq::rows_of(a.v);
@@ -592,9 +616,9 @@ int to_linear_attention_backward(const to_linear_attention_desc* desc,
   C.upd = 1.f;
   C.init = a.state_in;
   C.init_t = 1;
-  if ((st = run_chain(C, d.dtype, false, s))) return st;
+  if ((st = run_chain(C, d, false, a.workspace, s))) return st;
   // backwards; the gradients of shared heads go through f32 partial rows
-  float* part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + state_bytes(d));
+  float* part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + backward_state_bytes(d));
   auto target = [&](const to_rows& r, int width) {
     if (group == 1) return seq::rows_of(r);
     return Rows{reinterpret_cast<char*>(part), static_cast<long long>(d.q_heads) * width, width};
@@ -614,7 +638,7 @@ int to_linear_attention_backward(const to_linear_attention_desc* desc,
   C.db = d.value_dim;
   C.dc = d.key_dim;
   C.init_t = 1;
-  if ((st = run_chain(C, d.dtype, group > 1, s))) return st;
+  if ((st = run_chain(C, d, group > 1, a.workspace, s))) return st;
   if (group > 1) {
     st = d.dtype == TO_BF16 ? group_sum<__nv_bfloat16>(part, a.dk, d, d.key_dim, s)
                             : group_sum<float>(part, a.dk, d, d.key_dim, s);
@@ -629,7 +653,7 @@ int to_linear_attention_backward(const to_linear_attention_desc* desc,
   C.dc = d.value_dim;
   C.init_t = 0;
   C.fin = a.dstate_in;
-  if ((st = run_chain(C, d.dtype, group > 1, s))) return st;
+  if ((st = run_chain(C, d, group > 1, a.workspace, s))) return st;
   if (group > 1)
     return d.dtype == TO_BF16 ? group_sum<__nv_bfloat16>(part, a.dv, d, d.value_dim, s)
                               : group_sum<float>(part, a.dv, d, d.value_dim, s);
