@@ -35,16 +35,31 @@ struct SimtShape {
   }
 };
 
+// Rows of a chunk into shared memory as f32, four columns a thread; rows past
+// cnt and columns past width become zero.  `vec`: four columns are one access.
 template <typename T>
-__device__ __forceinline__ void load_rows(float* dst, int ld, const Rows& r, int head, long long row0,
-                                          int step, int cnt, int first, int width, int padded) {
-  // rows past cnt and columns past width become zero
-  for (int e = threadIdx.x; e < kRows * padded; e += kThreads) {
-    const int i = e / padded, x = e - i * padded;
-    float v = 0.f;
-    if (i < cnt && x < width)
-      v = seq::to_f32(seq::row_ptr<const T>(r, row0 + static_cast<long long>(step) * i, head)[first + x]);
-    dst[i * ld + x] = v;
+__device__ __forceinline__ void load_rows(float* dst, int ld, const Rows& r, int head, int row0, int step, int cnt,
+                                          int first, int width, int padded, bool vec) {
+  int lanes = 8;  // threads of a row: a power of two
+  while (lanes * 4 < padded) lanes *= 2;
+  const int x = (threadIdx.x & (lanes - 1)) * 4;
+  if (x >= padded) return;
+  const T* src = seq::row_ptr<const T>(r, row0, head) + first + x;
+  const long long hop = static_cast<long long>(step) * r.ts;
+#pragma unroll 4
+  for (int i = threadIdx.x / lanes; i < kRows; i += kThreads / lanes) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (i < cnt) {
+      const T* p = src + i * hop;
+      if (vec && x + 4 <= width) {
+        seq::load_vec<T, 4>(p, v);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (x + e < width) v[e] = seq::to_f32(p[e]);
+      }
+    }
+    *reinterpret_cast<float4*>(dst + i * ld + x) = make_float4(v[0], v[1], v[2], v[3]);
   }
 }
 
@@ -90,11 +105,11 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
   const int step = C.rev ? -1 : 1;
   for (int done = 0; done < len; done += kRows) {
     const int cnt = min(kRows, len - done), t = s0 + done;
-    const long long row0 = C.rev ? g.first + g.tokens - 1 - t : g.first + t;
+    const int row0 = C.rev ? g.first + g.tokens - 1 - t : g.first + t;
     __syncthreads();  // the last chunk's readers are done
-    if (!STATES) load_rows<T>(A, lda, C.a, head / C.a_div, row0, step, cnt, 0, C.db, dbp);
-    load_rows<T>(B, lda, C.b, head / C.b_div, row0, step, cnt, 0, C.db, dbp);
-    load_rows<T>(V, kColPad, C.c, head / C.c_div, row0, step, cnt, col0, ncols, DCB);
+    if (!STATES) load_rows<T>(A, lda, C.a, head / C.a_div, row0, step, cnt, 0, C.db, dbp, C.vec & 1);
+    load_rows<T>(B, lda, C.b, head / C.b_div, row0, step, cnt, 0, C.db, dbp, C.vec & 2);
+    load_rows<T>(V, kColPad, C.c, head / C.c_div, row0, step, cnt, col0, ncols, DCB, C.vec & 4);
     __syncthreads();
     if (!STATES) {
       float acc[4][4] = {};
@@ -167,31 +182,41 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
     }
     // X = l^cnt X + upd * sum_j l^(cnt-1+rev-j) b_j c_j
     const float keep = dec[cnt];
-    for (int k0 = 0; k0 < dbp; k0 += 64) {
-      const int k = k0 + ty * 4;
-      if (k >= dbp) continue;
-      float u[4][VC] = {};
+    // (a thread: rows k .. k+3 and k+64 .. k+67 at a time, so V is read half as often)
+    for (int k0 = 0; k0 < dbp; k0 += 128) {
+      const int k[2] = {k0 + ty * 4, k0 + 64 + ty * 4};
+      const bool on[2] = {k[0] < dbp, k[1] < dbp};
+      if (!on[0]) continue;
+      float u[2][4][VC] = {};
+#pragma unroll 4
       for (int j = 0; j < cnt; ++j) {
         const float d = C.upd * dec[cnt - 1 + C.rev - j];
-        const float4 b = *reinterpret_cast<const float4*>(B + j * lda + k);
         float v[VC];
         seq::load_vec<float, VC>(V + j * kColPad + tx * VC, v);
 #pragma unroll
-        for (int c = 0; c < VC; ++c) {
-          const float x = d * v[c];
-          u[0][c] = fmaf(b.x, x, u[0][c]);
-          u[1][c] = fmaf(b.y, x, u[1][c]);
-          u[2][c] = fmaf(b.z, x, u[2][c]);
-          u[3][c] = fmaf(b.w, x, u[3][c]);
+        for (int c = 0; c < VC; ++c) v[c] *= d;
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          if (!on[z]) continue;
+          float b[4];
+          seq::load_vec<float, 4>(B + j * lda + k[z], b);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int c = 0; c < VC; ++c) u[z][r][c] = fmaf(b[r], v[c], u[z][r][c]);
         }
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+      for (int z = 0; z < 2; ++z) {
+        if (!on[z]) continue;
 #pragma unroll
-        for (int c = 0; c < VC; ++c) {
-          float* x = X + (k + r) * kColPad + tx * VC + c;
-          *x = fmaf(keep, *x, u[r][c]);
-        }
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int c = 0; c < VC; ++c) {
+            float* x = X + (k[z] + r) * kColPad + tx * VC + c;
+            *x = fmaf(keep, *x, u[z][r][c]);
+          }
+      }
     }
   }
   __syncthreads();
@@ -485,6 +510,10 @@ int run_chain(Chain C, const to_linear_attention_desc& d, bool f32_out, void* st
     return lin::tc_outputs(C, f32_out, s);
   }
   cut(false);
+  const Rows* rows[3] = {&C.a, &C.b, &C.c};
+  const int bytes = 4 * seq::dtype_bytes(d.dtype);
+  for (int i = 0; i < 3; ++i)
+    if (aligned(rows[i]->p, size_t(bytes)) && rows[i]->ts % 4 == 0 && rows[i]->hs % 4 == 0) C.vec |= 1 << i;
   if (d.dtype == TO_F32) return run_simt<float, float>(C, s);
   return f32_out ? run_simt<__nv_bfloat16, float>(C, s) : run_simt<__nv_bfloat16, __nv_bfloat16>(C, s);
 }

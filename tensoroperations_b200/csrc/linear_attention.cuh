@@ -48,6 +48,7 @@ struct Chain {
   long long num_slots;
   float* seg_state;  // [segment slots][heads][db][dc]; null: one segment a sequence
   int seg;           // tokens of a segment
+  int vec;           // bits 0, 1, 2: rows of a, b, c can be read four values at a time
 };
 
 // Where a segment lies.  idx < 0: an unused slot.
