@@ -103,32 +103,10 @@ class Slab(C.Structure):
                 ("f_is_zero", C.c_int32)]
 
 
-class Rows(C.Structure):
-    """to_rows: values of [tokens][heads][width], strides in elements."""
-    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
-
-
 class QkDesc(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("dtype", "q_heads", "k_heads", "head_dim", "rotary_dim", "axes")] + \
         [("section", C.c_int32 * 4), ("interleaved", C.c_int32), ("reserved0", C.c_int32),
          ("theta", C.c_double), ("eps", C.c_double)]
-
-
-class LinearAttentionDesc(C.Structure):
-    _fields_ = [(n, C.c_int32) for n in ("dtype", "q_heads", "kv_heads", "key_dim", "value_dim", "nseq")] + \
-        [("tokens", C.c_int64), ("num_slots", C.c_int64), ("scale", C.c_double)]
-
-
-class LinearAttentionArgs(C.Structure):
-    _fields_ = [(n, Rows) for n in ("q", "k", "v", "o")] + \
-        [(n, C.c_void_p) for n in ("log_decay", "cu_seqlens", "slots", "state_in", "state_out", "workspace")] + \
-        [("workspace_bytes", C.c_size_t)]
-
-
-class LinearAttentionGradArgs(C.Structure):
-    _fields_ = [(n, Rows) for n in ("q", "k", "v", "d_o", "dq", "dk", "dv")] + \
-        [(n, C.c_void_p) for n in ("log_decay", "cu_seqlens", "state_in", "dstate_out", "dstate_in", "workspace")] + \
-        [("workspace_bytes", C.c_size_t)]
 
 
 NCCL_UNIQUE_ID_BYTES = 128
@@ -196,20 +174,18 @@ _sig("to_nccl_unique_id", C.c_int, [C.c_void_p])
 _sig("to_nccl_comm_init", C.c_int, [C.c_int32, C.c_int32, C.c_void_p, C.POINTER(C.c_void_p)])
 _sig("to_nccl_comm_destroy", C.c_int, [C.c_void_p])
 _sig("to_nccl_allreduce_sum_f64", C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p])
-_R = C.POINTER(Rows)
+_R = C.c_char_p  # a to_rows, packed (sequence.py); so are the linear-attention structures
 _sig("to_qk_plan_create", C.c_int, [C.POINTER(QkDesc), C.POINTER(C.c_void_p)])
 _sig("to_qk_plan_destroy", C.c_int, [C.c_void_p])
 _sig("to_qk_norm_rotary", C.c_int, [C.c_void_p, C.c_int64, _R, _R] + [C.c_void_p] * 3 + [_R, _R, C.c_void_p])
 _sig("to_qk_norm_rotary_workspace_bytes", C.c_size_t, [C.c_void_p, C.c_int64])
 _sig("to_qk_norm_rotary_backward", C.c_int, [C.c_void_p, C.c_int64, _R, _R] + [C.c_void_p] * 3 + [_R] * 4 +
      [C.c_void_p] * 3 + [C.c_size_t, C.c_void_p])
-_sig("to_linear_attention_workspace_bytes", C.c_size_t, [C.POINTER(LinearAttentionDesc)])
-_sig("to_linear_attention_backward_workspace_bytes", C.c_size_t, [C.POINTER(LinearAttentionDesc)])
-_sig("to_linear_attention", C.c_int, [C.POINTER(LinearAttentionDesc), C.POINTER(LinearAttentionArgs), C.c_void_p])
-_sig("to_linear_attention_backward", C.c_int, [C.POINTER(LinearAttentionDesc),
-                                               C.POINTER(LinearAttentionGradArgs), C.c_void_p])
-_sig("to_linear_attention_step", C.c_int, [C.POINTER(LinearAttentionDesc), C.POINTER(LinearAttentionArgs),
-                                           C.c_void_p])
+_sig("to_linear_attention_workspace_bytes", C.c_size_t, [C.c_char_p])
+_sig("to_linear_attention_backward_workspace_bytes", C.c_size_t, [C.c_char_p])
+_sig("to_linear_attention", C.c_int, [C.c_char_p, C.c_char_p, C.c_void_p])
+_sig("to_linear_attention_backward", C.c_int, [C.c_char_p, C.c_char_p, C.c_void_p])
+_sig("to_linear_attention_step", C.c_int, [C.c_char_p, C.c_char_p, C.c_void_p])
 
 
 def status_name(status: int) -> str:

@@ -15,11 +15,20 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import Optional, Sequence
 
 import torch
 
 from . import abi
+
+# to_rows, to_linear_attention_desc / _args / _grad_args as the C compiler lays
+# them out: a call packs its arguments into bytes of its own (a ctypes structure
+# filled field by field took longer than the smallest kernels).
+_ROWS = struct.Struct("@Pqq")
+_DESC = struct.Struct("@6i2qd")
+_ARGS = struct.Struct("@" + 4 * "Pqq" + "6PN")
+_GRAD_ARGS = struct.Struct("@" + 7 * "Pqq" + "6PN")
 
 DTYPES = {torch.bfloat16: abi.TO_BF16, torch.float32: abi.TO_F32}
 
@@ -31,32 +40,39 @@ def _dtype(dtype) -> torch.dtype:
     return kind
 
 
-def _rows(t, name: str, dtype: torch.dtype, tokens: int, heads: int, width: int, device) -> abi.Rows:
-    if t.shape != (tokens, heads, width):
-        raise ValueError(f"{name}: shape {tuple(t.shape)} is not {(tokens, heads, width)}")
-    if t.dtype != dtype:
-        raise ValueError(f"{name}: {t.dtype} is not {dtype}")
-    if t.device != device:
-        raise ValueError(f"{name}: on {t.device}, not on {device}")
-    if width > 1 and t.stride(2) != 1:
+def _rows(t, name: str, dtype: torch.dtype, shape, device):
+    """(data, token stride, head stride) of rows, as in to_rows."""
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        _refuse(t, name, dtype, shape, device)
+    stride = t.stride()
+    if stride[2] != 1 and shape[2] > 1:
         raise ValueError(f"{name}: the last dimension is not contiguous")
-    return abi.Rows(t.data_ptr() if t.numel() else None, t.stride(0), t.stride(1))
+    return t.data_ptr(), stride[0], stride[1]
 
 
-def _flat(t, name: str, dtype: torch.dtype, shape, device, optional: bool = False) -> Optional[int]:
+def _flat(t, name: str, dtype: torch.dtype, shape, device) -> int:
+    """Data of a contiguous tensor; 0 where there is none."""
     if t is None:
-        if optional:
-            return None
-        raise ValueError(f"{name} is missing")
-    if t.shape != tuple(shape):
-        raise ValueError(f"{name}: shape {tuple(t.shape)} is not {tuple(shape)}")
-    if t.dtype != dtype:
-        raise ValueError(f"{name}: {t.dtype} is not {dtype}")
-    if t.device != device:
-        raise ValueError(f"{name}: on {t.device}, not on {device}")
+        return 0
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        _refuse(t, name, dtype, shape, device)
     if not t.is_contiguous():
         raise ValueError(f"{name} is not contiguous")
     return t.data_ptr()
+
+
+def _refuse(t, name, dtype, shape, device):
+    if t.shape != shape:
+        raise ValueError(f"{name}: shape {tuple(t.shape)} is not {tuple(shape)}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name}: {t.dtype} is not {dtype}")
+    raise ValueError(f"{name}: on {t.device}, not on {device}")
+
+
+def _needed(t, name: str):
+    if t is None:
+        raise ValueError(f"{name} is missing")
+    return t
 
 
 def _cuda(t, name: str):
@@ -72,7 +88,7 @@ def _scratch(t, need: int, device):
     if t is None:
         if need:
             raise ValueError(f"a workspace of {need} bytes is needed")
-        return None, 0
+        return 0, 0
     if t.device != device or not t.is_contiguous():
         raise ValueError(f"workspace: on {t.device}, contiguous {t.is_contiguous()}; wanted on {device}")
     return t.data_ptr(), t.numel() * t.element_size()
@@ -109,15 +125,16 @@ class QkNormRotary:
             self._h = None
 
     def _pair(self, q, k, names, tokens, device):
-        return (C.byref(_rows(q, names[0], self.dtype, tokens, self.q_heads, self.head_dim, device)),
-                C.byref(_rows(k, names[1], self.dtype, tokens, self.k_heads, self.head_dim, device)))
+        d = self.head_dim
+        return (_ROWS.pack(*_rows(q, names[0], self.dtype, (tokens, self.q_heads, d), device)),
+                _ROWS.pack(*_rows(k, names[1], self.dtype, (tokens, self.k_heads, d), device)))
 
     def _fixed(self, positions, wq, wk, tokens, device):
-        pos = None
+        pos = 0
         if self.rotary_dim:
-            pos = _flat(positions, "positions", torch.int32, (self.axes, tokens), device)
-        w = [_flat(x, n, torch.float32, (self.head_dim,), device, True) for x, n in ((wq, "wq"), (wk, "wk"))]
-        return pos, w[0], w[1]
+            pos = _flat(_needed(positions, "positions"), "positions", torch.int32, (self.axes, tokens), device)
+        shape = (self.head_dim,)
+        return (pos, _flat(wq, "wq", torch.float32, shape, device), _flat(wk, "wk", torch.float32, shape, device))
 
     def forward(self, q, k, positions, wq, wk, q_out, k_out, stream: int = 0):
         """q_out, k_out <- the normed, weighted and rotated q, k (in place where they are q, k).
@@ -127,8 +144,10 @@ class QkNormRotary:
         tokens, device = q.shape[0], _cuda(q, "q")
         i = self._pair(q, k, ("q", "k"), tokens, device)
         o = self._pair(q_out, k_out, ("q_out", "k_out"), tokens, device)
-        abi.check(abi.lib.to_qk_norm_rotary(self._h, tokens, *i, *self._fixed(positions, wq, wk, tokens, device),
-                                            *o, stream), "to_qk_norm_rotary")
+        st = abi.lib.to_qk_norm_rotary(self._h, tokens, *i, *self._fixed(positions, wq, wk, tokens, device), *o,
+                                       stream)
+        if st:
+            abi.check(st, "to_qk_norm_rotary")
 
     def workspace_bytes(self, tokens: int) -> int:
         """Bytes of `workspace` that backward() needs."""
@@ -136,15 +155,15 @@ class QkNormRotary:
 
     def backward(self, q, k, positions, wq, wk, gq, gk, dq, dk, dwq, dwk, workspace, stream: int = 0):
         """dq, dk, dwq, dwk <- gradients from gq, gk (those of q_out, k_out); q, k are forward()'s inputs."""
-        tokens, device = q.shape[0], _cuda(q, "q")
+        tokens, device, shape = q.shape[0], _cuda(q, "q"), (self.head_dim,)
         i = self._pair(q, k, ("q", "k"), tokens, device)
         g = self._pair(gq, gk, ("gq", "gk"), tokens, device)
         o = self._pair(dq, dk, ("dq", "dk"), tokens, device)
-        dw = [_flat(x, n, torch.float32, (self.head_dim,), device, True) for x, n in ((dwq, "dwq"), (dwk, "dwk"))]
-        ws, size = _scratch(workspace, 1, device)
+        dw = _flat(dwq, "dwq", torch.float32, shape, device), _flat(dwk, "dwk", torch.float32, shape, device)
         abi.check(abi.lib.to_qk_norm_rotary_backward(self._h, tokens, *i,
                                                      *self._fixed(positions, wq, wk, tokens, device), *g, *o, *dw,
-                                                     ws, size, stream), "to_qk_norm_rotary_backward")
+                                                     *_scratch(workspace, 1, device), stream),
+                  "to_qk_norm_rotary_backward")
 
 
 class LinearAttention:
@@ -161,13 +180,11 @@ class LinearAttention:
         self.dtype = _dtype(dtype)
         self.q_heads, self.kv_heads, self.key_dim, self.value_dim = q_heads, kv_heads, key_dim, value_dim
         self.scale = 1.0 / math.sqrt(key_dim) if scale is None else scale
-        self._desc(0, 0)
-        abi.check(abi.lib.to_linear_attention(self._desc(0, 0), C.byref(abi.LinearAttentionArgs()), 0),
-                  "LinearAttention")
+        abi.check(abi.lib.to_linear_attention(self._desc(0, 0), bytes(_ARGS.size), 0), "LinearAttention")
 
-    def _desc(self, tokens: int, nseq: int, slots: int = 0):
-        return C.byref(abi.LinearAttentionDesc(DTYPES[self.dtype], self.q_heads, self.kv_heads, self.key_dim,
-                                               self.value_dim, nseq, tokens, slots, self.scale))
+    def _desc(self, tokens: int, nseq: int, slots: int = 0) -> bytes:
+        return _DESC.pack(DTYPES[self.dtype], self.q_heads, self.kv_heads, self.key_dim, self.value_dim, nseq, tokens,
+                          slots, self.scale)
 
     def workspace_bytes(self, tokens: int, sequences: int) -> int:
         """Bytes of `workspace` that forward() needs (0: none)."""
@@ -176,15 +193,15 @@ class LinearAttention:
     def backward_workspace_bytes(self, tokens: int, sequences: int) -> int:
         return abi.lib.to_linear_attention_backward_workspace_bytes(self._desc(tokens, sequences))
 
-    def _kv(self, t, name, tokens, width, device):
-        return _rows(t, name, self.dtype, tokens, self.kv_heads, width, device)
+    def _inputs(self, tokens, device, tensors):
+        """Rows of (tensor, name, is a query head's, width) each, in one list."""
+        out = []
+        for t, name, query, width in tensors:
+            out += _rows(t, name, self.dtype, (tokens, self.q_heads if query else self.kv_heads, width), device)
+        return out
 
-    def _q(self, t, name, tokens, width, device):
-        return _rows(t, name, self.dtype, tokens, self.q_heads, width, device)
-
-    def _state(self, t, name, device, slots=None):
-        n = t.shape[0] if slots is None and t is not None else slots
-        return _flat(t, name, torch.float32, (n, self.q_heads, self.key_dim, self.value_dim), device, True)
+    def _state(self, t, name, device, slots):
+        return _flat(t, name, torch.float32, (slots, self.q_heads, self.key_dim, self.value_dim), device)
 
     def _sequences(self, cu_seqlens, device):
         n = cu_seqlens.numel() - 1
@@ -193,7 +210,7 @@ class LinearAttention:
         return n, _flat(cu_seqlens, "cu_seqlens", torch.int32, (n + 1,), device)
 
     def _decay(self, log_decay, device):
-        return _flat(log_decay, "log_decay", torch.float32, (self.q_heads,), device)
+        return _flat(_needed(log_decay, "log_decay"), "log_decay", torch.float32, (self.q_heads,), device)
 
     def forward(self, q, k, v, log_decay, cu_seqlens, o, state_in=None, state_out=None, slots=None, workspace=None,
                 stream: int = 0):
@@ -205,32 +222,34 @@ class LinearAttention:
         """
         tokens, device = q.shape[0], _cuda(q, "q")
         n, cu = self._sequences(cu_seqlens, device)
-        have = next((t.shape[0] for t in (state_in, state_out) if t is not None), n)
+        have = n if state_in is None and state_out is None else (state_out if state_in is None else state_in).shape[0]
         if slots is None and have != n:
             raise ValueError(f"{have} states for {n} sequences, and no slots")
-        need = self.workspace_bytes(tokens, n)
-        ws, size = _scratch(workspace, need, device)
-        a = abi.LinearAttentionArgs(
-            self._q(q, "q", tokens, self.key_dim, device), self._kv(k, "k", tokens, self.key_dim, device),
-            self._kv(v, "v", tokens, self.value_dim, device), self._q(o, "o", tokens, self.value_dim, device),
-            self._decay(log_decay, device), cu, _flat(slots, "slots", torch.int32, (n,), device, True),
-            self._state(state_in, "state_in", device, have if state_in is not None else None),
-            self._state(state_out, "state_out", device, have if state_out is not None else None), ws, size)
-        abi.check(abi.lib.to_linear_attention(self._desc(tokens, n, have), C.byref(a), stream),
-                  "to_linear_attention")
+        desc, dk, dv = self._desc(tokens, n, have), self.key_dim, self.value_dim
+        args = _ARGS.pack(
+            *self._inputs(tokens, device, ((q, "q", True, dk), (k, "k", False, dk), (v, "v", False, dv),
+                                           (o, "o", True, dv))),
+            self._decay(log_decay, device), cu, _flat(slots, "slots", torch.int32, (n,), device),
+            self._state(state_in, "state_in", device, have), self._state(state_out, "state_out", device, have),
+            *_scratch(workspace, abi.lib.to_linear_attention_workspace_bytes(desc), device))
+        st = abi.lib.to_linear_attention(desc, args, stream)
+        if st:
+            abi.check(st, "to_linear_attention")
 
     def step(self, q, k, v, log_decay, state, o, slots=None, stream: int = 0):
         """One token of each request: its state is updated in place, o <- its output."""
-        tokens, device = q.shape[0], _cuda(q, "q")
-        if slots is None and state.shape[0] < tokens:
-            raise ValueError(f"{state.shape[0]} states for {tokens} requests, and no slots")
-        a = abi.LinearAttentionArgs(
-            self._q(q, "q", tokens, self.key_dim, device), self._kv(k, "k", tokens, self.key_dim, device),
-            self._kv(v, "v", tokens, self.value_dim, device), self._q(o, "o", tokens, self.value_dim, device),
-            self._decay(log_decay, device), None, _flat(slots, "slots", torch.int32, (tokens,), device, True),
-            None, self._state(state, "state", device))
-        abi.check(abi.lib.to_linear_attention_step(self._desc(tokens, 0, state.shape[0]), C.byref(a), stream),
-                  "to_linear_attention_step")
+        tokens, device, have = q.shape[0], _cuda(q, "q"), state.shape[0]
+        if slots is None and have < tokens:
+            raise ValueError(f"{have} states for {tokens} requests, and no slots")
+        dk, dv = self.key_dim, self.value_dim
+        args = _ARGS.pack(
+            *self._inputs(tokens, device, ((q, "q", True, dk), (k, "k", False, dk), (v, "v", False, dv),
+                                           (o, "o", True, dv))),
+            self._decay(log_decay, device), 0, _flat(slots, "slots", torch.int32, (tokens,), device), 0,
+            self._state(state, "state", device, have), 0, 0)
+        st = abi.lib.to_linear_attention_step(self._desc(tokens, 0, have), args, stream)
+        if st:
+            abi.check(st, "to_linear_attention_step")
 
     def backward(self, q, k, v, log_decay, cu_seqlens, do, dq, dk, dv, state_in=None, dstate_out=None,
                  dstate_in=None, workspace=None, stream: int = 0):
@@ -240,14 +259,14 @@ class LinearAttention:
         """
         tokens, device = q.shape[0], _cuda(q, "q")
         n, cu = self._sequences(cu_seqlens, device)
-        need = self.backward_workspace_bytes(tokens, n)
-        ws, size = _scratch(workspace, need, device)
-        states = [self._state(t, name, device, n) if t is not None else None
-                  for t, name in ((state_in, "state_in"), (dstate_out, "dstate_out"), (dstate_in, "dstate_in"))]
-        a = abi.LinearAttentionGradArgs(
-            self._q(q, "q", tokens, self.key_dim, device), self._kv(k, "k", tokens, self.key_dim, device),
-            self._kv(v, "v", tokens, self.value_dim, device), self._q(do, "do", tokens, self.value_dim, device),
-            self._q(dq, "dq", tokens, self.key_dim, device), self._kv(dk, "dk", tokens, self.key_dim, device),
-            self._kv(dv, "dv", tokens, self.value_dim, device), self._decay(log_decay, device), cu, *states, ws, size)
-        abi.check(abi.lib.to_linear_attention_backward(self._desc(tokens, n, n), C.byref(a), stream),
-                  "to_linear_attention_backward")
+        desc, wk, wv = self._desc(tokens, n, n), self.key_dim, self.value_dim
+        args = _GRAD_ARGS.pack(
+            *self._inputs(tokens, device, ((q, "q", True, wk), (k, "k", False, wk), (v, "v", False, wv),
+                                           (do, "do", True, wv), (dq, "dq", True, wk), (dk, "dk", False, wk),
+                                           (dv, "dv", False, wv))),
+            self._decay(log_decay, device), cu, self._state(state_in, "state_in", device, n),
+            self._state(dstate_out, "dstate_out", device, n), self._state(dstate_in, "dstate_in", device, n),
+            *_scratch(workspace, abi.lib.to_linear_attention_backward_workspace_bytes(desc), device))
+        st = abi.lib.to_linear_attention_backward(desc, args, stream)
+        if st:
+            abi.check(st, "to_linear_attention_backward")
