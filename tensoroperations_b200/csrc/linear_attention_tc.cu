@@ -1,34 +1,35 @@
 // linear_attention_tc.cu -- the decayed chain (linear_attention.cuh) of bf16
 // rows on the 5th-generation tensor cores: tcgen05 + TMEM + TMA.
 //
-// A work item is one segment of one head; a CTA walks its items and their
-// chunks of 128 tokens.  With Q, K, V the chunk's rows of a, b, c (tiles of
-// 128 x 128, narrower widths zero-filled by TMA) and X the state:
+// A CTA takes one segment of one head and walks its chunks of 128 tokens.  With
+// Q, K, V the chunk's rows of a, b, c (tiles of 128 x 128, narrower widths
+// zero-filled by TMA) and X the state:
 //   Sc = Q K^T                    P = Sc masked, decayed and scaled, bf16, in TMEM
 //   O  = Q X (bf16 X), its rows scaled in TMEM by inter l^(..), then O += P V
 //   U  = (decayed K)^T V          X = l^n X + U (f32, in registers)
-// all M = N = 128.  Six products of 128^3 a chunk with three planes of K, 3072
-// tensor cycles at the dense bf16 rate, against about 5600 for the chunk's 128
-// KB at this SM's share of the HBM.  What else bounds it is the shared memory's
-// 128 bytes a cycle: a product of two shared operands of this size takes all of
-// it, so P and decayed K are TMEM operands (K transposed into its lanes by
-// ldmatrix), which leaves 256 KB a chunk to the products.
+// all M = N = 128.  Five or six products of 128^3 a chunk, 2560 or 3072 tensor
+// cycles at the dense bf16 rate, against about 5600 for the chunk's 128 KB at
+// this SM's share of the HBM.  A product of two shared operands of this size
+// takes all of the shared memory's 128 bytes a cycle, so P and decayed K are
+// TMEM operands (K transposed into its lanes by ldmatrix).
 //
 // Precision: P and X each enter their product with one bf16 rounding, as the
-// result's own.  The state stays f32: decayed K is split into PLANES bf16
-// values (8 bits each; 3 reach f32, 2 are enough where only out reads the
-// state), smallest plane first, so few sums pass through the accumulator at
-// full size; a chunk's U is added to X in IEEE f32 registers.
+// result's own.  The state stays f32: decayed K is split into bf16 planes of 8
+// bits each -- three, which reach f32, where the state is written out, two where
+// only products read it -- smallest plane first, so few sums pass through the
+// accumulator at full size; a chunk's U is added to X in IEEE f32 registers.
 //
-// Roles (20 warps): one lane issues TMA loads into two stages of three
-// 32 KB tiles, one the products; warps 4-11 turn Sc into P (and make plane 0,
-// whose columns are theirs), scale O and store the results (a thread: one row,
-// 64 columns); warps 12-19 make the other planes and hold X (a thread: one row, 64 columns).  Products are issued Sc, Q X, P V, U:
-// the results are stored under U, and the next chunk's Sc runs under the state's
-// update.  Rows
-// past a chunk's end are masked: P and the planes by selection, V by zeroing
-// its rows, since 0 * NaN is not 0.  Rows of a reversed chain keep their order
-// in memory; only the masks and decays turn round.
+// Roles (20 warps): one lane issues TMA loads, two chunks ahead, one the
+// products; warps 4-11 turn Sc into P, scale O and store the results (a thread:
+// one row, 64 columns); warps 12-19 make planes 0 and 1 and hold X (a thread: one
+// row, 64 columns).  Plane 2 lies in O's columns between one chunk's results
+// and the next one's, so the row warps make it.  Products are issued U, Q X,
+// P V and the next chunk's Sc: the row warps store results and make the next P
+// while the state warps make the next planes.  In the states' launch there is
+// no Sc and no O: both groups make planes, into two buffers in turn.  Rows past
+// a chunk's end are masked: P by selection, K and V by zeroing their rows, since
+// 0 * NaN is not 0.  Rows of a reversed chain keep their order in memory; only
+// the masks and decays turn round.
 //
 // Every wait is bounded; on a timeout the kernel records TO_ERR_TIMEOUT in the
 // device status word, waits (bounded) for its copies in flight, frees its TMEM
@@ -56,23 +57,33 @@ constexpr int kRowWarps = 8, kStateWarps = 8;    // P and out; planes and X
 constexpr int kFirstRow = 4, kFirstState = kFirstRow + kRowWarps;  // warps 0, 1: loads, products; 2, 3: none
 constexpr int kThreads = 32 * (kFirstState + kStateWarps);
 constexpr uint32_t kMaxPolls = 1u << 22;
-constexpr int kStages = 2;                       // chunks in shared memory: tiles Q, K, V of each
-constexpr uint32_t kStageBytes = 3 * kTileBytes;
+constexpr int kMaxStages = 3;
+
+// Chunks in shared memory, 192 KB of them: tiles Q, K, V each, or K, V.
+template <bool STATES>
+struct Ring {
+  static constexpr int kStages = STATES ? 3 : 2;
+  static constexpr uint32_t kK = STATES ? 0 : kTileBytes, kV = kK + kTileBytes, kBytes = kV + kTileBytes;
+};
 
 // TMEM columns.  P of tokens [0, 64) and [64, 128) overwrites the first halves
-// of those tokens' columns of Sc; plane 0 takes the second halves, once Sc has
-// been read; planes 1 and 2 (the smaller ones) have columns of their own.
-constexpr uint32_t kColS = 0, kColO = 128, kColU = 256, kColPlane = 384;
+// of those tokens' columns of Sc.
+constexpr uint32_t kColS = 0, kColO = 128;
 template <bool STATES>
-__device__ __forceinline__ uint32_t plane_col(int plane, int token64) {
-  return plane == 0 ? kColS + 64 * token64 + (STATES ? 0 : 32) : kColPlane + 64 * (plane - 1) + 32 * token64;
+constexpr uint32_t kColU = STATES ? 0 : 256;
+// Plane p of a chunk, tokens [64 h, 64 h + 64): 32 columns.
+template <bool STATES>
+__device__ __forceinline__ uint32_t plane_col(uint32_t chunk, int p, int h) {
+  if (STATES) return 128 + 192 * (chunk & 1) + 64 * p + 32 * h;
+  return p == 2 ? kColO + 64 * h : 384 + 64 * p + 32 * h;
 }
 
 struct Barriers {
-  uint64_t full[kStages], empty[kStages];
+  uint64_t full[kMaxStages], empty[kMaxStages];      // (Q and) K of a chunk
+  uint64_t full_v[kMaxStages], empty_v[kMaxStages];  // its V
+  // once a chunk each
   uint64_t sc_full, p_ready, o1_full, o2_full, o_free;
-  uint64_t planes_ready, u_full, x_ready;
-  uint64_t row_table, state_table;
+  uint64_t planes_ready, u_full, u_free, x_ready;
   uint32_t tmem;
   int abort;
 };
@@ -232,23 +243,11 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ float low_half(uint32_t r) { return __uint_as_float(r << 16); }
 __device__ __forceinline__ float high_half(uint32_t r) { return __uint_as_float(r & 0xffff0000u); }
 
-// A table that the eight warps of a group make for their item, f(n) for n <
-// count.  Two tables in turn: a warp that has passed an item's barrier knows
-// that all have left the table before the last.
-constexpr int kRowTable = 164;    // l^n, n = 0 .. 128; the 32 factors of a block's columns from 132 on
-constexpr int kStateTable = 132;  // l^n, n = 0 .. 128
-template <typename F>
-__device__ __forceinline__ uint32_t make_table(Barriers* b, uint64_t* bar, float* tables, int size, uint32_t turn,
-                                               int t, bool* ok, F f) {
-  float* mine = tables + (turn & 1) * size;
-  if (t < size) mine[t] = f(t);
-  __syncwarp();
-  if ((t & 31) == 0) arrive(bar);
-  *ok = warp_wait(b, bar, turn & 1);
-  return smem_u32(mine);
-}
+// Tables: l^n, n = 0 .. 128, and from 132 on the 32 factors of a block's columns;
+// the first again times `upd`.
+constexpr int kTable = 164, kUpdTable = 132;
 
-// The chunks of an item (a segment of one head).
+// The segment of one head that a CTA walks.
 struct Walk {
   int seq, head;
   bool last, only;      // the sequence's last segment; its only one
@@ -280,16 +279,17 @@ __device__ __forceinline__ bool walk_of(const Chain& C, int item, Walk* w) {
   return true;
 }
 
-// Planes FROM .. TO-1 of decayed K: lanes [32 q, 32 q + 32) of K^T, tokens [64 h,
-// 64 h + 64), from the chunk's tile of K.  All but the last plane are cut off, not
-// rounded, so each is the product's own next eight bits.
-template <bool STATES, int PLANES, int FROM, int TO>
-__device__ __forceinline__ void make_planes(uint32_t tile, uint32_t lanes, uint32_t dec, int cnt, bool rev, float upd,
-                                            int q, int h, int lane) {
+// Planes FROM .. TO-1 of decayed K: lanes [32 q, 32 q + 32) of K^T, tokens 64 h + 16 g
+// .. for g of [g0, g1), from the chunk's tile of K; `lanes`: the quarter's TMEM address.
+// All but the last plane (three says whether that is plane 2) are cut off, not rounded,
+// so each is the product's own next eight bits.
+template <bool STATES, int FROM, int TO>
+__device__ __forceinline__ void make_planes(uint32_t tile, uint32_t lanes, uint32_t chunk, uint32_t dec, int cnt,
+                                            bool rev, bool three, int q, int h, int g0, int g1, int lane) {
   const uint32_t panel = tile + (q >> 1) * kPanel;
   if (cnt < kTile) {  // rows past the end: zero what this warp reads
-    for (int e = lane; e < 256; e += 32) {
-      const int row = 64 * h + (e >> 2);
+    for (int e = lane; e < 64 * (g1 - g0); e += 32) {
+      const int row = 64 * h + 16 * g0 + (e >> 2);
       if (row >= cnt) sts4(panel + row * 128 + (((4 * (q & 1) + (e & 3)) ^ (row & 7)) << 4), 0, 0, 0, 0);
     }
     fence_async();  // before the tile is loaded again
@@ -298,25 +298,27 @@ __device__ __forceinline__ void make_planes(uint32_t tile, uint32_t lanes, uint3
   // tile m of an ldmatrix: rows 8 (m & 1) .. of 16 lanes, tokens 8 (m >> 1) .. of 16
   const int m = lane >> 3;
 #pragma unroll 1
-  for (int g = 0; g < 4; ++g) {
+  for (int g = g0; g < g1; ++g) {
     const int row = 64 * h + 16 * g + 8 * (m >> 1) + (lane & 7);
     float2 d[2];
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
       const int j = 64 * h + 16 * g + 8 * z + 2 * (lane & 3), age = rev ? j + 1 : cnt - 1 - j;
-      d[z] = make_float2(upd * lds(dec + 4 * max(age, 0)), upd * lds(dec + 4 * max(rev ? age + 1 : age - 1, 0)));
+      d[z] = make_float2(lds(dec + 4 * max(age, 0)), lds(dec + 4 * max(rev ? age + 1 : age - 1, 0)));
     }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      uint32_t k[4], out[PLANES][4];
+      uint32_t k[4], out[TO][4];
       ldmatrix_t4(panel + row * 128 + (((4 * (q & 1) + 2 * half + (m & 1)) ^ (row & 7)) << 4), k);
 #pragma unroll
       for (int z = 0; z < 4; ++z) {
         float2 x = __fmul2_rn(make_float2(low_half(k[z]), high_half(k[z])), d[z >> 1]);
 #pragma unroll
         for (int p = 0; p < TO; ++p) {
-          out[p][z] = p == PLANES - 1 ? pack2(x.x, x.y)
-                                      : __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
+          if (p == 2 || (p == 1 && !three))
+            out[p][z] = pack2(x.x, x.y);
+          else
+            out[p][z] = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632);
           if (p + 1 < TO)
             x = __ffma2_rn(make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffff0000u),
                                        __uint_as_float(__float_as_uint(x.y) & 0xffff0000u)),
@@ -325,18 +327,18 @@ __device__ __forceinline__ void make_planes(uint32_t tile, uint32_t lanes, uint3
       }
 #pragma unroll
       for (int p = FROM; p < TO; ++p)
-        tmem_st_tiles(lanes + (uint32_t(16 * half) << 16) + 8 * g + plane_col<STATES>(p, h), out[p]);
+        tmem_st_tiles(lanes + (uint32_t(16 * half) << 16) + 8 * g + plane_col<STATES>(chunk, p, h), out[p]);
     }
   }
   tmem_st_wait();
 }
 
 // Shared memory
-constexpr uint32_t kX = kStages * kStageBytes;                             // bf16 X
-constexpr uint32_t kRowTables = kX + kTileBytes;
-constexpr uint32_t kStateTables = kRowTables + 2 * kRowTable * 4;
-constexpr uint32_t kBars = kStateTables + 2 * kStateTable * 4;
+constexpr uint32_t kX = 6 * kTileBytes;  // bf16 X, behind the chunks
+constexpr uint32_t kTables = kX + kTileBytes;
+constexpr uint32_t kBars = kTables + (kTable + kUpdTable) * 4;
 constexpr uint32_t kSmem = kBars + sizeof(Barriers);
+static_assert(Ring<true>::kStages * Ring<true>::kBytes <= kX && Ring<false>::kStages * Ring<false>::kBytes <= kX, "ring");
 static_assert(kBars % 8 == 0 && kSmem <= 232448, "shared memory of a CTA");
 
 // Registers: the launch gives each of the 20 warps 96; those that hold X take some of
@@ -350,38 +352,55 @@ __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.
 template <int N>
 __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
-template <typename TO, bool STATES, int PLANES>
+template <typename TO, bool STATES>
 __global__ void __launch_bounds__(kThreads, 1)
     chain_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
-                    const __grid_constant__ CUtensorMap mapC, const __grid_constant__ Chain C,
-                    const int items) {
+                    const __grid_constant__ CUtensorMap mapC, const __grid_constant__ Chain C) {
+  using R = Ring<STATES>;
+  constexpr int kStages = R::kStages;
   extern __shared__ __align__(1024) unsigned char sm[];
-  if (smem_u32(sm) & 1023) {  // the swizzled tiles need it; there is no room left to round up in
+  const int item = blockIdx.x;  // segment slot * heads + head
+  Walk w;
+  if (!walk_of<STATES>(C, item, &w)) return;
+  const uint32_t base = smem_u32(sm);
+  if (base & 1023) {  // the swizzled tiles need it; there is no room left to round up in
     if (threadIdx.x == 0) atomicExch(&g_sequence_status, int(TO_ERR_SCRATCH));
     return;
   }
   Barriers* bar = reinterpret_cast<Barriers*>(sm + kBars);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool rev = C.rev != 0;
+  // planes of this item: three where its state is a result
+  const bool three = C.fin && (STATES || w.last);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&bar->full[i], 1);
-      // a chunk's tiles are free when its products are done (a commit), its planes made and
-      // its results, which pass through Q's tile, stored
-      mbar_init(&bar->empty[i], 1 + kStateWarps + (STATES ? 0 : kRowWarps));
+      mbar_init(&bar->full_v[i], 1);
+      // Q and K are free when their products are done (a commit) and the planes made; V when
+      // its products are done and the results, which pass through its tile, stored
+      mbar_init(&bar->empty[i], kStateWarps + (STATES ? kRowWarps : three ? kRowWarps + 1 : 1));
+      mbar_init(&bar->empty_v[i], STATES ? 1 : kRowWarps);
     }
     mbar_init(&bar->sc_full, 1);
     mbar_init(&bar->p_ready, kRowWarps);
     mbar_init(&bar->o1_full, 1);
     mbar_init(&bar->o2_full, 1);
     mbar_init(&bar->o_free, kRowWarps);
-    mbar_init(&bar->planes_ready, kStateWarps + (STATES ? 0 : kRowWarps));
+    mbar_init(&bar->planes_ready, kStateWarps + (STATES || three ? kRowWarps : 0));
     mbar_init(&bar->u_full, 1);
+    mbar_init(&bar->u_free, kStateWarps);
     mbar_init(&bar->x_ready, kStateWarps);
-    mbar_init(&bar->row_table, kRowWarps);
-    mbar_init(&bar->state_table, kStateWarps);
     bar->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  {
+    float* table = reinterpret_cast<float*>(sm + kTables);
+    const float gl = lin::log_decay_of(C, w.head);
+    for (int t = threadIdx.x; t < kTable + kUpdTable; t += kThreads) {
+      const int n = t < 132 ? t : t < kTable ? (rev ? t - 132 : 163 - t) : t - kTable;
+      table[t] = expf(gl * static_cast<float>(n)) * (t < kTable ? 1.f : C.upd);
+    }
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&bar->tmem))
@@ -391,263 +410,261 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = bar->tmem;
-  const uint32_t base = smem_u32(sm);
-  auto stage_of = [&](uint32_t n) { return base + (n & 1) * kStageBytes; };
-  Walk w;
+  const uint32_t tmem = bar->tmem, dec = base + kTables, dec_upd = dec + kTable * 4;
+  auto stage_of = [&](uint32_t n) { return base + (STATES ? n % kStages : n & 1) * R::kBytes; };
+  auto turn_of = [&](uint32_t n) { return (n / kStages) & 1; };
+  bool ok = true;
 
   if (warp < kFirstRow) {
     registers_down<64>();
     if (warp == 0 && lane == 0) {
       // ---- loads: (Q,) K, V of each chunk ----
-      uint32_t n = 0;
-      bool ok = true;
-      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-        if (!walk_of<STATES>(C, item, &w)) continue;
-        for (int i = 0; i < w.n; ++i, ++n) {
-          const int token = w.first(C, i);
-          uint64_t* full = &bar->full[n & 1];
-          if (n >= kStages && !(ok = wait_for(bar, &bar->empty[n & 1], (n / kStages - 1) & 1))) break;
-          mbar_arrive_expect_tx(full, STATES ? 2 * kTileBytes : kStageBytes);
-          if (!STATES) tma_tile(stage_of(n), &mapA, w.head / C.a_div, token, full);
-          tma_tile(stage_of(n) + kTileBytes, &mapB, w.head / C.b_div, token, full);
-          tma_tile(stage_of(n) + 2 * kTileBytes, &mapC, w.head / C.c_div, token, full);
-        }
+      int i = 0, qk = 0;
+      for (; i < w.n; ++i) {
+        const int token = w.first(C, i);
+        uint64_t *full = &bar->full[i % kStages], *full_v = &bar->full_v[i % kStages];
+        if (i >= kStages && !(ok = wait_for(bar, &bar->empty[i % kStages], turn_of(i - kStages)))) break;
+        mbar_arrive_expect_tx(full, R::kV);
+        if (!STATES) tma_tile(stage_of(i), &mapA, w.head / C.a_div, token, full);
+        tma_tile(stage_of(i) + R::kK, &mapB, w.head / C.b_div, token, full);
+        qk = i + 1;
+        if (i >= kStages && !(ok = wait_for(bar, &bar->empty_v[i % kStages], turn_of(i - kStages)))) break;
+        mbar_arrive_expect_tx(full_v, kTileBytes);
+        tma_tile(stage_of(i) + R::kV, &mapC, w.head / C.c_div, token, full_v);
       }
       // copies still in flight land before the CTA ends
-      for (uint32_t t = n > kStages ? n - kStages : 0; t < n; ++t)
-        mbar_wait_bounded(&bar->full[t & 1], (t / kStages) & 1, kMaxPolls);
+      for (int t = qk > kStages ? qk - kStages : 0; t < qk; ++t) {
+        mbar_wait_bounded(&bar->full[t % kStages], turn_of(t), kMaxPolls);
+        if (t < i) mbar_wait_bounded(&bar->full_v[t % kStages], turn_of(t), kMaxPolls);
+      }
     } else if (warp == 1 && lane == 0) {
       // ---- products ----
-      uint32_t n = 0;  // chunks so far
-      bool ok = true;
-      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-        if (!walk_of<STATES>(C, item, &w)) continue;
-        for (int i = 0; i < w.n; ++i, ++n) {
-          const uint32_t turn = n & 1, sq = fresh(stage_of(n)), sk = sq + kTileBytes, sv = sk + kTileBytes;
-          const uint32_t tm = fresh(tmem), sx = fresh(base) + kX;
-          if (!(ok = wait_for(bar, &bar->full[turn], (n / kStages) & 1))) break;
-          if (!STATES) {
-            fence_after();
+      const int planes = three ? 3 : 2;
+      auto scores = [&](int i) {
+        const uint32_t sq = fresh(stage_of(i)), tm = fresh(tmem);
+        if (!(ok = wait_for(bar, &bar->full[i % kStages], turn_of(i)))) return;
+        fence_after();
 #pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
-              mma(tm + kColS, desc_k(sq, k), desc_k(sk, k), kIdesc, k > 0);
-            commit(&bar->sc_full);
-            if (!(ok = wait_for(bar, &bar->x_ready, turn) && (n == 0 || wait_for(bar, &bar->o_free, turn ^ 1)))) break;
-            fence_after();
-#pragma unroll
-            for (int k = 0; k < kTile / 16; ++k)
-              mma(tm + kColO, desc_k(sq, k), desc_mn(sx, k), kIdesc | kMnB, k > 0);
-            commit(&bar->o1_full);
-          }
-          if (!STATES) {
-            if (!(ok = wait_for(bar, &bar->p_ready, turn))) break;
-            fence_after();
+        for (int k = 0; k < kTile / 16; ++k) mma(tm + kColS, desc_k(sq, k), desc_k(sq + R::kK, k), kIdesc, k > 0);
+        commit(&bar->sc_full);
+      };
+      if (!STATES && w.n > 0) scores(0);
+      for (int i = 0; i < w.n && ok; ++i) {
+        const uint32_t turn = i & 1, sq = fresh(stage_of(i)), sv = sq + R::kV;
+        const uint32_t tm = fresh(tmem), sx = fresh(base) + kX;
+        if (i < w.updates) {
+          // (outputs: the state warps have read the last U before they make planes)
+          if (!(ok = wait_for(bar, &bar->full_v[i % kStages], turn_of(i)) && wait_for(bar, &bar->planes_ready, turn) &&
+                     (!STATES || i == 0 || wait_for(bar, &bar->u_free, turn ^ 1))))
+            break;
+          fence_after();
+#pragma unroll 1
+          for (int p = planes - 1; p >= 0; --p)
 #pragma unroll
             for (int k = 0; k < kTile / 16; ++k)  // 16 tokens: 8 columns
-              mma_ts(tm + kColO, tm + kColS + (k >> 2) * 64 + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB, true);
-            commit(&bar->o2_full);
-          }
-          if (i < w.updates) {
-            // also: the last chunk's U has been read
-            if (!(ok = wait_for(bar, &bar->planes_ready, turn))) break;
-            fence_after();
-#pragma unroll 1
-            for (int p = PLANES - 1; p >= 0; --p)
-#pragma unroll
-              for (int k = 0; k < kTile / 16; ++k)
-                mma_ts(tm + kColU, tm + plane_col<STATES>(p, k >> 2) + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB,
-                       p < PLANES - 1 || k > 0);
-            commit(&bar->u_full);
-          }
-          commit(&bar->empty[turn]);
+              mma_ts(tm + kColU<STATES>, tm + plane_col<STATES>(i, p, k >> 2) + (k & 3) * 8, desc_mn(sv, k),
+                     kIdesc | kMnB, p < planes - 1 || k > 0);
+          commit(&bar->u_full);
         }
+        if (!STATES) {
+          // x_ready also says that V's rows past the end are zero
+          if (!(ok = wait_for(bar, &bar->x_ready, turn) && (i == 0 || wait_for(bar, &bar->o_free, turn ^ 1)))) break;
+          fence_after();
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k)
+            mma(tm + kColO, desc_k(sq, k), desc_mn(sx, k), kIdesc | kMnB, k > 0);
+          commit(&bar->o1_full);
+          commit(&bar->empty[i % kStages]);
+          if (!(ok = wait_for(bar, &bar->full_v[i % kStages], turn_of(i)) && wait_for(bar, &bar->p_ready, turn))) break;
+          fence_after();
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k)
+            mma_ts(tm + kColO, tm + kColS + (k >> 2) * 64 + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB, true);
+          commit(&bar->o2_full);
+        }
+        if (STATES) commit(&bar->empty_v[i % kStages]);
+        else if (i + 1 < w.n) scores(i + 1);
       }
     }
   } else if (warp < kFirstState) {
     registers_down<88>();
-    if (!STATES) {
+    const int q = warp & 3, h = (warp - kFirstRow) >> 2;
+    const uint32_t lanes = tmem + (uint32_t(q * 32) << 16);
+    if (STATES) {
+      // ---- the planes of every second 32 tokens ----
+      for (int i = 0; i < w.n; ++i) {
+        if (!(ok = warp_wait(bar, &bar->full[i % kStages], turn_of(i)))) break;
+        if (three)
+          make_planes<STATES, 0, 3>(stage_of(i) + R::kK, lanes, i, dec_upd, w.rows(i), rev, true, q, h, 2, 4, lane);
+        else
+          make_planes<STATES, 0, 2>(stage_of(i) + R::kK, lanes, i, dec_upd, w.rows(i), rev, false, q, h, 2, 4, lane);
+        // the next planes go where those of chunk i - 1 are read (waited for here, before this
+        // chunk's product can end, so that the barrier is at most one turn ahead)
+        if (i > 0 && !(ok = warp_wait(bar, &bar->u_full, (i - 1) & 1))) break;
+        fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          arrive(&bar->planes_ready);
+          arrive(&bar->empty[i % kStages]);
+        }
+        fence_after();
+      }
+    } else {
       // ---- P, O and the results: row r of the chunk, columns [64 h, 64 h + 64) ----
-      const int q = warp & 3, h = (warp - kFirstRow) >> 2;
       const int r = q * 32 + lane;
-      const uint32_t lanes = tmem + (uint32_t(q * 32) << 16);
-      const bool rev = C.rev != 0;
       const float intra = C.intra, inter = C.inter;
       const long long pitch = C.out.ts;
-      uint32_t n = 0, tables = 0;
-      bool ok = true;
-      for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-        if (!walk_of<STATES>(C, item, &w)) continue;
-        const float gl = lin::log_decay_of(C, w.head);
-        const uint32_t dec = make_table(bar, &bar->row_table, reinterpret_cast<float*>(sm + kRowTables), kRowTable, tables++, threadIdx.x - 32 * kFirstRow, &ok, [&](int t) {
-                                        const int e = t < 132 ? t : C.rev ? t - 132 : 163 - t;
-                                        return expf(gl * static_cast<float>(e));
-                                      });
-        if (!ok) break;
-        for (int i = 0; i < w.n; ++i, ++n) {
-          const int cnt = w.rows(i);
-          // P[r][j] = intra Sc[r][j] l^|r - j| where j has been seen by r: blocks of 16
-          // columns, of which this warp's rows see all, a triangle, or nothing.  (Each block's
-          // P lands on columns of Sc that this warp has read by then.)
-          if (!(ok = warp_wait(bar, &bar->sc_full, n & 1))) break;
-          fence_after();
-#pragma unroll 1
-          for (int part = 0; part < 4; ++part) {
-            const int block = 4 * h + part, j0 = 16 * block;
-            uint32_t p[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = 0;
-            const bool diagonal = block >> 1 == q;
-            if (diagonal || (block < 2 * q) != rev) {
-              float x[16];
-              tmem_ld16(lanes + kColS + j0, x);
-              if (diagonal) {
-#pragma unroll
-                for (int j8 = 0; j8 < 16; j8 += 8) {
-                  float d[8];
-#pragma unroll
-                  for (int j = 0; j < 8; ++j) d[j] = lds(dec + 4 * abs(r - j0 - j8 - j));
-#pragma unroll
-                  for (int j = 0; j < 8; ++j) {
-                    const int at = j0 + j8 + j;
-                    x[j8 + j] = (rev ? at >= r : at <= r) ? x[j8 + j] * (intra * d[j]) : 0.f;
-                  }
-                }
-              } else {
-                const float base = intra * lds(dec + 4 * (rev ? j0 - r : r - j0 - 15));
-                const float2 b2 = make_float2(base, base);
-                const uint32_t col = dec + 4 * (rev ? 132 : 148);
-#pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                  const uint4 d = lds4(col + 4 * j);
-                  const float2 y0 = __fmul2_rn(make_float2(x[j], x[j + 1]),
-                                               __fmul2_rn(b2, make_float2(__uint_as_float(d.x), __uint_as_float(d.y))));
-                  const float2 y1 = __fmul2_rn(make_float2(x[j + 2], x[j + 3]),
-                                               __fmul2_rn(b2, make_float2(__uint_as_float(d.z), __uint_as_float(d.w))));
-                  x[j] = y0.x;
-                  x[j + 1] = y0.y;
-                  x[j + 2] = y1.x;
-                  x[j + 3] = y1.y;
-                }
-              }
-              if (cnt < kTile) {  // the columns of rows that are not this chunk's
-#pragma unroll
-                for (int j = 0; j < 16; ++j) x[j] = j0 + j < cnt ? x[j] : 0.f;
-              }
-#pragma unroll
-              for (int j = 0; j < 16; j += 2) p[j >> 1] = pack2(x[j], x[j + 1]);
-            }
-            tmem_st8(lanes + kColS + h * 64 + part * 8, p);
-          }
-          // Q X, decayed from the chunk's beginning
-          const float f = inter * lds(dec + 4 * max(rev ? cnt - 1 - r : r + 1, 0));
-          if (!(ok = warp_wait(bar, &bar->o1_full, n & 1))) break;
-          fence_after();
-#pragma unroll 1
-          for (int part = 0; part < 2; ++part) {
-            float x[32];
-            tmem_ld32(lanes + kColO + h * 64 + part * 32, x);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] *= f;
-            tmem_st32(lanes + kColO + h * 64 + part * 32, x);
-          }
-          tmem_st_wait();
+      for (int i = 0; i < w.n; ++i) {
+        const int cnt = w.rows(i);
+        const uint32_t turn = i & 1;
+        // plane 2 into this warp's part of O, which it has read
+        if (three && i < w.updates) {
+          if (!(ok = warp_wait(bar, &bar->full[i % kStages], turn_of(i)))) break;
+          make_planes<STATES, 2, 3>(stage_of(i) + R::kK, lanes, i, dec_upd, cnt, rev, true, q, h, 0, 4, lane);
           fence_before();
           __syncwarp();
-          if (lane == 0) arrive(&bar->p_ready);
-          // plane 0 into the other half of this warp's columns of Sc
-          if (i < w.updates)
-            make_planes<STATES, PLANES, 0, 1>(stage_of(n) + kTileBytes, lanes, dec, cnt, rev, C.upd, q, h, lane);
-          fence_before();
-          __syncwarp();
-          if (lane == 0) arrive(&bar->planes_ready);
-          // results
-          if (!(ok = warp_wait(bar, &bar->o2_full, n & 1))) break;
-          fence_after();
-          // through this warp's 4 KB of Q's tile (its products are done), 128 bytes a row:
-          // eight lanes then store a row's piece, instead of 32 rows at a time
-          const uint32_t stage = stage_of(n) + (warp - kFirstRow) * 4096;
-          constexpr int kParts = sizeof(TO) == 2 ? 1 : 2, kCols = 64 / kParts, kV = 16 / int(sizeof(TO));
-          const int piece = lane & 7, row0 = 32 * q + (lane >> 3);
-          TO* dst = reinterpret_cast<TO*>(C.out.p) + (w.first(C, i) + row0) * pitch + w.head / C.out_div * C.out.hs +
-                    h * 64 + piece * kV;
-#pragma unroll 1
-          for (int part = 0; part < 2; ++part) {
-            float x[32];
-            tmem_ld32(lanes + kColO + h * 64 + part * 32, x);
-            if (part == 1) {  // everything has been read
-              fence_before();
-              __syncwarp();
-              if (lane == 0) arrive(&bar->o_free);
-            }
-#pragma unroll
-            for (int j = 0; j < 32; j += kV) {
-              const uint32_t at = stage + lane * 128 + ((((part * 32 % kCols + j) / kV) ^ (lane & 7)) << 4);
-              if (sizeof(TO) == 2)
-                sts4(at, pack2(x[j], x[j + 1]), pack2(x[j + 2], x[j + 3]), pack2(x[j + 4], x[j + 5]),
-                     pack2(x[j + 6], x[j + 7]));
-              else
-                sts4(at, __float_as_uint(x[j]), __float_as_uint(x[j + 1]), __float_as_uint(x[j + 2]),
-                     __float_as_uint(x[j + 3]));
-            }
-            if (part == 1 || kParts == 2) {
-              __syncwarp();
-              const bool wide = h * 64 + (kParts == 2 ? part * 32 : 0) + piece * kV < C.dc;
-              TO* at = dst + (kParts == 2 ? part * 32 : 0);
-#pragma unroll 1
-              for (int k0 = 0; k0 < 8; k0 += 4) {
-                uint4 v[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const int row = 4 * (k0 + k) + (lane >> 3);
-                  v[k] = lds4(stage + row * 128 + ((piece ^ (row & 7)) << 4));
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k, at += 4 * pitch)
-                  if (wide && row0 + 4 * (k0 + k) < cnt) *reinterpret_cast<uint4*>(at) = v[k];
-              }
-              __syncwarp();
-            }
+          if (lane == 0) {
+            arrive(&bar->planes_ready);
+            arrive(&bar->empty[i % kStages]);
           }
-          fence_async();  // before the tile is loaded again
-          __syncwarp();
-          if (lane == 0) arrive(&bar->empty[n & 1]);
         }
+        // P[r][j] = intra Sc[r][j] l^|r - j| where j has been seen by r: blocks of 16
+        // columns, of which this warp's rows see all, a triangle, or nothing.  (Each block's
+        // P lands on columns of Sc that this warp has read by then.)
+        if (!(ok = warp_wait(bar, &bar->sc_full, turn))) break;
+        fence_after();
+#pragma unroll 1
+        for (int part = 0; part < 4; ++part) {
+          const int block = 4 * h + part, j0 = 16 * block;
+          uint32_t p[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[j] = 0;
+          const bool diagonal = block >> 1 == q;
+          if (diagonal || (block < 2 * q) != rev) {
+            float x[16];
+            tmem_ld16(lanes + kColS + j0, x);
+            if (diagonal) {
+#pragma unroll
+              for (int j8 = 0; j8 < 16; j8 += 8) {
+                float d[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) d[j] = lds(dec + 4 * abs(r - j0 - j8 - j));
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const int at = j0 + j8 + j;
+                  x[j8 + j] = (rev ? at >= r : at <= r) ? x[j8 + j] * (intra * d[j]) : 0.f;
+                }
+              }
+            } else {
+              const float top = intra * lds(dec + 4 * (rev ? j0 - r : r - j0 - 15));
+              const float2 b2 = make_float2(top, top);
+              const uint32_t col = dec + 4 * (rev ? 132 : 148);
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) {
+                const uint4 d = lds4(col + 4 * j);
+                const float2 y0 = __fmul2_rn(make_float2(x[j], x[j + 1]),
+                                             __fmul2_rn(b2, make_float2(__uint_as_float(d.x), __uint_as_float(d.y))));
+                const float2 y1 = __fmul2_rn(make_float2(x[j + 2], x[j + 3]),
+                                             __fmul2_rn(b2, make_float2(__uint_as_float(d.z), __uint_as_float(d.w))));
+                x[j] = y0.x;
+                x[j + 1] = y0.y;
+                x[j + 2] = y1.x;
+                x[j + 3] = y1.y;
+              }
+            }
+            if (cnt < kTile) {  // the columns of rows that are not this chunk's
+#pragma unroll
+              for (int j = 0; j < 16; ++j) x[j] = j0 + j < cnt ? x[j] : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) p[j >> 1] = pack2(x[j], x[j + 1]);
+          }
+          tmem_st8(lanes + kColS + h * 64 + part * 8, p);
+        }
+        // Q X, decayed from the chunk's beginning
+        const float f = inter * lds(dec + 4 * max(rev ? cnt - 1 - r : r + 1, 0));
+        if (!(ok = warp_wait(bar, &bar->o1_full, turn))) break;
+        fence_after();
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
+          float x[32];
+          tmem_ld32(lanes + kColO + h * 64 + part * 32, x);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) x[j] *= f;
+          tmem_st32(lanes + kColO + h * 64 + part * 32, x);
+        }
+        tmem_st_wait();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(&bar->p_ready);
+        // results
+        if (!(ok = warp_wait(bar, &bar->o2_full, turn))) break;
+        fence_after();
+        // through this warp's 4 KB of V's tile (its products are done), 128 bytes a row:
+        // eight lanes then store a row's piece, instead of 32 rows at a time
+        const uint32_t stage = stage_of(i) + R::kV + (warp - kFirstRow) * 4096;
+        constexpr int kParts = sizeof(TO) == 2 ? 1 : 2, kCols = 64 / kParts, kV = 16 / int(sizeof(TO));
+        const int piece = lane & 7, row0 = 32 * q + (lane >> 3);
+        TO* dst = reinterpret_cast<TO*>(C.out.p) + (w.first(C, i) + row0) * pitch + w.head / C.out_div * C.out.hs +
+                  h * 64 + piece * kV;
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
+          float x[32];
+          tmem_ld32(lanes + kColO + h * 64 + part * 32, x);
+          if (part == 1) {  // everything has been read
+            fence_before();
+            __syncwarp();
+            if (lane == 0) arrive(&bar->o_free);
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += kV) {
+            const uint32_t at = stage + lane * 128 + ((((part * 32 % kCols + j) / kV) ^ (lane & 7)) << 4);
+            if (sizeof(TO) == 2)
+              sts4(at, pack2(x[j], x[j + 1]), pack2(x[j + 2], x[j + 3]), pack2(x[j + 4], x[j + 5]),
+                   pack2(x[j + 6], x[j + 7]));
+            else
+              sts4(at, __float_as_uint(x[j]), __float_as_uint(x[j + 1]), __float_as_uint(x[j + 2]),
+                   __float_as_uint(x[j + 3]));
+          }
+          if (part == 1 || kParts == 2) {
+            __syncwarp();
+            const bool wide = h * 64 + (kParts == 2 ? part * 32 : 0) + piece * kV < C.dc;
+            TO* at = dst + (kParts == 2 ? part * 32 : 0);
+#pragma unroll 1
+            for (int k0 = 0; k0 < 8; k0 += 4) {
+              uint4 v[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int row = 4 * (k0 + k) + (lane >> 3);
+                v[k] = lds4(stage + row * 128 + ((piece ^ (row & 7)) << 4));
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k, at += 4 * pitch)
+                if (wide && row0 + 4 * (k0 + k) < cnt) *reinterpret_cast<uint4*>(at) = v[k];
+            }
+            __syncwarp();
+          }
+        }
+        fence_async();  // before the tile is loaded again
+        __syncwarp();
+        if (lane == 0) arrive(&bar->empty_v[i % kStages]);
       }
     }
   } else {
     registers_up<120>();
-    // ---- planes of decayed K, and the state: row b of X, columns [64 h, 64 h + 64).  Planes: the
-    // same rows of K^T (lanes of TMEM), tokens [64 h, 64 h + 64) ----
+    // ---- planes of decayed K (their lanes: the same rows of K^T), and the state: row b of
+    // X, columns [64 h, 64 h + 64) ----
     const int q = warp & 3, h = (warp - kFirstState) >> 2;
     const int b = q * 32 + lane, t = threadIdx.x - 32 * kFirstState;
     const uint32_t lanes = tmem + (uint32_t(q * 32) << 16);
-    const bool rev = C.rev != 0;
-    uint32_t n = 0, nu = 0, tables = 0;
-    bool ok = true;
-    auto write_x = [&](const float (&X)[64]) {
-      const uint32_t row = smem_u32(sm + kX) + h * kPanel + b * 128;
-#pragma unroll
-      for (int c = 0; c < 8; ++c)
-        sts4(row + ((c ^ (b & 7)) << 4), pack2(X[8 * c], X[8 * c + 1]), pack2(X[8 * c + 2], X[8 * c + 3]),
-             pack2(X[8 * c + 4], X[8 * c + 5]), pack2(X[8 * c + 6], X[8 * c + 7]));
-      fence_async();
-      __syncwarp();
-      if (lane == 0) arrive(&bar->x_ready);
-    };
-    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      if (!walk_of<STATES>(C, item, &w)) continue;
-      const float gl = lin::log_decay_of(C, w.head);
-      const uint32_t dec = make_table(bar, &bar->state_table, reinterpret_cast<float*>(sm + kStateTables), kStateTable,
-                                      tables++, t, &ok, [&](int e) { return expf(gl * static_cast<float>(e)); });
-      if (!ok) break;
-      float X[64];
+    float X[64];
+    {
       const float* src = nullptr;
       int src_t = 0;
       if (!STATES) {
         const long long slot = lin::state_slot(C, w.seq);
         if (!w.only) {
-          src = C.seg_state + static_cast<long long>(item) * C.db * C.dc;  // item = segment slot * heads + head
+          src = C.seg_state + static_cast<long long>(item) * C.db * C.dc;
         } else if (C.init && slot >= 0) {
           src = C.init + (slot * C.heads + w.head) * C.db * C.dc;
           src_t = C.init_t;
@@ -673,66 +690,89 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 64; ++c) X[c] = 0.f;
       }
-      for (int i = 0; i < w.n; ++i, ++n) {
-        const int cnt = w.rows(i);
-        const bool update = i < w.updates;
-        if (!(ok = warp_wait(bar, &bar->full[n & 1], (n / kStages) & 1))) break;
+    }
+    // chunk i of X = l^rows X + U
+    auto update = [&](int i) {
+      if (!(ok = warp_wait(bar, &bar->u_full, i & 1))) return;
+      fence_after();
+      const float keep = lds(dec + 4 * w.rows(i));
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        float x[32];
+        tmem_ld32(lanes + kColU<STATES> + h * 64 + part * 32, x);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) X[part * 32 + c] = fmaf(keep, X[part * 32 + c], x[c]);
+      }
+      fence_before();
+      __syncwarp();
+      if (STATES && lane == 0) arrive(&bar->u_free);
+    };
+    // one step past the last chunk, where its state is wanted
+    for (int i = 0; i <= w.updates || i < w.n; ++i) {
+      const bool chunk = i < w.n;
+      const int cnt = chunk ? w.rows(i) : 0;
+      if (chunk) {
+        if (!(ok = warp_wait(bar, &bar->full[i % kStages], turn_of(i)))) break;
         if (cnt < kTile) {
-          const uint32_t v = stage_of(n) + 2 * kTileBytes;
+          if (!(ok = warp_wait(bar, &bar->full_v[i % kStages], turn_of(i)))) break;
+          const uint32_t v = stage_of(i) + R::kV;
           for (int e = t; e < (kTile - cnt) * 16; e += 256)
             sts4(v + (e & 1) * kPanel + (cnt + (e >> 4)) * 128 + ((e >> 1) & 7) * 16, 0, 0, 0, 0);
           fence_async();
         }
-        if (!STATES) {  // once the product that read the last chunk's X is done; x_ready is V's too
-          if (n > 0 && !(ok = warp_wait(bar, &bar->o1_full, (n - 1) & 1))) break;
-          write_x(X);
-        }
-        if (update) {
-          make_planes<STATES, PLANES, STATES ? 0 : 1, PLANES>(stage_of(n) + kTileBytes, lanes, dec, cnt, rev, C.upd, q, h,
-                                                              lane);
-          fence_before();
-        }
+      }
+      if (!STATES && i > 0) {
+        update(i - 1);
+        if (!ok) break;
+      }
+      if (chunk && i < w.updates) {
+        constexpr int kG = STATES ? 2 : 4;
+        if (STATES && three)
+          make_planes<STATES, 0, STATES ? 3 : 2>(stage_of(i) + R::kK, lanes, i, dec_upd, cnt, rev, true, q, h, 0, kG, lane);
+        else
+          make_planes<STATES, 0, 2>(stage_of(i) + R::kK, lanes, i, dec_upd, cnt, rev, three, q, h, 0, kG, lane);
+        fence_before();
+      }
+      __syncwarp();
+      if (chunk && lane == 0) {
+        if (i < w.updates) arrive(&bar->planes_ready);
+        arrive(&bar->empty[i % kStages]);
+      }
+      if (STATES && i > 0) {
+        update(i - 1);
+        if (!ok) break;
+      }
+      if (!STATES && chunk) {  // once the product that read the last chunk's X is done
+        if (i > 0 && !(ok = warp_wait(bar, &bar->o1_full, (i - 1) & 1))) break;
+        const uint32_t row = base + kX + h * kPanel + b * 128;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          sts4(row + ((c ^ (b & 7)) << 4), pack2(X[8 * c], X[8 * c + 1]), pack2(X[8 * c + 2], X[8 * c + 3]),
+               pack2(X[8 * c + 4], X[8 * c + 5]), pack2(X[8 * c + 6], X[8 * c + 7]));
+        fence_async();
         __syncwarp();
-        if (lane == 0) {
-          arrive(&bar->planes_ready);
-          arrive(&bar->empty[n & 1]);
-        }
-        if (update) {
-          if (!(ok = warp_wait(bar, &bar->u_full, nu & 1))) break;
-          ++nu;
-          fence_after();
-          const float keep = lds(dec + 4 * cnt);
-#pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            float x[32];
-            tmem_ld32(lanes + kColU + h * 64 + part * 32, x);
-#pragma unroll
-            for (int c = 0; c < 32; ++c) X[part * 32 + c] = fmaf(keep, X[part * 32 + c], x[c]);
-          }
-          fence_before();  // (the next chunk's planes_ready says that U has been read)
-        }
+        if (lane == 0) arrive(&bar->x_ready);
       }
-      if (!ok) break;
-      float* dst = nullptr;
-      int dst_t = 0;
-      if (STATES) {
-        dst = C.seg_state + static_cast<long long>(item) * C.db * C.dc;
-      } else if (C.fin && w.last) {
-        const long long slot = lin::state_slot(C, w.seq);
-        if (slot >= 0) dst = C.fin + (slot * C.heads + w.head) * C.db * C.dc;
-        dst_t = C.fin_t;
-      }
-      if (dst && b < C.db) {
-        if (!dst_t && C.dc % 4 == 0) {
-          float4* p = reinterpret_cast<float4*>(dst + static_cast<long long>(b) * C.dc + h * 64);
+    }
+    float* dst = nullptr;
+    int dst_t = 0;
+    if (STATES) {
+      dst = C.seg_state + static_cast<long long>(item) * C.db * C.dc;
+    } else if (C.fin && w.last) {
+      const long long slot = lin::state_slot(C, w.seq);
+      if (slot >= 0) dst = C.fin + (slot * C.heads + w.head) * C.db * C.dc;
+      dst_t = C.fin_t;
+    }
+    if (ok && dst && b < C.db) {
+      if (!dst_t && C.dc % 4 == 0) {
+        float4* p = reinterpret_cast<float4*>(dst + static_cast<long long>(b) * C.dc + h * 64);
 #pragma unroll
-          for (int c = 0; c < 16; ++c)
-            if (h * 64 + 4 * c < C.dc) p[c] = make_float4(X[4 * c], X[4 * c + 1], X[4 * c + 2], X[4 * c + 3]);
-        } else {
+        for (int c = 0; c < 16; ++c)
+          if (h * 64 + 4 * c < C.dc) p[c] = make_float4(X[4 * c], X[4 * c + 1], X[4 * c + 2], X[4 * c + 3]);
+      } else {
 #pragma unroll
-          for (int c = 0; c < 64; ++c)
-            if (h * 64 + c < C.dc) dst[lin::state_index(C, dst_t, b, h * 64 + c)] = X[c];
-        }
+        for (int c = 0; c < 64; ++c)
+          if (h * 64 + c < C.dc) dst[lin::state_index(C, dst_t, b, h * 64 + c)] = X[c];
       }
     }
   }
@@ -765,19 +805,16 @@ bool rows_fit(const seq::Rows& r, int heads, long long tokens) {
          (tokens <= 1 || (r.ts % 8 == 0 && r.ts < most));
 }
 
-template <typename TO, bool STATES, int PLANES>
-int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const Chain& C, int sms,
-           cudaStream_t s) {
+template <typename TO, bool STATES>
+int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const Chain& C, cudaStream_t s) {
   static std::once_flag once;
   static cudaError_t attr = cudaSuccess;
   std::call_once(once, [] {
-    attr = cudaFuncSetAttribute(chain_tc_kernel<TO, STATES, PLANES>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                int(kSmem));
+    attr = cudaFuncSetAttribute(chain_tc_kernel<TO, STATES>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem));
   });
   TO_CUDA_TRY(attr);
   const int items = (C.seg_state ? lin::segment_slots(C.tokens, C.nseq, C.seg) : C.nseq) * C.heads;
-  chain_tc_kernel<TO, STATES, PLANES>
-      <<<unsigned(items), kThreads, kSmem, s>>>(a, b, c, C, items);
+  chain_tc_kernel<TO, STATES><<<unsigned(items), kThreads, kSmem, s>>>(a, b, c, C);
   TO_CUDA_TRY(cudaGetLastError());
   return ok();
 }
@@ -791,15 +828,8 @@ int run(const Chain& C, bool f32_out, cudaStream_t s) {
   if ((st = rows_map(enc, &a, C.a, C.heads / C.a_div, C.db, C.tokens))) return st;
   if ((st = rows_map(enc, &b, C.b, C.heads / C.b_div, C.db, C.tokens))) return st;
   if ((st = rows_map(enc, &c, C.c, C.heads / C.c_div, C.dc, C.tokens))) return st;
-  int dev = 0;
-  const int sms = device_sm_count(&dev);
-  if (sms <= 0) return -sms;
-  // three planes where the state itself is a result
-  if (STATES)
-    return C.fin ? launch<float, STATES, 3>(a, b, c, C, sms, s) : launch<float, STATES, 2>(a, b, c, C, sms, s);
-  if (f32_out) return C.fin ? launch<float, false, 3>(a, b, c, C, sms, s) : launch<float, false, 2>(a, b, c, C, sms, s);
-  return C.fin ? launch<__nv_bfloat16, false, 3>(a, b, c, C, sms, s)
-               : launch<__nv_bfloat16, false, 2>(a, b, c, C, sms, s);
+  if (STATES || f32_out) return launch<float, STATES>(a, b, c, C, s);
+  return launch<__nv_bfloat16, false>(a, b, c, C, s);
 }
 
 }  // namespace
