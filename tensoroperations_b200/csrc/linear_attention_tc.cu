@@ -21,9 +21,9 @@
 //
 // Roles (20 warps): one lane issues TMA loads, two chunks ahead, one the
 // products; warps 4-11 turn Sc into P, scale O and store the results (a thread:
-// one row, 64 columns); warps 12-19 make planes 0 and 1 and hold X (a thread: one
-// row, 64 columns).  Plane 2 lies in O's columns between one chunk's results
-// and the next one's, so the row warps make it.  Products are issued U, Q X,
+// one row, 64 columns); warps 12-19 make the planes and hold X (a thread: one row, 64
+// columns).  Plane 2 lies in O's columns between one chunk's results and the
+// next one's.  Products are issued U, Q X,
 // P V and the next chunk's Sc: the row warps store results and make the next P
 // while the state warps make the next planes.  In the states' launch there is
 // no Sc and no O: both groups make planes, into two buffers in turn.  Rows past
@@ -333,6 +333,58 @@ __device__ __forceinline__ void make_planes(uint32_t tile, uint32_t lanes, uint3
   tmem_st_wait();
 }
 
+// X of a warp (lane: a row, 64 columns from column `col` on) from or to rows row0 ..
+// of a [db][dc] matrix, dc a multiple of 4: through 2.5 KB of shared memory, 16
+// columns at a time, so that four lanes take 64 bytes of one row.  (32 lanes in 32
+// rows held up the load-store unit, and the other warps' shared loads behind it.)
+__device__ __forceinline__ void load_state(float (&X)[64], const float* m, uint32_t stage, int row0, int col, int db,
+                                           int dc, int lane) {
+  float4 v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int row = row0 + 8 * (i & 3) + (lane >> 2), c = col + 16 * (i >> 2) + 4 * (lane & 3);
+    v[i] = row < db && c < dc ? *reinterpret_cast<const float4*>(m + row * dc + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float4 x = v[4 * g + k];
+      sts4(stage + (8 * k + (lane >> 2)) * 80 + (lane & 3) * 16, __float_as_uint(x.x), __float_as_uint(x.y),
+           __float_as_uint(x.z), __float_as_uint(x.w));
+    }
+    __syncwarp();
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint4 x = lds4(stage + lane * 80 + 16 * e);
+      X[16 * g + 4 * e] = __uint_as_float(x.x);
+      X[16 * g + 4 * e + 1] = __uint_as_float(x.y);
+      X[16 * g + 4 * e + 2] = __uint_as_float(x.z);
+      X[16 * g + 4 * e + 3] = __uint_as_float(x.w);
+    }
+    __syncwarp();
+  }
+}
+
+__device__ __forceinline__ void store_state(const float (&X)[64], float* m, uint32_t stage, int row0, int col, int db,
+                                            int dc, int lane) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      sts4(stage + lane * 80 + 16 * e, __float_as_uint(X[16 * g + 4 * e]), __float_as_uint(X[16 * g + 4 * e + 1]),
+           __float_as_uint(X[16 * g + 4 * e + 2]), __float_as_uint(X[16 * g + 4 * e + 3]));
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int r = 8 * k + (lane >> 2), c = col + 16 * g + 4 * (lane & 3);
+      const uint4 x = lds4(stage + r * 80 + (lane & 3) * 16);
+      if (row0 + r < db && c < dc) *reinterpret_cast<uint4*>(m + (row0 + r) * dc + c) = x;
+    }
+    __syncwarp();
+  }
+}
+
 // Shared memory
 constexpr uint32_t kX = 6 * kTileBytes;  // bf16 X, behind the chunks
 constexpr uint32_t kTables = kX + kTileBytes;
@@ -360,6 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kStages = R::kStages;
   extern __shared__ __align__(1024) unsigned char sm[];
   const int item = blockIdx.x;  // segment slot * heads + head
+  const float gl = lin::log_decay_of(C, item % C.heads);
   Walk w;
   if (!walk_of<STATES>(C, item, &w)) return;
   const uint32_t base = smem_u32(sm);
@@ -379,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bar->full_v[i], 1);
       // Q and K are free when their products are done (a commit) and the planes made; V when
       // its products are done and the results, which pass through its tile, stored
-      mbar_init(&bar->empty[i], kStateWarps + (STATES ? kRowWarps : three ? kRowWarps + 1 : 1));
+      mbar_init(&bar->empty[i], kStateWarps + (STATES ? kRowWarps : 1));
       mbar_init(&bar->empty_v[i], STATES ? 1 : kRowWarps);
     }
     mbar_init(&bar->sc_full, 1);
@@ -387,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar->o1_full, 1);
     mbar_init(&bar->o2_full, 1);
     mbar_init(&bar->o_free, kRowWarps);
-    mbar_init(&bar->planes_ready, kStateWarps + (STATES || three ? kRowWarps : 0));
+    mbar_init(&bar->planes_ready, kStateWarps + (STATES ? kRowWarps : 0));
     mbar_init(&bar->u_full, 1);
     mbar_init(&bar->u_free, kStateWarps);
     mbar_init(&bar->x_ready, kStateWarps);
@@ -396,7 +449,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   {
     float* table = reinterpret_cast<float*>(sm + kTables);
-    const float gl = lin::log_decay_of(C, w.head);
     for (int t = threadIdx.x; t < kTable + kUpdTable; t += kThreads) {
       const int n = t < 132 ? t : t < kTable ? (rev ? t - 132 : 163 - t) : t - kTable;
       table[t] = expf(gl * static_cast<float>(n)) * (t < kTable ? 1.f : C.upd);
@@ -517,17 +569,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < w.n; ++i) {
         const int cnt = w.rows(i);
         const uint32_t turn = i & 1;
-        // plane 2 into this warp's part of O, which it has read
-        if (three && i < w.updates) {
-          if (!(ok = warp_wait(bar, &bar->full[i % kStages], turn_of(i)))) break;
-          make_planes<STATES, 2, 3>(stage_of(i) + R::kK, lanes, i, dec_upd, cnt, rev, true, q, h, 0, 4, lane);
-          fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            arrive(&bar->planes_ready);
-            arrive(&bar->empty[i % kStages]);
-          }
-        }
         // P[r][j] = intra Sc[r][j] l^|r - j| where j has been seen by r: blocks of 16
         // columns, of which this warp's rows see all, a triangle, or nothing.  (Each block's
         // P lands on columns of Sc that this warp has read by then.)
@@ -657,6 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int q = warp & 3, h = (warp - kFirstState) >> 2;
     const int b = q * 32 + lane, t = threadIdx.x - 32 * kFirstState;
     const uint32_t lanes = tmem + (uint32_t(q * 32) << 16);
+    const uint32_t own_x = base + kX + h * kPanel + q * 4096;  // the part of bf16 X that this warp writes
     float X[64];
     {
       const float* src = nullptr;
@@ -670,25 +712,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           src_t = C.init_t;
         }
       }
-      if (src && b < C.db) {
-        if (!src_t && C.dc % 4 == 0) {
-          const float4* p = reinterpret_cast<const float4*>(src + static_cast<long long>(b) * C.dc + h * 64);
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const float4 v = h * 64 + 4 * c < C.dc ? p[c] : make_float4(0.f, 0.f, 0.f, 0.f);
-            X[4 * c] = v.x;
-            X[4 * c + 1] = v.y;
-            X[4 * c + 2] = v.z;
-            X[4 * c + 3] = v.w;
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 64; ++c)
-            X[c] = h * 64 + c < C.dc ? src[lin::state_index(C, src_t, b, h * 64 + c)] : 0.f;
-        }
+      if (src && !src_t && C.dc % 4 == 0) {
+        load_state(X, src, own_x, 32 * q, 64 * h, C.db, C.dc, lane);
       } else {
 #pragma unroll
-        for (int c = 0; c < 64; ++c) X[c] = 0.f;
+        for (int c = 0; c < 64; ++c)
+          X[c] = src && b < C.db && h * 64 + c < C.dc ? src[lin::state_index(C, src_t, b, h * 64 + c)] : 0.f;
       }
     }
     // chunk i of X = l^rows X + U
@@ -731,6 +760,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           make_planes<STATES, 0, STATES ? 3 : 2>(stage_of(i) + R::kK, lanes, i, dec_upd, cnt, rev, true, q, h, 0, kG, lane);
         else
           make_planes<STATES, 0, 2>(stage_of(i) + R::kK, lanes, i, dec_upd, cnt, rev, three, q, h, 0, kG, lane);
+        if (!STATES && three) {  // plane 2, once the last results have been read from its columns
+          if (i > 0 && !(ok = warp_wait(bar, &bar->o_free, (i - 1) & 1))) break;
+          fence_after();
+          make_planes<STATES, 2, 3>(stage_of(i) + R::kK, lanes, i, dec_upd, cnt, rev, true, q, h, 0, kG, lane);
+        }
         fence_before();
       }
       __syncwarp();
@@ -744,7 +778,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!STATES && chunk) {  // once the product that read the last chunk's X is done
         if (i > 0 && !(ok = warp_wait(bar, &bar->o1_full, (i - 1) & 1))) break;
-        const uint32_t row = base + kX + h * kPanel + b * 128;
+        const uint32_t row = own_x + lane * 128;
 #pragma unroll
         for (int c = 0; c < 8; ++c)
           sts4(row + ((c ^ (b & 7)) << 4), pack2(X[8 * c], X[8 * c + 1]), pack2(X[8 * c + 2], X[8 * c + 3]),
@@ -763,13 +797,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (slot >= 0) dst = C.fin + (slot * C.heads + w.head) * C.db * C.dc;
       dst_t = C.fin_t;
     }
-    if (ok && dst && b < C.db) {
+    if (!STATES && ok && dst && w.n > 0) ok = warp_wait(bar, &bar->o1_full, (w.n - 1) & 1);  // bf16 X has been read
+    if (ok && dst) {
       if (!dst_t && C.dc % 4 == 0) {
-        float4* p = reinterpret_cast<float4*>(dst + static_cast<long long>(b) * C.dc + h * 64);
-#pragma unroll
-        for (int c = 0; c < 16; ++c)
-          if (h * 64 + 4 * c < C.dc) p[c] = make_float4(X[4 * c], X[4 * c + 1], X[4 * c + 2], X[4 * c + 3]);
-      } else {
+        store_state(X, dst, own_x, 32 * q, 64 * h, C.db, C.dc, lane);
+      } else if (b < C.db) {
 #pragma unroll
         for (int c = 0; c < 64; ++c)
           if (h * 64 + c < C.dc) dst[lin::state_index(C, dst_t, b, h * 64 + c)] = X[c];
