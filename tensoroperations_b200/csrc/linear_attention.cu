@@ -63,13 +63,15 @@ __device__ __forceinline__ void load_rows(float* dst, int ld, const Rows& r, int
   }
 }
 
-template <typename T, typename TO, int DCB, bool STATES>
-__global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_constant__ Chain C) {
+template <typename T, int DCB, bool STATES, int N>
+__global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_constant__ lin::Batch<N> batch) {
+  const Chain& C = batch.c[blockIdx.y % N];
   constexpr int kColPad = SimtShape<DCB>::kColPad;
   constexpr int VC = DCB / 16;  // columns of a thread
   const Segment g = lin::segment_of(C, blockIdx.x);
   if (g.idx < 0 || (STATES && g.idx == g.count - 1)) return;
-  const int head = blockIdx.z, col0 = blockIdx.y * DCB;
+  const int head = blockIdx.z, col0 = blockIdx.y / N * DCB;
+  if (col0 >= C.dc) return;
   const int dbp = (C.db + 3) & ~3, lda = dbp + 4;
   extern __shared__ __align__(16) float sm[];
   float* A = sm;
@@ -172,11 +174,16 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
       for (int r = 0; r < 4; ++r) {
         const int i = ty + 16 * r;
         if (i >= cnt) continue;
-        TO* dst = seq::row_ptr<TO>(C.out, row0 + static_cast<long long>(step) * i, head / C.out_div) + col0;
+        const long long token = row0 + static_cast<long long>(step) * i;
         const float f = C.inter * dec[i + 1 - C.rev];
 #pragma unroll
-        for (int c = 0; c < VC; ++c)
-          if (tx * VC + c < ncols) dst[tx * VC + c] = seq::from_f32<TO>(fmaf(f, w[r][c], o[r][c]));
+        for (int c = 0; c < VC; ++c) {
+          const int x = tx * VC + c;
+          const float v = fmaf(f, w[r][c], o[r][c]);
+          if (x >= ncols) continue;
+          if (C.out_f32) seq::row_ptr<float>(C.out, token, head / C.out_div)[col0 + x] = v;
+          else seq::row_ptr<T>(C.out, token, head / C.out_div)[col0 + x] = seq::from_f32<T>(v);
+        }
       }
       __syncthreads();  // X has been read
     }
@@ -240,13 +247,14 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
 // gets the X that enters it.  Sequences of one segment have nothing to scan.
 // A thread follows VEC values; the next kAhead segments are on their way while
 // one group is written, so a long sequence is not one memory latency a segment.
-template <int VEC>
-__global__ void __launch_bounds__(256) chain_scan_kernel(const __grid_constant__ Chain C) {
+template <int VEC, int N>
+__global__ void __launch_bounds__(256) chain_scan_kernel(const __grid_constant__ lin::Batch<N> batch) {
+  const Chain& C = batch.c[blockIdx.x % N];
   constexpr int kAhead = 8;
   const int s = blockIdx.z, head = blockIdx.y;
   const Segment g = lin::sequence_of(C, s);
   const int w0 = lin::first_slot(C, s);
-  const int n = C.db * C.dc, e = (blockIdx.x * 256 + threadIdx.x) * VEC;
+  const int n = C.db * C.dc, e = (blockIdx.x / N * 256 + threadIdx.x) * VEC;
   const int slots = lin::segment_slots(C.tokens, C.nseq, C.seg);
   const int count = min(g.count, slots - w0);
   if (count < 2 || e >= n) return;
@@ -277,17 +285,26 @@ __global__ void __launch_bounds__(256) chain_scan_kernel(const __grid_constant__
 }
 
 // ---- shared heads: sum the gradients of the heads of a group ---------------------------
+// blockIdx.y: dk or dv.
+struct GroupSum {
+  const float* part[2];
+  Rows out[2];
+  int width[2];
+  long long tokens;
+  int kv_heads, group;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(256) group_sum_kernel(const float* __restrict__ part, Rows out,
-                                                        long long tokens, int kv_heads, int group, int width) {
-  const long long per = static_cast<long long>(kv_heads) * width, total = tokens * per;
+__global__ void __launch_bounds__(256) group_sum_kernel(const __grid_constant__ GroupSum G) {
+  const int y = blockIdx.y, width = G.width[y];
+  const long long per = static_cast<long long>(G.kv_heads) * width, total = G.tokens * per;
   for (long long e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
     const long long t = e / per;
     const int r = static_cast<int>(e - t * per), h = r / width, x = r - h * width;
-    const float* p = part + ((t * kv_heads + h) * group) * width + x;
+    const float* p = G.part[y] + ((t * G.kv_heads + h) * G.group) * width + x;
     float v = 0.f;
-    for (int i = 0; i < group; ++i) v += p[static_cast<long long>(i) * width];
-    seq::row_ptr<T>(out, t, h)[x] = seq::from_f32<T>(v);
+    for (int i = 0; i < G.group; ++i) v += p[static_cast<long long>(i) * width];
+    seq::row_ptr<T>(G.out[y], t, h)[x] = seq::from_f32<T>(v);
   }
 }
 
@@ -413,10 +430,12 @@ int check_list(const char* who, const char* name, const void* p, bool need) {
 // leave shared memory for two an SM.
 constexpr int kOneSegment = 1 << 30;
 
-int plan_segment(const to_linear_attention_desc& d, bool tc, int db, int dc) {
+int plan_segment(const to_linear_attention_desc& d, bool tc, int chains) {
+  const int db = chains > 1 ? std::max(d.key_dim, d.value_dim) : d.key_dim;
+  const int dc = chains > 1 ? db : d.value_dim;
   const long long chunk = tc ? 128 : kRows, states = tc ? 2 : 1, begin = tc ? 3 : 2;
   const long long at_once = 148 * (!tc && db <= 64 ? 2 : 1);
-  const long long blocks = tc ? 1 : db <= 128 ? (dc + 63) / 64 : (dc + 31) / 32;
+  const long long blocks = chains * (tc ? 1ll : db <= 128 ? (dc + 63) / 64 : (dc + 31) / 32);
   const long long chunks = (d.tokens + chunk - 1) / chunk, pairs = d.nseq * blocks * d.q_heads;
   if (chunks <= 2 || pairs == 0) return kOneSegment;
   const long long mean = std::max(1ll, (chunks + d.nseq - 1) / d.nseq);
@@ -437,85 +456,103 @@ int plan_segment(const to_linear_attention_desc& d, bool tc, int db, int dc) {
 constexpr size_t kAlign = 256;
 size_t rounded(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
-// Bytes of the segments' states of a chain of these widths, on either kind of cores.
-size_t state_bytes(const to_linear_attention_desc& d, int db, int dc) {
+// Bytes of the segments' states of one of `chains` chains, on either kind of cores.
+size_t state_bytes(const to_linear_attention_desc& d, int chains) {
   size_t most = 0;
   for (const bool tc : {false, true}) {
-    const int seg = plan_segment(d, tc, db, dc);
+    const int seg = plan_segment(d, tc, chains);
     if (seg == kOneSegment || (tc && d.dtype == TO_F32)) continue;
     const size_t slots = size_t(lin::segment_slots(static_cast<int>(d.tokens), d.nseq, seg));
-    most = std::max(most, rounded(slots * d.q_heads * db * dc * 4));
+    most = std::max(most, rounded(slots * d.q_heads * d.key_dim * d.value_dim * 4));
   }
   return most;
 }
-size_t state_bytes(const to_linear_attention_desc& d) { return state_bytes(d, d.key_dim, d.value_dim); }
-// The backward pass runs chains of (key, value) and of (value, key) widths.
-size_t backward_state_bytes(const to_linear_attention_desc& d) {
-  return std::max(state_bytes(d), state_bytes(d, d.value_dim, d.key_dim));
+
+// f32 gradients of every query head, before the heads of a group are summed.
+size_t part_bytes(const to_linear_attention_desc& d, int width) {
+  return d.q_heads == d.kv_heads ? 0 : rounded(size_t(d.tokens) * d.q_heads * width * 4);
 }
 
-template <typename T, typename TO, int DCB, bool STATES>
-int launch_simt(const Chain& C, cudaStream_t s) {
+template <typename T, int DCB, bool STATES, int N>
+int launch_simt(const lin::Batch<N>& B, cudaStream_t s) {
   static std::once_flag once;
   static cudaError_t attr = cudaSuccess;
   const size_t most = SimtShape<DCB>::bytes(DCB == 64 ? 128 : 256);
   std::call_once(once, [&] {
-    attr = cudaFuncSetAttribute(chain_simt_kernel<T, TO, DCB, STATES>,
-                                cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+    attr = cudaFuncSetAttribute(chain_simt_kernel<T, DCB, STATES, N>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                static_cast<int>(most));
   });
   TO_CUDA_TRY(attr);
+  const Chain& C = B.c[0];
+  int db = 0, dc = 0;
+  for (const Chain& x : B.c) db = std::max(db, x.db), dc = std::max(dc, x.dc);
   const int slots = C.seg_state ? lin::segment_slots(C.tokens, C.nseq, C.seg) : C.nseq;
-  const dim3 grid(static_cast<unsigned>(slots), (C.dc + DCB - 1) / DCB, C.heads);
-  chain_simt_kernel<T, TO, DCB, STATES><<<grid, kThreads, SimtShape<DCB>::bytes((C.db + 3) & ~3), s>>>(C);
+  const dim3 grid(static_cast<unsigned>(slots), (dc + DCB - 1) / DCB * N, C.heads);
+  chain_simt_kernel<T, DCB, STATES, N><<<grid, kThreads, SimtShape<DCB>::bytes((db + 3) & ~3), s>>>(B);
   TO_CUDA_TRY(cudaGetLastError());
   return ok();
 }
 
-template <typename T, typename TO, bool STATES>
-int launch_simt(const Chain& C, cudaStream_t s) {
+template <typename T, bool STATES, int N>
+int launch_width(const lin::Batch<N>& B, cudaStream_t s) {
   // wider b takes narrower columns: both operands and X share 227 KB
-  return C.db <= 128 ? launch_simt<T, TO, 64, STATES>(C, s) : launch_simt<T, TO, 32, STATES>(C, s);
+  for (const Chain& C : B.c)
+    if (C.db > 128) return launch_simt<T, 32, STATES, N>(B, s);
+  return launch_simt<T, 64, STATES, N>(B, s);
 }
 
-int launch_scan(const Chain& C, cudaStream_t s) {
+template <int N>
+int launch_scan(const lin::Batch<N>& B, cudaStream_t s) {
+  const Chain& C = B.c[0];  // (db dc is the same for all)
   const int n = C.db * C.dc;
-  const dim3 grid(n % 4 ? (n + 255) / 256 : (n / 4 + 255) / 256, C.heads, C.nseq);
-  if (n % 4) chain_scan_kernel<1><<<grid, 256, 0, s>>>(C);
-  else chain_scan_kernel<4><<<grid, 256, 0, s>>>(C);
+  const dim3 grid((n % 4 ? (n + 255) / 256 : (n / 4 + 255) / 256) * N, C.heads, C.nseq);
+  if (n % 4) chain_scan_kernel<1, N><<<grid, 256, 0, s>>>(B);
+  else chain_scan_kernel<4, N><<<grid, 256, 0, s>>>(B);
   TO_CUDA_TRY(cudaGetLastError());
   return ok();
 }
 
-template <typename T, typename TO>
-int run_simt(const Chain& C, cudaStream_t s) {
-  if (C.seg_state) {
-    if (int st = launch_simt<T, TO, true>(C, s)) return st;
-    if (int st = launch_scan(C, s)) return st;
+template <typename T, int N>
+int run_simt(const lin::Batch<N>& B, cudaStream_t s) {
+  if (B.c[0].seg_state) {
+    if (int st = launch_width<T, true, N>(B, s)) return st;
+    if (int st = launch_scan<N>(B, s)) return st;
   }
-  return launch_simt<T, TO, false>(C, s);
+  return launch_width<T, false, N>(B, s);
 }
 
-// `states`: workspace for the segments' states.
-int run_chain(Chain C, const to_linear_attention_desc& d, bool f32_out, void* states, cudaStream_t s) {
+// `states`: workspace for the segments' states, state_bytes(d, N) for each chain.
+template <int N>
+int run_chains(lin::Batch<N>& B, const to_linear_attention_desc& d, void* states, cudaStream_t s) {
   auto cut = [&](bool tc) {
-    C.seg = plan_segment(d, tc, C.db, C.dc);
-    C.seg_state = C.seg == kOneSegment ? nullptr : static_cast<float*>(states);
-  };
-  cut(true);
-  if (d.dtype == TO_BF16 && lin::tc_takes(C, f32_out)) {
-    if (C.seg_state) {
-      if (int st = lin::tc_states(C, s)) return st;
-      if (int st = launch_scan(C, s)) return st;
+    const int seg = plan_segment(d, tc, N);
+    const size_t each = state_bytes(d, N);
+    for (int n = 0; n < N; ++n) {
+      B.c[n].seg = seg;
+      B.c[n].seg_state =
+          seg == kOneSegment ? nullptr : reinterpret_cast<float*>(static_cast<char*>(states) + n * each);
     }
-    return lin::tc_outputs(C, f32_out, s);
+  };
+  if (d.dtype == TO_BF16) {
+    cut(true);
+    bool all = true;
+    for (const Chain& C : B.c) all = all && lin::tc_takes(C);
+    if (all) {
+      if (B.c[0].seg_state) {
+        if (int st = lin::tc_states<N>(B, s)) return st;
+        if (int st = launch_scan<N>(B, s)) return st;
+      }
+      return lin::tc_outputs<N>(B, s);
+    }
   }
   cut(false);
-  const Rows* rows[3] = {&C.a, &C.b, &C.c};
   const int bytes = 4 * seq::dtype_bytes(d.dtype);
-  for (int i = 0; i < 3; ++i)
-    if (aligned(rows[i]->p, size_t(bytes)) && rows[i]->ts % 4 == 0 && rows[i]->hs % 4 == 0) C.vec |= 1 << i;
-  if (d.dtype == TO_F32) return run_simt<float, float>(C, s);
-  return f32_out ? run_simt<__nv_bfloat16, float>(C, s) : run_simt<__nv_bfloat16, __nv_bfloat16>(C, s);
+  for (Chain& C : B.c) {
+    const Rows* rows[3] = {&C.a, &C.b, &C.c};
+    for (int i = 0; i < 3; ++i)
+      if (aligned(rows[i]->p, size_t(bytes)) && rows[i]->ts % 4 == 0 && rows[i]->hs % 4 == 0) C.vec |= 1 << i;
+  }
+  return d.dtype == TO_F32 ? run_simt<float, N>(B, s) : run_simt<__nv_bfloat16, N>(B, s);
 }
 
 Chain base_chain(const to_linear_attention_desc& d, const int32_t* cu, const float* log_decay) {
@@ -529,15 +566,6 @@ Chain base_chain(const to_linear_attention_desc& d, const int32_t* cu, const flo
   return C;
 }
 
-template <typename T>
-int group_sum(const float* part, const to_rows& out, const to_linear_attention_desc& d, int width, cudaStream_t s) {
-  const long long total = d.tokens * d.kv_heads * width, want = (total + 255) / 256;
-  group_sum_kernel<T><<<static_cast<unsigned>(std::min(want, 148ll * 16)), 256, 0, s>>>(
-      part, seq::rows_of(out), d.tokens, d.kv_heads, d.q_heads / d.kv_heads, width);
-  TO_CUDA_TRY(cudaGetLastError());
-  return ok();
-}
-
 }  // namespace
 }  // namespace to_b200
 
@@ -547,16 +575,13 @@ extern "C" {
 
 size_t to_linear_attention_workspace_bytes(const to_linear_attention_desc* desc) {
   if (check_desc("to_linear_attention_workspace_bytes", desc)) return 0;
-  return state_bytes(*desc);
+  return state_bytes(*desc, 1);
 }
 
 size_t to_linear_attention_backward_workspace_bytes(const to_linear_attention_desc* desc) {
   if (check_desc("to_linear_attention_backward_workspace_bytes", desc)) return 0;
   const to_linear_attention_desc& d = *desc;
-  size_t n = backward_state_bytes(d);
-  if (d.q_heads != d.kv_heads)  // f32 gradients of each query head, before the heads of a group are summed
-    n += rounded(size_t(d.tokens) * d.q_heads * std::max(d.key_dim, d.value_dim) * 4);
-  return n;
+  return 3 * state_bytes(d, 3) + part_bytes(d, d.key_dim) + part_bytes(d, d.value_dim);
 }
 
 int to_linear_attention(const to_linear_attention_desc* desc, const to_linear_attention_args* args,
@@ -577,13 +602,14 @@ int to_linear_attention(const to_linear_attention_desc* desc, const to_linear_at
   if (!st) st = check_state(who, "state_in", a.state_in);
   if (!st) st = check_state(who, "state_out", a.state_out);
   if (st) return st;
-  const size_t need = state_bytes(d);
+  const size_t need = state_bytes(d, 1);
   if (need && (!a.workspace || a.workspace_bytes < need))
     return set_error(TO_ERR_INVALID_ARGUMENT, "%s: workspace %zu < %zu bytes", who,
                      a.workspace ? a.workspace_bytes : 0, need);
   if (need && !aligned(a.workspace, kAlign))
     return set_error(TO_ERR_ALIGNMENT, "%s: workspace is not 256-byte aligned", who);
-  Chain C = base_chain(d, a.cu_seqlens, a.log_decay);
+  lin::Batch<1> B{{base_chain(d, a.cu_seqlens, a.log_decay)}};
+  Chain& C = B.c[0];
   C.a = seq::rows_of(a.q);
   C.b = seq::rows_of(a.k);
   C.c = seq::rows_of(a.v);
@@ -597,7 +623,7 @@ int to_linear_attention(const to_linear_attention_desc* desc, const to_linear_at
   C.fin = a.state_out;
   C.slots = a.slots;
   C.num_slots = d.num_slots;
-  return run_chain(C, d, false, a.workspace, static_cast<cudaStream_t>(stream));
+  return run_chains<1>(B, d, a.workspace, static_cast<cudaStream_t>(stream));
 }
 
 int to_linear_attention_backward(const to_linear_attention_desc* desc,
@@ -632,60 +658,66 @@ int to_linear_attention_backward(const to_linear_attention_desc* desc,
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int group = d.q_heads / d.kv_heads;
   const float scale = static_cast<float>(d.scale);
-  Chain C = base_chain(d, a.cu_seqlens, a.log_decay);
-  // dq: forwards, a = do, b = v, c = k
-  C.a = seq::rows_of(a.d_o);
-  C.b = seq::rows_of(a.v);
-  C.c = seq::rows_of(a.k);
-  C.out = seq::rows_of(a.dq);
-  C.b_div = C.c_div = group;
-  C.db = d.value_dim;
-  C.dc = d.key_dim;
-  C.intra = C.inter = scale;
-  C.upd = 1.f;
-  C.init = a.state_in;
-  C.init_t = 1;
-  if ((st = run_chain(C, d, false, a.workspace, s))) return st;
-  // backwards; the gradients of shared heads go through f32 partial rows
-  float* part = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + backward_state_bytes(d));
-  auto target = [&](const to_rows& r, int width) {
-    if (group == 1) return seq::rows_of(r);
-    return Rows{reinterpret_cast<char*>(part), static_cast<long long>(d.q_heads) * width, width};
+  // the gradients of shared heads go through f32 rows of every query head
+  char* part = static_cast<char*>(a.workspace) + 3 * state_bytes(d, 3);
+  float* parts[2] = {reinterpret_cast<float*>(part), reinterpret_cast<float*>(part + part_bytes(d, d.key_dim))};
+  auto target = [&](Chain& C, const to_rows& r, int n, int width) {
+    C.out_f32 = group > 1;
+    C.out = group == 1 ? seq::rows_of(r)
+                       : Rows{reinterpret_cast<char*>(parts[n]), static_cast<long long>(d.q_heads) * width, width};
   };
-  C.rev = 1;
-  C.intra = scale;
-  C.inter = 1.f;
-  C.upd = scale;
-  C.init = a.dstate_out;
-  // dk: a = v, b = do, c = q
-  C.a = seq::rows_of(a.v);
-  C.b = seq::rows_of(a.d_o);
-  C.c = seq::rows_of(a.q);
-  C.out = target(a.dk, d.key_dim);
-  C.a_div = group;
-  C.b_div = C.c_div = 1;
-  C.db = d.value_dim;
-  C.dc = d.key_dim;
-  C.init_t = 1;
-  if ((st = run_chain(C, d, group > 1, a.workspace, s))) return st;
-  if (group > 1) {
-    st = d.dtype == TO_BF16 ? group_sum<__nv_bfloat16>(part, a.dk, d, d.key_dim, s)
-                            : group_sum<float>(part, a.dk, d, d.key_dim, s);
-    if (st) return st;
-  }
-  // dv: a = k, b = q, c = do
-  C.a = seq::rows_of(a.k);
-  C.b = seq::rows_of(a.q);
-  C.c = seq::rows_of(a.d_o);
-  C.out = target(a.dv, d.value_dim);
-  C.db = d.key_dim;
-  C.dc = d.value_dim;
-  C.init_t = 0;
-  C.fin = a.dstate_in;
-  if ((st = run_chain(C, d, group > 1, a.workspace, s))) return st;
-  if (group > 1)
-    return d.dtype == TO_BF16 ? group_sum<__nv_bfloat16>(part, a.dv, d, d.value_dim, s)
-                              : group_sum<float>(part, a.dv, d, d.value_dim, s);
+  const Chain base = base_chain(d, a.cu_seqlens, a.log_decay);
+  lin::Batch<3> B{{base, base, base}};
+  // dq: forwards, a = do, b = v, c = k
+  Chain& dq = B.c[0];
+  dq.a = seq::rows_of(a.d_o);
+  dq.b = seq::rows_of(a.v);
+  dq.c = seq::rows_of(a.k);
+  dq.out = seq::rows_of(a.dq);
+  dq.b_div = dq.c_div = group;
+  dq.db = d.value_dim;
+  dq.dc = d.key_dim;
+  dq.intra = dq.inter = scale;
+  dq.upd = 1.f;
+  dq.init = a.state_in;
+  dq.init_t = 1;
+  // dk: backwards, a = v, b = do, c = q
+  Chain& dk = B.c[1];
+  dk.a = seq::rows_of(a.v);
+  dk.b = seq::rows_of(a.d_o);
+  dk.c = seq::rows_of(a.q);
+  target(dk, a.dk, 0, d.key_dim);
+  dk.a_div = group;
+  dk.db = d.value_dim;
+  dk.dc = d.key_dim;
+  dk.rev = 1;
+  dk.intra = dk.upd = scale;
+  dk.inter = 1.f;
+  dk.init = a.dstate_out;
+  dk.init_t = 1;
+  // dv: backwards, a = k, b = q, c = do
+  Chain& dv = B.c[2];
+  dv.a = seq::rows_of(a.k);
+  dv.b = seq::rows_of(a.q);
+  dv.c = seq::rows_of(a.d_o);
+  target(dv, a.dv, 1, d.value_dim);
+  dv.a_div = group;
+  dv.db = d.key_dim;
+  dv.dc = d.value_dim;
+  dv.rev = 1;
+  dv.intra = dv.upd = scale;
+  dv.inter = 1.f;
+  dv.init = a.dstate_out;
+  dv.fin = a.dstate_in;
+  if ((st = run_chains<3>(B, d, a.workspace, s))) return st;
+  if (group == 1 || d.tokens == 0) return ok();
+  GroupSum G{{parts[0], parts[1]}, {seq::rows_of(a.dk), seq::rows_of(a.dv)}, {d.key_dim, d.value_dim},
+             d.tokens, d.kv_heads, group};
+  const long long want = (d.tokens * d.kv_heads * std::max(d.key_dim, d.value_dim) + 255) / 256;
+  const dim3 grid(static_cast<unsigned>(std::min(want, 148ll * 16)), 2);
+  if (d.dtype == TO_BF16) group_sum_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(G);
+  else group_sum_kernel<float><<<grid, 256, 0, s>>>(G);
+  TO_CUDA_TRY(cudaGetLastError());
   return ok();
 }
 

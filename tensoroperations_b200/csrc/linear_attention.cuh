@@ -49,6 +49,14 @@ struct Chain {
   float* seg_state;  // [segment slots][heads][db][dc]; null: one segment a sequence
   int seg;           // tokens of a segment
   int vec;           // bits 0, 1, 2: rows of a, b, c can be read four values at a time
+  int out_f32;       // out is f32, not of the rows' type
+};
+
+// The chains of one call, run by the same launches: one forwards, three for the
+// gradients.  Sequences and segments are the same for all.
+template <int N>
+struct Batch {
+  Chain c[N];
 };
 
 // Where a segment lies.  idx < 0: an unused slot.
@@ -113,11 +121,13 @@ __device__ __forceinline__ long long state_index(const Chain& C, int transposed,
   return transposed ? static_cast<long long>(c) * C.db + b : static_cast<long long>(b) * C.dc + c;
 }
 
-// The tensor-core form (linear_attention_tc.cu): whether it takes the chain's
-// rows, every segment's own X, and the outputs.
-bool tc_takes(const Chain& C, bool f32_out);
-int tc_states(const Chain& C, cudaStream_t s);
-int tc_outputs(const Chain& C, bool f32_out, cudaStream_t s);
+// The tensor-core form (linear_attention_tc.cu): whether it takes a chain's
+// rows, every segment's own X, and the outputs, N = 1 or 3.
+bool tc_takes(const Chain& C);
+template <int N>
+int tc_states(const Batch<N>& B, cudaStream_t s);
+template <int N>
+int tc_outputs(const Batch<N>& B, cudaStream_t s);
 
 }  // namespace lin
 }  // namespace to_b200

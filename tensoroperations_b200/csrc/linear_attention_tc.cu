@@ -404,10 +404,16 @@ __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.
 template <int N>
 __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
-template <typename TO, bool STATES>
+template <int N>
+struct Maps {
+  CUtensorMap m[N][3];  // rows of a, b, c
+};
+
+template <bool STATES, int N>
 __global__ void __launch_bounds__(kThreads, 1)
-    chain_tc_kernel(const __grid_constant__ CUtensorMap mapA, const __grid_constant__ CUtensorMap mapB,
-                    const __grid_constant__ CUtensorMap mapC, const __grid_constant__ Chain C) {
+    chain_tc_kernel(const __grid_constant__ Maps<N> maps, const __grid_constant__ lin::Batch<N> batch) {
+  const Chain& C = batch.c[N == 1 ? 0 : blockIdx.y];
+  const CUtensorMap* map = maps.m[N == 1 ? 0 : blockIdx.y];
   using R = Ring<STATES>;
   constexpr int kStages = R::kStages;
   extern __shared__ __align__(1024) unsigned char sm[];
@@ -477,12 +483,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint64_t *full = &bar->full[i % kStages], *full_v = &bar->full_v[i % kStages];
         if (i >= kStages && !(ok = wait_for(bar, &bar->empty[i % kStages], turn_of(i - kStages)))) break;
         mbar_arrive_expect_tx(full, R::kV);
-        if (!STATES) tma_tile(stage_of(i), &mapA, w.head / C.a_div, token, full);
-        tma_tile(stage_of(i) + R::kK, &mapB, w.head / C.b_div, token, full);
+        if (!STATES) tma_tile(stage_of(i), map, w.head / C.a_div, token, full);
+        tma_tile(stage_of(i) + R::kK, map + 1, w.head / C.b_div, token, full);
         qk = i + 1;
         if (i >= kStages && !(ok = wait_for(bar, &bar->empty_v[i % kStages], turn_of(i - kStages)))) break;
         mbar_arrive_expect_tx(full_v, kTileBytes);
-        tma_tile(stage_of(i) + R::kV, &mapC, w.head / C.c_div, token, full_v);
+        tma_tile(stage_of(i) + R::kV, map + 2, w.head / C.c_div, token, full_v);
       }
       // copies still in flight land before the CTA ends
       for (int t = qk > kStages ? qk - kStages : 0; t < qk; ++t) {
@@ -644,10 +650,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         // through this warp's 4 KB of V's tile (its products are done), 128 bytes a row:
         // eight lanes then store a row's piece, instead of 32 rows at a time
         const uint32_t stage = stage_of(i) + R::kV + (warp - kFirstRow) * 4096;
-        constexpr int kParts = sizeof(TO) == 2 ? 1 : 2, kCols = 64 / kParts, kV = 16 / int(sizeof(TO));
         const int piece = lane & 7, row0 = 32 * q + (lane >> 3);
-        TO* dst = reinterpret_cast<TO*>(C.out.p) + (w.first(C, i) + row0) * pitch + w.head / C.out_div * C.out.hs +
-                  h * 64 + piece * kV;
+        const long long first = (w.first(C, i) + row0) * pitch + w.head / C.out_div * C.out.hs + h * 64;
+        const bool f32 = C.out_f32;
 #pragma unroll 1
         for (int part = 0; part < 2; ++part) {
           float x[32];
@@ -657,20 +662,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) arrive(&bar->o_free);
           }
+          if (f32) {
 #pragma unroll
-          for (int j = 0; j < 32; j += kV) {
-            const uint32_t at = stage + lane * 128 + ((((part * 32 % kCols + j) / kV) ^ (lane & 7)) << 4);
-            if (sizeof(TO) == 2)
-              sts4(at, pack2(x[j], x[j + 1]), pack2(x[j + 2], x[j + 3]), pack2(x[j + 4], x[j + 5]),
-                   pack2(x[j + 6], x[j + 7]));
-            else
-              sts4(at, __float_as_uint(x[j]), __float_as_uint(x[j + 1]), __float_as_uint(x[j + 2]),
-                   __float_as_uint(x[j + 3]));
+            for (int j = 0; j < 32; j += 4)
+              sts4(stage + lane * 128 + (((j / 4) ^ (lane & 7)) << 4), __float_as_uint(x[j]), __float_as_uint(x[j + 1]),
+                   __float_as_uint(x[j + 2]), __float_as_uint(x[j + 3]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              sts4(stage + lane * 128 + (((part * 4 + j / 8) ^ (lane & 7)) << 4), pack2(x[j], x[j + 1]),
+                   pack2(x[j + 2], x[j + 3]), pack2(x[j + 4], x[j + 5]), pack2(x[j + 6], x[j + 7]));
           }
-          if (part == 1 || kParts == 2) {
+          if (part == 1 || f32) {
             __syncwarp();
-            const bool wide = h * 64 + (kParts == 2 ? part * 32 : 0) + piece * kV < C.dc;
-            TO* at = dst + (kParts == 2 ? part * 32 : 0);
+            const int col = f32 ? part * 32 + piece * 4 : piece * 8, bytes = f32 ? 4 : 2;
+            const bool wide = h * 64 + col < C.dc;
+            char* at = C.out.p + (first + col) * bytes;
 #pragma unroll 1
             for (int k0 = 0; k0 < 8; k0 += 4) {
               uint4 v[4];
@@ -680,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 v[k] = lds4(stage + row * 128 + ((piece ^ (row & 7)) << 4));
               }
 #pragma unroll
-              for (int k = 0; k < 4; ++k, at += 4 * pitch)
+              for (int k = 0; k < 4; ++k, at += 4 * pitch * bytes)
                 if (wide && row0 + 4 * (k0 + k) < cnt) *reinterpret_cast<uint4*>(at) = v[k];
             }
             __syncwarp();
@@ -831,37 +838,40 @@ int rows_map(EncodeTiled enc, CUtensorMap* m, const seq::Rows& r, int heads, int
   return ok();
 }
 
+long long items_of(const Chain& C) {
+  return (C.seg_state ? lin::segment_slots(C.tokens, C.nseq, C.seg) : C.nseq) * 1ll * C.heads;
+}
+
 bool rows_fit(const seq::Rows& r, int heads, long long tokens) {
   const long long most = 1ll << 38;  // bytes of a stride: below the map's 2^40
   return aligned(r.p, 16) && (heads <= 1 || (r.hs % 8 == 0 && r.hs < most)) &&
          (tokens <= 1 || (r.ts % 8 == 0 && r.ts < most));
 }
 
-template <typename TO, bool STATES>
-int launch(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& c, const Chain& C, cudaStream_t s) {
+template <bool STATES, int N>
+int run(const lin::Batch<N>& B, cudaStream_t s) {
   static std::once_flag once;
   static cudaError_t attr = cudaSuccess;
   std::call_once(once, [] {
-    attr = cudaFuncSetAttribute(chain_tc_kernel<TO, STATES>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem));
+    attr = cudaFuncSetAttribute(chain_tc_kernel<STATES, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem));
   });
   TO_CUDA_TRY(attr);
-  const int items = (C.seg_state ? lin::segment_slots(C.tokens, C.nseq, C.seg) : C.nseq) * C.heads;
-  chain_tc_kernel<TO, STATES><<<unsigned(items), kThreads, kSmem, s>>>(a, b, c, C);
-  TO_CUDA_TRY(cudaGetLastError());
-  return ok();
-}
-
-template <bool STATES>
-int run(const Chain& C, bool f32_out, cudaStream_t s) {
   int st = TO_OK;
   EncodeTiled enc = tensor_map_encoder(&st);
   if (!enc) return st;
-  CUtensorMap a, b, c;
-  if ((st = rows_map(enc, &a, C.a, C.heads / C.a_div, C.db, C.tokens))) return st;
-  if ((st = rows_map(enc, &b, C.b, C.heads / C.b_div, C.db, C.tokens))) return st;
-  if ((st = rows_map(enc, &c, C.c, C.heads / C.c_div, C.dc, C.tokens))) return st;
-  if (STATES || f32_out) return launch<float, STATES>(a, b, c, C, s);
-  return launch<__nv_bfloat16, false>(a, b, c, C, s);
+  Maps<N> maps;
+  for (int n = 0; n < N; ++n) {
+    const Chain& C = B.c[n];
+    CUtensorMap* m = maps.m[n];
+    if ((st = rows_map(enc, &m[1], C.b, C.heads / C.b_div, C.db, C.tokens))) return st;
+    if ((st = rows_map(enc, &m[2], C.c, C.heads / C.c_div, C.dc, C.tokens))) return st;
+    m[0] = m[1];  // (not used by the states' launch)
+    if (!STATES && (st = rows_map(enc, &m[0], C.a, C.heads / C.a_div, C.db, C.tokens))) return st;
+  }
+  const dim3 grid(unsigned(items_of(B.c[0])), N);
+  chain_tc_kernel<STATES, N><<<grid, kThreads, kSmem, s>>>(maps, B);
+  TO_CUDA_TRY(cudaGetLastError());
+  return ok();
 }
 
 }  // namespace
@@ -870,16 +880,22 @@ namespace lin {
 
 // bf16 rows of at most 128 values whose addresses TMA takes (16-byte rows) and
 // whose results can be stored 16 bytes at a time.
-bool tc_takes(const Chain& C, bool f32_out) {
-  const int per = f32_out ? 4 : 8;
-  const long long items = (C.seg_state ? lin::segment_slots(C.tokens, C.nseq, C.seg) : C.nseq) * 1ll * C.heads;
-  return C.tokens > 0 && items < INT32_MAX / 2 && C.db <= kTile && C.dc <= kTile && rows_fit(C.a, C.heads / C.a_div, C.tokens) &&
-         rows_fit(C.b, C.heads / C.b_div, C.tokens) && rows_fit(C.c, C.heads / C.c_div, C.tokens) &&
-         C.dc % per == 0 && aligned(C.out.p, 16) && C.out.ts % per == 0 && C.out.hs % per == 0;
+bool tc_takes(const Chain& C) {
+  const int per = C.out_f32 ? 4 : 8;
+  return C.tokens > 0 && items_of(C) < INT32_MAX / 2 && C.db <= kTile && C.dc <= kTile &&
+         rows_fit(C.a, C.heads / C.a_div, C.tokens) && rows_fit(C.b, C.heads / C.b_div, C.tokens) &&
+         rows_fit(C.c, C.heads / C.c_div, C.tokens) && C.dc % per == 0 && aligned(C.out.p, 16) &&
+         C.out.ts % per == 0 && C.out.hs % per == 0;
 }
 
-int tc_states(const Chain& C, cudaStream_t s) { return run<true>(C, false, s); }
-int tc_outputs(const Chain& C, bool f32_out, cudaStream_t s) { return run<false>(C, f32_out, s); }
+template <int N>
+int tc_states(const Batch<N>& B, cudaStream_t s) { return run<true, N>(B, s); }
+template <int N>
+int tc_outputs(const Batch<N>& B, cudaStream_t s) { return run<false, N>(B, s); }
+template int tc_states<1>(const Batch<1>&, cudaStream_t);
+template int tc_states<3>(const Batch<3>&, cudaStream_t);
+template int tc_outputs<1>(const Batch<1>&, cudaStream_t);
+template int tc_outputs<3>(const Batch<3>&, cudaStream_t);
 
 }  // namespace lin
 
