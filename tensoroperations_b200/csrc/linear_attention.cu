@@ -418,15 +418,16 @@ int check_list(const char* who, const char* name, const void* p, bool need) {
 
 // Tokens of a segment, from what the host knows: the tokens, the sequences and
 // the heads (taken for sequences of equal length).  Among cuts of a sequence
-// into k segments, the one with the least estimated time, in units of a quarter
-// of a chunk's outputs: rounds of items over the CTAs that run at a time, a
-// chunk taking 4 units in the outputs' launch and `states` in the states', an
-// item `begin` to begin, the scan and its launch 6 and what its bytes cost.  A
-// segment is at most 1.5 times an SM's share of all chunks, so that one long
-// sequence among short ones is cut too.  One segment for all where no sequence
-// can be longer than one.
-// Tensor cores: chunks of 128 tokens (about 4.7 us), one CTA an SM.  CUDA cores:
-// chunks of 64 (about 10 us), one CTA for each 64 or 32 columns; narrow rows
+// into k segments, the one with the least estimated time, in quarters of what a
+// chunk's outputs take: rounds of items over the CTAs that run at a time, a chunk
+// 4 in the outputs' launch and `states` in the states', an item `begin` to begin,
+// the scan and its launch 6 and what its bytes cost, and a quarter of an item
+// for SMs that come out late.  Real lengths differ, so a segment is also at most
+// an SM's share of all chunks (half of it on the CUDA cores, where a chunk takes
+// long): one long sequence among short ones is cut too.  One segment for all
+// where no sequence can be longer than one.
+// Tensor cores: chunks of 128 tokens (about 4 us), one CTA an SM.  CUDA cores:
+// chunks of 64 (about 20 us), one CTA for each 64 or 32 columns; narrow rows
 // leave shared memory for two an SM.
 constexpr int kOneSegment = 1 << 30;
 
@@ -442,13 +443,14 @@ int plan_segment(const to_linear_attention_desc& d, bool tc, int chains) {
   long long best = mean, least = INT64_MAX;
   for (long long k = 1; k <= 64 && k <= mean; ++k) {
     const long long per = (mean + k - 1) / k;
-    long long cost = at_once * ((pairs * k + at_once - 1) / at_once) * (4 * per + begin);
+    long long cost = at_once * (((pairs * k + at_once - 1) / at_once) * (4 * per + begin) + per);
     if (k > 1)
       cost += at_once * (((pairs * (k - 1) + at_once - 1) / at_once) * (states * per + begin) + 6) + 4 * pairs * k;
     if (cost < least) least = cost, best = per;
   }
-  const long long share = std::max(tc ? 4ll : 2ll, (3 * chunks * blocks * d.q_heads / 2 + at_once - 1) / at_once);
-  if (best == mean) best = std::max(best, std::min(chunks, 2 * mean));  // ragged ones stay whole too
+  const long long load = (chunks * blocks * d.q_heads + at_once - 1) / at_once;
+  const long long share = std::max(tc ? 4ll : 2ll, tc ? load : (load + 1) / 2);
+  if (tc && best == mean) best = std::max(best, std::min(chunks, 2 * mean));  // ragged ones stay whole too
   best = std::min(best, std::max(share, mean / 64 + 1));
   return best >= chunks ? kOneSegment : static_cast<int>(best * chunk);
 }

@@ -556,8 +556,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           make_planes<STATES, 0, 3>(stage_of(i) + R::kK, lanes, i, dec_upd, w.rows(i), rev, true, q, h, 2, 4, lane);
         else
           make_planes<STATES, 0, 2>(stage_of(i) + R::kK, lanes, i, dec_upd, w.rows(i), rev, false, q, h, 2, 4, lane);
-        // the next planes go where those of chunk i - 1 are read (waited for here, before this
-        // chunk's product can end, so that the barrier is at most one turn ahead)
+        // the next planes go where those of chunk i - 1 are read; waited for here, so that no warp
+        // arrives for a chunk before all have for the last, and no barrier is two turns ahead
         if (i > 0 && !(ok = warp_wait(bar, &bar->u_full, (i - 1) & 1))) break;
         fence_before();
         __syncwarp();
@@ -774,14 +774,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         fence_before();
       }
+      // (a warp that arrives for chunk i knows that all have arrived for chunk i - 1, whose
+      // product it has waited for: no warp can take another's place in the count)
+      if (STATES && i > 0) {
+        update(i - 1);
+        if (!ok) break;
+      }
       __syncwarp();
       if (chunk && lane == 0) {
         if (i < w.updates) arrive(&bar->planes_ready);
         arrive(&bar->empty[i % kStages]);
-      }
-      if (STATES && i > 0) {
-        update(i - 1);
-        if (!ok) break;
       }
       if (!STATES && chunk) {  // once the product that read the last chunk's X is done
         if (i > 0 && !(ok = warp_wait(bar, &bar->o1_full, (i - 1) & 1))) break;
