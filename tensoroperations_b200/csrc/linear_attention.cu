@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
+          for (int q = 0; q <= r; ++q)  // (rows 16 r .. see no columns past 16 r + 15)
             acc[r][q] = fmaf(x[r].w, y[q].w, fmaf(x[r].z, y[q].z, fmaf(x[r].y, y[q].y, fmaf(x[r].x, y[q].x, acc[r][q]))));
       }
 #pragma unroll
@@ -138,22 +138,26 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
       __syncthreads();
       // out = P V + inter * l^(i+1-rev) A X
       float o[4][VC] = {}, w[4][VC] = {};
-      for (int j = 0; j < kRows; j += 4) {
-        float4 p[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[r] = *reinterpret_cast<const float4*>(P + (ty + 16 * r) * (kRows + 4) + j);
+      for (int block = 0; block < 4; ++block)  // 16 columns of P: rows from 16 block on see them
+#pragma unroll 1
+        for (int j = 16 * block; j < 16 * block + 16; j += 4) {
+          float4 p[4];
 #pragma unroll
-        for (int jj = 0; jj < 4; ++jj) {
-          float v[VC];
-          seq::load_vec<float, VC>(V + (j + jj) * kColPad + tx * VC, v);
+          for (int r = block; r < 4; ++r)
+            p[r] = *reinterpret_cast<const float4*>(P + (ty + 16 * r) * (kRows + 4) + j);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float pv = jj == 0 ? p[r].x : jj == 1 ? p[r].y : jj == 2 ? p[r].z : p[r].w;
+          for (int jj = 0; jj < 4; ++jj) {
+            float v[VC];
+            seq::load_vec<float, VC>(V + (j + jj) * kColPad + tx * VC, v);
 #pragma unroll
-            for (int c = 0; c < VC; ++c) o[r][c] = fmaf(pv, v[c], o[r][c]);
+            for (int r = block; r < 4; ++r) {
+              const float pv = jj == 0 ? p[r].x : jj == 1 ? p[r].y : jj == 2 ? p[r].z : p[r].w;
+#pragma unroll
+              for (int c = 0; c < VC; ++c) o[r][c] = fmaf(pv, v[c], o[r][c]);
+            }
           }
         }
-      }
       for (int k = 0; k < dbp; k += 4) {
         float4 p[4];
 #pragma unroll

@@ -653,15 +653,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int piece = lane & 7, row0 = 32 * q + (lane >> 3);
         const long long first = (w.first(C, i) + row0) * pitch + w.head / C.out_div * C.out.hs + h * 64;
         const bool f32 = C.out_f32;
-#pragma unroll 1
+        float y[2][32];
+        tmem_ld32(lanes + kColO + h * 64, y[0]);
+        tmem_ld32(lanes + kColO + h * 64 + 32, y[1]);
+        fence_before();
+        __syncwarp();
+        if (lane == 0) arrive(&bar->o_free);
+#pragma unroll
         for (int part = 0; part < 2; ++part) {
-          float x[32];
-          tmem_ld32(lanes + kColO + h * 64 + part * 32, x);
-          if (part == 1) {  // everything has been read
-            fence_before();
-            __syncwarp();
-            if (lane == 0) arrive(&bar->o_free);
-          }
+          const float(&x)[32] = y[part];
           if (f32) {
 #pragma unroll
             for (int j = 0; j < 32; j += 4)
