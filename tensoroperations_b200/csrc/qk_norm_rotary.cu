@@ -159,7 +159,7 @@ __device__ __forceinline__ float sum_over(float x, int lanes) {
 // units of VP pairs a lane.  SHARE groups (of those that there are) compute a
 // token's sines together, VP / SHARE pairs each, and hand them round.
 template <typename T, int VP, int UPL, int SHARE, int HEADS, bool BACKWARD>
-__global__ void __launch_bounds__(32 * kWarps, 2) qk_kernel(const __grid_constant__ QkArgs A) {
+__global__ void __launch_bounds__(32 * kWarps, VP == 4 && !BACKWARD ? 3 : 2) qk_kernel(const __grid_constant__ QkArgs A) {
   extern __shared__ float sums[];  // backward: [kWarps][dim]
   using U = Unit<T, VP>;
   constexpr int kOwn = VP / SHARE, kP = U::kPacked, kB = BACKWARD ? 1 : 0;
@@ -363,20 +363,25 @@ __global__ void __launch_bounds__(32 * kWarps, 2) qk_kernel(const __grid_constan
 }
 
 // dw[e] = sum over CTAs of their partial sums, in a fixed order, in f64 (a few
-// hundred terms: f32 would add as much rounding again as the terms have).  A
-// warp takes one value of dwq or dwk, its lanes every 32nd CTA.
-__global__ void __launch_bounds__(256) qk_sum_kernel(const float* __restrict__ partial, int q_ctas, int ctas,
-                                                     int dim, float* dwq, float* dwk) {
-  const int e = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (e >= 2 * dim) return;
-  const bool q = e < dim;
-  const int x = q ? e : e - dim, first = q ? 0 : q_ctas, last = q ? q_ctas : ctas;
+// hundred terms: f32 would add as much rounding again as the terms have).
+// blockIdx.y: dwq or dwk; 32 values a CTA, every 32nd partial row a warp.
+__global__ void __launch_bounds__(1024) qk_sum_kernel(const float* __restrict__ partial, int q_ctas, int ctas, int dim,
+                                                      float* dwq, float* dwk) {
+  __shared__ double part[32][33];
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, x = blockIdx.x * 32 + lane;
+  const int first = blockIdx.y ? q_ctas : 0, last = blockIdx.y ? ctas : q_ctas;
   double v = 0;
+  if (x < dim) {
 #pragma unroll 8
-  for (int c = first + lane; c < last; c += 32) v += partial[static_cast<long long>(c) * dim + x];
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  float* dst = q ? dwq : dwk;
-  if (lane == 0 && dst) dst[x] = static_cast<float>(v);
+    for (int c = first + row; c < last; c += 32) v += partial[static_cast<long long>(c) * dim + x];
+  }
+  part[row][lane] = v;
+  __syncthreads();
+  float* dst = blockIdx.y ? dwk : dwq;
+  if (row == 0 && x < dim && dst) {
+    for (int k = 1; k < 32; ++k) v += part[k][lane];
+    dst[x] = static_cast<float>(v);
+  }
 }
 
 // CTAs for q and for k: `cap` CTAs in all, shared by the time that a token takes
@@ -404,9 +409,12 @@ int launch(QkArgs& A, const to_qk_desc& d, bool backward, int sms, cudaStream_t 
   if (backward) {
     const QkGrid g = backward_grid(d, A.tokens, sms);
     A.q_ctas = g.q;
-    qk_kernel<T, VP, UPL, SHARE, 1, true><<<g.q + g.k, 32 * kWarps, size_t(kWarps) * A.dim * sizeof(float), s>>>(A);
+    qk_kernel<T, VP, UPL, SHARE, VP == 4 ? 2 : 1, true><<<g.q + g.k, 32 * kWarps, size_t(kWarps) * A.dim * sizeof(float), s>>>(A);
   } else {
-    const QkGrid g = grid_of(d, A.tokens * A.splits[0], A.tokens * A.splits[1], 32ll * sms);
+    // eight CTAs an SM: a warp takes several tokens (its weights are read once, and the next
+    // token's rows while it works), and the last ones still even out (72 us with 32, 87 with 2,
+    // at 16384 tokens of 40 heads)
+    const QkGrid g = grid_of(d, A.tokens * A.splits[0], A.tokens * A.splits[1], 8ll * sms);
     A.q_ctas = g.q;
     // two heads a step (more loads in flight) where a lane holds one unit
     qk_kernel<T, VP, UPL, SHARE, UPL == 1 ? 2 : 1, false><<<g.q + g.k, 32 * kWarps, 0, s>>>(A);
@@ -500,6 +508,9 @@ int run(const char* who, const to_qk_plan* plan, int64_t tokens, const to_rows* 
     }
     return true;
   };
+  // (gradients hold twice the rows: four pairs a lane and two heads a step, 68 us against 77
+  // with eight pairs and one head at 8192 tokens of 40 heads)
+  if (backward && vp == 8) vp = 4;
   while (vp > 1 && !fits(vp)) vp /= 2;
   if (vp == 1 && d.interleaved && !fits(1))
     return set_error(TO_ERR_ALIGNMENT, "%s: interleaved pairs must be aligned to a pair (%d bytes)", who, 2 * e);
@@ -616,7 +627,7 @@ int to_qk_norm_rotary_backward(const to_qk_plan* plan, int64_t tokens, const to_
   if (sms <= 0) return -sms;
   const int dim = plan->desc.head_dim;
   const QkGrid g = backward_grid(plan->desc, tokens, sms);
-  qk_sum_kernel<<<(2 * dim + 7) / 8, 256, 0, s>>>(partial, g.q, g.q + g.k, dim, dwq, dwk);
+  qk_sum_kernel<<<dim3((dim + 31) / 32, 2), 1024, 0, s>>>(partial, g.q, g.q + g.k, dim, dwq, dwk);
   TO_CUDA_TRY(cudaGetLastError());
   return ok();
 }
