@@ -14,7 +14,9 @@
 // TMEM operands (K transposed into its lanes by ldmatrix).
 //
 // Precision: P and X each enter their product with one bf16 rounding, as the
-// result's own.  The state stays f32: decayed K is split into bf16 planes of 8
+// result's own; in chunks of at most 32 tokens, where a row's error is that of a
+// few P and does not average out, P has a second plane (in columns of Sc that are
+// not those tokens').  The state stays f32: decayed K is split into bf16 planes of 8
 // bits each -- three, which reach f32, where the state is written out and the chunk
 // has not decayed by then, two where only products read it -- smallest plane first, so few sums pass through the
 // accumulator at full size; a chunk's U is added to X in IEEE f32 registers.
@@ -58,6 +60,7 @@ constexpr int kFirstRow = 4, kFirstState = kFirstRow + kRowWarps;  // warps 0, 1
 constexpr int kThreads = 32 * (kFirstState + kStateWarps);
 constexpr uint32_t kMaxPolls = 1u << 22;
 constexpr int kMaxStages = 3;
+constexpr int kFew = 32;                         // tokens of a chunk whose P is taken to 16 bits
 
 // Chunks in shared memory, 192 KB of them: tiles Q, K, V each, or K, V.
 template <bool STATES>
@@ -543,6 +546,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 0; k < kTile / 16; ++k)
             mma_ts(tm + kColO, tm + kColS + (k >> 2) * 64 + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB, true);
+          if (w.rows(i) <= kFew) {
+#pragma unroll 1
+            for (int k = 0; k < kFew / 16; ++k)
+              mma_ts(tm + kColO, tm + kColS + 32 + k * 8, desc_mn(sv, k), kIdesc | kMnB, true);
+          }
           commit(&bar->o2_full);
         }
         if (STATES) commit(&bar->empty_v[i % kStages]);
@@ -630,7 +638,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
 #pragma unroll
             for (int j = 0; j < 16; j += 2) p[j >> 1] = pack2(x[j], x[j + 1]);
+            if (cnt <= kFew && j0 < kFew) {  // second plane: what the rounding left
+              uint32_t rest[8];
+#pragma unroll
+              for (int j = 0; j < 16; j += 2)
+                rest[j >> 1] = pack2(x[j] - low_half(p[j >> 1]), x[j + 1] - high_half(p[j >> 1]));
+              tmem_st8(lanes + kColS + 32 + part * 8, rest);
+            }
+          } else if (cnt <= kFew && j0 < kFew) {
+            tmem_st8(lanes + kColS + 32 + part * 8, p);
           }
+          // (columns of Sc from 32 on are not those tokens', and masked whatever they hold)
           tmem_st8(lanes + kColS + h * 64 + part * 8, p);
         }
         // Q X, decayed from the chunk's beginning

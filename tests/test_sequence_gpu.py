@@ -4,8 +4,9 @@ Tolerances (relative 2-norm), from the types alone:
 * f32 results: 2e-6.  A rounding is at most 2^-24 = 6e-8; every value is a sum of
   a few hundred products whose roundings add in quadrature (16 x 6e-8 = 1e-6) plus
   a decay factor from expf (2 ulp) whose argument is rounded once.
-* bf16 results: 2^-8.  The result's own rounding is at most 2^-9, and products of
-  bf16 rows go through one more bf16 operand (at most 2^-9).
+* bf16 results: 2^-8.  A rounding to 8 bits is half a spacing at most, 2^-9.2 of the
+  values in the mean square; products of bf16 rows go through one more bf16 operand,
+  so there are two, in quadrature 2^-8.7.
 * one value: 16 times that, relative to the larger of itself and the rms (a value's
   own error is not averaged).
 """
@@ -343,6 +344,20 @@ def test_attention_decays(dtype):
             close(got[:, h], want[:, h], TOL[dtype], f"gradient, head {h}")
         if h < 3:  # with stronger decays the entering state's gradient is nothing but tiny values
             close(dS[:, h], ref[3][:, h], 2 * TOL["f32"], f"dstate {h}")
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 17, 32])
+def test_attention_few_tokens_round_once(tokens):
+    """From nothing, few tokens: the result's own rounding alone (half the spacing of bf16 values,
+    2^-7 of the power of two below, and what two planes leave of P)."""
+    from tensoroperations_b200 import sequence
+    q, k, v, decay, cu = attention_inputs("bf16", [tokens], 4, 2, 128, 64, seed=31)
+    op = sequence.LinearAttention("bf16", 4, 2, 128, 64)
+    o = torch.empty(tokens, 4, 64, dtype=q.dtype, device="cuda")
+    op.forward(q, k, v, decay, cu, o)
+    ref, _ = attention_definition(q, k, v, decay, [tokens], 128 ** -0.5, torch.zeros(1, 4, 128, 64, device="cuda"))
+    half = 0.5 * 2.0 ** (ref.abs().clamp(min=1e-30).log2().floor() - 7)
+    assert ((o.double() - ref).abs() <= half + 2.0 ** -14 * ref.abs().amax(-1, True)).all()
 
 
 def test_attention_long_prompts_repeat_to_the_bit():
