@@ -33,6 +33,11 @@
 // 0 * NaN is not 0.  Rows of a reversed chain keep their order in memory; only
 // the masks and decays turn round.
 //
+// Measured on B200, 49152 tokens x 16 heads x 128: outputs 186 us (4.3 TB/s, 0.67 of
+// the copy rate), states 81 us (5.0 TB/s).  A chunk's outputs take about 7000
+// cycles: Q X, the scaling, P V, Sc and U wait for one another, and products with
+// two shared operands take about 110 cycles each instead of 64.
+//
 // Every wait is bounded; on a timeout the kernel records TO_ERR_TIMEOUT in the
 // device status word, waits (bounded) for its copies in flight, frees its TMEM
 // and returns.
