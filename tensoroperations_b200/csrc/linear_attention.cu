@@ -3,7 +3,6 @@
 // cores, the segment scan, the single-token step, and the C-ABI entries.
 #include <algorithm>
 #include <cmath>
-#include <mutex>
 
 #include "linear_attention.cuh"
 
@@ -486,14 +485,9 @@ size_t part_bytes(const to_linear_attention_desc& d, int width) {
 
 template <typename T, int DCB, bool STATES, int N>
 int launch_simt(const lin::Batch<N>& B, cudaStream_t s) {
-  static std::once_flag once;
-  static cudaError_t attr = cudaSuccess;
+  static std::atomic<uint64_t> done{0};
   const size_t most = SimtShape<DCB>::bytes(DCB == 64 ? 128 : 256);
-  std::call_once(once, [&] {
-    attr = cudaFuncSetAttribute(chain_simt_kernel<T, DCB, STATES, N>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                static_cast<int>(most));
-  });
-  TO_CUDA_TRY(attr);
+  if (int st = seq::allow_shared(chain_simt_kernel<T, DCB, STATES, N>, most, done)) return st;
   const Chain& C = B.c[0];
   int db = 0, dc = 0;
   for (const Chain& x : B.c) db = std::max(db, x.db), dc = std::max(dc, x.dc);

@@ -43,8 +43,6 @@
 // and returns.
 #include <cuda.h>
 
-#include <mutex>
-
 #include "linear_attention.cuh"
 #include "sm100_primitives.cuh"
 #include "tensor_map.hpp"
@@ -881,13 +879,9 @@ bool rows_fit(const seq::Rows& r, int heads, long long tokens) {
 
 template <bool STATES, int N>
 int run(const lin::Batch<N>& B, cudaStream_t s) {
-  static std::once_flag once;
-  static cudaError_t attr = cudaSuccess;
-  std::call_once(once, [] {
-    attr = cudaFuncSetAttribute(chain_tc_kernel<STATES, N>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kSmem));
-  });
-  TO_CUDA_TRY(attr);
-  int st = TO_OK;
+  static std::atomic<uint64_t> done{0};
+  int st = seq::allow_shared(chain_tc_kernel<STATES, N>, kSmem, done);
+  if (st) return st;
   EncodeTiled enc = tensor_map_encoder(&st);
   if (!enc) return st;
   Maps<N> maps;

@@ -5,6 +5,7 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "common.hpp"
@@ -77,6 +78,20 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
     for (int j = 0; j < kPer; ++j) u.t[j] = from_f32<T>(x[i * kPer + j]);
     *(reinterpret_cast<R*>(p) + i) = u.r;
   }
+}
+
+// Allow `kernel` its dynamic shared memory on the current device, once a device
+// (`done`: a bit for each of the first 64; others are set every time).
+template <typename K>
+int allow_shared(K* kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  const int sms = device_sm_count(&dev);
+  if (sms <= 0) return -sms;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return ok();
+  TO_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return ok();
 }
 
 inline int dtype_bytes(int32_t dtype) { return dtype == TO_BF16 ? 2 : 4; }

@@ -346,6 +346,41 @@ def test_attention_decays(dtype):
             close(dS[:, h], ref[3][:, h], 2 * TOL["f32"], f"dstate {h}")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_of_nothing(dtype):
+    """No tokens at all: empty sequences hand their states, and the states' gradients, on."""
+    from tensoroperations_b200 import sequence
+    op = sequence.LinearAttention(dtype, 4, 2, 64, 32)
+    q, k, v, decay, cu = attention_inputs(dtype, [0, 0, 0], 4, 2, 64, 32)
+    S, left = torch.randn(3, 4, 64, 32, generator=rng(1), device="cuda"), torch.empty(3, 4, 64, 32, device="cuda")
+    o = torch.empty(0, 4, 32, dtype=q.dtype, device="cuda")
+    op.forward(q, k, v, decay, cu, o, state_in=S, state_out=left, workspace=scratch(op.workspace_bytes(0, 3)))
+    assert torch.equal(S, left)
+    back = torch.empty_like(S)
+    op.backward(q, k, v, decay, cu, o, q.clone(), k.clone(), v.clone(), state_in=S, dstate_out=left, dstate_in=back,
+                workspace=scratch(op.backward_workspace_bytes(0, 3)))
+    assert torch.equal(back, left)
+    op.forward(q, k, v, decay, cu[:1].contiguous(), o)  # and no sequences
+    op.step(q, k, v, decay, S, o)
+
+
+def test_qk_without_keys():
+    from tensoroperations_b200 import sequence
+    q, _, pos, wq, _ = qk_inputs("bf16", 50, 3, 1, 64, 1)
+    op = sequence.QkNormRotary("bf16", 3, 0, 64)
+    none, y = q[:, :0], torch.empty(50, 3, 64, dtype=q.dtype, device="cuda")
+    op.forward(q, none, pos, wq, None, y, none)
+    close(y, qk_definition(q, wq, pos, 64, [32], False), TOL["bf16"])
+    g, dq, dw = torch.randn_like(y), torch.empty_like(y), torch.empty_like(wq)
+    ws = torch.empty(op.workspace_bytes(50), dtype=torch.uint8, device="cuda")
+    op.backward(q, none, pos, wq, None, g, none, dq, none, dw, None, ws)
+    x64 = q.double().requires_grad_()
+    w64 = wq.double().requires_grad_()
+    rx, rw = torch.autograd.grad((qk_definition(x64, w64, pos, 64, [32], False) * g.double()).sum(), (x64, w64))
+    close(dq, rx, TOL["bf16"])
+    close(dw, rw, 2 * TOL["f32"])
+
+
 @pytest.mark.parametrize("tokens", [1, 3, 17, 32])
 def test_attention_few_tokens_round_once(tokens):
     """From nothing, few tokens: the result's own rounding alone (half the spacing of bf16 values,
