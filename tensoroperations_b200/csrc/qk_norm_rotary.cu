@@ -408,6 +408,10 @@ QkGrid grid_of(const to_qk_desc& d, long long items_q, long long items_k, long l
   return {part(cost_q, items_q), part(cost_k, items_k)};
 }
 
+// Heads that a group of lanes takes in one step of the forward pass: two (more loads in flight)
+// where a lane holds one unit.
+constexpr int forward_heads(int upl) { return upl == 1 ? 2 : 1; }
+
 // Two CTAs of eight warps fit an SM; three rounds of them even out their lengths.
 QkGrid backward_grid(const to_qk_desc& d, long long tokens, int sms) { return grid_of(d, tokens, tokens, 6ll * sms); }
 
@@ -423,8 +427,7 @@ int launch(QkArgs& A, const to_qk_desc& d, bool backward, int sms, cudaStream_t 
     // at 16384 tokens of 40 heads)
     const QkGrid g = grid_of(d, A.tokens * A.splits[0], A.tokens * A.splits[1], 8ll * sms);
     A.q_ctas = g.q;
-    // two heads a step (more loads in flight) where a lane holds one unit
-    qk_kernel<T, VP, UPL, SHARE, UPL == 1 ? 2 : 1, false><<<g.q + g.k, 32 * kWarps, 0, s>>>(A);
+    qk_kernel<T, VP, UPL, SHARE, forward_heads(UPL), false><<<g.q + g.k, 32 * kWarps, 0, s>>>(A);
   }
   TO_CUDA_TRY(cudaGetLastError());
   return ok();
@@ -441,9 +444,11 @@ int dispatch(QkArgs& A, const to_qk_desc& d, int vp, bool backward, int sms, cud
   while (A.lanes < 32 && A.lanes < A.units) A.lanes *= 2;
   const int upl = (A.units + A.lanes - 1) / A.lanes, groups = 32 / A.lanes;
   // warps that share a token's heads: one, unless the tokens are too few to give
-  // every SM sixteen warps; then at most one a step of heads
+  // every SM sixteen warps; then at most one a step of heads, so that each has a first
+  // step (in its last one a warp fetches the rows of its next item)
   for (int t = 0; t < 2; ++t) {
-    const long long steps = (A.heads[t] + groups - 1) / groups;
+    const int a_step = groups * forward_heads(upl);
+    const long long steps = (A.heads[t] + a_step - 1) / a_step;
     long long n = backward || A.tokens == 0 ? 1 : (16ll * sms + A.tokens - 1) / A.tokens;
     A.splits[t] = static_cast<int>(n > steps ? (steps > 0 ? steps : 1) : n);
   }
