@@ -282,7 +282,9 @@ __global__ void __launch_bounds__(32 * kWarps, VP == 4 && !BACKWARD ? 3 : 2) qk_
             sq = __ffma2_rn(xa[u][i], xa[u][i], __ffma2_rn(xb[u][i], xb[u][i], sq));
           }
         }
-        const float r = rsqrtf(sum_over(sq.x + sq.y, A.lanes) * inv_dim + eps);
+        const float sum = sum_over(sq.x + sq.y, A.lanes);
+        // (a group past the heads holds zeros, which without eps have no norm: they count as nothing)
+        const float r = h < heads ? rsqrtf(sum * inv_dim + eps) : 0.f;
         const float2 r2 = make_float2(r, r);
         T* row = seq::row_ptr<T>(out, token, h < heads ? h : 0);
         if (!BACKWARD) {

@@ -1,12 +1,12 @@
 """The sequence operators at the edges of their ranges, against definitions in float64:
-heads split over warps.
+heads split over warps, rows without a length.
 
 Tolerances are those of test_sequence_gpu (derived there from the types alone) unless a
 test says otherwise.
 """
 import pytest
 
-from test_sequence_gpu import TOL, close, qk_definition, qk_inputs
+from test_sequence_gpu import TOL, close, normal, qk_definition, qk_inputs, rng
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -41,3 +41,24 @@ def test_qk_heads_split_over_warps(dtype, T, hq, hk, D, in_place):
 def test_qk_heads_at_every_count_of_tokens(dtype, hq, hk, D, inter):
     for T in list(range(300, 2400, 149)) + [1183, 1184, 1185, 2368, 2369]:
         check_qk_forward(dtype, T, hq, hk, D, inter)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("hq,hk,D", [(1, 1, 128), (3, 1, 128), (5, 2, 64), (1, 3, 256), (7, 1, 6)])
+def test_qk_gradients_without_eps(dtype, hq, hk, D):
+    """eps = 0, no row is zero: the gradients are finite, whatever heads a warp has left over."""
+    from tensoroperations_b200 import sequence
+    T, half = 41, [D // 2]
+    q, k, pos, wq, wk = qk_inputs(dtype, T, hq, hk, D, 1, seed=8)
+    g = rng(9)
+    gq, gk = normal(g, (T, hq, D), dtype), normal(g, (T, hk, D), dtype)
+    op = sequence.QkNormRotary(dtype, hq, hk, D, eps=0.0)
+    dq, dk, dwq, dwk = torch.empty_like(gq), torch.empty_like(gk), torch.empty_like(wq), torch.empty_like(wk)
+    ws = torch.empty(op.workspace_bytes(T), dtype=torch.uint8, device="cuda")
+    op.backward(q, k, pos, wq, wk, gq, gk, dq, dk, dwq, dwk, ws)
+    for x, w, gy, dx, dw, name in ((q, wq, gq, dq, dwq, "q"), (k, wk, gk, dk, dwk, "k")):
+        x64, w64 = x.double().requires_grad_(), w.double().requires_grad_()
+        y = qk_definition(x64, w64, pos, D, half, False, eps=0.0)
+        rx, rw = torch.autograd.grad((y * gy.double()).sum(), (x64, w64))
+        close(dx, rx, TOL[dtype], "d" + name)
+        close(dw, rw, TOL["f32"] * 2, "dw" + name)
