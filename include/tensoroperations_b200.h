@@ -675,7 +675,8 @@ int to_linear_attention(const to_linear_attention_desc* desc, const to_linear_at
  * from d_o and dstate_out (the gradient of the state left; NULL: zero).
  * log_decay is a constant of the model.  States and their gradients are
  * [nseq][q_heads][key_dim][value_dim] (no slots).  Gradients of heads that
- * share a key / value head are summed in f32 before their one rounding.
+ * share a key / value head are summed in f32 before their one rounding.  Rows
+ * of dq, dk, dv that belong to no sequence are left as they are.
  */
 typedef struct to_linear_attention_grad_args {
   to_rows q, k, v, d_o, dq, dk, dv;

@@ -291,20 +291,23 @@ __global__ void __launch_bounds__(256) chain_scan_kernel(const __grid_constant__
 }
 
 // ---- shared heads: sum the gradients of the heads of a group ---------------------------
-// blockIdx.y: dk or dv.
+// blockIdx.y: dk or dv.  Packed sequences lie between the first and the last of their bounds;
+// the chains have written no other rows, and none are summed.
 struct GroupSum {
   const float* part[2];
   Rows out[2];
   int width[2];
-  long long tokens;
+  const int32_t* cu;
+  int nseq, tokens;
   int kv_heads, group;
 };
 
 template <typename T>
 __global__ void __launch_bounds__(256) group_sum_kernel(const __grid_constant__ GroupSum G) {
   const int y = blockIdx.y, width = G.width[y];
-  const long long per = static_cast<long long>(G.kv_heads) * width, total = G.tokens * per;
-  for (long long e = blockIdx.x * 256ll + threadIdx.x; e < total; e += gridDim.x * 256ll) {
+  const long long per = static_cast<long long>(G.kv_heads) * width;
+  const int first = min(max(__ldg(G.cu), 0), G.tokens), last = min(max(__ldg(G.cu + G.nseq), 0), G.tokens);
+  for (long long e = first * per + blockIdx.x * 256ll + threadIdx.x; e < last * per; e += gridDim.x * 256ll) {
     const long long t = e / per;
     const int r = static_cast<int>(e - t * per), h = r / width, x = r - h * width;
     const float* p = G.part[y] + ((t * G.kv_heads + h) * G.group) * width + x;
@@ -717,7 +720,7 @@ int to_linear_attention_backward(const to_linear_attention_desc* desc,
   if ((st = run_chains<3>(B, d, a.workspace, s))) return st;
   if (group == 1 || d.tokens == 0) return ok();
   GroupSum G{{parts[0], parts[1]}, {seq::rows_of(a.dk), seq::rows_of(a.dv)}, {d.key_dim, d.value_dim},
-             d.tokens, d.kv_heads, group};
+             a.cu_seqlens, d.nseq, static_cast<int>(d.tokens), d.kv_heads, group};
   const long long want = (d.tokens * d.kv_heads * std::max(d.key_dim, d.value_dim) + 255) / 256;
   const dim3 grid(static_cast<unsigned>(std::min(want, 148ll * 16)), 2);
   if (d.dtype == TO_BF16) group_sum_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(G);

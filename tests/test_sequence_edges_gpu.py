@@ -1,12 +1,13 @@
 """The sequence operators at the edges of their ranges, against definitions in float64:
-heads split over warps, rows without a length.
+heads split over warps, rows without a length, rows of no sequence.
 
 Tolerances are those of test_sequence_gpu (derived there from the types alone) unless a
 test says otherwise.
 """
 import pytest
 
-from test_sequence_gpu import TOL, close, normal, qk_definition, qk_inputs, rng
+from test_sequence_gpu import (TOL, attention_definition, attention_inputs, close, normal, qk_definition, qk_inputs,
+                               rng, scratch)
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -62,3 +63,32 @@ def test_qk_gradients_without_eps(dtype, hq, hk, D):
         rx, rw = torch.autograd.grad((y * gy.double()).sum(), (x64, w64))
         close(dx, rx, TOL[dtype], "d" + name)
         close(dw, rw, TOL["f32"] * 2, "dw" + name)
+
+
+# ---- linear attention ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,hq,hk,dk,dv", [
+    ("f32", 2, 1, 64, 64), ("bf16", 4, 2, 128, 128), ("bf16", 6, 2, 64, 96), ("bf16", 2, 1, 13, 9)])
+def test_gradients_of_shared_heads_leave_rows_of_no_sequence(dtype, hq, hk, dk, dv):
+    """Padding before the first sequence and after the last one keeps its gradients, as it does
+    where no heads are shared, and whatever the workspace held."""
+    from tensoroperations_b200 import sequence
+    T, first, last = 700, 40, 650
+    q, k, v, decay, _ = attention_inputs(dtype, [T], hq, hk, dk, dv, seed=11)
+    do = normal(rng(12), (T, hq, dv), dtype)
+    op = sequence.LinearAttention(dtype, hq, hk, dk, dv)
+    grads = [torch.full(t.shape, 7.0, dtype=t.dtype, device="cuda") for t in (q, k, v)]
+    cu = torch.tensor([first, 240, 240, last], dtype=torch.int32, device="cuda")
+    op.backward(q, k, v, decay, cu, do, *grads, workspace=scratch(op.backward_workspace_bytes(T, 3)))
+    x = [t[first:last].double().requires_grad_() for t in (q, k, v)]
+    o, _ = attention_definition(*x, decay, [200, 0, 410], dk ** -0.5, torch.zeros(3, hq, dk, dv, device="cuda"))
+    ref = torch.autograd.grad((o * do[first:last].double()).sum(), x)
+    for got, want, name in zip(grads, ref, ("dq", "dk", "dv")):
+        close(got[first:last], want, TOL[dtype], name)
+        assert (got[:first] == 7).all() and (got[last:] == 7).all(), name
+    # and with no sequence that has tokens: nothing is written
+    grads = [torch.full(t.shape, 7.0, dtype=t.dtype, device="cuda") for t in (q, k, v)]
+    op.backward(q, k, v, decay, torch.full_like(cu, 77), do, *grads,
+                workspace=scratch(op.backward_workspace_bytes(T, 3)))
+    assert all((g == 7).all() for g in grads)
