@@ -568,8 +568,11 @@ typedef struct to_rows {
  * turns), so any int32 position, negative ones included, keeps f32 accuracy.
  * wq, wk: [head_dim] f32, NULL for 1.  Sums are f32; one rounding at the end.
  * head_dim even, at most 256.  k_heads may be 0 (no keys).
- * Outputs may be the inputs themselves (same pointer and strides); they may
- * not overlap them otherwise.
+ * Outputs may be their own inputs (q_out q, k_out k: same pointer and strides);
+ * they may share no memory with them, or with one another, otherwise.  What
+ * shares memory against these rules is refused with TO_ERR_INVALID_ARGUMENT
+ * where the library can tell: arrays, rows that begin at the same place, and
+ * rows with one token stride that holds a token's heads.
  */
 typedef struct to_qk_desc {
   int32_t dtype;
@@ -600,7 +603,8 @@ int to_qk_norm_rotary(const to_qk_plan* plan, int64_t tokens, const to_rows* q, 
  * forward pass's inputs) and dwq, dwk ([head_dim] f32, overwritten; both are
  * computed even where wq / wk is NULL, and either may be NULL to leave it
  * out).  Sums run in a fixed order.  workspace: 16-byte aligned device memory
- * of at least to_qk_norm_rotary_workspace_bytes.  dq / dk may be gq / gk.
+ * of at least to_qk_norm_rotary_workspace_bytes.  dq may be gq or q, dk may be
+ * gk or k, as above.
  */
 size_t to_qk_norm_rotary_workspace_bytes(const to_qk_plan* plan, int64_t tokens);
 int to_qk_norm_rotary_backward(const to_qk_plan* plan, int64_t tokens, const to_rows* q,
@@ -631,7 +635,9 @@ int to_qk_norm_rotary_backward(const to_qk_plan* plan, int64_t tokens, const to_
  * aligned.  slots (device int32 [nseq]) names each sequence's slot in
  * state_in and state_out; NULL: slot n is sequence n.  A slot outside
  * [0, num_slots) stands for no state: the sequence starts from zero and writes
- * none.  Two sequences may not share a slot.  state_out may be state_in.
+ * none.  Two sequences may not share a slot.  state_out may be state_in, and
+ * may overlap it in no other way.  o may share no memory with q, k or v (in the
+ * single-token call too): they are read while it is written.
  *
  * key_dim and value_dim 1 .. 256.  Products of bf16 rows run on the tensor
  * cores with f32 sums; states and their updates keep f32 accuracy (what has
@@ -676,7 +682,8 @@ int to_linear_attention(const to_linear_attention_desc* desc, const to_linear_at
  * log_decay is a constant of the model.  States and their gradients are
  * [nseq][q_heads][key_dim][value_dim] (no slots).  Gradients of heads that
  * share a key / value head are summed in f32 before their one rounding.  Rows
- * of dq, dk, dv that belong to no sequence are left as they are.
+ * of dq, dk, dv that belong to no sequence are left as they are.  dq, dk, dv and
+ * dstate_in may share no memory with the inputs or with one another.
  */
 typedef struct to_linear_attention_grad_args {
   to_rows q, k, v, d_o, dq, dk, dv;
@@ -684,7 +691,7 @@ typedef struct to_linear_attention_grad_args {
   const int32_t* cu_seqlens;
   const float* state_in;
   const float* dstate_out;
-  float* dstate_in; /* NULL: not wanted; may not be dstate_out               */
+  float* dstate_in; /* NULL: not wanted                                      */
   void* workspace;  /* device, 256-byte aligned                              */
   size_t workspace_bytes;
 } to_linear_attention_grad_args;

@@ -466,6 +466,21 @@ int plan_segment(const to_linear_attention_desc& d, bool tc, int chains) {
   return best >= chunks ? kOneSegment : static_cast<int>(best * chunk);
 }
 
+// The rows of a prompt or of single tokens: o is written while others read q, k and v.
+int check_outputs(const char* who, const to_linear_attention_desc& d, const to_linear_attention_args& a) {
+  auto span = [&](const char* name, const to_rows& r, int heads, int width) {
+    return seq::span_of(name, &r, d.tokens, heads, width, d.dtype);
+  };
+  const seq::Span rows[] = {span("o", a.o, d.q_heads, d.value_dim), span("q", a.q, d.q_heads, d.key_dim),
+                            span("k", a.k, d.kv_heads, d.key_dim), span("v", a.v, d.kv_heads, d.value_dim)};
+  return seq::check_apart(who, rows, 4, 1);
+}
+
+// Bytes of `slots` states.
+size_t states_bytes(const to_linear_attention_desc& d, long long slots) {
+  return size_t(slots) * d.q_heads * d.key_dim * d.value_dim * 4;
+}
+
 constexpr size_t kAlign = 256;
 size_t rounded(size_t n) { return (n + kAlign - 1) / kAlign * kAlign; }
 
@@ -616,6 +631,10 @@ int to_linear_attention(const to_linear_attention_desc* desc, const to_linear_at
                      a.workspace ? a.workspace_bytes : 0, need);
   if (need && !aligned(a.workspace, kAlign))
     return set_error(TO_ERR_ALIGNMENT, "%s: workspace is not 256-byte aligned", who);
+  if ((st = check_outputs(who, d, a))) return st;
+  if (a.state_in != a.state_out &&
+      seq::arrays_meet(a.state_in, a.state_out, states_bytes(d, a.slots ? d.num_slots : d.nseq)))
+    return set_error(TO_ERR_INVALID_ARGUMENT, "%s: state_in and state_out share memory in part", who);
   lin::Batch<1> B{{base_chain(d, a.cu_seqlens, a.log_decay)}};
   Chain& C = B.c[0];
   C.a = seq::rows_of(a.q);
@@ -655,16 +674,26 @@ int to_linear_attention_backward(const to_linear_attention_desc* desc,
   if (!st) st = check_state(who, "dstate_out", a.dstate_out);
   if (!st) st = check_state(who, "dstate_in", a.dstate_in);
   if (st) return st;
-  if (a.dstate_in && a.dstate_in == a.dstate_out)
-    return set_error(TO_ERR_INVALID_ARGUMENT, "%s: dstate_in is dstate_out", who);
+  // the three chains run at the same time: none may write what another reads
+  const size_t states = states_bytes(d, d.nseq);
+  if (seq::arrays_meet(a.dstate_in, a.dstate_out, states)) return seq::refuse_overlap(who, "dstate_in", "dstate_out");
+  if (seq::arrays_meet(a.dstate_in, a.state_in, states)) return seq::refuse_overlap(who, "dstate_in", "state_in");
   const size_t need = to_linear_attention_backward_workspace_bytes(desc);
   if (need && (!a.workspace || a.workspace_bytes < need))
     return set_error(TO_ERR_INVALID_ARGUMENT, "%s: workspace %zu < %zu bytes", who,
                      a.workspace ? a.workspace_bytes : 0, need);
   if (need && !aligned(a.workspace, kAlign))
     return set_error(TO_ERR_ALIGNMENT, "%s: workspace is not 256-byte aligned", who);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int group = d.q_heads / d.kv_heads;
+  auto span = [&](const char* name, const to_rows& r, int heads, int width) {
+    return seq::span_of(name, &r, d.tokens, heads, width, d.dtype);
+  };
+  const seq::Span rows[] = {span("dq", a.dq, d.q_heads, d.key_dim), span("dk", a.dk, d.kv_heads, d.key_dim),
+                            span("dv", a.dv, d.kv_heads, d.value_dim), span("q", a.q, d.q_heads, d.key_dim),
+                            span("k", a.k, d.kv_heads, d.key_dim), span("v", a.v, d.kv_heads, d.value_dim),
+                            span("d_o", a.d_o, d.q_heads, d.value_dim)};
+  if ((st = seq::check_apart(who, rows, 7, 3))) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
   const float scale = static_cast<float>(d.scale);
   // the gradients of shared heads go through f32 rows of every query head
   char* part = static_cast<char*>(a.workspace) + 3 * state_bytes(d, 3);
@@ -746,6 +775,7 @@ int to_linear_attention_step(const to_linear_attention_desc* desc,
   if (st) return st;
   if (!a.state_out) return set_error(TO_ERR_INVALID_ARGUMENT, "%s: state_out is null", who);
   if ((st = check_state(who, "state_out", a.state_out))) return st;
+  if ((st = check_outputs(who, d, a))) return st;
   StepArgs A{};
   A.q = seq::rows_of(a.q);
   A.k = seq::rows_of(a.k);

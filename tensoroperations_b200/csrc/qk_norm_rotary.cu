@@ -499,6 +499,27 @@ int run(const char* who, const to_qk_plan* plan, int64_t tokens, const to_rows* 
     A.g[t] = seq::rows_of(backward ? *gr[t] : none);
     A.out[t] = seq::rows_of(*out[t]);
   }
+  // a row is read by the lanes that write it: an output may be its own input, row for row, and
+  // shares memory with nothing else
+  seq::Span spans[6];
+  int n = 0;
+  for (const to_rows* const* set : {out, in, gr}) {
+    if (set == gr && !backward) continue;
+    for (int t = 0; t < 2; ++t, ++n)
+      spans[n] = A.heads[t] ? seq::span_of(names[set == out ? 2 : set == in ? 0 : 1][t], set[t], tokens, A.heads[t],
+                                           width, d.dtype)
+                            : seq::Span{};
+  }
+  for (int t = 0; t < 2 && tokens > 0; ++t) {
+    const seq::Span& o = spans[t];
+    if (!o.heads) continue;
+    if (seq::meets_itself(o)) return set_error(TO_ERR_INVALID_ARGUMENT, "%s: rows of %s share memory", who, o.name);
+    for (int j = t + 1; j < n; ++j) {
+      const seq::Span& x = spans[j];
+      const bool own = j > 1 && j % 2 == t && x.p == o.p && x.ts == o.ts && x.hs == o.hs;
+      if (!own && seq::meet(o, x)) return seq::refuse_overlap(who, o.name, x.name);
+    }
+  }
   A.w[0] = wq;
   A.w[1] = wk;
   for (const float* w : A.w)

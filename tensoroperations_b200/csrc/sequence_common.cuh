@@ -120,5 +120,82 @@ inline bool rows_aligned(const to_rows* r, int64_t tokens, int32_t heads, int32_
          (heads <= 1 || r->head_stride * e % bytes == 0);
 }
 
+// ---- outputs apart from what a call still reads -----------------------------------
+
+// Rows as they lie in memory, in bytes.
+struct Span {
+  const char* name;
+  const char* p;
+  long long ts, hs, width;
+  long long tokens;
+  int heads;
+  long long token_bytes() const { return (heads - 1) * hs + width; }  // a token's heads, first to last
+  long long bytes() const { return (tokens - 1) * ts + token_bytes(); }
+};
+
+inline Span span_of(const char* name, const to_rows* r, int64_t tokens, int32_t heads, int32_t width, int32_t dtype) {
+  const long long e = dtype_bytes(dtype);
+  return {name, static_cast<const char*>(r->data), tokens > 1 ? r->token_stride * e : 0,
+          heads > 1 ? r->head_stride * e : 0, width * e, tokens, heads};
+}
+
+// Whether two different tokens or heads of the rows share memory.
+inline bool meets_itself(const Span& a) {
+  if (a.tokens <= 1 || a.heads <= 1 || a.ts >= a.token_bytes() || a.hs >= (a.tokens - 1) * a.ts + a.width) return false;
+  for (long long h = 1; h < a.heads; ++h) {  // head h of one token and head 0 of a later one
+    const long long t = h * a.hs / a.ts;
+    if ((t < a.tokens && h * a.hs - t * a.ts < a.width) || (t + 1 < a.tokens && (t + 1) * a.ts - h * a.hs < a.width))
+      return true;
+  }
+  return false;
+}
+
+// Whether one token of a and one of b, `shift` bytes on, share memory.
+inline bool tokens_meet(const Span& a, const Span& b, long long shift) {
+  for (int i = 0, j = 0; i < a.heads && j < b.heads;) {
+    const long long x = i * a.hs, y = shift + j * b.hs;
+    if (x + a.width <= y) ++i;
+    else if (y + b.width <= x) ++j;
+    else return true;
+  }
+  return false;
+}
+
+// Whether rows of a and of b share memory.  Exact where both have one token stride that holds a
+// token's heads (views into the same packed rows); other layouts whose ranges cross, without
+// beginning at the same place, are taken for apart.
+inline bool meet(const Span& a, const Span& b) {
+  if (!a.heads || !b.heads || !a.tokens) return false;
+  const long long d = b.p - a.p;
+  if (d >= a.bytes() || -d >= b.bytes()) return false;
+  if (d == 0) return true;
+  if (a.tokens == 1) return tokens_meet(a, b, d);
+  if (a.ts != b.ts || a.ts < a.token_bytes() || b.ts < b.token_bytes()) return false;
+  const long long t = d / a.ts - (d % a.ts < 0);  // b begins in a's token t
+  return (t < a.tokens && -t < a.tokens && tokens_meet(a, b, d - t * a.ts)) ||
+         (t + 1 < a.tokens && tokens_meet(a, b, d - (t + 1) * a.ts));
+}
+
+inline int refuse_overlap(const char* who, const char* a, const char* b) {
+  return set_error(TO_ERR_INVALID_ARGUMENT, "%s: %s and %s share memory", who, a, b);
+}
+
+// The first `outs` of n row arguments are written by CTAs that run while others read the rest.
+inline int check_apart(const char* who, const Span* s, int n, int outs) {
+  for (int i = 0; i < outs; ++i) {
+    if (meets_itself(s[i]))
+      return set_error(TO_ERR_INVALID_ARGUMENT, "%s: rows of %s share memory", who, s[i].name);
+    for (int j = i + 1; j < n; ++j)
+      if (meet(s[i], s[j])) return refuse_overlap(who, s[i].name, s[j].name);
+  }
+  return ok();
+}
+
+// Two arrays of n bytes, either of which may be null.
+inline bool arrays_meet(const void* a, const void* b, size_t n) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && (x < y ? y - x : x - y) < n;
+}
+
 }  // namespace seq
 }  // namespace to_b200

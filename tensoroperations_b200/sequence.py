@@ -8,6 +8,8 @@ nothing.  Rows are tensors [tokens, heads, width] whose last dimension is
 contiguous; they may be views into wider packed rows.  Shapes, types, devices
 and sizes are checked here, the rest by the library; a failed check raises
 before anything is launched (ValueError here, abi.ToError from the library).
+Outputs share no memory with what the call reads, but for q_out, k_out and
+state_out, which may be the inputs themselves.
 The caller orders the streams: a tensor written on another stream has to be
 ready on `stream`, and may be freed or overwritten only after it.
 """

@@ -92,3 +92,63 @@ def test_gradients_of_shared_heads_leave_rows_of_no_sequence(dtype, hq, hk, dk, 
     op.backward(q, k, v, decay, torch.full_like(cu, 77), do, *grads,
                 workspace=scratch(op.backward_workspace_bytes(T, 3)))
     assert all((g == 7).all() for g in grads)
+
+
+def packed(T, parts, dtype, by_head):
+    """Views of one buffer: each token's parts one after the other, or each head's (all of one head count)."""
+    if by_head:
+        rows = torch.empty(T, parts[0][0], sum(w for _, w in parts), dtype=dtype, device="cuda")
+        return rows.split([w for _, w in parts], -1)
+    rows = torch.empty(T, sum(h * w for h, w in parts), dtype=dtype, device="cuda")
+    return [x.view(T, *p) for x, p in zip(rows.split([h * w for h, w in parts], -1), parts)]
+
+
+@pytest.mark.parametrize("by_head", [False, True])
+@pytest.mark.parametrize("dtype,hq,hk,dk,dv", [("bf16", 4, 4, 64, 128), ("f32", 3, 3, 24, 40), ("bf16", 4, 2, 64, 64)])
+def test_packed_rows_hold_inputs_and_outputs(dtype, hq, hk, dk, dv, by_head):
+    """Inputs and outputs side by side in the same packed rows share no memory, and are not refused."""
+    from tensoroperations_b200 import sequence
+    if by_head and hq != hk:
+        pytest.skip("heads of one count")
+    T, lengths = 390, [300, 90]
+    q, k, v, decay, cu = attention_inputs(dtype, lengths, hq, hk, dk, dv, seed=51)
+    do = normal(rng(52), (T, hq, dv), dtype)
+    parts = [(hq, dk), (hk, dk), (hk, dv), (hq, dv)]
+    views = packed(T, parts + parts[:3] + [parts[3]], q.dtype, by_head)
+    for view, x in zip(views, (q, k, v, do)):
+        view.copy_(x)
+    (q1, k1, v1, do1), (dq, dk_, dv_, o) = views[:4], views[4:]
+    op = sequence.LinearAttention(dtype, hq, hk, dk, dv)
+    op.forward(q1, k1, v1, decay, cu, o, workspace=scratch(op.workspace_bytes(T, 2)))
+    op.backward(q1, k1, v1, decay, cu, do1, dq, dk_, dv_, workspace=scratch(op.backward_workspace_bytes(T, 2)))
+    x = [t.double().requires_grad_() for t in (q, k, v)]
+    ref, _ = attention_definition(*x, decay, lengths, dk ** -0.5, torch.zeros(2, hq, dk, dv, device="cuda"))
+    close(o, ref.detach(), TOL[dtype], "o")
+    for got, want in zip((dq, dk_, dv_), torch.autograd.grad((ref * do.double()).sum(), x)):
+        close(got, want, TOL[dtype], "gradient")
+    for view, t in zip(views, (q, k, v, do)):
+        assert torch.equal(view, t)
+    state = torch.zeros(T, hq, dk, dv, device="cuda")
+    op.step(q1, k1, v1, decay, state, o)
+    group = hq // hk
+    kd, vd = k.double().repeat_interleave(group, 1), v.double().repeat_interleave(group, 1)
+    close(o, dk ** -0.5 * (q.double() * kd).sum(-1, keepdim=True) * vd, TOL[dtype], "step")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_qk_in_place_in_packed_rows(dtype):
+    from tensoroperations_b200 import sequence
+    T, hq, hk, D = 77, 5, 3, 64
+    q, k, pos, wq, wk = qk_inputs(dtype, T, hq, hk, D, 1, seed=53)
+    gq, gk = (normal(rng(54 + i), x.shape, dtype) for i, x in enumerate((q, k)))
+    op = sequence.QkNormRotary(dtype, hq, hk, D)
+    ws = torch.empty(op.workspace_bytes(T), dtype=torch.uint8, device="cuda")
+    dq, dk, dw = torch.empty_like(gq), torch.empty_like(gk), torch.empty(2, D, device="cuda")
+    op.backward(q, k, pos, wq, wk, gq, gk, dq, dk, dw[0], dw[1], ws)
+    q2, k2, _, _, _ = qk_inputs(dtype, T, hq, hk, D, 1, seed=53)  # the gradients over the inputs
+    op.backward(q2, k2, pos, wq, wk, gq, gk, q2, k2, None, None, ws)
+    assert torch.equal(q2, dq) and torch.equal(k2, dk)
+    want = [qk_definition(x, w, pos, D, [D // 2], False) for x, w in ((q, wq), (k, wk))]
+    op.forward(q, k, pos, wq, wk, q, k)
+    close(q, want[0], TOL[dtype], "q")
+    close(k, want[1], TOL[dtype], "k")
