@@ -17,9 +17,11 @@
 // result's own; in chunks of at most 32 tokens, where a row's error is that of a
 // few P and does not average out, P has a second plane (in columns of Sc that are
 // not those tokens').  The state stays f32: decayed K is split into bf16 planes of 8
-// bits each -- three, which reach f32, where the state is written out and the chunk
-// has not decayed by then, two where only products read it -- smallest plane first, so few sums pass through the
-// accumulator at full size; a chunk's U is added to X in IEEE f32 registers.
+// bits each -- three, which reach f32, where the sequence's state is a result, two where
+// only products read it -- smallest plane first, so few sums pass through the
+// accumulator at full size; a chunk's U is added to X in IEEE f32 registers.  (Two planes
+// for chunks that have decayed far by the sequence's end are not enough: the tokens after
+// them may weigh nothing.)
 //
 // Roles (20 warps): one lane issues TMA loads, two chunks ahead, one the
 // products; warps 4-11 turn Sc into P, scale O and store the results (a thread:
@@ -258,7 +260,7 @@ struct Walk {
   int seq, head;
   bool last, only;      // the sequence's last segment; its only one
   int edge;             // first row of the segment (forwards), or the row after it (backwards)
-  int len, after;       // its tokens, and those of the sequence that follow it
+  int len;              // its tokens
   int n, updates;       // chunks; those whose state is wanted (not the last's, where no one reads it)
   __device__ __forceinline__ int rows(int i) const { return min(len - i * kTile, kTile); }
   // First row in memory of chunk i.
@@ -279,7 +281,6 @@ __device__ __forceinline__ bool walk_of(const Chain& C, int item, Walk* w) {
   w->last = g.idx == g.count - 1;
   w->only = g.count == 1;
   w->len = min(C.seg, g.tokens - s0);
-  w->after = g.tokens - s0 - w->len;
   w->edge = C.rev ? g.first + g.tokens - s0 : g.first + s0;
   w->n = (w->len + kTile - 1) / kTile;
   w->updates = STATES || (C.fin && w->last) ? w->n : w->n - 1;
@@ -436,12 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Barriers* bar = reinterpret_cast<Barriers*>(sm + kBars);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool rev = C.rev != 0;
-  // three planes of chunk i?  Where the state is a result, for the chunks that are still
-  // there at a 256th or more at the sequence's end: two planes have 16 bits, and 8 more are gone
-  const bool exact = C.fin && (STATES || w.last);
-  auto three_at = [&](int i) {
-    return exact && gl * static_cast<float>(w.after + max(w.len - (i + 1) * kTile, 0)) > -5.55f;
-  };
+  const bool three = C.fin && (STATES || w.last);  // planes: the sequence's state is a result
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -521,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t turn = i & 1, sq = fresh(stage_of(i)), sv = sq + R::kV;
         const uint32_t tm = fresh(tmem), sx = fresh(base) + kX;
         if (i < w.updates) {
-          const int planes = three_at(i) ? 3 : 2;
+          const int planes = three ? 3 : 2;
           // (outputs: the state warps have read the last U before they make planes)
           if (!(ok = wait_for(bar, &bar->full_v[i % kStages], turn_of(i)) && wait_for(bar, &bar->planes_ready, turn) &&
                      (!STATES || i == 0 || wait_for(bar, &bar->u_free, turn ^ 1))))
@@ -568,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- the planes of every second 32 tokens ----
       for (int i = 0; i < w.n; ++i) {
         if (!(ok = warp_wait(bar, &bar->full[i % kStages], turn_of(i)))) break;
-        if (three_at(i))
+        if (three)
           make_planes<STATES, 0, 3>(stage_of(i) + R::kK, lanes, i, dec_upd, w.rows(i), rev, true, q, h, 2, 4, lane);
         else
           make_planes<STATES, 0, 2>(stage_of(i) + R::kK, lanes, i, dec_upd, w.rows(i), rev, false, q, h, 2, 4, lane);
@@ -789,7 +785,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (chunk && i < w.updates) {
         constexpr int kG = STATES ? 2 : 4;
-        const bool three = three_at(i);
         if (STATES && three)
           make_planes<STATES, 0, STATES ? 3 : 2>(stage_of(i) + R::kK, lanes, i, dec_upd, cnt, rev, true, q, h, 0, kG, lane);
         else

@@ -1,5 +1,6 @@
 """The sequence operators at the edges of their ranges, against definitions in float64:
-heads split over warps, rows without a length, rows of no sequence.
+heads split over warps, rows without a length, rows of no sequence, sequences that end in
+silence.
 
 Tolerances are those of test_sequence_gpu (derived there from the types alone) unless a
 test says otherwise.
@@ -152,3 +153,29 @@ def test_qk_in_place_in_packed_rows(dtype):
     op.forward(q, k, pos, wq, wk, q, k)
     close(q, want[0], TOL[dtype], "q")
     close(k, want[1], TOL[dtype], "k")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T,silent,rates", [(300, 172, [-0.04, -0.06, -0.09]), (6000, 1500, [-0.004, -0.006, -0.008])])
+def test_states_of_sequences_that_end_in_silence(dtype, T, silent, rates):
+    """Tokens of zero keys at the end (zero outputs' gradients at the beginning, for the state's
+    gradient): what is left of the others has decayed far, and is still exact to f32."""
+    from tensoroperations_b200 import sequence
+    d, H = 64, 3
+    q, k, v, _, cu = attention_inputs(dtype, [T], H, H, d, d, seed=21)
+    decay = torch.tensor(rates, device="cuda")
+    do = normal(rng(22), (T, H, d), dtype)
+    k[T - silent:] = 0
+    do[:silent] = 0
+    op = sequence.LinearAttention(dtype, H, H, d, d)
+    o, left, dS = torch.empty_like(q), torch.empty(1, H, d, d, device="cuda"), torch.empty(1, H, d, d, device="cuda")
+    op.forward(q, k, v, decay, cu, o, state_out=left, workspace=scratch(op.workspace_bytes(T, 1)))
+    grads = [torch.empty(t.shape, dtype=t.dtype, device="cuda") for t in (q, k, v)]
+    op.backward(q, k, v, decay, cu, do, *grads, dstate_in=dS, workspace=scratch(op.backward_workspace_bytes(T, 1)))
+    lam = decay.double()
+    age = torch.arange(T, device="cuda", dtype=torch.float64)
+    for h in range(H):
+        late = (lam[h] * (T - 1 - age)).exp()[:, None]
+        close(left[0, h], (k[:, h].double() * late).t() @ v[:, h].double(), TOL["f32"], f"state, head {h}")
+        early = d ** -0.5 * (lam[h] * (age + 1)).exp()[:, None]
+        close(dS[0, h], (q[:, h].double() * early).t() @ do[:, h].double(), TOL["f32"], f"dstate, head {h}")
