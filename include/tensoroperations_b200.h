@@ -640,8 +640,10 @@ int to_qk_norm_rotary_backward(const to_qk_plan* plan, int64_t tokens, const to_
  * single-token call too): they are read while it is written.
  *
  * key_dim and value_dim 1 .. 256.  Products of bf16 rows run on the tensor
- * cores with f32 sums; states and their updates keep f32 accuracy.  The
- * chunked form multiplies masked pairs of a 128-token chunk by zero, so a
+ * cores with f32 sums; states and their updates keep f32 accuracy.  Results take
+ * one rounding to bf16 for the first 128 tokens of a sequence that nothing
+ * enters (for dk and dv the last 128), the others one more of the products'
+ * operands.  The chunked form multiplies masked pairs of a 128-token chunk by zero, so a
  * non-finite value in one token's row can reach earlier tokens of its own
  * chunk; it never reaches another sequence.
  *

@@ -14,9 +14,9 @@
 // TMEM operands (K transposed into its lanes by ldmatrix).
 //
 // Precision: P and X each enter their product with one bf16 rounding, as the
-// result's own; in chunks of at most 32 tokens, where a row's error is that of a
-// few P and does not average out, P has a second plane (in columns of Sc that are
-// not those tokens').  The state stays f32: decayed K is split into bf16 planes of 8
+// result's own.  In the chain's first chunk of a sequence a row has few P and nothing
+// else, whose errors do not average out: there P has a second plane, so those tokens'
+// results are rounded once, whatever follows them.  The state stays f32: decayed K is split into bf16 planes of 8
 // bits each -- three, which reach f32, where the sequence's state is a result, two where
 // only products read it -- smallest plane first, so few sums pass through the
 // accumulator at full size; a chunk's U is added to X in IEEE f32 registers.  (Two planes
@@ -65,7 +65,6 @@ constexpr int kFirstRow = 4, kFirstState = kFirstRow + kRowWarps;  // warps 0, 1
 constexpr int kThreads = 32 * (kFirstState + kStateWarps);
 constexpr uint32_t kMaxPolls = 1u << 22;
 constexpr int kMaxStages = 3;
-constexpr int kFew = 32;                         // tokens of a chunk whose P is taken to 16 bits
 
 // Chunks in shared memory, 192 KB of them: tiles Q, K, V each, or K, V.
 template <bool STATES>
@@ -74,8 +73,8 @@ struct Ring {
   static constexpr uint32_t kK = STATES ? 0 : kTileBytes, kV = kK + kTileBytes, kBytes = kV + kTileBytes;
 };
 
-// TMEM columns.  P of tokens [0, 64) and [64, 128) overwrites the first halves
-// of those tokens' columns of Sc.
+// TMEM columns.  P of each 16 tokens overwrites the first half of their columns of Sc, its
+// second plane the other half.
 constexpr uint32_t kColS = 0, kColO = 128;
 template <bool STATES>
 constexpr uint32_t kColU = STATES ? 0 : 256;
@@ -258,7 +257,7 @@ constexpr int kTable = 164, kUpdTable = 132;
 // The segment of one head that a CTA walks.
 struct Walk {
   int seq, head;
-  bool last, only;      // the sequence's last segment; its only one
+  bool begins, last, only;  // the sequence's first segment; its last; its only one
   int edge;             // first row of the segment (forwards), or the row after it (backwards)
   int len;              // its tokens
   int n, updates;       // chunks; those whose state is wanted (not the last's, where no one reads it)
@@ -278,6 +277,7 @@ __device__ __forceinline__ bool walk_of(const Chain& C, int item, Walk* w) {
   const int s0 = g.idx * C.seg;  // no overflow: below the sequence's length
   w->seq = g.seq;
   w->head = item - slot * C.heads;
+  w->begins = g.idx == 0;
   w->last = g.idx == g.count - 1;
   w->only = g.count == 1;
   w->len = min(C.seg, g.tokens - s0);
@@ -544,11 +544,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_after();
 #pragma unroll
           for (int k = 0; k < kTile / 16; ++k)
-            mma_ts(tm + kColO, tm + kColS + (k >> 2) * 64 + (k & 3) * 8, desc_mn(sv, k), kIdesc | kMnB, true);
-          if (w.rows(i) <= kFew) {
+            mma_ts(tm + kColO, tm + kColS + k * 16, desc_mn(sv, k), kIdesc | kMnB, true);
+          if (w.begins && i == 0) {
 #pragma unroll 1
-            for (int k = 0; k < kFew / 16; ++k)
-              mma_ts(tm + kColO, tm + kColS + 32 + k * 8, desc_mn(sv, k), kIdesc | kMnB, true);
+            for (int k = 0; k < kTile / 16; ++k)
+              mma_ts(tm + kColO, tm + kColS + k * 16 + 8, desc_mn(sv, k), kIdesc | kMnB, true);
           }
           commit(&bar->o2_full);
         }
@@ -588,8 +588,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int cnt = w.rows(i);
         const uint32_t turn = i & 1;
         // P[r][j] = intra Sc[r][j] l^|r - j| where j has been seen by r: blocks of 16
-        // columns, of which this warp's rows see all, a triangle, or nothing.  (Each block's
-        // P lands on columns of Sc that this warp has read by then.)
+        // columns, of which this warp's rows see all, a triangle, or nothing.
+        const bool second = w.begins && i == 0;
         if (!(ok = warp_wait(bar, &bar->sc_full, turn))) break;
         fence_after();
 #pragma unroll 1
@@ -637,18 +637,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
 #pragma unroll
             for (int j = 0; j < 16; j += 2) p[j >> 1] = pack2(x[j], x[j + 1]);
-            if (cnt <= kFew && j0 < kFew) {  // second plane: what the rounding left
+            if (second) {  // what the rounding left
               uint32_t rest[8];
 #pragma unroll
               for (int j = 0; j < 16; j += 2)
                 rest[j >> 1] = pack2(x[j] - low_half(p[j >> 1]), x[j + 1] - high_half(p[j >> 1]));
-              tmem_st8(lanes + kColS + 32 + part * 8, rest);
+              tmem_st8(lanes + kColS + j0 + 8, rest);
             }
-          } else if (cnt <= kFew && j0 < kFew) {
-            tmem_st8(lanes + kColS + 32 + part * 8, p);
+          } else if (second) {
+            tmem_st8(lanes + kColS + j0 + 8, p);
           }
-          // (columns of Sc from 32 on are not those tokens', and masked whatever they hold)
-          tmem_st8(lanes + kColS + h * 64 + part * 8, p);
+          tmem_st8(lanes + kColS + j0, p);
         }
         // Q X, decayed from the chunk's beginning
         const float f = inter * lds(dec + 4 * max(rev ? cnt - 1 - r : r + 1, 0));

@@ -1,6 +1,6 @@
 """The sequence operators at the edges of their ranges, against definitions in float64:
 heads split over warps, rows without a length, rows of no sequence, sequences that end in
-silence.
+silence, first tokens.
 
 Tolerances are those of test_sequence_gpu (derived there from the types alone) unless a
 test says otherwise.
@@ -179,3 +179,33 @@ def test_states_of_sequences_that_end_in_silence(dtype, T, silent, rates):
         close(left[0, h], (k[:, h].double() * late).t() @ v[:, h].double(), TOL["f32"], f"state, head {h}")
         early = d ** -0.5 * (lam[h] * (age + 1)).exp()[:, None]
         close(dS[0, h], (q[:, h].double() * early).t() @ do[:, h].double(), TOL["f32"], f"dstate, head {h}")
+
+
+def rounded_once(got, ref, what):
+    """Half the spacing of bf16 values (2^-7 of the power of two below), and what two planes leave of P."""
+    half = 0.5 * 2.0 ** (ref.abs().clamp(min=1e-30).log2().floor() - 7)
+    off = ((got.double() - ref).abs() - half) / ref.abs().amax(-1, True)
+    assert (off <= 2.0 ** -14).all(), (what, float(off.max()))
+
+
+@pytest.mark.parametrize("tokens", [31, 32, 33, 48, 100, 128, 129, 400])
+def test_first_tokens_do_not_depend_on_how_many_follow(tokens):
+    """The first tokens of a sequence (the last ones, for dk and dv) have the result's own rounding
+    alone, however long the sequence is."""
+    from tensoroperations_b200 import sequence
+    H, d, n = 4, 128, min(tokens, 32)
+    q, k, v, decay, cu = attention_inputs("bf16", [tokens], H, H, d, 64, seed=31)
+    op = sequence.LinearAttention("bf16", H, H, d, 64)
+    o = torch.empty(tokens, H, 64, dtype=q.dtype, device="cuda")
+    op.forward(q, k, v, decay, cu, o, workspace=scratch(op.workspace_bytes(tokens, 1)))
+    none = torch.zeros(1, H, d, 64, device="cuda")
+    x = [t.double().requires_grad_() for t in (q, k, v)]
+    ref, _ = attention_definition(*x, decay, [tokens], d ** -0.5, none)
+    rounded_once(o[:n], ref.detach()[:n], "o")
+    do = normal(rng(32), (tokens, H, 64), "bf16")
+    grads = [torch.empty(t.shape, dtype=t.dtype, device="cuda") for t in (q, k, v)]
+    op.backward(q, k, v, decay, cu, do, *grads, workspace=scratch(op.backward_workspace_bytes(tokens, 1)))
+    dq, dk, dv = torch.autograd.grad((ref * do.double()).sum(), x)
+    rounded_once(grads[0][:n], dq[:n], "dq")
+    rounded_once(grads[1][tokens - n:], dk[tokens - n:], "dk")
+    rounded_once(grads[2][tokens - n:], dv[tokens - n:], "dv")
