@@ -39,13 +39,15 @@ struct SimtShape {
 
 // Rows of a chunk into shared memory as f32, four columns a thread; rows past
 // cnt and columns past width become zero.  `vec`: four columns are one access.
+// Whether this thread met an infinity or a NaN.
 template <typename T>
-__device__ __forceinline__ void load_rows(float* dst, int ld, const Rows& r, int head, int row0, int step, int cnt,
+__device__ __forceinline__ bool load_rows(float* dst, int ld, const Rows& r, int head, int row0, int step, int cnt,
                                           int first, int width, int padded, bool vec) {
   int lanes = 8;  // threads of a row: a power of two
   while (lanes * 4 < padded) lanes *= 2;
   const int x = (threadIdx.x & (lanes - 1)) * 4;
-  if (x >= padded) return;
+  if (x >= padded) return false;
+  float odd = 0.f;  // 0 times each value: 0 while all are finite
   const T* src = seq::row_ptr<const T>(r, row0, head) + first + x;
   const long long hop = static_cast<long long>(step) * r.ts;
 #pragma unroll 4
@@ -61,8 +63,11 @@ __device__ __forceinline__ void load_rows(float* dst, int ld, const Rows& r, int
           if (x + e < width) v[e] = seq::to_f32(p[e]);
       }
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) odd = fmaf(0.f, v[e], odd);
     *reinterpret_cast<float4*>(dst + i * ld + x) = make_float4(v[0], v[1], v[2], v[3]);
   }
+  return !(odd == 0.f);
 }
 
 template <typename T, int DCB, bool STATES, int N>
@@ -113,8 +118,9 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
     __syncthreads();  // the last chunk's readers are done
     if (!STATES) load_rows<T>(A, lda, C.a, head / C.a_div, row0, step, cnt, 0, C.db, dbp, C.vec & 1);
     load_rows<T>(B, lda, C.b, head / C.b_div, row0, step, cnt, 0, C.db, dbp, C.vec & 2);
-    load_rows<T>(V, kColPad, C.c, head / C.c_div, row0, step, cnt, col0, ncols, DCB, C.vec & 4);
-    __syncthreads();
+    const bool met = load_rows<T>(V, kColPad, C.c, head / C.c_div, row0, step, cnt, col0, ncols, DCB, C.vec & 4);
+    // a value of V that is not finite may not meet the zeros of P: 0 * inf is not 0
+    const bool masked = STATES ? (__syncthreads(), false) : __syncthreads_or(met);
     if (!STATES) {
       float acc[4][4] = {};
       for (int k = 0; k < dbp; k += 4) {
@@ -140,26 +146,40 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
       __syncthreads();
       // out = P V + inter * l^(i+1-rev) A X
       float o[4][VC] = {}, w[4][VC] = {};
+      if (masked) {
+        for (int j = 0; j < cnt; ++j) {
+          float v[VC];
+          seq::load_vec<float, VC>(V + j * kColPad + tx * VC, v);
 #pragma unroll
-      for (int block = 0; block < 4; ++block)  // 16 columns of P: rows from 16 block on see them
-#pragma unroll 1
-        for (int j = 16 * block; j < 16 * block + 16; j += 4) {
-          float4 p[4];
+          for (int r = 0; r < 4; ++r) {
+            if (ty + 16 * r < j) continue;
+            const float pv = P[(ty + 16 * r) * (kRows + 4) + j];
 #pragma unroll
-          for (int r = block; r < 4; ++r)
-            p[r] = *reinterpret_cast<const float4*>(P + (ty + 16 * r) * (kRows + 4) + j);
-#pragma unroll
-          for (int jj = 0; jj < 4; ++jj) {
-            float v[VC];
-            seq::load_vec<float, VC>(V + (j + jj) * kColPad + tx * VC, v);
-#pragma unroll
-            for (int r = block; r < 4; ++r) {
-              const float pv = jj == 0 ? p[r].x : jj == 1 ? p[r].y : jj == 2 ? p[r].z : p[r].w;
-#pragma unroll
-              for (int c = 0; c < VC; ++c) o[r][c] = fmaf(pv, v[c], o[r][c]);
-            }
+            for (int c = 0; c < VC; ++c) o[r][c] = fmaf(pv, v[c], o[r][c]);
           }
         }
+      } else {
+#pragma unroll
+        for (int block = 0; block < 4; ++block)  // 16 columns of P: rows from 16 block on see them
+#pragma unroll 1
+          for (int j = 16 * block; j < 16 * block + 16; j += 4) {
+            float4 p[4];
+#pragma unroll
+            for (int r = block; r < 4; ++r)
+              p[r] = *reinterpret_cast<const float4*>(P + (ty + 16 * r) * (kRows + 4) + j);
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+              float v[VC];
+              seq::load_vec<float, VC>(V + (j + jj) * kColPad + tx * VC, v);
+#pragma unroll
+              for (int r = block; r < 4; ++r) {
+                const float pv = jj == 0 ? p[r].x : jj == 1 ? p[r].y : jj == 2 ? p[r].z : p[r].w;
+#pragma unroll
+                for (int c = 0; c < VC; ++c) o[r][c] = fmaf(pv, v[c], o[r][c]);
+              }
+            }
+          }
+      }
       for (int k = 0; k < dbp; k += 4) {
         float4 p[4];
 #pragma unroll

@@ -1,10 +1,12 @@
 """The sequence operators at the edges of their ranges, against definitions in float64:
 heads split over warps, rows without a length, rows of no sequence, sequences that end in
-silence, first tokens.
+silence, first tokens, infinities and NaN.
 
 Tolerances are those of test_sequence_gpu (derived there from the types alone) unless a
 test says otherwise.
 """
+import math
+
 import pytest
 
 from test_sequence_gpu import (TOL, attention_definition, attention_inputs, close, normal, qk_definition, qk_inputs,
@@ -209,3 +211,114 @@ def test_first_tokens_do_not_depend_on_how_many_follow(tokens):
     rounded_once(grads[0][:n], dq[:n], "dq")
     rounded_once(grads[1][tokens - n:], dk[tokens - n:], "dk")
     rounded_once(grads[2][tokens - n:], dv[tokens - n:], "dv")
+
+
+# tokens j of the poisoned rows: inside chunks of 64 and 128, at their ends, in a later sequence's first chunk
+POISON = [("f32", 64, 48), ("f32", 130, 72), ("bf16", 40, 13), ("bf16", 136, 24)]
+SPOTS = [(0,), (63,), (64, 200), (100,), (127,), (128, 131), (255,), (299,)]
+
+
+def poisoned(t, spots, head, col, value):
+    """t with `value` at (spot, head, col), and t with zeros there."""
+    bad, clean = t.clone(), t.clone()
+    for s in spots:
+        bad[s, head, col], clean[s, head, col] = value, 0
+    return bad, clean
+
+
+def attention_sums(q, k, v, decay, lengths, scale):
+    """o as sums over the earlier tokens, in float64 (each head its own key and value head)."""
+    out, first = [], 0
+    for n in lengths:
+        a, b, c = (t[first:first + n].double().transpose(0, 1) for t in (q, k, v))
+        i = torch.arange(n, device="cuda", dtype=torch.float64)
+        gap = i[:, None] - i
+        weigh = torch.where(gap >= 0, (decay.double()[:, None, None] * gap.clamp(min=0)).exp(), 0.0)
+        out.append((scale * ((a @ b.transpose(1, 2)) * weigh) @ c).transpose(0, 1))
+        first += n
+    return torch.cat(out)
+
+
+def check_spread(got, ref, hit, dtype, what):
+    """`hit`: what depends on a poisoned value.  It is not finite, everything else is right."""
+    fin = torch.isfinite(got)
+    assert (fin == ~hit).all(), (what, "lost", int((~fin & ~hit).sum()), "kept", int((fin & hit).sum()))
+    close(torch.where(hit, torch.zeros_like(got), got), torch.where(hit, torch.zeros_like(ref), ref), TOL[dtype], what)
+
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("dtype,dk,dv", POISON)
+def test_non_finite_values_do_not_go_back_in_time(dtype, dk, dv, value):
+    """An infinite or NaN query, key or value makes what depends on it non-finite, and nothing else."""
+    from tensoroperations_b200 import sequence
+    lengths, H, scale = [300, 90], 2, 0.2
+    T = sum(lengths)
+    q, k, v, _, cu = attention_inputs(dtype, lengths, H, H, dk, dv, seed=41)
+    decay = torch.tensor([-0.01, -0.3], device="cuda")
+    op = sequence.LinearAttention(dtype, H, H, dk, dv, scale=scale)
+    t = torch.arange(T, device="cuda")
+    none = torch.zeros(2, H, dk, dv, device="cuda")
+    for n, spots in enumerate(SPOTS):
+        h, c = n % H, (7 * n + 3) % min(dk, dv)
+        for name in "qkv":
+            x = dict(q=q, k=k, v=v)
+            bad, clean = poisoned(x[name], spots, h, c, value)
+            ref = attention_sums(**{**x, name: clean}, decay=decay, lengths=lengths, scale=scale)
+            o, left = torch.empty(T, H, dv, dtype=q.dtype, device="cuda"), torch.empty_like(none)
+            op.forward(**{**x, name: bad}, log_decay=decay, cu_seqlens=cu, o=o, state_out=left,
+                       workspace=scratch(op.workspace_bytes(T, 2)))
+            hit, shit = torch.zeros(T, H, dv, dtype=torch.bool, device="cuda"), torch.zeros_like(none, dtype=torch.bool)
+            after = (t >= spots[0]) & (t < lengths[0])
+            if name == "q":
+                hit[list(spots), h] = True
+            elif name == "k":
+                hit[after, h] = True
+                shit[0, h, c] = True
+            else:
+                hit[after, h, c] = True
+                shit[0, h, :, c] = True
+            check_spread(o, ref, hit, dtype, f"o, {name} at {spots}")
+            assert (torch.isfinite(left) == ~shit).all(), (name, spots)
+
+
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+@pytest.mark.parametrize("dtype,dk,dv", POISON)
+def test_non_finite_values_in_gradients(dtype, dk, dv, value):
+    """dq sees earlier keys and values, dk and dv later queries and outputs' gradients, no others."""
+    from tensoroperations_b200 import sequence
+    lengths, H, scale = [300, 90], 2, 0.2
+    T = sum(lengths)
+    q, k, v, _, cu = attention_inputs(dtype, lengths, H, H, dk, dv, seed=42)
+    do = normal(rng(43), (T, H, dv), dtype)
+    decay = torch.tensor([-0.01, -0.3], device="cuda")
+    op = sequence.LinearAttention(dtype, H, H, dk, dv, scale=scale)
+    t = torch.arange(T, device="cuda")
+    for n, spots in enumerate(SPOTS):
+        h, c = n % H, (7 * n + 3) % min(dk, dv)
+        for name in ("q", "k", "v", "do"):
+            x = dict(q=q, k=k, v=v, do=do)
+            bad, clean = poisoned(x[name], spots, h, c, value)
+            y = {m: a.double().requires_grad_() for m, a in {**x, name: clean}.items()}
+            ref = attention_sums(y["q"], y["k"], y["v"], decay, lengths, scale)
+            refs = torch.autograd.grad((ref * y["do"]).sum(), (y["q"], y["k"], y["v"]))
+            grads = [torch.empty(a.shape, dtype=a.dtype, device="cuda") for a in (q, k, v)]
+            y = {**x, name: bad}
+            op.backward(y["q"], y["k"], y["v"], decay, cu, y["do"], *grads,
+                        workspace=scratch(op.backward_workspace_bytes(T, 2)))
+            hit = [torch.zeros(a.shape, dtype=torch.bool, device="cuda") for a in (q, k, v)]
+            after, upto, at = (t >= spots[0]) & (t < lengths[0]), t <= spots[-1], list(spots)
+            if name == "q":
+                hit[1][upto, h, c] = True
+                hit[2][upto, h] = True
+            elif name == "k":
+                hit[0][after, h, c] = True
+                hit[2][at, h] = True
+            elif name == "v":
+                hit[0][after, h] = True
+                hit[1][at, h] = True
+            else:
+                hit[0][at, h] = True
+                hit[1][upto, h] = True
+                hit[2][upto, h, c] = True
+            for got, want, where, what in zip(grads, refs, hit, ("dq", "dk", "dv")):
+                check_spread(got, want, where, dtype, f"{what}, {name} at {spots}")
