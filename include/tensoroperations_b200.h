@@ -643,9 +643,8 @@ int to_qk_norm_rotary_backward(const to_qk_plan* plan, int64_t tokens, const to_
  * cores with f32 sums; states and their updates keep f32 accuracy.  Results take
  * one rounding to bf16 for the first 128 tokens of a sequence that nothing
  * enters (for dk and dv the last 128), the others one more of the products'
- * operands.  The chunked form multiplies masked pairs of a 128-token chunk by zero, so a
- * non-finite value in one token's row can reach earlier tokens of its own
- * chunk; it never reaches another sequence.
+ * operands.  A value that is not finite makes what depends on it not finite
+ * (NaN, it may be, where the recurrence has an infinity), and nothing else.
  *
  * Results do not depend on timing (every sum has a fixed order).  Calls on
  * different streams need workspaces of their own.

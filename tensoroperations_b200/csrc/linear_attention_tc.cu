@@ -33,7 +33,10 @@
 // no Sc and no O: both groups make planes, into two buffers in turn.  Rows past
 // a chunk's end are masked: P by selection, K and V by zeroing their rows, since
 // 0 * NaN is not 0.  Rows of a reversed chain keep their order in memory; only
-// the masks and decays turn round.
+// the masks and decays turn round.  For the same reason P V, where P is 0 for the tokens
+// that a row does not see, may meet nothing but finite values: warps 2 and 3 look through
+// V (a panel each) and, where they find others, note their tokens and take them out once U
+// has had them; the row warps then make the results that see them NaN.
 //
 // Measured on B200, 49152 tokens x 16 heads x 128: outputs 186 us (4.3 TB/s, 0.67 of
 // the copy rate), states 81 us (5.0 TB/s).  A chunk's outputs take about 7000
@@ -61,7 +64,7 @@ constexpr int kTile = 128;                       // tokens of a chunk, and the p
 constexpr uint32_t kPanel = kTile * 128;         // 128 rows of 64 values
 constexpr uint32_t kTileBytes = 2 * kPanel;      // 32 KB
 constexpr int kRowWarps = 8, kStateWarps = 8;    // P and out; planes and X
-constexpr int kFirstRow = 4, kFirstState = kFirstRow + kRowWarps;  // warps 0, 1: loads, products; 2, 3: none
+constexpr int kFirstRow = 4, kFirstState = kFirstRow + kRowWarps;  // warps 0, 1: loads, products; 2, 3: V
 constexpr int kThreads = 32 * (kFirstState + kStateWarps);
 constexpr uint32_t kMaxPolls = 1u << 22;
 constexpr int kMaxStages = 3;
@@ -89,10 +92,15 @@ struct Barriers {
   uint64_t full[kMaxStages], empty[kMaxStages];      // (Q and) K of a chunk
   uint64_t full_v[kMaxStages], empty_v[kMaxStages];  // its V
   // once a chunk each
-  uint64_t sc_full, p_ready, o1_full, o2_full, o_free;
+  uint64_t sc_full, p_ready, o1_full, o_free;
   uint64_t planes_ready, u_full, u_free, x_ready;
+  // a chunk's stage: V without what is not finite, and then P V; whether a panel had any, and the
+  // first token (in the chain's direction) of each column that had
+  uint64_t clean[2], o2_full[2];
+  int odd[2][2];
   uint32_t tmem;
   int abort;
+  alignas(16) int seen[2][kTile];
 };
 
 __device__ __forceinline__ bool wait_for(Barriers* b, uint64_t* bar, uint32_t parity) {
@@ -221,6 +229,15 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&x)[16]) {
       : "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t addr) {
+  uint32_t x;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;"
+               : "=r"(x) : "r"(addr) : "memory");
+  return x;
+}
+__device__ __forceinline__ void tmem_st1(uint32_t addr, uint32_t x) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(addr), "r"(x) : "memory");
+}
 __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
                ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
@@ -237,8 +254,18 @@ __device__ __forceinline__ uint4 lds4(uint32_t addr) {
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(addr));
   return x;
 }
+__device__ __forceinline__ void sts1(uint32_t addr, uint32_t a) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(a) : "memory");
+}
 __device__ __forceinline__ void sts4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// Two bf16, lo: bits 0-15: zero times each added to sum, which stays +0 while all are finite.
+__device__ __forceinline__ uint32_t add_zero_times(uint32_t x, uint32_t sum) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(sum));
+  return r;
 }
 
 // (lo, hi) as two bf16 in one register, lo in the low half
@@ -399,7 +426,7 @@ constexpr uint32_t kTables = kX + kTileBytes;
 constexpr uint32_t kBars = kTables + (kTable + kUpdTable) * 4;
 constexpr uint32_t kSmem = kBars + sizeof(Barriers);
 static_assert(Ring<true>::kStages * Ring<true>::kBytes <= kX && Ring<false>::kStages * Ring<false>::kBytes <= kX, "ring");
-static_assert(kBars % 8 == 0 && kSmem <= 232448, "shared memory of a CTA");
+static_assert(kBars % 16 == 0 && kSmem <= 232448, "shared memory of a CTA");
 
 // Registers: the launch gives each of the 20 warps 96; those that hold X take some of
 // the others' (4 * 64 + 8 * 88 + 8 * 120 = 1920 = 20 * 96).  No kernel may
@@ -451,12 +478,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar->sc_full, 1);
     mbar_init(&bar->p_ready, kRowWarps);
     mbar_init(&bar->o1_full, 1);
-    mbar_init(&bar->o2_full, 1);
     mbar_init(&bar->o_free, kRowWarps);
     mbar_init(&bar->planes_ready, kStateWarps + (STATES ? kRowWarps : 0));
     mbar_init(&bar->u_full, 1);
     mbar_init(&bar->u_free, kStateWarps);
     mbar_init(&bar->x_ready, kStateWarps);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar->clean[i], 2);
+      mbar_init(&bar->o2_full[i], 3);  // the product, and the warps whose notes on V the row warps read
+    }
     bar->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -540,7 +570,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             mma(tm + kColO, desc_k(sq, k), desc_mn(sx, k), kIdesc | kMnB, k > 0);
           commit(&bar->o1_full);
           commit(&bar->empty[i % kStages]);
-          if (!(ok = wait_for(bar, &bar->full_v[i % kStages], turn_of(i)) && wait_for(bar, &bar->p_ready, turn))) break;
+          // (clean: V has come, too)
+          if (!(ok = wait_for(bar, &bar->clean[i & 1], turn_of(i)) && wait_for(bar, &bar->p_ready, turn))) break;
           fence_after();
 #pragma unroll
           for (int k = 0; k < kTile / 16; ++k)
@@ -550,10 +581,60 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int k = 0; k < kTile / 16; ++k)
               mma_ts(tm + kColO, tm + kColS + k * 16 + 8, desc_mn(sv, k), kIdesc | kMnB, true);
           }
-          commit(&bar->o2_full);
+          commit(&bar->o2_full[i & 1]);
         }
         if (STATES) commit(&bar->empty_v[i % kStages]);
         else if (i + 1 < w.n) scores(i + 1);
+      }
+    } else if (!STATES && warp >= 2) {
+      // ---- V without what is not finite: columns [64 p, 64 p + 64) ----
+      const int p = warp - 2;
+      for (int i = 0; i < w.n; ++i) {
+        if (!(ok = warp_wait(bar, &bar->full_v[i % kStages], turn_of(i)))) break;
+        const uint32_t panel = stage_of(i) + R::kV + p * kPanel;
+        const int pieces = 8 * w.rows(i);  // of 16 bytes
+        uint32_t sum[4] = {0, 0, 0, 0};
+#pragma unroll 1
+        for (int e = lane; e < pieces; e += 32) {
+          const uint4 x = lds4(panel + 16 * e);
+          sum[0] = add_zero_times(x.x, sum[0]);
+          sum[1] = add_zero_times(x.y, sum[1]);
+          sum[2] = add_zero_times(x.z, sum[2]);
+          sum[3] = add_zero_times(x.w, sum[3]);
+        }
+        const bool odd = __any_sync(0xffffffffu, (sum[0] | sum[1] | sum[2] | sum[3]) != 0);
+        if (odd) {
+          // U reads V as it came.  (U of chunk i - 2 is done, since V of chunk i has come; U of chunk
+          // i + 1 comes after this chunk's P V: one wait after the other, no turn is missed.)
+          if (i < w.updates && !(ok = (i == 0 || warp_wait(bar, &bar->u_full, (i - 1) & 1)) &&
+                                      warp_wait(bar, &bar->u_full, i & 1)))
+            break;
+          int* seen = bar->seen[i & 1] + 64 * p;
+          seen[lane] = seen[lane + 32] = rev ? -1 : kTile;
+          __syncwarp();
+#pragma unroll 1
+          for (int e = lane; e < 4 * pieces; e += 32) {  // (rare: two values at a time)
+            const int row = e >> 5, col = 8 * ((e >> 2 ^ row) & 7) + 2 * (e & 3);
+            const uint32_t x = __float_as_uint(lds(panel + 4 * e));
+            uint32_t left = x;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint32_t exponent = 0x7f80u << 16 * k;
+              if ((x & exponent) != exponent) continue;
+              left &= 0xffff0000u >> 16 * k;
+              if (rev) atomicMax(seen + col + k, row);
+              else atomicMin(seen + col + k, row);
+            }
+            if (left != x) sts1(panel + 4 * e, left);
+          }
+          fence_async();
+        }
+        __syncwarp();
+        if (lane == 0) {
+          bar->odd[i & 1][p] = odd;
+          arrive(&bar->clean[i & 1]);
+          arrive(&bar->o2_full[i & 1]);
+        }
       }
     }
   } else if (warp < kFirstState) {
@@ -666,8 +747,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) arrive(&bar->p_ready);
         // results
-        if (!(ok = warp_wait(bar, &bar->o2_full, turn))) break;
+        if (!(ok = warp_wait(bar, &bar->o2_full[i & 1], turn_of(i)))) break;
         fence_after();
+        if (bar->odd[i & 1][h]) {  // NaN for the results that see what has been taken out of V (rare: least code)
+#pragma unroll 1
+          for (int j = 64 * h; j < 64 * h + 64; ++j) {
+            const uint32_t x = tmem_ld1(lanes + kColO + j);
+            const int at = bar->seen[i & 1][j];
+            tmem_st1(lanes + kColO + j, (rev ? at >= r : at <= r) ? 0x7fffffff : x);
+          }
+          tmem_st_wait();
+        }
         // through this warp's 4 KB of V's tile (its products are done), 128 bytes a row:
         // eight lanes then store a row's piece, instead of 32 rows at a time
         const uint32_t stage = stage_of(i) + R::kV + (warp - kFirstRow) * 4096;

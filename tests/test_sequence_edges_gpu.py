@@ -214,7 +214,8 @@ def test_first_tokens_do_not_depend_on_how_many_follow(tokens):
 
 
 # tokens j of the poisoned rows: inside chunks of 64 and 128, at their ends, in a later sequence's first chunk
-POISON = [("f32", 64, 48), ("f32", 130, 72), ("bf16", 40, 13), ("bf16", 136, 24)]
+POISON = [("f32", 64, 48), ("f32", 130, 72), ("bf16", 40, 13), ("bf16", 136, 24),
+          ("bf16", 128, 128), ("bf16", 64, 80), ("bf16", 40, 16)]
 SPOTS = [(0,), (63,), (64, 200), (100,), (127,), (128, 131), (255,), (299,)]
 
 
