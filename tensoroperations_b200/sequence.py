@@ -3,15 +3,15 @@ and linear attention with a decay for each head.
 
 Both are thin callers of the C ABI (to_qk_norm_rotary*, to_linear_attention*):
 an object holds what stays fixed (type, heads, widths), a call takes torch
-tensors and the stream to launch on (0: the default stream) and allocates
-nothing.  Rows are tensors [tokens, heads, width] whose last dimension is
+tensors and the stream to launch on (torch's current one where none is given;
+0: the default stream) and allocates nothing.  Rows are tensors [tokens, heads, width] whose last dimension is
 contiguous; they may be views into wider packed rows.  Shapes, types, devices
 and sizes are checked here, the rest by the library; a failed check raises
 before anything is launched (ValueError here, abi.ToError from the library).
 Outputs share no memory with what the call reads, but for q_out, k_out and
 state_out, which may be the inputs themselves.
 The caller orders the streams: a tensor written on another stream has to be
-ready on `stream`, and may be freed or overwritten only after it.
+ready on the call's, and may be freed or overwritten only after it.
 """
 from __future__ import annotations
 
@@ -85,6 +85,10 @@ def _cuda(t, name: str):
     return t.device
 
 
+def _on(stream: Optional[int], device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
+
+
 def _scratch(t, need: int, device):
     """(pointer, bytes) of a workspace; none is needed where `need` is 0."""
     if t is None:
@@ -138,7 +142,7 @@ class QkNormRotary:
         shape = (self.head_dim,)
         return (pos, _flat(wq, "wq", torch.float32, shape, device), _flat(wk, "wk", torch.float32, shape, device))
 
-    def forward(self, q, k, positions, wq, wk, q_out, k_out, stream: int = 0):
+    def forward(self, q, k, positions, wq, wk, q_out, k_out, stream: Optional[int] = None):
         """q_out, k_out <- the normed, weighted and rotated q, k (in place where they are q, k).
 
         positions: int32 [axes, tokens]; wq, wk: f32 [head_dim] or None.
@@ -147,7 +151,7 @@ class QkNormRotary:
         i = self._pair(q, k, ("q", "k"), tokens, device)
         o = self._pair(q_out, k_out, ("q_out", "k_out"), tokens, device)
         st = abi.lib.to_qk_norm_rotary(self._h, tokens, *i, *self._fixed(positions, wq, wk, tokens, device), *o,
-                                       stream)
+                                       _on(stream, device))
         if st:
             abi.check(st, "to_qk_norm_rotary")
 
@@ -155,7 +159,7 @@ class QkNormRotary:
         """Bytes of `workspace` that backward() needs."""
         return abi.lib.to_qk_norm_rotary_workspace_bytes(self._h, tokens)
 
-    def backward(self, q, k, positions, wq, wk, gq, gk, dq, dk, dwq, dwk, workspace, stream: int = 0):
+    def backward(self, q, k, positions, wq, wk, gq, gk, dq, dk, dwq, dwk, workspace, stream: Optional[int] = None):
         """dq, dk, dwq, dwk <- gradients from gq, gk (those of q_out, k_out); q, k are forward()'s inputs."""
         tokens, device, shape = q.shape[0], _cuda(q, "q"), (self.head_dim,)
         i = self._pair(q, k, ("q", "k"), tokens, device)
@@ -164,7 +168,7 @@ class QkNormRotary:
         dw = _flat(dwq, "dwq", torch.float32, shape, device), _flat(dwk, "dwk", torch.float32, shape, device)
         abi.check(abi.lib.to_qk_norm_rotary_backward(self._h, tokens, *i,
                                                      *self._fixed(positions, wq, wk, tokens, device), *g, *o, *dw,
-                                                     *_scratch(workspace, 1, device), stream),
+                                                     *_scratch(workspace, 1, device), _on(stream, device)),
                   "to_qk_norm_rotary_backward")
 
 
@@ -215,7 +219,7 @@ class LinearAttention:
         return _flat(_needed(log_decay, "log_decay"), "log_decay", torch.float32, (self.q_heads,), device)
 
     def forward(self, q, k, v, log_decay, cu_seqlens, o, state_in=None, state_out=None, slots=None, workspace=None,
-                stream: int = 0):
+                stream: Optional[int] = None):
         """o <- the outputs of packed sequences; state_out (may be state_in) <- the states they leave.
 
         cu_seqlens: int32 [sequences + 1], on the device.  slots: int32
@@ -234,11 +238,11 @@ class LinearAttention:
             self._decay(log_decay, device), cu, _flat(slots, "slots", torch.int32, (n,), device),
             self._state(state_in, "state_in", device, have), self._state(state_out, "state_out", device, have),
             *_scratch(workspace, abi.lib.to_linear_attention_workspace_bytes(desc), device))
-        st = abi.lib.to_linear_attention(desc, args, stream)
+        st = abi.lib.to_linear_attention(desc, args, _on(stream, device))
         if st:
             abi.check(st, "to_linear_attention")
 
-    def step(self, q, k, v, log_decay, state, o, slots=None, stream: int = 0):
+    def step(self, q, k, v, log_decay, state, o, slots=None, stream: Optional[int] = None):
         """One token of each request: its state is updated in place, o <- its output."""
         tokens, device, have = q.shape[0], _cuda(q, "q"), state.shape[0]
         if slots is None and have < tokens:
@@ -249,12 +253,12 @@ class LinearAttention:
                                            (o, "o", True, dv))),
             self._decay(log_decay, device), 0, _flat(slots, "slots", torch.int32, (tokens,), device), 0,
             self._state(state, "state", device, have), 0, 0)
-        st = abi.lib.to_linear_attention_step(self._desc(tokens, 0, have), args, stream)
+        st = abi.lib.to_linear_attention_step(self._desc(tokens, 0, have), args, _on(stream, device))
         if st:
             abi.check(st, "to_linear_attention_step")
 
     def backward(self, q, k, v, log_decay, cu_seqlens, do, dq, dk, dv, state_in=None, dstate_out=None,
-                 dstate_in=None, workspace=None, stream: int = 0):
+                 dstate_in=None, workspace=None, stream: Optional[int] = None):
         """dq, dk, dv (and dstate_in) <- gradients of forward() from do and dstate_out.
 
         State tensors hold one state a sequence, in order.  log_decay gets no gradient.
@@ -269,6 +273,6 @@ class LinearAttention:
             self._decay(log_decay, device), cu, self._state(state_in, "state_in", device, n),
             self._state(dstate_out, "dstate_out", device, n), self._state(dstate_in, "dstate_in", device, n),
             *_scratch(workspace, abi.lib.to_linear_attention_backward_workspace_bytes(desc), device))
-        st = abi.lib.to_linear_attention_backward(desc, args, stream)
+        st = abi.lib.to_linear_attention_backward(desc, args, _on(stream, device))
         if st:
             abi.check(st, "to_linear_attention_backward")

@@ -1,6 +1,6 @@
 """The sequence operators at the edges of their ranges, against definitions in float64:
 heads split over warps, rows without a length, rows of no sequence, sequences that end in
-silence, first tokens, infinities and NaN.
+silence, first tokens, infinities and NaN, streams.
 
 Tolerances are those of test_sequence_gpu (derived there from the types alone) unless a
 test says otherwise.
@@ -323,3 +323,57 @@ def test_non_finite_values_in_gradients(dtype, dk, dv, value):
                 hit[2][upto, h, c] = True
             for got, want, where, what in zip(grads, refs, hit, ("dq", "dk", "dv")):
                 check_spread(got, want, where, dtype, f"{what}, {name} at {spots}")
+
+
+# ---- streams and autograd ---------------------------------------------------------------
+
+
+def every_call(stream=None):
+    """The five calls on small tensors: (what they write, the call) each; `stream` as in the calls."""
+    from tensoroperations_b200 import sequence
+    T, H, d = 200, 2, 64
+    q, k, v, decay, cu = attention_inputs("bf16", [T], H, H, d, d, seed=61)
+    more = {} if stream is None else dict(stream=stream)
+    pos = torch.arange(T, dtype=torch.int32, device="cuda").view(1, T)
+    qk, la = sequence.QkNormRotary("bf16", H, H, d), sequence.LinearAttention("bf16", H, H, d, d)
+    w = [torch.ones(d, device="cuda") for _ in range(4)]
+    out = lambda: torch.zeros(T, H, d, dtype=q.dtype, device="cuda")  # noqa: E731
+    ws = scratch(max(qk.workspace_bytes(T), la.workspace_bytes(T, 1), la.backward_workspace_bytes(T, 1), 256))
+    a, b, c, o, g = out(), out(), out(), out(), normal(rng(62), (T, H, d), "bf16")
+    state, left = torch.zeros(T, H, d, d, device="cuda"), torch.zeros(1, H, d, d, device="cuda")
+    first, second = out(), out()
+    yield (a, b), lambda: qk.forward(q, k, pos, w[0], w[1], a, b, **more)
+    yield (first, second, w[2], w[3]), lambda: qk.backward(q, k, pos, w[0], w[1], g, g, first, second, w[2], w[3], ws,
+                                                           **more)
+    yield (o, left), lambda: la.forward(q, k, v, decay, cu, o, state_out=left, workspace=ws, **more)
+    o1 = out()
+    yield (o1, state), lambda: la.step(q, k, v, decay, state, o1, **more)
+    dq, dk, dS = out(), out(), torch.zeros_like(left)
+    yield (dq, dk, c, dS), lambda: la.backward(q, k, v, decay, cu, g, dq, dk, c, dstate_out=left, dstate_in=dS,
+                                               workspace=ws, **more)
+
+
+def test_calls_run_on_the_current_stream():
+    """Without a stream a call runs on torch's current one, as what torch does to its tensors."""
+    for written, call in every_call():
+        before = [t.clone() for t in written]
+        side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):  # (a launch on any other stream is not recorded)
+            call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, b) for t, b in zip(written, before))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not any(torch.equal(t, b) for t, b in zip(written, before))
+
+
+def test_stream_zero_is_the_default_stream():
+    want = []
+    for written, call in every_call():
+        call()
+        want.append([t.clone() for t in written])
+    for (written, call), ref in zip(every_call(stream=0), want):
+        call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(t, r) for t, r in zip(written, ref))
