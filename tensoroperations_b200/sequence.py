@@ -10,6 +10,8 @@ and sizes are checked here, the rest by the library; a failed check raises
 before anything is launched (ValueError here, abi.ToError from the library).
 Outputs share no memory with what the call reads, but for q_out, k_out and
 state_out, which may be the inputs themselves.
+No call records a graph for autograd; a torch.autograd.Function around forward
+and backward does.  Autograd is told what a call has written.
 The caller orders the streams: a tensor written on another stream has to be
 ready on the call's, and may be freed or overwritten only after it.
 """
@@ -21,6 +23,7 @@ import struct
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd.graph import increment_version  # tells autograd that a saved tensor has changed
 
 from . import abi
 
@@ -154,6 +157,7 @@ class QkNormRotary:
                                        _on(stream, device))
         if st:
             abi.check(st, "to_qk_norm_rotary")
+        increment_version((q_out, k_out))
 
     def workspace_bytes(self, tokens: int) -> int:
         """Bytes of `workspace` that backward() needs."""
@@ -170,6 +174,7 @@ class QkNormRotary:
                                                      *self._fixed(positions, wq, wk, tokens, device), *g, *o, *dw,
                                                      *_scratch(workspace, 1, device), _on(stream, device)),
                   "to_qk_norm_rotary_backward")
+        increment_version([t for t in (dq, dk, dwq, dwk) if t is not None])
 
 
 class LinearAttention:
@@ -241,6 +246,7 @@ class LinearAttention:
         st = abi.lib.to_linear_attention(desc, args, _on(stream, device))
         if st:
             abi.check(st, "to_linear_attention")
+        increment_version((o,) if state_out is None else (o, state_out))
 
     def step(self, q, k, v, log_decay, state, o, slots=None, stream: Optional[int] = None):
         """One token of each request: its state is updated in place, o <- its output."""
@@ -256,6 +262,7 @@ class LinearAttention:
         st = abi.lib.to_linear_attention_step(self._desc(tokens, 0, have), args, _on(stream, device))
         if st:
             abi.check(st, "to_linear_attention_step")
+        increment_version((o, state))
 
     def backward(self, q, k, v, log_decay, cu_seqlens, do, dq, dk, dv, state_in=None, dstate_out=None,
                  dstate_in=None, workspace=None, stream: Optional[int] = None):
@@ -276,3 +283,4 @@ class LinearAttention:
         st = abi.lib.to_linear_attention_backward(desc, args, _on(stream, device))
         if st:
             abi.check(st, "to_linear_attention_backward")
+        increment_version((dq, dk, dv) if dstate_in is None else (dq, dk, dv, dstate_in))

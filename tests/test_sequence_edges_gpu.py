@@ -1,6 +1,6 @@
 """The sequence operators at the edges of their ranges, against definitions in float64:
 heads split over warps, rows without a length, rows of no sequence, sequences that end in
-silence, first tokens, infinities and NaN, streams.
+silence, first tokens, infinities and NaN, streams, autograd.
 
 Tolerances are those of test_sequence_gpu (derived there from the types alone) unless a
 test says otherwise.
@@ -377,3 +377,28 @@ def test_stream_zero_is_the_default_stream():
         call()
         torch.cuda.synchronize()
         assert all(torch.equal(t, r) for t, r in zip(written, ref))
+
+
+# ---- autograd: what is written is known to be
+
+
+def test_written_tensors_are_known_to_autograd():
+    """A tensor that autograd has saved and a call overwrites is an error in the backward pass, not a
+    wrong gradient; what a call reads stays as it was."""
+    for written, call in every_call():
+        x = [torch.ones(t.shape, device="cuda", requires_grad=True) for t in written]
+        y = [a * t for a, t in zip(x, written)]  # saves t
+        before = [t._version for t in written]
+        call()
+        assert all(t._version > b for t, b in zip(written, before))
+        for out in y:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                out.sum().backward()
+    q, k, v, decay, cu = attention_inputs("bf16", [50], 2, 2, 64, 64)
+    from tensoroperations_b200 import sequence
+    op, o, S = sequence.LinearAttention("bf16", 2, 2, 64, 64), torch.empty_like(q), torch.zeros(1, 2, 64, 64, device="cuda")
+    before = [t._version for t in (q, k, v, decay, cu, S)]
+    op.forward(q, k, v, decay, cu, o, state_in=S)
+    assert [t._version for t in (q, k, v, decay, cu, S)] == before
+    with torch.inference_mode():  # tensors without versions
+        op.forward(q, k, v, decay, cu, torch.empty_like(q), state_in=S)
