@@ -45,6 +45,13 @@ def _dtype(dtype) -> torch.dtype:
     return kind
 
 
+def _sizes(**sizes):
+    """Sizes that the descriptors hold (32-bit fields, which would cut longer ones short)."""
+    for name, n in sizes.items():
+        if not -2**31 <= n < 2**31:
+            raise ValueError(f"{name} {n} does not fit 32 bits")
+
+
 def _rows(t, name: str, dtype: torch.dtype, shape, device):
     """(data, token stride, head stride) of rows, as in to_rows."""
     if t.shape != shape or t.dtype != dtype or t.device != device:
@@ -121,6 +128,8 @@ class QkNormRotary:
         if not 1 <= len(sections) <= 4:
             raise ValueError(f"{len(sections)} axes: 1 to 4 are supported")
         self.axes = len(sections)
+        _sizes(q_heads=q_heads, k_heads=k_heads, head_dim=head_dim, rotary_dim=self.rotary_dim,
+               section=max(sections, key=abs))
         d = abi.QkDesc(DTYPES[self.dtype], q_heads, k_heads, head_dim, self.rotary_dim, self.axes)
         d.section[:self.axes] = sections
         d.interleaved, d.theta, d.eps = int(bool(interleaved)), theta, eps
@@ -190,7 +199,8 @@ class LinearAttention:
                  scale: Optional[float] = None):
         self.dtype = _dtype(dtype)
         self.q_heads, self.kv_heads, self.key_dim, self.value_dim = q_heads, kv_heads, key_dim, value_dim
-        self.scale = 1.0 / math.sqrt(key_dim) if scale is None else scale
+        _sizes(q_heads=q_heads, kv_heads=kv_heads, key_dim=key_dim, value_dim=value_dim)
+        self.scale = 1.0 / math.sqrt(max(key_dim, 1)) if scale is None else scale  # (widths below 1 are refused)
         abi.check(abi.lib.to_linear_attention(self._desc(0, 0), bytes(_ARGS.size), 0), "LinearAttention")
 
     def _desc(self, tokens: int, nseq: int, slots: int = 0) -> bytes:

@@ -109,3 +109,22 @@ def test_norm_and_rotation_outputs(backward):
                 assert refused(status(**{out: rows(at + 2 * D, HQ)}), out, other)
                 assert refused(status(**{out: (at, 2 * HQ * D, D)}), out, other)  # other strides
         assert refused(status(**{out: (AT[7], D, D)}), out)
+
+
+@pytest.mark.parametrize("bad", [dict(q_heads=2**32 + 4), dict(k_heads=2**32), dict(head_dim=2**32 + 64),
+                                 dict(rotary_dim=2**32 + 64), dict(sections=[2**32 + 32]), dict(q_heads=-2**32 + 4)])
+def test_sizes_past_32_bits_are_not_cut_short(bad):
+    args = dict(dtype="bf16", q_heads=4, k_heads=2, head_dim=64)
+    args.update(bad)
+    with pytest.raises((ValueError, abi.ToError)):
+        sequence.QkNormRotary(**args)
+    args = {n: v for n, v in args.items() if n in ("dtype", "q_heads")}
+    if "q_heads" in bad:
+        with pytest.raises((ValueError, abi.ToError)):
+            sequence.LinearAttention(**args, kv_heads=2, key_dim=64, value_dim=64)
+
+
+@pytest.mark.parametrize("key_dim", [0, -4, 2**32 + 64])
+def test_key_widths_are_refused_before_their_root_is_taken(key_dim):
+    with pytest.raises((ValueError, abi.ToError)):
+        sequence.LinearAttention("f32", 4, 2, key_dim, 32)
