@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
           const int x = tx * VC + c;
           const float v = fmaf(f, w[r][c], o[r][c]);
           if (x >= ncols) continue;
-          if (C.out_f32) seq::row_ptr<float>(C.out, token, head / C.out_div)[col0 + x] = v;
-          else seq::row_ptr<T>(C.out, token, head / C.out_div)[col0 + x] = seq::from_f32<T>(v);
+          if (C.out_f32) seq::row_ptr<float>(C.out, token, head)[col0 + x] = v;
+          else seq::row_ptr<T>(C.out, token, head)[col0 + x] = seq::from_f32<T>(v);
         }
       }
       __syncthreads();  // X has been read
@@ -254,17 +254,15 @@ __global__ void __launch_bounds__(kThreads) chain_simt_kernel(const __grid_const
   }
   __syncthreads();
   float* dst = nullptr;
-  int dst_t = 0;
   if (STATES) {
     dst = C.seg_state + (static_cast<long long>(blockIdx.x) * C.heads + head) * C.db * C.dc;
   } else if (C.fin && slot >= 0 && g.idx == g.count - 1) {
     dst = C.fin + (slot * C.heads + head) * C.db * C.dc;
-    dst_t = C.fin_t;
   }
   if (dst)
     for (int e = tid; e < C.db * DCB; e += kThreads) {
       const int b = e / DCB, c = e - b * DCB;
-      if (c < ncols) dst[lin::state_index(C, dst_t, b, col0 + c)] = X[b * kColPad + c];
+      if (c < ncols) dst[lin::state_index(C, 0, b, col0 + c)] = X[b * kColPad + c];
     }
 }
 
@@ -605,7 +603,7 @@ Chain base_chain(const to_linear_attention_desc& d, const int32_t* cu, const flo
   C.tokens = static_cast<int>(d.tokens);
   C.cu = cu;
   C.log_decay = log_decay;
-  C.a_div = C.b_div = C.c_div = C.out_div = 1;
+  C.a_div = C.b_div = C.c_div = 1;
   return C;
 }
 

@@ -31,7 +31,7 @@ using seq::Rows;
 
 struct Chain {
   Rows a, b, c, out;
-  int a_div, b_div, c_div, out_div;  // head h reads head h / div
+  int a_div, b_div, c_div;  // head h reads head h / div
   int heads, nseq;
   int db, dc;  // widths of b (and a) and of c (and out)
   int tokens;
@@ -39,11 +39,11 @@ struct Chain {
   const float* log_decay;
   float intra, inter, upd;
   int rev;
-  // entering and leaving X of whole sequences: [slot][heads] matrices [db][dc],
-  // or [dc][db] when transposed
+  // entering and leaving X of whole sequences: [slot][heads] matrices [db][dc]
+  // (the entering one [dc][db] when init_t)
   const float* init;
   float* fin;
-  int init_t, fin_t;
+  int init_t;
   const int32_t* slots;
   long long num_slots;
   float* seg_state;  // [segment slots][heads][db][dc]; null: one segment a sequence

@@ -369,7 +369,7 @@ __device__ __forceinline__ void make_planes(uint32_t tile, uint32_t lanes, uint3
 }
 
 // X of a warp (lane: a row, 64 columns from column `col` on) from or to rows row0 ..
-// of a [db][dc] matrix, dc a multiple of 4: through 2.5 KB of shared memory, 16
+// of a [db][dc] matrix (dc a multiple of 4, as tc_takes asks): through 2.5 KB of shared memory, 16
 // columns at a time, so that four lanes take 64 bytes of one row.  (32 lanes in 32
 // rows held up the load-store unit, and the other warps' shared loads behind it.)
 __device__ __forceinline__ void load_state(float (&X)[64], const float* m, uint32_t stage, int row0, int col, int db,
@@ -762,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // eight lanes then store a row's piece, instead of 32 rows at a time
         const uint32_t stage = stage_of(i) + R::kV + (warp - kFirstRow) * 4096;
         const int piece = lane & 7, row0 = 32 * q + (lane >> 3);
-        const long long first = (w.first(C, i) + row0) * pitch + w.head / C.out_div * C.out.hs + h * 64;
+        const long long first = (w.first(C, i) + row0) * pitch + w.head * C.out.hs + h * 64;
         const bool f32 = C.out_f32;
         float y[2][32];
         tmem_ld32(lanes + kColO + h * 64, y[0]);
@@ -830,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           src_t = C.init_t;
         }
       }
-      if (src && !src_t && C.dc % 4 == 0) {
+      if (src && !src_t) {
         load_state(X, src, own_x, 32 * q, 64 * h, C.db, C.dc, lane);
       } else {
 #pragma unroll
@@ -909,24 +909,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     float* dst = nullptr;
-    int dst_t = 0;
     if (STATES) {
       dst = C.seg_state + static_cast<long long>(item) * C.db * C.dc;
     } else if (C.fin && w.last) {
       const long long slot = lin::state_slot(C, w.seq);
       if (slot >= 0) dst = C.fin + (slot * C.heads + w.head) * C.db * C.dc;
-      dst_t = C.fin_t;
     }
     if (!STATES && ok && dst && w.n > 0) ok = warp_wait(bar, &bar->o1_full, (w.n - 1) & 1);  // bf16 X has been read
-    if (ok && dst) {
-      if (!dst_t && C.dc % 4 == 0) {
-        store_state(X, dst, own_x, 32 * q, 64 * h, C.db, C.dc, lane);
-      } else if (b < C.db) {
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (h * 64 + c < C.dc) dst[lin::state_index(C, dst_t, b, h * 64 + c)] = X[c];
-      }
-    }
+    if (ok && dst) store_state(X, dst, own_x, 32 * q, 64 * h, C.db, C.dc, lane);
   }
   __syncwarp();
   fence_before();
