@@ -422,7 +422,9 @@ int launch(QkArgs& A, const to_qk_desc& d, bool backward, int sms, cudaStream_t 
   if (backward) {
     const QkGrid g = backward_grid(d, A.tokens, sms);
     A.q_ctas = g.q;
-    qk_kernel<T, VP, UPL, SHARE, VP == 4 ? 2 : 1, true><<<g.q + g.k, 32 * kWarps, size_t(kWarps) * A.dim * sizeof(float), s>>>(A);
+    if constexpr (VP < 8)  // (gradients take four pairs at most)
+      qk_kernel<T, VP, UPL, SHARE, VP == 4 ? 2 : 1, true>
+          <<<g.q + g.k, 32 * kWarps, size_t(kWarps) * A.dim * sizeof(float), s>>>(A);
   } else {
     // eight CTAs an SM: a warp takes several tokens (its weights are read once, and the next
     // token's rows while it works), and the last ones still even out (72 us with 32, 87 with 2,
