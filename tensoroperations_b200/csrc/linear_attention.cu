@@ -22,7 +22,7 @@ constexpr int kMaxDim = 256;
 // in f32 in shared memory, 4 x 4 results a thread.  At most 128 flops come
 // from 8 16-byte shared loads, so the shared-memory pipe bounds it at about
 // half of the f32 rate.  Measured on B200: 2500 tokens x 12 heads x 64 f32 in
-// 78 us with its states' launch and scan (52 us the outputs).  Each segment is
+// 74 us with its states' launch and scan (49 us the outputs).  Each segment is
 // cut to about two chunks there, and waiting for rows, shared memory and the
 // other warps takes as long as the sums.
 constexpr int kRows = 64;  // tokens of a chunk
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(256) group_sum_kernel(const __grid_constant__ 
 // Memory bound: the state is read and written once, 8 bytes a value, for 4
 // flops.  A CTA takes `cols` columns of one request's head; a lane holds VEC
 // consecutive columns and walks the rows of the state, kUnroll of them in flight.
-// Measured on B200: 192 requests x 32 heads x 128 x 128 in 130 us, 6.2 TB/s (0.96
+// Measured on B200: 192 requests x 32 heads x 128 x 128 in 129 us, 6.3 TB/s (0.97
 // of the copy rate).
 struct StepArgs {
   Rows q, k, v, o;

@@ -7,29 +7,28 @@
 //   Sc = Q K^T                    P = Sc masked, decayed and scaled, bf16, in TMEM
 //   O  = Q X (bf16 X), its rows scaled in TMEM by inter l^(..), then O += P V
 //   U  = (decayed K)^T V          X = l^n X + U (f32, in registers)
-// all M = N = 128.  Five or six products of 128^3 a chunk, 2560 or 3072 tensor
-// cycles at the dense bf16 rate, against about 5600 for the chunk's 128 KB at
-// this SM's share of the HBM.  A product of two shared operands of this size
-// takes all of the shared memory's 128 bytes a cycle, so P and decayed K are
-// TMEM operands (K transposed into its lanes by ldmatrix).
+// all M = N = 128.  Five or six products of 128^3 a chunk (one more in a sequence's
+// first), 2560 or 3072 tensor cycles at the dense bf16 rate, against about 5600 for
+// the chunk's 128 KB at this SM's share of the HBM.  A product of two shared operands
+// of this size takes all of the shared memory's 128 bytes a cycle, so P and decayed K
+// are TMEM operands (K transposed into its lanes by ldmatrix).
 //
 // Precision: P and X each enter their product with one bf16 rounding, as the
-// result's own.  In the chain's first chunk of a sequence a row has few P and nothing
-// else, whose errors do not average out: there P has a second plane, so those tokens'
-// results are rounded once, whatever follows them.  The state stays f32: decayed K is split into bf16 planes of 8
-// bits each -- three, which reach f32, where the sequence's state is a result, two where
-// only products read it -- smallest plane first, so few sums pass through the
-// accumulator at full size; a chunk's U is added to X in IEEE f32 registers.  (Two planes
-// for chunks that have decayed far by the sequence's end are not enough: the tokens after
-// them may weigh nothing.)
+// result's own.  In the chain's first chunk of a sequence a row has few P and, where no
+// state enters, nothing else, so that their errors do not average out: there P has a
+// second plane, and the result of such a token is rounded once, whatever follows it.
+// The state stays f32: decayed K is split into bf16 planes of 8 bits each -- three, which
+// reach f32, where the sequence's state is a result, two where only products read it --
+// smallest plane first, so few sums pass through the accumulator at full size; a chunk's
+// U is added to X in IEEE f32 registers.  (Two planes for chunks that have decayed far by
+// the sequence's end are not enough: the tokens after them may weigh nothing.)
 //
 // Roles (20 warps): one lane issues TMA loads, two chunks ahead, one the
 // products; warps 4-11 turn Sc into P, scale O and store the results (a thread:
 // one row, 64 columns); warps 12-19 make the planes and hold X (a thread: one row, 64
 // columns).  Plane 2 lies in O's columns between one chunk's results and the
-// next one's.  Products are issued U, Q X,
-// P V and the next chunk's Sc: the row warps store results and make the next P
-// while the state warps make the next planes.  In the states' launch there is
+// next one's.  Products are issued U, Q X, P V and the next chunk's Sc: the row warps
+// store results and make the next P while the state warps make the next planes.  In the states' launch there is
 // no Sc and no O: both groups make planes, into two buffers in turn.  Rows past
 // a chunk's end are masked: P by selection, K and V by zeroing their rows, since
 // 0 * NaN is not 0.  Rows of a reversed chain keep their order in memory; only
@@ -38,10 +37,11 @@
 // V (a panel each) and, where they find others, note their tokens and take them out once U
 // has had them; the row warps then make the results that see them NaN.
 //
-// Measured on B200, 49152 tokens x 16 heads x 128: outputs 186 us (4.3 TB/s, 0.67 of
-// the copy rate), states 81 us (5.0 TB/s).  A chunk's outputs take about 7000
-// cycles: Q X, the scaling, P V, Sc and U wait for one another, and products with
-// two shared operands take about 110 cycles each instead of 64.
+// Measured on B200, 49152 tokens x 16 heads x 128: outputs 197 to 204 us (4.0 TB/s, 0.61 of
+// the copy rate), states 89 to 91 us (4.5 TB/s), each by itself; a call with the scan of 7 us
+// 302 us, 350 us back to back on a hot card.  A chunk's outputs take about 7000 cycles:
+// Q X, the scaling, P V, Sc and U wait for one another, and products with two shared
+// operands take about 110 cycles each instead of 64.
 //
 // Every wait is bounded; on a timeout the kernel records TO_ERR_TIMEOUT in the
 // device status word, waits (bounded) for its copies in flight, frees its TMEM

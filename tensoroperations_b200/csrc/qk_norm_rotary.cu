@@ -14,10 +14,10 @@
 // the next rows are on their way while it works (without that, 112 us for the
 // first figure).
 //
-// Measured on B200: 16384 tokens x 40 heads x 128 bf16 in 65 us, 5.2 TB/s (0.80
-// of the copy rate); 6137 x 24 x 96 f32, three axes, 27 us, 4.2 TB/s; gradients of
-// 8192 x 40 x 128 bf16 in 68 us and 6 us for the weights' sums, 3.4 TB/s: two
-// sums over a row one after the other, which sixteen warps an SM do not hide.
+// Measured on B200: 16384 tokens x 40 heads x 128 bf16 in 65.6 us, 5.1 TB/s (0.79
+// of the copy rate); 6137 x 24 x 96 f32, three axes, 26 us, 4.4 TB/s; gradients of
+// 8192 x 40 x 128 bf16 in 69 us and 6 us for the weights' sums, 3.4 TB/s: two
+// sums over a row, taken one after the other, which sixteen warps an SM do not hide.
 //
 // Angles: a pair's frequency is a 64-bit fixed-point number of turns F =
 // theta^(-2j/R) / 2 pi * 2^64, so position * F modulo 2^64 is the angle's
