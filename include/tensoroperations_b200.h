@@ -710,6 +710,200 @@ int to_linear_attention_backward(const to_linear_attention_desc* desc,
 int to_linear_attention_step(const to_linear_attention_desc* desc,
                              const to_linear_attention_args* args, void* stream);
 
+/* ---------------------------------------------------------------------- */
+/* Rows kept in 8 bits                                                     */
+/* ---------------------------------------------------------------------- */
+/*
+ * [tokens][width] values as int8 codes and one scale byte for every 32
+ * neighbouring values (the last group of a row may be shorter):
+ *   value = code * 2^(scale - 127),
+ * the scale the least power of two with |x| <= 127 * 2^(scale - 127) in the
+ * group (not below 2^-127), code = x / 2^(scale - 127) rounded to the nearest
+ * integer, ties to even.  Both steps are exact but for that one rounding (of
+ * at most half a scale, 1/127 of the group's largest |x|): codes do not depend on
+ * how they were computed.  A group that holds an infinity or a NaN has the scale byte 255 and
+ * reads as NaN.  Strides count elements (bytes) from token to token.
+ */
+typedef struct to_rows8 {
+  void* codes;  /* int8  [tokens][width]                                     */
+  void* scales; /* uint8 [tokens][(width + 31) / 32]                         */
+  int64_t code_stride;
+  int64_t scale_stride;
+} to_rows8;
+
+/* x (rows of one head, head_stride not used) into 8 bits, and back: x = the value. */
+int to_rows8_pack(int32_t dtype, int32_t width, int64_t tokens, const to_rows* x,
+                  const to_rows8* out, void* stream);
+int to_rows8_unpack(int32_t dtype, int32_t width, int64_t tokens, const to_rows8* in,
+                    const to_rows* x, void* stream);
+
+/* ---------------------------------------------------------------------- */
+/* Gated linear recurrence                                                 */
+/* ---------------------------------------------------------------------- */
+/*
+ * For every channel c of a sequence, t = 0 .. L-1:
+ *   a_t = sigmoid(f_t + bias_c)
+ *   h_t = a_t h_{t-1} + (1 - a_t) x_t     (complement = 1)
+ *   h_t = a_t h_{t-1} + x_t               (complement = 0)
+ * x, f, h: rows [tokens][channels] (one head: head_stride is not used).  bias:
+ * device f32 [channels], NULL for 0.  h_{-1} is the entering state (state_in,
+ * zero when NULL); h_{L-1}, before its rounding, is written to state_out (when
+ * not NULL).  a and 1 - a keep f32 accuracy relative to themselves; the
+ * recurrence is f32 throughout, h takes one rounding.
+ *
+ * Sequences are packed as in to_linear_attention, and so are the rules for
+ * cu_seqlens, lengths 0 and 1, rows of no sequence, slots (states are f32
+ * [slots][channels], 16-byte aligned) and values that are not finite.
+ *
+ * For the gradients the call writes, when `saved` is not NULL, the state that
+ * enters each TO_RECURRENCE_SEGMENT tokens of every sequence (f32
+ * [to_gated_recurrence_saved_rows][channels], 16-byte aligned), and, where
+ * keep_x / keep_f have codes, x and f in 8 bits.
+ *
+ * h may share no memory with x or f, nor any output with another one or with
+ * what the call reads, but state_out, which may be state_in.
+ * Results do not depend on timing (every sum has a fixed order).  channels 1 ..
+ * 65536.  Calls that overlap need workspaces of their own.
+ */
+#define TO_RECURRENCE_SEGMENT 128
+
+typedef struct to_gated_recurrence_desc {
+  int32_t dtype;
+  int32_t channels;
+  int32_t nseq;       /* >= 0                                                */
+  int32_t complement; /* 0 or 1                                              */
+  int64_t tokens;     /* rows of x, f, h; < 2^31                             */
+  int64_t num_slots;  /* slots of state_in / state_out (slots NULL: nseq)    */
+} to_gated_recurrence_desc;
+
+typedef struct to_gated_recurrence_args {
+  to_rows x, f, h;
+  to_rows8 keep_x, keep_f; /* codes NULL: not kept                           */
+  const float* bias;
+  const int32_t* cu_seqlens;
+  const int32_t* slots;
+  const float* state_in;
+  float* state_out;
+  float* saved;
+  void* workspace; /* device, 256-byte aligned                               */
+  size_t workspace_bytes;
+} to_gated_recurrence_args;
+
+/* Rows of `saved`, and bytes of the workspace (0: none), of a call of this size. */
+int64_t to_gated_recurrence_saved_rows(const to_gated_recurrence_desc* desc);
+size_t to_gated_recurrence_workspace_bytes(const to_gated_recurrence_desc* desc);
+int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_recurrence_args* args,
+                        void* stream);
+
+/*
+ * Gradients of the call above with respect to x, f, bias and the entering
+ * state, from dh and dstate_out (the gradient of the state left, NULL: zero).
+ * x and f are the forward pass's, as they were or (x8, f8 with codes) as it
+ * kept them; `saved` is what it saved.  With G_t = dh_t + a_{t+1} G_{t+1}
+ * (behind the last token dstate_out):
+ *   dx_t = (1 - a_t) G_t,  df_t = G_t a_t (1 - a_t) (h_{t-1} - x_t)   (complement)
+ *   dx_t = G_t,            df_t = G_t a_t (1 - a_t) h_{t-1}
+ *   dbias = sum df_t,      dstate_in = a_0 G_0  (dstate_out for an empty sequence)
+ * h_{t-1} runs from the saved states over the x and f given.  State gradients
+ * are [nseq][channels] (no slots).  dbias (f32 [channels]) and dstate_in are
+ * overwritten, and may be NULL.  Rows of dx, df that belong to no sequence are
+ * left as they are.  Outputs may share no memory with what is read or with one
+ * another.
+ */
+typedef struct to_gated_recurrence_grad_args {
+  to_rows x, f, dh, dx, df;
+  to_rows8 x8, f8; /* codes not NULL: in the place of x, f                   */
+  const float* bias;
+  const int32_t* cu_seqlens;
+  const float* saved;
+  const float* dstate_out;
+  float* dstate_in;
+  float* dbias;
+  void* workspace; /* device, 256-byte aligned                               */
+  size_t workspace_bytes;
+} to_gated_recurrence_grad_args;
+
+size_t to_gated_recurrence_backward_workspace_bytes(const to_gated_recurrence_desc* desc);
+int to_gated_recurrence_backward(const to_gated_recurrence_desc* desc,
+                                 const to_gated_recurrence_grad_args* args, void* stream);
+
+/*
+ * One token of each of desc->tokens requests: the state in the request's slot
+ * (state_out) becomes h in place.  A request whose slot lies outside
+ * [0, num_slots) touches no state and gets a row of zeros.  nseq, cu_seqlens,
+ * state_in, saved, keep_x, keep_f and the workspace are not used.
+ */
+int to_gated_recurrence_step(const to_gated_recurrence_desc* desc,
+                             const to_gated_recurrence_args* args, void* stream);
+
+/* ---------------------------------------------------------------------- */
+/* Norms around a block, with its gate and residual scale                  */
+/* ---------------------------------------------------------------------- */
+/*
+ * Between two blocks: the block's output y joins the residual stream r, and the
+ * next block's input n is made of the sum, for every row:
+ *   u = w_post * y / sqrt(mean(y^2) + eps)        (post_norm = 0: u = w_post * y)
+ *   r_out = r + scale * u * act(g)                (gate NONE: r + scale * u)
+ *   n = w_pre * r_out / sqrt(mean(r_out^2) + eps)
+ * y, g, n: rows of dtype; r, r_out: rows of residual (TO_F32, or dtype), all
+ * [tokens][width] (one head: head_stride is not used).  act(g): g, sigmoid(g) or
+ * g * sigmoid(g).  w_post, w_pre: device f32 [width], NULL for 1.  y NULL (a model's
+ * first norm): n is made of r, and there is no r_out, g or keep_y.  n NULL: only
+ * r_out is made.  Sums are f32; each output takes one rounding, n from r_out
+ * before its own.  width 1 .. 16384.
+ *
+ * keep_r, keep_y, keep_g (codes not NULL): r_out before its rounding (r, where there
+ * is no y), y and g are also written in 8 bits, for the gradients.
+ * r_out may be r (same pointer and stride); otherwise outputs share no memory
+ * with what is read or with one another.
+ */
+typedef enum to_gate { TO_GATE_NONE = 0, TO_GATE_LINEAR = 1, TO_GATE_SIGMOID = 2, TO_GATE_SILU = 3 } to_gate;
+
+typedef struct to_block_norm_desc {
+  int32_t dtype;
+  int32_t residual;  /* dtype of r and r_out                                 */
+  int32_t width;
+  int32_t gate;      /* to_gate                                              */
+  int32_t post_norm; /* 0 or 1                                               */
+  int32_t reserved0;
+  double scale;      /* finite                                               */
+  double eps;        /* >= 0                                                 */
+} to_block_norm_desc;
+
+typedef struct to_block_norm_args {
+  to_rows r, y, g, r_out, n;
+  to_rows8 keep_r, keep_y, keep_g;
+  const float* w_post;
+  const float* w_pre;
+} to_block_norm_args;
+
+int to_block_norm(const to_block_norm_desc* desc, int64_t tokens, const to_block_norm_args* args,
+                  void* stream);
+
+/*
+ * Gradients: r_out, y, g as the forward pass had them, or (r8, y8, g8 with codes)
+ * as it kept them; dr_out (residual's type, NULL data: zero) and dn (NULL data:
+ * zero) of its outputs -> dr (residual's type), dy, dg of its inputs, and dw_post,
+ * dw_pre (f32 [width], overwritten, computed even where the weight is NULL; either
+ * may be NULL).  Without y: dr and dw_pre alone.  Sums run in a fixed order.  dr may be
+ * dr_out; otherwise outputs share no memory with what is read or with one another.
+ * workspace: 16-byte aligned device memory.
+ */
+typedef struct to_block_norm_grad_args {
+  to_rows r_out, y, g, dr_out, dn, dr, dy, dg;
+  to_rows8 r8, y8, g8;
+  const float* w_post;
+  const float* w_pre;
+  float* dw_post;
+  float* dw_pre;
+  void* workspace;
+  size_t workspace_bytes;
+} to_block_norm_grad_args;
+
+size_t to_block_norm_workspace_bytes(const to_block_norm_desc* desc, int64_t tokens);
+int to_block_norm_backward(const to_block_norm_desc* desc, int64_t tokens,
+                           const to_block_norm_grad_args* args, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -186,6 +186,16 @@ _sig("to_linear_attention_backward_workspace_bytes", C.c_size_t, [C.c_char_p])
 _sig("to_linear_attention", C.c_int, [C.c_char_p, C.c_char_p, C.c_void_p])
 _sig("to_linear_attention_backward", C.c_int, [C.c_char_p, C.c_char_p, C.c_void_p])
 _sig("to_linear_attention_step", C.c_int, [C.c_char_p, C.c_char_p, C.c_void_p])
+for _name in ("to_gated_recurrence", "to_gated_recurrence_backward", "to_gated_recurrence_step"):
+    _sig(_name, C.c_int, [C.c_char_p, C.c_char_p, C.c_void_p])
+_sig("to_gated_recurrence_saved_rows", C.c_int64, [C.c_char_p])
+_sig("to_gated_recurrence_workspace_bytes", C.c_size_t, [C.c_char_p])
+_sig("to_gated_recurrence_backward_workspace_bytes", C.c_size_t, [C.c_char_p])
+for _name in ("to_block_norm", "to_block_norm_backward"):
+    _sig(_name, C.c_int, [C.c_char_p, C.c_int64, C.c_char_p, C.c_void_p])
+_sig("to_block_norm_workspace_bytes", C.c_size_t, [C.c_char_p, C.c_int64])
+for _name in ("to_rows8_pack", "to_rows8_unpack"):
+    _sig(_name, C.c_int, [C.c_int32, C.c_int32, C.c_int64, _R, _R, C.c_void_p])
 
 
 def status_name(status: int) -> str:

@@ -36,8 +36,9 @@ int device_sm_count(int* device_out);
 // own device symbol): *value = 0 or a to_status; reset clears it.
 int chain_device_status(int reset, int* value);
 
-// The same for the linear-attention kernels.
+// The same for the linear-attention kernels and for the gated recurrence's.
 int sequence_device_status(int reset, int* value);
+int recurrence_device_status(int reset, int* value);
 
 inline bool aligned(const void* p, size_t a) {
   return (reinterpret_cast<uintptr_t>(p) % a) == 0;

@@ -1,15 +1,17 @@
 """Sequence operators on device tensors: the query/key norm with its rotation,
-and linear attention with a decay for each head.
+linear attention with a decay for each head, the gated linear recurrence of
+channels, the norms around a block with its gate and residual scale, and rows
+kept in 8 bits for a backward pass.
 
-Both are thin callers of the C ABI (to_qk_norm_rotary*, to_linear_attention*):
-an object holds what stays fixed (type, heads, widths), a call takes torch
+All are thin callers of the C ABI (to_qk_norm_rotary*, to_linear_attention*,
+to_gated_recurrence*, to_block_norm*, to_rows8*): an object holds what stays fixed (type, heads, widths), a call takes torch
 tensors and the stream to launch on (torch's current one where none is given;
-0: the default stream) and allocates nothing.  Rows are tensors [tokens, heads, width] whose last dimension is
-contiguous; they may be views into wider packed rows.  Shapes, types, devices
+0: the default stream) and allocates nothing.  Rows are tensors [tokens, heads, width] or, without heads,
+[tokens, width], whose last dimension is contiguous; they may be views into wider packed rows.  Shapes, types, devices
 and sizes are checked here, the rest by the library; a failed check raises
 before anything is launched (ValueError here, abi.ToError from the library).
-Outputs share no memory with what the call reads, but for q_out, k_out and
-state_out, which may be the inputs themselves.
+Outputs share no memory with what the call reads, but for q_out, k_out,
+state_out, r_out and dr, which may be the inputs themselves.
 No call records a graph for autograd; a torch.autograd.Function around forward
 and backward does.  Autograd is told what a call has written.
 The caller orders the streams: a tensor written on another stream has to be
@@ -20,7 +22,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import struct
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 from torch.autograd.graph import increment_version  # tells autograd that a saved tensor has changed
@@ -34,6 +36,15 @@ _ROWS = struct.Struct("@Pqq")
 _DESC = struct.Struct("@6i2qd")
 _ARGS = struct.Struct("@" + 4 * "Pqq" + "6PN")
 _GRAD_ARGS = struct.Struct("@" + 7 * "Pqq" + "6PN")
+# to_rows8; to_gated_recurrence_desc / _args / _grad_args; to_block_norm_desc / _args / _grad_args
+_ROWS8 = struct.Struct("@PPqq")
+_REC_DESC = struct.Struct("@4i2q")
+_REC_ARGS = struct.Struct("@" + 3 * "Pqq" + 2 * "PPqq" + "7PN")
+_REC_GRAD_ARGS = struct.Struct("@" + 5 * "Pqq" + 2 * "PPqq" + "7PN")
+_NORM_DESC = struct.Struct("@6i2d")
+_NORM_ARGS = struct.Struct("@" + 5 * "Pqq" + 3 * "PPqq" + "2P")
+_NORM_GRAD_ARGS = struct.Struct("@" + 8 * "Pqq" + 3 * "PPqq" + "5PN")
+_NO_ROWS, _NO_ROWS8 = (0, 0, 0), (0, 0, 0, 0)
 
 DTYPES = {torch.bfloat16: abi.TO_BF16, torch.float32: abi.TO_F32}
 
@@ -71,6 +82,43 @@ def _flat(t, name: str, dtype: torch.dtype, shape, device) -> int:
     if not t.is_contiguous():
         raise ValueError(f"{name} is not contiguous")
     return t.data_ptr()
+
+
+def _row(t, name: str, dtype: torch.dtype, shape, device):
+    """(data, token stride, 0) of rows without heads, as in to_rows."""
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        _refuse(t, name, dtype, shape, device)
+    stride = t.stride()
+    if stride[1] != 1 and shape[1] > 1:
+        raise ValueError(f"{name}: the last dimension is not contiguous")
+    return t.data_ptr(), stride[0], 0
+
+
+def _row8(t, name: str, tokens: int, width: int, device):
+    """(codes, scales, their token strides) of rows in 8 bits, as in to_rows8."""
+    if not isinstance(t, Rows8):
+        raise ValueError(f"{name}: {type(t).__name__} is not Rows8")
+    codes = _row(t.codes, f"{name}.codes", torch.int8, (tokens, width), device)
+    scales = _row(t.scales, f"{name}.scales", torch.uint8, (tokens, -(-width // GROUP8)), device)
+    return codes[0], scales[0], codes[1], scales[1]
+
+
+def _row_or_8(t, name: str, dtype: torch.dtype, shape, device):
+    """A to_rows and a to_rows8, one of them empty."""
+    if isinstance(t, Rows8):
+        return _NO_ROWS, _row8(t, name, *shape, device)
+    return _row(t, name, dtype, shape, device), _NO_ROWS8
+
+
+def _written(*outputs):
+    """Tells autograd which tensors a call has written (None, tensors and Rows8)."""
+    seen = []
+    for t in outputs:
+        if isinstance(t, Rows8):
+            seen += t
+        elif t is not None:
+            seen.append(t)
+    increment_version(seen)
 
 
 def _refuse(t, name, dtype, shape, device):
@@ -294,3 +342,255 @@ class LinearAttention:
         if st:
             abi.check(st, "to_linear_attention_backward")
         increment_version((dq, dk, dv) if dstate_in is None else (dq, dk, dv, dstate_in))
+
+
+GROUP8 = 32  # neighbouring values of Rows8 that share a scale
+
+
+class Rows8(NamedTuple):
+    """Rows in 8 bits: value = codes * 2^(scales - 127), a scale for every 32 neighbouring values.
+
+    codes: int8 [tokens, width]; scales: uint8 [tokens, ceil(width / 32)]
+    (255: the group held an infinity or a NaN and reads as NaN).  A value is off
+    by at most half a scale, 1/127 of the largest one of its 32.
+    """
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @classmethod
+    def empty(cls, tokens: int, width: int, device="cuda") -> "Rows8":
+        """Uninitialised rows."""
+        return cls(torch.empty(tokens, width, dtype=torch.int8, device=device),
+                   torch.empty(tokens, -(-width // GROUP8), dtype=torch.uint8, device=device))
+
+
+class Checkpoint8:
+    """Activations into 8 bits (Rows8) and back.
+
+    GatedRecurrence and BlockNorm write the same form while they hold the rows
+    (keep_*), and their backward passes read it in the place of the rows.
+    """
+
+    def __init__(self, dtype, width: int):
+        self.dtype, self.width = _dtype(dtype), width
+        _sizes(width=width)
+        abi.check(abi.lib.to_rows8_pack(DTYPES[self.dtype], width, 0, bytes(_ROWS.size), bytes(_ROWS8.size), 0),
+                  "Checkpoint8")
+
+    def _call(self, fn, name, x, x8, first, stream, device):
+        tokens = x.shape[0]
+        rows = _ROWS.pack(*_row(x, "x", self.dtype, (tokens, self.width), device))
+        kept = _ROWS8.pack(*_row8(x8, "x8", tokens, self.width, device))
+        st = fn(DTYPES[self.dtype], self.width, tokens, *((rows, kept) if first else (kept, rows)), _on(stream, device))
+        if st:
+            abi.check(st, name)
+
+    def pack(self, x, x8: Rows8, stream: Optional[int] = None):
+        """x8 <- x in 8 bits."""
+        self._call(abi.lib.to_rows8_pack, "to_rows8_pack", x, x8, True, stream, _cuda(x, "x"))
+        _written(x8)
+
+    def unpack(self, x8: Rows8, x, stream: Optional[int] = None):
+        """x <- the values that x8 stands for."""
+        self._call(abi.lib.to_rows8_unpack, "to_rows8_unpack", x, x8, False, stream, _cuda(x, "x"))
+        _written(x)
+
+
+class GatedRecurrence:
+    """h_t = a_t h_{t-1} + (1 - a_t) x_t for every channel, with a_t = sigmoid(f_t + bias).
+
+    With complement=False x_t is added as it is.  Prompts (`forward`) are packed
+    sequences, single tokens (`step`) update the states in place, `backward`
+    gives the gradients of `forward`.  bias: f32 [channels] or None.  States:
+    f32 [slots, channels].
+    """
+
+    def __init__(self, dtype, channels: int, complement: bool = True):
+        self.dtype, self.channels, self.complement = _dtype(dtype), channels, bool(complement)
+        _sizes(channels=channels)
+        abi.check(abi.lib.to_gated_recurrence(self._desc(0, 0), bytes(_REC_ARGS.size), 0), "GatedRecurrence")
+
+    def _desc(self, tokens: int, nseq: int, slots: int = 0) -> bytes:
+        return _REC_DESC.pack(DTYPES[self.dtype], self.channels, nseq, self.complement, tokens, slots)
+
+    def saved_rows(self, tokens: int, sequences: int) -> int:
+        """Rows of `saved` (f32 [rows, channels]): a state for every 128 tokens begun, at most."""
+        return abi.lib.to_gated_recurrence_saved_rows(self._desc(tokens, sequences))
+
+    def workspace_bytes(self, tokens: int, sequences: int) -> int:
+        """Bytes of `workspace` that forward() needs (0: none)."""
+        return abi.lib.to_gated_recurrence_workspace_bytes(self._desc(tokens, sequences))
+
+    def backward_workspace_bytes(self, tokens: int, sequences: int) -> int:
+        return abi.lib.to_gated_recurrence_backward_workspace_bytes(self._desc(tokens, sequences))
+
+    def _flat(self, t, name, rows, device):
+        return _flat(t, name, torch.float32, (rows, self.channels), device)
+
+    def _bias(self, bias, device, name="bias"):
+        return _flat(bias, name, torch.float32, (self.channels,), device)
+
+    def _sequences(self, cu_seqlens, device):
+        n = cu_seqlens.numel() - 1
+        if n < 0:
+            raise ValueError("cu_seqlens is empty")
+        return n, _flat(cu_seqlens, "cu_seqlens", torch.int32, (n + 1,), device)
+
+    def forward(self, x, f, bias, cu_seqlens, h, state_in=None, state_out=None, slots=None, saved=None,
+                keep_x: Optional[Rows8] = None, keep_f: Optional[Rows8] = None, workspace=None,
+                stream: Optional[int] = None):
+        """h <- the outputs of packed sequences; state_out (may be state_in) <- the states they leave.
+
+        cu_seqlens: int32 [sequences + 1], on the device.  slots: int32
+        [sequences], each sequence's place in state_in and state_out (None:
+        its number); one outside them means no state.  For backward(): saved
+        <- the states that enter every 128 tokens, keep_x, keep_f <- x, f in 8 bits.
+        """
+        tokens, device = x.shape[0], _cuda(x, "x")
+        n, cu = self._sequences(cu_seqlens, device)
+        have = n if state_in is None and state_out is None else (state_out if state_in is None else state_in).shape[0]
+        if slots is None and have != n:
+            raise ValueError(f"{have} states for {n} sequences, and no slots")
+        desc, shape = self._desc(tokens, n, have), (tokens, self.channels)
+        args = _REC_ARGS.pack(
+            *_row(x, "x", self.dtype, shape, device), *_row(f, "f", self.dtype, shape, device),
+            *_row(h, "h", self.dtype, shape, device),
+            *(_NO_ROWS8 if keep_x is None else _row8(keep_x, "keep_x", *shape, device)),
+            *(_NO_ROWS8 if keep_f is None else _row8(keep_f, "keep_f", *shape, device)),
+            self._bias(bias, device), cu, _flat(slots, "slots", torch.int32, (n,), device),
+            self._flat(state_in, "state_in", have, device), self._flat(state_out, "state_out", have, device),
+            0 if saved is None else self._flat(saved, "saved", abi.lib.to_gated_recurrence_saved_rows(desc), device),
+            *_scratch(workspace, abi.lib.to_gated_recurrence_workspace_bytes(desc), device))
+        st = abi.lib.to_gated_recurrence(desc, args, _on(stream, device))
+        if st:
+            abi.check(st, "to_gated_recurrence")
+        _written(h, state_out, saved, keep_x, keep_f)
+
+    def step(self, x, f, bias, state, h, slots=None, stream: Optional[int] = None):
+        """One token of each request: its state is updated in place, h <- its output."""
+        tokens, device, have = x.shape[0], _cuda(x, "x"), state.shape[0]
+        if slots is None and have < tokens:
+            raise ValueError(f"{have} states for {tokens} requests, and no slots")
+        shape = (tokens, self.channels)
+        args = _REC_ARGS.pack(
+            *_row(x, "x", self.dtype, shape, device), *_row(f, "f", self.dtype, shape, device),
+            *_row(h, "h", self.dtype, shape, device), *_NO_ROWS8, *_NO_ROWS8, self._bias(bias, device), 0,
+            _flat(slots, "slots", torch.int32, (tokens,), device), 0, self._flat(state, "state", have, device), 0, 0, 0)
+        st = abi.lib.to_gated_recurrence_step(self._desc(tokens, 0, have), args, _on(stream, device))
+        if st:
+            abi.check(st, "to_gated_recurrence_step")
+        increment_version((h, state))
+
+    def backward(self, x, f, bias, cu_seqlens, saved, dh, dx, df, dbias=None, dstate_out=None, dstate_in=None,
+                 workspace=None, stream: Optional[int] = None):
+        """dx, df (and dbias, dstate_in) <- gradients of forward() from dh and dstate_out.
+
+        x, f: forward()'s rows, or what it kept of them (Rows8); saved: what it
+        saved.  State gradients hold one row a sequence, in order.
+        """
+        tokens, device = dh.shape[0], _cuda(dh, "dh")
+        n, cu = self._sequences(cu_seqlens, device)
+        desc, shape = self._desc(tokens, n, n), (tokens, self.channels)
+        (rx, x8), (rf, f8) = (_row_or_8(t, name, self.dtype, shape, device) for t, name in ((x, "x"), (f, "f")))
+        args = _REC_GRAD_ARGS.pack(
+            *rx, *rf, *_row(dh, "dh", self.dtype, shape, device), *_row(dx, "dx", self.dtype, shape, device),
+            *_row(df, "df", self.dtype, shape, device), *x8, *f8, self._bias(bias, device), cu,
+            self._flat(_needed(saved, "saved"), "saved", abi.lib.to_gated_recurrence_saved_rows(desc), device),
+            self._flat(dstate_out, "dstate_out", n, device), self._flat(dstate_in, "dstate_in", n, device),
+            self._bias(dbias, device, "dbias"),
+            *_scratch(workspace, abi.lib.to_gated_recurrence_backward_workspace_bytes(desc), device))
+        st = abi.lib.to_gated_recurrence_backward(desc, args, _on(stream, device))
+        if st:
+            abi.check(st, "to_gated_recurrence_backward")
+        _written(dx, df, dbias, dstate_in)
+
+
+class BlockNorm:
+    """What lies between two blocks: norm of a block's output, gate, residual sum and the next block's norm.
+
+    u = w_post * y / rms(y), r_out = r + scale * u * act(g), n = w_pre * r_out / rms(r_out).
+
+    residual: type of r and r_out (dtype by default, or f32).  gate: None, "linear"
+    (act(g) = g), "sigmoid" or "silu".  post_norm=False leaves u = w_post * y.
+    w_post, w_pre: f32 [width] or None.
+    """
+
+    GATES = {None: 0, "linear": 1, "sigmoid": 2, "silu": 3}
+
+    def __init__(self, dtype, width: int, residual=None, gate: Optional[str] = None, post_norm: bool = True,
+                 scale: float = 1.0, eps: float = 1e-6):
+        self.dtype, self.width = _dtype(dtype), width
+        self.residual = self.dtype if residual is None else _dtype(residual)
+        if gate not in self.GATES:
+            raise ValueError(f"gate {gate!r}: None, 'linear', 'sigmoid' or 'silu'")
+        self.gate = gate
+        _sizes(width=width)
+        self._desc = _NORM_DESC.pack(DTYPES[self.dtype], DTYPES[self.residual], width, self.GATES[gate],
+                                     int(bool(post_norm)), 0, scale, eps)
+        abi.check(abi.lib.to_block_norm(self._desc, 0, bytes(_NORM_ARGS.size), 0), "BlockNorm")
+
+    def _gate(self, g, y, name):
+        if (g is not None) != (self.gate is not None and y is not None):
+            raise ValueError(f"{name} is {'missing' if g is None else 'given'} with gate {self.gate!r}"
+                             f"{'' if y is not None else ' and no y'}")
+
+    def forward(self, r, y, g, w_post, w_pre, r_out, n, keep_r: Optional[Rows8] = None,
+                keep_y: Optional[Rows8] = None, keep_g: Optional[Rows8] = None, stream: Optional[int] = None):
+        """r_out (may be r) <- the residual stream with y joined, n <- the next block's input.
+
+        Without y (None, then r_out and g are None too) n is made of r alone; n
+        may be None.  keep_r, keep_y, keep_g <- r_out (r without y), y, g in 8 bits.
+        """
+        tokens, device = r.shape[0], _cuda(r, "r")
+        self._gate(g, y, "g")
+        if (y is None) != (r_out is None):
+            raise ValueError("y and r_out: one is None, the other is not")
+        if y is None and (n is None or keep_y is not None):
+            raise ValueError("without y there has to be n, and no keep_y")
+        if g is None and keep_g is not None:
+            raise ValueError("keep_g without g")
+        shape = (tokens, self.width)
+        row = lambda t, name, kind: _NO_ROWS if t is None else _row(t, name, kind, shape, device)  # noqa: E731
+        kept = lambda t, name: _NO_ROWS8 if t is None else _row8(t, name, *shape, device)  # noqa: E731
+        args = _NORM_ARGS.pack(
+            *_row(r, "r", self.residual, shape, device), *row(y, "y", self.dtype), *row(g, "g", self.dtype),
+            *row(r_out, "r_out", self.residual), *row(n, "n", self.dtype),
+            *kept(keep_r, "keep_r"), *kept(keep_y, "keep_y"), *kept(keep_g, "keep_g"),
+            _flat(w_post, "w_post", torch.float32, (self.width,), device),
+            _flat(w_pre, "w_pre", torch.float32, (self.width,), device))
+        st = abi.lib.to_block_norm(self._desc, tokens, args, _on(stream, device))
+        if st:
+            abi.check(st, "to_block_norm")
+        _written(r_out, n, keep_r, keep_y, keep_g)
+
+    def workspace_bytes(self, tokens: int) -> int:
+        """Bytes of `workspace` that backward() needs."""
+        return abi.lib.to_block_norm_workspace_bytes(self._desc, tokens)
+
+    def backward(self, r_out, y, g, w_post, w_pre, dr_out, dn, dr, dy, dg, dw_post, dw_pre, workspace,
+                 stream: Optional[int] = None):
+        """dr (may be dr_out), dy, dg, dw_post, dw_pre <- gradients from dr_out and dn (None: zero).
+
+        r_out, y, g: forward()'s rows (r_out without y: r), or what it kept of
+        them (Rows8).  dw_post, dw_pre: f32 [width] or None.
+        """
+        tokens, device = dr.shape[0], _cuda(dr, "dr")
+        self._gate(g, y, "g")
+        if (y is None) != (dy is None) or (g is None) != (dg is None) or (y is None and dw_post is not None):
+            raise ValueError("y and dy, g and dg: one is None, the other is not; or dw_post without y")
+        shape = (tokens, self.width)
+        row = lambda t, name, kind: _NO_ROWS if t is None else _row(t, name, kind, shape, device)  # noqa: E731
+        read = [(_NO_ROWS, _NO_ROWS8) if t is None else _row_or_8(t, name, kind, shape, device)
+                for t, name, kind in ((_needed(r_out, "r_out"), "r_out", self.residual), (y, "y", self.dtype),
+                                      (g, "g", self.dtype))]
+        weights = [_flat(t, name, torch.float32, (self.width,), device)
+                   for t, name in ((w_post, "w_post"), (w_pre, "w_pre"), (dw_post, "dw_post"), (dw_pre, "dw_pre"))]
+        args = _NORM_GRAD_ARGS.pack(
+            *read[0][0], *read[1][0], *read[2][0], *row(dr_out, "dr_out", self.residual), *row(dn, "dn", self.dtype),
+            *_row(dr, "dr", self.residual, shape, device), *row(dy, "dy", self.dtype), *row(dg, "dg", self.dtype),
+            *read[0][1], *read[1][1], *read[2][1], *weights,
+            *_scratch(workspace, int(dw_post is not None or dw_pre is not None), device))
+        st = abi.lib.to_block_norm_backward(self._desc, tokens, args, _on(stream, device))
+        if st:
+            abi.check(st, "to_block_norm_backward")
+        _written(dr, dy, dg, dw_post, dw_pre)
