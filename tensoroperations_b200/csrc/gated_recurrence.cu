@@ -14,20 +14,25 @@
 // reciprocal) leave it memory bound.
 //
 // Gates: with u = exp(-|f|), u / (1 + u) is the smaller of a and 1 - a, accurate to
-// f32 relative to itself.  It is kept with f's sign ("s": 1 - a where positive, -a
-// where negative), and every step adds s times a difference to the larger term:
+// f32 relative to itself.  It is kept with a sign ("c": a where positive, -(1 - a)
+// where negative), and every step adds c times a difference to the larger term:
 //   f >= 0:  h + (1 - a)(x - h)      f < 0:  x + a (h - x)
-// so a memory of thousands of tokens does not take over a rounding of a near 1.
+// so a memory of thousands of tokens does not take over a rounding of a near 1, and
+// what is left of a state after a token that almost forgets it stays exact.
 //
 // Joining the segments: a CTA takes segments in the order of a counter (so a
 // segment's predecessors have been taken by CTAs that run), publishes its map as
 // soon as it has reduced its tokens, and folds the maps of its predecessors from
-// the nearest one whose number is a multiple of 16, whose entering state is
-// published too.  What is folded, and in which order, goes by the segment's number
-// alone: results do not depend on timing.  Waits are bounded.
+// the nearest one whose number is a multiple of 8, whose entering state is
+// published too.  Its warps fetch a map each.  What is folded, and in which
+// order, goes by the segment's number alone: results do not depend on timing.  A
+// published word is a value and its mark in 8 bytes, written and read at once, so
+// no fence and no flag is waited for; the words are cleared before the launch.  Waits
+// are bounded.
 #include <algorithm>
 
 #include "rows8.cuh"
+#include "sm100_primitives.cuh"
 
 namespace to_b200 {
 namespace {
@@ -39,29 +44,66 @@ constexpr int kSegment = TO_RECURRENCE_SEGMENT;
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kTok = kSegment / kWarps;  // tokens of a warp
 constexpr int kRowBytes = 128;           // of a tile's row of values
-constexpr int kChain = 16;               // segments between published states
+constexpr int kTile = kSegment * kRowBytes;
+constexpr int kChain = 8;                // segments between published states: a warp fetches one map
 constexpr uint32_t kPolls = 1u << 20;    // of a flag, about half a second
 
 __device__ int g_recurrence_status;
 
+// A lane's channels: one 32-bit word of a row, as one f32 or two in a register pair
+// (packed f32x2 instructions).
+template <int V>
+struct Vals;
+template <>
+struct Vals<1> {
+  float v[1];
+};
+template <>
+struct Vals<2> {
+  float v[2];
+};
+template <int V>
+__device__ __forceinline__ Vals<V> all(float x) {
+  Vals<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = x;
+  return r;
+}
+__device__ __forceinline__ Vals<1> fma(Vals<1> a, Vals<1> b, Vals<1> c) { return {{fmaf(a.v[0], b.v[0], c.v[0])}}; }
+__device__ __forceinline__ Vals<2> fma(Vals<2> a, Vals<2> b, Vals<2> c) {
+  const float2 r = __ffma2_rn(make_float2(a.v[0], a.v[1]), make_float2(b.v[0], b.v[1]), make_float2(c.v[0], c.v[1]));
+  return {{r.x, r.y}};
+}
+__device__ __forceinline__ Vals<1> mul(Vals<1> a, Vals<1> b) { return {{a.v[0] * b.v[0]}}; }
+__device__ __forceinline__ Vals<2> mul(Vals<2> a, Vals<2> b) {
+  const float2 r = __fmul2_rn(make_float2(a.v[0], a.v[1]), make_float2(b.v[0], b.v[1]));
+  return {{r.x, r.y}};
+}
+__device__ __forceinline__ Vals<1> add(Vals<1> a, Vals<1> b) { return {{a.v[0] + b.v[0]}}; }
+__device__ __forceinline__ Vals<2> add(Vals<2> a, Vals<2> b) {
+  const float2 r = __fadd2_rn(make_float2(a.v[0], a.v[1]), make_float2(b.v[0], b.v[1]));
+  return {{r.x, r.y}};
+}
+template <int V>
+__device__ __forceinline__ Vals<V> sub(Vals<V> a, Vals<V> b) {
+  return fma(b, all<V>(-1.f), a);
+}
+
 template <typename T>
-struct Lane {  // a lane's channels: one 32-bit word of a row
+struct Lane {
   static constexpr int kVec = 4 / int(sizeof(T));
   static constexpr int kChannels = kRowBytes / int(sizeof(T));  // of a tile
-  __device__ __forceinline__ static void unpack(uint32_t w, float (&v)[kVec]) {
-    if constexpr (kVec == 1) {
-      v[0] = __uint_as_float(w);
-    } else {
-      v[0] = __uint_as_float(w << 16);
-      v[1] = __uint_as_float(w & 0xffff0000u);
-    }
+  using P = Vals<kVec>;
+  __device__ __forceinline__ static P unpack(uint32_t w) {
+    if constexpr (kVec == 1) return {{__uint_as_float(w)}};
+    else return {{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)}};
   }
-  __device__ __forceinline__ static uint32_t pack(const float (&v)[kVec]) {
+  __device__ __forceinline__ static uint32_t pack(const P& p) {
     if constexpr (kVec == 1) {
-      return __float_as_uint(v[0]);
+      return __float_as_uint(p.v[0]);
     } else {
-      const __nv_bfloat162 p = __floats2bfloat162_rn(v[0], v[1]);
-      return *reinterpret_cast<const uint32_t*>(&p);
+      const __nv_bfloat162 b = __floats2bfloat162_rn(p.v[0], p.v[1]);
+      return *reinterpret_cast<const uint32_t*>(&b);
     }
   }
 };
@@ -70,16 +112,15 @@ struct Lane {  // a lane's channels: one 32-bit word of a row
 struct Chain {
   const int32_t* cu;
   int nseq, tokens, channels, slabs, slots;  // slabs: tiles of channels; slots: segments that there may be
-  unsigned long long* ticket;                // null: no sequence is longer than a segment
+  unsigned* ticket;                          // null: no sequence is longer than a segment
   int* gave_up;                              // set once a wait of this call has run out
-  int* flags;                                // [slots][slabs][2]: the map, the entering state
-  float2* maps;                              // [slots][slabs * kChannels]
-  float* states;
+  // [slots][slabs * kChannels] words of two f32, zero until they are published
+  uint64_t* maps;    // (H, A with its sign bit set)
+  uint64_t* states;  // (the entering state, 1)
 };
 
 struct Item {
-  long long tile;  // number of the segment and slab; -1: no more
-  int slot, slab, idx, count, seq, row0, n;
+  int slot, slab, idx, count, seq, row0, n;  // slot -1: no more
 };
 
 __device__ __forceinline__ int bound_of(const Chain& C, int s) {
@@ -109,57 +150,54 @@ __device__ __forceinline__ void find_segment(const Chain& C, int w, int lane, It
   it.slot = w;
 }
 
+__device__ __forceinline__ void next_ticket(const Chain& C, unsigned& ticket, int lane) {
+  if (!C.ticket) ticket += gridDim.x;
+  else if (lane == 0) ticket = atomicAdd(C.ticket, 1u);
+}
+
+// The item of a warp's ticket (lane 0's); a slot that no segment has goes to `unused`,
+// and the next ticket is taken.  `ticket`: the one that the item has.
 template <bool BACKWARD, typename UNUSED>
-__device__ __forceinline__ Item next_item(const Chain& C, unsigned long long ticket, int lane, UNUSED&& unused) {
+__device__ __forceinline__ Item next_item(const Chain& C, unsigned& ticket, int lane, UNUSED&& unused) {
   Item it;
   for (;;) {
     ticket = __shfl_sync(0xffffffffu, ticket, 0);
-    const unsigned long long total = static_cast<unsigned long long>(C.slots) * C.slabs;
-    if (ticket >= total) {
-      it.tile = -1;
+    const unsigned at = ticket / static_cast<unsigned>(C.slabs);
+    if (at >= static_cast<unsigned>(C.slots)) {
+      it.slot = -1;
       return it;
     }
-    const int at = static_cast<int>(ticket / C.slabs);
-    it.slab = static_cast<int>(ticket - static_cast<unsigned long long>(at) * C.slabs);
-    find_segment(C, BACKWARD ? C.slots - 1 - at : at, lane, it);
-    it.tile = static_cast<long long>(it.slot) * C.slabs + it.slab;
+    it.slab = static_cast<int>(ticket - at * C.slabs);
+    find_segment(C, BACKWARD ? C.slots - 1 - static_cast<int>(at) : static_cast<int>(at), lane, it);
     if (it.idx >= 0) return it;
-    unused(it);  // a slot that no segment has
-    if (C.ticket) {
-      if (lane == 0) ticket = atomicAdd(C.ticket, 1ull);
-    } else {
-      ticket += gridDim.x;
-    }
+    unused(it);
+    next_ticket(C, ticket, lane);
   }
 }
 
 // ---- tiles in shared memory ----------------------------------------------------------
 
 // `rows` rows of ROWB bytes into shared memory, ACCESS bytes at a time; the
-// columns from `valid` bytes on become zero.
+// columns from `valid` bytes on become zero.  A thread keeps its column.
 template <int ACCESS, int ROWB>
 __device__ __forceinline__ void load_tile(char* dst, const char* src, long long pitch, int rows, int valid) {
-  constexpr int kPer = ROWB / ACCESS;
+  constexpr int kPer = ROWB / ACCESS, kStep = kThreads / kPer;  // threads of a row, rows of an iteration
+  const int col = (threadIdx.x % kPer) * ACCESS, row0 = threadIdx.x / kPer;
+  const int bytes = max(0, min(ACCESS, valid - col));
+  const char* s = src + row0 * pitch + (bytes ? col : 0);
+  dst += row0 * ROWB + col;
+  const long long step = kStep * pitch;
 #pragma unroll 4
-  for (int i = threadIdx.x; i < rows * kPer; i += kThreads) {
-    const int row = i / kPer, col = (i % kPer) * ACCESS;
-    const int bytes = max(0, min(ACCESS, valid - col));
-    char* d = dst + row * ROWB + col;
-    const char* s = bytes ? src + row * pitch + col : src;
+  for (int row = row0; row < rows; row += kStep, s += step, dst += kStep * ROWB) {
     if constexpr (ACCESS >= 16) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                       static_cast<uint32_t>(__cvta_generic_to_shared(d))),
-                   "l"(s), "r"(bytes)
-                   : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(s), "r"(bytes) : "memory");
     } else if constexpr (ACCESS >= 4) {
-      asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(
-                       static_cast<uint32_t>(__cvta_generic_to_shared(d))),
-                   "l"(s), "n"(ACCESS), "r"(bytes)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(dst)), "l"(s), "n"(ACCESS), "r"(bytes)
                    : "memory");
     } else if constexpr (ACCESS == 2) {
-      *reinterpret_cast<uint16_t*>(d) = bytes ? *reinterpret_cast<const uint16_t*>(s) : uint16_t(0);
+      *reinterpret_cast<uint16_t*>(dst) = bytes ? *reinterpret_cast<const uint16_t*>(s) : uint16_t(0);
     } else {
-      *reinterpret_cast<uint8_t*>(d) = bytes ? *reinterpret_cast<const uint8_t*>(s) : uint8_t(0);
+      *reinterpret_cast<uint8_t*>(dst) = bytes ? *reinterpret_cast<const uint8_t*>(s) : uint8_t(0);
     }
   }
 }
@@ -173,8 +211,11 @@ __device__ __forceinline__ void load_tile(int access, char* dst, const char* src
   else load_tile<1, ROWB>(dst, src, pitch, rows, valid);
 }
 
+__device__ __forceinline__ void close_tiles() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// until at most N of the closed groups are still on their way
+template <int N>
 __device__ __forceinline__ void wait_tiles() {
-  asm volatile("cp.async.commit_group;\ncp.async.wait_group 0;" ::: "memory");
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 struct Source {  // x or f of a call: rows, or rows in 8 bits
@@ -191,32 +232,68 @@ __device__ __forceinline__ void load_rows(char* dst, const Rows& r, int access, 
 
 // ---- the recurrence ------------------------------------------------------------------
 
-// The smaller of sigmoid(f) and 1 - sigmoid(f), with f's sign.
-__device__ __forceinline__ float gate_of(float f) {
-  const float u = __expf(-fabsf(f));
-  return copysignf(__fdividef(u, 1.f + u), f);
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-__device__ __forceinline__ bool is_decay(float s) { return __float_as_int(s) < 0; }
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// c of a gate's f (with its bias); below 2^-126 it counts as zero.
+template <int V>
+__device__ __forceinline__ Vals<V> gate_of(Vals<V> f) {
+  const Vals<V> t = mul(f, all<V>(1.4426950408889634f));
+  Vals<V> u, r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) u.v[i] = exp2_fast(-fabsf(t.v[i]));
+  r = add(u, all<V>(1.f));
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = reciprocal(r.v[i]);
+  r = mul(u, r);
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    r.v[i] = __uint_as_float(__float_as_uint(r.v[i]) | (~__float_as_uint(f.v[i]) & 0x80000000u));
+  return r;
+}
+// c is -(1 - a)
+__device__ __forceinline__ bool is_rest(float c) { return __float_as_int(c) < 0; }
 // a h
-__device__ __forceinline__ float decayed(float s, float h) { return fmaf(-s, h, is_decay(s) ? 0.f : h); }
+template <int V>
+__device__ __forceinline__ Vals<V> decayed(Vals<V> c, Vals<V> h) {
+  Vals<V> base;
+#pragma unroll
+  for (int i = 0; i < V; ++i) base.v[i] = is_rest(c.v[i]) ? h.v[i] : 0.f;
+  return fma(c, h, base);
+}
 // one step of the recurrence
-__device__ __forceinline__ float stepped(bool complement, float s, float x, float h) {
-  return complement ? fmaf(s, x - h, is_decay(s) ? x : h) : fmaf(-s, h, is_decay(s) ? x : h + x);
+template <bool COMPLEMENT, int V>
+__device__ __forceinline__ Vals<V> stepped(Vals<V> c, Vals<V> x, Vals<V> h) {
+  const Vals<V> other = COMPLEMENT ? h : add(h, x);
+  Vals<V> base;
+#pragma unroll
+  for (int i = 0; i < V; ++i) base.v[i] = is_rest(c.v[i]) ? other.v[i] : x.v[i];
+  return fma(c, COMPLEMENT ? sub(h, x) : h, base);
 }
 
 // ---- segments joined while the CTAs run ------------------------------------------------
 
-__device__ __forceinline__ int flag_at(const int* p) {
-  int v;
-  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
+__device__ __forceinline__ uint64_t word_of(float value, uint32_t mark) {
+  return static_cast<uint64_t>(mark) << 32 | __float_as_uint(value);
+}
+__device__ __forceinline__ void publish(uint64_t* p, uint64_t w) {
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(w) : "memory");
+}
+__device__ __forceinline__ uint64_t published(const uint64_t* p) {
+  uint64_t w;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(w) : "l"(p) : "memory");
+  return w;
 }
 
-__device__ __forceinline__ void raise(int* p) {
-  asm volatile("st.release.gpu.global.s32 [%0], 1;" ::"l"(p) : "memory");
-}
-
-// What one warp has to do with the other segments of its sequence: position p of
+// What a CTA has to do with the other segments of its sequence: position p of
 // `count` in the chain's direction, whose slots lie at origin + dir * position.
 template <typename T>
 struct Links {
@@ -224,59 +301,82 @@ struct Links {
   const Chain& C;
   int lane, slab, origin, dir, p, count;
 
-  __device__ __forceinline__ int slot(int at) const { return origin + dir * at; }
-  __device__ __forceinline__ int* flag(int at) const {
-    return C.flags + (static_cast<long long>(slot(at)) * C.slabs + slab) * 2;
-  }
   __device__ __forceinline__ long long place(int at) const {
-    return (static_cast<long long>(slot(at)) * C.slabs + slab) * CH + lane * V;
+    return (static_cast<long long>(origin + dir * at) * C.slabs + slab) * CH + lane * V;
   }
+  __device__ __forceinline__ int base() const { return (p - 1) / kChain * kChain; }  // of p > 0
   // The segment's own map, for those behind it.
-  __device__ __forceinline__ void publish_map(const float (&a)[V], const float (&h)[V]) const {
+  __device__ __forceinline__ void publish_map(const Vals<V>& a, const Vals<V>& h) const {
     if (p + 1 >= count) return;
 #pragma unroll
-    for (int v = 0; v < V; ++v) __stcg(C.maps + place(p) + v, make_float2(a[v], h[v]));
-    __threadfence();
-    __syncwarp();
-    if (lane == 0) raise(flag(p));
+    for (int v = 0; v < V; ++v)
+      publish(C.maps + place(p) + v, word_of(h.v[v], __float_as_uint(a.v[v]) | 0x80000000u));
   }
-  __device__ __forceinline__ void publish_state(const float (&h)[V]) const {
+  __device__ __forceinline__ void publish_state(const Vals<V>& h) const {
     if (p + 1 >= count || p % kChain) return;
 #pragma unroll
-    for (int v = 0; v < V; ++v) __stcg(C.states + place(p) + v, h[v]);
-    __threadfence();
-    __syncwarp();
-    if (lane == 0) raise(flag(p) + 1);
+    for (int v = 0; v < V; ++v) publish(C.states + place(p) + v, word_of(h.v[v], 1u));
   }
-  // The state that enters position p > 0.
-  __device__ __forceinline__ void entering(float (&h)[V]) const {
-    const int base = (p - 1) / kChain * kChain, n = p - base;
-    const int* f = lane < n ? flag(base + lane) : lane == kChain ? flag(base) + 1 : nullptr;
-    bool waiting = f != nullptr;
-    for (uint32_t polls = 0; __any_sync(0xffffffffu, waiting); ++polls) {
-      if (waiting && flag_at(f)) waiting = false;
+  // Words that another CTA publishes, by the whole warp.
+  __device__ __forceinline__ void fetch(const uint64_t* from, uint64_t (&w)[V]) const {
+    for (uint32_t polls = 0;; ++polls) {
+      bool there = true;
+#pragma unroll
+      for (int v = 0; v < V; ++v) w[v] = published(from + v);
+#pragma unroll
+      for (int v = 0; v < V; ++v) there = there && w[v] != 0;
+      if (__all_sync(0xffffffffu, there)) return;
       if (polls % 256 == 255) {  // (once a wait has run out, the others of the call need not)
-        const bool out = polls > kPolls || flag_at(C.gave_up);
-        if (waiting && out) {
-          atomicExch(C.gave_up, 1);
-          atomicExch(&g_recurrence_status, TO_ERR_TIMEOUT);
-          waiting = false;
+        bool out = polls > kPolls;
+        if (lane == 0 && !out) out = *reinterpret_cast<volatile int*>(C.gave_up) != 0;
+        if (__any_sync(0xffffffffu, out)) {
+          if (lane == 0) {
+            atomicExch(C.gave_up, 1);
+            atomicExch(&g_recurrence_status, TO_ERR_TIMEOUT);
+          }
+          return;
         }
       }
     }
-    __syncwarp();
+  }
+  // What enters position p > 0, into shared memory by all warps: the state at base()
+  // into enter, the maps from there on into before.
+  __device__ __forceinline__ void gather(int warp, float (&enter)[CH], float2 (&before)[kChain][CH]) const {
+    const int b = base(), n = p - b;
+    uint64_t w[V];
+    static_assert(kChain == kWarps, "a warp fetches one map");
+    if (warp < n) {
+      fetch(C.maps + place(b + warp), w);
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = __ldcg(C.states + place(base) + v);
-#pragma unroll 8
-    for (int k = 0; k < n; ++k) {
+      for (int v = 0; v < V; ++v)
+        before[warp][lane * V + v] = make_float2(__uint_as_float(static_cast<uint32_t>(w[v] >> 32) & 0x7fffffffu),
+                                              __uint_as_float(static_cast<uint32_t>(w[v])));
+    }
+    if (warp == kWarps - 1) {
+      fetch(C.states + place(b), w);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float2 m = __ldcg(C.maps + place(base + k) + v);
-        h[v] = fmaf(m.x, h[v], m.y);
-      }
+      for (int v = 0; v < V; ++v) enter[lane * V + v] = __uint_as_float(static_cast<uint32_t>(w[v]));
     }
   }
 };
+
+// A lane's values of an array in shared memory, and maps there applied to a state.
+template <int V>
+__device__ __forceinline__ Vals<V> lane_of(const float* p, int lane) {
+  Vals<V> r;
+#pragma unroll
+  for (int v = 0; v < V; ++v) r.v[v] = p[lane * V + v];
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vals<V> mapped(const float2* m, int lane, Vals<V> h) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const float2 x = m[lane * V + v];
+    h.v[v] = fmaf(x.x, h.v[v], x.y);
+  }
+  return h;
+}
 
 // ---- forward -----------------------------------------------------------------------
 
@@ -292,7 +392,6 @@ struct ForwardArgs {
   const float* state_in;
   float* state_out;
   float* saved;
-  int complement;
 };
 
 template <typename T>
@@ -348,139 +447,122 @@ __device__ __forceinline__ void keep_tile(const char* tile, const Packed& out, i
   }
 }
 
-template <typename T, bool KEEP>
+template <typename T, bool KEEP, bool COMPLEMENT>
 __global__ void __launch_bounds__(kThreads, 3) forward_kernel(const __grid_constant__ ForwardArgs A) {
   using L = Lane<T>;
+  using P = typename L::P;
   constexpr int V = L::kVec, CH = L::kChannels;
-  __shared__ alignas(16) char xs[kSegment * kRowBytes];
-  __shared__ alignas(16) char fs[kSegment * kRowBytes];
-  __shared__ float2 maps[kWarps][CH];
-  __shared__ float enter[CH];
-  __shared__ Item items[2];
+  extern __shared__ __align__(16) char tiles[];  // two stages of x and f
+  __shared__ alignas(16) float2 maps[kWarps][CH], before[kChain][CH];
+  __shared__ alignas(16) float enter[CH];
+  __shared__ Item items[3];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Chain& C = A.C;
-  const bool complement = A.complement;
-  unsigned long long ticket = blockIdx.x;
-  auto take = [&] {
-    if (C.ticket) {
-      if (lane == 0) ticket = atomicAdd(C.ticket, 1ull);
-    } else {
-      ticket += gridDim.x;
+  unsigned ticket = blockIdx.x;
+  auto fetch = [&](const Item& it, char* to) {
+    if (it.slot >= 0 && it.n > 0) {
+      load_rows<T>(to, A.x, A.x_access, it, it.slab * CH, C.channels);
+      load_rows<T>(to + kTile, A.f, A.f_access, it, it.slab * CH, C.channels);
     }
-  };
-  auto fetch = [&](const Item& it) {
-    if (it.tile < 0 || it.n <= 0) return;
-    load_rows<T>(xs, A.x, A.x_access, it, it.slab * CH, C.channels);
-    load_rows<T>(fs, A.f, A.f_access, it, it.slab * CH, C.channels);
+    close_tiles();
   };
   auto no_slot = [](const Item&) {};
   if (warp == kWarps - 1) {
-    if (C.ticket && lane == 0) ticket = atomicAdd(C.ticket, 1ull);
-    const Item first = next_item<false>(C, ticket, lane, no_slot);
-    if (!C.ticket && first.tile >= 0) ticket = first.tile;
-    if (lane == 0) items[0] = first;
+    for (int k = 0; k < 2; ++k) {
+      if (k || C.ticket) next_ticket(C, ticket, lane);
+      const Item first = next_item<false>(C, ticket, lane, no_slot);
+      if (lane == 0) items[k] = first;
+    }
   }
   __syncthreads();
-  fetch(items[0]);
-  for (int cur = 0;; cur ^= 1) {
-    const Item it = items[cur];
-    if (it.tile < 0) break;
-    wait_tiles();
+  fetch(items[0], tiles);
+  fetch(items[1], tiles + 2 * kTile);
+  for (int at = 0, stage = 0;; at = at == 2 ? 0 : at + 1, stage ^= 1) {
+    const Item it = items[at];
+    if (it.slot < 0) break;
+    char* const xs = tiles + stage * 2 * kTile;
+    char* const fs = xs + kTile;
+    Item& later = items[at == 0 ? 2 : at - 1];  // the next but one
+    const int ch = it.slab * CH, c0 = ch + lane * V, nc = min(V, C.channels - c0), t0 = warp * kTok;
+    P bias = all<V>(0.f);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (A.bias && v < nc) bias.v[v] = __ldg(A.bias + c0 + v);
+    wait_tiles<1>();
     __syncthreads();
-    if (warp == kWarps - 1) take();
-    const int ch = it.slab * CH, c0 = ch + lane * V, nc = min(V, C.channels - c0);
+    if (warp == kWarps - 1) next_ticket(C, ticket, lane);
     if (KEEP) {
       if (A.keep_x.codes) keep_tile<T>(xs, A.keep_x, A.keep_access, it, ch, C.channels);
       if (A.keep_f.codes) keep_tile<T>(fs, A.keep_f, A.keep_access, it, ch, C.channels);
     }
-    float bias[V], a[V], h[V], s[kTok][V];
-    uint32_t x[kTok];
+    // the map of a warp's first tokens, up to every one of them
+    P a[kTok], h[kTok];
+    auto reduce = [&](auto whole) {
+      P at = all<V>(1.f), ht = all<V>(0.f);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      bias[v] = A.bias && v < nc ? __ldg(A.bias + c0 + v) : 0.f;
-      a[v] = 1.f, h[v] = 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      const int t = warp * kTok + i;
-      x[i] = 0;
-#pragma unroll
-      for (int v = 0; v < V; ++v) s[i][v] = 0.f;  // (a token that is not there changes nothing)
-      if (t < it.n) {
-        x[i] = *reinterpret_cast<const uint32_t*>(xs + t * kRowBytes + lane * 4);
-        float f[V];
-        L::unpack(*reinterpret_cast<const uint32_t*>(fs + t * kRowBytes + lane * 4), f);
-#pragma unroll
-        for (int v = 0; v < V; ++v) s[i][v] = gate_of(f[v] + bias[v]);
+      for (int i = 0; i < kTok; ++i) {
+        const uint32_t x = *reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4);
+        const uint32_t f = *reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4);
+        if (decltype(whole)::value || t0 + i < it.n) {
+          const P c = gate_of(add(L::unpack(f), bias));
+          at = decayed(c, at);
+          ht = stepped<COMPLEMENT>(c, L::unpack(x), ht);
+        }
+        a[i] = at, h[i] = ht;
       }
-      float xv[V];
-      L::unpack(x[i], xv);
+    };
+    if (it.n == kSegment) reduce(std::true_type{});
+    else reduce(std::false_type{});
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        a[v] = decayed(s[i][v], a[v]);
-        h[v] = stepped(complement, s[i][v], xv[v], h[v]);
-      }
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) maps[warp][lane * V + v] = make_float2(a[v], h[v]);
+    for (int v = 0; v < V; ++v) maps[warp][lane * V + v] = make_float2(a[kTok - 1].v[v], h[kTok - 1].v[v]);
     if (warp == kWarps - 1) {
       const Item next = next_item<false>(C, ticket, lane, no_slot);
-      if (!C.ticket && next.tile >= 0) ticket = next.tile;
-      if (lane == 0) items[cur ^ 1] = next;
+      if (lane == 0) later = next;
     }
     __syncthreads();
-    fetch(items[cur ^ 1]);  // the tiles have been read
+    fetch(later, xs);  // the tiles have been read
+    const Links<T> links{C, lane, it.slab, it.slot - it.idx, 1, it.idx, it.count};
+    const long long state = A.slots ? __ldg(A.slots + it.seq) : it.seq;
+    const bool has_state = state >= 0 && state < A.num_slots;
+    P sa = all<V>(1.f), sh = all<V>(0.f);  // the segment's map
     if (warp == 0) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) a[v] = 1.f, h[v] = 0.f;
+      for (int w = 0; w < kWarps; ++w) {
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w)
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float2 m = maps[w][lane * V + v];
-          a[v] *= m.x;
-          h[v] = fmaf(m.x, h[v], m.y);
-        }
-      const Links<T> links{C, lane, it.slab, it.slot - it.idx, 1, it.idx, it.count};
-      links.publish_map(a, h);
-      const long long state = A.slots ? __ldg(A.slots + it.seq) : it.seq;
-      const bool has_state = state >= 0 && state < A.num_slots;
-      float e[V];
-      if (it.idx > 0) {
-        links.entering(e);
-      } else {
+        for (int v = 0; v < V; ++v) sa.v[v] *= maps[w][lane * V + v].x;
+        sh = mapped(maps[w], lane, sh);
+      }
+      links.publish_map(sa, sh);
+      if (it.idx == 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v)
-          e[v] = A.state_in && has_state && v < nc ? A.state_in[state * C.channels + c0 + v] : 0.f;
+          enter[lane * V + v] = A.state_in && has_state && v < nc ? A.state_in[state * C.channels + c0 + v] : 0.f;
       }
+    }
+    if (it.idx > 0) links.gather(warp, enter, before);
+    __syncthreads();
+    P e = lane_of<V>(enter, lane);
+    const int n = it.idx > 0 ? it.idx - links.base() : 0;
+    for (int k = 0; k < n; ++k) e = mapped(before[k], lane, e);
+    if (warp == 0) {
       links.publish_state(e);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        enter[lane * V + v] = e[v];
-        if (v < nc) {
-          if (A.saved) A.saved[static_cast<long long>(it.slot) * C.channels + c0 + v] = e[v];
-          if (A.state_out && has_state && it.idx == it.count - 1)
-            A.state_out[state * C.channels + c0 + v] = fmaf(a[v], e[v], h[v]);
-        }
+        if (v >= nc) continue;
+        if (A.saved) A.saved[static_cast<long long>(it.slot) * C.channels + c0 + v] = e.v[v];
+        if (A.state_out && has_state && it.idx == it.count - 1)
+          A.state_out[state * C.channels + c0 + v] = fmaf(sa.v[v], e.v[v], sh.v[v]);
       }
     }
-    __syncthreads();
+    for (int w = 0; w < warp; ++w) e = mapped(maps[w], lane, e);
+    T* row = seq::row_ptr<T>(A.h, it.row0 + static_cast<long long>(t0), 0) + c0;
+    if (A.pairs && nc == V && it.n == kSegment) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = enter[lane * V + v];
-    for (int w = 0; w < warp; ++w)
+      for (int i = 0; i < kTok; ++i, row += A.h.ts) *reinterpret_cast<uint32_t*>(row) = L::pack(fma(a[i], e, h[i]));
+    } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float2 m = maps[w][lane * V + v];
-        h[v] = fmaf(m.x, h[v], m.y);
-      }
-    T* row = seq::row_ptr<T>(A.h, it.row0 + static_cast<long long>(warp * kTok), 0) + c0;
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      float xv[V];
-      L::unpack(x[i], xv);
-#pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = stepped(complement, s[i][v], xv[v], h[v]);
-      if (warp * kTok + i < it.n) store_word<T>(row + i * A.h.ts, L::pack(h), nc, A.pairs);
+      for (int i = 0; i < kTok; ++i)
+        if (t0 + i < it.n) store_word<T>(row + i * A.h.ts, L::pack(fma(a[i], e, h[i])), nc, A.pairs);
     }
   }
 }
@@ -497,32 +579,32 @@ struct BackwardArgs {
   const float* dstate_out;
   float* dstate_in;
   float* partial;  // [slots][slabs * kChannels] sums of df; null: not wanted
-  int complement;
 };
 
 // The gradients' own chain runs from a sequence's end: what leaves token t is a_t G_t,
 // with G_t = dh_t + what left token t + 1; the map of some tokens is their A and what
 // leaves them when nothing enters.  h runs forwards again from the saved state (so
 // the map (A, H) of each warp is needed too).
-template <typename T>
+template <typename T, bool COMPLEMENT>
 __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_constant__ BackwardArgs A) {
   using L = Lane<T>;
+  using P = typename L::P;
   constexpr int V = L::kVec, CH = L::kChannels, kGroups = CH / seq::kGroup8;
   extern __shared__ __align__(16) char tiles[];
   char* const xs = tiles;
-  char* const fs = tiles + kSegment * kRowBytes;
-  char* const gs = tiles + 2 * kSegment * kRowBytes;
-  __shared__ float2 maps[kWarps][CH];
-  __shared__ float ends[kWarps][CH], enter[CH], sums[kWarps][CH];
+  char* const fs = tiles + kTile;
+  char* const gs = tiles + 2 * kTile;
+  // maps: of h, ends: of the gradients' chain (they share A)
+  __shared__ alignas(16) float2 maps[kWarps][CH], ends[kWarps][CH], before[kChain][CH];
+  __shared__ alignas(16) float enter[CH], sums[kWarps][CH];
   __shared__ uint8_t scales[2][kSegment][kGroups];
   __shared__ Item items[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Chain& C = A.C;
-  const bool complement = A.complement;
-  unsigned long long ticket = blockIdx.x;
+  unsigned ticket = blockIdx.x;
   uint8_t byte[kGroups] = {};  // scales of the next tile, this thread's row
   auto fetch = [&](const Item& it) {
-    if (it.tile < 0 || it.n <= 0) return;
+    if (it.slot < 0 || it.n <= 0) return;
     const int ch = it.slab * CH;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -542,185 +624,178 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
       }
     }
     load_rows<T>(gs, A.dh, A.dh_access, it, ch, C.channels);
+    close_tiles();
   };
   auto no_slot = [&](const Item& it) {  // its sums count too
     if (A.partial)
 #pragma unroll
-      for (int v = 0; v < V; ++v) A.partial[it.tile * CH + lane * V + v] = 0.f;
+      for (int v = 0; v < V; ++v)
+        A.partial[(static_cast<long long>(it.slot) * C.slabs + it.slab) * CH + lane * V + v] = 0.f;
   };
   if (warp == kWarps - 1) {
-    if (C.ticket && lane == 0) ticket = atomicAdd(C.ticket, 1ull);
+    if (C.ticket) next_ticket(C, ticket, lane);
     const Item first = next_item<true>(C, ticket, lane, no_slot);
-    if (!C.ticket && first.tile >= 0)
-      ticket = static_cast<unsigned long long>(C.slots - 1 - first.slot) * C.slabs + first.slab;
     if (lane == 0) items[0] = first;
   }
   __syncthreads();
   fetch(items[0]);
   for (int cur = 0;; cur ^= 1) {
     const Item it = items[cur];
-    if (it.tile < 0) break;
-    wait_tiles();
+    if (it.slot < 0) break;
+    const int ch = it.slab * CH, c0 = ch + lane * V, nc = min(V, C.channels - c0), t0 = warp * kTok;
+    P bias = all<V>(0.f), first = all<V>(0.f);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (v >= nc) continue;
+      if (A.bias) bias.v[v] = __ldg(A.bias + c0 + v);
+      first.v[v] = __ldg(A.saved + static_cast<long long>(it.slot) * C.channels + c0 + v);
+    }
+    wait_tiles<0>();
 #pragma unroll
     for (int j = 0; j < kGroups; ++j) scales[threadIdx.x / kSegment][threadIdx.x % kSegment][j] = byte[j];
     __syncthreads();
-    if (warp == kWarps - 1) {
-      if (C.ticket) {
-        if (lane == 0) ticket = atomicAdd(C.ticket, 1ull);
-      } else {
-        ticket += gridDim.x;
-      }
-    }
-    const int ch = it.slab * CH, c0 = ch + lane * V, nc = min(V, C.channels - c0);
+    if (warp == kWarps - 1) next_ticket(C, ticket, lane);
     const int group = lane * V / seq::kGroup8;
-    float a[V], h[V], r[V], bias[V], first[V], s[kTok][V], w[kTok][V];
+    P a = all<V>(1.f), h = all<V>(0.f), r = all<V>(0.f), c[kTok];
     uint32_t x[kTok], g[kTok];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      bias[v] = A.bias && v < nc ? __ldg(A.bias + c0 + v) : 0.f;
-      first[v] = v < nc ? __ldg(A.saved + static_cast<long long>(it.slot) * C.channels + c0 + v) : 0.f;
-      a[v] = 1.f, h[v] = r[v] = 0.f;
-    }
-    auto value = [&](const char* tile, int k, int t, float (&out)[V]) {  // of rows in 8 bits
+    auto value = [&](const char* tile, int k, int t) {  // of rows in 8 bits
       const float scale = seq::scale_of(scales[k][t][group]);
       const int8_t* code = reinterpret_cast<const int8_t*>(tile) + t * CH + lane * V;
-#pragma unroll
-      for (int v = 0; v < V; ++v) out[v] = seq::code_to_f32(code[v], scale);
+      P out;
+      if constexpr (V == 2) {  // (one access)
+        const uint16_t both = *reinterpret_cast<const uint16_t*>(code);
+        out.v[0] = seq::code_to_f32(static_cast<int8_t>(both & 0xff), scale);
+        out.v[1] = seq::code_to_f32(static_cast<int8_t>(both >> 8), scale);
+      } else {
+        out.v[0] = seq::code_to_f32(code[0], scale);
+      }
+      return out;
     };
+    if (A.x.packed.codes) {
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) x[i] = L::pack(value(xs, 0, t0 + i));  // (7 bits and a sign: exact)
+    } else {
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) x[i] = *reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4);
+    }
+    if (A.f.packed.codes) {
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) c[i] = value(fs, 1, t0 + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kTok; ++i)
+        c[i] = L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4));
+    }
 #pragma unroll
     for (int i = 0; i < kTok; ++i) {
-      const int t = warp * kTok + i;
-      x[i] = g[i] = 0;
+      g[i] = *reinterpret_cast<const uint32_t*>(gs + (t0 + i) * kRowBytes + lane * 4);
+      c[i] = gate_of(add(c[i], bias));
+    }
+    if (it.n < kSegment) {  // a token that is not there changes nothing
 #pragma unroll
-      for (int v = 0; v < V; ++v) s[i][v] = 0.f;
-      if (t < it.n) {
-        float f[V], xv[V];
-        if (A.x.packed.codes) {
-          value(xs, 0, t, xv);
-          x[i] = L::pack(xv);  // (7 bits and a sign: exact)
-        } else {
-          x[i] = *reinterpret_cast<const uint32_t*>(xs + t * kRowBytes + lane * 4);
-        }
-        if (A.f.packed.codes) value(fs, 1, t, f);
-        else L::unpack(*reinterpret_cast<const uint32_t*>(fs + t * kRowBytes + lane * 4), f);
-        g[i] = *reinterpret_cast<const uint32_t*>(gs + t * kRowBytes + lane * 4);
-#pragma unroll
-        for (int v = 0; v < V; ++v) s[i][v] = gate_of(f[v] + bias[v]);
-      }
-      float xv[V];
-      L::unpack(x[i], xv);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        a[v] = decayed(s[i][v], a[v]);
-        h[v] = stepped(complement, s[i][v], xv[v], h[v]);
-      }
+      for (int i = 0; i < kTok; ++i)
+        if (t0 + i >= it.n) x[i] = g[i] = 0, c[i] = all<V>(-0.f);
     }
 #pragma unroll
-    for (int i = kTok - 1; i >= 0; --i) {
-      float gv[V];
-      L::unpack(g[i], gv);
-#pragma unroll
-      for (int v = 0; v < V; ++v) r[v] = decayed(s[i][v], gv[v] + r[v]);
+    for (int i = 0; i < kTok; ++i) {
+      a = decayed(c[i], a);
+      h = stepped<COMPLEMENT>(c[i], L::unpack(x[i]), h);
     }
+#pragma unroll
+    for (int i = kTok - 1; i >= 0; --i) r = decayed(c[i], add(L::unpack(g[i]), r));
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      maps[warp][lane * V + v] = make_float2(a[v], h[v]);
-      ends[warp][lane * V + v] = r[v];
+      maps[warp][lane * V + v] = make_float2(a.v[v], h.v[v]);
+      ends[warp][lane * V + v] = make_float2(a.v[v], r.v[v]);
     }
     if (warp == kWarps - 1) {
       const Item next = next_item<true>(C, ticket, lane, no_slot);
-      if (!C.ticket && next.tile >= 0)
-        ticket = static_cast<unsigned long long>(C.slots - 1 - next.slot) * C.slabs + next.slab;
       if (lane == 0) items[cur ^ 1] = next;
     }
     __syncthreads();
     fetch(items[cur ^ 1]);
+    const int p = it.count - 1 - it.idx;
+    const Links<T> links{C, lane, it.slab, it.slot + p, -1, p, it.count};
+    const long long state = static_cast<long long>(it.seq) * C.channels + c0;
     if (warp == 0) {
+      a = all<V>(1.f), r = all<V>(0.f);
 #pragma unroll
-      for (int v = 0; v < V; ++v) a[v] = 1.f, r[v] = 0.f;
+      for (int k = kWarps - 1; k >= 0; --k) {
 #pragma unroll
-      for (int k = kWarps - 1; k >= 0; --k)
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float m = maps[k][lane * V + v].x;
-          a[v] *= m;
-          r[v] = fmaf(m, r[v], ends[k][lane * V + v]);
-        }
-      const int p = it.count - 1 - it.idx;
-      const Links<T> links{C, lane, it.slab, it.slot + p, -1, p, it.count};
-      links.publish_map(a, r);
-      float e[V];
-      const long long state = static_cast<long long>(it.seq) * C.channels + c0;
-      if (p > 0) {
-        links.entering(e);
-      } else {
-#pragma unroll
-        for (int v = 0; v < V; ++v) e[v] = A.dstate_out && v < nc ? __ldg(A.dstate_out + state + v) : 0.f;
+        for (int v = 0; v < V; ++v) a.v[v] *= ends[k][lane * V + v].x;
+        r = mapped(ends[k], lane, r);
       }
-      links.publish_state(e);
+      links.publish_map(a, r);
+      if (p == 0) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        enter[lane * V + v] = e[v];
-        if (A.dstate_in && it.idx == 0 && v < nc) A.dstate_in[state + v] = fmaf(a[v], e[v], r[v]);
+        for (int v = 0; v < V; ++v) enter[lane * V + v] = A.dstate_out && v < nc ? __ldg(A.dstate_out + state + v) : 0.f;
       }
     }
     // the states before every token, and df_t / G_t
-#pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = first[v];
-    for (int k = 0; k < warp; ++k)
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float2 m = maps[k][lane * V + v];
-        h[v] = fmaf(m.x, h[v], m.y);
-      }
+    P w[kTok];
+    for (int k = 0; k < warp; ++k) first = mapped(maps[k], lane, first);
 #pragma unroll
     for (int i = 0; i < kTok; ++i) {
-      float xv[V];
-      L::unpack(x[i], xv);
+      const P xv = L::unpack(x[i]), square = mul(c[i], c[i]);
+      P slope;  // a (1 - a)
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float small = fabsf(s[i][v]);
-        w[i][v] = fmaf(-small, small, small) * (complement ? h[v] - xv[v] : h[v]);
-        h[v] = stepped(complement, s[i][v], xv[v], h[v]);
-      }
+      for (int v = 0; v < V; ++v) slope.v[v] = fabsf(c[i].v[v]) - square.v[v];
+      w[i] = mul(slope, COMPLEMENT ? sub(first, xv) : first);
+      first = stepped<COMPLEMENT>(c[i], xv, first);
     }
+    if (p > 0) links.gather(warp, enter, before);
     __syncthreads();
-    float sum[V];
+    P e = lane_of<V>(enter, lane);
+    const int n = p > 0 ? p - links.base() : 0;
+    for (int k = 0; k < n; ++k) e = mapped(before[k], lane, e);
+    if (warp == 0) {
+      links.publish_state(e);
 #pragma unroll
-    for (int v = 0; v < V; ++v) r[v] = enter[lane * V + v], sum[v] = 0.f;
-    for (int k = kWarps - 1; k > warp; --k)
-#pragma unroll
-      for (int v = 0; v < V; ++v) r[v] = fmaf(maps[k][lane * V + v].x, r[v], ends[k][lane * V + v]);
-    T* dx = seq::row_ptr<T>(A.dx, it.row0 + static_cast<long long>(warp * kTok), 0) + c0;
-    T* df = seq::row_ptr<T>(A.df, it.row0 + static_cast<long long>(warp * kTok), 0) + c0;
-#pragma unroll
-    for (int i = kTok - 1; i >= 0; --i) {
-      float gv[V], ox[V], of[V];
-      L::unpack(g[i], gv);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float G = gv[v] + r[v];
-        // (1 - a) G is s G, or G less a G
-        r[v] = decayed(s[i][v], G);
-        ox[v] = complement ? (is_decay(s[i][v]) ? fmaf(s[i][v], G, G) : s[i][v] * G) : G;
-        of[v] = G * w[i][v];
-      }
-      if (warp * kTok + i < it.n) {
-        store_word<T>(dx + i * A.dx.ts, L::pack(ox), nc, A.pairs);
-        store_word<T>(df + i * A.df.ts, L::pack(of), nc, A.pairs);
-#pragma unroll
-        for (int v = 0; v < V; ++v) sum[v] += of[v];
-      }
+      for (int v = 0; v < V; ++v)
+        if (A.dstate_in && it.idx == 0 && v < nc) A.dstate_in[state + v] = fmaf(a.v[v], e.v[v], r.v[v]);
     }
+    P sum = all<V>(0.f);
+    for (int k = kWarps - 1; k > warp; --k) e = mapped(ends[k], lane, e);
+    T* dx = seq::row_ptr<T>(A.dx, it.row0 + static_cast<long long>(t0), 0) + c0;
+    T* df = seq::row_ptr<T>(A.df, it.row0 + static_cast<long long>(t0), 0) + c0;
+    auto finish = [&](auto whole) {
+      constexpr bool kWhole = decltype(whole)::value;
+#pragma unroll
+      for (int i = kTok - 1; i >= 0; --i) {
+        if (!kWhole && t0 + i >= it.n) continue;
+        const P G = add(L::unpack(g[i]), e), of = mul(G, w[i]);
+        P ox = G;
+        if (COMPLEMENT) {  // (1 - a) G
+          P base, minus;
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            base.v[v] = is_rest(c[i].v[v]) ? 0.f : G.v[v];
+            minus.v[v] = -G.v[v];
+          }
+          ox = fma(c[i], minus, base);
+        }
+        e = decayed(c[i], G);
+        if (kWhole) {
+          *reinterpret_cast<uint32_t*>(dx + i * A.dx.ts) = L::pack(ox);
+          *reinterpret_cast<uint32_t*>(df + i * A.df.ts) = L::pack(of);
+        } else {
+          store_word<T>(dx + i * A.dx.ts, L::pack(ox), nc, A.pairs);
+          store_word<T>(df + i * A.df.ts, L::pack(of), nc, A.pairs);
+        }
+        sum = add(sum, of);
+      }
+    };
+    if (A.pairs && nc == V && it.n == kSegment) finish(std::true_type{});
+    else finish(std::false_type{});
     if (A.partial) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) sums[warp][lane * V + v] = sum[v];
+      for (int v = 0; v < V; ++v) sums[warp][lane * V + v] = sum.v[v];
       __syncthreads();
       if (threadIdx.x < CH) {
         float total = 0.f;
 #pragma unroll
         for (int k = 0; k < kWarps; ++k) total += sums[k][threadIdx.x];
-        A.partial[it.tile * CH + threadIdx.x] = total;
+        A.partial[(static_cast<long long>(it.slot) * C.slabs + it.slab) * CH + threadIdx.x] = total;
       }
     }
   }
@@ -775,8 +850,10 @@ __global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ StepA
     seq::load_vec<T, V>(seq::row_ptr<const T>(A.x, token, 0) + c, x);
     seq::load_vec<T, V>(seq::row_ptr<const T>(A.f, token, 0) + c, f);
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      h[v] = stepped(A.complement, gate_of(f[v] + (A.bias ? __ldg(A.bias + c + v) : 0.f)), x[v], h[v]);
+    for (int v = 0; v < V; ++v) {
+      const Vals<1> g = gate_of(Vals<1>{{f[v] + (A.bias ? __ldg(A.bias + c + v) : 0.f)}}), xv{{x[v]}}, hv{{h[v]}};
+      h[v] = (A.complement ? stepped<true>(g, xv, hv) : stepped<false>(g, xv, hv)).v[0];
+    }
     seq::store_vec<float, V>(state, h);
     seq::store_vec<T, V>(out, h);
   }
@@ -812,17 +889,16 @@ int slabs_of(const to_gated_recurrence_desc& d) {
 int slots_of(const to_gated_recurrence_desc& d) { return static_cast<int>(d.tokens / kSegment) + d.nseq; }
 bool chained(const to_gated_recurrence_desc& d) { return d.tokens > kSegment && d.nseq > 0; }
 
-struct Layout {  // of the workspace: the counter and the flags, the maps, the states, the partial sums
-  size_t flags, maps, states, partial, end;
+struct Layout {  // of the workspace: the counter, the maps and the states (cleared), the partial sums
+  size_t maps, states, partial, end;
 };
 Layout layout_of(const to_gated_recurrence_desc& d, bool backward) {
-  const size_t tiles = size_t(slots_of(d)) * slabs_of(d), values = tiles * channels_of_tile(d);
+  const size_t values = size_t(slots_of(d)) * slabs_of(d) * channels_of_tile(d);
   Layout l{};
   if (chained(d)) {
-    l.flags = kAlign;
-    l.maps = l.flags + padded(tiles * 2 * sizeof(int));
-    l.states = l.maps + padded(values * sizeof(float2));
-    l.partial = l.states + padded(values * sizeof(float));
+    l.maps = kAlign;
+    l.states = l.maps + padded(values * sizeof(uint64_t));
+    l.partial = l.states + padded(values * sizeof(uint64_t));
   }
   l.end = l.partial + (backward && d.nseq ? padded(values * sizeof(float)) : 0);
   return l;
@@ -866,11 +942,10 @@ Chain chain_of(const to_gated_recurrence_desc& d, const int32_t* cu, const Layou
   C.slots = slots_of(d);
   if (chained(d)) {
     char* w = static_cast<char*>(workspace);
-    C.ticket = reinterpret_cast<unsigned long long*>(w);
-    C.gave_up = reinterpret_cast<int*>(w + sizeof(unsigned long long));
-    C.flags = reinterpret_cast<int*>(w + l.flags);
-    C.maps = reinterpret_cast<float2*>(w + l.maps);
-    C.states = reinterpret_cast<float*>(w + l.states);
+    C.ticket = reinterpret_cast<unsigned*>(w);
+    C.gave_up = reinterpret_cast<int*>(w + sizeof(unsigned));
+    C.maps = reinterpret_cast<uint64_t*>(w + l.maps);
+    C.states = reinterpret_cast<uint64_t*>(w + l.states);
   }
   return C;
 }
@@ -965,21 +1040,29 @@ int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_rec
   A.state_in = a.state_in;
   A.state_out = a.state_out;
   A.saved = a.saved;
-  A.complement = d.complement;
   int dev = 0;
   const int sms = device_sm_count(&dev);
   if (sms <= 0) return -sms;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.maps, s));
+  if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.partial, s));
   const unsigned grid = grid_of(A.C, sms, 3);
-  const bool keep = a.keep_x.codes || a.keep_f.codes;
-  if (d.dtype == TO_BF16) {
-    if (keep) forward_kernel<__nv_bfloat16, true><<<grid, kThreads, 0, s>>>(A);
-    else forward_kernel<__nv_bfloat16, false><<<grid, kThreads, 0, s>>>(A);
-  } else {
-    if (keep) forward_kernel<float, true><<<grid, kThreads, 0, s>>>(A);
-    else forward_kernel<float, false><<<grid, kThreads, 0, s>>>(A);
-  }
+  constexpr size_t kShared = 4 * size_t(kTile);
+  static std::atomic<uint64_t> done[8];
+  auto launch = [&](auto t, auto keep, auto complement) {
+    auto* kernel = forward_kernel<decltype(t), decltype(keep)::value, decltype(complement)::value>;
+    const int which = 4 * (sizeof(t) == 4) + 2 * decltype(keep)::value + decltype(complement)::value;
+    if (int bad = seq::allow_shared(kernel, kShared, done[which])) return bad;
+    kernel<<<grid, kThreads, kShared, s>>>(A);
+    return ok();
+  };
+  auto with = [&](auto t) {
+    const bool keep = a.keep_x.codes || a.keep_f.codes;
+    if (d.complement)
+      return keep ? launch(t, std::true_type{}, std::true_type{}) : launch(t, std::false_type{}, std::true_type{});
+    return keep ? launch(t, std::true_type{}, std::false_type{}) : launch(t, std::false_type{}, std::false_type{});
+  };
+  st = d.dtype == TO_BF16 ? with(__nv_bfloat16{}) : with(float{});
+  if (st) return st;
   TO_CUDA_TRY(cudaGetLastError());
   return ok();
 }
@@ -1041,21 +1124,22 @@ int to_gated_recurrence_backward(const to_gated_recurrence_desc* desc, const to_
   A.dstate_out = a.dstate_out;
   A.dstate_in = a.dstate_in;
   A.partial = a.dbias ? reinterpret_cast<float*>(static_cast<char*>(a.workspace) + l.partial) : nullptr;
-  A.complement = d.complement;
   int dev = 0;
   const int sms = device_sm_count(&dev);
   if (sms <= 0) return -sms;
-  if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.maps, s));
+  if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.partial, s));
   const unsigned grid = grid_of(A.C, sms, 2);
-  constexpr size_t kShared = 3 * size_t(kSegment) * kRowBytes;
-  static std::atomic<uint64_t> done[2];
-  if (d.dtype == TO_BF16) {
-    if ((st = seq::allow_shared(backward_kernel<__nv_bfloat16>, kShared, done[0]))) return st;
-    backward_kernel<__nv_bfloat16><<<grid, kThreads, kShared, s>>>(A);
-  } else {
-    if ((st = seq::allow_shared(backward_kernel<float>, kShared, done[1]))) return st;
-    backward_kernel<float><<<grid, kThreads, kShared, s>>>(A);
-  }
+  constexpr size_t kShared = 3 * size_t(kTile);
+  static std::atomic<uint64_t> done[4];
+  auto launch = [&](auto t, auto complement) {
+    auto* kernel = backward_kernel<decltype(t), decltype(complement)::value>;
+    if (int bad = seq::allow_shared(kernel, kShared, done[2 * (sizeof(t) == 4) + decltype(complement)::value])) return bad;
+    kernel<<<grid, kThreads, kShared, s>>>(A);
+    return ok();
+  };
+  if (d.dtype == TO_BF16) st = d.complement ? launch(__nv_bfloat16{}, std::true_type{}) : launch(__nv_bfloat16{}, std::false_type{});
+  else st = d.complement ? launch(float{}, std::true_type{}) : launch(float{}, std::false_type{});
+  if (st) return st;
   TO_CUDA_TRY(cudaGetLastError());
   if (a.dbias) {
     bias_sum_kernel<<<(d.channels + 31) / 32, 1024, 0, s>>>(
