@@ -33,6 +33,7 @@
 
 #include "rows8.cuh"
 #include "sm100_primitives.cuh"
+#include "tensor_map.hpp"
 
 namespace to_b200 {
 namespace {
@@ -224,6 +225,19 @@ struct Source {  // x or f of a call: rows, or rows in 8 bits
   int access;  // bytes that one access may take
 };
 
+// A tile through TMA: `rows` of a tensor map of [tokens][channels] from (row, channel) on.
+__device__ __forceinline__ void tma_tile(char* dst, const CUtensorMap* map, int channel, int row, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(channel), "r"(row), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void wait_full(uint64_t* bar, uint32_t parity) {
+  if (!mbar_wait_bounded(bar, parity, 4 * kPolls)) atomicExch(&g_recurrence_status, TO_ERR_TIMEOUT);
+}
+
 template <typename T>
 __device__ __forceinline__ void load_rows(char* dst, const Rows& r, int access, const Item& it, int ch, int channels) {
   load_tile<kRowBytes>(access, dst, reinterpret_cast<const char*>(seq::row_ptr<const T>(r, it.row0, 0) + ch),
@@ -352,7 +366,7 @@ struct Links {
         before[warp][lane * V + v] = make_float2(__uint_as_float(static_cast<uint32_t>(w[v] >> 32) & 0x7fffffffu),
                                               __uint_as_float(static_cast<uint32_t>(w[v])));
     }
-    if (warp == kWarps - 1) {
+    if (warp == kWarps - 2) {
       fetch(C.states + place(b), w);
 #pragma unroll
       for (int v = 0; v < V; ++v) enter[lane * V + v] = __uint_as_float(static_cast<uint32_t>(w[v]));
@@ -381,6 +395,7 @@ __device__ __forceinline__ Vals<V> mapped(const float2* m, int lane, Vals<V> h) 
 // ---- forward -----------------------------------------------------------------------
 
 struct ForwardArgs {
+  CUtensorMap x_map, f_map;  // (TMA)
   Chain C;
   Rows x, f, h;
   int x_access, f_access, pairs;  // pairs: a lane's word of h is one access
@@ -447,50 +462,78 @@ __device__ __forceinline__ void keep_tile(const char* tile, const Packed& out, i
   }
 }
 
-template <typename T, bool KEEP, bool COMPLEMENT>
-__global__ void __launch_bounds__(kThreads, 3) forward_kernel(const __grid_constant__ ForwardArgs A) {
+// The last warp is also the one that knows what comes next: it takes tickets two
+// tiles ahead and, where TMA takes the rows, loads the tiles.  Two barriers a tile.
+template <typename T, bool KEEP, bool COMPLEMENT, bool TMA>
+__global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_constant__ ForwardArgs A) {
   using L = Lane<T>;
   using P = typename L::P;
   constexpr int V = L::kVec, CH = L::kChannels;
-  extern __shared__ __align__(16) char tiles[];  // two stages of x and f
-  __shared__ alignas(16) float2 maps[kWarps][CH], before[kChain][CH];
+  extern __shared__ __align__(128) char tiles[];  // two stages of x and f
+  __shared__ alignas(16) float2 all_maps[2][kWarps][CH], before[kChain][CH];
   __shared__ alignas(16) float enter[CH];
   __shared__ Item items[3];
+  __shared__ uint64_t full[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Chain& C = A.C;
   unsigned ticket = blockIdx.x;
-  auto fetch = [&](const Item& it, char* to) {
+  uint32_t parities = 0;  // a bit a stage
+  auto fetch = [&](const Item& it, char* to) {  // by all threads
     if (it.slot >= 0 && it.n > 0) {
       load_rows<T>(to, A.x, A.x_access, it, it.slab * CH, C.channels);
       load_rows<T>(to + kTile, A.f, A.f_access, it, it.slab * CH, C.channels);
     }
     close_tiles();
   };
+  auto load = [&](const Item& it, int stage) {  // by one
+    if (it.slot < 0 || it.n <= 0) return;
+    char* to = tiles + stage * 2 * kTile;
+    mbar_arrive_expect_tx(&full[stage], 2 * kTile);
+    tma_tile(to, &A.x_map, it.slab * CH, it.row0, &full[stage]);
+    tma_tile(to + kTile, &A.f_map, it.slab * CH, it.row0, &full[stage]);
+  };
   auto no_slot = [](const Item&) {};
+  if (TMA && threadIdx.x == 0) {
+    mbar_init(&full[0], 1);
+    mbar_init(&full[1], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
   if (warp == kWarps - 1) {
     for (int k = 0; k < 2; ++k) {
       if (k || C.ticket) next_ticket(C, ticket, lane);
       const Item first = next_item<false>(C, ticket, lane, no_slot);
-      if (lane == 0) items[k] = first;
+      if (lane == 0) {
+        items[k] = first;
+        if (TMA) load(first, k);
+      }
     }
   }
   __syncthreads();
-  fetch(items[0], tiles);
-  fetch(items[1], tiles + 2 * kTile);
+  if (!TMA) {
+    fetch(items[0], tiles);
+    fetch(items[1], tiles + 2 * kTile);
+  }
   for (int at = 0, stage = 0;; at = at == 2 ? 0 : at + 1, stage ^= 1) {
     const Item it = items[at];
     if (it.slot < 0) break;
     char* const xs = tiles + stage * 2 * kTile;
     char* const fs = xs + kTile;
     Item& later = items[at == 0 ? 2 : at - 1];  // the next but one
+    float2(*const maps)[CH] = all_maps[stage];
     const int ch = it.slab * CH, c0 = ch + lane * V, nc = min(V, C.channels - c0), t0 = warp * kTok;
     P bias = all<V>(0.f);
 #pragma unroll
     for (int v = 0; v < V; ++v)
       if (A.bias && v < nc) bias.v[v] = __ldg(A.bias + c0 + v);
-    wait_tiles<1>();
-    __syncthreads();
     if (warp == kWarps - 1) next_ticket(C, ticket, lane);
+    if (!TMA) {
+      wait_tiles<1>();
+      __syncthreads();
+    } else if (it.n > 0) {
+      wait_full(&full[stage], parities >> stage & 1);
+      parities ^= 1u << stage;
+    }
     if (KEEP) {
       if (A.keep_x.codes) keep_tile<T>(xs, A.keep_x, A.keep_access, it, ch, C.channels);
       if (A.keep_f.codes) keep_tile<T>(fs, A.keep_f, A.keep_access, it, ch, C.channels);
@@ -515,15 +558,13 @@ __global__ void __launch_bounds__(kThreads, 3) forward_kernel(const __grid_const
     else reduce(std::false_type{});
 #pragma unroll
     for (int v = 0; v < V; ++v) maps[warp][lane * V + v] = make_float2(a[kTok - 1].v[v], h[kTok - 1].v[v]);
-    if (warp == kWarps - 1) {
-      const Item next = next_item<false>(C, ticket, lane, no_slot);
-      if (lane == 0) later = next;
-    }
     __syncthreads();
-    fetch(later, xs);  // the tiles have been read
     const Links<T> links{C, lane, it.slab, it.slot - it.idx, 1, it.idx, it.count};
-    const long long state = A.slots ? __ldg(A.slots + it.seq) : it.seq;
-    const bool has_state = state >= 0 && state < A.num_slots;
+    long long state = -1;
+    if (warp == 0) {
+      state = A.slots ? __ldg(A.slots + it.seq) : it.seq;
+      if (state >= A.num_slots) state = -1;
+    }
     P sa = all<V>(1.f), sh = all<V>(0.f);  // the segment's map
     if (warp == 0) {
 #pragma unroll
@@ -536,11 +577,19 @@ __global__ void __launch_bounds__(kThreads, 3) forward_kernel(const __grid_const
       if (it.idx == 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v)
-          enter[lane * V + v] = A.state_in && has_state && v < nc ? A.state_in[state * C.channels + c0 + v] : 0.f;
+          enter[lane * V + v] = A.state_in && state >= 0 && v < nc ? A.state_in[state * C.channels + c0 + v] : 0.f;
+      }
+    }
+    if (warp == kWarps - 1) {
+      const Item next = next_item<false>(C, ticket, lane, no_slot);
+      if (lane == 0) {
+        later = next;
+        if (TMA) load(next, stage);  // the tiles have been read
       }
     }
     if (it.idx > 0) links.gather(warp, enter, before);
     __syncthreads();
+    if (!TMA) fetch(later, xs);
     P e = lane_of<V>(enter, lane);
     const int n = it.idx > 0 ? it.idx - links.base() : 0;
     for (int k = 0; k < n; ++k) e = mapped(before[k], lane, e);
@@ -550,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 3) forward_kernel(const __grid_const
       for (int v = 0; v < V; ++v) {
         if (v >= nc) continue;
         if (A.saved) A.saved[static_cast<long long>(it.slot) * C.channels + c0 + v] = e.v[v];
-        if (A.state_out && has_state && it.idx == it.count - 1)
+        if (A.state_out && state >= 0 && it.idx == it.count - 1)
           A.state_out[state * C.channels + c0 + v] = fmaf(sa.v[v], e.v[v], sh.v[v]);
       }
     }
@@ -932,6 +981,26 @@ int access_of(const to_rows8& r, int64_t tokens) {
   return n;
 }
 
+// Whether TMA takes rows, and their tensor map (tiles of kSegment tokens).
+bool tma_takes(const to_rows& r, const to_gated_recurrence_desc& d) {
+  return chained(d) && seq::rows_aligned(&r, d.tokens, 1, d.dtype, 16);
+}
+int map_of(CUtensorMap* map, CUtensorMapDataType type, int bytes, const void* data, long long pitch, int row,
+           const to_gated_recurrence_desc& d) {
+  int st = ok();
+  const EncodeTiled encode = tensor_map_encoder(&st);
+  if (!encode) return st;
+  const cuuint64_t dims[2] = {cuuint64_t(d.channels), cuuint64_t(d.tokens)}, strides[1] = {cuuint64_t(pitch * bytes)};
+  const cuuint32_t box[2] = {cuuint32_t(row / bytes), cuuint32_t(kSegment)}, steps[2] = {1, 1};
+  const CUresult e = encode(map, type, 2, const_cast<void*>(data), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return e == CUDA_SUCCESS ? ok() : set_error(TO_ERR_CUDA, "cuTensorMapEncodeTiled: %d", static_cast<int>(e));
+}
+int map_of(CUtensorMap* map, const to_rows& r, const to_gated_recurrence_desc& d) {
+  return d.dtype == TO_BF16 ? map_of(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, r.data, r.token_stride, kRowBytes, d)
+                            : map_of(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, r.data, r.token_stride, kRowBytes, d);
+}
+
 Chain chain_of(const to_gated_recurrence_desc& d, const int32_t* cu, const Layout& l, void* workspace) {
   Chain C{};
   C.cu = cu;
@@ -1045,23 +1114,28 @@ int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_rec
   if (sms <= 0) return -sms;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.partial, s));
-  const unsigned grid = grid_of(A.C, sms, 3);
+  const unsigned grid = grid_of(A.C, sms, 2);
   constexpr size_t kShared = 4 * size_t(kTile);
-  static std::atomic<uint64_t> done[8];
-  auto launch = [&](auto t, auto keep, auto complement) {
-    auto* kernel = forward_kernel<decltype(t), decltype(keep)::value, decltype(complement)::value>;
-    const int which = 4 * (sizeof(t) == 4) + 2 * decltype(keep)::value + decltype(complement)::value;
+  static std::atomic<uint64_t> done[16];
+  auto launch = [&](auto t, auto keep, auto complement, auto tma) {
+    using K = decltype(keep);
+    using M = decltype(complement);
+    auto* kernel = forward_kernel<decltype(t), K::value, M::value, decltype(tma)::value>;
+    const int which = 8 * (sizeof(t) == 4) + 4 * K::value + 2 * M::value + decltype(tma)::value;
     if (int bad = seq::allow_shared(kernel, kShared, done[which])) return bad;
     kernel<<<grid, kThreads, kShared, s>>>(A);
     return ok();
   };
-  auto with = [&](auto t) {
-    const bool keep = a.keep_x.codes || a.keep_f.codes;
-    if (d.complement)
-      return keep ? launch(t, std::true_type{}, std::true_type{}) : launch(t, std::false_type{}, std::true_type{});
-    return keep ? launch(t, std::true_type{}, std::false_type{}) : launch(t, std::false_type{}, std::false_type{});
+  const bool keep = a.keep_x.codes || a.keep_f.codes, tma = tma_takes(a.x, d) && tma_takes(a.f, d);
+  if (tma && ((st = map_of(&A.x_map, a.x, d)) || (st = map_of(&A.f_map, a.f, d)))) return st;
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  auto with = [&](auto t, auto m) {
+    if (tma) return keep ? launch(t, yes, m, yes) : launch(t, no, m, yes);
+    return keep ? launch(t, yes, m, no) : launch(t, no, m, no);
   };
-  st = d.dtype == TO_BF16 ? with(__nv_bfloat16{}) : with(float{});
+  if (d.dtype == TO_BF16) st = d.complement ? with(__nv_bfloat16{}, yes) : with(__nv_bfloat16{}, no);
+  else st = d.complement ? with(float{}, yes) : with(float{}, no);
   if (st) return st;
   TO_CUDA_TRY(cudaGetLastError());
   return ok();
