@@ -43,10 +43,10 @@ using seq::Rows;
 
 constexpr int kSegment = TO_RECURRENCE_SEGMENT;
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
-constexpr int kTok = kSegment / kWarps;  // tokens of a warp
 constexpr int kRowBytes = 128;           // of a tile's row of values
-constexpr int kTile = kSegment * kRowBytes;
-constexpr int kChain = 8;                // segments between published states: a warp fetches one map
+constexpr int kChained = 1024;           // tokens between published states
+// Tokens of a tile, forwards and backwards (the latter begins where a state is saved).
+constexpr int kForward = 128, kBackward = kSegment;
 constexpr uint32_t kPolls = 1u << 20;    // of a flag, about half a second
 
 __device__ int g_recurrence_status;
@@ -130,12 +130,13 @@ __device__ __forceinline__ int bound_of(const Chain& C, int s) {
 }
 
 // The segment of slot w, by the warp together: sequence s owns the slots
-// cu[s] / 128 + s and up, enough for its segments (an empty sequence has one).
+// cu[s] / SEG + s and up, enough for its segments (an empty sequence has one).
+template <int SEG>
 __device__ __forceinline__ void find_segment(const Chain& C, int w, int lane, Item& it) {
   int lo = 0, hi = C.nseq;
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32, probe = lo + lane * step;
-    const bool below = probe < hi && bound_of(C, probe) / kSegment + probe <= w;
+    const bool below = probe < hi && bound_of(C, probe) / SEG + probe <= w;
     const int found = __popc(__ballot_sync(0xffffffffu, below));
     lo += found > 1 ? (found - 1) * step : 0;
     hi = min(hi, lo + step);
@@ -143,12 +144,18 @@ __device__ __forceinline__ void find_segment(const Chain& C, int w, int lane, It
   const int first = bound_of(C, lo), end = bound_of(C, lo + 1);
   const int tokens = end > first ? end - first : 0;
   it.seq = lo;
-  it.count = tokens ? (tokens - 1) / kSegment + 1 : 1;
-  it.idx = w - (first / kSegment + lo);
+  it.count = tokens ? (tokens - 1) / SEG + 1 : 1;
+  it.idx = w - (first / SEG + lo);
   if (it.idx < 0 || it.idx >= it.count) it.idx = -1;
-  it.row0 = first + it.idx * kSegment;
-  it.n = min(kSegment, tokens - it.idx * kSegment);
+  it.row0 = first + it.idx * SEG;
+  it.n = min(SEG, tokens - it.idx * SEG);
   it.slot = w;
+}
+
+// The row of `saved` for an item that begins where a state is saved.
+template <int SEG>
+__device__ __forceinline__ int saved_row(const Chain& C, const Item& it) {
+  return (it.row0 - it.idx * SEG) / kSegment + it.seq + it.idx / (kSegment / SEG);
 }
 
 __device__ __forceinline__ void next_ticket(const Chain& C, unsigned& ticket, int lane) {
@@ -158,7 +165,7 @@ __device__ __forceinline__ void next_ticket(const Chain& C, unsigned& ticket, in
 
 // The item of a warp's ticket (lane 0's); a slot that no segment has goes to `unused`,
 // and the next ticket is taken.  `ticket`: the one that the item has.
-template <bool BACKWARD, typename UNUSED>
+template <int SEG, bool BACKWARD, typename UNUSED>
 __device__ __forceinline__ Item next_item(const Chain& C, unsigned& ticket, int lane, UNUSED&& unused) {
   Item it;
   for (;;) {
@@ -169,7 +176,7 @@ __device__ __forceinline__ Item next_item(const Chain& C, unsigned& ticket, int 
       return it;
     }
     it.slab = static_cast<int>(ticket - at * C.slabs);
-    find_segment(C, BACKWARD ? C.slots - 1 - static_cast<int>(at) : static_cast<int>(at), lane, it);
+    find_segment<SEG>(C, BACKWARD ? C.slots - 1 - static_cast<int>(at) : static_cast<int>(at), lane, it);
     if (it.idx >= 0) return it;
     unused(it);
     next_ticket(C, ticket, lane);
@@ -257,10 +264,11 @@ __device__ __forceinline__ float reciprocal(float x) {
   return y;
 }
 
-// c of a gate's f (with its bias); below 2^-126 it counts as zero.
+constexpr float kLog2e = 1.4426950408889634f;
+
+// c of a gate, from t = log2(e) (f + bias); below 2^-126 it counts as zero.
 template <int V>
-__device__ __forceinline__ Vals<V> gate_of(Vals<V> f) {
-  const Vals<V> t = mul(f, all<V>(1.4426950408889634f));
+__device__ __forceinline__ Vals<V> gate_of(Vals<V> t) {
   Vals<V> u, r;
 #pragma unroll
   for (int i = 0; i < V; ++i) u.v[i] = exp2_fast(-fabsf(t.v[i]));
@@ -270,8 +278,21 @@ __device__ __forceinline__ Vals<V> gate_of(Vals<V> f) {
   r = mul(u, r);
 #pragma unroll
   for (int i = 0; i < V; ++i)
-    r.v[i] = __uint_as_float(__float_as_uint(r.v[i]) | (~__float_as_uint(f.v[i]) & 0x80000000u));
+    r.v[i] = __uint_as_float(__float_as_uint(r.v[i]) | (~__float_as_uint(t.v[i]) & 0x80000000u));
   return r;
+}
+// -(1 - a) where t >= kCommon: a is 1/17 at least, so that 1 - (1 - a) loses no more than
+// 17 of its roundings and the other form of a step is not needed.
+constexpr float kCommon = -4.f;
+template <int V>
+__device__ __forceinline__ Vals<V> rest_of(Vals<V> t) {
+  Vals<V> e, r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) e.v[i] = exp2_fast(-t.v[i]);
+  r = add(e, all<V>(1.f));
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = reciprocal(-r.v[i]);
+  return mul(e, r);
 }
 // c is -(1 - a)
 __device__ __forceinline__ bool is_rest(float c) { return __float_as_int(c) < 0; }
@@ -293,6 +314,21 @@ __device__ __forceinline__ Vals<V> stepped(Vals<V> c, Vals<V> x, Vals<V> h) {
   return fma(c, COMPLEMENT ? sub(h, x) : h, base);
 }
 
+// The same where c is -(1 - a).
+template <bool COMPLEMENT, int V>
+__device__ __forceinline__ Vals<V> stepped_rest(Vals<V> c, Vals<V> x, Vals<V> h) {
+  return COMPLEMENT ? fma(c, sub(h, x), h) : fma(c, h, add(h, x));
+}
+
+// h -> a h + b of a lane's channels.
+template <int V>
+struct alignas(8 * V) Map {
+  Vals<V> a, b;
+  __device__ __forceinline__ Vals<V> operator()(Vals<V> h) const { return fma(a, h, b); }
+  // this map, then m
+  __device__ __forceinline__ Map then(const Map& m) const { return {mul(a, m.a), m(b)}; }
+};
+
 // ---- segments joined while the CTAs run ------------------------------------------------
 
 __device__ __forceinline__ uint64_t word_of(float value, uint32_t mark) {
@@ -309,8 +345,9 @@ __device__ __forceinline__ uint64_t published(const uint64_t* p) {
 
 // What a CTA has to do with the other segments of its sequence: position p of
 // `count` in the chain's direction, whose slots lie at origin + dir * position.
-template <typename T>
+template <typename T, int SEG>
 struct Links {
+  static constexpr int kChain = kChained / SEG;
   static constexpr int V = Lane<T>::kVec, CH = Lane<T>::kChannels;
   const Chain& C;
   int lane, slab, origin, dir, p, count;
@@ -320,11 +357,11 @@ struct Links {
   }
   __device__ __forceinline__ int base() const { return (p - 1) / kChain * kChain; }  // of p > 0
   // The segment's own map, for those behind it.
-  __device__ __forceinline__ void publish_map(const Vals<V>& a, const Vals<V>& h) const {
+  __device__ __forceinline__ void publish_map(const Map<V>& m) const {
     if (p + 1 >= count) return;
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      publish(C.maps + place(p) + v, word_of(h.v[v], __float_as_uint(a.v[v]) | 0x80000000u));
+      publish(C.maps + place(p) + v, word_of(m.b.v[v], __float_as_uint(m.a.v[v]) | 0x80000000u));
   }
   __device__ __forceinline__ void publish_state(const Vals<V>& h) const {
     if (p + 1 >= count || p % kChain) return;
@@ -353,44 +390,37 @@ struct Links {
       }
     }
   }
-  // What enters position p > 0, into shared memory by all warps: the state at base()
-  // into enter, the maps from there on into before.
-  __device__ __forceinline__ void gather(int warp, float (&enter)[CH], float2 (&before)[kChain][CH]) const {
+  // What enters position p > 0, by all warps: each of them brings a map behind the state at
+  // base() to shared memory, and warp 0, which has fetched that state, applies them in order.
+  __device__ __forceinline__ Vals<V> entering(int warp, Map<V> (&before)[kChain][32]) const {
+    static_assert(kChain == kWarps, "a warp fetches one map");
     const int b = base(), n = p - b;
     uint64_t w[V];
-    static_assert(kChain == kWarps, "a warp fetches one map");
     if (warp < n) {
       fetch(C.maps + place(b + warp), w);
+      Map<V> m;
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        before[warp][lane * V + v] = make_float2(__uint_as_float(static_cast<uint32_t>(w[v] >> 32) & 0x7fffffffu),
-                                              __uint_as_float(static_cast<uint32_t>(w[v])));
+      for (int v = 0; v < V; ++v) {
+        m.a.v[v] = __uint_as_float(static_cast<uint32_t>(w[v] >> 32) & 0x7fffffffu);
+        m.b.v[v] = __uint_as_float(static_cast<uint32_t>(w[v]));
+      }
+      before[warp][lane] = m;
     }
-    if (warp == kWarps - 2) {
-      fetch(C.states + place(b), w);
+    Vals<V> e = all<V>(0.f);
+    if (warp) {
+      asm volatile("bar.arrive 1, %0;" ::"n"(kThreads) : "memory");
+      return e;
+    }
+    fetch(C.states + place(b), w);
 #pragma unroll
-      for (int v = 0; v < V; ++v) enter[lane * V + v] = __uint_as_float(static_cast<uint32_t>(w[v]));
-    }
+    for (int v = 0; v < V; ++v) e.v[v] = __uint_as_float(static_cast<uint32_t>(w[v]));
+    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
+#pragma unroll
+    for (int k = 0; k < kChain; ++k)
+      if (k < n) e = before[k][lane](e);
+    return e;
   }
 };
-
-// A lane's values of an array in shared memory, and maps there applied to a state.
-template <int V>
-__device__ __forceinline__ Vals<V> lane_of(const float* p, int lane) {
-  Vals<V> r;
-#pragma unroll
-  for (int v = 0; v < V; ++v) r.v[v] = p[lane * V + v];
-  return r;
-}
-template <int V>
-__device__ __forceinline__ Vals<V> mapped(const float2* m, int lane, Vals<V> h) {
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const float2 x = m[lane * V + v];
-    h.v[v] = fmaf(x.x, h.v[v], x.y);
-  }
-  return h;
-}
 
 // ---- forward -----------------------------------------------------------------------
 
@@ -428,7 +458,7 @@ template <typename T>
 __device__ __forceinline__ void keep_tile(const char* tile, const Packed& out, int access, const Item& it, int ch,
                                           int channels) {
   constexpr int kParts = Lane<T>::kChannels / 16;
-  for (int i = threadIdx.x; i < kSegment * kParts; i += kThreads) {  // (whole warps)
+  for (int i = threadIdx.x; i < kForward * kParts; i += kThreads) {  // (whole warps)
     const int row = i / kParts, part = i % kParts, c = ch + part * 16;
     float x[16];
     seq::load_vec<T, 16>(reinterpret_cast<const T*>(tile + row * kRowBytes) + part * 16, x);
@@ -462,16 +492,19 @@ __device__ __forceinline__ void keep_tile(const char* tile, const Packed& out, i
   }
 }
 
-// The last warp is also the one that knows what comes next: it takes tickets two
-// tiles ahead and, where TMA takes the rows, loads the tiles.  Two barriers a tile.
+// Warp 1 knows what comes next: it takes tickets two tiles ahead and, where TMA
+// takes the rows, loads the tiles.  Between the barriers of a tile a warp joins the
+// maps of the warps before it (the last one so has the segment's, and publishes it) and
+// fetches its part of what enters.
 template <typename T, bool KEEP, bool COMPLEMENT, bool TMA>
 __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_constant__ ForwardArgs A) {
   using L = Lane<T>;
   using P = typename L::P;
-  constexpr int V = L::kVec, CH = L::kChannels;
+  constexpr int V = L::kVec, CH = L::kChannels, kTok = kForward / kWarps, kTile = kForward * kRowBytes;
+  constexpr int kChain = Links<T, kForward>::kChain, kNext = 1;
   extern __shared__ __align__(128) char tiles[];  // two stages of x and f
-  __shared__ alignas(16) float2 all_maps[2][kWarps][CH], before[kChain][CH];
-  __shared__ alignas(16) float enter[CH];
+  __shared__ Map<V> all_maps[2][kWarps][32], before[kChain][32];
+  __shared__ P enter[32];
   __shared__ Item items[3];
   __shared__ uint64_t full[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -499,10 +532,10 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_const
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
-  if (warp == kWarps - 1) {
+  if (warp == kNext) {
     for (int k = 0; k < 2; ++k) {
       if (k || C.ticket) next_ticket(C, ticket, lane);
-      const Item first = next_item<false>(C, ticket, lane, no_slot);
+      const Item first = next_item<kForward, false>(C, ticket, lane, no_slot);
       if (lane == 0) {
         items[k] = first;
         if (TMA) load(first, k);
@@ -514,19 +547,26 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_const
     fetch(items[0], tiles);
     fetch(items[1], tiles + 2 * kTile);
   }
-  for (int at = 0, stage = 0;; at = at == 2 ? 0 : at + 1, stage ^= 1) {
-    const Item it = items[at];
+  auto bias_of = [&](const Item& it) {  
+    P b = all<V>(0.f);
+    if (A.bias && it.slot >= 0) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (it.slab * CH + lane * V + v < C.channels) b.v[v] = __ldg(A.bias + it.slab * CH + lane * V + v);
+    }
+    return b;
+  };
+  P next_bias = bias_of(items[0]);
+  for (int turn = 0, stage = 0;; turn = turn == 2 ? 0 : turn + 1, stage ^= 1) {
+    const Item it = items[turn];
     if (it.slot < 0) break;
     char* const xs = tiles + stage * 2 * kTile;
     char* const fs = xs + kTile;
-    Item& later = items[at == 0 ? 2 : at - 1];  // the next but one
-    float2(*const maps)[CH] = all_maps[stage];
+    Item& later = items[turn == 0 ? 2 : turn - 1];  // the next but one
+    Map<V>(*const maps)[32] = all_maps[stage];
     const int ch = it.slab * CH, c0 = ch + lane * V, nc = min(V, C.channels - c0), t0 = warp * kTok;
-    P bias = all<V>(0.f);
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (A.bias && v < nc) bias.v[v] = __ldg(A.bias + c0 + v);
-    if (warp == kWarps - 1) next_ticket(C, ticket, lane);
+    const P bias = next_bias;
+    next_bias = bias_of(items[turn == 2 ? 0 : turn + 1]);
     if (!TMA) {
       wait_tiles<1>();
       __syncthreads();
@@ -538,74 +578,88 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_const
       if (A.keep_x.codes) keep_tile<T>(xs, A.keep_x, A.keep_access, it, ch, C.channels);
       if (A.keep_f.codes) keep_tile<T>(fs, A.keep_f, A.keep_access, it, ch, C.channels);
     }
-    // the map of a warp's first tokens, up to every one of them
+    // the map of a warp's first tokens, up to every one of them; a[i] is t before
     P a[kTok], h[kTok];
-    auto reduce = [&](auto whole) {
-      P at = all<V>(1.f), ht = all<V>(0.f);
+    float least = 0.f;
+    const P bias_t = mul(bias, all<V>(kLog2e));
+#pragma unroll
+    for (int i = 0; i < kTok; ++i) {
+      a[i] = fma(L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4)), all<V>(kLog2e), bias_t);
+#pragma unroll
+      for (int v = 0; v < V; ++v) least = fminf(least, a[i].v[v]);
+    }
+    if (it.n < kForward) least = kCommon - 1;  // (tokens that are not there: below)
+    P at = all<V>(1.f), ht = all<V>(0.f);
+    if (__all_sync(0xffffffffu, least >= kCommon)) {
 #pragma unroll
       for (int i = 0; i < kTok; ++i) {
-        const uint32_t x = *reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4);
-        const uint32_t f = *reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4);
-        if (decltype(whole)::value || t0 + i < it.n) {
-          const P c = gate_of(add(L::unpack(f), bias));
+        const P c = rest_of(a[i]), x = L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4));
+        a[i] = at = fma(c, at, at);
+        h[i] = ht = stepped_rest<COMPLEMENT>(c, x, ht);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) {
+        if (t0 + i < it.n) {
+          const P c = gate_of(a[i]), x = L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4));
           at = decayed(c, at);
-          ht = stepped<COMPLEMENT>(c, L::unpack(x), ht);
+          ht = stepped<COMPLEMENT>(c, x, ht);
         }
         a[i] = at, h[i] = ht;
       }
-    };
-    if (it.n == kSegment) reduce(std::true_type{});
-    else reduce(std::false_type{});
-#pragma unroll
-    for (int v = 0; v < V; ++v) maps[warp][lane * V + v] = make_float2(a[kTok - 1].v[v], h[kTok - 1].v[v]);
+    }
+    maps[warp][lane] = {at, ht};
+    if (warp == kNext) next_ticket(C, ticket, lane);
     __syncthreads();
-    const Links<T> links{C, lane, it.slab, it.slot - it.idx, 1, it.idx, it.count};
-    long long state = -1;
-    if (warp == 0) {
-      state = A.slots ? __ldg(A.slots + it.seq) : it.seq;
-      if (state >= A.num_slots) state = -1;
-    }
-    P sa = all<V>(1.f), sh = all<V>(0.f);  // the segment's map
-    if (warp == 0) {
+    const Links<T, kForward> links{C, lane, it.slab, it.slot - it.idx, 1, it.idx, it.count};
+    Map<V> upto{all<V>(1.f), all<V>(0.f)};  // of the warps before this one
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) sa.v[v] *= maps[w][lane * V + v].x;
-        sh = mapped(maps[w], lane, sh);
-      }
-      links.publish_map(sa, sh);
-      if (it.idx == 0) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          enter[lane * V + v] = A.state_in && state >= 0 && v < nc ? A.state_in[state * C.channels + c0 + v] : 0.f;
-      }
-    }
-    if (warp == kWarps - 1) {
-      const Item next = next_item<false>(C, ticket, lane, no_slot);
+    for (int w = 0; w < kWarps - 1; ++w)
+      if (w < warp) upto = upto.then(maps[w][lane]);
+    const bool last = warp == kWarps - 1;
+    if (last) links.publish_map(upto.then({at, ht}));
+    if (warp == kNext) {
+      const Item next = next_item<kForward, false>(C, ticket, lane, no_slot);
       if (lane == 0) {
         later = next;
         if (TMA) load(next, stage);  // the tiles have been read
       }
     }
-    if (it.idx > 0) links.gather(warp, enter, before);
-    __syncthreads();
-    if (!TMA) fetch(later, xs);
-    P e = lane_of<V>(enter, lane);
-    const int n = it.idx > 0 ? it.idx - links.base() : 0;
-    for (int k = 0; k < n; ++k) e = mapped(before[k], lane, e);
-    if (warp == 0) {
-      links.publish_state(e);
+    auto state_of = [&] {  // the place of the sequence's state; -1: none
+      const long long slot = A.slots ? __ldg(A.slots + it.seq) : it.seq;
+      return slot >= 0 && slot < A.num_slots ? slot * C.channels + c0 : -1;
+    };
+    P e = all<V>(0.f);
+    if (it.idx > 0) {
+      e = links.entering(warp, before);
+    } else if (warp == 0 && A.state_in) {
+      const long long state = state_of();
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        if (v >= nc) continue;
-        if (A.saved) A.saved[static_cast<long long>(it.slot) * C.channels + c0 + v] = e.v[v];
-        if (A.state_out && state >= 0 && it.idx == it.count - 1)
-          A.state_out[state * C.channels + c0 + v] = fmaf(sa.v[v], e.v[v], sh.v[v]);
+      for (int v = 0; v < V; ++v)
+        if (state >= 0 && v < nc) e.v[v] = A.state_in[state + v];
+    }
+    if (warp == 0) {
+      enter[lane] = e;
+      links.publish_state(e);
+      if (A.saved && it.idx % (kSegment / kForward) == 0) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (v < nc) A.saved[static_cast<long long>(saved_row<kForward>(C, it)) * C.channels + c0 + v] = e.v[v];
       }
     }
-    for (int w = 0; w < warp; ++w) e = mapped(maps[w], lane, e);
+    __syncthreads();
+    if (!TMA) fetch(later, xs);
+    e = enter[lane];
+    if (last && A.state_out && it.idx == it.count - 1) {
+      const long long state = state_of();
+      const P left = upto.then({at, ht})(e);
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (state >= 0 && v < nc) A.state_out[state + v] = left.v[v];
+    }
+    e = upto(e);
     T* row = seq::row_ptr<T>(A.h, it.row0 + static_cast<long long>(t0), 0) + c0;
-    if (A.pairs && nc == V && it.n == kSegment) {
+    if (A.pairs && nc == V && it.n == kForward) {
 #pragma unroll
       for (int i = 0; i < kTok; ++i, row += A.h.ts) *reinterpret_cast<uint32_t*>(row) = L::pack(fma(a[i], e, h[i]));
     } else {
@@ -639,14 +693,16 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
   using L = Lane<T>;
   using P = typename L::P;
   constexpr int V = L::kVec, CH = L::kChannels, kGroups = CH / seq::kGroup8;
-  extern __shared__ __align__(16) char tiles[];
+  constexpr int kTok = kBackward / kWarps, kTile = kBackward * kRowBytes, kChain = Links<T, kBackward>::kChain;
+  extern __shared__ __align__(128) char tiles[];
   char* const xs = tiles;
   char* const fs = tiles + kTile;
   char* const gs = tiles + 2 * kTile;
   // maps: of h, ends: of the gradients' chain (they share A)
-  __shared__ alignas(16) float2 maps[kWarps][CH], ends[kWarps][CH], before[kChain][CH];
-  __shared__ alignas(16) float enter[CH], sums[kWarps][CH];
-  __shared__ uint8_t scales[2][kSegment][kGroups];
+  __shared__ Map<V> maps[kWarps][32], ends[kWarps][32], before[kChain][32];
+  __shared__ P enter[32];
+  __shared__ float sums[kWarps][CH];
+  __shared__ uint8_t scales[2][kBackward][kGroups];
   __shared__ Item items[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Chain& C = A.C;
@@ -665,8 +721,8 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
       }
       load_tile<CH>(S.access, dst, reinterpret_cast<const char*>(S.packed.codes) + it.row0 * S.packed.code_stride + ch,
                     S.packed.code_stride, it.n, C.channels - ch);
-      const int row = threadIdx.x % kSegment;
-      if (static_cast<int>(threadIdx.x) / kSegment == k && row < it.n) {
+      const int row = threadIdx.x % kBackward;
+      if (static_cast<int>(threadIdx.x) / kBackward == k && row < it.n) {
         const uint8_t* from = S.packed.scales + (it.row0 + static_cast<long long>(row)) * S.packed.scale_stride + ch / 32;
 #pragma unroll
         for (int j = 0; j < kGroups; ++j) byte[j] = ch + 32 * j < C.channels ? __ldg(from + j) : 0;
@@ -683,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
   };
   if (warp == kWarps - 1) {
     if (C.ticket) next_ticket(C, ticket, lane);
-    const Item first = next_item<true>(C, ticket, lane, no_slot);
+    const Item first = next_item<kBackward, true>(C, ticket, lane, no_slot);
     if (lane == 0) items[0] = first;
   }
   __syncthreads();
@@ -696,12 +752,12 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       if (v >= nc) continue;
-      if (A.bias) bias.v[v] = __ldg(A.bias + c0 + v);
-      first.v[v] = __ldg(A.saved + static_cast<long long>(it.slot) * C.channels + c0 + v);
+      if (A.bias) bias.v[v] = kLog2e * __ldg(A.bias + c0 + v);
+      first.v[v] = __ldg(A.saved + static_cast<long long>(saved_row<kBackward>(C, it)) * C.channels + c0 + v);
     }
     wait_tiles<0>();
 #pragma unroll
-    for (int j = 0; j < kGroups; ++j) scales[threadIdx.x / kSegment][threadIdx.x % kSegment][j] = byte[j];
+    for (int j = 0; j < kGroups; ++j) scales[threadIdx.x / kBackward][threadIdx.x % kBackward][j] = byte[j];
     __syncthreads();
     if (warp == kWarps - 1) next_ticket(C, ticket, lane);
     const int group = lane * V / seq::kGroup8;
@@ -738,9 +794,9 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
 #pragma unroll
     for (int i = 0; i < kTok; ++i) {
       g[i] = *reinterpret_cast<const uint32_t*>(gs + (t0 + i) * kRowBytes + lane * 4);
-      c[i] = gate_of(add(c[i], bias));
+      c[i] = gate_of(fma(c[i], all<V>(kLog2e), bias));
     }
-    if (it.n < kSegment) {  // a token that is not there changes nothing
+    if (it.n < kBackward) {  // a token that is not there changes nothing
 #pragma unroll
       for (int i = 0; i < kTok; ++i)
         if (t0 + i >= it.n) x[i] = g[i] = 0, c[i] = all<V>(-0.f);
@@ -752,37 +808,28 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
     }
 #pragma unroll
     for (int i = kTok - 1; i >= 0; --i) r = decayed(c[i], add(L::unpack(g[i]), r));
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      maps[warp][lane * V + v] = make_float2(a.v[v], h.v[v]);
-      ends[warp][lane * V + v] = make_float2(a.v[v], r.v[v]);
-    }
+    maps[warp][lane] = {a, h};
+    ends[warp][lane] = {a, r};
     if (warp == kWarps - 1) {
-      const Item next = next_item<true>(C, ticket, lane, no_slot);
+      const Item next = next_item<kBackward, true>(C, ticket, lane, no_slot);
       if (lane == 0) items[cur ^ 1] = next;
     }
     __syncthreads();
     fetch(items[cur ^ 1]);
     const int p = it.count - 1 - it.idx;
-    const Links<T> links{C, lane, it.slab, it.slot + p, -1, p, it.count};
+    const Links<T, kBackward> links{C, lane, it.slab, it.slot + p, -1, p, it.count};
     const long long state = static_cast<long long>(it.seq) * C.channels + c0;
-    if (warp == 0) {
-      a = all<V>(1.f), r = all<V>(0.f);
+    // joined from the last warp on: the first one has the segment's map
+    Map<V> upto{all<V>(1.f), all<V>(0.f)};
 #pragma unroll
-      for (int k = kWarps - 1; k >= 0; --k) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) a.v[v] *= ends[k][lane * V + v].x;
-        r = mapped(ends[k], lane, r);
-      }
-      links.publish_map(a, r);
-      if (p == 0) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) enter[lane * V + v] = A.dstate_out && v < nc ? __ldg(A.dstate_out + state + v) : 0.f;
-      }
-    }
+    for (int k = kWarps - 1; k > 0; --k)
+      if (k > warp) upto = upto.then(ends[k][lane]);
+    if (warp == 0) links.publish_map(upto.then({a, r}));
     // the states before every token, and df_t / G_t
     P w[kTok];
-    for (int k = 0; k < warp; ++k) first = mapped(maps[k], lane, first);
+#pragma unroll
+    for (int k = 0; k < kWarps - 1; ++k)
+      if (k < warp) first = maps[k][lane](first);
 #pragma unroll
     for (int i = 0; i < kTok; ++i) {
       const P xv = L::unpack(x[i]), square = mul(c[i], c[i]);
@@ -792,19 +839,27 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
       w[i] = mul(slope, COMPLEMENT ? sub(first, xv) : first);
       first = stepped<COMPLEMENT>(c[i], xv, first);
     }
-    if (p > 0) links.gather(warp, enter, before);
-    __syncthreads();
-    P e = lane_of<V>(enter, lane);
-    const int n = p > 0 ? p - links.base() : 0;
-    for (int k = 0; k < n; ++k) e = mapped(before[k], lane, e);
-    if (warp == 0) {
-      links.publish_state(e);
+    P e = all<V>(0.f);
+    if (p > 0) {
+      e = links.entering(warp, before);
+    } else if (warp == 0 && A.dstate_out) {
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        if (A.dstate_in && it.idx == 0 && v < nc) A.dstate_in[state + v] = fmaf(a.v[v], e.v[v], r.v[v]);
+        if (v < nc) e.v[v] = __ldg(A.dstate_out + state + v);
     }
+    if (warp == 0) {
+      enter[lane] = e;
+      links.publish_state(e);
+      if (A.dstate_in && it.idx == 0) {
+        const P left = upto.then({a, r})(e);
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+          if (v < nc) A.dstate_in[state + v] = left.v[v];
+      }
+    }
+    __syncthreads();
+    e = upto(enter[lane]);
     P sum = all<V>(0.f);
-    for (int k = kWarps - 1; k > warp; --k) e = mapped(ends[k], lane, e);
     T* dx = seq::row_ptr<T>(A.dx, it.row0 + static_cast<long long>(t0), 0) + c0;
     T* df = seq::row_ptr<T>(A.df, it.row0 + static_cast<long long>(t0), 0) + c0;
     auto finish = [&](auto whole) {
@@ -834,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
         sum = add(sum, of);
       }
     };
-    if (A.pairs && nc == V && it.n == kSegment) finish(std::true_type{});
+    if (A.pairs && nc == V && it.n == kBackward) finish(std::true_type{});
     else finish(std::false_type{});
     if (A.partial) {
 #pragma unroll
@@ -900,7 +955,7 @@ __global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ StepA
     seq::load_vec<T, V>(seq::row_ptr<const T>(A.f, token, 0) + c, f);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const Vals<1> g = gate_of(Vals<1>{{f[v] + (A.bias ? __ldg(A.bias + c + v) : 0.f)}}), xv{{x[v]}}, hv{{h[v]}};
+      const Vals<1> g = gate_of(Vals<1>{{kLog2e * (f[v] + (A.bias ? __ldg(A.bias + c + v) : 0.f))}}), xv{{x[v]}}, hv{{h[v]}};
       h[v] = (A.complement ? stepped<true>(g, xv, hv) : stepped<false>(g, xv, hv)).v[0];
     }
     seq::store_vec<float, V>(state, h);
@@ -934,17 +989,18 @@ int channels_of_tile(const to_gated_recurrence_desc& d) { return kRowBytes / seq
 int slabs_of(const to_gated_recurrence_desc& d) {
   return (d.channels + channels_of_tile(d) - 1) / channels_of_tile(d);
 }
-// Segments that there may be, whatever the lengths are.
-int slots_of(const to_gated_recurrence_desc& d) { return static_cast<int>(d.tokens / kSegment) + d.nseq; }
-bool chained(const to_gated_recurrence_desc& d) { return d.tokens > kSegment && d.nseq > 0; }
+// Segments of `tokens` that there may be, whatever the lengths are.
+int slots_of(const to_gated_recurrence_desc& d, int tokens) { return static_cast<int>(d.tokens / tokens) + d.nseq; }
+bool chained(const to_gated_recurrence_desc& d, int tokens) { return d.tokens > tokens && d.nseq > 0; }
 
 struct Layout {  // of the workspace: the counter, the maps and the states (cleared), the partial sums
   size_t maps, states, partial, end;
 };
 Layout layout_of(const to_gated_recurrence_desc& d, bool backward) {
-  const size_t values = size_t(slots_of(d)) * slabs_of(d) * channels_of_tile(d);
+  const int seg = backward ? kBackward : kForward;
+  const size_t values = size_t(slots_of(d, seg)) * slabs_of(d) * channels_of_tile(d);
   Layout l{};
-  if (chained(d)) {
+  if (chained(d, seg)) {
     l.maps = kAlign;
     l.states = l.maps + padded(values * sizeof(uint64_t));
     l.partial = l.states + padded(values * sizeof(uint64_t));
@@ -981,35 +1037,35 @@ int access_of(const to_rows8& r, int64_t tokens) {
   return n;
 }
 
-// Whether TMA takes rows, and their tensor map (tiles of kSegment tokens).
+// Whether TMA takes rows (the smallest calls do without the two tensor maps), and their tensor map.
 bool tma_takes(const to_rows& r, const to_gated_recurrence_desc& d) {
-  return chained(d) && seq::rows_aligned(&r, d.tokens, 1, d.dtype, 16);
+  return d.tokens >= kSegment && seq::rows_aligned(&r, d.tokens, 1, d.dtype, 16);
 }
-int map_of(CUtensorMap* map, CUtensorMapDataType type, int bytes, const void* data, long long pitch, int row,
+int map_of(CUtensorMap* map, CUtensorMapDataType type, int bytes, const void* data, long long pitch, int row, int seg,
            const to_gated_recurrence_desc& d) {
   int st = ok();
   const EncodeTiled encode = tensor_map_encoder(&st);
   if (!encode) return st;
   const cuuint64_t dims[2] = {cuuint64_t(d.channels), cuuint64_t(d.tokens)}, strides[1] = {cuuint64_t(pitch * bytes)};
-  const cuuint32_t box[2] = {cuuint32_t(row / bytes), cuuint32_t(kSegment)}, steps[2] = {1, 1};
+  const cuuint32_t box[2] = {cuuint32_t(row / bytes), cuuint32_t(seg)}, steps[2] = {1, 1};
   const CUresult e = encode(map, type, 2, const_cast<void*>(data), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return e == CUDA_SUCCESS ? ok() : set_error(TO_ERR_CUDA, "cuTensorMapEncodeTiled: %d", static_cast<int>(e));
 }
-int map_of(CUtensorMap* map, const to_rows& r, const to_gated_recurrence_desc& d) {
-  return d.dtype == TO_BF16 ? map_of(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, r.data, r.token_stride, kRowBytes, d)
-                            : map_of(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, r.data, r.token_stride, kRowBytes, d);
+int map_of(CUtensorMap* map, const to_rows& r, int seg, const to_gated_recurrence_desc& d) {
+  return d.dtype == TO_BF16 ? map_of(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, r.data, r.token_stride, kRowBytes, seg, d)
+                            : map_of(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, r.data, r.token_stride, kRowBytes, seg, d);
 }
 
-Chain chain_of(const to_gated_recurrence_desc& d, const int32_t* cu, const Layout& l, void* workspace) {
+Chain chain_of(const to_gated_recurrence_desc& d, const int32_t* cu, const Layout& l, void* workspace, int seg) {
   Chain C{};
   C.cu = cu;
   C.nseq = d.nseq;
   C.tokens = static_cast<int>(d.tokens);
   C.channels = d.channels;
   C.slabs = slabs_of(d);
-  C.slots = slots_of(d);
-  if (chained(d)) {
+  C.slots = slots_of(d, seg);
+  if (chained(d, seg)) {
     char* w = static_cast<char*>(workspace);
     C.ticket = reinterpret_cast<unsigned*>(w);
     C.gave_up = reinterpret_cast<int*>(w + sizeof(unsigned));
@@ -1044,7 +1100,7 @@ using namespace to_b200;
 extern "C" {
 
 int64_t to_gated_recurrence_saved_rows(const to_gated_recurrence_desc* desc) {
-  return check_desc("to_gated_recurrence_saved_rows", desc) ? 0 : slots_of(*desc);
+  return check_desc("to_gated_recurrence_saved_rows", desc) ? 0 : slots_of(*desc, kSegment);
 }
 
 size_t to_gated_recurrence_workspace_bytes(const to_gated_recurrence_desc* desc) {
@@ -1088,10 +1144,10 @@ int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_rec
   if (a.state_in != a.state_out && seq::arrays_meet(a.state_in, a.state_out, states))
     return set_error(TO_ERR_INVALID_ARGUMENT, "%s: state_in and state_out share memory in part", who);
   for (const float* p : {a.state_in, static_cast<const float*>(a.state_out)})
-    if (p && a.saved && p < a.saved + size_t(slots_of(d)) * d.channels && a.saved < p + states / sizeof(float))
+    if (p && a.saved && p < a.saved + size_t(slots_of(d, kSegment)) * d.channels && a.saved < p + states / sizeof(float))
       return seq::refuse_overlap(who, "saved", p == a.state_in ? "state_in" : "state_out");
   ForwardArgs A{};
-  A.C = chain_of(d, a.cu_seqlens, l, a.workspace);
+  A.C = chain_of(d, a.cu_seqlens, l, a.workspace, kForward);
   A.x = seq::rows_of(a.x);
   A.f = seq::rows_of(a.f);
   A.h = seq::rows_of(a.h);
@@ -1115,7 +1171,7 @@ int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_rec
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.partial, s));
   const unsigned grid = grid_of(A.C, sms, 2);
-  constexpr size_t kShared = 4 * size_t(kTile);
+  constexpr size_t kShared = 4 * size_t(kForward) * kRowBytes;
   static std::atomic<uint64_t> done[16];
   auto launch = [&](auto t, auto keep, auto complement, auto tma) {
     using K = decltype(keep);
@@ -1127,7 +1183,7 @@ int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_rec
     return ok();
   };
   const bool keep = a.keep_x.codes || a.keep_f.codes, tma = tma_takes(a.x, d) && tma_takes(a.f, d);
-  if (tma && ((st = map_of(&A.x_map, a.x, d)) || (st = map_of(&A.f_map, a.f, d)))) return st;
+  if (tma && ((st = map_of(&A.x_map, a.x, kForward, d)) || (st = map_of(&A.f_map, a.f, kForward, d)))) return st;
   constexpr std::true_type yes{};
   constexpr std::false_type no{};
   auto with = [&](auto t, auto m) {
@@ -1182,10 +1238,10 @@ int to_gated_recurrence_backward(const to_gated_recurrence_desc* desc, const to_
   const size_t states = size_t(d.nseq) * d.channels;
   if (seq::arrays_meet(a.dstate_in, a.dstate_out, states * sizeof(float)))
     return seq::refuse_overlap(who, "dstate_in", "dstate_out");
-  if (a.dstate_in && a.dstate_in < a.saved + size_t(slots_of(d)) * d.channels && a.saved < a.dstate_in + states)
+  if (a.dstate_in && a.dstate_in < a.saved + size_t(slots_of(d, kSegment)) * d.channels && a.saved < a.dstate_in + states)
     return seq::refuse_overlap(who, "dstate_in", "saved");
   BackwardArgs A{};
-  A.C = chain_of(d, a.cu_seqlens, l, a.workspace);
+  A.C = chain_of(d, a.cu_seqlens, l, a.workspace, kBackward);
   A.x = {seq::rows_of(a.x), seq::packed_of(a.x8), a.x8.codes ? access_of(a.x8, d.tokens) : access_of(a.x, d.tokens, d.dtype)};
   A.f = {seq::rows_of(a.f), seq::packed_of(a.f8), a.f8.codes ? access_of(a.f8, d.tokens) : access_of(a.f, d.tokens, d.dtype)};
   A.dh = seq::rows_of(a.dh);
@@ -1203,7 +1259,7 @@ int to_gated_recurrence_backward(const to_gated_recurrence_desc* desc, const to_
   if (sms <= 0) return -sms;
   if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.partial, s));
   const unsigned grid = grid_of(A.C, sms, 2);
-  constexpr size_t kShared = 3 * size_t(kTile);
+  constexpr size_t kShared = 3 * size_t(kBackward) * kRowBytes;
   static std::atomic<uint64_t> done[4];
   auto launch = [&](auto t, auto complement) {
     auto* kernel = backward_kernel<decltype(t), decltype(complement)::value>;

@@ -170,22 +170,22 @@ def test_recurrence_many_segments():
 
 
 def test_recurrence_without_states_and_single_segments():
-    """Calls of at most 128 tokens need no workspace; no states, no gradients of bias and states."""
+    """Calls of at most 64 tokens need no workspace; no states, no gradients of bias and states."""
     op = sequence.GatedRecurrence("f32", 50)
-    assert op.workspace_bytes(128, 4) == 0
+    assert op.workspace_bytes(64, 4) == 0
     gen = torch.Generator("cuda").manual_seed(1)
-    x, f, dh = (cuda(128, 50, gen=gen) for _ in range(3))
-    cu = torch.tensor([0, 100, 100, 128], dtype=torch.int32, device="cuda")
+    x, f, dh = (cuda(64, 50, gen=gen) for _ in range(3))
+    cu = torch.tensor([0, 50, 50, 64], dtype=torch.int32, device="cuda")
     h, dx, df = (torch.empty_like(x) for _ in range(3))
-    saved = torch.empty(op.saved_rows(128, 3), 50, device="cuda")
+    saved = torch.empty(op.saved_rows(64, 3), 50, device="cuda")
     op.forward(x, f, None, cu, h, saved=saved)
-    ws = torch.empty(op.backward_workspace_bytes(128, 3), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(op.backward_workspace_bytes(64, 3), dtype=torch.uint8, device="cuda")
     op.backward(x, f, None, cu, saved, dh, dx, df, workspace=ws)
     zero = torch.zeros(3, 50, dtype=torch.float64)
-    want, before, _, a, z = R.recurrence(d(x), d(f), None, [100, 0, 28], zero, True)
-    wx, wf, *_ = R.recurrence_grad(d(x), a, z, before, [100, 0, 28], d(dh), zero, True)
+    want, before, _, a, z = R.recurrence(d(x), d(f), None, [50, 0, 14], zero, True)
+    wx, wf, *_ = R.recurrence_grad(d(x), a, z, before, [50, 0, 14], d(dh), zero, True)
     close(h, want, R.chain_bound(z, d(f), d(x).abs().amax(0)), "h")
-    g = R.chain_bound(z, d(f), 100 * d(dh).abs().amax(0))
+    g = R.chain_bound(z, d(f), 50 * d(dh).abs().amax(0))
     close(dx, wx, g, "dx")
     close(df, wf, 20 * g, "df")
 
