@@ -159,8 +159,9 @@ __device__ __forceinline__ int saved_row(const Chain& C, const Item& it) {
 }
 
 __device__ __forceinline__ void next_ticket(const Chain& C, unsigned& ticket, int lane) {
+  // (as PTX: atomicAdd is turned into one for the warp, whose result is waited for at once)
   if (!C.ticket) ticket += gridDim.x;
-  else if (lane == 0) ticket = atomicAdd(C.ticket, 1u);
+  else if (lane == 0) asm volatile("atom.relaxed.gpu.global.add.u32 %0, [%1], 1;" : "=r"(ticket) : "l"(C.ticket) : "memory");
 }
 
 // The item of a warp's ticket (lane 0's); a slot that no segment has goes to `unused`,
@@ -368,14 +369,17 @@ struct Links {
 #pragma unroll
     for (int v = 0; v < V; ++v) publish(C.states + place(p) + v, word_of(h.v[v], 1u));
   }
-  // Words that another CTA publishes, by the whole warp.
-  __device__ __forceinline__ void fetch(const uint64_t* from, uint64_t (&w)[V]) const {
+  // Words that other CTAs publish, from two places at once (or one, twice), by the whole warp.
+  __device__ __forceinline__ void fetch(const uint64_t* from, uint64_t (&w)[V], const uint64_t* from2, uint64_t (&w2)[V]) const {
     for (uint32_t polls = 0;; ++polls) {
       bool there = true;
 #pragma unroll
-      for (int v = 0; v < V; ++v) w[v] = published(from + v);
+      for (int v = 0; v < V; ++v) {
+        w[v] = published(from + v);
+        if (from2) w2[v] = published(from2 + v);
+      }
 #pragma unroll
-      for (int v = 0; v < V; ++v) there = there && w[v] != 0;
+      for (int v = 0; v < V; ++v) there = there && w[v] != 0 && (!from2 || w2[v] != 0);
       if (__all_sync(0xffffffffu, there)) return;
       if (polls % 256 == 255) {  // (once a wait has run out, the others of the call need not)
         bool out = polls > kPolls;
@@ -395,25 +399,23 @@ struct Links {
   __device__ __forceinline__ Vals<V> entering(int warp, Map<V> (&before)[kChain][32]) const {
     static_assert(kChain == kWarps, "a warp fetches one map");
     const int b = base(), n = p - b;
-    uint64_t w[V];
-    if (warp < n) {
-      fetch(C.maps + place(b + warp), w);
+    Vals<V> e = all<V>(0.f);
+    if (warp < n) {  // (n is one at least)
+      uint64_t w[V], state[V];
+      fetch(C.maps + place(b + warp), w, warp ? nullptr : C.states + place(b), state);
       Map<V> m;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         m.a.v[v] = __uint_as_float(static_cast<uint32_t>(w[v] >> 32) & 0x7fffffffu);
         m.b.v[v] = __uint_as_float(static_cast<uint32_t>(w[v]));
+        if (warp == 0) e.v[v] = __uint_as_float(static_cast<uint32_t>(state[v]));
       }
       before[warp][lane] = m;
     }
-    Vals<V> e = all<V>(0.f);
     if (warp) {
       asm volatile("bar.arrive 1, %0;" ::"n"(kThreads) : "memory");
       return e;
     }
-    fetch(C.states + place(b), w);
-#pragma unroll
-    for (int v = 0; v < V; ++v) e.v[v] = __uint_as_float(static_cast<uint32_t>(w[v]));
     asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
 #pragma unroll
     for (int k = 0; k < kChain; ++k)
