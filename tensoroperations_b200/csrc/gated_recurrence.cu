@@ -42,7 +42,7 @@ using seq::Packed;
 using seq::Rows;
 
 constexpr int kSegment = TO_RECURRENCE_SEGMENT;
-constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr int kWarps = 8, kThreads = 32 * kWarps;  // that compute; one more looks ahead
 constexpr int kRowBytes = 128;           // of a tile's row of values
 constexpr int kChained = 1024;           // tokens between published states
 // Tokens of a tile, forwards and backwards (the latter begins where a state is saved).
@@ -282,18 +282,28 @@ __device__ __forceinline__ Vals<V> gate_of(Vals<V> t) {
     r.v[i] = __uint_as_float(__float_as_uint(r.v[i]) | (~__float_as_uint(t.v[i]) & 0x80000000u));
   return r;
 }
-// -(1 - a) where t >= kCommon: a is 1/17 at least, so that 1 - (1 - a) loses no more than
-// 17 of its roundings and the other form of a step is not needed.
+// -(1 - a) of four tokens where t >= kCommon: a is 1/17 at least, so that 1 - (1 - a) loses no
+// more than 17 of its roundings and the other form of a step is not needed.  The four 1 + exp(-f)
+// share a reciprocal (their product's, at most 17^4): 10 special functions for 8 values, not 16.
 constexpr float kCommon = -4.f;
 template <int V>
-__device__ __forceinline__ Vals<V> rest_of(Vals<V> t) {
-  Vals<V> e, r;
+__device__ __forceinline__ void rest_of(Vals<V> (&t)[4]) {
+  Vals<V> d[4];
 #pragma unroll
-  for (int i = 0; i < V; ++i) e.v[i] = exp2_fast(-t.v[i]);
-  r = add(e, all<V>(1.f));
+  for (int k = 0; k < 4; ++k) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = reciprocal(-r.v[i]);
-  return mul(e, r);
+    for (int i = 0; i < V; ++i) t[k].v[i] = exp2_fast(-t[k].v[i]);
+    d[k] = add(t[k], all<V>(1.f));
+  }
+  const Vals<V> d01 = mul(d[0], d[1]), d23 = mul(d[2], d[3]), product = mul(d01, d23);
+  Vals<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = reciprocal(-product.v[i]);
+  const Vals<V> r01 = mul(r, d23), r23 = mul(r, d01);
+  t[0] = mul(t[0], mul(r01, d[1]));
+  t[1] = mul(t[1], mul(r01, d[0]));
+  t[2] = mul(t[2], mul(r23, d[3]));
+  t[3] = mul(t[3], mul(r23, d[2]));
 }
 // c is -(1 - a)
 __device__ __forceinline__ bool is_rest(float c) { return __float_as_int(c) < 0; }
@@ -369,18 +379,31 @@ struct Links {
 #pragma unroll
     for (int v = 0; v < V; ++v) publish(C.states + place(p) + v, word_of(h.v[v], 1u));
   }
-  // Words that other CTAs publish, from two places at once (or one, twice), by the whole warp.
-  __device__ __forceinline__ void fetch(const uint64_t* from, uint64_t (&w)[V], const uint64_t* from2, uint64_t (&w2)[V]) const {
+  // The state that enters position p > 0, by one warp: the state at base() and the maps from
+  // there on, applied in order.
+  __device__ __forceinline__ Vals<V> entering() const {
+    const int b = base(), n = p - b;
+    uint64_t w[kChain][V], state[V];
+    uint32_t missing = (1u << n) - 1 | 1u << kChain;
     for (uint32_t polls = 0;; ++polls) {
-      bool there = true;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        w[v] = published(from + v);
-        if (from2) w2[v] = published(from2 + v);
+      for (int k = 0; k <= kChain; ++k) {
+        if (!(missing >> k & 1)) continue;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          if (k < kChain) w[k < kChain ? k : 0][v] = published(C.maps + place(b + k) + v);
+          else state[v] = published(C.states + place(b) + v);
+        }
       }
 #pragma unroll
-      for (int v = 0; v < V; ++v) there = there && w[v] != 0 && (!from2 || w2[v] != 0);
-      if (__all_sync(0xffffffffu, there)) return;
+      for (int k = 0; k <= kChain; ++k) {
+        if (!(missing >> k & 1)) continue;
+        bool there = true;
+#pragma unroll
+        for (int v = 0; v < V; ++v) there = there && (k < kChain ? w[k < kChain ? k : 0][v] : state[v]) != 0;
+        if (__all_sync(0xffffffffu, there)) missing &= ~(1u << k);
+      }
+      if (!missing) break;
       if (polls % 256 == 255) {  // (once a wait has run out, the others of the call need not)
         bool out = polls > kPolls;
         if (lane == 0 && !out) out = *reinterpret_cast<volatile int*>(C.gave_up) != 0;
@@ -389,37 +412,24 @@ struct Links {
             atomicExch(C.gave_up, 1);
             atomicExch(&g_recurrence_status, TO_ERR_TIMEOUT);
           }
-          return;
+          break;
         }
       }
     }
-  }
-  // What enters position p > 0, by all warps: each of them brings a map behind the state at
-  // base() to shared memory, and warp 0, which has fetched that state, applies them in order.
-  __device__ __forceinline__ Vals<V> entering(int warp, Map<V> (&before)[kChain][32]) const {
-    static_assert(kChain == kWarps, "a warp fetches one map");
-    const int b = base(), n = p - b;
-    Vals<V> e = all<V>(0.f);
-    if (warp < n) {  // (n is one at least)
-      uint64_t w[V], state[V];
-      fetch(C.maps + place(b + warp), w, warp ? nullptr : C.states + place(b), state);
+    Vals<V> e;
+#pragma unroll
+    for (int v = 0; v < V; ++v) e.v[v] = __uint_as_float(static_cast<uint32_t>(state[v]));
+#pragma unroll
+    for (int k = 0; k < kChain; ++k) {
+      if (k >= n) continue;
       Map<V> m;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        m.a.v[v] = __uint_as_float(static_cast<uint32_t>(w[v] >> 32) & 0x7fffffffu);
-        m.b.v[v] = __uint_as_float(static_cast<uint32_t>(w[v]));
-        if (warp == 0) e.v[v] = __uint_as_float(static_cast<uint32_t>(state[v]));
+        m.a.v[v] = __uint_as_float(static_cast<uint32_t>(w[k][v] >> 32) & 0x7fffffffu);
+        m.b.v[v] = __uint_as_float(static_cast<uint32_t>(w[k][v]));
       }
-      before[warp][lane] = m;
+      e = m(e);
     }
-    if (warp) {
-      asm volatile("bar.arrive 1, %0;" ::"n"(kThreads) : "memory");
-      return e;
-    }
-    asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory");
-#pragma unroll
-    for (int k = 0; k < kChain; ++k)
-      if (k < n) e = before[k][lane](e);
     return e;
   }
 };
@@ -494,99 +504,178 @@ __device__ __forceinline__ void keep_tile(const char* tile, const Packed& out, i
   }
 }
 
-// Warp 1 knows what comes next: it takes tickets two tiles ahead and, where TMA
-// takes the rows, loads the tiles.  Between the barriers of a tile a warp joins the
-// maps of the warps before it (the last one so has the segment's, and publishes it) and
-// fetches its part of what enters.
+// Ten warps: eight compute.  One looks ahead: it takes tickets, reads what a tile's
+// channels need once (bias, and backwards the saved state) and, where TMA takes the
+// rows, loads the tiles, two stages ahead.  One finds out what enters a tile while the
+// eight reduce it; these join the maps of the warps before them (the last one so has the
+// segment's, and publishes it).
+constexpr int kAhead = kWarps, kEntering = kWarps + 1, kLaunched = kThreads + 64;
+
+struct Stages {
+  uint64_t known[2], full[2], empty[2];  // the item, its tile, its tile has been read
+  uint64_t entered[4];                   // (a tile's is read after its stage is empty: twice as many)
+  Item items[2];
+};
+
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void open_stages(Stages& S) {
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < 2; ++k) {
+      mbar_init(&S.known[k], 1);
+      mbar_init(&S.full[k], 1);
+      mbar_init(&S.empty[k], kWarps + 1);
+    }
+    for (uint64_t& b : S.entered) mbar_init(&b, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+}
+
+// The warp that looks ahead.  fill(item, stage): the whole warp; load(item, stage): one lane,
+// arrives at full[stage].
+template <int SEG, bool BACKWARD, typename UNUSED, typename FILL, typename LOAD>
+__device__ __forceinline__ void look_ahead(const Chain& C, Stages& S, UNUSED&& unused, FILL&& fill, LOAD&& load) {
+  const int lane = threadIdx.x & 31;
+  unsigned ticket = blockIdx.x;
+  for (uint32_t k = 0;; ++k) {
+    const int stage = k & 1;
+    // (a ticket taken while its stage is still in use would keep the segments behind it waiting)
+    if (k >= 2) wait_full(&S.empty[stage], (k / 2 - 1) & 1);
+    if (k || C.ticket) next_ticket(C, ticket, lane);
+    const Item it = next_item<SEG, BACKWARD>(C, ticket, lane, unused);
+    if (it.slot >= 0) fill(it, stage);
+    if (lane == 0) S.items[stage] = it;
+    __syncwarp();
+    if (lane == 0) {
+      arrive(&S.known[stage]);
+      if (it.slot >= 0 && it.n > 0) load(it, stage);
+      else arrive(&S.full[stage]);
+    }
+    if (it.slot < 0) return;
+  }
+}
+
+// The warp that finds what enters.  first(item): what enters a sequence; done(item, state).
+template <typename T, int SEG, bool BACKWARD, typename FIRST, typename DONE>
+__device__ __forceinline__ void find_entering(const Chain& C, Stages& S, Vals<Lane<T>::kVec> (&enter)[4][32], FIRST&& first,
+                                              DONE&& done) {
+  const int lane = threadIdx.x & 31;
+  for (uint32_t k = 0;; ++k) {
+    const int stage = k & 1;
+    wait_full(&S.known[stage], k / 2 & 1);
+    const Item it = S.items[stage];
+    __syncwarp();
+    if (lane == 0) arrive(&S.empty[stage]);
+    if (it.slot < 0) return;
+    const int p = BACKWARD ? it.count - 1 - it.idx : it.idx;
+    const Links<T, SEG> links{C, lane, it.slab, it.slot - (BACKWARD ? -p : p), BACKWARD ? -1 : 1, p, it.count};
+    const Vals<Lane<T>::kVec> e = p > 0 ? links.entering() : first(it);
+    links.publish_state(e);
+    enter[k & 3][lane] = e;
+    __syncwarp();
+    if (lane == 0) arrive(&S.entered[k & 3]);
+    done(it, e);
+  }
+}
+
 template <typename T, bool KEEP, bool COMPLEMENT, bool TMA>
-__global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_constant__ ForwardArgs A) {
+__global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_constant__ ForwardArgs A) {
   using L = Lane<T>;
   using P = typename L::P;
   constexpr int V = L::kVec, CH = L::kChannels, kTok = kForward / kWarps, kTile = kForward * kRowBytes;
-  constexpr int kChain = Links<T, kForward>::kChain, kNext = 1;
   extern __shared__ __align__(128) char tiles[];  // two stages of x and f
-  __shared__ Map<V> all_maps[2][kWarps][32], before[kChain][32];
-  __shared__ P enter[32];
-  __shared__ Item items[3];
-  __shared__ uint64_t full[2];
+  __shared__ Map<V> all_maps[2][kWarps][32];
+  __shared__ P enter[4][32], biases[2][32];
+  __shared__ Stages S;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Chain& C = A.C;
-  unsigned ticket = blockIdx.x;
-  uint32_t parities = 0;  // a bit a stage
-  auto fetch = [&](const Item& it, char* to) {  // by all threads
+  open_stages(S);
+  if (warp == kAhead) {
+    look_ahead<kForward, false>(
+        C, S, [](const Item&) {},
+        [&](const Item& it, int stage) {
+          P b = all<V>(0.f);
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (A.bias && it.slab * CH + lane * V + v < C.channels)
+              b.v[v] = kLog2e * __ldg(A.bias + it.slab * CH + lane * V + v);
+          biases[stage][lane] = b;
+        },
+        [&](const Item& it, int stage) {
+          if (!TMA) return arrive(&S.full[stage]);
+          char* to = tiles + stage * 2 * kTile;
+          mbar_arrive_expect_tx(&S.full[stage], 2 * kTile);
+          tma_tile(to, &A.x_map, it.slab * CH, it.row0, &S.full[stage]);
+          tma_tile(to + kTile, &A.f_map, it.slab * CH, it.row0, &S.full[stage]);
+        });
+    return;
+  }
+  auto state_of = [&](const Item& it) {  // the place of the sequence's state; -1: none
+    const long long slot = A.slots ? __ldg(A.slots + it.seq) : it.seq;
+    return slot >= 0 && slot < A.num_slots ? slot * C.channels + it.slab * CH + lane * V : -1;
+  };
+  if (warp == kEntering) {
+    find_entering<T, kForward, false>(
+        C, S, enter,
+        [&](const Item& it) {
+          P e = all<V>(0.f);
+          const long long state = A.state_in ? state_of(it) : -1;
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (state >= 0 && it.slab * CH + lane * V + v < C.channels) e.v[v] = A.state_in[state + v];
+          return e;
+        },
+        [&](const Item& it, const P& e) {
+          if (!A.saved || it.idx % (kSegment / kForward)) return;
+          const int c = it.slab * CH + lane * V;
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (c + v < C.channels) A.saved[static_cast<long long>(saved_row<kForward>(C, it)) * C.channels + c + v] = e.v[v];
+        });
+    return;
+  }
+  auto fetch = [&](int stage) {  // the next tile, by the warps that compute
+    const Item& it = S.items[stage];
+    char* to = tiles + stage * 2 * kTile;
     if (it.slot >= 0 && it.n > 0) {
       load_rows<T>(to, A.x, A.x_access, it, it.slab * CH, C.channels);
       load_rows<T>(to + kTile, A.f, A.f_access, it, it.slab * CH, C.channels);
     }
     close_tiles();
   };
-  auto load = [&](const Item& it, int stage) {  // by one
-    if (it.slot < 0 || it.n <= 0) return;
-    char* to = tiles + stage * 2 * kTile;
-    mbar_arrive_expect_tx(&full[stage], 2 * kTile);
-    tma_tile(to, &A.x_map, it.slab * CH, it.row0, &full[stage]);
-    tma_tile(to + kTile, &A.f_map, it.slab * CH, it.row0, &full[stage]);
-  };
-  auto no_slot = [](const Item&) {};
-  if (TMA && threadIdx.x == 0) {
-    mbar_init(&full[0], 1);
-    mbar_init(&full[1], 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  __syncthreads();
-  if (warp == kNext) {
-    for (int k = 0; k < 2; ++k) {
-      if (k || C.ticket) next_ticket(C, ticket, lane);
-      const Item first = next_item<kForward, false>(C, ticket, lane, no_slot);
-      if (lane == 0) {
-        items[k] = first;
-        if (TMA) load(first, k);
-      }
-    }
-  }
-  __syncthreads();
   if (!TMA) {
-    fetch(items[0], tiles);
-    fetch(items[1], tiles + 2 * kTile);
+    wait_full(&S.full[0], 0);
+    fetch(0);
   }
-  auto bias_of = [&](const Item& it) {  
-    P b = all<V>(0.f);
-    if (A.bias && it.slot >= 0) {
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (it.slab * CH + lane * V + v < C.channels) b.v[v] = __ldg(A.bias + it.slab * CH + lane * V + v);
+  for (uint32_t turn = 0;; ++turn) {
+    const int stage = turn & 1;
+    if (TMA) {
+      wait_full(&S.full[stage], turn / 2 & 1);
+    } else {
+      wait_tiles<0>();
+      compute_sync();
     }
-    return b;
-  };
-  P next_bias = bias_of(items[0]);
-  for (int turn = 0, stage = 0;; turn = turn == 2 ? 0 : turn + 1, stage ^= 1) {
-    const Item it = items[turn];
+    const Item it = S.items[stage];
     if (it.slot < 0) break;
     char* const xs = tiles + stage * 2 * kTile;
     char* const fs = xs + kTile;
-    Item& later = items[turn == 0 ? 2 : turn - 1];  // the next but one
-    Map<V>(*const maps)[32] = all_maps[stage];
     const int ch = it.slab * CH, c0 = ch + lane * V, nc = min(V, C.channels - c0), t0 = warp * kTok;
-    const P bias = next_bias;
-    next_bias = bias_of(items[turn == 2 ? 0 : turn + 1]);
-    if (!TMA) {
-      wait_tiles<1>();
-      __syncthreads();
-    } else if (it.n > 0) {
-      wait_full(&full[stage], parities >> stage & 1);
-      parities ^= 1u << stage;
-    }
     if (KEEP) {
       if (A.keep_x.codes) keep_tile<T>(xs, A.keep_x, A.keep_access, it, ch, C.channels);
       if (A.keep_f.codes) keep_tile<T>(fs, A.keep_f, A.keep_access, it, ch, C.channels);
     }
     // the map of a warp's first tokens, up to every one of them; a[i] is t before
     P a[kTok], h[kTok];
+    const P bias = biases[stage][lane];
     float least = 0.f;
-    const P bias_t = mul(bias, all<V>(kLog2e));
 #pragma unroll
     for (int i = 0; i < kTok; ++i) {
-      a[i] = fma(L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4)), all<V>(kLog2e), bias_t);
+      a[i] = fma(L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4)), all<V>(kLog2e), bias);
 #pragma unroll
       for (int v = 0; v < V; ++v) least = fminf(least, a[i].v[v]);
     }
@@ -594,10 +683,16 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_const
     P at = all<V>(1.f), ht = all<V>(0.f);
     if (__all_sync(0xffffffffu, least >= kCommon)) {
 #pragma unroll
-      for (int i = 0; i < kTok; ++i) {
-        const P c = rest_of(a[i]), x = L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4));
-        a[i] = at = fma(c, at, at);
-        h[i] = ht = stepped_rest<COMPLEMENT>(c, x, ht);
+      for (int j = 0; j < kTok; j += 4) {
+        P c[4] = {a[j], a[j + 1], a[j + 2], a[j + 3]};
+        rest_of(c);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = j + k;
+          a[i] = at = fma(c[k], at, at);
+          h[i] = ht = stepped_rest<COMPLEMENT>(
+              c[k], L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4)), ht);
+        }
       }
     } else {
 #pragma unroll
@@ -610,51 +705,28 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_const
         a[i] = at, h[i] = ht;
       }
     }
-    maps[warp][lane] = {at, ht};
-    if (warp == kNext) next_ticket(C, ticket, lane);
-    __syncthreads();
+    const Map<V> own{at, ht};
+    Map<V>(*const maps)[32] = all_maps[stage];
+    maps[warp][lane] = own;
+    __syncwarp();
+    if (lane == 0) arrive(&S.empty[stage]);
+    compute_sync();
+    if (!TMA) {
+      wait_full(&S.full[stage ^ 1], (turn + 1) / 2 & 1);
+      fetch(stage ^ 1);
+    }
     const Links<T, kForward> links{C, lane, it.slab, it.slot - it.idx, 1, it.idx, it.count};
     Map<V> upto{all<V>(1.f), all<V>(0.f)};  // of the warps before this one
 #pragma unroll
     for (int w = 0; w < kWarps - 1; ++w)
       if (w < warp) upto = upto.then(maps[w][lane]);
     const bool last = warp == kWarps - 1;
-    if (last) links.publish_map(upto.then({at, ht}));
-    if (warp == kNext) {
-      const Item next = next_item<kForward, false>(C, ticket, lane, no_slot);
-      if (lane == 0) {
-        later = next;
-        if (TMA) load(next, stage);  // the tiles have been read
-      }
-    }
-    auto state_of = [&] {  // the place of the sequence's state; -1: none
-      const long long slot = A.slots ? __ldg(A.slots + it.seq) : it.seq;
-      return slot >= 0 && slot < A.num_slots ? slot * C.channels + c0 : -1;
-    };
-    P e = all<V>(0.f);
-    if (it.idx > 0) {
-      e = links.entering(warp, before);
-    } else if (warp == 0 && A.state_in) {
-      const long long state = state_of();
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (state >= 0 && v < nc) e.v[v] = A.state_in[state + v];
-    }
-    if (warp == 0) {
-      enter[lane] = e;
-      links.publish_state(e);
-      if (A.saved && it.idx % (kSegment / kForward) == 0) {
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (v < nc) A.saved[static_cast<long long>(saved_row<kForward>(C, it)) * C.channels + c0 + v] = e.v[v];
-      }
-    }
-    __syncthreads();
-    if (!TMA) fetch(later, xs);
-    e = enter[lane];
+    if (last) links.publish_map(upto.then(own));
+    wait_full(&S.entered[turn & 3], turn / 4 & 1);
+    P e = enter[turn & 3][lane];
     if (last && A.state_out && it.idx == it.count - 1) {
-      const long long state = state_of();
-      const P left = upto.then({at, ht})(e);
+      const long long state = state_of(it);
+      const P left = upto.then(own)(e);
 #pragma unroll
       for (int v = 0; v < V; ++v)
         if (state >= 0 && v < nc) A.state_out[state + v] = left.v[v];
@@ -675,6 +747,7 @@ __global__ void __launch_bounds__(kThreads, 2) forward_kernel(const __grid_const
 // ---- backward ----------------------------------------------------------------------
 
 struct BackwardArgs {
+  CUtensorMap x_map, f_map, dh_map;  // (TMA)
   Chain C;
   Source x, f;
   Rows dh, dx, df;
@@ -689,187 +762,273 @@ struct BackwardArgs {
 // The gradients' own chain runs from a sequence's end: what leaves token t is a_t G_t,
 // with G_t = dh_t + what left token t + 1; the map of some tokens is their A and what
 // leaves them when nothing enters.  h runs forwards again from the saved state (so
-// the map (A, H) of each warp is needed too).
-template <typename T, bool COMPLEMENT>
-__global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_constant__ BackwardArgs A) {
+// the map (A, H) of each warp is needed too).  x and dh stay in shared memory until the
+// last walk.
+template <typename T>
+struct BackwardTiles {  // of a stage: x and f as they are (or their codes at the same places), dh
+  static constexpr int kTile = kBackward * kRowBytes, kStage = 3 * kTile;
+};
+
+template <typename T, bool COMPLEMENT, bool TMA>
+__global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_constant__ BackwardArgs A) {
   using L = Lane<T>;
   using P = typename L::P;
   constexpr int V = L::kVec, CH = L::kChannels, kGroups = CH / seq::kGroup8;
-  constexpr int kTok = kBackward / kWarps, kTile = kBackward * kRowBytes, kChain = Links<T, kBackward>::kChain;
-  extern __shared__ __align__(128) char tiles[];
-  char* const xs = tiles;
-  char* const fs = tiles + kTile;
-  char* const gs = tiles + 2 * kTile;
+  constexpr int kTok = kBackward / kWarps, kTile = BackwardTiles<T>::kTile, kStage = BackwardTiles<T>::kStage;
+  extern __shared__ __align__(128) char tiles[];  // two stages
   // maps: of h, ends: of the gradients' chain (they share A)
-  __shared__ Map<V> maps[kWarps][32], ends[kWarps][32], before[kChain][32];
-  __shared__ P enter[32];
+  __shared__ Map<V> maps[kWarps][32], ends[kWarps][32];
+  __shared__ P enter[4][32], biases[2][32], firsts[2][32];
   __shared__ float sums[kWarps][CH];
-  __shared__ uint8_t scales[2][kBackward][kGroups];
-  __shared__ Item items[2];
+  __shared__ uint8_t scales[2][2][kBackward][kGroups];
+  __shared__ Stages S;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Chain& C = A.C;
-  unsigned ticket = blockIdx.x;
-  uint8_t byte[kGroups] = {};  // scales of the next tile, this thread's row
-  auto fetch = [&](const Item& it) {
-    if (it.slot < 0 || it.n <= 0) return;
-    const int ch = it.slab * CH;
+  open_stages(S);
+  if (warp == kAhead) {
+    look_ahead<kBackward, true>(
+        C, S,
+        [&](const Item& it) {  // its sums count too
+          if (A.partial)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const Source& S = k ? A.f : A.x;
-      char* dst = k ? fs : xs;
-      if (!S.packed.codes) {
-        load_rows<T>(dst, S.rows, S.access, it, ch, C.channels);
-        continue;
-      }
-      load_tile<CH>(S.access, dst, reinterpret_cast<const char*>(S.packed.codes) + it.row0 * S.packed.code_stride + ch,
-                    S.packed.code_stride, it.n, C.channels - ch);
-      const int row = threadIdx.x % kBackward;
-      if (static_cast<int>(threadIdx.x) / kBackward == k && row < it.n) {
-        const uint8_t* from = S.packed.scales + (it.row0 + static_cast<long long>(row)) * S.packed.scale_stride + ch / 32;
+            for (int v = 0; v < V; ++v)
+              A.partial[(static_cast<long long>(it.slot) * C.slabs + it.slab) * CH + lane * V + v] = 0.f;
+        },
+        [&](const Item& it, int stage) {
+          const int ch = it.slab * CH;
+          P b = all<V>(0.f), first = all<V>(0.f);
 #pragma unroll
-        for (int j = 0; j < kGroups; ++j) byte[j] = ch + 32 * j < C.channels ? __ldg(from + j) : 0;
+          for (int v = 0; v < V; ++v) {
+            const int c = ch + lane * V + v;
+            if (c >= C.channels) continue;
+            if (A.bias) b.v[v] = kLog2e * __ldg(A.bias + c);
+            first.v[v] = __ldg(A.saved + static_cast<long long>(saved_row<kBackward>(C, it)) * C.channels + c);
+          }
+          biases[stage][lane] = b;
+          firsts[stage][lane] = first;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const Packed& from = k ? A.f.packed : A.x.packed;
+            if (!from.codes) continue;
+#pragma unroll
+            for (int r = 0; r < kBackward; r += 32) {
+              if (r + lane >= it.n) continue;
+              const uint8_t* row = from.scales + (it.row0 + static_cast<long long>(r + lane)) * from.scale_stride + ch / 32;
+#pragma unroll
+              for (int j = 0; j < kGroups; ++j)
+                scales[stage][k][r + lane][j] = ch + 32 * j < C.channels ? __ldg(row + j) : 0;
+            }
+          }
+        },
+        [&](const Item& it, int stage) {
+          if (!TMA) return arrive(&S.full[stage]);
+          char* to = tiles + stage * kStage;
+          const int ch = it.slab * CH, x = A.x.packed.codes ? kBackward * CH : kTile, f = A.f.packed.codes ? kBackward * CH : kTile;
+          mbar_arrive_expect_tx(&S.full[stage], x + f + kTile);
+          tma_tile(to, &A.x_map, ch, it.row0, &S.full[stage]);
+          tma_tile(to + kTile, &A.f_map, ch, it.row0, &S.full[stage]);
+          tma_tile(to + 2 * kTile, &A.dh_map, ch, it.row0, &S.full[stage]);
+        });
+    return;
+  }
+  if (warp == kEntering) {
+    find_entering<T, kBackward, true>(
+        C, S, enter,
+        [&](const Item& it) {
+          P e = all<V>(0.f);
+          const int c = it.slab * CH + lane * V;
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            if (A.dstate_out && c + v < C.channels) e.v[v] = __ldg(A.dstate_out + static_cast<long long>(it.seq) * C.channels + c + v);
+          return e;
+        },
+        [](const Item&, const P&) {});
+    return;
+  }
+  auto fetch = [&](int stage) {  // the next tile, by the warps that compute
+    const Item& it = S.items[stage];
+    char* to = tiles + stage * kStage;
+    if (it.slot >= 0 && it.n > 0) {
+      const int ch = it.slab * CH;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const Source& from = k ? A.f : A.x;
+        if (from.packed.codes)
+          load_tile<CH>(from.access, to + k * kTile,
+                        reinterpret_cast<const char*>(from.packed.codes) + it.row0 * from.packed.code_stride + ch,
+                        from.packed.code_stride, it.n, C.channels - ch);
+        else
+          load_rows<T>(to + k * kTile, from.rows, from.access, it, ch, C.channels);
       }
+      load_rows<T>(to + 2 * kTile, A.dh, A.dh_access, it, ch, C.channels);
     }
-    load_rows<T>(gs, A.dh, A.dh_access, it, ch, C.channels);
     close_tiles();
   };
-  auto no_slot = [&](const Item& it) {  // its sums count too
-    if (A.partial)
-#pragma unroll
-      for (int v = 0; v < V; ++v)
-        A.partial[(static_cast<long long>(it.slot) * C.slabs + it.slab) * CH + lane * V + v] = 0.f;
-  };
-  if (warp == kWarps - 1) {
-    if (C.ticket) next_ticket(C, ticket, lane);
-    const Item first = next_item<kBackward, true>(C, ticket, lane, no_slot);
-    if (lane == 0) items[0] = first;
+  if (!TMA) {
+    wait_full(&S.full[0], 0);
+    fetch(0);
   }
-  __syncthreads();
-  fetch(items[0]);
-  for (int cur = 0;; cur ^= 1) {
-    const Item it = items[cur];
-    if (it.slot < 0) break;
-    const int ch = it.slab * CH, c0 = ch + lane * V, nc = min(V, C.channels - c0), t0 = warp * kTok;
-    P bias = all<V>(0.f), first = all<V>(0.f);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (v >= nc) continue;
-      if (A.bias) bias.v[v] = kLog2e * __ldg(A.bias + c0 + v);
-      first.v[v] = __ldg(A.saved + static_cast<long long>(saved_row<kBackward>(C, it)) * C.channels + c0 + v);
+  for (uint32_t turn = 0;; ++turn) {
+    const int stage = turn & 1;
+    if (TMA) {
+      wait_full(&S.full[stage], turn / 2 & 1);
+    } else {
+      wait_tiles<0>();
+      compute_sync();
     }
-    wait_tiles<0>();
-#pragma unroll
-    for (int j = 0; j < kGroups; ++j) scales[threadIdx.x / kBackward][threadIdx.x % kBackward][j] = byte[j];
-    __syncthreads();
-    if (warp == kWarps - 1) next_ticket(C, ticket, lane);
+    const Item it = S.items[stage];
+    if (it.slot < 0) break;
+    const char* const xs = tiles + stage * kStage;
+    const char* const fs = xs + kTile;
+    const char* const gs = fs + kTile;
+    const int c0 = it.slab * CH + lane * V, nc = min(V, C.channels - c0), t0 = warp * kTok;
     const int group = lane * V / seq::kGroup8;
-    P a = all<V>(1.f), h = all<V>(0.f), r = all<V>(0.f), c[kTok];
-    uint32_t x[kTok], g[kTok];
     auto value = [&](const char* tile, int k, int t) {  // of rows in 8 bits
-      const float scale = seq::scale_of(scales[k][t][group]);
-      const int8_t* code = reinterpret_cast<const int8_t*>(tile) + t * CH + lane * V;
+      const float scale = seq::scale_of(scales[stage][k][t][group]);
       P out;
-      if constexpr (V == 2) {  // (one access)
-        const uint16_t both = *reinterpret_cast<const uint16_t*>(code);
-        out.v[0] = seq::code_to_f32(static_cast<int8_t>(both & 0xff), scale);
-        out.v[1] = seq::code_to_f32(static_cast<int8_t>(both >> 8), scale);
+      if constexpr (V == 2) {
+        const uint32_t both = *reinterpret_cast<const uint16_t*>(tile + t * CH + lane * V) ^ 0x8080u;  // codes + 128
+        out = {{__uint_as_float(0x4b000000u | (both & 0xffu)), __uint_as_float(0x4b000000u | (both >> 8))}};
+        out = mul(add(out, all<V>(-8388736.f)), all<V>(scale));
       } else {
-        out.v[0] = seq::code_to_f32(code[0], scale);
+        out.v[0] = seq::code_to_f32(reinterpret_cast<const int8_t*>(tile)[t * CH + lane], scale);
       }
       return out;
     };
-    if (A.x.packed.codes) {
-#pragma unroll
-      for (int i = 0; i < kTok; ++i) x[i] = L::pack(value(xs, 0, t0 + i));  // (7 bits and a sign: exact)
-    } else {
-#pragma unroll
-      for (int i = 0; i < kTok; ++i) x[i] = *reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4);
-    }
+    auto x_of = [&](int i) {
+      return A.x.packed.codes ? value(xs, 0, t0 + i)
+                              : L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4));
+    };
+    auto dh_of = [&](int i) { return L::unpack(*reinterpret_cast<const uint32_t*>(gs + (t0 + i) * kRowBytes + lane * 4)); };
+    P c[kTok], w[kTok];  // c[i] is t before; w: x, then df_t / G_t
+    const P bias = biases[stage][lane];
+    float least = 0.f;
     if (A.f.packed.codes) {
 #pragma unroll
-      for (int i = 0; i < kTok; ++i) c[i] = value(fs, 1, t0 + i);
+      for (int i = 0; i < kTok; ++i) c[i] = fma(value(fs, 1, t0 + i), all<V>(kLog2e), bias);
     } else {
 #pragma unroll
       for (int i = 0; i < kTok; ++i)
-        c[i] = L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4));
+        c[i] = fma(L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4)), all<V>(kLog2e), bias);
     }
 #pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      g[i] = *reinterpret_cast<const uint32_t*>(gs + (t0 + i) * kRowBytes + lane * 4);
-      c[i] = gate_of(fma(c[i], all<V>(kLog2e), bias));
-    }
-    if (it.n < kBackward) {  // a token that is not there changes nothing
+    for (int i = 0; i < kTok; ++i)
 #pragma unroll
-      for (int i = 0; i < kTok; ++i)
-        if (t0 + i >= it.n) x[i] = g[i] = 0, c[i] = all<V>(-0.f);
-    }
+      for (int v = 0; v < V; ++v) least = fminf(least, c[i].v[v]);
+    const bool common = __all_sync(0xffffffffu, it.n == kBackward && least >= kCommon);
+    P a = all<V>(1.f), h = all<V>(0.f), r = all<V>(0.f);
+    if (A.x.packed.codes) {
 #pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      a = decayed(c[i], a);
-      h = stepped<COMPLEMENT>(c[i], L::unpack(x[i]), h);
-    }
+      for (int i = 0; i < kTok; ++i) w[i] = value(xs, 0, t0 + i);
+    } else {
 #pragma unroll
-    for (int i = kTok - 1; i >= 0; --i) r = decayed(c[i], add(L::unpack(g[i]), r));
+      for (int i = 0; i < kTok; ++i) w[i] = L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4));
+    }
+    if (common) {
+#pragma unroll
+      for (int j = 0; j < kTok; j += 4) {
+        P four[4] = {c[j], c[j + 1], c[j + 2], c[j + 3]};
+        rest_of(four);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = j + k;
+          c[i] = four[k];
+          a = fma(c[i], a, a);
+          h = stepped_rest<COMPLEMENT>(c[i], w[i], h);
+        }
+      }
+#pragma unroll
+      for (int i = kTok - 1; i >= 0; --i) {
+        const P G = add(dh_of(i), r);
+        r = fma(c[i], G, G);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kTok; ++i) {
+        if (t0 + i >= it.n) continue;  // a token that is not there changes nothing
+        c[i] = gate_of(c[i]);
+        a = decayed(c[i], a);
+        h = stepped<COMPLEMENT>(c[i], w[i], h);
+      }
+#pragma unroll
+      for (int i = kTok - 1; i >= 0; --i)
+        if (t0 + i < it.n) r = decayed(c[i], add(dh_of(i), r));
+    }
     maps[warp][lane] = {a, h};
-    ends[warp][lane] = {a, r};
-    if (warp == kWarps - 1) {
-      const Item next = next_item<kBackward, true>(C, ticket, lane, no_slot);
-      if (lane == 0) items[cur ^ 1] = next;
-    }
-    __syncthreads();
-    fetch(items[cur ^ 1]);
+    const Map<V> own{a, r};
+    ends[warp][lane] = own;
+    compute_sync();
     const int p = it.count - 1 - it.idx;
     const Links<T, kBackward> links{C, lane, it.slab, it.slot + p, -1, p, it.count};
-    const long long state = static_cast<long long>(it.seq) * C.channels + c0;
     // joined from the last warp on: the first one has the segment's map
     Map<V> upto{all<V>(1.f), all<V>(0.f)};
 #pragma unroll
     for (int k = kWarps - 1; k > 0; --k)
       if (k > warp) upto = upto.then(ends[k][lane]);
-    if (warp == 0) links.publish_map(upto.then({a, r}));
-    // the states before every token, and df_t / G_t
-    P w[kTok];
+    if (warp == 0) links.publish_map(upto.then(own));
+    // the states before every token, and df_t / G_t (with the other sign where c is -(1 - a))
+    h = firsts[stage][lane];
 #pragma unroll
     for (int k = 0; k < kWarps - 1; ++k)
-      if (k < warp) first = maps[k][lane](first);
+      if (k < warp) h = maps[k][lane](h);
+    if (common) {
 #pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      const P xv = L::unpack(x[i]), square = mul(c[i], c[i]);
-      P slope;  // a (1 - a)
+      for (int i = 0; i < kTok; ++i) {
+        const P x = w[i], rest = fma(c[i], c[i], c[i]), off = sub(h, x);  // -a (1 - a)
+        w[i] = mul(rest, COMPLEMENT ? off : h);
+        h = COMPLEMENT ? fma(c[i], off, h) : fma(c[i], h, add(h, x));
+      }
+    } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) slope.v[v] = fabsf(c[i].v[v]) - square.v[v];
-      w[i] = mul(slope, COMPLEMENT ? sub(first, xv) : first);
-      first = stepped<COMPLEMENT>(c[i], xv, first);
-    }
-    P e = all<V>(0.f);
-    if (p > 0) {
-      e = links.entering(warp, before);
-    } else if (warp == 0 && A.dstate_out) {
+      for (int i = 0; i < kTok; ++i) {
+        if (t0 + i >= it.n) continue;
+        const P x = w[i], square = mul(c[i], c[i]);
+        P slope;  // a (1 - a)
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        if (v < nc) e.v[v] = __ldg(A.dstate_out + state + v);
-    }
-    if (warp == 0) {
-      enter[lane] = e;
-      links.publish_state(e);
-      if (A.dstate_in && it.idx == 0) {
-        const P left = upto.then({a, r})(e);
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          if (v < nc) A.dstate_in[state + v] = left.v[v];
+        for (int v = 0; v < V; ++v) slope.v[v] = fabsf(c[i].v[v]) - square.v[v];
+        w[i] = mul(slope, COMPLEMENT ? sub(h, x) : h);
+        h = stepped<COMPLEMENT>(c[i], x, h);
       }
     }
-    __syncthreads();
-    e = upto(enter[lane]);
+    compute_sync();  // (maps and ends have been read)
+    wait_full(&S.entered[turn & 3], turn / 4 & 1);
+    P e = enter[turn & 3][lane];
+    if (warp == 0 && A.dstate_in && it.idx == 0) {
+      const P left = upto.then(own)(e);
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (v < nc) A.dstate_in[static_cast<long long>(it.seq) * C.channels + c0 + v] = left.v[v];
+    }
+    e = upto(e);
     P sum = all<V>(0.f);
     T* dx = seq::row_ptr<T>(A.dx, it.row0 + static_cast<long long>(t0), 0) + c0;
     T* df = seq::row_ptr<T>(A.df, it.row0 + static_cast<long long>(t0), 0) + c0;
-    auto finish = [&](auto whole) {
-      constexpr bool kWhole = decltype(whole)::value;
+    auto finish = [&](auto words) {  // all of it with the other sign
+      e = mul(e, all<V>(-1.f));
 #pragma unroll
       for (int i = kTok - 1; i >= 0; --i) {
-        if (!kWhole && t0 + i >= it.n) continue;
-        const P G = add(L::unpack(g[i]), e), of = mul(G, w[i]);
+        const P G = sub(e, dh_of(i)), of = mul(G, w[i]), ox = mul(c[i], G);
+        e = fma(c[i], G, G);
+        const uint32_t wx = L::pack(COMPLEMENT ? ox : mul(G, all<V>(-1.f))), wf = L::pack(of);
+        if (decltype(words)::value) {
+          *reinterpret_cast<uint32_t*>(dx + i * A.dx.ts) = wx;
+          *reinterpret_cast<uint32_t*>(df + i * A.df.ts) = wf;
+        } else {
+          store_word<T>(dx + i * A.dx.ts, wx, nc, A.pairs);
+          store_word<T>(df + i * A.df.ts, wf, nc, A.pairs);
+        }
+        sum = add(sum, of);
+      }
+    };
+    if (common && A.pairs && nc == V) {
+      finish(std::true_type{});
+    } else if (common) {
+      finish(std::false_type{});
+    } else {
+#pragma unroll
+      for (int i = kTok - 1; i >= 0; --i) {
+        if (t0 + i >= it.n) continue;
+        const P G = add(dh_of(i), e), of = mul(G, w[i]);
         P ox = G;
         if (COMPLEMENT) {  // (1 - a) G
           P base, minus;
@@ -881,22 +1040,23 @@ __global__ void __launch_bounds__(kThreads, 2) backward_kernel(const __grid_cons
           ox = fma(c[i], minus, base);
         }
         e = decayed(c[i], G);
-        if (kWhole) {
-          *reinterpret_cast<uint32_t*>(dx + i * A.dx.ts) = L::pack(ox);
-          *reinterpret_cast<uint32_t*>(df + i * A.df.ts) = L::pack(of);
-        } else {
-          store_word<T>(dx + i * A.dx.ts, L::pack(ox), nc, A.pairs);
-          store_word<T>(df + i * A.df.ts, L::pack(of), nc, A.pairs);
-        }
+        store_word<T>(dx + i * A.dx.ts, L::pack(ox), nc, A.pairs);
+        store_word<T>(df + i * A.df.ts, L::pack(of), nc, A.pairs);
         sum = add(sum, of);
       }
-    };
-    if (A.pairs && nc == V && it.n == kBackward) finish(std::true_type{});
-    else finish(std::false_type{});
+    }
     if (A.partial) {
 #pragma unroll
       for (int v = 0; v < V; ++v) sums[warp][lane * V + v] = sum.v[v];
-      __syncthreads();
+    }
+    __syncwarp();
+    if (lane == 0) arrive(&S.empty[stage]);
+    if (!TMA) {
+      wait_full(&S.full[stage ^ 1], (turn + 1) / 2 & 1);
+      fetch(stage ^ 1);
+    }
+    if (A.partial) {
+      compute_sync();
       if (threadIdx.x < CH) {
         float total = 0.f;
 #pragma unroll
@@ -1054,6 +1214,12 @@ int map_of(CUtensorMap* map, CUtensorMapDataType type, int bytes, const void* da
                             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return e == CUDA_SUCCESS ? ok() : set_error(TO_ERR_CUDA, "cuTensorMapEncodeTiled: %d", static_cast<int>(e));
 }
+bool tma_takes(const to_rows8& r, const to_gated_recurrence_desc& d) {
+  return d.tokens >= kSegment && aligned(r.codes, 16) && r.code_stride % 16 == 0;
+}
+int map_of(CUtensorMap* map, const to_rows8& r, int seg, const to_gated_recurrence_desc& d) {
+  return map_of(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, r.codes, r.code_stride, channels_of_tile(d), seg, d);
+}
 int map_of(CUtensorMap* map, const to_rows& r, int seg, const to_gated_recurrence_desc& d) {
   return d.dtype == TO_BF16 ? map_of(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, r.data, r.token_stride, kRowBytes, seg, d)
                             : map_of(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, r.data, r.token_stride, kRowBytes, seg, d);
@@ -1181,7 +1347,7 @@ int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_rec
     auto* kernel = forward_kernel<decltype(t), K::value, M::value, decltype(tma)::value>;
     const int which = 8 * (sizeof(t) == 4) + 4 * K::value + 2 * M::value + decltype(tma)::value;
     if (int bad = seq::allow_shared(kernel, kShared, done[which])) return bad;
-    kernel<<<grid, kThreads, kShared, s>>>(A);
+    kernel<<<grid, kLaunched, kShared, s>>>(A);
     return ok();
   };
   const bool keep = a.keep_x.codes || a.keep_f.codes, tma = tma_takes(a.x, d) && tma_takes(a.f, d);
@@ -1261,16 +1427,30 @@ int to_gated_recurrence_backward(const to_gated_recurrence_desc* desc, const to_
   if (sms <= 0) return -sms;
   if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.partial, s));
   const unsigned grid = grid_of(A.C, sms, 2);
-  constexpr size_t kShared = 3 * size_t(kBackward) * kRowBytes;
-  static std::atomic<uint64_t> done[4];
-  auto launch = [&](auto t, auto complement) {
-    auto* kernel = backward_kernel<decltype(t), decltype(complement)::value>;
-    if (int bad = seq::allow_shared(kernel, kShared, done[2 * (sizeof(t) == 4) + decltype(complement)::value])) return bad;
-    kernel<<<grid, kThreads, kShared, s>>>(A);
+  constexpr size_t kShared = 2 * size_t(BackwardTiles<float>::kStage);
+  static std::atomic<uint64_t> done[8];
+  auto launch = [&](auto t, auto complement, auto tma) {
+    auto* kernel = backward_kernel<decltype(t), decltype(complement)::value, decltype(tma)::value>;
+    const int which = 4 * (sizeof(t) == 4) + 2 * decltype(complement)::value + decltype(tma)::value;
+    if (int bad = seq::allow_shared(kernel, kShared, done[which])) return bad;
+    kernel<<<grid, kLaunched, kShared, s>>>(A);
     return ok();
   };
-  if (d.dtype == TO_BF16) st = d.complement ? launch(__nv_bfloat16{}, std::true_type{}) : launch(__nv_bfloat16{}, std::false_type{});
-  else st = d.complement ? launch(float{}, std::true_type{}) : launch(float{}, std::false_type{});
+  const bool tma = tma_takes(a.dh, d) && (a.x8.codes ? tma_takes(a.x8, d) : tma_takes(a.x, d)) &&
+                   (a.f8.codes ? tma_takes(a.f8, d) : tma_takes(a.f, d));
+  if (tma) {
+    st = a.x8.codes ? map_of(&A.x_map, a.x8, kBackward, d) : map_of(&A.x_map, a.x, kBackward, d);
+    if (!st) st = a.f8.codes ? map_of(&A.f_map, a.f8, kBackward, d) : map_of(&A.f_map, a.f, kBackward, d);
+    if (!st) st = map_of(&A.dh_map, a.dh, kBackward, d);
+    if (st) return st;
+  }
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  auto with = [&](auto t) {
+    if (tma) return d.complement ? launch(t, yes, yes) : launch(t, no, yes);
+    return d.complement ? launch(t, yes, no) : launch(t, no, no);
+  };
+  st = d.dtype == TO_BF16 ? with(__nv_bfloat16{}) : with(float{});
   if (st) return st;
   TO_CUDA_TRY(cudaGetLastError());
   if (a.dbias) {
