@@ -9,10 +9,11 @@
 //             dw_pre = sum dn r^,  dw_post = sum q act(g) y^
 //
 // Memory bound: 15 to 40 flops a value, of which each is read once and written
-// once.  A row lies in the registers of one warp, or of all warps of a CTA: eight
-// values a thread (sixteen above 8192), as one 16-byte access of bf16; where
-// addresses or widths do not allow that, neighbouring threads take neighbouring
-// values.  The two sums of the forward pass follow one another, the gradients' three
+// once.  A row lies in the registers of one warp, or of all warps of a CTA: sixteen
+// values a thread (eight up to 256 values a row), each eight of them one 16-byte access
+// of bf16; where addresses or widths do not allow that, neighbouring threads take
+// neighbouring values.  (With eight values a thread the sums over a row took as many
+// instructions as the values.)  The two sums of the forward pass follow one another, the gradients' three
 // first ones are taken together.
 #include <algorithm>
 #include <cmath>
@@ -171,42 +172,60 @@ __device__ __forceinline__ void load_kept(const Packed& in, long long token, con
 // of two buffers, so that one barrier a sum is enough.
 template <int N>
 struct RowSums {
-  float (*part)[kMaxWarps][N];
+  float (*part)[N][kMaxWarps];
   int turn = 0;
   __device__ __forceinline__ void operator()(float (&v)[N]) {
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+    for (int o = 16; o; o >>= 1)
 #pragma unroll
-      for (int o = 16; o; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+      for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
     const int warps = blockDim.x / 32;
     if (warps == 1) return;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     if (lane == 0) {
 #pragma unroll
-      for (int n = 0; n < N; ++n) part[turn][warp][n] = v[n];
+      for (int n = 0; n < N; ++n) part[turn][n][warp] = v[n];
     }
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      v[n] = lane < warps ? part[turn][lane][n] : 0.f;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+      v[n] = 0.f;
+      const float4* from = reinterpret_cast<const float4*>(part[turn][n]);
+      for (int w = 0; w < warps; w += 4) {  // (the rest of a four is zero)
+        const float4 x = from[w / 4];
+        v[n] += (x.x + x.y) + (x.z + x.w);
+      }
     }
     turn ^= 1;
   }
+  __device__ __forceinline__ void clear() {
+    for (int i = threadIdx.x; i < 2 * N * kMaxWarps; i += blockDim.x) (&part[0][0][0])[i] = 0.f;
+    __syncthreads();
+  }
 };
 
-// The gate's factor and its slope.
-struct Gate {
-  float factor, slope;
-};
-__device__ __forceinline__ Gate gate_of(int kind, float g) {
-  if (kind == TO_GATE_NONE) return {1.f, 0.f};
-  if (kind == TO_GATE_LINEAR) return {g, 1.f};
-  const float e = __expf(g < -80.f ? 80.f : -g);  // (below -80 sigmoid(g) counts as e^-80)
-  const float p = __fdividef(1.f, 1.f + e), q = e * p;  // sigmoid(g), 1 - sigmoid(g)
-  if (kind == TO_GATE_SIGMOID) return {p, p * q};
-  return {g * p, fmaf(g * p, q, p)};
+// The gate's factors and, for the gradients, their slopes.  (One branch for eight values.)
+template <bool SLOPES, typename T>
+__device__ __forceinline__ void gate_of(int kind, const Unit<T>& g, float (&factor)[kVals], float (&slope)[kVals]) {
+  if (kind == TO_GATE_NONE) {
+#pragma unroll
+    for (int k = 0; k < kVals; ++k) factor[k] = 1.f;
+  } else if (kind == TO_GATE_LINEAR) {
+#pragma unroll
+    for (int k = 0; k < kVals; ++k) {
+      factor[k] = g[k];
+      if (SLOPES) slope[k] = 1.f;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kVals; ++k) {
+      const float t = -1.4426950408889634f * g[k];
+      const float e = seq::exp2_fast(t > 115.f ? 115.f : t);  // (below -80 sigmoid(g) counts as e^-80)
+      const float p = seq::reciprocal(1.f + e);               // sigmoid(g); 1 - sigmoid(g) is e p
+      factor[k] = kind == TO_GATE_SIGMOID ? p : g[k] * p;
+      if (SLOPES) slope[k] = kind == TO_GATE_SIGMOID ? p * (e * p) : fmaf(factor[k], e * p, p);
+    }
+  }
 }
 
 // ---- forward -----------------------------------------------------------------------
@@ -221,63 +240,78 @@ struct ForwardArgs {
   float scale, eps;
 };
 
-template <typename T, typename R, int U, bool WIDE>
-__global__ void __launch_bounds__(32 * kMaxWarps) forward_kernel(const __grid_constant__ ForwardArgs A) {
-  __shared__ float part[2][kMaxWarps][1];
+template <typename T, typename R, int U, bool WIDE, int MOST>
+__global__ void __launch_bounds__(MOST, MOST == 256 ? 3 : MOST == 512 ? 2 : 1) forward_kernel(const __grid_constant__ ForwardArgs A) {
+  __shared__ alignas(16) float part[2][1][kMaxWarps];
   RowSums<1> sums{part};
   const float inv = 1.f / static_cast<float>(A.width);
+  const bool has_y = A.y.p, keeps = A.keep_r.codes || A.keep_y.codes || A.keep_g.codes;
+  const int gate = A.g.p ? A.gate : TO_GATE_NONE;
+  if (blockDim.x > 32) sums.clear();
   for (long long t = blockIdx.x * static_cast<long long>(blockDim.y) + threadIdx.y; t < A.tokens;
        t += gridDim.x * static_cast<long long>(blockDim.y)) {
     Unit<R> r[U];
     Unit<T> y[U], g[U];
-    float x[U][kVals];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const Place<WIDE> pl(u, A.width);
       load_unit<R>(seq::row_ptr<const R>(A.r, t, 0), pl, r[u]);
-      if (A.y.p) load_unit<T>(seq::row_ptr<const T>(A.y, t, 0), pl, y[u]);
-      if (A.g.p) load_unit<T>(seq::row_ptr<const T>(A.g, t, 0), pl, g[u]);
+      if (has_y) load_unit<T>(seq::row_ptr<const T>(A.y, t, 0), pl, y[u]);
+      if (gate != TO_GATE_NONE) load_unit<T>(seq::row_ptr<const T>(A.g, t, 0), pl, g[u]);
     }
-    float f = A.scale;
-    if (A.y.p && A.post_norm) {
-      float s[1] = {0.f};
+    float x[U][kVals], s[1] = {0.f};
+    if (has_y) {
+      float f = A.scale;
+      if (A.post_norm) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int k = 0; k < kVals; ++k) s[0] = fmaf(y[u][k], y[u][k], s[0]);
+        sums(s);
+        f *= rsqrtf(fmaf(s[0], inv, A.eps));
+        s[0] = 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float w[kVals], a[kVals], none[kVals];
+        load_weights<WIDE>(A.w_post, Place<WIDE>(u, A.width), w);
+        gate_of<false>(gate, g[u], a, none);
+#pragma unroll
+        for (int k = 0; k < kVals; ++k) x[u][k] = fmaf(f * w[k] * a[k], y[u][k], r[u][k]);
+      }
+    } else {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int k = 0; k < kVals; ++k) s[0] = fmaf(y[u][k], y[u][k], s[0]);
-      sums(s);
-      f *= rsqrtf(fmaf(s[0], inv, A.eps));
+        for (int k = 0; k < kVals; ++k) x[u][k] = r[u][k];
     }
-    float s[1] = {0.f};
+    if (A.r_out.p) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const Place<WIDE> pl(u, A.width);
-      float w[kVals];
-      if (A.y.p) load_weights<WIDE>(A.w_post, pl, w);
+      for (int u = 0; u < U; ++u) store_unit<R>(seq::row_ptr<R>(A.r_out, t, 0), Place<WIDE>(u, A.width), x[u]);
+    }
+    if (keeps) {
 #pragma unroll
-      for (int k = 0; k < kVals; ++k) {
-        x[u][k] = r[u][k];
-        if (A.y.p) {
-          const float a = A.g.p ? gate_of(A.gate, g[u][k]).factor : 1.f;
-          x[u][k] = fmaf(f * w[k] * a, y[u][k], x[u][k]);
+      for (int u = 0; u < U; ++u) {
+        const Place<WIDE> pl(u, A.width);
+        float v[kVals];
+        if (A.keep_r.codes) keep_unit<WIDE>(A.keep_r, t, pl, x[u]);
+        if (A.keep_y.codes) {
+#pragma unroll
+          for (int k = 0; k < kVals; ++k) v[k] = y[u][k];
+          keep_unit<WIDE>(A.keep_y, t, pl, v);
         }
-        s[0] = fmaf(x[u][k], x[u][k], s[0]);
-      }
-      if (A.r_out.p) store_unit<R>(seq::row_ptr<R>(A.r_out, t, 0), pl, x[u]);
-      if (A.keep_r.codes) keep_unit<WIDE>(A.keep_r, t, pl, x[u]);
-      float v[kVals];
-      if (A.keep_y.codes) {
+        if (A.keep_g.codes) {
 #pragma unroll
-        for (int k = 0; k < kVals; ++k) v[k] = y[u][k];
-        keep_unit<WIDE>(A.keep_y, t, pl, v);
-      }
-      if (A.keep_g.codes) {
-#pragma unroll
-        for (int k = 0; k < kVals; ++k) v[k] = g[u][k];
-        keep_unit<WIDE>(A.keep_g, t, pl, v);
+          for (int k = 0; k < kVals; ++k) v[k] = g[u][k];
+          keep_unit<WIDE>(A.keep_g, t, pl, v);
+        }
       }
     }
     if (!A.n.p) continue;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < kVals; ++k) s[0] = fmaf(x[u][k], x[u][k], s[0]);
     sums(s);
     const float m = rsqrtf(fmaf(s[0], inv, A.eps));
 #pragma unroll
@@ -305,13 +339,18 @@ struct BackwardArgs {
   float scale, eps;
 };
 
-template <typename T, typename R, int U, bool WIDE>
-__global__ void __launch_bounds__(32 * kMaxWarps) backward_kernel(const __grid_constant__ BackwardArgs A) {
-  __shared__ float part[2][kMaxWarps][3], part_d[2][kMaxWarps][1];
+template <typename T, typename R, int U, bool WIDE, int MOST>
+__global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) backward_kernel(const __grid_constant__ BackwardArgs A) {
+  __shared__ alignas(16) float part[2][3][kMaxWarps], part_d[2][1][kMaxWarps];
   extern __shared__ __align__(16) float rows[];  // several rows a CTA: [rows][2][width]
   RowSums<3> sums{part};
   RowSums<1> sum_d{part_d};
   const float inv = 1.f / static_cast<float>(A.width);
+  const int gate = A.has_y ? A.gate : TO_GATE_NONE;
+  if (blockDim.x > 32) {
+    sums.clear();
+    sum_d.clear();
+  }
   float pre[U][kVals], post[U][kVals];  // this thread's columns of dw_pre, dw_post
 #pragma unroll
   for (int u = 0; u < U; ++u)
@@ -321,21 +360,23 @@ __global__ void __launch_bounds__(32 * kMaxWarps) backward_kernel(const __grid_c
        t += gridDim.x * static_cast<long long>(blockDim.y)) {
     Unit<R> r[U], dr[U];
     Unit<T> y[U], g[U], dn[U];
-    float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const Place<WIDE> pl(u, A.width);
       const float zero[kVals] = {};
-      y[u].set(zero), g[u].set(zero), dn[u].set(zero), dr[u].set(zero);
       if (A.r8.codes) load_kept<R>(A.r8, t, pl, r[u]);
       else load_unit<R>(seq::row_ptr<const R>(A.r, t, 0), pl, r[u]);
+      if (A.dn.p) load_unit<T>(seq::row_ptr<const T>(A.dn, t, 0), pl, dn[u]);
+      else dn[u].set(zero);
+      if (A.dr_out.p) load_unit<R>(seq::row_ptr<const R>(A.dr_out, t, 0), pl, dr[u]);
+      else dr[u].set(zero);
       if (A.y8.codes) load_kept<T>(A.y8, t, pl, y[u]);
       else if (A.y.p) load_unit<T>(seq::row_ptr<const T>(A.y, t, 0), pl, y[u]);
+      else y[u].set(zero);
       if (A.g8.codes) load_kept<T>(A.g8, t, pl, g[u]);
       else if (A.g.p) load_unit<T>(seq::row_ptr<const T>(A.g, t, 0), pl, g[u]);
-      if (A.dn.p) load_unit<T>(seq::row_ptr<const T>(A.dn, t, 0), pl, dn[u]);
-      if (A.dr_out.p) load_unit<R>(seq::row_ptr<const R>(A.dr_out, t, 0), pl, dr[u]);
     }
+    float s[3] = {0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float w[kVals];
@@ -350,8 +391,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps) backward_kernel(const __grid_c
     sums(s);
     const float mr = rsqrtf(fmaf(s[0], inv, A.eps)), my = A.post_norm ? rsqrtf(fmaf(s[1], inv, A.eps)) : 1.f;
     const float back = mr * mr * mr * s[2] * inv;
-    float d[1] = {0.f};
-    float e[U][kVals];
+    float d[1] = {0.f}, e[U][kVals];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const Place<WIDE> pl(u, A.width);
@@ -359,23 +399,24 @@ __global__ void __launch_bounds__(32 * kMaxWarps) backward_kernel(const __grid_c
       load_weights<WIDE>(A.w_pre, pl, w);
 #pragma unroll
       for (int k = 0; k < kVals; ++k) {
-        out[k] = fmaf(mr * w[k], dn[u][k], fmaf(-back, r[u][k], dr[u][k]));
-        pre[u][k] = fmaf(dn[u][k], mr * r[u][k], pre[u][k]);
+        const float m = mr * dn[u][k];
+        out[k] = fmaf(w[k], m, fmaf(-back, r[u][k], dr[u][k]));
+        pre[u][k] = fmaf(m, r[u][k], pre[u][k]);
       }
       store_unit<R>(seq::row_ptr<R>(A.dr, t, 0), pl, out);
       if (!A.has_y) continue;
+      float a[kVals], slope[kVals];
       load_weights<WIDE>(A.w_post, pl, w);
+      gate_of<true>(gate, g[u], a, slope);
 #pragma unroll
       for (int k = 0; k < kVals; ++k) {
-        const Gate a = gate_of(A.gate, g[u][k]);
-        const float q = A.scale * out[k], yh = my * y[u][k];
-        out[k] = q * (w[k] * yh) * a.slope;
-        const float du = q * a.factor;
+        const float q = A.scale * out[k], yh = my * y[u][k], du = q * a[k];
+        if (gate != TO_GATE_NONE) out[k] = q * (w[k] * yh) * slope[k];
         post[u][k] = fmaf(du, yh, post[u][k]);
         e[u][k] = w[k] * du;
         d[0] = fmaf(e[u][k], yh, d[0]);
       }
-      if (A.dg.p) store_unit<T>(seq::row_ptr<T>(A.dg, t, 0), pl, out);
+      if (gate != TO_GATE_NONE) store_unit<T>(seq::row_ptr<T>(A.dg, t, 0), pl, out);
     }
     if (!A.has_y) continue;
     float m = 0.f;
@@ -452,7 +493,7 @@ struct Shape {
   int threads, rows, units;
 };
 Shape shape_of(int width) {
-  const int units = width > 8192 ? 2 : 1;
+  const int units = width > 256 ? 2 : 1;
   const int per = (width + kVals * units - 1) / (kVals * units);  // threads
   const int threads = (per + 31) / 32 * 32;
   return {threads, threads == 32 ? 8 : 1, units};
@@ -461,20 +502,22 @@ Shape shape_of(int width) {
 // CTAs of the gradients: what fits the SMs at once (their sums are added up afterwards).
 int backward_ctas(int width, long long tokens, int sms) {
   const Shape s = shape_of(width);
-  const long long per_sm = std::max(1, 1024 / (s.threads * s.rows));
+  const long long per_sm = std::max(1, 512 / (s.threads * s.rows));
   return static_cast<int>(std::max<long long>(1, std::min(per_sm * sms, (tokens + s.rows - 1) / s.rows)));
 }
 
-template <typename Args, typename F>
-int each_type(const to_block_norm_desc& d, bool wide, int units, F&& launch) {
-  auto with = [&](auto t, auto r) {
-    using T = decltype(t);
-    using R = decltype(r);
-    if (wide) return units == 1 ? launch(T{}, R{}, std::integral_constant<int, 1>{}, std::true_type{})
-                                : launch(T{}, R{}, std::integral_constant<int, 2>{}, std::true_type{});
-    return units == 1 ? launch(T{}, R{}, std::integral_constant<int, 1>{}, std::false_type{})
-                      : launch(T{}, R{}, std::integral_constant<int, 2>{}, std::false_type{});
+// launch(T, R, units, wide, threads of the largest CTA)
+template <typename F>
+int each_kernel(const to_block_norm_desc& d, bool wide, const Shape& shape, F&& launch) {
+  auto sized = [&](auto t, auto r, auto w) {
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    if (shape.units == 1) return launch(t, r, One{}, w, std::integral_constant<int, 256>{});
+    if (shape.threads * shape.rows <= 256) return launch(t, r, Two{}, w, std::integral_constant<int, 256>{});
+    if (shape.threads <= 512) return launch(t, r, Two{}, w, std::integral_constant<int, 512>{});
+    return launch(t, r, Two{}, w, std::integral_constant<int, 1024>{});
   };
+  auto with = [&](auto t, auto r) { return wide ? sized(t, r, std::true_type{}) : sized(t, r, std::false_type{}); };
   if (d.dtype == TO_F32) return with(float{}, float{});
   return d.residual == TO_F32 ? with(__nv_bfloat16{}, float{}) : with(__nv_bfloat16{}, __nv_bfloat16{});
 }
@@ -582,8 +625,8 @@ int to_block_norm(const to_block_norm_desc* desc, int64_t tokens, const to_block
   const Shape shape = shape_of(d.width);
   const unsigned grid = static_cast<unsigned>(std::min<long long>((tokens + shape.rows - 1) / shape.rows, 64ll * sms));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return each_type<ForwardArgs>(d, S.wide, shape.units, [&](auto t, auto r, auto units, auto wide) {
-    forward_kernel<decltype(t), decltype(r), decltype(units)::value, decltype(wide)::value>
+  return each_kernel(d, S.wide, shape, [&](auto t, auto r, auto units, auto wide, auto most) {
+    forward_kernel<decltype(t), decltype(r), decltype(units)::value, decltype(wide)::value, decltype(most)::value>
         <<<grid, dim3(shape.threads, shape.rows), 0, s>>>(A);
     TO_CUDA_TRY(cudaGetLastError());
     return ok();
@@ -664,8 +707,8 @@ int to_block_norm_backward(const to_block_norm_desc* desc, int64_t tokens, const
   A.eps = static_cast<float>(d.eps);
   const Shape shape = shape_of(d.width);
   const size_t shared = shape.rows > 1 ? size_t(shape.rows) * 2 * d.width * sizeof(float) : 0;  // (16 KB at most)
-  st = each_type<BackwardArgs>(d, S.wide, shape.units, [&](auto t, auto r, auto units, auto wide) {
-    backward_kernel<decltype(t), decltype(r), decltype(units)::value, decltype(wide)::value>
+  st = each_kernel(d, S.wide, shape, [&](auto t, auto r, auto units, auto wide, auto most) {
+    backward_kernel<decltype(t), decltype(r), decltype(units)::value, decltype(wide)::value, decltype(most)::value>
         <<<ctas, dim3(shape.threads, shape.rows), shared, s>>>(A);
     TO_CUDA_TRY(cudaGetLastError());
     return ok();

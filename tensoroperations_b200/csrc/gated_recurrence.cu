@@ -254,16 +254,8 @@ __device__ __forceinline__ void load_rows(char* dst, const Rows& r, int access, 
 
 // ---- the recurrence ------------------------------------------------------------------
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float reciprocal(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+using seq::exp2_fast;
+using seq::reciprocal;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
