@@ -19,6 +19,7 @@
 #include <cmath>
 
 #include "rows8.cuh"
+#include "sm100_primitives.cuh"
 
 namespace to_b200 {
 namespace {
@@ -38,6 +39,10 @@ struct Unit {
   __device__ __forceinline__ float operator[](int k) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(raw[k]);
     else return __uint_as_float(k & 1 ? raw[k / 2] & 0xffff0000u : raw[k / 2] << 16);
+  }
+  __device__ __forceinline__ V2<float> pair(int k) const {  // values 2 k, 2 k + 1
+    if constexpr (sizeof(T) == 4) return mk2(__uint_as_float(raw[2 * k]), __uint_as_float(raw[2 * k + 1]));
+    else return mk2(__uint_as_float(raw[k] << 16), __uint_as_float(raw[k] & 0xffff0000u));
   }
   __device__ __forceinline__ void set(const float (&x)[kVals]) {
     if constexpr (sizeof(T) == 4) {
@@ -145,27 +150,38 @@ __device__ __forceinline__ void keep_unit(const Packed& out, long long token, co
   }
 }
 
+// A unit's codes (WIDE: in its first two words) and its scale, and their values afterwards: the
+// codes of all rows are on their way before the first of them is waited for.
 template <typename T, bool WIDE>
-__device__ __forceinline__ void load_kept(const Packed& in, long long token, const Place<WIDE>& pl, Unit<T>& x) {
+__device__ __forceinline__ int load_kept(const Packed& in, long long token, const Place<WIDE>& pl, Unit<T>& x) {
   const int8_t* codes = in.codes + token * in.code_stride;
   const uint8_t* scales = in.scales + token * in.scale_stride;
-  float v[kVals] = {};
   if constexpr (WIDE) {
-    if (pl.on(0)) {
-      const uint2 w = *reinterpret_cast<const uint2*>(codes + pl.first);
-      const float scale = seq::scale_of(scales[pl.first / seq::kGroup8]);
-      float a[4], b[4];
-      seq::codes_to_f32(w.x, scale, a);
-      seq::codes_to_f32(w.y, scale, b);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = a[k], v[4 + k] = b[k];
-    }
+    x.raw[0] = x.raw[1] = 0;
+    if (!pl.on(0)) return 0;
+    const uint2 w = *reinterpret_cast<const uint2*>(codes + pl.first);
+    x.raw[0] = w.x, x.raw[1] = w.y;
+    return scales[pl.first / seq::kGroup8];
   } else {
+    float v[kVals];
 #pragma unroll
     for (int k = 0; k < kVals; ++k)
-      if (pl.on(k)) v[k] = seq::code_to_f32(codes[pl.col(k)], seq::scale_of(scales[pl.col(k) / seq::kGroup8]));
+      v[k] = pl.on(k) ? seq::code_to_f32(codes[pl.col(k)], seq::scale_of(scales[pl.col(k) / seq::kGroup8])) : 0.f;
+    x.set(v);  // (7 bits and a sign: exact in either type)
+    return 0;
   }
-  x.set(v);  // (7 bits and a sign: exact in either type)
+}
+template <bool WIDE, typename T>
+__device__ __forceinline__ void expand(Unit<T>& x, int byte) {
+  if constexpr (WIDE) {
+    const float scale = seq::scale_of(byte);
+    float a[4], b[4], v[kVals];
+    seq::codes_to_f32(x.raw[0], scale, a);
+    seq::codes_to_f32(x.raw[1], scale, b);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = a[k], v[4 + k] = b[k];
+    x.set(v);
+  }
 }
 
 // Sums over a row: of the warp, then of the CTA's warps in order.  `turn` picks one
@@ -219,8 +235,9 @@ __device__ __forceinline__ void gate_of(int kind, const Unit<T>& g, float (&fact
   } else {
 #pragma unroll
     for (int k = 0; k < kVals; ++k) {
-      const float t = -1.4426950408889634f * g[k];
-      const float e = seq::exp2_fast(t > 115.f ? 115.f : t);  // (below -80 sigmoid(g) counts as e^-80)
+      float t = -1.4426950408889634f * g[k];
+      asm("min.NaN.f32 %0, %1, 0f42E60000;" : "=f"(t) : "f"(t));  // 115: below -80 sigmoid(g) counts as e^-80
+      const float e = seq::exp2_fast(t);
       const float p = seq::reciprocal(1.f + e);               // sigmoid(g); 1 - sigmoid(g) is e p
       factor[k] = kind == TO_GATE_SIGMOID ? p : g[k] * p;
       if (SLOPES) slope[k] = kind == TO_GATE_SIGMOID ? p * (e * p) : fmaf(factor[k], e * p, p);
@@ -342,7 +359,10 @@ struct BackwardArgs {
 template <typename T, typename R, int U, bool WIDE, int MOST>
 __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) backward_kernel(const __grid_constant__ BackwardArgs A) {
   __shared__ alignas(16) float part[2][3][kMaxWarps], part_d[2][1][kMaxWarps];
-  extern __shared__ __align__(16) float rows[];  // several rows a CTA: [rows][2][width]
+  // this thread's columns of dw_pre and dw_post, four at a time: in registers they would take the
+  // room of values that would be unpacked again at each use (a quarter of all instructions)
+  extern __shared__ __align__(16) char shared[];
+  constexpr int kPairs = kVals / 2;
   RowSums<3> sums{part};
   RowSums<1> sum_d{part_d};
   const float inv = 1.f / static_cast<float>(A.width);
@@ -351,103 +371,141 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) backward_kernel(con
     sums.clear();
     sum_d.clear();
   }
-  float pre[U][kVals], post[U][kVals];  // this thread's columns of dw_pre, dw_post
+  const int threads = blockDim.x * blockDim.y, thread = threadIdx.y * blockDim.x + threadIdx.x;
+  auto columns = [&](int which, int u, int half) -> float4& {
+    return reinterpret_cast<float4*>(shared)[((which * U + u) * 2 + half) * threads + thread];
+  };
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+  for (int u = 0; u < 2 * U; ++u)
 #pragma unroll
-    for (int k = 0; k < kVals; ++k) pre[u][k] = post[u][k] = 0.f;
-  for (long long t = blockIdx.x * static_cast<long long>(blockDim.y) + threadIdx.y; t < A.tokens;
-       t += gridDim.x * static_cast<long long>(blockDim.y)) {
-    Unit<R> r[U], dr[U];
-    Unit<T> y[U], g[U], dn[U];
+    for (int h = 0; h < 2; ++h) columns(u / U, u % U, h) = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto gather = [&](int which, int u, const V2<float> (&x)[kPairs]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float4 c = columns(which, u, h);
+      const V2<float> a = add2(mk2(c.x, c.y), x[2 * h]), b = add2(mk2(c.z, c.w), x[2 * h + 1]);
+      columns(which, u, h) = make_float4(a.v.x, a.v.y, b.v.x, b.v.y);
+    }
+  };
+  const long long stride = gridDim.x * static_cast<long long>(blockDim.y);
+  for (long long t = blockIdx.x * static_cast<long long>(blockDim.y) + threadIdx.y; t < A.tokens; t += stride) {
+    Unit<R> r_[U], dr_[U];
+    Unit<T> y_[U], g[U], dn_[U];
+    int bytes[U][3];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const Place<WIDE> pl(u, A.width);
       const float zero[kVals] = {};
-      if (A.r8.codes) load_kept<R>(A.r8, t, pl, r[u]);
-      else load_unit<R>(seq::row_ptr<const R>(A.r, t, 0), pl, r[u]);
-      if (A.dn.p) load_unit<T>(seq::row_ptr<const T>(A.dn, t, 0), pl, dn[u]);
-      else dn[u].set(zero);
-      if (A.dr_out.p) load_unit<R>(seq::row_ptr<const R>(A.dr_out, t, 0), pl, dr[u]);
-      else dr[u].set(zero);
-      if (A.y8.codes) load_kept<T>(A.y8, t, pl, y[u]);
-      else if (A.y.p) load_unit<T>(seq::row_ptr<const T>(A.y, t, 0), pl, y[u]);
-      else y[u].set(zero);
-      if (A.g8.codes) load_kept<T>(A.g8, t, pl, g[u]);
+      if (A.r8.codes) bytes[u][0] = load_kept<R>(A.r8, t, pl, r_[u]);
+      else load_unit<R>(seq::row_ptr<const R>(A.r, t, 0), pl, r_[u]);
+      if (A.dn.p) load_unit<T>(seq::row_ptr<const T>(A.dn, t, 0), pl, dn_[u]);
+      else dn_[u].set(zero);
+      if (A.dr_out.p) load_unit<R>(seq::row_ptr<const R>(A.dr_out, t, 0), pl, dr_[u]);
+      else dr_[u].set(zero);
+      if (A.y8.codes) bytes[u][1] = load_kept<T>(A.y8, t, pl, y_[u]);
+      else if (A.y.p) load_unit<T>(seq::row_ptr<const T>(A.y, t, 0), pl, y_[u]);
+      else y_[u].set(zero);
+      if (A.g8.codes) bytes[u][2] = load_kept<T>(A.g8, t, pl, g[u]);
       else if (A.g.p) load_unit<T>(seq::row_ptr<const T>(A.g, t, 0), pl, g[u]);
     }
-    float s[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (A.r8.codes) expand<WIDE>(r_[u], bytes[u][0]);
+      if (A.y8.codes) expand<WIDE>(y_[u], bytes[u][1]);
+      if (A.g8.codes) expand<WIDE>(g[u], bytes[u][2]);
+    }
+    V2<float> r[U][kPairs], y[U][kPairs], dn[U][kPairs];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < kPairs; ++k) r[u][k] = r_[u].pair(k), y[u][k] = y_[u].pair(k), dn[u][k] = dn_[u].pair(k);
+    V2<float> s0 = mk2(0.f, 0.f), s1 = s0, s2 = s0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float w[kVals];
       load_weights<WIDE>(A.w_pre, Place<WIDE>(u, A.width), w);
 #pragma unroll
-      for (int k = 0; k < kVals; ++k) {
-        s[0] = fmaf(r[u][k], r[u][k], s[0]);
-        s[1] = fmaf(y[u][k], y[u][k], s[1]);
-        s[2] = fmaf(w[k] * dn[u][k], r[u][k], s[2]);
+      for (int k = 0; k < kPairs; ++k) {
+        s0 = fma2(r[u][k], r[u][k], s0);
+        s1 = fma2(y[u][k], y[u][k], s1);
+        s2 = fma2(mul2(mk2(w[2 * k], w[2 * k + 1]), dn[u][k]), r[u][k], s2);
       }
     }
+    float s[3] = {s0.v.x + s0.v.y, s1.v.x + s1.v.y, s2.v.x + s2.v.y};
     sums(s);
     const float mr = rsqrtf(fmaf(s[0], inv, A.eps)), my = A.post_norm ? rsqrtf(fmaf(s[1], inv, A.eps)) : 1.f;
-    const float back = mr * mr * mr * s[2] * inv;
-    float d[1] = {0.f}, e[U][kVals];
+    const float back = -mr * mr * mr * s[2] * inv;
+    const V2<float> mr2 = mk2(mr, mr), my2 = mk2(my, my), back2 = mk2(back, back), scale2 = mk2(A.scale, A.scale);
+    V2<float> d2 = mk2(0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const Place<WIDE> pl(u, A.width);
       float w[kVals], out[kVals];
       load_weights<WIDE>(A.w_pre, pl, w);
+      V2<float> q[kPairs], add[kPairs];
 #pragma unroll
-      for (int k = 0; k < kVals; ++k) {
-        const float m = mr * dn[u][k];
-        out[k] = fmaf(w[k], m, fmaf(-back, r[u][k], dr[u][k]));
-        pre[u][k] = fmaf(m, r[u][k], pre[u][k]);
+      for (int k = 0; k < kPairs; ++k) {
+        const V2<float> m = mul2(mr2, dn[u][k]);
+        q[k] = fma2(mk2(w[2 * k], w[2 * k + 1]), m, fma2(back2, r[u][k], dr_[u].pair(k)));
+        add[k] = mul2(m, r[u][k]);
+        out[2 * k] = q[k].v.x, out[2 * k + 1] = q[k].v.y;
       }
+      if (A.partial) gather(0, u, add);
       store_unit<R>(seq::row_ptr<R>(A.dr, t, 0), pl, out);
       if (!A.has_y) continue;
-      float a[kVals], slope[kVals];
       load_weights<WIDE>(A.w_post, pl, w);
+      float a[kVals], slope[kVals];
       gate_of<true>(gate, g[u], a, slope);
 #pragma unroll
-      for (int k = 0; k < kVals; ++k) {
-        const float q = A.scale * out[k], yh = my * y[u][k], du = q * a[k];
-        if (gate != TO_GATE_NONE) out[k] = q * (w[k] * yh) * slope[k];
-        post[u][k] = fmaf(du, yh, post[u][k]);
-        e[u][k] = w[k] * du;
-        d[0] = fmaf(e[u][k], yh, d[0]);
+      for (int k = 0; k < kPairs; ++k) {
+        const V2<float> sq = mul2(scale2, q[k]), du = mul2(sq, mk2(a[2 * k], a[2 * k + 1]));
+        const V2<float> wk = mk2(w[2 * k], w[2 * k + 1]);
+        y[u][k] = mul2(my2, y[u][k]);  // y^
+        if (gate != TO_GATE_NONE) {
+          const V2<float> o = mul2(mul2(sq, mk2(slope[2 * k], slope[2 * k + 1])), mul2(wk, y[u][k]));
+          out[2 * k] = o.v.x, out[2 * k + 1] = o.v.y;
+        }
+        add[k] = mul2(du, y[u][k]);
+        dn[u][k] = mul2(wk, du);
+        d2 = fma2(dn[u][k], y[u][k], d2);
       }
+      if (A.partial) gather(1, u, add);
       if (gate != TO_GATE_NONE) store_unit<T>(seq::row_ptr<T>(A.dg, t, 0), pl, out);
     }
     if (!A.has_y) continue;
     float m = 0.f;
     if (A.post_norm) {
+      float d[1] = {d2.v.x + d2.v.y};
       sum_d(d);
-      m = my * d[0] * inv;
+      m = -d[0] * inv;
     }
+    const V2<float> m2 = mk2(m, m);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const Place<WIDE> pl(u, A.width);
+      float out[kVals];
 #pragma unroll
-      for (int k = 0; k < kVals; ++k) e[u][k] = my * fmaf(-m, y[u][k], e[u][k]);
-      store_unit<T>(seq::row_ptr<T>(A.dy, t, 0), pl, e[u]);
+      for (int k = 0; k < kPairs; ++k) {
+        const V2<float> o = mul2(my2, fma2(m2, y[u][k], dn[u][k]));
+        out[2 * k] = o.v.x, out[2 * k + 1] = o.v.y;
+      }
+      store_unit<T>(seq::row_ptr<T>(A.dy, t, 0), Place<WIDE>(u, A.width), out);
     }
   }
   if (!A.partial) return;
   // the CTA's rows in order
-  const bool many = blockDim.y > 1;
-  float* to = many ? rows + threadIdx.y * 2ll * A.width : A.partial + blockIdx.x * 2ll * A.width;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const Place<WIDE> pl(u, A.width);
-    store_unit<float>(to, pl, pre[u]);
-    store_unit<float>(to + A.width, pl, post[u]);
-  }
-  if (!many) return;
   __syncthreads();
-  for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < 2 * A.width; i += blockDim.x * blockDim.y) {
-    float v = 0.f;
-    for (int k = 0; k < static_cast<int>(blockDim.y); ++k) v += rows[k * 2ll * A.width + i];
-    A.partial[blockIdx.x * 2ll * A.width + i] = v;
+  float* to = A.partial + blockIdx.x * 2ll * A.width;
+  if (threadIdx.y) return;
+#pragma unroll
+  for (int u = 0; u < 2 * U; ++u) {
+    float x[kVals] = {};
+    for (int row = 0; row < static_cast<int>(blockDim.y); ++row)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4 c = (&columns(u / U, u % U, h))[row * blockDim.x];
+        x[4 * h] += c.x, x[4 * h + 1] += c.y, x[4 * h + 2] += c.z, x[4 * h + 3] += c.w;
+      }
+    store_unit<float>(to + (u / U) * A.width, Place<WIDE>(u % U, A.width), x);
   }
 }
 
@@ -706,10 +764,13 @@ int to_block_norm_backward(const to_block_norm_desc* desc, int64_t tokens, const
   A.scale = static_cast<float>(d.scale);
   A.eps = static_cast<float>(d.eps);
   const Shape shape = shape_of(d.width);
-  const size_t shared = shape.rows > 1 ? size_t(shape.rows) * 2 * d.width * sizeof(float) : 0;  // (16 KB at most)
   st = each_kernel(d, S.wide, shape, [&](auto t, auto r, auto units, auto wide, auto most) {
-    backward_kernel<decltype(t), decltype(r), decltype(units)::value, decltype(wide)::value, decltype(most)::value>
-        <<<ctas, dim3(shape.threads, shape.rows), shared, s>>>(A);
+    constexpr int kUnits = decltype(units)::value, kMost = decltype(most)::value;
+    constexpr size_t kColumns = size_t(2) * kUnits * kVals * sizeof(float);  // of a thread
+    auto* kernel = backward_kernel<decltype(t), decltype(r), kUnits, decltype(wide)::value, kMost>;
+    static std::atomic<uint64_t> done;
+    if (int bad = seq::allow_shared(kernel, kColumns * kMost, done)) return bad;
+    kernel<<<ctas, dim3(shape.threads, shape.rows), kColumns * shape.threads * shape.rows, s>>>(A);
     TO_CUDA_TRY(cudaGetLastError());
     return ok();
   });
