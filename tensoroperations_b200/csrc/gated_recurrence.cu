@@ -90,6 +90,15 @@ __device__ __forceinline__ Vals<V> sub(Vals<V> a, Vals<V> b) {
   return fma(b, all<V>(-1.f), a);
 }
 
+// The same values, which the compiler keeps in registers: packed instructions take no
+// immediates, and made anew for each they cost two moves.
+template <int V>
+__device__ __forceinline__ Vals<V> kept(Vals<V> x) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) asm volatile("" : "+f"(x.v[i]));
+  return x;
+}
+
 template <typename T>
 struct Lane {
   static constexpr int kVec = 4 / int(sizeof(T));
@@ -164,10 +173,58 @@ __device__ __forceinline__ void next_ticket(const Chain& C, unsigned& ticket, in
   else if (lane == 0) asm volatile("atom.relaxed.gpu.global.add.u32 %0, [%1], 1;" : "=r"(ticket) : "l"(C.ticket) : "memory");
 }
 
+// The order of the segments.  Segments of one sequence that are in work at the same time wait
+// for one another's maps, so sequences are taken side by side: the slots are cut into at most
+// kSides parts, each at the beginning of a sequence, and every part in turn gives its next slot
+// (backwards: from its end).  A sequence lies in one part, so its segments keep their order.
+// (Four sequences of 4096 tokens, one after the other: 157 and 240 us forwards and backwards.)
+constexpr int kSides = 8;
+
+template <int SEG>
+struct Order {  // of a whole warp: lane g < kSides holds part g
+  int begin = 0, size = 0;
+
+  __device__ __forceinline__ Order(const Chain& C, int lane) {
+    if (lane < kSides) {
+      const int target = static_cast<int>(static_cast<long long>(C.slots) * lane / kSides);
+      int lo = 0, hi = lane ? C.nseq : 1;  // the last sequence that begins at or before it
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (bound_of(C, mid) / SEG + mid <= target) lo = mid;
+        else hi = mid;
+      }
+      begin = lane ? min(bound_of(C, lo) / SEG + lo, target) : 0;
+    }
+    const int next = __shfl_down_sync(0xffffffffu, begin, 1);
+    if (lane < kSides) size = max(0, (lane + 1 < kSides ? next : C.slots) - begin);
+  }
+  __device__ __forceinline__ int before(int round, int lane) const {  // slots of the rounds before
+    int n = min(size, round);
+#pragma unroll
+    for (int o = kSides / 2; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return __shfl_sync(0xffffffffu, n, 0);
+  }
+  // The n-th slot.
+  template <bool BACKWARD>
+  __device__ __forceinline__ int slot(int n, int most, int lane) const {
+    int lo = 0, hi = most;  // the round: before(lo) <= n < before(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (before(mid, lane) <= n) lo = mid;
+      else hi = mid;
+    }
+    const int k = n - before(lo, lane);
+    const uint32_t active = __ballot_sync(0xffffffffu, size > lo);
+    const bool mine = size > lo && __popc(active & ((1u << lane) - 1)) == k;
+    const int from = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+    return __shfl_sync(0xffffffffu, BACKWARD ? begin + size - 1 - lo : begin + lo, from);
+  }
+};
+
 // The item of a warp's ticket (lane 0's); a slot that no segment has goes to `unused`,
 // and the next ticket is taken.  `ticket`: the one that the item has.
 template <int SEG, bool BACKWARD, typename UNUSED>
-__device__ __forceinline__ Item next_item(const Chain& C, unsigned& ticket, int lane, UNUSED&& unused) {
+__device__ __forceinline__ Item next_item(const Chain& C, const Order<SEG>& order, unsigned& ticket, int lane, UNUSED&& unused) {
   Item it;
   for (;;) {
     ticket = __shfl_sync(0xffffffffu, ticket, 0);
@@ -177,7 +234,7 @@ __device__ __forceinline__ Item next_item(const Chain& C, unsigned& ticket, int 
       return it;
     }
     it.slab = static_cast<int>(ticket - at * C.slabs);
-    find_segment<SEG>(C, BACKWARD ? C.slots - 1 - static_cast<int>(at) : static_cast<int>(at), lane, it);
+    find_segment<SEG>(C, order.template slot<BACKWARD>(static_cast<int>(at), C.slots, lane), lane, it);
     if (it.idx >= 0) return it;
     unused(it);
     next_ticket(C, ticket, lane);
@@ -242,6 +299,11 @@ __device__ __forceinline__ void tma_tile(char* dst, const CUtensorMap* map, int 
       : "memory");
 }
 
+// (without an arrival)
+__device__ __forceinline__ void expect_bytes(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
 __device__ __forceinline__ void wait_full(uint64_t* bar, uint32_t parity) {
   if (!mbar_wait_bounded(bar, parity, 4 * kPolls)) atomicExch(&g_recurrence_status, TO_ERR_TIMEOUT);
 }
@@ -279,13 +341,13 @@ __device__ __forceinline__ Vals<V> gate_of(Vals<V> t) {
 // share a reciprocal (their product's, at most 17^4): 10 special functions for 8 values, not 16.
 constexpr float kCommon = -4.f;
 template <int V>
-__device__ __forceinline__ void rest_of(Vals<V> (&t)[4]) {
+__device__ __forceinline__ void rest_of(Vals<V> (&t)[4], const Vals<V>& one) {
   Vals<V> d[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
 #pragma unroll
     for (int i = 0; i < V; ++i) t[k].v[i] = exp2_fast(-t[k].v[i]);
-    d[k] = add(t[k], all<V>(1.f));
+    d[k] = add(t[k], one);
   }
   const Vals<V> d01 = mul(d[0], d[1]), d23 = mul(d[2], d[3]), product = mul(d01, d23);
   Vals<V> r;
@@ -528,26 +590,26 @@ __device__ __forceinline__ void open_stages(Stages& S) {
   __syncthreads();
 }
 
-// The warp that looks ahead.  fill(item, stage): the whole warp; load(item, stage): one lane,
-// arrives at full[stage].
+// The warp that looks ahead.  load(item, stage): one lane; fill(item, stage): the whole warp.
 template <int SEG, bool BACKWARD, typename UNUSED, typename FILL, typename LOAD>
 __device__ __forceinline__ void look_ahead(const Chain& C, Stages& S, UNUSED&& unused, FILL&& fill, LOAD&& load) {
   const int lane = threadIdx.x & 31;
+  const Order<SEG> order(C, lane);
   unsigned ticket = blockIdx.x;
   for (uint32_t k = 0;; ++k) {
     const int stage = k & 1;
     // (a ticket taken while its stage is still in use would keep the segments behind it waiting)
     if (k >= 2) wait_full(&S.empty[stage], (k / 2 - 1) & 1);
     if (k || C.ticket) next_ticket(C, ticket, lane);
-    const Item it = next_item<SEG, BACKWARD>(C, ticket, lane, unused);
-    if (it.slot >= 0) fill(it, stage);
-    if (lane == 0) S.items[stage] = it;
-    __syncwarp();
+    const Item it = next_item<SEG, BACKWARD>(C, order, ticket, lane, unused);
     if (lane == 0) {
+      S.items[stage] = it;
       arrive(&S.known[stage]);
       if (it.slot >= 0 && it.n > 0) load(it, stage);
-      else arrive(&S.full[stage]);
     }
+    if (it.slot >= 0) fill(it, stage);  // (while the tile is on its way)
+    __syncwarp();
+    if (lane == 0) arrive(&S.full[stage]);
     if (it.slot < 0) return;
   }
 }
@@ -599,9 +661,9 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
           biases[stage][lane] = b;
         },
         [&](const Item& it, int stage) {
-          if (!TMA) return arrive(&S.full[stage]);
+          if (!TMA) return;
           char* to = tiles + stage * 2 * kTile;
-          mbar_arrive_expect_tx(&S.full[stage], 2 * kTile);
+          expect_bytes(&S.full[stage], 2 * kTile);
           tma_tile(to, &A.x_map, it.slab * CH, it.row0, &S.full[stage]);
           tma_tile(to + kTile, &A.f_map, it.slab * CH, it.row0, &S.full[stage]);
         });
@@ -677,7 +739,7 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
 #pragma unroll
       for (int j = 0; j < kTok; j += 4) {
         P c[4] = {a[j], a[j + 1], a[j + 2], a[j + 3]};
-        rest_of(c);
+        rest_of(c, all<V>(1.f));
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int i = j + k;
@@ -772,7 +834,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
   __shared__ Map<V> maps[kWarps][32], ends[kWarps][32];
   __shared__ P enter[4][32], biases[2][32], firsts[2][32];
   __shared__ float sums[kWarps][CH];
-  __shared__ uint8_t scales[2][2][kBackward][kGroups];
+  __shared__ float scales[2][2][kBackward][kGroups];
   __shared__ Stages S;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Chain& C = A.C;
@@ -798,25 +860,35 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
           }
           biases[stage][lane] = b;
           firsts[stage][lane] = first;
+          // scales: all of them asked for before the first is waited for (rows and groups that are
+          // not there: others in their place)
+          constexpr int kRows = kBackward / 32;
+          uint8_t bytes[2][kRows][kGroups];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const Packed& from = k ? A.f.packed : A.x.packed;
-            if (!from.codes) continue;
+            if (!from.codes || it.n <= 0) continue;
 #pragma unroll
-            for (int r = 0; r < kBackward; r += 32) {
-              if (r + lane >= it.n) continue;
-              const uint8_t* row = from.scales + (it.row0 + static_cast<long long>(r + lane)) * from.scale_stride + ch / 32;
+            for (int r = 0; r < kRows; ++r) {
+              const uint8_t* row = from.scales + (it.row0 + static_cast<long long>(min(32 * r + lane, it.n - 1))) * from.scale_stride;
 #pragma unroll
-              for (int j = 0; j < kGroups; ++j)
-                scales[stage][k][r + lane][j] = ch + 32 * j < C.channels ? __ldg(row + j) : 0;
+              for (int j = 0; j < kGroups; ++j) bytes[k][r][j] = __ldg(row + min(ch / 32 + j, (C.channels - 1) / 32));
             }
+          }
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (!(k ? A.f.packed : A.x.packed).codes || it.n <= 0) continue;
+#pragma unroll
+            for (int r = 0; r < kRows; ++r)
+#pragma unroll
+              for (int j = 0; j < kGroups; ++j) scales[stage][k][32 * r + lane][j] = seq::scale_of(bytes[k][r][j]);
           }
         },
         [&](const Item& it, int stage) {
-          if (!TMA) return arrive(&S.full[stage]);
+          if (!TMA) return;
           char* to = tiles + stage * kStage;
           const int ch = it.slab * CH, x = A.x.packed.codes ? kBackward * CH : kTile, f = A.f.packed.codes ? kBackward * CH : kTile;
-          mbar_arrive_expect_tx(&S.full[stage], x + f + kTile);
+          expect_bytes(&S.full[stage], x + f + kTile);
           tma_tile(to, &A.x_map, ch, it.row0, &S.full[stage]);
           tma_tile(to + kTile, &A.f_map, ch, it.row0, &S.full[stage]);
           tma_tile(to + 2 * kTile, &A.dh_map, ch, it.row0, &S.full[stage]);
@@ -856,6 +928,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
     }
     close_tiles();
   };
+  const P one = kept(all<V>(1.f)), log2e = kept(all<V>(kLog2e)), offset = kept(all<V>(-8388736.f));
   if (!TMA) {
     wait_full(&S.full[0], 0);
     fetch(0);
@@ -876,12 +949,12 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
     const int c0 = it.slab * CH + lane * V, nc = min(V, C.channels - c0), t0 = warp * kTok;
     const int group = lane * V / seq::kGroup8;
     auto value = [&](const char* tile, int k, int t) {  // of rows in 8 bits
-      const float scale = seq::scale_of(scales[stage][k][t][group]);
+      const float scale = scales[stage][k][t][group];
       P out;
       if constexpr (V == 2) {
         const uint32_t both = *reinterpret_cast<const uint16_t*>(tile + t * CH + lane * V) ^ 0x8080u;  // codes + 128
         out = {{__uint_as_float(0x4b000000u | (both & 0xffu)), __uint_as_float(0x4b000000u | (both >> 8))}};
-        out = mul(add(out, all<V>(-8388736.f)), all<V>(scale));
+        out = mul(add(out, offset), all<V>(scale));
       } else {
         out.v[0] = seq::code_to_f32(reinterpret_cast<const int8_t*>(tile)[t * CH + lane], scale);
       }
@@ -897,11 +970,11 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
     float least = 0.f;
     if (A.f.packed.codes) {
 #pragma unroll
-      for (int i = 0; i < kTok; ++i) c[i] = fma(value(fs, 1, t0 + i), all<V>(kLog2e), bias);
+      for (int i = 0; i < kTok; ++i) c[i] = fma(value(fs, 1, t0 + i), log2e, bias);
     } else {
 #pragma unroll
       for (int i = 0; i < kTok; ++i)
-        c[i] = fma(L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4)), all<V>(kLog2e), bias);
+        c[i] = fma(L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4)), log2e, bias);
     }
 #pragma unroll
     for (int i = 0; i < kTok; ++i)
@@ -920,7 +993,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
 #pragma unroll
       for (int j = 0; j < kTok; j += 4) {
         P four[4] = {c[j], c[j + 1], c[j + 2], c[j + 3]};
-        rest_of(four);
+        rest_of(four, one);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int i = j + k;
