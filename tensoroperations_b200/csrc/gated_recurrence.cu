@@ -124,6 +124,7 @@ struct Chain {
   int nseq, tokens, channels, slabs, slots;  // slabs: tiles of channels; slots: segments that there may be
   unsigned* ticket;                          // null: no sequence is longer than a segment
   int* gave_up;                              // set once a wait of this call has run out
+  int late;                                  // tickets are taken as late as can be (see is_late)
   // [slots][slabs * kChannels] words of two f32, zero until they are published
   uint64_t* maps;    // (H, A with its sign bit set)
   uint64_t* states;  // (the entering state, 1)
@@ -183,6 +184,7 @@ constexpr int kSides = 8;
 template <int SEG>
 struct Order {  // of a whole warp: lane g < kSides holds part g
   int begin = 0, size = 0;
+  int round = 0, before = 0;  // before: upto(round)
 
   __device__ __forceinline__ Order(const Chain& C, int lane) {
     if (lane < kSides) {
@@ -198,33 +200,24 @@ struct Order {  // of a whole warp: lane g < kSides holds part g
     const int next = __shfl_down_sync(0xffffffffu, begin, 1);
     if (lane < kSides) size = max(0, (lane + 1 < kSides ? next : C.slots) - begin);
   }
-  __device__ __forceinline__ int before(int round, int lane) const {  // slots of the rounds before
-    int n = min(size, round);
-#pragma unroll
-    for (int o = kSides / 2; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    return __shfl_sync(0xffffffffu, n, 0);
+  __device__ __forceinline__ int upto(int rounds) const {  // slots of the first rounds
+    return __reduce_add_sync(0xffffffffu, min(size, rounds));
   }
-  // The n-th slot.
+  // The n-th slot; n never falls from one call to the next.
   template <bool BACKWARD>
-  __device__ __forceinline__ int slot(int n, int most, int lane) const {
-    int lo = 0, hi = most;  // the round: before(lo) <= n < before(hi)
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (before(mid, lane) <= n) lo = mid;
-      else hi = mid;
-    }
-    const int k = n - before(lo, lane);
-    const uint32_t active = __ballot_sync(0xffffffffu, size > lo);
-    const bool mine = size > lo && __popc(active & ((1u << lane) - 1)) == k;
+  __device__ __forceinline__ int slot(int n, int lane) {
+    for (int next; (next = upto(round + 1)) <= n; ++round) before = next;
+    const uint32_t active = __ballot_sync(0xffffffffu, size > round);
+    const bool mine = size > round && __popc(active & ((1u << lane) - 1)) == n - before;
     const int from = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
-    return __shfl_sync(0xffffffffu, BACKWARD ? begin + size - 1 - lo : begin + lo, from);
+    return __shfl_sync(0xffffffffu, BACKWARD ? begin + size - 1 - round : begin + round, from);
   }
 };
 
 // The item of a warp's ticket (lane 0's); a slot that no segment has goes to `unused`,
 // and the next ticket is taken.  `ticket`: the one that the item has.
 template <int SEG, bool BACKWARD, typename UNUSED>
-__device__ __forceinline__ Item next_item(const Chain& C, const Order<SEG>& order, unsigned& ticket, int lane, UNUSED&& unused) {
+__device__ __forceinline__ Item next_item(const Chain& C, Order<SEG>& order, unsigned& ticket, int lane, UNUSED&& unused) {
   Item it;
   for (;;) {
     ticket = __shfl_sync(0xffffffffu, ticket, 0);
@@ -234,7 +227,7 @@ __device__ __forceinline__ Item next_item(const Chain& C, const Order<SEG>& orde
       return it;
     }
     it.slab = static_cast<int>(ticket - at * C.slabs);
-    find_segment<SEG>(C, order.template slot<BACKWARD>(static_cast<int>(at), C.slots, lane), lane, it);
+    find_segment<SEG>(C, order.template slot<BACKWARD>(static_cast<int>(at), lane), lane, it);
     if (it.idx >= 0) return it;
     unused(it);
     next_ticket(C, ticket, lane);
@@ -594,14 +587,16 @@ __device__ __forceinline__ void open_stages(Stages& S) {
 template <int SEG, bool BACKWARD, typename UNUSED, typename FILL, typename LOAD>
 __device__ __forceinline__ void look_ahead(const Chain& C, Stages& S, UNUSED&& unused, FILL&& fill, LOAD&& load) {
   const int lane = threadIdx.x & 31;
-  const Order<SEG> order(C, lane);
+  Order<SEG> order(C, lane);
   unsigned ticket = blockIdx.x;
+  if (C.ticket) next_ticket(C, ticket, lane);
   for (uint32_t k = 0;; ++k) {
     const int stage = k & 1;
-    // (a ticket taken while its stage is still in use would keep the segments behind it waiting)
-    if (k >= 2) wait_full(&S.empty[stage], (k / 2 - 1) & 1);
-    if (k || C.ticket) next_ticket(C, ticket, lane);
+    if (k >= 2 && C.late) wait_full(&S.empty[stage], (k / 2 - 1) & 1);
+    if (k && C.late) next_ticket(C, ticket, lane);
     const Item it = next_item<SEG, BACKWARD>(C, order, ticket, lane, unused);
+    if (!C.late) next_ticket(C, ticket, lane);  // (its answer takes as long as a load from L2: one tile ahead)
+    if (k >= 2 && !C.late) wait_full(&S.empty[stage], (k / 2 - 1) & 1);
     if (lane == 0) {
       S.items[stage] = it;
       arrive(&S.known[stage]);
@@ -763,7 +758,7 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
     Map<V>(*const maps)[32] = all_maps[stage];
     maps[warp][lane] = own;
     __syncwarp();
-    if (lane == 0) arrive(&S.empty[stage]);
+    if (lane == 0 && !C.late) arrive(&S.empty[stage]);
     compute_sync();
     if (!TMA) {
       wait_full(&S.full[stage ^ 1], (turn + 1) / 2 & 1);
@@ -795,6 +790,7 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
       for (int i = 0; i < kTok; ++i)
         if (t0 + i < it.n) store_word<T>(row + i * A.h.ts, L::pack(fma(a[i], e, h[i])), nc, A.pairs);
     }
+    if (lane == 0 && C.late) arrive(&S.empty[stage]);
   }
 }
 
@@ -1313,6 +1309,13 @@ unsigned grid_of(const Chain& C, int sms, int per_sm) {
   return static_cast<unsigned>(std::min(static_cast<long long>(C.slots) * C.slabs, static_cast<long long>(sms) * per_sm));
 }
 
+// Whether tickets are taken as late as can be: where few chains of segments (one a tile of channels
+// and a sequence side by side) keep all CTAs busy, the segments of one are in work at the same time,
+// and every tile that a CTA holds for later keeps those behind it waiting.
+bool is_late(const Chain& C, unsigned grid) {
+  return C.ticket && 2ll * C.slabs * std::min(C.nseq, kSides) < grid;
+}
+
 }  // namespace
 
 int recurrence_device_status(int reset, int* value) {
@@ -1404,6 +1407,7 @@ int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_rec
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.partial, s));
   const unsigned grid = grid_of(A.C, sms, 2);
+  A.C.late = is_late(A.C, grid);
   constexpr size_t kShared = 4 * size_t(kForward) * kRowBytes;
   static std::atomic<uint64_t> done[16];
   auto launch = [&](auto t, auto keep, auto complement, auto tma) {
@@ -1492,6 +1496,7 @@ int to_gated_recurrence_backward(const to_gated_recurrence_desc* desc, const to_
   if (sms <= 0) return -sms;
   if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.partial, s));
   const unsigned grid = grid_of(A.C, sms, 2);
+  A.C.late = is_late(A.C, grid);
   constexpr size_t kShared = 2 * size_t(BackwardTiles<float>::kStage);
   static std::atomic<uint64_t> done[8];
   auto launch = [&](auto t, auto complement, auto tma) {
