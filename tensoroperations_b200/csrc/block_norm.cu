@@ -236,7 +236,7 @@ __device__ __forceinline__ void gate_of(int kind, const Unit<T>& g, float (&fact
 #pragma unroll
     for (int k = 0; k < kVals; ++k) {
       float t = -1.4426950408889634f * g[k];
-      asm("min.NaN.f32 %0, %1, 0f42E60000;" : "=f"(t) : "f"(t));  // 115: below -80 sigmoid(g) counts as e^-80
+      asm("min.NaN.f32 %0, %1, 0f42FC0000;" : "=f"(t) : "f"(t));  // 126: sigmoid(g) is 2^-126 at least
       const float e = seq::exp2_fast(t);
       const float p = seq::reciprocal(1.f + e);               // sigmoid(g); 1 - sigmoid(g) is e p
       factor[k] = kind == TO_GATE_SIGMOID ? p : g[k] * p;
@@ -732,8 +732,7 @@ int to_block_norm_backward(const to_block_norm_desc* desc, int64_t tokens, const
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int dev = 0;
   const int sms = device_sm_count(&dev);
-  if (sms <= 0) return -sms;
-  const int ctas = backward_ctas(d.width, tokens, sms);
+  const int ctas = backward_ctas(d.width, tokens, sms > 0 ? sms : 148);
   const bool sums = a.dw_post || a.dw_pre;
   if (sums) {
     const size_t need = size_t(ctas) * 2 * d.width * sizeof(float);
@@ -741,6 +740,7 @@ int to_block_norm_backward(const to_block_norm_desc* desc, int64_t tokens, const
       return set_error(TO_ERR_INVALID_ARGUMENT, "%s: workspace %zu < %zu bytes", who, a.workspace ? a.workspace_bytes : 0, need);
     if (!aligned(a.workspace, 16)) return set_error(TO_ERR_ALIGNMENT, "%s: workspace is not 16-byte aligned", who);
   }
+  if (sms <= 0) return -sms;
   BackwardArgs A{};
   A.r = seq::rows_of(a.r_out);
   A.y = seq::rows_of(a.y);

@@ -400,3 +400,249 @@ def test_norm_of_no_rows():
     ws = torch.empty(op.workspace_bytes(0), dtype=torch.uint8, device="cuda")
     op.backward(e, e, e, w, w, None, e.clone(), e.clone(), e.clone(), e.clone(), dw, dv, ws)
     assert (dw == 0).all() and (dv == 0).all()
+
+
+# ---- edges ---------------------------------------------------------------------------
+
+
+def block(tokens, channels, n, dtype=BF16, complement=True, seed=0):
+    """A recurrence's call of equal sequences: (op, inputs, buffers)."""
+    gen = torch.Generator("cuda").manual_seed(seed)
+    x, f, dh = cuda(tokens, channels, gen=gen, dtype=dtype), cuda(tokens, channels, gen=gen, dtype=dtype, scale=2.0), \
+        cuda(tokens, channels, gen=gen, dtype=dtype)
+    cu = torch.tensor([tokens * i // n for i in range(n + 1)], dtype=torch.int32, device="cuda")
+    op = sequence.GatedRecurrence(dtype, channels, complement)
+    ws = torch.empty(max(op.workspace_bytes(tokens, n), op.backward_workspace_bytes(tokens, n)), dtype=torch.uint8, device="cuda")
+    return op, x, f, dh, 2 + cuda(channels, gen=gen), cu, ws
+
+
+def both(op, x, f, dh, bias, cu, ws, keep=False, stream=None):
+    """Outputs of a forward and a backward call."""
+    tokens, channels, n = x.shape[0], x.shape[1], cu.numel() - 1
+    h, dx, df = (torch.zeros_like(x) for _ in range(3))
+    state, into, dbias = torch.zeros(n, channels, device="cuda"), torch.zeros(n, channels, device="cuda"), torch.zeros(channels, device="cuda")
+    saved = torch.zeros(op.saved_rows(tokens, n), channels, device="cuda")
+    kept = {"keep_" + k: sequence.Rows8.empty(tokens, channels) for k in "xf"} if keep else {}
+
+    def run():
+        op.forward(x, f, bias, cu, h, state_out=state, saved=saved, workspace=ws, stream=stream, **kept)
+        op.backward(kept.get("keep_x", x), kept.get("keep_f", f), bias, cu, saved, dh, dx, df, dbias, dstate_in=into,
+                    workspace=ws, stream=stream)
+
+    return run, (h, state, dx, df, dbias, into)
+
+
+@pytest.mark.parametrize("tokens,channels,n,keep", [(40000, 64, 1, False), (20000, 700, 1, True), (9000, 1024, 7, False),
+                                                    (4000, 333, 3, False)])
+def test_recurrence_repeats_to_the_bit(tokens, channels, n, keep):
+    call = block(tokens, channels, n, seed=tokens)
+    run, out = both(*call, keep=keep)
+    run()
+    first = [t.clone() for t in out]
+    for _ in range(40):
+        run()
+    torch.cuda.synchronize()
+    assert abi.lib.to_device_status(1) == 0
+    for a, b in zip(first, out):
+        assert torch.equal(a, b)
+
+
+def test_recurrence_many_sequences_as_one_by_one():
+    """Sequences taken side by side, of very different lengths, against each as a call of its own."""
+    lengths = [5000, 1, 0, 130, 2000, 129, 128, 0, 700, 3, 1500, 64, 900]
+    gen = torch.Generator("cuda").manual_seed(5)
+    tokens, n = sum(lengths), len(lengths)
+    op, x, f, dh, bias, _, _ = block(tokens, 200, 1, dtype=F32, seed=5)
+    ends = [sum(lengths[:i]) for i in range(n + 1)]
+    ws = torch.empty(max(op.workspace_bytes(tokens, n), op.backward_workspace_bytes(tokens, n)), dtype=torch.uint8, device="cuda")
+    run, out = both(op, x, f, dh, bias, torch.tensor(ends, dtype=torch.int32, device="cuda"), ws)
+    run()
+    for i in range(n):
+        a, b = ends[i], ends[i + 1]
+        one = torch.tensor([0, b - a], dtype=torch.int32, device="cuda")
+        single, want = both(op, x[a:b], f[a:b], dh[a:b], bias, one, ws)
+        single()
+        for got, w in zip((out[0][a:b], out[1][i:i + 1], out[2][a:b], out[3][a:b], out[5][i:i + 1]), (*want[:4], want[5])):
+            assert torch.equal(got, w), i
+
+
+def test_calls_on_two_streams_and_on_the_current_one():
+    calls = [block(6000, 256, 2, seed=s) for s in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    want = []
+    for call in calls:
+        run, out = both(*call)
+        run()
+        want.append([t.clone() for t in out])
+    torch.cuda.synchronize()
+    runs = [both(*call, stream=s.cuda_stream) for call, s in zip(calls, streams)]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for run, _ in runs:
+            run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    run, out = both(*calls[0][:-1], torch.empty_like(calls[0][-1]))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):  # no stream given: torch's current one
+        run()
+    torch.cuda.synchronize()
+    for w, (_, got) in zip(want + want[:1], runs + [(None, out)]):
+        for a, b in zip(w, got):
+            assert torch.equal(a, b)
+
+
+def test_captured_calls_replay():
+    """Two graphs that share a workspace, and new inputs between replays."""
+    call = block(3000, 256, 3)
+    run, out = both(*call, keep=True)
+    norm = sequence.BlockNorm("bf16", 256, gate="silu")
+    gen = torch.Generator("cuda").manual_seed(9)
+    r, g, ro, n = (cuda(3000, 256, gen=gen, dtype=BF16) for _ in range(4))
+    dr, dy, dg = (torch.zeros_like(r) for _ in range(3))
+    dw, dv = torch.zeros(256, device="cuda"), torch.zeros(256, device="cuda")
+    ws = torch.empty(norm.workspace_bytes(3000), dtype=torch.uint8, device="cuda")
+
+    def step():
+        run()
+        norm.forward(r, out[0], g, None, None, ro, n)
+        norm.backward(ro, out[0], g, None, None, r, n, dr, dy, dg, dw, dv, ws)
+
+    every = (*out, ro, n, dr, dy, dg, dw, dv)
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        graphs.append(graph)
+    for seed in (1, 2):
+        call[1].copy_(cuda(3000, 256, gen=torch.Generator("cuda").manual_seed(seed), dtype=BF16))
+        step()
+        want = [t.clone() for t in every]
+        for graph in graphs:
+            for t in every:
+                t.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(want, every):
+                assert torch.equal(a, b)
+
+
+def test_autograd_sees_what_is_written():
+    op, x, f, dh, bias, cu, ws = block(64, 32, 1)
+    h, state = torch.zeros_like(x), torch.zeros(1, 32, device="cuda")
+    kept = sequence.Rows8.empty(64, 32)
+    before = [t._version for t in (h, state, *kept)]
+    op.forward(x, f, bias, cu, h, state_out=state, keep_x=kept)
+    assert [t._version for t in (h, state, *kept)] == [v + 1 for v in before]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_infinities_stay_with_what_they_reach(dtype):
+    """An infinite or NaN value reaches its channel's later tokens (gradients: the earlier ones) and no others."""
+    op, x, f, dh, bias, cu, ws = block(1000, 96, 2, dtype=dtype, seed=4)
+    run, out = both(op, x, f, dh, bias, cu, ws)
+    run()
+    want = [t.clone() for t in out]
+    x[300, 7], f[620, 40], dh[200, 70] = float("inf"), float("nan"), float("nan")
+    run()
+    h, state, dx, df, dbias, into = out
+    spoilt = torch.zeros(1000, 96, dtype=torch.bool, device="cuda")
+    spoilt[300:500, 7] = spoilt[620:, 40] = True
+    assert not torch.isfinite(h[spoilt]).any() and torch.equal(h[~spoilt], want[0][~spoilt])
+    assert not torch.isfinite(state[0, 7]) and not torch.isfinite(state[1, 40])
+    assert torch.isfinite(state[0, torch.arange(96) != 7]).all()
+    back = torch.zeros_like(spoilt)
+    back[:201, 70] = back[500:621, 40] = True
+    assert not torch.isfinite(dx[back]).any() and torch.equal(dx[~back], want[2][~back])
+    assert not torch.isfinite(into[0, 70]) and not torch.isfinite(into[1, 40])
+    clean = torch.ones(96, dtype=torch.bool, device="cuda")
+    clean[[7, 40, 70]] = False
+    assert torch.equal(df[:, clean], want[3][:, clean]) and torch.equal(dbias[clean], want[4][clean])
+
+
+def test_gates_at_their_ends():
+    """Tokens that forget everything or nothing are exact, and what is left of a far decayed state keeps its digits."""
+    op = sequence.GatedRecurrence("f32", 4)
+    x = torch.zeros(700, 4, device="cuda")
+    f = torch.full((700, 4), 30.0, device="cuda")
+    f[:, 1] = float("inf")
+    f[350:, 2] = -13.0  # a = 2.3e-6 at every token: three leave 1e-17 of the state
+    f[353:, 2] = 30.0
+    f[400, 3], x[400, 3] = float("-inf"), 1e-3
+    state = torch.tensor([[2.0, 3.0, 5.0, 1e4]], device="cuda")
+    h, left = torch.empty_like(x), torch.empty_like(state)
+    ws = torch.empty(op.workspace_bytes(700, 1), dtype=torch.uint8, device="cuda")
+    op.forward(x, f, None, torch.tensor([0, 700], dtype=torch.int32, device="cuda"), h, state_in=state, state_out=left, workspace=ws)
+    assert h[-1, 1] == 3.0 and left[0, 1] == 3.0
+    want = 5.0 * torch.sigmoid(torch.tensor(-13.0, dtype=torch.float64)) ** 3
+    for got in (h[-1, 2], left[0, 2]):  # (700 tokens that forget 1e-13 each)
+        assert abs(float(got) / float(want) - 1) < (3 * (13 + 16) + 700 * 2) * U
+    assert h[400, 3] == x[400, 3] and abs(float(left[0, 3]) / 1e-3 - 1) < 300 * 4 * U
+
+
+@pytest.mark.parametrize("complement", [True, False])
+def test_gradients_against_differences(complement):
+    """dx, df, dbias and dstate against central differences of the 64-bit form, along random directions."""
+    lengths = [150, 0, 40]
+    op, x, f, dh, bias, _, ws = block(190, 24, 1, dtype=F32, complement=complement, seed=8)
+    gen = torch.Generator("cuda").manual_seed(8)
+    state, dstate = cuda(3, 24, gen=gen), cuda(3, 24, gen=gen)
+    cu = torch.tensor([0, 150, 150, 190], dtype=torch.int32, device="cuda")
+    h, dx, df = (torch.empty_like(x) for _ in range(3))
+    saved, into, dbias = torch.empty(op.saved_rows(190, 3), 24, device="cuda"), torch.empty_like(state), torch.empty_like(bias)
+    ws = torch.empty(max(op.workspace_bytes(190, 3), op.backward_workspace_bytes(190, 3)), dtype=torch.uint8, device="cuda")
+    op.forward(x, f, bias, cu, h, state_in=state, saved=saved, workspace=ws)
+    op.backward(x, f, bias, cu, saved, dh, dx, df, dbias, dstate_out=dstate, dstate_in=into, workspace=ws)
+    at = [d(t) for t in (x, f, bias, state)]
+
+    def loss(v):
+        hh, _, left, *_ = R.recurrence(v[0], v[1], v[2], lengths, v[3], complement)
+        return float((hh * d(dh)).sum() + (left * d(dstate)).sum())
+
+    cpu = torch.Generator().manual_seed(8)
+    for k, grad in enumerate((dx, df, dbias, into)):
+        way = torch.randn(at[k].shape, generator=cpu, dtype=torch.float64)
+        step = 1e-5
+        ends = [loss([v + s * step * way if j == k else v for j, v in enumerate(at)]) for s in (1, -1)]
+        # differences: step^2 of the third derivative, and the loss's rounding over the step; f32: its digits
+        slope, got = (ends[0] - ends[1]) / (2 * step), float((d(grad) * way).sum())
+        room = 1e-6 * float((d(grad) * way).abs().sum()) + 1e-6 * abs(slope) + 1e-6
+        assert abs(slope - got) < 200 * room, (k, slope, got)
+
+
+def test_norm_rows_keep_to_themselves():
+    """An infinity or NaN in a row leaves the other rows as they are."""
+    gen = torch.Generator("cuda").manual_seed(2)
+    op = sequence.BlockNorm("bf16", 264, residual="f32", gate="sigmoid")
+    r, y, g = cuda(20, 264, gen=gen), cuda(20, 264, gen=gen, dtype=BF16), cuda(20, 264, gen=gen, dtype=BF16)
+    out = []
+    for _ in range(2):
+        ro, n = torch.empty_like(r), torch.empty_like(y)
+        op.forward(r, y, g, None, None, ro, n)
+        out.append((ro, n))
+        y[3, 5], g[7, 100], r[11, 0] = float("inf"), float("nan"), float("-inf")
+    rows = torch.ones(20, dtype=torch.bool, device="cuda")
+    rows[[3, 7, 11]] = False
+    for a, b in zip(*out):
+        assert torch.equal(a[rows], b[rows]) and not torch.isfinite(b[~rows]).all(1).any()
+
+
+def test_largest_gates_and_smallest_rows():
+    """Gates of +-100, rows of zeros without eps (n has no value there) and with it."""
+    g = torch.tensor([[100.0, -100.0, 0.0, 30.0]], device="cuda")
+    y = torch.ones(1, 4, device="cuda")
+    for gate in ("sigmoid", "silu"):
+        op = sequence.BlockNorm("f32", 4, gate=gate, post_norm=False)
+        r, ro, n = torch.zeros(1, 4, device="cuda"), torch.empty(1, 4, device="cuda"), torch.empty(1, 4, device="cuda")
+        op.forward(r, y, g, None, None, ro, n)
+        p = torch.sigmoid(d(g))
+        want = p if gate == "sigmoid" else d(g) * p
+        # (where sigmoid(g) lies below 2^-126 the kernel has 2^-126)
+        close(ro, want, (2 * d(g).abs() + 16) * U * want.abs() + 2.0 ** -126 * d(g).abs().clamp(min=1), gate)
+    op = sequence.BlockNorm("f32", 4)
+    zero = torch.zeros(2, 4, device="cuda")
+    op.forward(zero, zero, None, None, None, ro2 := torch.empty(2, 4, device="cuda"), n2 := torch.empty(2, 4, device="cuda"))
+    assert (ro2 == 0).all() and (n2 == 0).all()
