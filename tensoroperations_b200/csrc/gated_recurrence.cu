@@ -347,7 +347,13 @@ __device__ __forceinline__ Vals<V> gate_of(Vals<V> t) {
 // -(1 - a) of four tokens where t >= kCommon: a is 1/17 at least, so that 1 - (1 - a) loses no
 // more than 17 of its roundings and the other form of a step is not needed.  The four 1 + exp(-f)
 // share a reciprocal (their product's, at most 17^4): 10 special functions for 8 values, not 16.
+// A NaN among them would reach the other tokens: it does not count as common (least_of).
 constexpr float kCommon = -4.f;
+__device__ __forceinline__ float least_of(float a, float b) {
+  float c;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
+}
 template <int V>
 __device__ __forceinline__ void rest_of(Vals<V> (&t)[4], const Vals<V>& one) {
   Vals<V> d[4];
@@ -741,7 +747,7 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
     for (int i = 0; i < kTok; ++i) {
       a[i] = fma(L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4)), all<V>(kLog2e), bias);
 #pragma unroll
-      for (int v = 0; v < V; ++v) least = fminf(least, a[i].v[v]);
+      for (int v = 0; v < V; ++v) least = least_of(least, a[i].v[v]);
     }
     if (it.n < kForward) least = kCommon - 1;  // (tokens that are not there: below)
     P at = all<V>(1.f), ht = all<V>(0.f);
@@ -990,7 +996,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
 #pragma unroll
     for (int i = 0; i < kTok; ++i)
 #pragma unroll
-      for (int v = 0; v < V; ++v) least = fminf(least, c[i].v[v]);
+      for (int v = 0; v < V; ++v) least = least_of(least, c[i].v[v]);
     const bool common = __all_sync(0xffffffffu, it.n == kBackward && least >= kCommon);
     P a = all<V>(1.f), h = all<V>(0.f), r = all<V>(0.f);
     if (A.x.packed.codes) {
@@ -1277,7 +1283,7 @@ int access_of(const to_rows8& r, int64_t tokens) {
 
 // Whether TMA takes rows (the smallest calls do without the two tensor maps), and their tensor map.
 bool tma_takes(const to_rows& r, const to_gated_recurrence_desc& d) {
-  return d.tokens >= kSegment && seq::rows_aligned(&r, d.tokens, 1, d.dtype, 16);
+  return d.tokens >= kSegment && r.token_stride < (1ll << 37) && seq::rows_aligned(&r, d.tokens, 1, d.dtype, 16);
 }
 int map_of(CUtensorMap* map, CUtensorMapDataType type, int bytes, const void* data, long long pitch, int row, int seg,
            const to_gated_recurrence_desc& d) {
@@ -1291,7 +1297,7 @@ int map_of(CUtensorMap* map, CUtensorMapDataType type, int bytes, const void* da
   return e == CUDA_SUCCESS ? ok() : set_error(TO_ERR_CUDA, "cuTensorMapEncodeTiled: %d", static_cast<int>(e));
 }
 bool tma_takes(const to_rows8& r, const to_gated_recurrence_desc& d) {
-  return d.tokens >= kSegment && aligned(r.codes, 16) && r.code_stride % 16 == 0;
+  return d.tokens >= kSegment && r.code_stride < (1ll << 37) && aligned(r.codes, 16) && r.code_stride % 16 == 0;
 }
 int map_of(CUtensorMap* map, const to_rows8& r, int seg, const to_gated_recurrence_desc& d) {
   return map_of(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, r.codes, r.code_stride, channels_of_tile(d), seg, d);
@@ -1493,6 +1499,11 @@ int to_gated_recurrence_backward(const to_gated_recurrence_desc* desc, const to_
     return seq::refuse_overlap(who, "dstate_in", "dstate_out");
   if (a.dstate_in && a.dstate_in < a.saved + size_t(slots_of(d, kSegment)) * d.channels && a.saved < a.dstate_in + states)
     return seq::refuse_overlap(who, "dstate_in", "saved");
+  for (const float* p : {static_cast<const float*>(a.dstate_in), a.dstate_out})
+    if (a.dbias && p && a.dbias < p + states && p < a.dbias + d.channels)
+      return seq::refuse_overlap(who, "dbias", p == a.dstate_in ? "dstate_in" : "dstate_out");
+  if (a.dbias && a.dbias < a.saved + size_t(slots_of(d, kSegment)) * d.channels && a.saved < a.dbias + d.channels)
+    return seq::refuse_overlap(who, "dbias", "saved");
   BackwardArgs A{};
   A.C = chain_of(d, a.cu_seqlens, l, a.workspace, kBackward);
   A.x = {seq::rows_of(a.x), seq::packed_of(a.x8), a.x8.codes ? access_of(a.x8, d.tokens) : access_of(a.x, d.tokens, d.dtype)};

@@ -2,7 +2,8 @@
 //
 // Memory bound: a value is read once and its code written once (3.03 bytes for
 // bf16), with about 5 instructions a value.  A thread takes 16 values, two threads a
-// group; they exchange nothing but their maxima.
+// group; they exchange nothing but their maxima.  Measured on B200: 16384 x 4096 bf16
+// in 45 us, 4.5 TB/s (0.69 of the copy rate), and back in 41 us, 5.0 TB/s.
 #include <algorithm>
 
 #include "rows8.cuh"

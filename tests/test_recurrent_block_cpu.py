@@ -96,14 +96,15 @@ def test_recurrence_other_refusals():
     assert step(op._desc(3, 0, 3), rec_args(s_out=FAR[8], h=(FAR[0], 64, 0)), 0) == BAD
     assert step(op._desc(0, 0), rec_args(x=(0, 0, 0)), 0) == abi.TO_OK
 
-    def grad(x=FAR[0], x8=(0, 0, 0, 0), dx=FAR[3], df=FAR[4], saved=FAR[5], d_out=0, d_in=0, ws=0, n=0):
+    def grad(x=FAR[0], x8=(0, 0, 0, 0), dx=FAR[3], df=FAR[4], saved=FAR[5], d_out=0, d_in=0, db=0, ws=0, n=0):
         rows = [(p, 64, 0) for p in (x, FAR[1], FAR[2], dx, df)]
-        return sequence._REC_GRAD_ARGS.pack(*sum(rows, ()), *x8, 0, 0, 0, 0, 0, BOGUS, saved, d_out, d_in, 0, ws, n)
+        return sequence._REC_GRAD_ARGS.pack(*sum(rows, ()), *x8, 0, 0, 0, 0, 0, BOGUS, saved, d_out, d_in, db, ws, n)
 
     back = abi.lib.to_gated_recurrence_backward
     need = op.backward_workspace_bytes(60, 1)
     for kw, want in ((dict(saved=0), BAD), (dict(saved=BOGUS + 8), ODD), (dict(dx=FAR[0]), BAD), (dict(df=FAR[3]), BAD),
                      (dict(d_out=FAR[6], d_in=FAR[6]), BAD), (dict(d_in=FAR[5]), BAD), (dict(d_in=BOGUS + 4), ODD),
+                     (dict(d_in=FAR[6], db=FAR[6] + 128), BAD), (dict(db=FAR[5]), BAD), (dict(db=BOGUS + 1), ODD),
                      (dict(x8=(FAR[7], 0, 64, 2)), BAD), (dict(x8=(FAR[3], FAR[7], 64, 2)), BAD)):
         assert back(op._desc(60, 1, 1), grad(ws=FAR[11], n=need, **kw), 0) == want, kw
     assert back(op._desc(60, 1, 1), grad(), 0) == BAD and b"workspace" in abi.lib.to_last_error()
@@ -158,6 +159,7 @@ def test_norm_other_refusals():
     assert back(op._desc, 9, grad(good, tail=(0, 0, FAR[8], 0, 0, 0)), 0) == BAD and b"workspace" in abi.lib.to_last_error()
     assert back(op._desc, 9, grad(good, tail=(0, 0, FAR[8] + 2, 0, FAR[9], 1 << 30)), 0) == ODD
     assert back(op._desc, 9, grad(good, tail=(0, 0, FAR[8], 0, FAR[9] + 8, 1 << 30)), 0) == ODD
+    assert back(op._desc, 9, grad(good, tail=(0, 0, FAR[8], FAR[8] + 128, FAR[9], 1 << 30)), 0) == BAD  # weights' gradients that meet
     assert back(op._desc, 9, None, 0) == BAD and back(None, 9, grad(good), 0) == BAD
 
 
