@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import os
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -56,6 +57,7 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     objs = []
     headers = [d for d in deps if d.suffix in (".cuh", ".hpp", ".h")]
     newest_header = max((h.stat().st_mtime for h in headers), default=0.0)
+    commands = []
     for src in _sources():
         obj = OBJ_DIR / (src.name + ".o")
         if force or not obj.exists() or obj.stat().st_mtime < max(src.stat().st_mtime, newest_header):
@@ -64,10 +66,12 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
                 cmd = [NVCC, "-x", "cu"] + NVCC_FLAGS + ["-c", str(src), "-o", str(obj)]
             if verbose:
                 cmd.insert(1, "-Xptxas=-v")
-            r = _run(cmd)
+            commands.append(cmd)
+        objs.append(obj)
+    with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:  # (each runs its own nvcc)
+        for r in pool.map(_run, commands):
             if verbose:
                 print(r.stderr)
-        objs.append(obj)
     tmp = LIB.with_suffix(".so.tmp")
     _run([NVCC] + ARCH + ["-shared", "-Xcompiler", "-fopenmp", "-o", str(tmp)] +
          [str(o) for o in objs] + ["-lcudart", "-ldl"])
