@@ -977,10 +977,6 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
       }
       return out;
     };
-    auto x_of = [&](int i) {
-      return A.x.packed.codes ? value(xs, 0, t0 + i)
-                              : L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4));
-    };
     auto dh_of = [&](int i) { return L::unpack(*reinterpret_cast<const uint32_t*>(gs + (t0 + i) * kRowBytes + lane * 4)); };
     P c[kTok], w[kTok];  // c[i] is t before; w: x, then df_t / G_t
     const P bias = biases[stage][lane];

@@ -144,7 +144,8 @@ def _cuda(t, name: str):
 
 
 def _on(stream: Optional[int], device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
+    # (torch.cuda.current_stream makes an object, which takes longer than the smallest kernels)
+    return torch._C._cuda_getCurrentRawStream(device.index) if stream is None else stream
 
 
 def _scratch(t, need: int, device):
