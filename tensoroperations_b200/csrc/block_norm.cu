@@ -136,11 +136,9 @@ __device__ __forceinline__ void keep_unit(const Packed& out, long long token, co
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
     const int byte = seq::scale_byte(most);
     const float inverse = seq::inverse_scale(byte);
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int k = 0; k < kVals; ++k) w[k / 4] |= seq::code_of(x[k], inverse, byte != 255) << (8 * (k % 4));
     if (!pl.on(0)) return;
-    *reinterpret_cast<uint2*>(codes + pl.first) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(codes + pl.first) =
+        make_uint2(seq::codes_of(x, inverse, byte != 255), seq::codes_of(x + 4, inverse, byte != 255));
     if (threadIdx.x % 4 == 0) scales[pl.first / seq::kGroup8] = static_cast<uint8_t>(byte);
   } else {
 #pragma unroll

@@ -543,18 +543,21 @@ __device__ __forceinline__ void keep_tile(const char* tile, const Packed& out, i
     float x[16];
     seq::load_vec<T, 16>(reinterpret_cast<const T*>(tile + row * kRowBytes) + part * 16, x);
     uint32_t most = 0;
+    if constexpr (sizeof(T) == 2) {  // two at a time, as they lie
+      const uint4* raw = reinterpret_cast<const uint4*>(tile + row * kRowBytes + part * 32);
+      const uint4 a = raw[0], b = raw[1];
+      for (const uint32_t w : {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}) most = __vmaxu2(most, w & 0x7fff7fffu);
+      most = max(most << 16, most & 0xffff0000u);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 16; ++k) most = max(most, seq::abs_bits(x[k]));
+      for (int k = 0; k < 16; ++k) most = max(most, seq::abs_bits(x[k]));
+    }
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
     const int byte = seq::scale_byte(most);
     const float inverse = seq::inverse_scale(byte);
     union { uint4 v; uint32_t w[4]; uint8_t b[16]; } u;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      u.w[k] = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) u.w[k] |= seq::code_of(x[4 * k + j], inverse, byte != 255) << (8 * j);
-    }
+    for (int k = 0; k < 4; ++k) u.w[k] = seq::codes_of(x + 4 * k, inverse, byte != 255);
     if (row >= it.n || c >= channels) continue;
     int8_t* to = out.codes + (it.row0 + static_cast<long long>(row)) * out.code_stride + c;
     const int n = min(16, channels - c);

@@ -53,11 +53,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const __grid_constant__ Rows8
     const float inverse = seq::inverse_scale(byte);
     union { uint4 v; uint32_t w[4]; } u;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      u.w[k] = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) u.w[k] |= seq::code_of(x[4 * k + j], inverse, byte != 255) << (8 * j);
-    }
+    for (int k = 0; k < 4; ++k) u.w[k] = seq::codes_of(x + 4 * k, inverse, byte != 255);
     if (n <= 0) continue;
     int8_t* to = A.p.codes + token * A.p.code_stride + c;
     if (A.wide && n == kUnit) {

@@ -46,10 +46,19 @@ __device__ __forceinline__ float inverse_scale(int byte) {
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// x / scale to the nearest integer, as the low byte (adding 1.5 * 2^23 leaves the
+// x / scale to the nearest integer, in the low byte (adding 1.5 * 2^23 leaves the
 // integer in the sum's last bits; |x / scale| <= 127).
+__device__ __forceinline__ uint32_t code_bits(float x, float inverse) {
+  return __float_as_uint(fmaf(x, inverse, 12582912.f));
+}
 __device__ __forceinline__ uint32_t code_of(float x, float inverse, bool finite) {
-  return finite ? __float_as_uint(fmaf(x, inverse, 12582912.f)) & 0xffu : 0u;
+  return finite ? code_bits(x, inverse) & 0xffu : 0u;
+}
+// Four of them as a word.
+__device__ __forceinline__ uint32_t codes_of(const float* x, float inverse, bool finite) {
+  const uint32_t low = __byte_perm(code_bits(x[0], inverse), code_bits(x[1], inverse), 0x0040);
+  const uint32_t high = __byte_perm(code_bits(x[2], inverse), code_bits(x[3], inverse), 0x0040);
+  return finite ? __byte_perm(low, high, 0x5410) : 0u;
 }
 
 // Four codes of a word.
