@@ -18,10 +18,11 @@
 // Measured on B200 (bf16): 49152 tokens x 4096 channels, one sequence, in 261 us, 4.6
 // TB/s (0.71 of the copy rate): its 64 chains of segments keep 296 CTAs busy, so four or
 // five segments of a chain are in work at once and wait for one another's maps (without
-// those waits 200 us).  4 x 4096 tokens x 4096 with 8-bit copies 136 us, 4.0 TB/s; gradients
-// of these 170 us, 3.9 TB/s, from 8 bits 212 us, 2.6 TB/s: 30 instructions a value, 16 warps
-// an SM.  Eight more warps that only reduce, a tile ahead, and eight that walk (no maps in
-// registers) needed half as many instructions again: 277 us for the first figure.
+// those waits 200 us).  4 x 4096 tokens x 4096 with 8-bit copies 126 us, 4.3 TB/s, 44
+// instructions a value, near what 20 warps an SM issue; gradients of these 167 us, 4.0 TB/s,
+// from 8 bits 212 us, 2.6 TB/s: they wait for tiles and for the slowest of eight warps.  Eight
+// more warps that only reduce, a tile ahead, and eight that walk (no maps in registers) needed
+// half as many instructions again: 277 us for the first figure.
 //
 // Gates: with u = exp(-|f|), u / (1 + u) is the smaller of a and 1 - a, accurate to
 // f32 relative to itself.  It is kept with a sign ("c": a where positive, -(1 - a)
@@ -188,7 +189,7 @@ __device__ __forceinline__ void next_ticket(const Chain& C, unsigned& ticket, in
 // for one another's maps, so sequences are taken side by side: the slots are cut into at most
 // kSides parts, each at the beginning of a sequence, and every part in turn gives its next slot
 // (backwards: from its end).  A sequence lies in one part, so its segments keep their order.
-// (Four sequences of 4096 tokens, 4096 channels, forwards: 157 us one after the other, 136 so.)
+// (Four sequences of 4096 tokens, 4096 channels, forwards: 157 us one after the other, then 136.)
 constexpr int kSides = 8;
 
 template <int SEG>
