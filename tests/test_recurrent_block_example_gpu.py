@@ -27,7 +27,7 @@ def test_serving_agrees_with_whole_sequences():
     assert _example().serve(128, 2, [300, 1, 140], 4) <= 2 * 2.0 ** -7 * 4
 
 
-def _plain(stack, x, lengths, kept=True):
+def _plain(stack, x, lengths):
     """The stack from elementary operations in 64 bits, on leaves that autograd follows."""
     leaves = [p.detach().cpu().double().requires_grad_() for p in stack.parameters()]
     n = stack.blocks
@@ -67,7 +67,7 @@ def test_gradients_of_the_stack():
     y = stack.forward(x, cu, kept=kept)
     want, leaves = _plain(stack, x, lengths)
     # (products in f32, TF32 off: 64 sums of 2^-24 each, through two blocks)
-    assert float((y.cpu().double() - want).norm() / want.norm()) < 1e-4
+    assert float((y.cpu().double() - want.detach()).norm() / want.detach().norm()) < 1e-4
     (want * dy.cpu().double()).sum().backward()
     for got, leaf in zip(stack.backward(dy, cu, kept), leaves):
         off = float((got.cpu().double() - leaf.grad).norm() / leaf.grad.norm())
