@@ -437,7 +437,9 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) backward_kernel(con
     float s[3] = {s0.v.x + s0.v.y, s1.v.x + s1.v.y, s2.v.x + s2.v.y};
     sums(s);
     const float mr = rsqrtf(fmaf(s[0], inv, A.eps)), my = A.post_norm ? rsqrtf(fmaf(s[1], inv, A.eps)) : 1.f;
-    const float back = -mr * mr * mr * s[2] * inv;
+    // -mean(e r^) / rms: made of mean(e r) / rms, so that no power of 1 / rms leaves f32 before dr does
+    // (1 / rms^3 is infinite below an rms of 1.4e-13 and zero above 1e15)
+    const float back = -(mr * s[2] * inv) * mr;
     const V2<float> mr2 = mk2(mr, mr), my2 = mk2(my, my), back2 = mk2(back, back), scale2 = mk2(A.scale, A.scale);
     V2<float> d2 = mk2(0.f, 0.f);
 #pragma unroll
@@ -448,9 +450,9 @@ __global__ void __launch_bounds__(MOST, MOST == 256 ? 2 : 1) backward_kernel(con
       V2<float> q[kPairs], add[kPairs];
 #pragma unroll
       for (int k = 0; k < kPairs; ++k) {
-        const V2<float> m = mul2(mr2, dn[u][k]);
-        q[k] = fma2(mk2(w[2 * k], w[2 * k + 1]), m, fma2(back2, r[u][k], dr_[u].pair(k)));
-        add[k] = mul2(m, r[u][k]);
+        const V2<float> m = mul2(mr2, dn[u][k]), rh = mul2(mr2, r[u][k]);  // rh: r^
+        q[k] = fma2(mk2(w[2 * k], w[2 * k + 1]), m, fma2(back2, rh, dr_[u].pair(k)));
+        add[k] = mul2(dn[u][k], rh);
         out[2 * k] = q[k].v.x, out[2 * k + 1] = q[k].v.y;
       }
       if (A.partial) gather(0, u, add);
