@@ -849,8 +849,9 @@ int to_gated_recurrence_step(const to_gated_recurrence_desc* desc,
  * [tokens][width] (one head: head_stride is not used).  act(g): g, sigmoid(g) or
  * g * sigmoid(g).  w_post, w_pre: device f32 [width], NULL for 1.  y NULL (a model's
  * first norm): n is made of r, and there is no r_out, g or keep_y.  n NULL: only
- * r_out is made.  Sums are f32; each output takes one rounding, n from r_out
- * before its own.  width 1 .. 16384.
+ * r_out is made.  Sums are f32, of squares too: a row's sum of squares has to lie
+ * in f32's range, and with eps = 0 above 2^-126.  Each output takes one rounding,
+ * n from r_out before its own.  width 1 .. 16384.
  *
  * keep_r, keep_y, keep_g (codes not NULL): r_out before its rounding (r, where there
  * is no y), y and g are also written in 8 bits, for the gradients.
@@ -866,8 +867,8 @@ typedef struct to_block_norm_desc {
   int32_t gate;      /* to_gate                                              */
   int32_t post_norm; /* 0 or 1                                               */
   int32_t reserved0;
-  double scale;      /* finite                                               */
-  double eps;        /* >= 0                                                 */
+  double scale;      /* finite in f32                                        */
+  double eps;        /* 0, or in f32's range (not below 2^-149)              */
 } to_block_norm_desc;
 
 typedef struct to_block_norm_args {

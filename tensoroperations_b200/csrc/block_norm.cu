@@ -546,7 +546,9 @@ int check_desc(const char* who, const to_block_norm_desc* desc) {
   if (d.gate < TO_GATE_NONE || d.gate > TO_GATE_SILU) return set_error(TO_ERR_INVALID_ARGUMENT, "%s: gate %d", who, d.gate);
   if (d.post_norm != 0 && d.post_norm != 1)
     return set_error(TO_ERR_INVALID_ARGUMENT, "%s: post_norm %d", who, d.post_norm);
-  if (!std::isfinite(d.scale) || !(d.eps >= 0) || !std::isfinite(d.eps))
+  // (the kernels hold both in f32: one that is infinite there, or an eps that becomes zero, is refused too)
+  if (!std::isfinite(static_cast<float>(d.scale)) || !(d.eps >= 0) || !std::isfinite(static_cast<float>(d.eps)) ||
+      (d.eps > 0 && static_cast<float>(d.eps) == 0))
     return set_error(TO_ERR_INVALID_ARGUMENT, "%s: scale %g, eps %g", who, d.scale, d.eps);
   return ok();
 }
