@@ -330,7 +330,12 @@ using seq::reciprocal;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// c of a gate, from t = log2(e) (f + bias); below 2^-126 it counts as zero.
+// t = log2(e) (f + bias).  The sum comes first: its rounding is relative to f + bias, also where the two cancel.
+template <int V>
+__device__ __forceinline__ Vals<V> argument_of(Vals<V> f, Vals<V> bias, const Vals<V>& log2e) {
+  return mul(add(f, bias), log2e);
+}
+// c of a gate, from its argument; below 2^-126 it counts as zero.
 template <int V>
 __device__ __forceinline__ Vals<V> gate_of(Vals<V> t) {
   Vals<V> u, r;
@@ -677,7 +682,7 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
 #pragma unroll
           for (int v = 0; v < V; ++v)
             if (A.bias && it.slab * CH + lane * V + v < C.channels)
-              b.v[v] = kLog2e * __ldg(A.bias + it.slab * CH + lane * V + v);
+              b.v[v] = __ldg(A.bias + it.slab * CH + lane * V + v);
           biases[stage][lane] = b;
         },
         [&](const Item& it, int stage) {
@@ -722,6 +727,7 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
     }
     close_tiles();
   };
+  const P log2e = kept(all<V>(kLog2e));
   if (!TMA) {
     wait_full(&S.full[0], 0);
     fetch(0);
@@ -749,7 +755,7 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
     float least = 0.f;
 #pragma unroll
     for (int i = 0; i < kTok; ++i) {
-      a[i] = fma(L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4)), all<V>(kLog2e), bias);
+      a[i] = argument_of(L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4)), bias, log2e);
 #pragma unroll
       for (int v = 0; v < V; ++v) least = least_of(least, a[i].v[v]);
     }
@@ -876,7 +882,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
           for (int v = 0; v < V; ++v) {
             const int c = ch + lane * V + v;
             if (c >= C.channels) continue;
-            if (A.bias) b.v[v] = kLog2e * __ldg(A.bias + c);
+            if (A.bias) b.v[v] = __ldg(A.bias + c);
             first.v[v] = __ldg(A.saved + static_cast<long long>(saved_row<kBackward>(C, it)) * C.channels + c);
           }
           biases[stage][lane] = b;
@@ -987,11 +993,11 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
     float least = 0.f;
     if (A.f.packed.codes) {
 #pragma unroll
-      for (int i = 0; i < kTok; ++i) c[i] = fma(value(fs, 1, t0 + i), log2e, bias);
+      for (int i = 0; i < kTok; ++i) c[i] = argument_of(value(fs, 1, t0 + i), bias, log2e);
     } else {
 #pragma unroll
       for (int i = 0; i < kTok; ++i)
-        c[i] = fma(L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4)), log2e, bias);
+        c[i] = argument_of(L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4)), bias, log2e);
     }
 #pragma unroll
     for (int i = 0; i < kTok; ++i)
@@ -1199,7 +1205,8 @@ __global__ void __launch_bounds__(256) step_kernel(const __grid_constant__ StepA
     seq::load_vec<T, V>(seq::row_ptr<const T>(A.f, token, 0) + c, f);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const Vals<1> g = gate_of(Vals<1>{{kLog2e * (f[v] + (A.bias ? __ldg(A.bias + c + v) : 0.f))}}), xv{{x[v]}}, hv{{h[v]}};
+      const Vals<1> b{{A.bias ? __ldg(A.bias + c + v) : 0.f}}, fv{{f[v]}}, xv{{x[v]}}, hv{{h[v]}};
+      const Vals<1> g = gate_of(argument_of(fv, b, all<1>(kLog2e)));
       h[v] = (A.complement ? stepped<true>(g, xv, hv) : stepped<false>(g, xv, hv)).v[0];
     }
     seq::store_vec<float, V>(state, h);
