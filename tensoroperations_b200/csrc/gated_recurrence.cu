@@ -11,8 +11,8 @@
 // maps of the warps are joined in shared memory, those of the segments through
 // global memory while the CTAs run (below), and with the state that enters every
 // output is one multiply-add.  So x and f are read once and h is written once; 8
-// flops and two special functions a value (exp and a share of a reciprocal) leave
-// it memory bound in principle.  Gradients keep the gates and df_t / G_t instead,
+// flops, two special functions a value (exp and a reciprocal) and three selections
+// leave it memory bound in principle.  Gradients keep the gates and df_t / G_t instead,
 // and walk back once what enters from behind is known.
 //
 // Measured on B200 (bf16): 49152 tokens x 4096 channels, one sequence, in 261 us, 4.6
@@ -29,7 +29,10 @@
 // where negative), and every step adds c times a difference to the larger term:
 //   f >= 0:  h + (1 - a)(x - h)      f < 0:  x + a (h - x)
 // so a memory of thousands of tokens does not take over a rounding of a near 1, and
-// what is left of a state after a token that almost forgets it stays exact.
+// what is left of a state after a token that almost forgets it stays exact.  All gates
+// take these steps: a path without the selections, for tiles whose gates all lie above
+// -2.77 (a made of 1 - a, four tokens' reciprocals shared), was 4 to 8 % faster forwards, but
+// lost up to 6 bits of a there, and a channel's digits went by its neighbours' gates.
 //
 // Joining the segments: a CTA takes segments in the order of a counter (so a
 // segment's predecessors have been taken by CTAs that run), publishes its map as
@@ -350,35 +353,6 @@ __device__ __forceinline__ Vals<V> gate_of(Vals<V> t) {
     r.v[i] = __uint_as_float(__float_as_uint(r.v[i]) | (~__float_as_uint(t.v[i]) & 0x80000000u));
   return r;
 }
-// -(1 - a) of four tokens where t >= kCommon: a is 1/17 at least, so that 1 - (1 - a) loses no
-// more than 17 of its roundings and the other form of a step is not needed.  The four 1 + exp(-f)
-// share a reciprocal (their product's, at most 17^4): 10 special functions for 8 values, not 16.
-// A NaN among them would reach the other tokens: it does not count as common (least_of).
-constexpr float kCommon = -4.f;
-__device__ __forceinline__ float least_of(float a, float b) {
-  float c;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
-  return c;
-}
-template <int V>
-__device__ __forceinline__ void rest_of(Vals<V> (&t)[4], const Vals<V>& one) {
-  Vals<V> d[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) t[k].v[i] = exp2_fast(-t[k].v[i]);
-    d[k] = add(t[k], one);
-  }
-  const Vals<V> d01 = mul(d[0], d[1]), d23 = mul(d[2], d[3]), product = mul(d01, d23);
-  Vals<V> r;
-#pragma unroll
-  for (int i = 0; i < V; ++i) r.v[i] = reciprocal(-product.v[i]);
-  const Vals<V> r01 = mul(r, d23), r23 = mul(r, d01);
-  t[0] = mul(t[0], mul(r01, d[1]));
-  t[1] = mul(t[1], mul(r01, d[0]));
-  t[2] = mul(t[2], mul(r23, d[3]));
-  t[3] = mul(t[3], mul(r23, d[2]));
-}
 // c is -(1 - a)
 __device__ __forceinline__ bool is_rest(float c) { return __float_as_int(c) < 0; }
 // a h
@@ -397,12 +371,6 @@ __device__ __forceinline__ Vals<V> stepped(Vals<V> c, Vals<V> x, Vals<V> h) {
 #pragma unroll
   for (int i = 0; i < V; ++i) base.v[i] = is_rest(c.v[i]) ? other.v[i] : x.v[i];
   return fma(c, COMPLEMENT ? sub(h, x) : h, base);
-}
-
-// The same where c is -(1 - a).
-template <bool COMPLEMENT, int V>
-__device__ __forceinline__ Vals<V> stepped_rest(Vals<V> c, Vals<V> x, Vals<V> h) {
-  return COMPLEMENT ? fma(c, sub(h, x), h) : fma(c, h, add(h, x));
 }
 
 // h -> a h + b of a lane's channels.
@@ -749,42 +717,25 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
       if (A.keep_x.codes) keep_tile<T>(xs, A.keep_x, A.keep_access, it, ch, C.channels);
       if (A.keep_f.codes) keep_tile<T>(fs, A.keep_f, A.keep_access, it, ch, C.channels);
     }
-    // the map of a warp's first tokens, up to every one of them; a[i] is t before
+    // the map of a warp's first tokens, up to every one of them
     P a[kTok], h[kTok];
     const P bias = biases[stage][lane];
-    float least = 0.f;
-#pragma unroll
-    for (int i = 0; i < kTok; ++i) {
-      a[i] = argument_of(L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4)), bias, log2e);
-#pragma unroll
-      for (int v = 0; v < V; ++v) least = least_of(least, a[i].v[v]);
-    }
-    if (it.n < kForward) least = kCommon - 1;  // (tokens that are not there: below)
     P at = all<V>(1.f), ht = all<V>(0.f);
-    if (__all_sync(0xffffffffu, least >= kCommon)) {
-#pragma unroll
-      for (int j = 0; j < kTok; j += 4) {
-        P c[4] = {a[j], a[j + 1], a[j + 2], a[j + 3]};
-        rest_of(c, all<V>(1.f));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int i = j + k;
-          a[i] = at = fma(c[k], at, at);
-          h[i] = ht = stepped_rest<COMPLEMENT>(
-              c[k], L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4)), ht);
-        }
-      }
-    } else {
+    auto reduce = [&](auto whole) {  // (a token that is not there changes nothing)
 #pragma unroll
       for (int i = 0; i < kTok; ++i) {
-        if (t0 + i < it.n) {
-          const P c = gate_of(a[i]), x = L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4));
+        if (decltype(whole)::value || t0 + i < it.n) {
+          const P f = L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4));
+          const P x = L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4));
+          const P c = gate_of(argument_of(f, bias, log2e));
           at = decayed(c, at);
           ht = stepped<COMPLEMENT>(c, x, ht);
         }
         a[i] = at, h[i] = ht;
       }
-    }
+    };
+    if (it.n == kForward) reduce(std::true_type{});
+    else reduce(std::false_type{});
     const Map<V> own{at, ht};
     Map<V>(*const maps)[32] = all_maps[stage];
     maps[warp][lane] = own;
@@ -955,7 +906,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
     }
     close_tiles();
   };
-  const P one = kept(all<V>(1.f)), log2e = kept(all<V>(kLog2e)), offset = kept(all<V>(-8388736.f));
+  const P log2e = kept(all<V>(kLog2e)), offset = kept(all<V>(-8388736.f));
   if (!TMA) {
     wait_full(&S.full[0], 0);
     fetch(0);
@@ -968,7 +919,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
       wait_tiles<0>();
       compute_sync();
     }
-    const Item it = S.items[stage];
+    const Item& it = S.items[stage];  // (read again where it is used: registers are short)
     if (it.slot < 0) break;
     const char* const xs = tiles + stage * kStage;
     const char* const fs = xs + kTile;
@@ -988,9 +939,8 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
       return out;
     };
     auto dh_of = [&](int i) { return L::unpack(*reinterpret_cast<const uint32_t*>(gs + (t0 + i) * kRowBytes + lane * 4)); };
-    P c[kTok], w[kTok];  // c[i] is t before; w: x, then df_t / G_t
+    P c[kTok], w[kTok];  // c[i] is t before; w: x, then -df_t / G_t
     const P bias = biases[stage][lane];
-    float least = 0.f;
     if (A.f.packed.codes) {
 #pragma unroll
       for (int i = 0; i < kTok; ++i) c[i] = argument_of(value(fs, 1, t0 + i), bias, log2e);
@@ -999,11 +949,6 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
       for (int i = 0; i < kTok; ++i)
         c[i] = argument_of(L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4)), bias, log2e);
     }
-#pragma unroll
-    for (int i = 0; i < kTok; ++i)
-#pragma unroll
-      for (int v = 0; v < V; ++v) least = least_of(least, c[i].v[v]);
-    const bool common = __all_sync(0xffffffffu, it.n == kBackward && least >= kCommon);
     P a = all<V>(1.f), h = all<V>(0.f), r = all<V>(0.f);
     if (A.x.packed.codes) {
 #pragma unroll
@@ -1012,36 +957,19 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
 #pragma unroll
       for (int i = 0; i < kTok; ++i) w[i] = L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4));
     }
-    if (common) {
-#pragma unroll
-      for (int j = 0; j < kTok; j += 4) {
-        P four[4] = {c[j], c[j + 1], c[j + 2], c[j + 3]};
-        rest_of(four, one);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int i = j + k;
-          c[i] = four[k];
-          a = fma(c[i], a, a);
-          h = stepped_rest<COMPLEMENT>(c[i], w[i], h);
-        }
-      }
-#pragma unroll
-      for (int i = kTok - 1; i >= 0; --i) {
-        const P G = add(dh_of(i), r);
-        r = fma(c[i], G, G);
-      }
-    } else {
+    const bool whole = it.n == kBackward;  // (a token that is not there changes nothing)
+    auto reduce = [&](auto all_there) {
 #pragma unroll
       for (int i = 0; i < kTok; ++i) {
-        if (t0 + i >= it.n) continue;  // a token that is not there changes nothing
+        if (!decltype(all_there)::value && t0 + i >= it.n) continue;
         c[i] = gate_of(c[i]);
         a = decayed(c[i], a);
         h = stepped<COMPLEMENT>(c[i], w[i], h);
+        r = fma(a, dh_of(i), r);  // what leaves the first token is the sum of a_0 .. a_t dh_t
       }
-#pragma unroll
-      for (int i = kTok - 1; i >= 0; --i)
-        if (t0 + i < it.n) r = decayed(c[i], add(dh_of(i), r));
-    }
+    };
+    if (whole) reduce(std::true_type{});
+    else reduce(std::false_type{});
     maps[warp][lane] = {a, h};
     const Map<V> own{a, r};
     ends[warp][lane] = own;
@@ -1054,30 +982,25 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
     for (int k = kWarps - 1; k > 0; --k)
       if (k > warp) upto = upto.then(ends[k][lane]);
     if (warp == 0) links.publish_map(upto.then(own));
-    // the states before every token, and df_t / G_t (with the other sign where c is -(1 - a))
+    // the states before every token, and -df_t / G_t
     h = firsts[stage][lane];
 #pragma unroll
     for (int k = 0; k < kWarps - 1; ++k)
       if (k < warp) h = maps[k][lane](h);
-    if (common) {
+    auto walk = [&](auto all_there) {
 #pragma unroll
       for (int i = 0; i < kTok; ++i) {
-        const P x = w[i], rest = fma(c[i], c[i], c[i]), off = sub(h, x);  // -a (1 - a)
-        w[i] = mul(rest, COMPLEMENT ? off : h);
-        h = COMPLEMENT ? fma(c[i], off, h) : fma(c[i], h, add(h, x));
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kTok; ++i) {
-        if (t0 + i >= it.n) continue;
+        if (!decltype(all_there)::value && t0 + i >= it.n) continue;
         const P x = w[i], square = mul(c[i], c[i]);
-        P slope;  // a (1 - a)
+        P slope;  // -a (1 - a)
 #pragma unroll
-        for (int v = 0; v < V; ++v) slope.v[v] = fabsf(c[i].v[v]) - square.v[v];
+        for (int v = 0; v < V; ++v) slope.v[v] = square.v[v] - fabsf(c[i].v[v]);
         w[i] = mul(slope, COMPLEMENT ? sub(h, x) : h);
         h = stepped<COMPLEMENT>(c[i], x, h);
       }
-    }
+    };
+    if (whole) walk(std::true_type{});
+    else walk(std::false_type{});
     compute_sync();  // (maps and ends have been read)
     wait_full(&S.entered[turn & 3], turn / 4 & 1);
     P e = enter[turn & 3][lane];
@@ -1091,13 +1014,23 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
     P sum = all<V>(0.f);
     T* dx = seq::row_ptr<T>(A.dx, it.row0 + static_cast<long long>(t0), 0) + c0;
     T* df = seq::row_ptr<T>(A.df, it.row0 + static_cast<long long>(t0), 0) + c0;
-    auto finish = [&](auto words) {  // all of it with the other sign
-      e = mul(e, all<V>(-1.f));
+    e = mul(e, all<V>(-1.f));
+    auto finish = [&](auto all_there, auto words) {  // with -G and -e
 #pragma unroll
       for (int i = kTok - 1; i >= 0; --i) {
-        const P G = sub(e, dh_of(i)), of = mul(G, w[i]), ox = mul(c[i], G);
-        e = fma(c[i], G, G);
-        const uint32_t wx = L::pack(COMPLEMENT ? ox : mul(G, all<V>(-1.f))), wf = L::pack(of);
+        if (!decltype(all_there)::value && t0 + i >= it.n) continue;
+        const P G = sub(e, dh_of(i)), of = mul(G, w[i]);
+        P ox;
+        if (COMPLEMENT) {  // (1 - a) G
+          P base;
+#pragma unroll
+          for (int v = 0; v < V; ++v) base.v[v] = is_rest(c[i].v[v]) ? 0.f : -G.v[v];
+          ox = fma(c[i], G, base);
+        } else {
+          ox = mul(G, all<V>(-1.f));
+        }
+        e = decayed(c[i], G);
+        const uint32_t wx = L::pack(ox), wf = L::pack(of);
         if (decltype(words)::value) {
           *reinterpret_cast<uint32_t*>(dx + i * A.dx.ts) = wx;
           *reinterpret_cast<uint32_t*>(df + i * A.df.ts) = wf;
@@ -1108,35 +1041,13 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
         sum = add(sum, of);
       }
     };
-    if (common && A.pairs && nc == V) {
-      finish(std::true_type{});
-    } else if (common) {
-      finish(std::false_type{});
-    } else {
-#pragma unroll
-      for (int i = kTok - 1; i >= 0; --i) {
-        if (t0 + i >= it.n) continue;
-        const P G = add(dh_of(i), e), of = mul(G, w[i]);
-        P ox = G;
-        if (COMPLEMENT) {  // (1 - a) G
-          P base, minus;
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            base.v[v] = is_rest(c[i].v[v]) ? 0.f : G.v[v];
-            minus.v[v] = -G.v[v];
-          }
-          ox = fma(c[i], minus, base);
-        }
-        e = decayed(c[i], G);
-        store_word<T>(dx + i * A.dx.ts, L::pack(ox), nc, A.pairs);
-        store_word<T>(df + i * A.df.ts, L::pack(of), nc, A.pairs);
-        sum = add(sum, of);
-      }
-    }
+    if (whole && A.pairs && nc == V) finish(std::true_type{}, std::true_type{});
+    else finish(std::false_type{}, std::false_type{});
     if (A.partial) {
 #pragma unroll
       for (int v = 0; v < V; ++v) sums[warp][lane * V + v] = sum.v[v];
     }
+    const long long sums_at = (static_cast<long long>(it.slot) * C.slabs + it.slab) * CH;
     __syncwarp();
     if (lane == 0) arrive(&S.empty[stage]);
     if (!TMA) {
@@ -1149,7 +1060,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
         float total = 0.f;
 #pragma unroll
         for (int k = 0; k < kWarps; ++k) total += sums[k][threadIdx.x];
-        A.partial[(static_cast<long long>(it.slot) * C.slabs + it.slab) * CH + threadIdx.x] = total;
+        A.partial[sums_at + threadIdx.x] = total;
       }
     }
   }
