@@ -796,6 +796,16 @@ int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_rec
                         void* stream);
 
 /*
+ * How long, in microseconds, the waits within a launch of later calls last at most: a
+ * segment's for the maps of others (2 s), a block's warps' for one another and for rows
+ * on their way (8 s).  Negative: as at the start; 0: maps that are not there at once, or any
+ * wait of a block's warps, counts as run out.  At most an hour.  Where a wait runs out, to_device_status reports
+ * TO_ERR_TIMEOUT, and outputs and states that depend on what did not come are NaN or
+ * have not been written.  Holds for the process.
+ */
+int to_gated_recurrence_wait_limits(int64_t maps_us, int64_t tiles_us);
+
+/*
  * Gradients of the call above with respect to x, f, bias and the entering
  * state, from dh and dstate_out (the gradient of the state left, NULL: zero).
  * x and f are the forward pass's, as they were or (x8, f8 with codes) as it

@@ -189,6 +189,7 @@ _sig("to_linear_attention_step", C.c_int, [C.c_char_p, C.c_char_p, C.c_void_p])
 for _name in ("to_gated_recurrence", "to_gated_recurrence_backward", "to_gated_recurrence_step"):
     _sig(_name, C.c_int, [C.c_char_p, C.c_char_p, C.c_void_p])
 _sig("to_gated_recurrence_saved_rows", C.c_int64, [C.c_char_p])
+_sig("to_gated_recurrence_wait_limits", C.c_int, [C.c_int64, C.c_int64])
 _sig("to_gated_recurrence_workspace_bytes", C.c_size_t, [C.c_char_p])
 _sig("to_gated_recurrence_backward_workspace_bytes", C.c_size_t, [C.c_char_p])
 for _name in ("to_block_norm", "to_block_norm_backward"):

@@ -41,8 +41,13 @@
 // published too.  One of its warps does that while others reduce.  What is folded, and in
 // which order, goes by the segment's number alone: results do not depend on timing.  A
 // published word is a value and its mark in 8 bytes, written and read at once, so
-// no fence and no flag is waited for; the words are cleared before the launch.  Waits
-// are bounded.
+// no fence and no flag is waited for; the words are cleared before the launch.
+//
+// Waits are bounded.  Where a map does not come, what enters is NaN, and so is all that
+// depends on it.  Where a barrier of a CTA's own warps does not, the CTA ends: the warp that
+// has waited sets a flag which ends the other warps' waits, the eight that compute agree on
+// it at their next barrier (which all of them reach), and the one that looks ahead leaves
+// when its tiles have landed.  Both set the device status.
 #include <algorithm>
 
 #include "rows8.cuh"
@@ -61,7 +66,9 @@ constexpr int kRowBytes = 128;                    // of a tile's row of values
 constexpr int kChained = 1024;                    // tokens between published states
 // Tokens of a tile, forwards and backwards (the latter begins where a state is saved).
 constexpr int kForward = 128, kBackward = kSegment;
-constexpr uint32_t kPolls = 1u << 20;             // of a word, about a second
+// How long a segment waits for others' maps, and a CTA's warps for one another and for tiles.
+constexpr long long kMapsWait = 2000000, kTilesWait = 8000000;  // microseconds
+constexpr uint32_t kDrain = 1u << 22;                            // polls for tiles in flight, at a CTA's end
 
 __device__ int g_recurrence_status;
 
@@ -137,7 +144,8 @@ struct Chain {
   const int32_t* cu;
   int nseq, tokens, channels, slabs, slots;  // slabs: tiles of channels; slots: segments that there may be
   unsigned* ticket;                          // null: no sequence is longer than a segment
-  int* gave_up;                              // set once a wait of this call has run out
+  int* gave_up;                              // set once a wait of this call has run out; null where ticket is
+  long long maps_wait, tiles_wait;           // nanoseconds
   int late;                                  // tickets are taken as late as can be (is_late)
   // [slots][slabs * kChannels] words of two f32, zero until they are published
   uint64_t* maps;    // (H, A with its sign bit set)
@@ -316,8 +324,10 @@ __device__ __forceinline__ void expect_bytes(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
-__device__ __forceinline__ void wait_full(uint64_t* bar, uint32_t parity) {
-  if (!mbar_wait_bounded(bar, parity, 4 * kPolls)) atomicExch(&g_recurrence_status, TO_ERR_TIMEOUT);
+__device__ __forceinline__ long long nanoseconds() {
+  long long t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t)::"memory");
+  return t;
 }
 
 template <typename T>
@@ -396,6 +406,11 @@ __device__ __forceinline__ uint64_t published(const uint64_t* p) {
   return w;
 }
 
+__device__ __forceinline__ void give_up(const Chain& C) {
+  if (C.gave_up) atomicExch(C.gave_up, 1);
+  atomicExch(&g_recurrence_status, TO_ERR_TIMEOUT);
+}
+
 // What a CTA has to do with the other segments of its sequence: position p of
 // `count` in the chain's direction, whose slots lie at origin + dir * position.
 template <typename T, int SEG>
@@ -422,9 +437,10 @@ struct Links {
     for (int v = 0; v < V; ++v) publish(C.states + place(p) + v, word_of(h.v[v], 1u));
   }
   // The state that enters position p > 0, by one warp: the state at base() and the maps from
-  // there on, applied in order.
+  // there on, applied in order.  NaN where they do not come.
   __device__ __forceinline__ Vals<V> entering() const {
     const int b = base(), n = p - b;
+    long long since = 0;
     uint64_t w[kChain][V], state[V];
     uint32_t missing = (1u << n) - 1 | 1u << kChain;
     for (uint32_t polls = 0;; ++polls) {
@@ -446,15 +462,14 @@ struct Links {
         if (__all_sync(0xffffffffu, there)) missing &= ~(1u << k);
       }
       if (!missing) break;
-      if (polls % 256 == 255) {  // (once a wait has run out, the others of the call need not)
-        bool out = polls > kPolls;
+      if (polls % 64 == 63 || !C.maps_wait) {  // (once a wait has run out, the others of the call need not)
+        const long long now = nanoseconds();
+        if (!since) since = now;
+        bool out = now - since >= C.maps_wait;
         if (lane == 0 && !out) out = *reinterpret_cast<volatile int*>(C.gave_up) != 0;
         if (__any_sync(0xffffffffu, out)) {
-          if (lane == 0) {
-            atomicExch(C.gave_up, 1);
-            atomicExch(&g_recurrence_status, TO_ERR_TIMEOUT);
-          }
-          break;
+          if (lane == 0) give_up(C);
+          return all<V>(__int_as_float(0x7fc00000));
         }
       }
     }
@@ -560,8 +575,52 @@ struct Stages {
   uint64_t known[2], full[2], empty[2];  // the item, its tile, its tile has been read
   uint64_t entered[4];                   // (a tile's is read after its stage is empty: twice as many)
   Item items[2];
+  int lost;  // a wait for one of the barriers has run out
 };
 
+// Until a barrier's phase is complete; false: it does not come, or another warp has given up.
+// By whole warps, which agree on the answer (no phase follows before its warp has gone on).
+// The two warps that do not compute watch the time.
+__device__ __forceinline__ bool wait_for(const Chain& C, Stages& S, uint64_t* bar, uint32_t parity) {
+  volatile int* const lost = &S.lost;
+  long long since = 0;
+  for (uint32_t n = 1; C.tiles_wait; ++n) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    bool out = *lost != 0;
+    if (n % 16 == 0) {  // (the clock is read seldom: it takes longer than a probe)
+      const long long now = nanoseconds();
+      if (!since) since = now;
+      out = out || now - since >= C.tiles_wait;
+    }
+    if (__any_sync(0xffffffffu, out)) break;
+  }
+  *lost = 1;
+  give_up(C);
+  return false;
+}
+// Those that compute wait for these two, or for tiles that the first one will miss (kMost: at last).
+__device__ __forceinline__ bool wait_here(Stages& S, uint64_t* bar, uint32_t parity) {
+  constexpr uint32_t kMost = 1u << 28;
+  volatile int* const lost = &S.lost;
+  for (uint32_t n = 0; n < kMost; ++n) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *lost)) return false;
+  }
+  *lost = 1;
+  atomicExch(&g_recurrence_status, TO_ERR_TIMEOUT);
+  return false;
+}
+
+// A barrier of the eight warps; whether any of them has lost a wait.
+__device__ __forceinline__ bool any_lost(bool lost) {
+  int any;
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.s32 p, %1, 0;\nbar.red.or.pred q, 1, %2, p;\nselp.s32 %0, 1, 0, q;\n}"
+      : "=r"(any)
+      : "r"(static_cast<int>(lost)), "n"(kThreads)
+      : "memory");
+  return any != 0;
+}
 __device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
 __device__ __forceinline__ void arrive(uint64_t* bar) {
@@ -570,6 +629,7 @@ __device__ __forceinline__ void arrive(uint64_t* bar) {
 
 __device__ __forceinline__ void open_stages(Stages& S) {
   if (threadIdx.x == 0) {
+    S.lost = 0;
     for (int k = 0; k < 2; ++k) {
       mbar_init(&S.known[k], 1);
       mbar_init(&S.full[k], 1);
@@ -590,17 +650,26 @@ __device__ __forceinline__ void look_ahead(const Chain& C, Stages& S, UNUSED&& u
   if (C.ticket) next_ticket(C, ticket, lane);
   for (uint32_t k = 0;; ++k) {
     const int stage = k & 1;
-    if (k >= 2 && C.late) wait_full(&S.empty[stage], (k / 2 - 1) & 1);
+    auto free = [&] { return k < 2 || wait_for(C, S, &S.empty[stage], (k / 2 - 1) & 1); };
+    auto drain = [&] {  // the tiles before this one have landed
+      for (uint32_t j = k < 2 ? 0 : k - 2; j < k; ++j) {
+        if (mbar_wait_bounded(&S.full[j & 1], j / 2 & 1, kDrain)) continue;
+        *const_cast<volatile int*>(&S.lost) = 1;
+        give_up(C);
+      }
+    };
+    if (C.late && !free()) return drain();
     if (k && C.late) next_ticket(C, ticket, lane);
     const Item it = next_item<SEG, BACKWARD>(C, order, ticket, lane, unused);
     if (!C.late) next_ticket(C, ticket, lane);  // (its answer takes as long as a load from L2: one tile ahead)
-    if (k >= 2 && !C.late) wait_full(&S.empty[stage], (k / 2 - 1) & 1);
+    if (!C.late && !free()) return drain();
     if (lane == 0) {
       S.items[stage] = it;
       arrive(&S.known[stage]);
       if (it.slot >= 0 && it.n > 0) load(it, stage);
     }
     if (it.slot >= 0) fill(it, stage);  // (while the tile is on its way)
+    else drain();                       // (nor may the last tiles outlive a CTA that ends early)
     __syncwarp();
     if (lane == 0) arrive(&S.full[stage]);
     if (it.slot < 0) return;
@@ -614,7 +683,7 @@ __device__ __forceinline__ void find_entering(const Chain& C, Stages& S, Vals<La
   const int lane = threadIdx.x & 31;
   for (uint32_t k = 0;; ++k) {
     const int stage = k & 1;
-    wait_full(&S.known[stage], k / 2 & 1);
+    if (!wait_for(C, S, &S.known[stage], k / 2 & 1)) return;
     const Item it = S.items[stage];
     __syncwarp();
     if (lane == 0) arrive(&S.empty[stage]);
@@ -696,20 +765,25 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
     close_tiles();
   };
   const P log2e = kept(all<V>(kLog2e));
-  if (!TMA) {
-    wait_full(&S.full[0], 0);
-    fetch(0);
-  }
+  bool lost = false;
+  auto next_tile = [&](uint32_t t) {  // (not TMA) asks for it
+    lost = lost || !wait_here(S, &S.full[t & 1], t / 2 & 1);
+    if (!lost) fetch(t & 1);
+  };
+  if (!TMA) next_tile(0);
   for (uint32_t turn = 0;; ++turn) {
     const int stage = turn & 1;
     if (TMA) {
-      wait_full(&S.full[stage], turn / 2 & 1);
+      lost = lost || !wait_here(S, &S.full[stage], turn / 2 & 1);
     } else {
       wait_tiles<0>();
-      compute_sync();
+      lost = any_lost(lost);
+    }
+    if (lost || S.items[stage].slot < 0) {  // (where others have a tile, they come to the barrier behind the reduction)
+      any_lost(lost);
+      break;
     }
     const Item it = S.items[stage];
-    if (it.slot < 0) break;
     char* const xs = tiles + stage * 2 * kTile;
     char* const fs = xs + kTile;
     const int ch = it.slab * CH, c0 = ch + lane * V, nc = min(V, C.channels - c0), t0 = warp * kTok;
@@ -741,11 +815,8 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
     maps[warp][lane] = own;
     __syncwarp();
     if (lane == 0 && !C.late) arrive(&S.empty[stage]);
-    compute_sync();
-    if (!TMA) {
-      wait_full(&S.full[stage ^ 1], (turn + 1) / 2 & 1);
-      fetch(stage ^ 1);
-    }
+    if (any_lost(false)) break;
+    if (!TMA) next_tile(turn + 1);
     const Links<T, kForward> links{C, lane, it.slab, it.slot - it.idx, 1, it.idx, it.count};
     Map<V> upto{all<V>(1.f), all<V>(0.f)};  // of the warps before this one
 #pragma unroll
@@ -753,8 +824,9 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
       if (w < warp) upto = upto.then(maps[w][lane]);
     const bool last = warp == kWarps - 1;
     if (last) links.publish_map(upto.then(own));
-    wait_full(&S.entered[turn & 3], turn / 4 & 1);
-    P e = enter[turn & 3][lane];
+    P e = all<V>(__int_as_float(0x7fc00000));
+    if (wait_here(S, &S.entered[turn & 3], turn / 4 & 1)) e = enter[turn & 3][lane];
+    else lost = true;
     if (last && A.state_out && it.idx == it.count - 1) {
       const long long state = state_of(it);
       const P left = upto.then(own)(e);
@@ -907,20 +979,25 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
     close_tiles();
   };
   const P log2e = kept(all<V>(kLog2e)), offset = kept(all<V>(-8388736.f));
-  if (!TMA) {
-    wait_full(&S.full[0], 0);
-    fetch(0);
-  }
+  bool lost = false;
+  auto next_tile = [&](uint32_t t) {  // (not TMA) asks for it
+    lost = lost || !wait_here(S, &S.full[t & 1], t / 2 & 1);
+    if (!lost) fetch(t & 1);
+  };
+  if (!TMA) next_tile(0);
   for (uint32_t turn = 0;; ++turn) {
     const int stage = turn & 1;
     if (TMA) {
-      wait_full(&S.full[stage], turn / 2 & 1);
+      lost = lost || !wait_here(S, &S.full[stage], turn / 2 & 1);
     } else {
       wait_tiles<0>();
-      compute_sync();
+      lost = any_lost(lost);
     }
     const Item& it = S.items[stage];  // (read again where it is used: registers are short)
-    if (it.slot < 0) break;
+    if (lost || it.slot < 0) {        // (where others have a tile, they come to the barrier behind the reduction)
+      any_lost(lost);
+      break;
+    }
     const char* const xs = tiles + stage * kStage;
     const char* const fs = xs + kTile;
     const char* const gs = fs + kTile;
@@ -973,7 +1050,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
     maps[warp][lane] = {a, h};
     const Map<V> own{a, r};
     ends[warp][lane] = own;
-    compute_sync();
+    if (any_lost(false)) break;
     const int p = it.count - 1 - it.idx;
     const Links<T, kBackward> links{C, lane, it.slab, it.slot + p, -1, p, it.count};
     // joined from the last warp on: the first one has the segment's map
@@ -1002,8 +1079,9 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
     if (whole) walk(std::true_type{});
     else walk(std::false_type{});
     compute_sync();  // (maps and ends have been read)
-    wait_full(&S.entered[turn & 3], turn / 4 & 1);
-    P e = enter[turn & 3][lane];
+    P e = all<V>(__int_as_float(0x7fc00000));
+    if (wait_here(S, &S.entered[turn & 3], turn / 4 & 1)) e = enter[turn & 3][lane];
+    else lost = true;
     if (warp == 0 && A.dstate_in && it.idx == 0) {
       const P left = upto.then(own)(e);
 #pragma unroll
@@ -1050,10 +1128,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
     const long long sums_at = (static_cast<long long>(it.slot) * C.slabs + it.slab) * CH;
     __syncwarp();
     if (lane == 0) arrive(&S.empty[stage]);
-    if (!TMA) {
-      wait_full(&S.full[stage ^ 1], (turn + 1) / 2 & 1);
-      fetch(stage ^ 1);
-    }
+    if (!TMA) next_tile(turn + 1);
     if (A.partial) {
       compute_sync();
       if (threadIdx.x < CH) {
@@ -1066,9 +1141,10 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
   }
 }
 
-// dbias[c] = sum over the segments of their sums, in a fixed order, in f64.
+// dbias[c] = sum over the segments of their sums, in a fixed order, in f64; NaN where the call gave up
+// (sums may be missing; calls that wait for no maps have no flag of their own).
 __global__ void __launch_bounds__(1024) bias_sum_kernel(const float* __restrict__ partial, long long pitch, int slots,
-                                                        int channels, float* dbias) {
+                                                        int channels, const int* gave_up, float* dbias) {
   __shared__ double part[32][33];
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, x = blockIdx.x * 32 + lane;
   double v = 0;
@@ -1080,7 +1156,8 @@ __global__ void __launch_bounds__(1024) bias_sum_kernel(const float* __restrict_
   __syncthreads();
   if (row == 0 && x < channels) {
     for (int k = 1; k < 32; ++k) v += part[k][lane];
-    dbias[x] = static_cast<float>(v);
+    const int missing = gave_up ? *gave_up : *const_cast<const volatile int*>(&g_recurrence_status);
+    dbias[x] = missing ? __int_as_float(0x7fc00000) : static_cast<float>(v);
   }
 }
 
@@ -1225,8 +1302,12 @@ int map_of(CUtensorMap* map, const to_rows& r, int seg, const to_gated_recurrenc
                             : map_of(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, r.data, r.token_stride, kRowBytes, seg, d);
 }
 
+std::atomic<long long> g_maps_wait{kMapsWait}, g_tiles_wait{kTilesWait};  // microseconds
+
 Chain chain_of(const to_gated_recurrence_desc& d, const int32_t* cu, const Layout& l, void* workspace, int seg) {
   Chain C{};
+  C.maps_wait = 1000 * g_maps_wait.load(std::memory_order_relaxed);
+  C.tiles_wait = 1000 * g_tiles_wait.load(std::memory_order_relaxed);
   C.cu = cu;
   C.nseq = d.nseq;
   C.tokens = static_cast<int>(d.tokens);
@@ -1285,6 +1366,16 @@ size_t to_gated_recurrence_workspace_bytes(const to_gated_recurrence_desc* desc)
 
 size_t to_gated_recurrence_backward_workspace_bytes(const to_gated_recurrence_desc* desc) {
   return check_desc("to_gated_recurrence_backward_workspace_bytes", desc) ? 0 : layout_of(*desc, true).end;
+}
+
+int to_gated_recurrence_wait_limits(int64_t maps_us, int64_t tiles_us) {
+  constexpr int64_t kMost = 3600ll * 1000000;
+  if (maps_us > kMost || tiles_us > kMost)
+    return set_error(TO_ERR_INVALID_ARGUMENT, "to_gated_recurrence_wait_limits: %lld, %lld us", (long long)maps_us,
+                     (long long)tiles_us);
+  g_maps_wait.store(maps_us < 0 ? kMapsWait : maps_us, std::memory_order_relaxed);
+  g_tiles_wait.store(tiles_us < 0 ? kTilesWait : tiles_us, std::memory_order_relaxed);
+  return ok();
 }
 
 int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_recurrence_args* args, void* stream) {
@@ -1470,7 +1561,7 @@ int to_gated_recurrence_backward(const to_gated_recurrence_desc* desc, const to_
   TO_CUDA_TRY(cudaGetLastError());
   if (a.dbias) {
     bias_sum_kernel<<<(d.channels + 31) / 32, 1024, 0, s>>>(
-        A.partial, static_cast<long long>(A.C.slabs) * channels_of_tile(d), A.C.slots, d.channels, a.dbias);
+        A.partial, static_cast<long long>(A.C.slabs) * channels_of_tile(d), A.C.slots, d.channels, A.C.gave_up, a.dbias);
     TO_CUDA_TRY(cudaGetLastError());
   }
   return ok();
