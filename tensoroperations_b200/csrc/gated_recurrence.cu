@@ -795,15 +795,19 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
     P a[kTok], h[kTok];
     const P bias = biases[stage][lane];
     P at = all<V>(1.f), ht = all<V>(0.f);
-    auto reduce = [&](auto whole) {  // (a token that is not there changes nothing)
+    auto reduce = [&](auto whole) {
 #pragma unroll
       for (int i = 0; i < kTok; ++i) {
-        if (decltype(whole)::value || t0 + i < it.n) {
-          const P f = L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4));
-          const P x = L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4));
-          const P c = gate_of(argument_of(f, bias, log2e));
-          at = decayed(c, at);
-          ht = stepped<COMPLEMENT>(c, x, ht);
+        const P f = L::unpack(*reinterpret_cast<const uint32_t*>(fs + (t0 + i) * kRowBytes + lane * 4));
+        const P x = L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4));
+        const P c = gate_of(argument_of(f, bias, log2e)), as = decayed(c, at), hs = stepped<COMPLEMENT>(c, x, ht);
+        // a token that is not there changes nothing, whatever lies in its place (selected: with a branch
+        // around each, their gates follow one another; 11 prompts 47 us, then 45)
+        const bool there = decltype(whole)::value || t0 + i < it.n;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          at.v[v] = there ? as.v[v] : at.v[v];
+          ht.v[v] = there ? hs.v[v] : ht.v[v];
         }
         a[i] = at, h[i] = ht;
       }
