@@ -60,12 +60,10 @@ namespace {
 using seq::Packed;
 using seq::Rows;
 
-constexpr int kSegment = TO_RECURRENCE_SEGMENT;
+constexpr int kSegment = TO_RECURRENCE_SEGMENT;   // tokens of a tile; a state is saved at the head of each
 constexpr int kWarps = 8, kThreads = 32 * kWarps;  // that compute
 constexpr int kRowBytes = 128;                    // of a tile's row of values
 constexpr int kChained = 1024;                    // tokens between published states
-// Tokens of a tile, forwards and backwards (the latter begins where a state is saved).
-constexpr int kForward = 128, kBackward = kSegment;
 // How long a segment waits for others' maps, and a CTA's warps for one another and for tiles.
 constexpr long long kMapsWait = 2000000, kTilesWait = 8000000;  // microseconds
 constexpr uint32_t kDrain = 1u << 22;                            // polls for tiles in flight, at a CTA's end
@@ -162,13 +160,12 @@ __device__ __forceinline__ int bound_of(const Chain& C, int s) {
 }
 
 // The segment of slot w, by the warp together: sequence s owns the slots
-// cu[s] / SEG + s and up, enough for its segments (an empty sequence has one).
-template <int SEG>
+// cu[s] / kSegment + s and up, enough for its segments (an empty sequence has one).
 __device__ __forceinline__ void find_segment(const Chain& C, int w, int lane, Item& it) {
   int lo = 0, hi = C.nseq;
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32, probe = lo + lane * step;
-    const bool below = probe < hi && bound_of(C, probe) / SEG + probe <= w;
+    const bool below = probe < hi && bound_of(C, probe) / kSegment + probe <= w;
     const int found = __popc(__ballot_sync(0xffffffffu, below));
     lo += found > 1 ? (found - 1) * step : 0;
     hi = min(hi, lo + step);
@@ -176,18 +173,12 @@ __device__ __forceinline__ void find_segment(const Chain& C, int w, int lane, It
   const int first = bound_of(C, lo), end = bound_of(C, lo + 1);
   const int tokens = end > first ? end - first : 0;
   it.seq = lo;
-  it.count = tokens ? (tokens - 1) / SEG + 1 : 1;
-  it.idx = w - (first / SEG + lo);
+  it.count = tokens ? (tokens - 1) / kSegment + 1 : 1;
+  it.idx = w - (first / kSegment + lo);
   if (it.idx < 0 || it.idx >= it.count) it.idx = -1;
-  it.row0 = first + it.idx * SEG;
-  it.n = min(SEG, tokens - it.idx * SEG);
+  it.row0 = first + it.idx * kSegment;
+  it.n = min(kSegment, tokens - it.idx * kSegment);
   it.slot = w;
-}
-
-// The row of `saved` for an item that begins where a state is saved.
-template <int SEG>
-__device__ __forceinline__ int saved_row(const Chain& C, const Item& it) {
-  return (it.row0 - it.idx * SEG) / kSegment + it.seq + it.idx / (kSegment / SEG);
 }
 
 __device__ __forceinline__ void next_ticket(const Chain& C, unsigned& ticket, int lane) {
@@ -203,7 +194,6 @@ __device__ __forceinline__ void next_ticket(const Chain& C, unsigned& ticket, in
 // (Four sequences of 4096 tokens, 4096 channels, forwards: 157 us one after the other, then 136.)
 constexpr int kSides = 8;
 
-template <int SEG>
 struct Order {  // of a whole warp: lane g < kSides holds part g
   int begin = 0, size = 0;
   int round = 0, before = 0;  // before: upto(round)
@@ -214,10 +204,10 @@ struct Order {  // of a whole warp: lane g < kSides holds part g
       int lo = 0, hi = lane ? C.nseq : 1;  // the last sequence that begins at or before it
       while (hi - lo > 1) {
         const int mid = (lo + hi) / 2;
-        if (bound_of(C, mid) / SEG + mid <= target) lo = mid;
+        if (bound_of(C, mid) / kSegment + mid <= target) lo = mid;
         else hi = mid;
       }
-      begin = lane ? min(bound_of(C, lo) / SEG + lo, target) : 0;
+      begin = lane ? min(bound_of(C, lo) / kSegment + lo, target) : 0;
     }
 #pragma unroll
     for (int o = 1; o < kSides; o <<= 1) {  // (no part begins before another one, whatever cu holds)
@@ -243,8 +233,8 @@ struct Order {  // of a whole warp: lane g < kSides holds part g
 
 // The item of a warp's ticket (lane 0's); a slot that no segment has goes to `unused`,
 // and the next ticket is taken.  `ticket`: the one that the item has.
-template <int SEG, bool BACKWARD, typename UNUSED>
-__device__ __forceinline__ Item next_item(const Chain& C, Order<SEG>& order, unsigned& ticket, int lane, UNUSED&& unused) {
+template <bool BACKWARD, typename UNUSED>
+__device__ __forceinline__ Item next_item(const Chain& C, Order& order, unsigned& ticket, int lane, UNUSED&& unused) {
   Item it;
   for (;;) {
     ticket = __shfl_sync(0xffffffffu, ticket, 0);
@@ -254,7 +244,7 @@ __device__ __forceinline__ Item next_item(const Chain& C, Order<SEG>& order, uns
       return it;
     }
     it.slab = static_cast<int>(ticket - at * C.slabs);
-    find_segment<SEG>(C, order.template slot<BACKWARD>(static_cast<int>(at), lane), lane, it);
+    find_segment(C, order.slot<BACKWARD>(static_cast<int>(at), lane), lane, it);
     if (it.idx >= 0) return it;
     unused(it);
     next_ticket(C, ticket, lane);
@@ -413,9 +403,9 @@ __device__ __forceinline__ void give_up(const Chain& C) {
 
 // What a CTA has to do with the other segments of its sequence: position p of
 // `count` in the chain's direction, whose slots lie at origin + dir * position.
-template <typename T, int SEG>
+template <typename T>
 struct Links {
-  static constexpr int kChain = kChained / SEG;
+  static constexpr int kChain = kChained / kSegment;
   static constexpr int V = Lane<T>::kVec, CH = Lane<T>::kChannels;
   const Chain& C;
   int lane, slab, origin, dir, p, count;
@@ -527,7 +517,7 @@ template <typename T>
 __device__ __forceinline__ void keep_tile(const char* tile, const Packed& out, int access, const Item& it, int ch,
                                           int channels) {
   constexpr int kParts = Lane<T>::kChannels / 16;
-  for (int i = threadIdx.x; i < kForward * kParts; i += kThreads) {  // (whole warps)
+  for (int i = threadIdx.x; i < kSegment * kParts; i += kThreads) {  // (whole warps)
     const int row = i / kParts, part = i % kParts, c = ch + part * 16;
     float x[16];
     seq::load_vec<T, 16>(reinterpret_cast<const T*>(tile + row * kRowBytes) + part * 16, x);
@@ -642,10 +632,10 @@ __device__ __forceinline__ void open_stages(Stages& S) {
 }
 
 // The warp that looks ahead.  load(item, stage): one lane; fill(item, stage): the whole warp.
-template <int SEG, bool BACKWARD, typename UNUSED, typename FILL, typename LOAD>
+template <bool BACKWARD, typename UNUSED, typename FILL, typename LOAD>
 __device__ __forceinline__ void look_ahead(const Chain& C, Stages& S, UNUSED&& unused, FILL&& fill, LOAD&& load) {
   const int lane = threadIdx.x & 31;
-  Order<SEG> order(C, lane);
+  Order order(C, lane);
   unsigned ticket = blockIdx.x;
   if (C.ticket) next_ticket(C, ticket, lane);
   for (uint32_t k = 0;; ++k) {
@@ -660,7 +650,7 @@ __device__ __forceinline__ void look_ahead(const Chain& C, Stages& S, UNUSED&& u
     };
     if (C.late && !free()) return drain();
     if (k && C.late) next_ticket(C, ticket, lane);
-    const Item it = next_item<SEG, BACKWARD>(C, order, ticket, lane, unused);
+    const Item it = next_item<BACKWARD>(C, order, ticket, lane, unused);
     if (!C.late) next_ticket(C, ticket, lane);  // (its answer takes as long as a load from L2: one tile ahead)
     if (!C.late && !free()) return drain();
     if (lane == 0) {
@@ -677,7 +667,7 @@ __device__ __forceinline__ void look_ahead(const Chain& C, Stages& S, UNUSED&& u
 }
 
 // The warp that finds what enters.  first(item): what enters a sequence; done(item, state).
-template <typename T, int SEG, bool BACKWARD, typename FIRST, typename DONE>
+template <typename T, bool BACKWARD, typename FIRST, typename DONE>
 __device__ __forceinline__ void find_entering(const Chain& C, Stages& S, Vals<Lane<T>::kVec> (&enter)[4][32], FIRST&& first,
                                               DONE&& done) {
   const int lane = threadIdx.x & 31;
@@ -689,7 +679,7 @@ __device__ __forceinline__ void find_entering(const Chain& C, Stages& S, Vals<La
     if (lane == 0) arrive(&S.empty[stage]);
     if (it.slot < 0) return;
     const int p = BACKWARD ? it.count - 1 - it.idx : it.idx;
-    const Links<T, SEG> links{C, lane, it.slab, it.slot - (BACKWARD ? -p : p), BACKWARD ? -1 : 1, p, it.count};
+    const Links<T> links{C, lane, it.slab, it.slot - (BACKWARD ? -p : p), BACKWARD ? -1 : 1, p, it.count};
     const Vals<Lane<T>::kVec> e = p > 0 ? links.entering() : first(it);
     links.publish_state(e);
     enter[k & 3][lane] = e;
@@ -703,7 +693,7 @@ template <typename T, bool KEEP, bool COMPLEMENT, bool TMA>
 __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_constant__ ForwardArgs A) {
   using L = Lane<T>;
   using P = typename L::P;
-  constexpr int V = L::kVec, CH = L::kChannels, kTok = kForward / kWarps, kTile = kForward * kRowBytes;
+  constexpr int V = L::kVec, CH = L::kChannels, kTok = kSegment / kWarps, kTile = kSegment * kRowBytes;
   extern __shared__ __align__(128) char tiles[];  // two stages of x and f
   __shared__ Map<V> all_maps[2][kWarps][32];
   __shared__ P enter[4][32], biases[2][32];
@@ -712,7 +702,7 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
   const Chain& C = A.C;
   open_stages(S);
   if (warp == kAhead) {
-    look_ahead<kForward, false>(
+    look_ahead<false>(
         C, S, [](const Item&) {},
         [&](const Item& it, int stage) {
           P b = all<V>(0.f);
@@ -736,7 +726,7 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
     return slot >= 0 && slot < A.num_slots ? slot * C.channels + it.slab * CH + lane * V : -1;
   };
   if (warp == kEntering) {
-    find_entering<T, kForward, false>(
+    find_entering<T, false>(
         C, S, enter,
         [&](const Item& it) {
           P e = all<V>(0.f);
@@ -747,11 +737,11 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
           return e;
         },
         [&](const Item& it, const P& e) {
-          if (!A.saved || it.idx % (kSegment / kForward)) return;
+          if (!A.saved) return;
           const int c = it.slab * CH + lane * V;
 #pragma unroll
           for (int v = 0; v < V; ++v)
-            if (c + v < C.channels) A.saved[static_cast<long long>(saved_row<kForward>(C, it)) * C.channels + c + v] = e.v[v];
+            if (c + v < C.channels) A.saved[static_cast<long long>(it.slot) * C.channels + c + v] = e.v[v];
         });
     return;
   }
@@ -812,7 +802,7 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
         a[i] = at, h[i] = ht;
       }
     };
-    if (it.n == kForward) reduce(std::true_type{});
+    if (it.n == kSegment) reduce(std::true_type{});
     else reduce(std::false_type{});
     const Map<V> own{at, ht};
     Map<V>(*const maps)[32] = all_maps[stage];
@@ -821,7 +811,7 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
     if (lane == 0 && !C.late) arrive(&S.empty[stage]);
     if (any_lost(false)) break;
     if (!TMA) next_tile(turn + 1);
-    const Links<T, kForward> links{C, lane, it.slab, it.slot - it.idx, 1, it.idx, it.count};
+    const Links<T> links{C, lane, it.slab, it.slot - it.idx, 1, it.idx, it.count};
     Map<V> upto{all<V>(1.f), all<V>(0.f)};  // of the warps before this one
 #pragma unroll
     for (int w = 0; w < kWarps - 1; ++w)
@@ -840,7 +830,7 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
     }
     e = upto(e);
     T* row = seq::row_ptr<T>(A.h, it.row0 + static_cast<long long>(t0), 0) + c0;
-    if (A.pairs && nc == V && it.n == kForward) {
+    if (A.pairs && nc == V && it.n == kSegment) {
 #pragma unroll
       for (int i = 0; i < kTok; ++i, row += A.h.ts) *reinterpret_cast<uint32_t*>(row) = L::pack(fma(a[i], e, h[i]));
     } else {
@@ -872,29 +862,27 @@ struct BackwardArgs {
 // leaves them when nothing enters.  h runs forwards again from the saved state (so
 // the map (A, H) of each warp is needed too).  x and dh stay in shared memory until the
 // last walk.
-template <typename T>
-struct BackwardTiles {  // of a stage: x and f as they are (or their codes at the same places), dh
-  static constexpr int kTile = kBackward * kRowBytes, kStage = 3 * kTile;
-};
+// A stage: x and f as they are (or their codes at the same places), dh.
+constexpr int kBackwardStage = 3 * kSegment * kRowBytes;
 
 template <typename T, bool COMPLEMENT, bool TMA>
 __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_constant__ BackwardArgs A) {
   using L = Lane<T>;
   using P = typename L::P;
   constexpr int V = L::kVec, CH = L::kChannels, kGroups = CH / seq::kGroup8;
-  constexpr int kTok = kBackward / kWarps, kTile = BackwardTiles<T>::kTile, kStage = BackwardTiles<T>::kStage;
+  constexpr int kTok = kSegment / kWarps, kTile = kSegment * kRowBytes, kStage = kBackwardStage;
   extern __shared__ __align__(128) char tiles[];  // two stages
   // maps: of h, ends: of the gradients' chain (they share A)
   __shared__ Map<V> maps[kWarps][32], ends[kWarps][32];
   __shared__ P enter[4][32], biases[2][32], firsts[2][32];
   __shared__ float sums[kWarps][CH];
-  __shared__ float scales[2][2][kBackward][kGroups];
+  __shared__ float scales[2][2][kSegment][kGroups];
   __shared__ Stages S;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Chain& C = A.C;
   open_stages(S);
   if (warp == kAhead) {
-    look_ahead<kBackward, true>(
+    look_ahead<true>(
         C, S,
         [&](const Item& it) {  // its sums count too
           if (A.partial)
@@ -910,13 +898,13 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
             const int c = ch + lane * V + v;
             if (c >= C.channels) continue;
             if (A.bias) b.v[v] = __ldg(A.bias + c);
-            first.v[v] = __ldg(A.saved + static_cast<long long>(saved_row<kBackward>(C, it)) * C.channels + c);
+            first.v[v] = __ldg(A.saved + static_cast<long long>(it.slot) * C.channels + c);
           }
           biases[stage][lane] = b;
           firsts[stage][lane] = first;
           // scales: all of them asked for before the first is waited for (rows and groups that are
           // not there: others in their place)
-          constexpr int kRows = kBackward / 32;
+          constexpr int kRows = kSegment / 32;
           uint8_t bytes[2][kRows][kGroups];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
@@ -941,7 +929,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
         [&](const Item& it, int stage) {
           if (!TMA) return;
           char* to = tiles + stage * kStage;
-          const int ch = it.slab * CH, x = A.x.packed.codes ? kBackward * CH : kTile, f = A.f.packed.codes ? kBackward * CH : kTile;
+          const int ch = it.slab * CH, x = A.x.packed.codes ? kSegment * CH : kTile, f = A.f.packed.codes ? kSegment * CH : kTile;
           expect_bytes(&S.full[stage], x + f + kTile);
           tma_tile(to, &A.x_map, ch, it.row0, &S.full[stage]);
           tma_tile(to + kTile, &A.f_map, ch, it.row0, &S.full[stage]);
@@ -950,7 +938,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
     return;
   }
   if (warp == kEntering) {
-    find_entering<T, kBackward, true>(
+    find_entering<T, true>(
         C, S, enter,
         [&](const Item& it) {
           P e = all<V>(0.f);
@@ -1038,7 +1026,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
 #pragma unroll
       for (int i = 0; i < kTok; ++i) w[i] = L::unpack(*reinterpret_cast<const uint32_t*>(xs + (t0 + i) * kRowBytes + lane * 4));
     }
-    const bool whole = it.n == kBackward;  // (a token that is not there changes nothing)
+    const bool whole = it.n == kSegment;  // (a token that is not there changes nothing)
     auto reduce = [&](auto all_there) {
 #pragma unroll
       for (int i = 0; i < kTok; ++i) {
@@ -1056,7 +1044,7 @@ __global__ void __launch_bounds__(kLaunched, 2) backward_kernel(const __grid_con
     ends[warp][lane] = own;
     if (any_lost(false)) break;
     const int p = it.count - 1 - it.idx;
-    const Links<T, kBackward> links{C, lane, it.slab, it.slot + p, -1, p, it.count};
+    const Links<T> links{C, lane, it.slab, it.slot + p, -1, p, it.count};
     // joined from the last warp on: the first one has the segment's map
     Map<V> upto{all<V>(1.f), all<V>(0.f)};
 #pragma unroll
@@ -1232,18 +1220,17 @@ int channels_of_tile(const to_gated_recurrence_desc& d) { return kRowBytes / seq
 int slabs_of(const to_gated_recurrence_desc& d) {
   return (d.channels + channels_of_tile(d) - 1) / channels_of_tile(d);
 }
-// Segments of `tokens` that there may be, whatever the lengths are.
-int slots_of(const to_gated_recurrence_desc& d, int tokens) { return static_cast<int>(d.tokens / tokens) + d.nseq; }
-bool chained(const to_gated_recurrence_desc& d, int tokens) { return d.tokens > tokens && d.nseq > 0; }
+// Segments that there may be, whatever the lengths are.
+int slots_of(const to_gated_recurrence_desc& d) { return static_cast<int>(d.tokens / kSegment) + d.nseq; }
+bool chained(const to_gated_recurrence_desc& d) { return d.tokens > kSegment && d.nseq > 0; }
 
 struct Layout {  // of the workspace: the counter, the maps and the states (cleared), the partial sums
   size_t maps, states, partial, end;
 };
 Layout layout_of(const to_gated_recurrence_desc& d, bool backward) {
-  const int seg = backward ? kBackward : kForward;
-  const size_t values = size_t(slots_of(d, seg)) * slabs_of(d) * channels_of_tile(d);
+  const size_t values = size_t(slots_of(d)) * slabs_of(d) * channels_of_tile(d);
   Layout l{};
-  if (chained(d, seg)) {
+  if (chained(d)) {
     l.maps = kAlign;
     l.states = l.maps + padded(values * sizeof(uint64_t));
     l.partial = l.states + padded(values * sizeof(uint64_t));
@@ -1284,13 +1271,13 @@ int access_of(const to_rows8& r, int64_t tokens) {
 bool tma_takes(const to_rows& r, const to_gated_recurrence_desc& d) {
   return d.tokens >= kSegment && r.token_stride < (1ll << 37) && seq::rows_aligned(&r, d.tokens, 1, d.dtype, 16);
 }
-int map_of(CUtensorMap* map, CUtensorMapDataType type, int bytes, const void* data, long long pitch, int row, int seg,
+int map_of(CUtensorMap* map, CUtensorMapDataType type, int bytes, const void* data, long long pitch, int row,
            const to_gated_recurrence_desc& d) {
   int st = ok();
   const EncodeTiled encode = tensor_map_encoder(&st);
   if (!encode) return st;
   const cuuint64_t dims[2] = {cuuint64_t(d.channels), cuuint64_t(d.tokens)}, strides[1] = {cuuint64_t(pitch * bytes)};
-  const cuuint32_t box[2] = {cuuint32_t(row / bytes), cuuint32_t(seg)}, steps[2] = {1, 1};
+  const cuuint32_t box[2] = {cuuint32_t(row / bytes), cuuint32_t(kSegment)}, steps[2] = {1, 1};
   const CUresult e = encode(map, type, 2, const_cast<void*>(data), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return e == CUDA_SUCCESS ? ok() : set_error(TO_ERR_CUDA, "cuTensorMapEncodeTiled: %d", static_cast<int>(e));
@@ -1298,17 +1285,17 @@ int map_of(CUtensorMap* map, CUtensorMapDataType type, int bytes, const void* da
 bool tma_takes(const to_rows8& r, const to_gated_recurrence_desc& d) {
   return d.tokens >= kSegment && r.code_stride < (1ll << 37) && aligned(r.codes, 16) && r.code_stride % 16 == 0;
 }
-int map_of(CUtensorMap* map, const to_rows8& r, int seg, const to_gated_recurrence_desc& d) {
-  return map_of(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, r.codes, r.code_stride, channels_of_tile(d), seg, d);
+int map_of(CUtensorMap* map, const to_rows8& r, const to_gated_recurrence_desc& d) {
+  return map_of(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, r.codes, r.code_stride, channels_of_tile(d), d);
 }
-int map_of(CUtensorMap* map, const to_rows& r, int seg, const to_gated_recurrence_desc& d) {
-  return d.dtype == TO_BF16 ? map_of(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, r.data, r.token_stride, kRowBytes, seg, d)
-                            : map_of(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, r.data, r.token_stride, kRowBytes, seg, d);
+int map_of(CUtensorMap* map, const to_rows& r, const to_gated_recurrence_desc& d) {
+  return d.dtype == TO_BF16 ? map_of(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, r.data, r.token_stride, kRowBytes, d)
+                            : map_of(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, r.data, r.token_stride, kRowBytes, d);
 }
 
 std::atomic<long long> g_maps_wait{kMapsWait}, g_tiles_wait{kTilesWait};  // microseconds
 
-Chain chain_of(const to_gated_recurrence_desc& d, const int32_t* cu, const Layout& l, void* workspace, int seg) {
+Chain chain_of(const to_gated_recurrence_desc& d, const int32_t* cu, const Layout& l, void* workspace) {
   Chain C{};
   C.maps_wait = 1000 * g_maps_wait.load(std::memory_order_relaxed);
   C.tiles_wait = 1000 * g_tiles_wait.load(std::memory_order_relaxed);
@@ -1317,8 +1304,8 @@ Chain chain_of(const to_gated_recurrence_desc& d, const int32_t* cu, const Layou
   C.tokens = static_cast<int>(d.tokens);
   C.channels = d.channels;
   C.slabs = slabs_of(d);
-  C.slots = slots_of(d, seg);
-  if (chained(d, seg)) {
+  C.slots = slots_of(d);
+  if (chained(d)) {
     char* w = static_cast<char*>(workspace);
     C.ticket = reinterpret_cast<unsigned*>(w);
     C.gave_up = reinterpret_cast<int*>(w + sizeof(unsigned));
@@ -1361,7 +1348,7 @@ using namespace to_b200;
 extern "C" {
 
 int64_t to_gated_recurrence_saved_rows(const to_gated_recurrence_desc* desc) {
-  return check_desc("to_gated_recurrence_saved_rows", desc) ? 0 : slots_of(*desc, kSegment);
+  return check_desc("to_gated_recurrence_saved_rows", desc) ? 0 : slots_of(*desc);
 }
 
 size_t to_gated_recurrence_workspace_bytes(const to_gated_recurrence_desc* desc) {
@@ -1415,10 +1402,10 @@ int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_rec
   if (a.state_in != a.state_out && seq::arrays_meet(a.state_in, a.state_out, states))
     return set_error(TO_ERR_INVALID_ARGUMENT, "%s: state_in and state_out share memory in part", who);
   for (const float* p : {a.state_in, static_cast<const float*>(a.state_out)})
-    if (p && a.saved && p < a.saved + size_t(slots_of(d, kSegment)) * d.channels && a.saved < p + states / sizeof(float))
+    if (p && a.saved && p < a.saved + size_t(slots_of(d)) * d.channels && a.saved < p + states / sizeof(float))
       return seq::refuse_overlap(who, "saved", p == a.state_in ? "state_in" : "state_out");
   ForwardArgs A{};
-  A.C = chain_of(d, a.cu_seqlens, l, a.workspace, kForward);
+  A.C = chain_of(d, a.cu_seqlens, l, a.workspace);
   A.x = seq::rows_of(a.x);
   A.f = seq::rows_of(a.f);
   A.h = seq::rows_of(a.h);
@@ -1443,7 +1430,7 @@ int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_rec
   if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.partial, s));
   const unsigned grid = grid_of(A.C, sms, 2);
   A.C.late = is_late(A.C, grid);
-  constexpr size_t kShared = 4 * size_t(kForward) * kRowBytes;
+  constexpr size_t kShared = 4 * size_t(kSegment) * kRowBytes;
   static std::atomic<uint64_t> done[16];
   auto launch = [&](auto t, auto keep, auto complement, auto tma) {
     using K = decltype(keep);
@@ -1455,7 +1442,7 @@ int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_rec
     return ok();
   };
   const bool keep = a.keep_x.codes || a.keep_f.codes, tma = tma_takes(a.x, d) && tma_takes(a.f, d);
-  if (tma && ((st = map_of(&A.x_map, a.x, kForward, d)) || (st = map_of(&A.f_map, a.f, kForward, d)))) return st;
+  if (tma && ((st = map_of(&A.x_map, a.x, d)) || (st = map_of(&A.f_map, a.f, d)))) return st;
   constexpr std::true_type yes{};
   constexpr std::false_type no{};
   auto with = [&](auto t, auto m) {
@@ -1510,15 +1497,15 @@ int to_gated_recurrence_backward(const to_gated_recurrence_desc* desc, const to_
   const size_t states = size_t(d.nseq) * d.channels;
   if (seq::arrays_meet(a.dstate_in, a.dstate_out, states * sizeof(float)))
     return seq::refuse_overlap(who, "dstate_in", "dstate_out");
-  if (a.dstate_in && a.dstate_in < a.saved + size_t(slots_of(d, kSegment)) * d.channels && a.saved < a.dstate_in + states)
+  if (a.dstate_in && a.dstate_in < a.saved + size_t(slots_of(d)) * d.channels && a.saved < a.dstate_in + states)
     return seq::refuse_overlap(who, "dstate_in", "saved");
   for (const float* p : {static_cast<const float*>(a.dstate_in), a.dstate_out})
     if (a.dbias && p && a.dbias < p + states && p < a.dbias + d.channels)
       return seq::refuse_overlap(who, "dbias", p == a.dstate_in ? "dstate_in" : "dstate_out");
-  if (a.dbias && a.dbias < a.saved + size_t(slots_of(d, kSegment)) * d.channels && a.saved < a.dbias + d.channels)
+  if (a.dbias && a.dbias < a.saved + size_t(slots_of(d)) * d.channels && a.saved < a.dbias + d.channels)
     return seq::refuse_overlap(who, "dbias", "saved");
   BackwardArgs A{};
-  A.C = chain_of(d, a.cu_seqlens, l, a.workspace, kBackward);
+  A.C = chain_of(d, a.cu_seqlens, l, a.workspace);
   A.x = {seq::rows_of(a.x), seq::packed_of(a.x8), a.x8.codes ? access_of(a.x8, d.tokens) : access_of(a.x, d.tokens, d.dtype)};
   A.f = {seq::rows_of(a.f), seq::packed_of(a.f8), a.f8.codes ? access_of(a.f8, d.tokens) : access_of(a.f, d.tokens, d.dtype)};
   A.dh = seq::rows_of(a.dh);
@@ -1537,7 +1524,7 @@ int to_gated_recurrence_backward(const to_gated_recurrence_desc* desc, const to_
   if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.partial, s));
   const unsigned grid = grid_of(A.C, sms, 2);
   A.C.late = is_late(A.C, grid);
-  constexpr size_t kShared = 2 * size_t(BackwardTiles<float>::kStage);
+  constexpr size_t kShared = 2 * size_t(kBackwardStage);
   static std::atomic<uint64_t> done[8];
   auto launch = [&](auto t, auto complement, auto tma) {
     auto* kernel = backward_kernel<decltype(t), decltype(complement)::value, decltype(tma)::value>;
@@ -1549,9 +1536,9 @@ int to_gated_recurrence_backward(const to_gated_recurrence_desc* desc, const to_
   const bool tma = tma_takes(a.dh, d) && (a.x8.codes ? tma_takes(a.x8, d) : tma_takes(a.x, d)) &&
                    (a.f8.codes ? tma_takes(a.f8, d) : tma_takes(a.f, d));
   if (tma) {
-    st = a.x8.codes ? map_of(&A.x_map, a.x8, kBackward, d) : map_of(&A.x_map, a.x, kBackward, d);
-    if (!st) st = a.f8.codes ? map_of(&A.f_map, a.f8, kBackward, d) : map_of(&A.f_map, a.f, kBackward, d);
-    if (!st) st = map_of(&A.dh_map, a.dh, kBackward, d);
+    st = a.x8.codes ? map_of(&A.x_map, a.x8, d) : map_of(&A.x_map, a.x, d);
+    if (!st) st = a.f8.codes ? map_of(&A.f_map, a.f8, d) : map_of(&A.f_map, a.f, d);
+    if (!st) st = map_of(&A.dh_map, a.dh, d);
     if (st) return st;
   }
   constexpr std::true_type yes{};
