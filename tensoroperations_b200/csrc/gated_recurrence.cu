@@ -144,7 +144,6 @@ struct Chain {
   unsigned* ticket;                          // null: no sequence is longer than a segment
   int* gave_up;                              // set once a wait of this call has run out; null where ticket is
   long long maps_wait, tiles_wait;           // nanoseconds
-  int late;                                  // tickets are taken as late as can be (is_late)
   // [slots][slabs * kChannels] words of two f32, zero until they are published
   uint64_t* maps;    // (H, A with its sign bit set)
   uint64_t* states;  // (the entering state, 1)
@@ -632,6 +631,9 @@ __device__ __forceinline__ void open_stages(Stages& S) {
 }
 
 // The warp that looks ahead.  load(item, stage): one lane; fill(item, stage): the whole warp.
+// A ticket is taken when its stage is free: the segments of a chain are in work at the same time,
+// and a tile that is held for later keeps those behind it waiting (a tile ahead, 49152 tokens x
+// 4096 channels took 328 us for 266, 4 x 4096 with 8-bit copies 134 for 129, without them 86 for 90).
 template <bool BACKWARD, typename UNUSED, typename FILL, typename LOAD>
 __device__ __forceinline__ void look_ahead(const Chain& C, Stages& S, UNUSED&& unused, FILL&& fill, LOAD&& load) {
   const int lane = threadIdx.x & 31;
@@ -648,11 +650,9 @@ __device__ __forceinline__ void look_ahead(const Chain& C, Stages& S, UNUSED&& u
         give_up(C);
       }
     };
-    if (C.late && !free()) return drain();
-    if (k && C.late) next_ticket(C, ticket, lane);
+    if (!free()) return drain();
+    if (k) next_ticket(C, ticket, lane);
     const Item it = next_item<BACKWARD>(C, order, ticket, lane, unused);
-    if (!C.late) next_ticket(C, ticket, lane);  // (its answer takes as long as a load from L2: one tile ahead)
-    if (!C.late && !free()) return drain();
     if (lane == 0) {
       S.items[stage] = it;
       arrive(&S.known[stage]);
@@ -808,7 +808,6 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
     Map<V>(*const maps)[32] = all_maps[stage];
     maps[warp][lane] = own;
     __syncwarp();
-    if (lane == 0 && !C.late) arrive(&S.empty[stage]);
     if (any_lost(false)) break;
     if (!TMA) next_tile(turn + 1);
     const Links<T> links{C, lane, it.slab, it.slot - it.idx, 1, it.idx, it.count};
@@ -838,7 +837,8 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
       for (int i = 0; i < kTok; ++i)
         if (t0 + i < it.n) store_word<T>(row + i * A.h.ts, L::pack(fma(a[i], e, h[i])), nc, A.pairs);
     }
-    if (lane == 0 && C.late) arrive(&S.empty[stage]);
+    __syncwarp();
+    if (lane == 0) arrive(&S.empty[stage]);
   }
 }
 
@@ -1320,14 +1320,6 @@ unsigned grid_of(const Chain& C, int sms, int per_sm) {
   return static_cast<unsigned>(std::min(static_cast<long long>(C.slots) * C.slabs, static_cast<long long>(sms) * per_sm));
 }
 
-// Whether tickets are taken as late as can be: where few chains of segments (one a tile of channels
-// and a sequence side by side) keep all CTAs busy, the segments of one are in work at the same time,
-// and every tile that a CTA holds for later keeps those behind it waiting (49152 tokens x 4096
-// channels 261 us, and 318 with tickets a tile ahead; 11 prompts 48 and 44).
-bool is_late(const Chain& C, unsigned grid) {
-  return C.ticket && 2ll * C.slabs * std::min(C.nseq, kSides) < grid;
-}
-
 }  // namespace
 
 int recurrence_device_status(int reset, int* value) {
@@ -1429,7 +1421,6 @@ int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_rec
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.partial, s));
   const unsigned grid = grid_of(A.C, sms, 2);
-  A.C.late = is_late(A.C, grid);
   constexpr size_t kShared = 4 * size_t(kSegment) * kRowBytes;
   static std::atomic<uint64_t> done[16];
   auto launch = [&](auto t, auto keep, auto complement, auto tma) {
@@ -1523,7 +1514,6 @@ int to_gated_recurrence_backward(const to_gated_recurrence_desc* desc, const to_
   if (sms <= 0) return -sms;
   if (A.C.ticket) TO_CUDA_TRY(cudaMemsetAsync(a.workspace, 0, l.partial, s));
   const unsigned grid = grid_of(A.C, sms, 2);
-  A.C.late = is_late(A.C, grid);
   constexpr size_t kShared = 2 * size_t(kBackwardStage);
   static std::atomic<uint64_t> done[8];
   auto launch = [&](auto t, auto complement, auto tma) {
