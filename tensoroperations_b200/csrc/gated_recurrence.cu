@@ -820,6 +820,7 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
     P e = all<V>(__int_as_float(0x7fc00000));
     if (wait_here(S, &S.entered[turn & 3], turn / 4 & 1)) e = enter[turn & 3][lane];
     else lost = true;
+    if (lane == 0) arrive(&S.empty[stage]);  // (the tile was read before the barrier)
     if (last && A.state_out && it.idx == it.count - 1) {
       const long long state = state_of(it);
       const P left = upto.then(own)(e);
@@ -837,8 +838,6 @@ __global__ void __launch_bounds__(kLaunched, 2) forward_kernel(const __grid_cons
       for (int i = 0; i < kTok; ++i)
         if (t0 + i < it.n) store_word<T>(row + i * A.h.ts, L::pack(fma(a[i], e, h[i])), nc, A.pairs);
     }
-    __syncwarp();
-    if (lane == 0) arrive(&S.empty[stage]);
   }
 }
 
