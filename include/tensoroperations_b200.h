@@ -748,8 +748,9 @@ int to_rows8_unpack(int32_t dtype, int32_t width, int64_t tokens, const to_rows8
  * x, f, h: rows [tokens][channels] (one head: head_stride is not used).  bias:
  * device f32 [channels], NULL for 0.  h_{-1} is the entering state (state_in,
  * zero when NULL); h_{L-1}, before its rounding, is written to state_out (when
- * not NULL).  a and 1 - a keep f32 accuracy relative to themselves; the
- * recurrence is f32 throughout, h takes one rounding.
+ * not NULL).  a and 1 - a keep f32 accuracy relative to themselves, whatever the
+ * gates of other tokens and channels are; the recurrence is f32 throughout (with
+ * complement, h - x has to be finite there), h takes one rounding.
  *
  * Sequences are packed as in to_linear_attention, and so are the rules for
  * cu_seqlens, lengths 0 and 1, rows of no sequence, slots (states are f32

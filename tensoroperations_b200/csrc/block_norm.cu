@@ -17,9 +17,11 @@
 // gradients' three first ones are taken together.
 //
 // Measured on B200: 16384 x 4096 bf16 with a silu gate and an f32 stream in 164 us, 5.7 TB/s
-// (0.88 of the copy rate); gradients of 8192 x 4096 bf16 in 146 us, 3.7 TB/s, from 8 bits 157 us,
-// 2.8 TB/s: two rows an SM, whose loads, sums and about 80 instructions a value follow one
-// another; 6137 x 1003 f32 without a gate 67 us.
+// (0.88 of the copy rate), 8192 x 4096 f32 119 us (0.87), bf16 with 8-bit copies 109 us, 4.0
+// TB/s.  Gradients of 8192 x 4096 bf16 in 145 us, 3.7 TB/s, from 8 bits 157 us, 2.8 TB/s: two
+// rows an SM, whose loads, sums and 85 instructions a value follow one another; f32 199 us, 5.4
+// TB/s.  6137 x 1003 f32 without a gate 242 us (registers of the single-value form are spilled),
+// gradients 65 us.
 #include <algorithm>
 #include <cmath>
 

@@ -15,14 +15,17 @@
 // leave it memory bound in principle.  Gradients keep the gates and df_t / G_t instead,
 // and walk back once what enters from behind is known.
 //
-// Measured on B200 (bf16): 49152 tokens x 4096 channels, one sequence, in 261 us, 4.6
-// TB/s (0.71 of the copy rate): its 64 chains of segments keep 296 CTAs busy, so four or
-// five segments of a chain are in work at once and wait for one another's maps (without
-// those waits 200 us).  4 x 4096 tokens x 4096 with 8-bit copies 126 us, 4.3 TB/s, 44
-// instructions a value, near what 20 warps an SM issue; gradients of these 167 us, 4.0 TB/s,
-// from 8 bits 212 us, 2.6 TB/s: they wait for tiles and for the slowest of eight warps.  Eight
-// more warps that only reduce, a tile ahead, and eight that walk (no maps in registers) needed
-// half as many instructions again: 277 us for the first figure.
+// Measured on B200 (behind an L2 flush; gates do not change it): 49152 tokens x 4096 channels
+// bf16, one sequence, in 262 us, 4.6 TB/s (0.71 of the copy rate): its 64 chains of segments
+// keep 296 CTAs busy, so four or five segments of a chain are in work at once and wait for one
+// another's maps (a form that took 261 us took 200 without those waits; eight more warps that
+// only reduce, a tile ahead, and eight that walk needed half as many instructions again, and
+// 277).  24576 x 4096 f32 215 us, 5.6 TB/s, its gradients 326 us, 6.2 TB/s.  4 x 4096 tokens x
+// 4096 bf16 with 8-bit copies 128 us, 4.2 TB/s, 43 instructions a value, near what 20 warps an
+// SM issue; gradients of these 174 us, 3.9 TB/s, from 8 bits 211 us, 2.6 TB/s, 57 instructions:
+// they wait for tiles and for the slowest of eight warps.  Rows that TMA does not take are
+// copied by the warps that compute: 16384 x 4091 bf16 279 us, gradients 514 us, with 8-bit
+// copies 680 and 606 us.
 //
 // Gates: with u = exp(-|f|), u / (1 + u) is the smaller of a and 1 - a, accurate to
 // f32 relative to itself.  It is kept with a sign ("c": a where positive, -(1 - a)
@@ -31,7 +34,7 @@
 // so a memory of thousands of tokens does not take over a rounding of a near 1, and
 // what is left of a state after a token that almost forgets it stays exact.  All gates
 // take these steps: a path without the selections, for tiles whose gates all lie above
-// -2.77 (a made of 1 - a, four tokens' reciprocals shared), was 4 to 8 % faster forwards, but
+// -2.77 (a made of 1 - a, four tokens' reciprocals shared), was 2 to 4 % faster forwards, but
 // lost up to 6 bits of a there, and a channel's digits went by its neighbours' gates.
 //
 // Joining the segments: a CTA takes segments in the order of a counter (so a

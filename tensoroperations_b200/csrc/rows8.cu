@@ -2,8 +2,10 @@
 //
 // Memory bound: a value is read once and its code written once (3.03 bytes for
 // bf16), with about 5 instructions a value.  A thread takes 16 values, two threads a
-// group; they exchange nothing but their maxima.  Measured on B200: 16384 x 4096 bf16
-// in 42 us, 4.9 TB/s (0.75 of the copy rate), and back in 40 us, 5.1 TB/s.
+// group; they exchange nothing but their maxima.  Measured on B200, each behind an L2
+// flush: 16384 x 4096 bf16 in 41 us, 5.0 TB/s (0.76 of the copy rate), and back in 39 us,
+// 5.2 TB/s; 8192 x 4096 f32 33 and 45 us; single-value accesses, 16384 x 4093 bf16, 184 and
+// 358 us.
 #include <algorithm>
 
 #include "rows8.cuh"
