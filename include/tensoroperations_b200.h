@@ -802,7 +802,9 @@ int to_gated_recurrence(const to_gated_recurrence_desc* desc, const to_gated_rec
  * on their way (8 s).  Negative: as at the start; 0: maps that are not there at once, or any
  * wait of a block's warps, counts as run out.  At most an hour.  Where a wait runs out, to_device_status reports
  * TO_ERR_TIMEOUT, and outputs and states that depend on what did not come are NaN or
- * have not been written.  Holds for the process.
+ * have not been written.  dbias is NaN then (of sequences of one segment each, which wait
+ * for no maps, also as long as an earlier TO_ERR_TIMEOUT has not been read).  Holds for
+ * the process; a captured call keeps the limits of its capture.
  */
 int to_gated_recurrence_wait_limits(int64_t maps_us, int64_t tiles_us);
 
